@@ -43,7 +43,8 @@ const char* kh_error_string(int code);
  * kh_profile_begin and kh_profile_end every kernel of this library is launched with its own HIP
  * start/stop event pair on the launch stream.  kh_profile_end waits for them and writes, in launch
  * order, a kernel tag (1 lora_gemm, 2 lora_gemm_f32, 3 attention, 4 group_norm stats, 5 group_norm apply,
- * 6 layer_norm, 7 geglu, 8 residual_add, 9 concat_residual, 10 sgmv_shrink, 11 sgmv_expand, 12 lora_shrink, 13 conv3x3, 14 cfg_euler, 15 upsample, 16 lora_merge, 17 conv_out + guidance + Euler) and the
+ * 6 layer_norm, 7 geglu, 8 residual_add, 9 concat_residual, 10 sgmv_shrink, 11 sgmv_expand, 12 lora_shrink, 13 conv3x3, 14 cfg_euler, 15 upsample, 16 lora_merge, 17 conv_out + guidance + Euler,
+ * 18 fused segmented shrink + expand, 19 lora_pack, 20 block_norm, 21 quantize_w4, 22 dequantize_w4, 23 w4_linear, 24 its shrink, 25 linear attention) and the
  * duration in ms into HOST arrays; returns the number of launches (or -hipError_t).  Do not use under
  * graph capture. */
 int kh_profile_begin(void);
@@ -465,6 +466,51 @@ int kh_lora_linear_desc_bf16(const KhLinearDesc* desc, const void* x, const void
 int kh_transformer_block_needs(const KhBlockDesc* desc, int64_t B, int64_t T, int64_t S, int own_kv, int64_t* workspace_bytes,
                                int64_t* counter_ints);
 int kh_transformer_block_bf16(const KhBlockDesc* desc, const KhBlockCall* call, void* stream);
+
+/* ---- Operators of a block that answers token by token -------------------------------------------
+ * No counterpart in the reference, whose text encoders run once a prompt; they stand beside K1, K3 and K4.
+ * type: 0 bf16, 1 fp16, 2 fp32.
+ *
+ * The norms before and after a block with the gate and the residual between them (beside kh_layer_norm_bf16):
+ *   h_out = residual_scale * h + gate * N(y; post_w, post_b),   u = N(h_out; pre_w, pre_b)      rows [M, D], D <= 32768
+ * N: root-mean-square norm, or layer norm with flags bit 0; y is normed with flags bit 1 only; u == NULL: no norm behind the sum (which
+ * is normed before it is rounded).  y == NULL: u = N(h) alone (no gate, no h_out).  Weights and biases [D] may be NULL; gate [M / gate_rows, D]
+ * may be NULL: row m takes gate row m / gate_rows.  y, u, gate and the affine terms are `type`, h and h_out `stream_type`: the same, or fp32.
+ * h_out may be h, u may be y. */
+int kh_block_norm(const void* y, const void* h, const void* gate, int64_t gate_rows, const void* post_w, const void* post_b,
+                  const void* pre_w, const void* pre_b, void* h_out, void* u, int64_t M, int64_t D, float residual_scale, float eps, int flags,
+                  int type, int stream_type, void* stream);
+/* Weights in 4 bits: w[n][k] = scale[n][k / group] * (code[n][k] - zero[n][k / group]), group 32, 64 or 128, zero = 8 where it is NULL.
+ *   q      [N, ceil(K / 32) * 16] bytes: code 2i in the low half of byte i, 2i + 1 in the high one, filled up to 32 codes
+ *   scale  [N, ceil(groups / 4) * 4] bf16, zero [the same] uint8 (0..15), groups = ceil(K / group)
+ * kh_quantize_w4: scale = bf16(largest magnitude / 7), or with zero points bf16((max(w, 0) - min(w, 0)) / 15) and zero = rint(-min / scale); codes are
+ * rint(w / scale) + zero within 0..15 (halves to even).  A group that holds a NaN gets a NaN as its scale, one that holds an infinity an infinity.
+ * kh_dequantize_w4: the values in `type`, rounded once, [N, K].
+ * kh_w4_linear: y[M,N] = x w^T + bias + ((x A_cat^T) * col_scale) B_cat^T (+ residual), the adapter operands as for kh_lora_linear_bf16 (R % 32 == 0,
+ * R <= 128, any K and N), type 0 or 1.  Products with the codes are exact and summed in 32 bits; the rank-R product stays in 32 bits.  A row of x
+ * that holds an infinity gives NaN.  workspace: kh_w4_linear_workspace_bytes (0 without an adapter; then it may be NULL). */
+int kh_quantize_w4(const void* w, void* q, void* scale, void* zero, int64_t N, int64_t K, int64_t group, int type, void* stream);
+int kh_dequantize_w4(const void* q, const void* scale, const void* zero, void* out, int64_t N, int64_t K, int64_t group, int type, void* stream);
+int64_t kh_w4_linear_workspace_bytes(int64_t M, int64_t K, int64_t R);
+int kh_w4_linear(const void* x, const void* q, const void* scale, const void* zero, const void* bias, const void* a_cat, const void* b_cat,
+                 const float* col_scale, const void* residual, void* y, void* workspace, int64_t M, int64_t N, int64_t K, int64_t R,
+                 int64_t group, int type, void* stream);
+/* Linear attention with a decay for each head:  S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T,   o_t = scale * q_t S_t.
+ * q [.., H * dk], k [.., kv_heads * dk], v [.., kv_heads * dv], o [.., H * dv] bf16, dk 64 or 128, dv a multiple of 64 up to 1024; query head h takes
+ * key head h / (H / kv_heads).  log_decay float [H], <= 0 (-inf: no memory).  Rows through strides in elements (multiples of 8): dense [B, T] with
+ * batch strides, or, with seg_start (int32 [B + 1], device), packed: sequence b is rows seg_start[b] .. seg_start[b + 1] - 1 of `rows`, T the
+ * longest (a longer one is cut off there), batch strides unused; other rows of o are left as they were.
+ * state_in / state_out: float [n_slots, H, dk, dv]; sequence b starts from and leaves slot b, or slots[b] (int32 [B], device; distinct): a slot
+ * outside 0 .. n_slots - 1 leaves the whole sequence out.  state_in NULL: zeros (not for the step); the two may be the same.
+ * workspace: kh_linear_attention_workspace_bytes (0: may be NULL).  kh_linear_attention_step_bf16: one token a sequence, rows [B]. */
+int64_t kh_linear_attention_workspace_bytes(int64_t B, int64_t H, int64_t T, int64_t dk, int64_t dv);
+int kh_linear_attention_bf16(const void* q, const void* k, const void* v, void* o, const float* log_decay, const float* state_in,
+                             float* state_out, const int32_t* slots, int64_t n_slots, const int32_t* seg_start, int64_t rows, void* workspace,
+                             int64_t B, int64_t H, int64_t kv_heads, int64_t T, int64_t dk, int64_t dv, int64_t ldq, int64_t ldk, int64_t ldv,
+                             int64_t ldo, int64_t bsq, int64_t bsk, int64_t bsv, int64_t bso, float scale, void* stream);
+int kh_linear_attention_step_bf16(const void* q, const void* k, const void* v, void* o, const float* log_decay, const float* state_in,
+                                  float* state_out, const int32_t* slots, int64_t n_slots, int64_t B, int64_t H, int64_t kv_heads, int64_t dk,
+                                  int64_t dv, int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo, float scale, void* stream);
 
 #ifdef __cplusplus
 }

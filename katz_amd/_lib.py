@@ -66,6 +66,14 @@ SIGNATURES = {
     "kh_lora_linear_desc_bf16": (c_int, [_P] * 6 + [_I, c_int, _P]),
     "kh_transformer_block_needs": (c_int, [_P, _I, _I, _I, c_int, _P, _P]),
     "kh_transformer_block_bf16": (c_int, [_P, _P, _P]),
+    "kh_block_norm": (c_int, [_P, _P, _P, _I] + [_P] * 6 + [_I, _I, c_float, c_float, c_int, c_int, c_int, _P]),
+    "kh_quantize_w4": (c_int, [_P] * 4 + [_I] * 3 + [c_int, _P]),
+    "kh_dequantize_w4": (c_int, [_P] * 4 + [_I] * 3 + [c_int, _P]),
+    "kh_w4_linear_workspace_bytes": (_I, [_I] * 3),
+    "kh_w4_linear": (c_int, [_P] * 11 + [_I] * 5 + [c_int, _P]),
+    "kh_linear_attention_workspace_bytes": (_I, [_I] * 5),
+    "kh_linear_attention_bf16": (c_int, [_P] * 8 + [_I, _P, _I, _P] + [_I] * 14 + [c_float, _P]),
+    "kh_linear_attention_step_bf16": (c_int, [_P] * 8 + [_I] * 10 + [c_float, _P]),
 }
 
 _lib = None
