@@ -160,11 +160,20 @@ __device__ __forceinline__ u32x4 interleaved(const u32x4 v) {
 #endif
 }
 
+// The mask and the power of two in registers: one instruction then takes both (and-or), where two constants in the code would take two.
 template <typename T>
-__device__ __forceinline__ u32x4 operands(uint32_t word) {
-  return u32x4{(word & 0x000f000fu) | Num<T>::P, ((word >> 4) & 0x000f000fu) | Num<T>::P, ((word >> 8) & 0x000f000fu) | Num<T>::P,
-               ((word >> 12) & 0x000f000fu) | Num<T>::P};
-}
+struct Unpack {
+  uint32_t mask = 0x000f000fu, power = Num<T>::P;
+  __device__ __forceinline__ Unpack() {
+#if __HIP_DEVICE_COMPILE__
+    asm("" : "+s"(mask));
+    asm("" : "+v"(power));
+#endif
+  }
+  __device__ __forceinline__ u32x4 operator()(uint32_t word) const {
+    return u32x4{(word & mask) | power, ((word >> 4) & mask) | power, ((word >> 8) & mask) | power, ((word >> 12) & mask) | power};
+  }
+};
 
 // Lane group g (of 16 lanes) holds words 4g .. 4g+3 of a block of 128 codes of its row; afterwards words g, g+4, g+8, g+12: the k-step
 // j of 32 codes takes register j of all four groups.
@@ -190,104 +199,522 @@ struct LinParams {
   void* y;
   long M, N;
   int K, R, t_splits, row_bytes, gstride;
+  int dma;                 // rows of x are aligned to four bytes
 };
 
-constexpr int LW = 8;      // waves of a workgroup, which share the blocks of 128 codes
+// The rank-R product of a 16 x 16 tile in 32 bits, a step of 16 ranks: t [M][R] in `splits` parts, B_cat rows of T.
+template <typename T>
+__device__ __forceinline__ f32x4 rank_step(const LinParams& p, long m, long n, int r, f32x4 acc) {
+  const float* tr = p.t + m * p.R + r;
+  const long part = p.M * p.R;
+  f32x4 t = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int sp = 0; sp < p.t_splits; sp += 4) {      // four on their way at a time, added in order
+    f32x4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = sp + i < p.t_splits ? *reinterpret_cast<const f32x4*>(tr + (sp + i) * part) : f32x4{0.f, 0.f, 0.f, 0.f};
+    t = (((t + v[0]) + v[1]) + v[2]) + v[3];
+  }
+  T b[4];
+  __builtin_memcpy(b, (const T*)p.b_cat + n * p.R + r, sizeof(b));
+#if __HIP_DEVICE_COMPILE__
+#pragma unroll
+  for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(t[e], (float)b[e], acc, 0, 0, 0);
+#endif
+  return acc;
+}
 
-// 16 columns of y (rows of codes) and MB * 16 rows of x to a workgroup; its waves take every LW-th block of 128 codes and are summed
-// in order at the end.
-template <typename T, int G, bool ZERO, int MB>
+template <int BYTES> struct Word;
+template <> struct Word<1> { typedef uint8_t type; };
+template <> struct Word<2> { typedef uint16_t type; };
+template <> struct Word<4> { typedef uint32_t type; };
+template <> struct Word<8> { typedef uint64_t type; };
+
+typedef __attribute__((address_space(3))) void* lptr_t;
+
+template <int VM>
+__device__ __forceinline__ void wait_vm() {  // vmcnt = VM, the other counters unconstrained (gfx9 encoding)
+  __builtin_amdgcn_s_waitcnt((VM & 15) | (7 << 4) | (15 << 8) | ((VM >> 4) << 14));
+  asm volatile("" ::: "memory");
+}
+
+// What a wave keeps of a block of 128 codes in LDS: codes of NB x 16 rows, x in the order of its operands, scales, zero points.  P loads.
+template <int G, bool ZERO, int MB, int NB, bool FOUR>
+struct Stage {
+  static constexpr int X = FOUR ? 1 : 4 * MB;                // loads of 1 KB
+  static constexpr int S = G == 32 ? 2 : 1, Z = ZERO ? 1 : 0;  // loads of 256 bytes: four bytes of a row, the lane groups take a tile of 16 rows each
+  static constexpr int P = NB + X + S + Z;
+  static constexpr int WAT = 0, XAT = NB * 1024, SAT = XAT + X * 1024, ZAT = SAT + S * 256, BYTES = ZAT + Z * 256;
+};
+
+// A few rows: NB * 16 columns of y (rows of codes) and MB * 16 rows of x to a workgroup.  Its LW waves take every LW-th block of 128 codes and are
+// summed in order at the end.  A wave's blocks go straight to a ring of ST of its own in LDS, ST - 1 ahead of the one that is multiplied: nobody else
+// reads them, so there is no barrier, and the loads in flight cost no registers.
+// FOUR: at most four rows (MB 1), which lie at every fourth row of the product: then they are in the first register of every lane, and the other three
+// need no scale.
+template <typename T, int G, bool ZERO, int MB, int NB, int LW, int ST, bool FOUR>
 __global__ __launch_bounds__(LW * 64) void w4_few_rows(const LinParams p) {
-  extern __shared__ float part[];    // [LW][MB * 16][17]
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int l = lane & 15, g = lane >> 4;
-  const long n = (long)blockIdx.x * 16 + l, nc = n < p.N ? n : p.N - 1;
-  const long m0 = (long)blockIdx.y * (MB * 16);
-  const int blocks = (p.row_bytes + 63) / 64;
-  const uint8_t* qr = p.q + nc * p.row_bytes + g * 16;
-  const bf16_t* sr = p.scale + nc * p.gstride;
-  const uint8_t* zr = ZERO ? p.zero + nc * p.gstride : nullptr;
-  const int groups = (p.K + G - 1) / G;
+#if __HIP_DEVICE_COMPILE__
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  typedef Stage<G, ZERO, MB, NB, FOUR> Sg;
   constexpr int GB = 128 / G;        // groups in a block
   constexpr int SG = 4 / GB;         // k-steps in a group
-  f32x4 out[MB];
+  constexpr int E = FOUR ? 1 : 4;
+  typedef typename Word<GB * 2>::type SW_t;
+  typedef typename Word<GB>::type ZW_t;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int l = lane & 15, g = lane >> 4;
+  const long m0 = (long)blockIdx.y * (MB * 16), n0 = (long)blockIdx.x * (NB * 16);
+  const int rows = (int)(p.M - m0 < MB * 16 ? p.M - m0 : MB * 16);
+  // the workgroup's first rows, and what a lane is from there (below 2^31: K <= 2^24)
+  const uint8_t* q0 = p.q + n0 * p.row_bytes;
+  const bf16_t* s0 = p.scale + n0 * p.gstride;
+  const uint8_t* z0 = ZERO ? p.zero + n0 * p.gstride : nullptr;
+  const T* x0 = (const T*)p.x + m0 * p.K;
+  const uint32_t last = (uint32_t)(p.N - 1 - n0 < NB * 16 - 1 ? p.N - 1 - n0 : NB * 16 - 1);
+  uint32_t qo[NB];
 #pragma unroll
-  for (int b = 0; b < MB; ++b) out[b] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const T* xr[MB];
+  for (int j = 0; j < NB; ++j) {
+    const uint32_t r = j * 16 + l;
+    qo[j] = (r < last ? r : last) * (uint32_t)p.row_bytes + g * 16;
+  }
+  const uint32_t mr = (g < NB ? g : NB - 1) * 16 + l, so = (mr < last ? mr : last) * (uint32_t)p.gstride;    // row whose scales the lane fetches
+  int xm[MB];
+  uint32_t xo[MB];
 #pragma unroll
   for (int b = 0; b < MB; ++b) {
-    const long m = m0 + b * 16 + l;
-    xr[b] = (const T*)p.x + (m < p.M ? m : p.M - 1) * p.K;
+    const int r = FOUR ? l >> 2 : b * 16 + l;
+    xm[b] = r < rows ? r : rows - 1;
+    xo[b] = (uint32_t)xm[b] * (uint32_t)p.K + g * 8;
   }
-  for (int kb = wave; kb < blocks; kb += LW) {
-    u32x4 w = u32x4{0, 0, 0, 0};
-    if (kb * 64 + g * 16 < p.row_bytes) w = *reinterpret_cast<const u32x4*>(qr + (long)kb * 64);
-    float s[GB];
-    uint32_t c[GB];
-#pragma unroll
-    for (int i = 0; i < GB; ++i) {
-      const int gi = kb * GB + i;
-      s[i] = gi < groups ? (float)sr[gi] : 0.f;
-      c[i] = (Num<T>::P | Num<T>::NEG) | (ZERO ? (gi < groups ? zr[gi] : 0u) * 0x10001u : 0x00080008u);
-    }
-    w = across_groups(w);
-    u32x4 wv[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) wv[j] = operands<T>(w[j]);
-#pragma unroll
-    for (int b = 0; b < MB; ++b) {
-      u32x4 xv[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int k = kb * 128 + j * 32 + g * 8;
-        T v[8];
-        load8<T>(xr[b] + k, (long)p.K - k, v);
-        xv[j] = interleaved(__builtin_bit_cast(u32x4, v));
-      }
-#pragma unroll
-      for (int i = 0; i < GB; ++i) {
-        f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
-        const u32x4 cv = u32x4{c[i], c[i], c[i], c[i]};
-#pragma unroll
-        for (int j = 0; j < SG; ++j) {
-          acc = Num<T>::mfma(xv[i * SG + j], wv[i * SG + j], acc);
-          acc = Num<T>::mfma(xv[i * SG + j], cv, acc);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) out[b][e] = fmaf(s[i], acc[e], out[b][e]);
-      }
-    }
-  }
+  const uint32_t x4 = ((uint32_t)(g < rows ? g : rows - 1) * (uint32_t)p.K + l * 8) * 2;   // FOUR: row g, piece l
+  const Unpack<T> unpack;
+  const f32x4 none = f32x4{0.f, 0.f, 0.f, 0.f};
+  f32x4 out[MB][NB];
 #pragma unroll
   for (int b = 0; b < MB; ++b)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) part[(wave * (MB * 16) + b * 16 + g * 4 + e) * 17 + l] = out[b][e];
-  __syncthreads();
-  for (int i = threadIdx.x; i < MB * 256; i += LW * 64) {
-    const int r = i >> 4, col = i & 15;
-    const long m = m0 + r, nn = (long)blockIdx.x * 16 + col;
-    if (m >= p.M || nn >= p.N) continue;
-    float v = 0.f;
+    for (int j = 0; j < NB; ++j) out[b][j] = none;
+
+  auto multiply = [&](const u32x4 (&w0)[NB], const u32x4 (&x)[MB][4], const SW_t (&sw)[NB], const ZW_t (&zw)[NB], int groups) {
+    u32x4 xv[MB][4];                          // groups: of this block; what rows of scales are filled up with is not used
 #pragma unroll
-    for (int w = 0; w < LW; ++w) v += part[(w * (MB * 16) + r) * 17 + col];
-    if (p.R > 0) {
-      const T* bc = (const T*)p.b_cat + nn * p.R;
-      const float* t = p.t + m * p.R;
-      for (int k = 0; k < p.R; k += 8) {
-        T bv[8];
-        __builtin_memcpy(bv, bc + k, sizeof(bv));
+    for (int b = 0; b < MB; ++b)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float tv = 0.f;
-          for (int sp = 0; sp < p.t_splits; ++sp) tv += t[(long)sp * p.M * p.R + k + e];
-          v = fmaf(tv, (float)bv[e], v);
+      for (int j = 0; j < 4; ++j) xv[b][j] = interleaved(x[b][j]);
+    f32x4 base[MB][GB];                       // without zero points the constant is the same for all columns
+    if (!ZERO) {
+      constexpr uint32_t c = Num<T>::P | Num<T>::NEG | 0x00080008u;
+#pragma unroll
+      for (int b = 0; b < MB; ++b)
+#pragma unroll
+        for (int i = 0; i < GB; ++i)
+#pragma unroll
+          for (int k = 0; k < SG; ++k) base[b][i] = Num<T>::mfma(xv[b][i * SG + k], u32x4{c, c, c, c}, k == 0 ? none : base[b][i]);
+    }
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const u32x4 w = across_groups(w0[j]);
+#pragma unroll
+      for (int i = 0; i < GB; ++i) {
+        const float s = i < groups ? bf16_bits_to_f32((uint32_t)(sw[j] >> (16 * i)) & 0xffffu) : 0.f;
+        uint32_t c = 0;
+        if (ZERO) c = (Num<T>::P | Num<T>::NEG) | ((uint32_t)(zw[j] >> (8 * i)) & 15u) * 0x10001u;
+        f32x4 acc[MB];
+#pragma unroll
+        for (int b = 0; b < MB; ++b) acc[b] = ZERO ? none : base[b][i];
+#pragma unroll
+        for (int k = 0; k < SG; ++k) {
+          const u32x4 wv = unpack(w[i * SG + k]);
+#pragma unroll
+          for (int b = 0; b < MB; ++b) {
+            acc[b] = Num<T>::mfma(xv[b][i * SG + k], wv, acc[b]);
+            if (ZERO) acc[b] = Num<T>::mfma(xv[b][i * SG + k], u32x4{c, c, c, c}, acc[b]);
+          }
         }
+#pragma unroll
+        for (int b = 0; b < MB; ++b)
+#pragma unroll
+          for (int e = 0; e < E; ++e) out[b][j][e] = fmaf(s, acc[b][e], out[b][j][e]);
       }
     }
-    if (p.bias) v += (float)((const T*)p.bias)[nn];
-    if (p.residual) v += (float)((const T*)p.residual)[m * p.N + nn];
-    ((T*)p.y)[m * p.N + nn] = (T)v;
+  };
+
+  const int full = p.dma ? p.K / 128 : 0, blocks = (p.row_bytes + 63) / 64;
+  const int mine = wave < full ? (full - 1 - wave) / LW + 1 : 0;   // whole blocks of this wave
+  char* ring = smem + wave * (ST * Sg::BYTES);
+  auto bytes = [](long n) { return (int)(uint32_t)(n < 0xffffffffL ? n : 0xffffffffL); };
+  const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(q0), 0, bytes((p.N - n0) * p.row_bytes), 0x00020000);
+  const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(x0), 0, bytes((p.M - m0) * p.K * 2), 0x00020000);
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16_t*>(s0), 0, bytes((p.N - n0) * p.gstride * 2), 0x00020000);
+  const __amdgpu_buffer_rsrc_t rz = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(ZERO ? z0 : q0), 0, bytes((p.N - n0) * p.gstride), 0x00020000);
+  // the four bytes that hold a block's scales (128: half of them) or zero points
+  auto s_word = [&](int kb) { return kb * GB * 2 & ~3; };
+  auto z_word = [&](int kb) { return kb * GB & ~3; };
+  auto fetch = [&](int i, int st) {           // the wave's i-th block into a stage
+    const int kb = wave + i * LW;
+    char* to = ring + st * Sg::BYTES;
+#pragma unroll
+    for (int j = 0; j < NB; ++j) __builtin_amdgcn_raw_ptr_buffer_load_lds(rq, (lptr_t)(to + Sg::WAT + j * 1024), 16, qo[j], kb * 64, 0, 0);
+    if constexpr (FOUR) {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lptr_t)(to + Sg::XAT), 16, x4, kb * 256, 0, 0);
+    } else {
+#pragma unroll
+      for (int b = 0; b < MB; ++b)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lptr_t)(to + Sg::XAT + (b * 4 + j) * 1024), 16, xo[b] * 2, kb * 256 + j * 64, 0, 0);
+    }
+#pragma unroll
+    for (int j = 0; j < Sg::S; ++j) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lptr_t)(to + Sg::SAT + j * 256), 4, so * 2, s_word(kb) + j * 4, 0, 0);
+    if constexpr (ZERO) __builtin_amdgcn_raw_ptr_buffer_load_lds(rz, (lptr_t)(to + Sg::ZAT), 4, so, z_word(kb), 0, 0);
+  };
+  auto use = [&](int i, int st) {
+    const int kb = wave + i * LW;
+    const char* at = ring + st * Sg::BYTES;
+    u32x4 w[NB], x[MB][4];
+    SW_t sw[NB];
+    ZW_t zw[NB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      w[j] = *reinterpret_cast<const u32x4*>(at + Sg::WAT + j * 1024 + lane * 16);
+      const char* sa = at + Sg::SAT + (j * 16 + l) * 4;
+      if constexpr (G == 32) sw[j] = (SW_t)*reinterpret_cast<const uint32_t*>(sa) | (SW_t)((uint64_t)*reinterpret_cast<const uint32_t*>(sa + 256) << 32);
+      else sw[j] = (SW_t)(*reinterpret_cast<const uint32_t*>(sa) >> (kb * GB * 16 & 31));
+      if constexpr (ZERO) zw[j] = (ZW_t)(*reinterpret_cast<const uint32_t*>(at + Sg::ZAT + (j * 16 + l) * 4) >> (kb * GB * 8 & 31));
+    }
+#pragma unroll
+    for (int b = 0; b < MB; ++b)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        x[b][j] = *reinterpret_cast<const u32x4*>(at + Sg::XAT + (FOUR ? (l >> 2) * 256 + (j * 4 + g) * 16 : (b * 4 + j) * 1024 + lane * 16));
+    multiply(w, x, sw, zw, GB);
+  };
+  {
+    int st = 0;                               // stage of block i
+    auto ahead = [&](int n) { return st + n < ST ? st + n : st + n - ST; };
+#pragma unroll
+    for (int i = 0; i < ST - 1; ++i)
+      if (i < mine) fetch(i, i);
+    // the adapters while the first blocks are on their way
+    for (int r = wave * 16; r < p.R; r += LW * 16)
+#pragma unroll
+      for (int b = 0; b < MB; ++b)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          const long n = n0 + j * 16 + l;
+          out[b][j] = rank_step<T>(p, m0 + xm[b], n < p.N ? n : p.N - 1, r + 4 * g, out[b][j]);
+        }
+    int i = 0;
+    for (; i + ST - 1 < mine; ++i) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the block before has been read; its stage is the next one's
+      fetch(i + ST - 1, ahead(ST - 1));
+      wait_vm<(ST - 1) * Sg::P>();
+      use(i, st);
+      st = ahead(1);
+    }
+    if constexpr (ST > 3)
+      if (i + 2 < mine) { wait_vm<2 * Sg::P>(); use(i++, st); st = ahead(1); }
+    if constexpr (ST > 2)
+      if (i + 1 < mine) { wait_vm<Sg::P>(); use(i++, st); st = ahead(1); }
+    if (i < mine) { wait_vm<0>(); use(i, st); }
   }
+  // what there is of the last block (of rows of x that are not aligned to four bytes: every block)
+  for (int kb = full + (wave - full % LW + LW) % LW; kb < blocks; kb += LW) {
+    u32x4 w[NB], x[MB][4];
+    SW_t sw[NB];
+    ZW_t zw[NB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const uint32_t r = j * 16 + l, rc = (r < last ? r : last) * (uint32_t)p.gstride;
+      w[j] = u32x4{0, 0, 0, 0};
+      if (kb * 64 + g * 16 < p.row_bytes) w[j] = *reinterpret_cast<const u32x4*>(q0 + (long)kb * 64 + qo[j]);
+      sw[j] = *reinterpret_cast<const SW_t*>(s0 + kb * GB + rc);           // (rows of scales and zero points are filled up to whole blocks)
+      if (ZERO) zw[j] = *reinterpret_cast<const ZW_t*>(z0 + kb * GB + rc);
+    }
+#pragma unroll
+    for (int b = 0; b < MB; ++b)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        T v[8];
+        load8<T>(x0 + kb * 128 + (xo[b] + j * 32), (long)p.K - (kb * 128 + j * 32 + g * 8), v);
+        x[b][j] = __builtin_bit_cast(u32x4, v);
+      }
+    const int left = (p.K - kb * 128 + G - 1) / G;
+    multiply(w, x, sw, zw, left < GB ? left : GB);
+  }
+  __syncthreads();                            // the rings are dead
+  float* part = reinterpret_cast<float*>(smem);      // [LW][rows][NB * 16 + 1]
+#pragma unroll
+  for (int b = 0; b < MB; ++b)
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int r = FOUR ? g : b * 16 + g * 4 + e;
+      if (r < rows)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) part[(wave * rows + r) * (NB * 16 + 1) + j * 16 + l] = out[b][j][e];
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows * (NB * 16); i += LW * 64) {
+    const int r = i / (NB * 16), col = i % (NB * 16);
+    const long m = m0 + r, n = n0 + col;
+    if (n >= p.N) continue;
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < LW; ++w) v += part[(w * rows + r) * (NB * 16 + 1) + col];
+    if (p.bias) v += (float)((const T*)p.bias)[n];
+    if (p.residual) v += (float)((const T*)p.residual)[m * p.N + n];
+    ((T*)p.y)[m * p.N + n] = (T)v;
+  }
+#endif
+}
+
+// Many rows: 128 rows of x and 256 columns of y to a workgroup of four waves, 64 columns each.  Blocks of 128 codes with their x come by DMA into three
+// stages in LDS, x in the order of its operands, codes and scales to the wave that uses them.
+// The numbers multiplied are P + q without zero points and P + 16 + q - z with them (z taken off in the integers, four codes at a time); what they are too
+// large by is one constant then, and its product with a group's x the same for all columns: a wave computes it for 32 rows of the next block and leaves it in
+// LDS, where every wave's accumulators start from it.
+// Of the 2048 clocks that the matrix unit needs for a block (128 products of 16 x 16 x 32 on each SIMD), a third more goes to the vector unit beside it: codes to
+// operands and, for every group, the scaled sum.
+constexpr int MR_M = 8, MR_N = 4, MR_W = 4, MR_ST = 3;     // tiles of 16 rows; of 16 columns of a wave; waves; stages
+
+template <int G, bool ZERO>
+struct ManyStage {
+  static constexpr int S = G == 32 ? 2 : 1, Z = ZERO ? 1 : 0, GB = 128 / G;
+  static constexpr int P = MR_M * 4 / MR_W + MR_N + S + Z;                     // loads of a wave
+  static constexpr int XAT = 0, WAT = MR_M * 4096, SAT = WAT + MR_W * MR_N * 1024, ZAT = SAT + MR_W * S * 256, BYTES = ZAT + MR_W * Z * 256;
+  static constexpr int SUMS = MR_ST * BYTES, RING = SUMS + 2 * GB * MR_M * 16 * 4;
+  static constexpr int PITCH = MR_N * 16 + 4, OUT = MR_W * MR_M * 16 * PITCH * 4;   // the outputs in 32 bits, on their way to whole rows
+  static constexpr int LDS = RING > OUT ? RING : OUT;
+};
+
+template <typename T, int G, bool ZERO>
+__global__ __launch_bounds__(MR_W * 64, 1) void w4_many_rows(const LinParams p) {
+#if __HIP_DEVICE_COMPILE__
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  typedef ManyStage<G, ZERO> Sg;
+  constexpr int GB = 128 / G, SG = 4 / GB;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int l = lane & 15, g = lane >> 4;
+  const uint32_t mt = (uint32_t)((p.M + MR_M * 16 - 1) / (MR_M * 16));
+  const uint32_t unit = xcd_remap(blockIdx.x, gridDim.x);                      // an XCD has neighbouring columns, with all rows
+  const long m0 = (long)(unit % mt) * (MR_M * 16), n0 = (long)(unit / mt) * (MR_W * MR_N * 16) + wave * (MR_N * 16);
+  const int rows = (int)(p.M - m0 < MR_M * 16 ? p.M - m0 : MR_M * 16);
+  const bool some = n0 < p.N;                                                  // (a wave past the last column repeats it)
+  const long nb = some ? n0 : p.N - 1;
+  const uint8_t* q0 = p.q + nb * p.row_bytes;
+  const bf16_t* s0 = p.scale + nb * p.gstride;
+  const uint8_t* z0 = ZERO ? p.zero + nb * p.gstride : nullptr;
+  const T* x0 = (const T*)p.x + m0 * p.K;
+  const uint32_t last = (uint32_t)(p.N - 1 - nb < MR_N * 16 - 1 ? p.N - 1 - nb : MR_N * 16 - 1);
+  uint32_t qo[MR_N], xo[MR_M / MR_W];
+#pragma unroll
+  for (int j = 0; j < MR_N; ++j) {
+    const uint32_t r = j * 16 + l;
+    qo[j] = (r < last ? r : last) * (uint32_t)p.row_bytes + g * 16;
+  }
+#pragma unroll
+  for (int b = 0; b < MR_M / MR_W; ++b) {
+    const int r = (wave * (MR_M / MR_W) + b) * 16 + l;
+    xo[b] = (uint32_t)(r < rows ? r : rows - 1) * (uint32_t)p.K + g * 8;
+  }
+  const uint32_t so = ((uint32_t)lane < last ? (uint32_t)lane : last) * (uint32_t)p.gstride;
+  auto bytes = [](long n) { return (int)(uint32_t)(n < 0xffffffffL ? n : 0xffffffffL); };
+  const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(q0), 0, bytes((p.N - nb) * p.row_bytes), 0x00020000);
+  const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(x0), 0, bytes((p.M - m0) * p.K * 2), 0x00020000);
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16_t*>(s0), 0, bytes((p.N - nb) * p.gstride * 2), 0x00020000);
+  const __amdgpu_buffer_rsrc_t rz = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(ZERO ? z0 : q0), 0, bytes((p.N - nb) * p.gstride), 0x00020000);
+
+  const int blocks = (p.row_bytes + 63) / 64, whole = p.dma ? p.K / 128 : 0, groups = (p.K + G - 1) / G;
+  auto fetch = [&](int kb, int st) {
+    char* to = smem + st * Sg::BYTES;
+#pragma unroll
+    for (int b = 0; b < MR_M / MR_W; ++b)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        char* at = to + Sg::XAT + ((wave * (MR_M / MR_W) + b) * 4 + j) * 1024;
+        if (kb < whole) {
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lptr_t)at, 16, xo[b] * 2, kb * 256 + j * 64, 0, 0);
+        } else {                              // the end of the rows, or rows that are not aligned to four bytes
+          T v[8];
+          load8<T>(x0 + kb * 128 + (xo[b] + j * 32), (long)p.K - (kb * 128 + j * 32 + g * 8), v);
+          *reinterpret_cast<u32x4*>(at + lane * 16) = __builtin_bit_cast(u32x4, v);
+        }
+      }
+#pragma unroll
+    for (int j = 0; j < MR_N; ++j) __builtin_amdgcn_raw_ptr_buffer_load_lds(rq, (lptr_t)(to + Sg::WAT + (wave * MR_N + j) * 1024), 16, qo[j], kb * 64, 0, 0);
+#pragma unroll
+    for (int j = 0; j < Sg::S; ++j)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lptr_t)(to + Sg::SAT + (wave * Sg::S + j) * 256), 4, so * 2, (kb * GB * 2 & ~3) + j * 4, 0, 0);
+    if constexpr (ZERO) __builtin_amdgcn_raw_ptr_buffer_load_lds(rz, (lptr_t)(to + Sg::ZAT + wave * 256), 4, so, kb * GB & ~3, 0, 0);
+  };
+  const f32x4 none = f32x4{0.f, 0.f, 0.f, 0.f};
+  constexpr uint32_t over = (Num<T>::P | Num<T>::NEG) | (ZERO ? 0x00100010u : 0x00080008u);    // -(P + 16), -(P + 8)
+  auto x_at = [&](int st, int b, int j) { return *reinterpret_cast<const u32x4*>(smem + st * Sg::BYTES + Sg::XAT + (b * 4 + j) * 1024 + lane * 16); };
+  auto sums = [&](int st, int odd) {          // a constant's products with the groups of this wave's rows
+#pragma unroll
+    for (int b = 0; b < MR_M / MR_W; ++b)
+#pragma unroll
+      for (int i = 0; i < GB; ++i) {
+        f32x4 a = none;
+#pragma unroll
+        for (int k = 0; k < SG; ++k) a = Num<T>::mfma(x_at(st, wave * (MR_M / MR_W) + b, i * SG + k), u32x4{over, over, over, over}, a);
+        if (l == 0) *reinterpret_cast<f32x4*>(smem + Sg::SUMS + ((odd * GB + i) * MR_M * 16 + (wave * (MR_M / MR_W) + b) * 16 + g * 4) * 4) = a;
+      }
+  };
+  f32x4 out[MR_M][MR_N];
+#pragma unroll
+  for (int b = 0; b < MR_M; ++b)
+#pragma unroll
+    for (int j = 0; j < MR_N; ++j) out[b][j] = none;
+  uint32_t low = 0x0f0f0f0fu, sixteen = 0x10101010u, power = Num<T>::P;
+  asm("" : "+s"(low));
+  asm("" : "+v"(sixteen));
+  asm("" : "+s"(power));
+  auto multiply = [&](int kb, int st, int odd) {
+    const char* at = smem + st * Sg::BYTES;
+    u32x4 w[MR_N];
+    uint64_t sw[MR_N];
+    uint32_t zw[MR_N];
+#pragma unroll
+    for (int j = 0; j < MR_N; ++j) {
+      w[j] = across_groups(*reinterpret_cast<const u32x4*>(at + Sg::WAT + (wave * MR_N + j) * 1024 + lane * 16));
+      const char* sa = at + Sg::SAT + wave * Sg::S * 256 + (j * 16 + l) * 4;
+      sw[j] = *reinterpret_cast<const uint32_t*>(sa);
+      if constexpr (G == 32) sw[j] |= (uint64_t)*reinterpret_cast<const uint32_t*>(sa + 256) << 32;
+      else sw[j] >>= (kb * GB * 16 & 31);
+      if constexpr (ZERO) zw[j] = *reinterpret_cast<const uint32_t*>(at + Sg::ZAT + wave * 256 + (j * 16 + l) * 4) >> (kb * GB * 8 & 31);
+    }
+#pragma unroll
+    for (int i = 0; i < GB; ++i) {
+      float s[MR_N];
+      uint32_t z[MR_N];
+#pragma unroll
+      for (int j = 0; j < MR_N; ++j) {
+        s[j] = kb * GB + i < groups ? bf16_bits_to_f32((uint32_t)(sw[j] >> (16 * i)) & 0xffffu) : 0.f;    // what rows of scales are filled up with is not used
+        if constexpr (ZERO) z[j] = ((zw[j] >> (8 * i)) & 15u) * 0x01010101u;
+      }
+      f32x4 acc[MR_M][MR_N];
+#pragma unroll
+      for (int b = 0; b < MR_M; ++b) {
+        const f32x4 base = *reinterpret_cast<const f32x4*>(smem + Sg::SUMS + ((odd * GB + i) * MR_M * 16 + b * 16 + g * 4) * 4);
+#pragma unroll
+        for (int j = 0; j < MR_N; ++j) acc[b][j] = base;
+      }
+#pragma unroll
+      for (int k = 0; k < SG; ++k) {
+        u32x4 wv[MR_N];
+#pragma unroll
+        for (int j = 0; j < MR_N; ++j) {      // bytes of even and of odd codes, put beside one another: the order of x
+          const uint32_t word = w[j][i * SG + k];
+          uint32_t even = ZERO ? ((word & low) | sixteen) - z[j] : word & low;
+          uint32_t uneven = ZERO ? (((word >> 4) & low) | sixteen) - z[j] : (word >> 4) & low;
+          wv[j] = u32x4{__builtin_amdgcn_perm(uneven, even, 0x0c040c00u) | power, __builtin_amdgcn_perm(uneven, even, 0x0c050c01u) | power,
+                        __builtin_amdgcn_perm(uneven, even, 0x0c060c02u) | power, __builtin_amdgcn_perm(uneven, even, 0x0c070c03u) | power};
+        }
+#pragma unroll
+        for (int b = 0; b < MR_M; ++b) {
+          const u32x4 xv = x_at(st, b, i * SG + k);
+#pragma unroll
+          for (int j = 0; j < MR_N; ++j) acc[b][j] = Num<T>::mfma(xv, wv[j], acc[b][j]);
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < MR_M; ++b)
+#pragma unroll
+        for (int j = 0; j < MR_N; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) out[b][j][e] = fmaf(s[j], acc[b][j][e], out[b][j][e]);
+    }
+  };
+  auto barrier = []() {                       // what this wave has written to LDS is there, and everybody has arrived
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  fetch(0, 0);
+  if (blocks > 1) fetch(1, 1);
+  wait_vm<0>();
+  barrier();
+  sums(0, 0);
+  for (int kb = 0, st = 0; kb < blocks; ++kb) {
+    const int s1 = st == MR_ST - 1 ? 0 : st + 1, s2 = s1 == MR_ST - 1 ? 0 : s1 + 1;
+    wait_vm<0>();                             // this wave's share of the next block, requested a block ago
+    barrier();                                // everybody's; this block's sums; and nobody reads the block before any more
+    if (kb + 2 < blocks) fetch(kb + 2, s2);
+    if (kb + 1 < blocks) sums(s1, (kb + 1) & 1);
+    multiply(kb, st, kb & 1);
+    st = s1;
+  }
+  // the adapters: t lies in two pieces of bf16, B_cat is exact in one (fp16: in two)
+  const bf16_t* th = (const bf16_t*)p.t;
+  for (int r = 0; r < p.R; r += 32) {
+    bf16x8 bh[MR_N], bl[MR_N];
+#pragma unroll
+    for (int j = 0; j < MR_N; ++j) {
+      T v[8];
+      const long n = nb + (j * 16 + l < (int)last ? j * 16 + l : (int)last);
+      __builtin_memcpy(v, (const T*)p.b_cat + n * p.R + r + g * 8, sizeof(v));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        bh[j][e] = (bf16_t)(float)v[e];
+        bl[j][e] = (bf16_t)((float)v[e] - (float)bh[j][e]);
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < MR_M; ++b) {
+      const int r0 = b * 16 + l;
+      const bf16_t* at = th + (m0 + (r0 < rows ? r0 : rows - 1)) * p.R + r + g * 8;
+      const bf16x8 hi = *reinterpret_cast<const bf16x8*>(at), lo = *reinterpret_cast<const bf16x8*>(at + p.M * p.R);
+#pragma unroll
+      for (int j = 0; j < MR_N; ++j) {
+        out[b][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, bh[j], out[b][j], 0, 0, 0);
+        out[b][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, bh[j], out[b][j], 0, 0, 0);
+        if constexpr (sizeof(T) == 2 && !__is_same(T, bf16_t)) out[b][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, bl[j], out[b][j], 0, 0, 0);
+      }
+    }
+  }
+  barrier();                                  // the stages are dead
+  float* mine = reinterpret_cast<float*>(smem) + wave * (MR_M * 16 * Sg::PITCH);
+#pragma unroll
+  for (int b = 0; b < MR_M; ++b)
+#pragma unroll
+    for (int j = 0; j < MR_N; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mine[(b * 16 + g * 4 + e) * Sg::PITCH + j * 16 + l] = out[b][j][e];
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");         // (written and read by this wave alone)
+  if (!some) return;
+  const int c = (lane & 7) * 8;               // a lane's eight columns of eight rows at a time
+  const long n = n0 + c;
+  float bias[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) bias[e] = p.bias && n + e < p.N ? (float)((const T*)p.bias)[n + e] : 0.f;
+  const bool vec = n + 8 <= p.N;
+  for (int r = lane >> 3; r < rows; r += 8) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) {
+      const f32x4 t = *reinterpret_cast<const f32x4*>(mine + r * Sg::PITCH + c + e);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[e + i] = t[i] + bias[e + i];
+    }
+    const long at = (m0 + r) * p.N + n;
+    if (p.residual) {
+      T res[8];
+      load8<T>((const T*)p.residual + at, p.N - n, res);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += (float)res[e];
+    }
+    T o[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = (T)v[e];
+    if (vec) {
+      __builtin_memcpy((T*)p.y + at, o, sizeof(o));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (n + e < p.N) ((T*)p.y)[at + e] = o[e];
+    }
+  }
+#endif
 }
 
 // t[split][m][r] = col_scale[r] * sum over the split's k of x[m][k] A[r][k], in 32 bits: grid (R / 16, M / 16, splits)
@@ -297,10 +724,12 @@ struct ShrinkParams {
   float* t;
   long M;
   int K, R, per;           // per: k of a split, a multiple of 32
+  int pieces;              // one split, and t in two pieces of bf16 [2][M][R] instead
 };
+constexpr int SW = 8;      // waves of a workgroup
 template <typename T>
-__global__ __launch_bounds__(LW * 64) void w4_shrink(const ShrinkParams p) {
-  __shared__ float part[LW][16][17];
+__global__ __launch_bounds__(SW * 64) void w4_shrink(const ShrinkParams p) {
+  __shared__ float part[SW][16][17];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int l = lane & 15, g = lane >> 4;
   const int r0 = blockIdx.x * 16;
@@ -309,7 +738,7 @@ __global__ __launch_bounds__(LW * 64) void w4_shrink(const ShrinkParams p) {
   const T* xr = (const T*)p.x + (m0 + l < p.M ? m0 + l : p.M - 1) * p.K;
   const int k0 = blockIdx.z * p.per, k1 = k0 + p.per < p.K ? k0 + p.per : p.K;
   f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int k = k0 + wave * 32; k < k1; k += LW * 32) {
+  for (int k = k0 + wave * 32; k < k1; k += SW * 32) {
     T a[8], x[8];
     load8<T>(ar + k + g * 8, (long)k1 - k - g * 8, a);
     load8<T>(xr + k + g * 8, (long)k1 - k - g * 8, x);
@@ -322,43 +751,83 @@ __global__ __launch_bounds__(LW * 64) void w4_shrink(const ShrinkParams p) {
     const int r = threadIdx.x >> 4, col = threadIdx.x & 15;
     float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < LW; ++w) v += part[w][r][col];
-    if (m0 + r < p.M) p.t[((long)blockIdx.z * p.M + m0 + r) * p.R + r0 + col] = v * p.col_scale[r0 + col];
+    for (int w = 0; w < SW; ++w) v += part[w][r][col];
+    if (m0 + r >= p.M) return;
+    v *= p.col_scale[r0 + col];
+    if (p.pieces) {
+      bf16_t* t = (bf16_t*)p.t + (m0 + r) * p.R + r0 + col;
+      const bf16_t hi = (bf16_t)v;
+      t[0] = hi;
+      t[p.M * p.R] = (bf16_t)(v - (float)hi);
+    } else {
+      p.t[((long)blockIdx.z * p.M + m0 + r) * p.R + r0 + col] = v;
+    }
   }
 }
 
 int shrink_splits(long M, long K, long R) {
-  // enough workgroups that the rows of A are read by many CUs at once, at least 1024 of k each
+  // enough workgroups that the rows of A are read by many CUs at once, at least 512 of k each (two steps of a wave)
   const long tiles = R / 16 * ((M + 15) / 16);
-  long s = tiles >= 64 ? 1 : 64 / tiles;
-  const long most = (K + 1023) / 1024;
+  long s = tiles >= 128 ? 1 : 128 / tiles;
+  const long most = (K + 511) / 512;
   if (s > most) s = most;
-  if (s > 8) s = 8;
+  if (s > 16) s = 16;
   return (int)(s < 1 ? 1 : s);
 }
 
-template <typename T, int G, bool ZERO>
-void launch_few(const LinParams& p, hipStream_t s) {
-  const unsigned nb = (unsigned)((p.N + 15) / 16);
-  const long mt = (p.M + 15) / 16;
-  auto go = [&](auto kernel, int mb) {
-    kh_launch(KH_TAG_W4_LINEAR, kernel, dim3(nb, (unsigned)((mt + mb - 1) / mb)), dim3(LW * 64), (size_t)LW * mb * 16 * 17 * 4, s, p);
-  };
-  if (mt == 1) go(w4_few_rows<T, G, ZERO, 1>, 1);
-  else if (mt == 2) go(w4_few_rows<T, G, ZERO, 2>, 2);
-  else go(w4_few_rows<T, G, ZERO, 4>, 4);
-}
-template <typename T>
-void launch_linear(const LinParams& p, int G, hipStream_t s) {
-  if (p.zero) {
-    if (G == 32) launch_few<T, 32, true>(p, s);
-    else if (G == 64) launch_few<T, 64, true>(p, s);
-    else launch_few<T, 128, true>(p, s);
-  } else {
-    if (G == 32) launch_few<T, 32, false>(p, s);
-    else if (G == 64) launch_few<T, 64, false>(p, s);
-    else launch_few<T, 128, false>(p, s);
+template <typename T, int G, bool ZERO, int MB, int NB, int LW, int ST, bool FOUR>
+int launch_few_as(const LinParams& p, hipStream_t s) {
+  const long mt = (p.M + MB * 16 - 1) / (MB * 16), rows = p.M < MB * 16 ? p.M : MB * 16;
+  const int ring = LW * ST * Stage<G, ZERO, MB, NB, FOUR>::BYTES, part = LW * (int)rows * (NB * 16 + 1) * 4, lds = ring > part ? ring : part;
+  if (lds > 65536) {
+    const hipError_t e = kh_allow_lds<w4_few_rows<T, G, ZERO, MB, NB, LW, ST, FOUR>>(lds);
+    if (e != hipSuccess) return (int)e;
   }
+  kh_launch(KH_TAG_W4_LINEAR, w4_few_rows<T, G, ZERO, MB, NB, LW, ST, FOUR>, dim3((unsigned)((p.N + NB * 16 - 1) / (NB * 16)), (unsigned)mt), dim3(LW * 64), lds, s, p);
+  return KH_OK;
+}
+// Tiles of 16 columns to a workgroup: as few as leave every CU at most one workgroup, up to four (a tile's columns share the loads of x).  Waves and stages
+// as measured over N 320 .. 16384, K 640 .. 8192 (us, cold codes, groups of 64, tiles 1 | 2 | 4): one row 8192 x 8192 12.1 | 9.6 | 13.9, 16384 x 8192 21.7 | 18.4 | 18.7,
+// 1280 x 5120 4.9 | 6.0 | 8.9; 16 rows 5120 x 1280 5.6 | 4.6 | 5.7, 10240 x 1280 7.6 | 6.7 | 5.8, 16384 x 8192 45 | 30 | 24.6; 32 rows 16384 x 8192 73 | 46 | 33.
+// Four, eight or sixteen waves and two, three or four stages are within 0.5 us of one another where LDS lets two workgroups on a CU or there is only one.
+template <typename T, int G, bool ZERO>
+int launch_few(const LinParams& p, hipStream_t s) {
+  const long nb = (p.N + 15) / 16;
+  if (p.M <= 4) {
+    if (nb <= 256) return launch_few_as<T, G, ZERO, 1, 1, 8, 3, true>(p, s);
+    if (nb <= 512) return launch_few_as<T, G, ZERO, 1, 2, 8, 3, true>(p, s);
+    return launch_few_as<T, G, ZERO, 1, 4, 8, 2, true>(p, s);
+  }
+  if (p.M <= 16) {
+    if (nb <= 256) return launch_few_as<T, G, ZERO, 1, 1, 8, 2, false>(p, s);
+    if (nb <= 512) return launch_few_as<T, G, ZERO, 1, 2, 4, 3, false>(p, s);
+    return launch_few_as<T, G, ZERO, 1, 4, 8, 2, false>(p, s);
+  }
+  if (nb <= 256) return launch_few_as<T, G, ZERO, 2, 1, 4, 2, false>(p, s);
+  if (nb <= 512) return launch_few_as<T, G, ZERO, 2, 2, 4, 2, false>(p, s);
+  return launch_few_as<T, G, ZERO, 2, 4, 4, 2, false>(p, s);
+}
+template <typename T, int G, bool ZERO>
+int launch_many(const LinParams& p, hipStream_t s) {
+  const hipError_t e = kh_allow_lds<w4_many_rows<T, G, ZERO>>(ManyStage<G, ZERO>::LDS);
+  if (e != hipSuccess) return (int)e;
+  const long units = (p.M + MR_M * 16 - 1) / (MR_M * 16) * ((p.N + MR_W * MR_N * 16 - 1) / (MR_W * MR_N * 16));
+  kh_launch(KH_TAG_W4_LINEAR, w4_many_rows<T, G, ZERO>, dim3((unsigned)units), dim3(MR_W * 64), ManyStage<G, ZERO>::LDS, s, p);
+  return KH_OK;
+}
+bool many_rows(long M, long N, long K) {
+  const long units = (M + MR_M * 16 - 1) / (MR_M * 16) * ((N + MR_W * MR_N * 16 - 1) / (MR_W * MR_N * 16));
+  return M > 64 && units >= 64;
+}
+
+template <typename T>
+int launch_linear(const LinParams& p, int G, hipStream_t s) {
+  if (many_rows(p.M, p.N, p.K)) {
+    if (p.zero) return G == 32 ? launch_many<T, 32, true>(p, s) : G == 64 ? launch_many<T, 64, true>(p, s) : launch_many<T, 128, true>(p, s);
+    return G == 32 ? launch_many<T, 32, false>(p, s) : G == 64 ? launch_many<T, 64, false>(p, s) : launch_many<T, 128, false>(p, s);
+  }
+  if (p.zero) return G == 32 ? launch_few<T, 32, true>(p, s) : G == 64 ? launch_few<T, 64, true>(p, s) : launch_few<T, 128, true>(p, s);
+  return G == 32 ? launch_few<T, 32, false>(p, s) : G == 64 ? launch_few<T, 64, false>(p, s) : launch_few<T, 128, false>(p, s);
 }
 
 bool group_ok(int64_t g) { return g == 32 || g == 64 || g == 128; }
@@ -413,19 +882,21 @@ KH_EXPORT int kh_w4_linear(const void* x, const void* q, const void* scale, cons
   if (R > 128 || K > (1L << 24) || N > (1L << 24) || (M + 15) / 16 > 65535) return KH_ERR_TOO_LARGE;
   if (!kh_aligned16(q) || !kh_aligned16(scale)) return KH_ERR_ALIGNMENT;
   hipStream_t s = (hipStream_t)stream;
-  const int splits = R > 0 ? shrink_splits(M, K, R) : 0;
+  const bool many = many_rows(M, N, K);
+  const int splits = R == 0 ? 0 : many ? 1 : shrink_splits(M, K, R);
   if (R > 0) {
     const int per = (int)(((K + splits - 1) / splits + 31) / 32 * 32);
-    ShrinkParams sp{x, a_cat, col_scale, (float*)workspace, (long)M, (int)K, (int)R, per};
+    ShrinkParams sp{x, a_cat, col_scale, (float*)workspace, (long)M, (int)K, (int)R, per, many};
     const dim3 grid((unsigned)(R / 16), (unsigned)((M + 15) / 16), (unsigned)splits);
-    if (type == 0) kh_launch(KH_TAG_W4_SHRINK, w4_shrink<bf16_t>, grid, dim3(LW * 64), 0, s, sp);
-    else kh_launch(KH_TAG_W4_SHRINK, w4_shrink<_Float16>, grid, dim3(LW * 64), 0, s, sp);
+    if (type == 0) kh_launch(KH_TAG_W4_SHRINK, w4_shrink<bf16_t>, grid, dim3(SW * 64), 0, s, sp);
+    else kh_launch(KH_TAG_W4_SHRINK, w4_shrink<_Float16>, grid, dim3(SW * 64), 0, s, sp);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
   }
   LinParams p{x, (const uint8_t*)q, (const bf16_t*)scale, (const uint8_t*)zero, bias, b_cat, residual, (const float*)workspace, y, (long)M,
-              (long)N, (int)K, (int)R, splits, (int)((K + 31) / 32 * 16), (int)(((K + group - 1) / group + 3) / 4 * 4)};
-  if (type == 0) launch_linear<bf16_t>(p, (int)group, s);
-  else launch_linear<_Float16>(p, (int)group, s);
+              (long)N, (int)K, (int)R, splits, (int)((K + 31) / 32 * 16), (int)(((K + group - 1) / group + 3) / 4 * 4),
+              ((uintptr_t)x & 3) == 0 && K % 2 == 0};
+  const int rc = type == 0 ? launch_linear<bf16_t>(p, (int)group, s) : launch_linear<_Float16>(p, (int)group, s);
+  if (rc != KH_OK) return rc;
   KH_RETURN_LAST_ERROR();
 }

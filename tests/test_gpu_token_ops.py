@@ -282,6 +282,21 @@ LINEAR_CASES = [
     (300, 257, 333, 32, True, 32, True, True, BF),
     (129, 512, 1280, 128, True, 128, False, True, FP16),
     (616, 384, 1280, 64, False, 96, True, False, BF),
+    (3, 5000, 1001, 64, True, 32, True, False, BF),        # rows of x on odd addresses, 313 tiles of columns
+    (4, 8200, 3001, 32, False, 0, False, True, FP16),
+    (9, 9000, 640, 128, True, 64, False, False, BF),
+    (16, 6001, 385, 32, True, 0, True, False, BF),
+    (2, 40, 20000, 128, True, 128, False, False, FP16),    # many blocks to a wave
+    (30, 8300, 514, 64, True, 32, False, True, BF),
+    (20, 5000, 1536, 128, False, 0, True, False, FP16),
+    # many rows
+    (130, 8200, 200, 64, False, 32, True, True, BF),
+    (1100, 2050, 385, 32, True, 96, True, True, FP16),
+    (1030, 1800, 1280, 128, True, 128, False, False, BF),
+    (616, 4000, 640, 64, False, 0, True, False, BF),
+    (200, 8209, 130, 128, False, 64, False, True, BF),
+    (70, 16500, 64, 64, True, 0, True, False, FP16),
+    (513, 3330, 1000, 32, False, 64, True, True, BF),
     (200, 1000, 96, 32, False, 0, False, True, BF),
 ]
 
