@@ -13,7 +13,7 @@
 
 namespace {
 
-constexpr int C = 64;          // tokens of a block, columns of v of a workgroup
+constexpr int C = 64;          // tokens of a block; columns of v of four waves
 
 struct LaParams {
   const bf16_t *q, *k, *v;
@@ -23,7 +23,7 @@ struct LaParams {
   float* s_out;
   const int32_t* seg_start;    // NULL: [B][T] rows through batch strides
   const int32_t* slots;
-  float* ws;                   // [unit][segment][dk * 64]: a segment's gain, then the state before it
+  float* ws;                   // [unit][segment][dk * TV]: a segment's gain, then the state before it
   long ldq, ldk, ldv, ldo, bsq, bsk, bsv, bso;
   long rows;                   // of packed tensors
   int B, H, share;             // share: query heads of a key head
@@ -31,17 +31,18 @@ struct LaParams {
   float scale;
 };
 
-struct Unit {                  // one (sequence, head, 64 columns of v)
+struct Unit {                  // one (sequence, head, range of columns of v)
   int b, h, tile, len, slot;
   long q0, k0, v0, o0;         // first elements
   float g;
 };
 
-__device__ __forceinline__ bool unit_of(const LaParams& p, long u, int DK, Unit& r) {
-  const int tiles = p.dv / C;
-  r.tile = (int)(u % tiles);
-  r.h = (int)(u / tiles % p.H);
-  r.b = (int)(u / tiles / p.H);
+// TV: columns of v of a unit
+__device__ __forceinline__ bool unit_of(const LaParams& p, int b, int ht, int DK, int TV, Unit& r) {
+  const int tiles = p.dv / TV;
+  r.tile = ht % tiles;
+  r.h = ht / tiles;
+  r.b = b;
   r.slot = p.slots ? p.slots[r.b] : r.b;
   if (r.slot < 0 || r.slot >= p.n_slots) return false;
   long row = 0;
@@ -58,8 +59,8 @@ __device__ __forceinline__ bool unit_of(const LaParams& p, long u, int DK, Unit&
   const int hk = r.h / p.share;
   r.q0 += row * p.ldq + (long)r.h * DK;
   r.k0 += row * p.ldk + (long)hk * DK;
-  r.v0 += row * p.ldv + (long)hk * p.dv + r.tile * C;
-  r.o0 += row * p.ldo + (long)r.h * p.dv + r.tile * C;
+  r.v0 += row * p.ldv + (long)hk * p.dv + r.tile * TV;
+  r.o0 += row * p.ldo + (long)r.h * p.dv + r.tile * TV;
   const float g = p.log_decay[r.h];
   r.g = g < -1.0e4f ? -1.0e4f : g;     // (-inf, no memory at all, times a distance of 0 would be no number)
   return true;
@@ -73,249 +74,378 @@ __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
 #endif
 }
 
-typedef __attribute__((address_space(3))) bf16x4* ltr_t;
+typedef __attribute__((address_space(3))) void* lptr_t;
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
 
-// Element i of rows r .. r+3 and r+4 .. r+7 (i = lane % 16) of a bf16 tile in LDS: at = address of row (lane%16)/4 of the first four,
-// column 4 (lane % 4) of the sixteen.
-__device__ __forceinline__ bf16x8 transposed(const char* at, int row_bytes) {
-  bf16x8 v;
+__device__ __forceinline__ void wait_all_loads() {
+  __builtin_amdgcn_s_waitcnt(0 | (7 << 4) | (15 << 8));   // vmcnt = 0, the other counters unconstrained (gfx9 encoding)
+  asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void barrier() {                // what this wave has written to LDS is there, and everybody has arrived
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// A block's 64 x W tile in LDS, rows unpadded (they come by DMA), their 16-byte pieces swizzled so that the 16 rows of an operand lie on
+// different banks.
+template <int W>
+struct Tile {
+  static constexpr int PIECES = W / 8, ROW = W * 2, BYTES = C * ROW;
+  static __device__ __forceinline__ int swz(int row) { return row & (PIECES < 16 ? PIECES - 1 : 15); }
+  // rows 0 .. left-1 from src (rows behind them: zeros), NW waves
+  template <int NW>
+  static __device__ __forceinline__ void fetch(const bf16_t* src, long ld, int left, char* dst) {
 #if __HIP_DEVICE_COMPILE__
-  const bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((ltr_t)(at));
-  const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((ltr_t)(at + 4 * row_bytes));
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16_t*>(src), 0, (int)(uint32_t)((((left < C ? left : C) - 1) * ld + W) * 2), 0x00020000);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) { v[e] = a[e]; v[4 + e] = b[e]; }
+    for (int i = 0; i < BYTES / 1024 / NW; ++i) {
+      const int id = (wave * (BYTES / 1024 / NW) + i) * 64 + lane, row = id / PIECES, piece = (id % PIECES) ^ swz(row);
+      // (rows of 2^24 elements and more are refused, so offsets stay below 2^32; a row behind the last gets one that lies outside the buffer)
+      const uint32_t off = row < left ? (uint32_t)row * (uint32_t)ld * 2u + (uint32_t)piece * 16u : 0xfffffff0u;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lptr_t)(dst + (wave * (BYTES / 1024 / NW) + i) * 1024), 16, off, 0, 0, 0);
+    }
 #endif
-  return v;
-}
-
-// The 64 x W tile of rows t0 .. t0+63 of a sequence into LDS (row pitch PITCH bytes); rows at and behind len are zero.
-template <int W, int PITCH>
-__device__ __forceinline__ void tile_in(const bf16_t* src, long ld, int t0, int len, char* dst) {
-#pragma unroll
-  for (int i = 0; i < C * W / 8 / 256; ++i) {
-    const int id = i * 256 + threadIdx.x, row = id / (W / 8), piece = id % (W / 8);
-    u32x4 v = u32x4{0, 0, 0, 0};
-    if (t0 + row < len) v = *reinterpret_cast<const u32x4*>(src + (long)(t0 + row) * ld + piece * 8);
-    *reinterpret_cast<u32x4*>(dst + row * PITCH + piece * 16) = v;
   }
-}
+  // operand whose lane has row `row`, eight elements from column c (a multiple of 8)
+  static __device__ __forceinline__ bf16x8 rows8(const char* t, int row, int c) {
+    return *reinterpret_cast<const bf16x8*>(t + row * ROW + ((c / 8) ^ swz(row)) * 16);
+  }
+  static __device__ __forceinline__ bf16x4 rows4(const char* t, int row, int c) {     // four elements from column c
+    return *reinterpret_cast<const bf16x4*>(t + row * ROW + ((c / 8) ^ swz(row)) * 16 + (c & 4) * 2);
+  }
+  // LDS addresses, for columns(), of row 8 (lane / 16) + (lane % 16) / 4 and of the row four further: a transposing read gives lane i of 16 the i-th element
+  // of four rows, of which lanes 4 r .. 4 r + 3 address the r-th
+  static __device__ __forceinline__ void column_rows(const char* t, uint32_t (&at)[2]) {
+#if __HIP_DEVICE_COMPILE__
+    const int lane = threadIdx.x & 63, l = lane & 15;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = 8 * (lane >> 4) + (l >> 2) + 4 * h;
+      at[h] = (uint32_t)(uintptr_t)(lptr_t)(const_cast<char*>(t)) + row * ROW + (((l & 3) >> 1) ^ swz(row)) * 16 + (l & 1) * 8;
+    }
+#endif
+  }
+  // N operands whose lanes have the columns 16 (t0 + n) + lane % 16 of rows 32 s + 8 (lane / 16) .. + 7, s = 0, 1.  The reads are written out, with their wait:
+  // in front of one of its own the compiler waits for every load that is on its way to LDS, the next block's among them.
+  template <int N>
+  static __device__ __forceinline__ void columns(const uint32_t (&at)[2], int t0, bf16x8 (&v)[N][2]) {
+#if __HIP_DEVICE_COMPILE__
+    static_assert(N == 1 || N == 2, "one or two tiles of columns");
+    u32x2 r[N][4];
+    const uint32_t a0 = at[0] ^ (uint32_t)(t0 << 5), b0 = at[1] ^ (uint32_t)(t0 << 5);
+    if constexpr (N == 1) {
+      asm volatile("ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %5\n\tds_read_b64_tr_b16 %2, %4 offset:%6\n\tds_read_b64_tr_b16 %3, %5 offset:%6\n\t"
+                   "s_waitcnt lgkmcnt(0)"
+                   : "=&v"(r[0][0]), "=&v"(r[0][1]), "=&v"(r[0][2]), "=&v"(r[0][3]) : "v"(a0), "v"(b0), "i"(32 * ROW) : "memory");
+    } else {
+      const uint32_t a1 = at[0] ^ (uint32_t)((t0 + 1) << 5), b1 = at[1] ^ (uint32_t)((t0 + 1) << 5);
+      asm volatile("ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %9\n\tds_read_b64_tr_b16 %2, %8 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
+                   "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %11\n\tds_read_b64_tr_b16 %6, %10 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\t"
+                   "s_waitcnt lgkmcnt(0)"
+                   : "=&v"(r[0][0]), "=&v"(r[0][1]), "=&v"(r[0][2]), "=&v"(r[0][3]), "=&v"(r[1][0]), "=&v"(r[1][1]), "=&v"(r[1][2]), "=&v"(r[1][3])
+                   : "v"(a0), "v"(b0), "v"(a1), "v"(b1), "i"(32 * ROW) : "memory");
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) v[n][s] = __builtin_bit_cast(bf16x8, u32x4{r[n][2 * s][0], r[n][2 * s][1], r[n][2 * s + 1][0], r[n][2 * s + 1][1]});
+#endif
+  }
+};
 
-// A state (or a segment's gain) in registers: wave w has the columns 16 w .. 16 w + 15 of the 64, lane l of a group g rows 16 t + 4 g + r of column l.
+// A state (or a segment's gain) in registers: wave w has the columns 16 w .. 16 w + 15, lane l of a group g rows 16 t + 4 g + r of column l.
 template <int DK>
 struct State {
   f32x4 s[DK / 16];
 };
 
-template <int DK>
-struct Shape {
-  static constexpr int KP = DK * 2 + 16, VP = C * 2 + 16, PP = C * 2 + 16;   // pitches in bytes: 16-byte pieces of neighbouring rows on other banks
-};
-
-// S = lambda^n S + sum_j lambda^(n-1-j) k_j v_j^T over the n tokens of a block whose K and V lie in LDS.
-template <int DK>
-__device__ __forceinline__ void add_block(State<DK>& st, const char* kt, const char* vt, int n, float g) {
-  typedef Shape<DK> Sh;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, grp = lane >> 4;
-  bf16x8 v[2][3];
+// lambda^(n-1-j) of the tokens j = 32 s + 8 g + e of a block of n
+__device__ __forceinline__ void powers(float g, int n, float (&w)[2][8]) {
+  const int grp = (threadIdx.x & 63) >> 4;
 #pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    const bf16x8 raw = transposed(vt + (32 * s + 8 * grp + (l >> 2)) * Sh::VP + wave * 32 + (l & 3) * 8, Sh::VP);
+  for (int s = 0; s < 2; ++s)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int left = n - 1 - (32 * s + 8 * grp + e);
-      float w = (float)raw[e] * expf(g * (float)(left < 0 ? 0 : left));
+      w[s][e] = expf(g * (float)(left < 0 ? 0 : left));
+    }
+}
+
+// S = decay S + sum_j w_j k_j v_j^T over a block whose K and V lie in LDS; decayed values in PIECES pieces of bf16.
+template <int DK, int TV, int PIECES>
+__device__ __forceinline__ void add_block(State<DK>& st, const char* kt, const char* vt, float decay, const float (&w)[2][8]) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  bf16x8 v[2][PIECES], raw[1][2];
+  uint32_t at[2];
+  Tile<TV>::column_rows(vt, at);
+  Tile<TV>::template columns<1>(at, wave, raw);
 #pragma unroll
-      for (int i = 0; i < 3; ++i) {
-        v[s][i][e] = (bf16_t)w;
-        w -= (float)v[s][i][e];
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float x = (float)raw[0][s][e] * w[s][e];
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        v[s][i][e] = (bf16_t)x;
+        x -= (float)v[s][i][e];
       }
     }
-  }
-  const float decay = expf(g * (float)n);
+  Tile<DK>::column_rows(kt, at);
 #pragma unroll
-  for (int t = 0; t < DK / 16; ++t) {
+  for (int t = 0; t < DK / 16; t += 2) {
+    bf16x8 k[2][2];
+    Tile<DK>::template columns<2>(at, t, k);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) st.s[t][e] *= decay;
+    for (int n = 0; n < 2; ++n) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const bf16x8 k = transposed(kt + (32 * s + 8 * grp + (l >> 2)) * Sh::KP + t * 32 + (l & 3) * 8, Sh::KP);
+      for (int e = 0; e < 4; ++e) st.s[t + n][e] *= decay;
 #pragma unroll
-      for (int i = 0; i < 3; ++i) st.s[t] = mfma(k, v[s][i], st.s[t]);
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) st.s[t + n] = mfma(k[n][s], v[s][i], st.s[t + n]);
     }
   }
 }
 
-// The state of a slot, dk x dv in rows, to and from the registers' order.
+// Row 16 t + 4 g of column l of a wave's share of a slot's state, dk x dv in rows.
+template <int DK, int TV>
+__device__ __forceinline__ long state_at(const LaParams& p, const Unit& u, int wave, int t) {
+  const int lane = threadIdx.x & 63;
+  return (((long)u.slot * p.H + u.h) * DK + 16 * t + 4 * (lane >> 4)) * p.dv + u.tile * TV + wave * 16 + (lane & 15);
+}
 template <int DK>
-__device__ __forceinline__ long state_at(const LaParams& p, const Unit& u, int t) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  return (((long)u.slot * p.H + u.h) * DK + 16 * t + 4 * (lane >> 4)) * p.dv + u.tile * C + wave * 16 + (lane & 15);
+__device__ __forceinline__ int ws_at(int wave, int t) { return ((wave * (DK / 16) + t) * 64 + (threadIdx.x & 63)) * 4; }
+
+// The workgroup's unit and segment.  Units that share keys and values are neighbours on one XCD; such clusters go round the eight, segment by segment, since
+// sequences differ in length.
+template <int DK, int TV>
+__device__ __forceinline__ bool work_of(const LaParams& p, Unit& u, int& sg, long& unit) {
+  const uint32_t tiles = (uint32_t)(p.dv / TV), size = tiles * (uint32_t)p.share, kv = (uint32_t)p.H / (uint32_t)p.share;
+  const uint32_t local = blockIdx.x / 8, cluster = local / size * 8 + blockIdx.x % 8, rest = cluster / kv;
+  const uint32_t b = rest / (uint32_t)p.nseg;
+  if (b >= (uint32_t)p.B) return false;
+  sg = (int)(rest % (uint32_t)p.nseg);
+  const int ht = (int)((cluster % kv) * size + local % size);
+  unit = (long)b * ((long)p.H * tiles) + ht;
+  return unit_of(p, (int)b, ht, DK, TV, u);
 }
 
-template <int DK>
-__global__ __launch_bounds__(256) void la_gain(const LaParams p) {
-  typedef Shape<DK> Sh;
-  __shared__ __attribute__((aligned(16))) char kt[C * Sh::KP], vt[C * Sh::VP];
+template <int DK, int TV>
+__global__ __launch_bounds__(TV * 4) void la_gain(const LaParams p) {
+  constexpr int NW = TV / 16, STAGE = Tile<DK>::BYTES + Tile<TV>::BYTES;
+  extern __shared__ __attribute__((aligned(16))) char smem[];   // two stages of K, V
   Unit u;
-  const long unit = blockIdx.x / p.nseg;
-  const int sg = (int)(blockIdx.x % p.nseg);
-  if (!unit_of(p, unit, DK, u)) return;
+  int sg;
+  long unit;
+  if (!work_of<DK, TV>(p, u, sg, unit)) return;
   const int t0 = sg * p.seg, t1 = u.len < t0 + p.seg ? u.len : t0 + p.seg;
   if (t0 >= t1) return;
+  auto fetch = [&](int c, int st) {
+    Tile<DK>::template fetch<NW>(p.k + u.k0 + (long)c * p.ldk, p.ldk, t1 - c, smem + st * STAGE);
+    Tile<TV>::template fetch<NW>(p.v + u.v0 + (long)c * p.ldv, p.ldv, t1 - c, smem + st * STAGE + Tile<DK>::BYTES);
+  };
+  fetch(t0, 0);
   State<DK> st;
 #pragma unroll
   for (int t = 0; t < DK / 16; ++t) st.s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int c = t0; c < t1; c += C) {
-    tile_in<DK, Sh::KP>(p.k + u.k0, p.ldk, c, t1, kt);
-    tile_in<C, Sh::VP>(p.v + u.v0, p.ldv, c, t1, vt);
-    __syncthreads();
-    add_block<DK>(st, kt, vt, t1 - c < C ? t1 - c : C, u.g);
-    __syncthreads();
+  float w[2][8];
+  powers(u.g, C, w);
+  float decay = expf(u.g * (float)C);
+  for (int c = t0, i = 0; c < t1; c += C, i ^= 1) {
+    wait_all_loads();
+    barrier();                             // everybody's share of this block; and nobody reads the block before any more
+    if (c + C < t1) fetch(c + C, i ^ 1);
+    if (t1 - c < C) {
+      powers(u.g, t1 - c, w);
+      decay = expf(u.g * (float)(t1 - c));
+    }
+    add_block<DK, TV, 3>(st, smem + i * STAGE, smem + i * STAGE + Tile<DK>::BYTES, decay, w);
   }
-  float* w = p.ws + (unit * p.nseg + sg) * (DK * C);
+  float* ws = p.ws + (unit * p.nseg + sg) * (DK * TV);
 #pragma unroll
-  for (int t = 0; t < DK / 16; ++t) *reinterpret_cast<f32x4*>(w + (((threadIdx.x >> 6) * (DK / 16) + t) * 64 + (threadIdx.x & 63)) * 4) = st.s[t];
+  for (int t = 0; t < DK / 16; ++t) *reinterpret_cast<f32x4*>(ws + ws_at<DK>(threadIdx.x >> 6, t)) = st.s[t];
 }
 
 // Gains to the states before each segment, in place; the state behind the last one to its slot.  A thread has the four rows of la_gain's lane: grid
 // (DK / 16, units).
-template <int DK>
-__global__ __launch_bounds__(256) void la_scan(const LaParams p) {
+template <int DK, int TV>
+__global__ __launch_bounds__(TV * 4) void la_scan(const LaParams p) {
   Unit u;
-  if (!unit_of(p, blockIdx.y, DK, u)) return;
-  const int t = blockIdx.x;
-  const long at = state_at<DK>(p, u, t);
+  const int heads = p.H * (p.dv / TV);
+  if (!unit_of(p, blockIdx.y / heads, blockIdx.y % heads, DK, TV, u)) return;
+  const int t = blockIdx.x, wave = threadIdx.x >> 6;
+  const long at = state_at<DK, TV>(p, u, wave, t);
   f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
   if (p.s_in)
 #pragma unroll
     for (int r = 0; r < 4; ++r) s[r] = p.s_in[at + (long)r * p.dv];
-  float* w = p.ws + (long)blockIdx.y * p.nseg * (DK * C) + (((threadIdx.x >> 6) * (DK / 16) + t) * 64 + (threadIdx.x & 63)) * 4;
-  for (int sg = 0; sg * p.seg < u.len; ++sg, w += DK * C) {
-    const f32x4 gain = *reinterpret_cast<const f32x4*>(w);
-    *reinterpret_cast<f32x4*>(w) = s;
-    const int n = u.len - sg * p.seg < p.seg ? u.len - sg * p.seg : p.seg;
-    const float d = expf(u.g * (float)n);
+  float* w = p.ws + (long)blockIdx.y * p.nseg * (DK * TV) + ws_at<DK>(wave, t);
+  const int n = (u.len + p.seg - 1) / p.seg;
+  const float d = expf(u.g * (float)p.seg), dl = expf(u.g * (float)(u.len - (n - 1) * p.seg));
+  for (int s0 = 0; s0 < n; s0 += 4) {      // four gains on their way at a time
+    f32x4 gain[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) s[r] = fmaf(d, s[r], gain[r]);
+    for (int i = 0; i < 4; ++i)
+      if (s0 + i < n) gain[i] = *reinterpret_cast<const f32x4*>(w + (long)(s0 + i) * (DK * TV));
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (s0 + i < n) {
+        *reinterpret_cast<f32x4*>(w + (long)(s0 + i) * (DK * TV)) = s;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[r] = fmaf(s0 + i == n - 1 ? dl : d, s[r], gain[i][r]);
+      }
   }
 #pragma unroll
   for (int r = 0; r < 4; ++r) p.s_out[at + (long)r * p.dv] = s[r];
 }
 
-// A segment's outputs from the state before it.  nseg == 1: the whole sequence from the slot's state, whose successor it leaves.
-template <int DK>
-__global__ __launch_bounds__(256) void la_out(const LaParams p) {
-  typedef Shape<DK> Sh;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  char* kt = smem;                         // [64][KP]
-  char* qt = kt + C * Sh::KP;
-  char* vt = qt + C * Sh::KP;              // [64][VP]
-  char* ph = vt + C * Sh::VP;              // [64][PP]: decayed scores, upper and lower pieces
-  char* pl = ph + C * Sh::PP;
+// A segment's outputs from the state before it.  ONE: the whole sequence from the slot's state, whose successor it leaves.
+template <int DK, int TV>
+struct OutShape {
+  static constexpr int PP = C * 2 + 16;    // pitch of the scores in bytes: 16-byte pieces of neighbouring rows on other banks
+  static constexpr int STAGE = 2 * Tile<DK>::BYTES + Tile<TV>::BYTES, LDS = 2 * STAGE + 2 * C * PP;
+};
+template <int DK, int TV, bool ONE>
+__global__ __launch_bounds__(TV * 4) void la_out(const LaParams p) {
+  typedef OutShape<DK, TV> Sh;
+  constexpr int NW = TV / 16;
+  extern __shared__ __attribute__((aligned(16))) char smem[];   // two stages of K, Q, V; decayed scores, upper and lower pieces
+  char* const ph = smem + 2 * Sh::STAGE;
+  char* const pl = ph + C * Sh::PP;
   Unit u;
-  const long unit = blockIdx.x / p.nseg;
-  const int sg = (int)(blockIdx.x % p.nseg);
-  if (!unit_of(p, unit, DK, u)) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, grp = lane >> 4;
-  const int t0 = sg * p.seg, t1 = u.len < t0 + p.seg ? u.len : t0 + p.seg;
+  int sg;
+  long unit;
+  if (!work_of<DK, TV>(p, u, sg, unit)) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 15, grp = lane >> 4;
+  const int t0 = sg * p.seg, t1 = ONE || u.len < t0 + p.seg ? u.len : t0 + p.seg;
+  if (!ONE && t0 >= t1) return;
+  auto fetch = [&](int c, int st) {
+    char* to = smem + st * Sh::STAGE;
+    Tile<DK>::template fetch<NW>(p.k + u.k0 + (long)c * p.ldk, p.ldk, t1 - c, to);
+    Tile<DK>::template fetch<NW>(p.q + u.q0 + (long)c * p.ldq, p.ldq, t1 - c, to + Tile<DK>::BYTES);
+    Tile<TV>::template fetch<NW>(p.v + u.v0 + (long)c * p.ldv, p.ldv, t1 - c, to + 2 * Tile<DK>::BYTES);
+  };
+  if (t0 < t1) fetch(t0, 0);
   State<DK> st;
-  if (p.nseg > 1) {
-    if (t0 >= t1) return;
-    const float* w = p.ws + (unit * p.nseg + sg) * (DK * C);
 #pragma unroll
-    for (int t = 0; t < DK / 16; ++t) st.s[t] = *reinterpret_cast<const f32x4*>(w + ((wave * (DK / 16) + t) * 64 + lane) * 4);
-  } else {
-#pragma unroll
-    for (int t = 0; t < DK / 16; ++t) {
-      const long at = state_at<DK>(p, u, t);
+  for (int t = 0; t < DK / 16; ++t) {
+    if (ONE) {
+      const long at = state_at<DK, TV>(p, u, wave, t);
 #pragma unroll
       for (int r = 0; r < 4; ++r) st.s[t][r] = p.s_in ? p.s_in[at + (long)r * p.dv] : 0.f;
+    } else {
+      st.s[t] = *reinterpret_cast<const f32x4*>(p.ws + (unit * p.nseg + sg) * (DK * TV) + ws_at<DK>(wave, t));
     }
   }
-  // lambda^(i - j) of a tile of scores on the diagonal (rows j = 4 grp + r, column i = l) and, times lambda^(16 m), of the tiles m + 1 beside it
-  float diag[4], off[4];
+  // scale * lambda^(i - j) of a tile of scores on the diagonal (rows j = 4 grp + r, column i = l) and, but for lambda^(16 m), of the tiles m + 1 beside it
+  float diag[4], off[4], far[3], rise[4], w[2][8];
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const int d = l - 4 * grp - r;
     diag[r] = d < 0 ? 0.f : p.scale * expf(u.g * (float)d);
     off[r] = p.scale * expf(u.g * (float)(16 + d));
+    rise[r] = p.scale * expf(u.g * (float)(16 * r + l + 1));   // of the state, for the tokens 16 r + l
   }
-  for (int c = t0; c < t1; c += C) {
-    tile_in<DK, Sh::KP>(p.k + u.k0, p.ldk, c, t1, kt);
-    tile_in<DK, Sh::KP>(p.q + u.q0, p.ldq, c, t1, qt);
-    tile_in<C, Sh::VP>(p.v + u.v0, p.ldv, c, t1, vt);
-    __syncthreads();
-    // scores of the 16 tokens of this wave against those before them: column i = 16 wave + l, rows j = 16 jt + 4 grp + r
+#pragma unroll
+  for (int m = 0; m < 3; ++m) far[m] = expf(u.g * (float)(16 * m));
+  powers(u.g, C, w);
+  float decay = expf(u.g * (float)C);
+  // the 16 tokens whose scores a wave computes, and (of eight waves) every other tile of the tokens before them
+  const int it0 = wave & 3, j0 = NW == 8 ? wave >> 2 : 0;
+  constexpr int JS = NW == 8 ? 2 : 1;
+  for (int c = t0, stage = 0; c < t1; c += C, stage ^= 1) {
+    const char* kt = smem + stage * Sh::STAGE;
+    const char* qt = kt + Tile<DK>::BYTES;
+    const char* vt = qt + Tile<DK>::BYTES;
+    wait_all_loads();
+    barrier();                             // everybody's share of this block; and nobody reads the block before any more
+    if (c + C < t1) fetch(c + C, stage ^ 1);
     {
       bf16x8 qf[DK / 32];
 #pragma unroll
-      for (int s = 0; s < DK / 32; ++s) qf[s] = *reinterpret_cast<const bf16x8*>(qt + (16 * wave + l) * Sh::KP + s * 64 + grp * 16);
-      for (int jt = 0; jt <= (wave | 1); ++jt) {
+      for (int s = 0; s < DK / 32; ++s) qf[s] = Tile<DK>::rows8(qt, 16 * it0 + l, 32 * s + 8 * grp);
+#pragma unroll
+      for (int i = 0; i < 4 / JS; ++i) {
+        const int jt = j0 + JS * i;        // (the tile behind an even one on the diagonal is read with it: zeros)
+        if (jt > (it0 | 1)) continue;
         f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (jt <= wave) {
+        if (jt <= it0) {
 #pragma unroll
-          for (int s = 0; s < DK / 32; ++s) a = mfma(*reinterpret_cast<const bf16x8*>(kt + (16 * jt + l) * Sh::KP + s * 64 + grp * 16), qf[s], a);
-          const float far = jt == wave ? 1.f : expf(u.g * (float)(16 * (wave - jt - 1)));
+          for (int s = 0; s < DK / 32; ++s) a = mfma(Tile<DK>::rows8(kt, 16 * jt + l, 32 * s + 8 * grp), qf[s], a);
+          const int m = it0 - jt;
+          const float f = m == 0 ? 1.f : m == 1 ? far[0] : m == 2 ? far[1] : far[2];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) a[r] *= jt == wave ? diag[r] : off[r] * far;
+          for (int r = 0; r < 4; ++r) a[r] *= m == 0 ? diag[r] : off[r] * f;
         }
         bf16x4 hi, lo;
 #pragma unroll
         for (int r = 0; r < 4; ++r) { hi[r] = (bf16_t)a[r]; lo[r] = (bf16_t)(a[r] - (float)hi[r]); }
-        const int at = (16 * wave + l) * Sh::PP + (16 * jt + 4 * grp) * 2;
+        const int at = (16 * it0 + l) * Sh::PP + (16 * jt + 4 * grp) * 2;
         *reinterpret_cast<bf16x4*>(ph + at) = hi;
         *reinterpret_cast<bf16x4*>(pl + at) = lo;
       }
     }
-    __syncthreads();
-    // outputs of the 16 columns of this wave: rows of the product 4 grp + r of them, column i = 16 it + l
-    bf16x8 vf[2];
+    // the state's share of the outputs of this wave's 16 columns: rows of the product 4 grp + r of them, columns i = 16 it + l
+    f32x4 a[4];
+    {
+      bf16x8 sh[DK / 32], sl[DK / 32];     // k-slots e < 4 are rows 32 s + 4 grp + e, the others 16 rows further
 #pragma unroll
-    for (int s = 0; s < 2; ++s) vf[s] = transposed(vt + (32 * s + 8 * grp + (l >> 2)) * Sh::VP + wave * 32 + (l & 3) * 8, Sh::VP);
-    bf16x8 sh[DK / 32], sl[DK / 32];       // the state: k-slots e < 4 are rows 32 s + 4 grp + e, the others 16 rows further
+      for (int s = 0; s < DK / 32; ++s)
 #pragma unroll
-    for (int s = 0; s < DK / 32; ++s)
+        for (int e = 0; e < 8; ++e) {
+          const float x = st.s[2 * s + e / 4][e % 4];
+          sh[s][e] = (bf16_t)x;
+          sl[s][e] = (bf16_t)(x - (float)sh[s][e]);
+        }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float x = st.s[2 * s + e / 4][e % 4];
-        sh[s][e] = (bf16_t)x;
-        sl[s][e] = (bf16_t)(x - (float)sh[s][e]);
+      for (int it = 0; it < 4; ++it) {
+        a[it] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < DK / 32; ++s) {
+          const bf16x4 q0 = Tile<DK>::rows4(qt, 16 * it + l, 32 * s + 4 * grp), q1 = Tile<DK>::rows4(qt, 16 * it + l, 32 * s + 16 + 4 * grp);
+          bf16x8 qf;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) { qf[e] = q0[e]; qf[4 + e] = q1[e]; }
+          a[it] = mfma(sh[s], qf, a[it]);
+          a[it] = mfma(sl[s], qf, a[it]);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) a[it][r] *= rise[it];
       }
+    }
+    barrier();                             // the scores
+    bf16x8 vf[1][2];
+    uint32_t vat[2];
+    Tile<TV>::column_rows(vt, vat);
+    Tile<TV>::template columns<1>(vat, wave, vf);
 #pragma unroll
     for (int it = 0; it < 4; ++it) {
-      f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int s = 0; s < DK / 32; ++s) {
-        const char* at = qt + (16 * it + l) * Sh::KP + s * 64 + grp * 8;
-        const bf16x4 q0 = *reinterpret_cast<const bf16x4*>(at), q1 = *reinterpret_cast<const bf16x4*>(at + 32);
-        bf16x8 qf;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) { qf[e] = q0[e]; qf[4 + e] = q1[e]; }
-        a = mfma(sh[s], qf, a);
-        a = mfma(sl[s], qf, a);
-      }
-      const float d = p.scale * expf(u.g * (float)(16 * it + l + 1));
-#pragma unroll
-      for (int r = 0; r < 4; ++r) a[r] *= d;
 #pragma unroll
       for (int s = 0; s <= it / 2; ++s) {
         const int at = (16 * it + l) * Sh::PP + s * 64 + grp * 16;
-        a = mfma(vf[s], *reinterpret_cast<const bf16x8*>(ph + at), a);
-        a = mfma(vf[s], *reinterpret_cast<const bf16x8*>(pl + at), a);
+        a[it] = mfma(vf[0][s], *reinterpret_cast<const bf16x8*>(ph + at), a[it]);
+        a[it] = mfma(vf[0][s], *reinterpret_cast<const bf16x8*>(pl + at), a[it]);
       }
       const int i = c + 16 * it + l;
       if (i < t1) {
-        const u32x2 v = u32x2{pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3])};
+        const u32x2 v = u32x2{pack_bf16x2(a[it][0], a[it][1]), pack_bf16x2(a[it][2], a[it][3])};
         *reinterpret_cast<u32x2*>(p.o + u.o0 + (long)i * p.ldo + wave * 16 + grp * 4) = v;
       }
     }
-    if (p.nseg == 1 || c + C < t1) add_block<DK>(st, kt, vt, t1 - c < C ? t1 - c : C, u.g);
-    __syncthreads();
+    if (ONE || c + C < t1) {
+      if (ONE && t1 - c < C) {
+        powers(u.g, t1 - c, w);
+        decay = expf(u.g * (float)(t1 - c));
+      }
+      add_block<DK, TV, ONE ? 3 : 2>(st, kt, vt, decay, w);   // (inside a segment the state only makes outputs)
+    }
   }
-  if (p.nseg == 1)
+  if (ONE)
 #pragma unroll
     for (int t = 0; t < DK / 16; ++t) {
-      const long at = state_at<DK>(p, u, t);
+      const long at = state_at<DK, TV>(p, u, wave, t);
 #pragma unroll
       for (int r = 0; r < 4; ++r) p.s_out[at + (long)r * p.dv] = st.s[t][r];
     }
@@ -326,7 +456,8 @@ template <int DK>
 __global__ __launch_bounds__(256) void la_step(const LaParams p) {
   __shared__ float red[4][C];
   Unit u;
-  if (!unit_of(p, blockIdx.x, DK, u)) return;
+  const int tiles = p.H * (p.dv / C);
+  if (!unit_of(p, blockIdx.x / tiles, blockIdx.x % tiles, DK, C, u)) return;
   const int c4 = (threadIdx.x & 15) * 4, r0 = threadIdx.x >> 4;
   const float d = expf(u.g);
   const bf16x4 vb = *reinterpret_cast<const bf16x4*>(p.v + u.v0 + c4);
@@ -357,19 +488,21 @@ __global__ __launch_bounds__(256) void la_step(const LaParams p) {
   }
 }
 
-struct Plan { long units; int nseg, seg; };
+struct Plan { long units; int tv, nseg, seg; };
 
-// Segments where heads, columns and sequences alone give the CUs too little: about four workgroups a CU, two blocks of 64 tokens each at least.
-Plan plan_of(long B, long H, long dv, long T) {
+// 128 columns of v to a workgroup (which computes the scores once for them) where dv has them.  Segments where the sequences are long enough that
+// units alone give the CUs too little: about two workgroups a CU, four blocks of 64 tokens each at least.
+Plan plan_of(long B, long H, long dv, long T, long rows) {
   Plan r;
-  r.units = B * H * (dv / C);
-  const long blocks = (T + C - 1) / C;
-  long n = (1024 + r.units - 1) / r.units;
-  if (n > (blocks + 1) / 2) n = (blocks + 1) / 2;
-  if (n < 1) n = 1;
-  const long per = (blocks + n - 1) / n;
+  r.tv = dv % 128 == 0 ? 128 : 64;
+  r.units = B * H * (dv / r.tv);
+  const long blocks = (T + C - 1) / C, all = (rows + C - 1) / C;
+  long per = (all * H * (dv / r.tv) + 511) / 512;
+  if (per < 4) per = 4;
+  if (per > blocks) per = blocks;
   r.seg = (int)(per * C);
   r.nseg = (int)((blocks + per - 1) / per);
+  if (r.units > 65535) { r.nseg = 1; r.seg = (int)(blocks * C); }   // (la_scan's grid; CUs have enough)
   return r;
 }
 
@@ -386,30 +519,37 @@ int check(const LaParams& p, int64_t B, int64_t H, int64_t Hk, int64_t dk, int64
   return KH_OK;
 }
 
-template <int DK>
+template <int DK, int TV>
 int prompt(const LaParams& p, long units, hipStream_t s) {
-  typedef Shape<DK> Sh;
-  constexpr int lds = C * (2 * Sh::KP + Sh::VP + 2 * Sh::PP);
-  if (p.nseg > 1) {
-    kh_launch(KH_TAG_LINEAR_ATTENTION, la_gain<DK>, dim3((unsigned)(units * p.nseg)), dim3(256), 0, s, p);
-    kh_launch(KH_TAG_LINEAR_ATTENTION, la_scan<DK>, dim3(DK / 16, (unsigned)units), dim3(256), 0, s, p);
+  constexpr int lds = OutShape<DK, TV>::LDS, gain_lds = 2 * (Tile<DK>::BYTES + Tile<TV>::BYTES);
+  const long size = p.share * (p.dv / TV), clusters = units / size * p.nseg;
+  const dim3 grid((unsigned)((clusters + 7) / 8 * 8 * size)), block(TV * 4);
+  if (p.nseg == 1) {
+    if (lds > 65536) {
+      const hipError_t e = kh_allow_lds<la_out<DK, TV, true>>(lds);
+      if (e != hipSuccess) return (int)e;
+    }
+    kh_launch(KH_TAG_LINEAR_ATTENTION, la_out<DK, TV, true>, grid, block, lds, s, p);
+  } else {
+    if (lds > 65536) {
+      const hipError_t e = kh_allow_lds<la_out<DK, TV, false>>(lds);
+      if (e != hipSuccess) return (int)e;
+    }
+    kh_launch(KH_TAG_LINEAR_ATTENTION, la_gain<DK, TV>, grid, block, gain_lds, s, p);
+    kh_launch(KH_TAG_LINEAR_ATTENTION, la_scan<DK, TV>, dim3(DK / 16, (unsigned)units), block, 0, s, p);
+    kh_launch(KH_TAG_LINEAR_ATTENTION, la_out<DK, TV, false>, grid, block, lds, s, p);
   }
-  if (lds > 65536) {
-    const hipError_t e = kh_allow_lds<la_out<DK>>(lds);
-    if (e != hipSuccess) return (int)e;
-  }
-  kh_launch(KH_TAG_LINEAR_ATTENTION, la_out<DK>, dim3((unsigned)(units * p.nseg)), dim3(256), lds, s, p);
   KH_RETURN_LAST_ERROR();
 }
 
 }  // namespace
 
-KH_EXPORT int64_t kh_linear_attention_workspace_bytes(int64_t B, int64_t H, int64_t T, int64_t dk, int64_t dv) {
-  if (B <= 0 || H <= 0 || T <= 0 || dv <= 0) return KH_ERR_INVALID_ARG;
+KH_EXPORT int64_t kh_linear_attention_workspace_bytes(int64_t B, int64_t H, int64_t T, int64_t rows, int64_t dk, int64_t dv) {
+  if (B <= 0 || H <= 0 || T <= 0 || rows <= 0 || dv <= 0) return KH_ERR_INVALID_ARG;
   if ((dk != 64 && dk != 128) || dv % C != 0 || dv > 1024) return KH_ERR_UNSUPPORTED;
   if (B > (1 << 20) || H > (1 << 16) || B * H * (dv / C) > (1L << 30) || T > (1L << 30)) return KH_ERR_TOO_LARGE;
-  const Plan r = plan_of(B, H, dv, T);
-  return r.nseg > 1 ? (int64_t)r.units * r.nseg * dk * C * 4 : 0;
+  const Plan r = plan_of(B, H, dv, T, rows);
+  return r.nseg > 1 ? (int64_t)r.units * r.nseg * dk * r.tv * 4 : 0;
 }
 
 KH_EXPORT int kh_linear_attention_bf16(const void* q, const void* k, const void* v, void* o, const float* log_decay, const float* state_in,
@@ -426,13 +566,16 @@ KH_EXPORT int kh_linear_attention_bf16(const void* q, const void* k, const void*
   if (T <= 0 || (seg_start && rows < 0)) return KH_ERR_INVALID_ARG;
   if (ldq < H * dk || ldk < kv_heads * dk || ldv < kv_heads * dv || ldo < H * dv) return KH_ERR_INVALID_ARG;
   if (T > (1L << 30)) return KH_ERR_TOO_LARGE;
-  const Plan r = plan_of(B, H, dv, T);
+  if ((ldq | ldk | ldv) >= (1L << 24)) return KH_ERR_TOO_LARGE;
+  const Plan r = plan_of(B, H, dv, T, seg_start ? (rows > 0 ? rows : 1) : B * T);
   p.nseg = r.nseg;
   p.seg = r.seg;
   if (p.nseg > 1 && !workspace) return KH_ERR_INVALID_ARG;
   if (!kh_aligned16(workspace)) return KH_ERR_ALIGNMENT;
-  if (r.units * r.nseg > 0x7fffffffL) return KH_ERR_TOO_LARGE;   // (more than 65535 units are never cut: la_scan's grid)
-  return dk == 64 ? prompt<64>(p, r.units, (hipStream_t)stream) : prompt<128>(p, r.units, (hipStream_t)stream);
+  if (r.units * r.nseg > 0x7fffffffL - 8 * r.units) return KH_ERR_TOO_LARGE;
+  hipStream_t s = (hipStream_t)stream;
+  if (r.tv == 64) return dk == 64 ? prompt<64, 64>(p, r.units, s) : prompt<128, 64>(p, r.units, s);
+  return dk == 64 ? prompt<64, 128>(p, r.units, s) : prompt<128, 128>(p, r.units, s);
 }
 
 KH_EXPORT int kh_linear_attention_step_bf16(const void* q, const void* k, const void* v, void* o, const float* log_decay, const float* state_in,

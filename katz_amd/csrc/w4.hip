@@ -467,19 +467,18 @@ __global__ __launch_bounds__(LW * 64) void w4_few_rows(const LinParams p) {
 #endif
 }
 
-// Many rows: 128 rows of x and 256 columns of y to a workgroup of four waves, 64 columns each.  Blocks of 128 codes with their x come by DMA into three
-// stages in LDS, x in the order of its operands, codes and scales to the wave that uses them.
+// Many rows: 80 rows of x (a prompt of 77 tokens) and 384 columns of y to a workgroup of eight waves, 48 columns each.  Blocks of 128 codes with their x come
+// by DMA into three stages in LDS, x in the order of its operands, codes and scales to the wave that uses them.
 // The numbers multiplied are P + q without zero points and P + 16 + q - z with them (z taken off in the integers, four codes at a time); what they are too
-// large by is one constant then, and its product with a group's x the same for all columns: a wave computes it for 32 rows of the next block and leaves it in
+// large by is one constant then, and its product with a group's x the same for all columns: a wave computes it for 16 rows of the next block and leaves it in
 // LDS, where every wave's accumulators start from it.
-// Of the 2048 clocks that the matrix unit needs for a block (128 products of 16 x 16 x 32 on each SIMD), a third more goes to the vector unit beside it: codes to
-// operands and, for every group, the scaled sum.
-constexpr int MR_M = 8, MR_N = 4, MR_W = 4, MR_ST = 3;     // tiles of 16 rows; of 16 columns of a wave; waves; stages
+// A block is 1920 clocks of the matrix unit (two waves of 60 products of 16 x 16 x 32 on a SIMD), about 2100 of the vector unit (codes to operands, the scaled sum of
+// every group) and 1650 of LDS: sums of a group and of the row in 32 bits each are 120 registers of the 256 that two waves leave each other.
+constexpr int MR_M = 5, MR_N = 3, MR_W = 8, MR_ST = 3;     // tiles of 16 rows; of 16 columns of a wave; waves; stages
 
 template <int G, bool ZERO>
 struct ManyStage {
   static constexpr int S = G == 32 ? 2 : 1, Z = ZERO ? 1 : 0, GB = 128 / G;
-  static constexpr int P = MR_M * 4 / MR_W + MR_N + S + Z;                     // loads of a wave
   static constexpr int XAT = 0, WAT = MR_M * 4096, SAT = WAT + MR_W * MR_N * 1024, ZAT = SAT + MR_W * S * 256, BYTES = ZAT + MR_W * Z * 256;
   static constexpr int SUMS = MR_ST * BYTES, RING = SUMS + 2 * GB * MR_M * 16 * 4;
   static constexpr int PITCH = MR_N * 16 + 4, OUT = MR_W * MR_M * 16 * PITCH * 4;   // the outputs in 32 bits, on their way to whole rows
@@ -487,7 +486,7 @@ struct ManyStage {
 };
 
 template <typename T, int G, bool ZERO>
-__global__ __launch_bounds__(MR_W * 64, 1) void w4_many_rows(const LinParams p) {
+__global__ __launch_bounds__(MR_W * 64) void w4_many_rows(const LinParams p) {
 #if __HIP_DEVICE_COMPILE__
   extern __shared__ __attribute__((aligned(16))) char smem[];
   typedef ManyStage<G, ZERO> Sg;
@@ -505,16 +504,17 @@ __global__ __launch_bounds__(MR_W * 64, 1) void w4_many_rows(const LinParams p) 
   const uint8_t* z0 = ZERO ? p.zero + nb * p.gstride : nullptr;
   const T* x0 = (const T*)p.x + m0 * p.K;
   const uint32_t last = (uint32_t)(p.N - 1 - nb < MR_N * 16 - 1 ? p.N - 1 - nb : MR_N * 16 - 1);
-  uint32_t qo[MR_N], xo[MR_M / MR_W];
+  constexpr int XL = (MR_M * 4 + MR_W - 1) / MR_W;                             // loads of x of a wave, at most
+  uint32_t qo[MR_N], xo[XL];
 #pragma unroll
   for (int j = 0; j < MR_N; ++j) {
     const uint32_t r = j * 16 + l;
     qo[j] = (r < last ? r : last) * (uint32_t)p.row_bytes + g * 16;
   }
 #pragma unroll
-  for (int b = 0; b < MR_M / MR_W; ++b) {
-    const int r = (wave * (MR_M / MR_W) + b) * 16 + l;
-    xo[b] = (uint32_t)(r < rows ? r : rows - 1) * (uint32_t)p.K + g * 8;
+  for (int i = 0; i < XL; ++i) {              // load wave + 8 i: step j of the operands of a tile of 16 rows
+    const int id = wave + i * MR_W, r = (id >> 2) * 16 + l;
+    xo[i] = (uint32_t)(r < rows ? r : rows - 1) * (uint32_t)p.K + (id & 3) * 32 + g * 8;
   }
   const uint32_t so = ((uint32_t)lane < last ? (uint32_t)lane : last) * (uint32_t)p.gstride;
   auto bytes = [](long n) { return (int)(uint32_t)(n < 0xffffffffL ? n : 0xffffffffL); };
@@ -526,19 +526,19 @@ __global__ __launch_bounds__(MR_W * 64, 1) void w4_many_rows(const LinParams p) 
   const int blocks = (p.row_bytes + 63) / 64, whole = p.dma ? p.K / 128 : 0, groups = (p.K + G - 1) / G;
   auto fetch = [&](int kb, int st) {
     char* to = smem + st * Sg::BYTES;
+    if (kb < whole) {
 #pragma unroll
-    for (int b = 0; b < MR_M / MR_W; ++b)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        char* at = to + Sg::XAT + ((wave * (MR_M / MR_W) + b) * 4 + j) * 1024;
-        if (kb < whole) {
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lptr_t)at, 16, xo[b] * 2, kb * 256 + j * 64, 0, 0);
-        } else {                              // the end of the rows, or rows that are not aligned to four bytes
-          T v[8];
-          load8<T>(x0 + kb * 128 + (xo[b] + j * 32), (long)p.K - (kb * 128 + j * 32 + g * 8), v);
-          *reinterpret_cast<u32x4*>(at + lane * 16) = __builtin_bit_cast(u32x4, v);
-        }
+      for (int i = 0; i < XL; ++i)
+        if (wave + i * MR_W < MR_M * 4) __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lptr_t)(to + Sg::XAT + (wave + i * MR_W) * 1024), 16, xo[i] * 2, kb * 256, 0, 0);
+    } else {                                  // the end of the rows, or rows that are not aligned to four bytes
+#pragma unroll 1
+      for (int id = wave; id < MR_M * 4; id += MR_W) {
+        const int r = (id >> 2) * 16 + l, k = kb * 128 + (id & 3) * 32 + g * 8;
+        T v[8];
+        load8<T>(x0 + (long)(r < rows ? r : rows - 1) * p.K + k, (long)p.K - k, v);
+        *reinterpret_cast<u32x4*>(to + Sg::XAT + id * 1024 + lane * 16) = __builtin_bit_cast(u32x4, v);
       }
+    }
 #pragma unroll
     for (int j = 0; j < MR_N; ++j) __builtin_amdgcn_raw_ptr_buffer_load_lds(rq, (lptr_t)(to + Sg::WAT + (wave * MR_N + j) * 1024), 16, qo[j], kb * 64, 0, 0);
 #pragma unroll
@@ -549,16 +549,15 @@ __global__ __launch_bounds__(MR_W * 64, 1) void w4_many_rows(const LinParams p) 
   const f32x4 none = f32x4{0.f, 0.f, 0.f, 0.f};
   constexpr uint32_t over = (Num<T>::P | Num<T>::NEG) | (ZERO ? 0x00100010u : 0x00080008u);    // -(P + 16), -(P + 8)
   auto x_at = [&](int st, int b, int j) { return *reinterpret_cast<const u32x4*>(smem + st * Sg::BYTES + Sg::XAT + (b * 4 + j) * 1024 + lane * 16); };
-  auto sums = [&](int st, int odd) {          // a constant's products with the groups of this wave's rows
+  auto sums = [&](int st, int odd) {          // a constant's products with the groups of 16 rows
+    if (wave >= MR_M) return;
 #pragma unroll
-    for (int b = 0; b < MR_M / MR_W; ++b)
+    for (int i = 0; i < GB; ++i) {
+      f32x4 a = none;
 #pragma unroll
-      for (int i = 0; i < GB; ++i) {
-        f32x4 a = none;
-#pragma unroll
-        for (int k = 0; k < SG; ++k) a = Num<T>::mfma(x_at(st, wave * (MR_M / MR_W) + b, i * SG + k), u32x4{over, over, over, over}, a);
-        if (l == 0) *reinterpret_cast<f32x4*>(smem + Sg::SUMS + ((odd * GB + i) * MR_M * 16 + (wave * (MR_M / MR_W) + b) * 16 + g * 4) * 4) = a;
-      }
+      for (int k = 0; k < SG; ++k) a = Num<T>::mfma(x_at(st, wave, i * SG + k), u32x4{over, over, over, over}, a);
+      if (l == 0) *reinterpret_cast<f32x4*>(smem + Sg::SUMS + ((odd * GB + i) * MR_M * 16 + wave * 16 + g * 4) * 4) = a;
+    }
   };
   f32x4 out[MR_M][MR_N];
 #pragma unroll
@@ -592,37 +591,33 @@ __global__ __launch_bounds__(MR_W * 64, 1) void w4_many_rows(const LinParams p) 
         s[j] = kb * GB + i < groups ? bf16_bits_to_f32((uint32_t)(sw[j] >> (16 * i)) & 0xffffu) : 0.f;    // what rows of scales are filled up with is not used
         if constexpr (ZERO) z[j] = ((zw[j] >> (8 * i)) & 15u) * 0x01010101u;
       }
-      f32x4 acc[MR_M][MR_N];
+      u32x4 xv[SG][MR_M];
+      f32x4 base[MR_M];
 #pragma unroll
       for (int b = 0; b < MR_M; ++b) {
-        const f32x4 base = *reinterpret_cast<const f32x4*>(smem + Sg::SUMS + ((odd * GB + i) * MR_M * 16 + b * 16 + g * 4) * 4);
+        base[b] = *reinterpret_cast<const f32x4*>(smem + Sg::SUMS + ((odd * GB + i) * MR_M * 16 + b * 16 + g * 4) * 4);
 #pragma unroll
-        for (int j = 0; j < MR_N; ++j) acc[b][j] = base;
+        for (int k = 0; k < SG; ++k) xv[k][b] = x_at(st, b, i * SG + k);
       }
+      // A tile of columns at a time: the scaled sum of one and the operands of the next run beside the products
 #pragma unroll
-      for (int k = 0; k < SG; ++k) {
-        u32x4 wv[MR_N];
+      for (int j = 0; j < MR_N; ++j) {
+        f32x4 acc[MR_M];
 #pragma unroll
-        for (int j = 0; j < MR_N; ++j) {      // bytes of even and of odd codes, put beside one another: the order of x
+        for (int k = 0; k < SG; ++k) {        // bytes of even and of odd codes, put beside one another: the order of x
           const uint32_t word = w[j][i * SG + k];
-          uint32_t even = ZERO ? ((word & low) | sixteen) - z[j] : word & low;
-          uint32_t uneven = ZERO ? (((word >> 4) & low) | sixteen) - z[j] : (word >> 4) & low;
-          wv[j] = u32x4{__builtin_amdgcn_perm(uneven, even, 0x0c040c00u) | power, __builtin_amdgcn_perm(uneven, even, 0x0c050c01u) | power,
-                        __builtin_amdgcn_perm(uneven, even, 0x0c060c02u) | power, __builtin_amdgcn_perm(uneven, even, 0x0c070c03u) | power};
+          const uint32_t even = ZERO ? ((word & low) | sixteen) - z[j] : word & low;
+          const uint32_t uneven = ZERO ? (((word >> 4) & low) | sixteen) - z[j] : (word >> 4) & low;
+          const u32x4 wv = u32x4{__builtin_amdgcn_perm(uneven, even, 0x0c040c00u) | power, __builtin_amdgcn_perm(uneven, even, 0x0c050c01u) | power,
+                                 __builtin_amdgcn_perm(uneven, even, 0x0c060c02u) | power, __builtin_amdgcn_perm(uneven, even, 0x0c070c03u) | power};
+#pragma unroll
+          for (int b = 0; b < MR_M; ++b) acc[b] = Num<T>::mfma(xv[k][b], wv, k == 0 ? base[b] : acc[b]);
         }
 #pragma unroll
-        for (int b = 0; b < MR_M; ++b) {
-          const u32x4 xv = x_at(st, b, i * SG + k);
+        for (int b = 0; b < MR_M; ++b)
 #pragma unroll
-          for (int j = 0; j < MR_N; ++j) acc[b][j] = Num<T>::mfma(xv, wv[j], acc[b][j]);
-        }
+          for (int e = 0; e < 4; ++e) out[b][j][e] = fmaf(s[j], acc[b][e], out[b][j][e]);
       }
-#pragma unroll
-      for (int b = 0; b < MR_M; ++b)
-#pragma unroll
-        for (int j = 0; j < MR_N; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) out[b][j][e] = fmaf(s[j], acc[b][j][e], out[b][j][e]);
     }
   };
   auto barrier = []() {                       // what this wave has written to LDS is there, and everybody has arrived
@@ -630,21 +625,13 @@ __global__ __launch_bounds__(MR_W * 64, 1) void w4_many_rows(const LinParams p) 
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
-  fetch(0, 0);
-  if (blocks > 1) fetch(1, 1);
-  wait_vm<0>();
-  barrier();
-  sums(0, 0);
-  for (int kb = 0, st = 0; kb < blocks; ++kb) {
-    const int s1 = st == MR_ST - 1 ? 0 : st + 1, s2 = s1 == MR_ST - 1 ? 0 : s1 + 1;
-    wait_vm<0>();                             // this wave's share of the next block, requested a block ago
-    barrier();                                // everybody's; this block's sums; and nobody reads the block before any more
-    if (kb + 2 < blocks) fetch(kb + 2, s2);
-    if (kb + 1 < blocks) sums(s1, (kb + 1) & 1);
-    multiply(kb, st, kb & 1);
-    st = s1;
-  }
-  // the adapters: t lies in two pieces of bf16, B_cat is exact in one (fp16: in two)
+  // Workgroups of other columns begin with other blocks: rows of x are often a multiple of the memory channels' period apart, and all of them at the same
+  // place of the rows would ask few channels (616 x 10240 x 1280 38.0 -> 35.0 us).
+  const int rot = (int)((unit / mt) * 5 % (uint32_t)blocks);
+  auto turned = [&](int i) { return i + rot < blocks ? i + rot : i + rot - blocks; };
+  fetch(turned(0), 0);
+  if (blocks > 1) fetch(turned(1), 1);
+  // the adapters while the first blocks are on their way: t lies in two pieces of bf16, B_cat is exact in one (fp16: in two)
   const bf16_t* th = (const bf16_t*)p.t;
   for (int r = 0; r < p.R; r += 32) {
     bf16x8 bh[MR_N], bl[MR_N];
@@ -672,6 +659,18 @@ __global__ __launch_bounds__(MR_W * 64, 1) void w4_many_rows(const LinParams p) 
       }
     }
   }
+  wait_vm<0>();
+  barrier();
+  sums(0, 0);
+  for (int kb = 0, st = 0; kb < blocks; ++kb) {
+    const int s1 = st == MR_ST - 1 ? 0 : st + 1, s2 = s1 == MR_ST - 1 ? 0 : s1 + 1;
+    wait_vm<0>();                             // this wave's share of the next block, requested a block ago
+    barrier();                                // everybody's; this block's sums; and nobody reads the block before any more
+    if (kb + 2 < blocks) fetch(turned(kb + 2), s2);
+    if (kb + 1 < blocks) sums(s1, (kb + 1) & 1);
+    multiply(turned(kb), st, kb & 1);
+    st = s1;
+  }
   barrier();                                  // the stages are dead
   float* mine = reinterpret_cast<float*>(smem) + wave * (MR_M * 16 * Sg::PITCH);
 #pragma unroll
@@ -682,13 +681,15 @@ __global__ __launch_bounds__(MR_W * 64, 1) void w4_many_rows(const LinParams p) 
       for (int e = 0; e < 4; ++e) mine[(b * 16 + g * 4 + e) * Sg::PITCH + j * 16 + l] = out[b][j][e];
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");         // (written and read by this wave alone)
   if (!some) return;
-  const int c = (lane & 7) * 8;               // a lane's eight columns of eight rows at a time
+  constexpr int PIECES = MR_N * 2, AT_ONCE = 64 / PIECES;    // a lane's eight columns of ten rows at a time
+  const int c = lane % PIECES * 8;
+  if (lane >= PIECES * AT_ONCE) return;
   const long n = n0 + c;
   float bias[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) bias[e] = p.bias && n + e < p.N ? (float)((const T*)p.bias)[n + e] : 0.f;
   const bool vec = n + 8 <= p.N;
-  for (int r = lane >> 3; r < rows; r += 8) {
+  for (int r = lane / PIECES; r < rows; r += AT_ONCE) {
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; e += 4) {

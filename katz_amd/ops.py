@@ -1597,7 +1597,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: i
                                                B, heads, kv, dk, dv, *s0, float(scale), _stream())
         _lib.check(rc, "kh_linear_attention_step_bf16")
         return out, state_out
-    nbytes = lib.kh_linear_attention_workspace_bytes(B, heads, T, dk, dv)
+    nbytes = lib.kh_linear_attention_workspace_bytes(B, heads, T, rows if packed else B * T, dk, dv)
     if nbytes < 0:
         _lib.check(int(nbytes), "kh_linear_attention_workspace_bytes")
     ws = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device) if nbytes else None

@@ -61,8 +61,8 @@ def test_linear_attention_entry_points(lib):
     assert prompt(ld=260) == -3 and prompt(q=8) == -3 and prompt(so=4) == -3 and prompt(ws=8) == -3
     assert prompt(T=1 << 31) == -4 and prompt(n=1 << 31) == -4
     size = lib.kh_linear_attention_workspace_bytes
-    assert size(2, 4, 0, 64, 64) == -1 and size(2, 4, 10, 80, 64) == -2 and size(2, 4, 64, 64, 64) == 0
-    assert size(1, 1, 1 << 20, 128, 128) > 0 and size(1 << 21, 1, 1, 64, 64) == -4
+    assert size(2, 4, 0, 1, 64, 64) == -1 and size(2, 4, 10, 20, 80, 64) == -2 and size(2, 4, 64, 128, 64, 64) == 0
+    assert size(1, 1, 1 << 20, 1 << 20, 128, 128) > 0 and size(1 << 21, 1, 1, 1 << 21, 64, 64) == -4
 
     def step(s=16, so=16, B=2, dk=64, ld=256, n=2):
         return lib.kh_linear_attention_step_bf16(16, 16, 16, 16, 16, s, so, None, n, B, 4, 4, dk, 64, *([ld] * 4), 0.1, None)
