@@ -10,6 +10,7 @@
 // bf16 operands carry 8 bits, so what is no input is fed to the matrix unit in pieces: scores and states as two (16 bits: their results are
 // rounded to bf16), the decayed values that make the state as three (24 bits: the state stays in 32).
 #include "kh_common.h"
+#include <type_traits>
 
 namespace {
 
@@ -34,7 +35,7 @@ struct LaParams {
 struct Unit {                  // one (sequence, head, range of columns of v)
   int b, h, tile, len, slot;
   long q0, k0, v0, o0;         // first elements
-  float g;
+  float g;                     // log2 of the decay
 };
 
 // TV: columns of v of a unit
@@ -62,8 +63,17 @@ __device__ __forceinline__ bool unit_of(const LaParams& p, int b, int ht, int DK
   r.v0 += row * p.ldv + (long)hk * p.dv + r.tile * TV;
   r.o0 += row * p.ldo + (long)r.h * p.dv + r.tile * TV;
   const float g = p.log_decay[r.h];
-  r.g = g < -1.0e4f ? -1.0e4f : g;     // (-inf, no memory at all, times a distance of 0 would be no number)
+  r.g = (g < -1.0e4f ? -1.0e4f : g) * 1.4426950408889634f;     // (-inf, no memory at all, times a distance of 0 would be no number)
   return true;
+}
+
+// lambda^n (the product's rounding is 2^-24 of the exponent, which is small wherever the power is not)
+__device__ __forceinline__ float power(float g, int n) {
+#if __HIP_DEVICE_COMPILE__
+  return __builtin_amdgcn_exp2f(g * (float)n);
+#else
+  return g;
+#endif
 }
 
 __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
@@ -108,13 +118,10 @@ struct Tile {
     }
 #endif
   }
-  // operand whose lane has row `row`, eight elements from column c (a multiple of 8)
-  static __device__ __forceinline__ bf16x8 rows8(const char* t, int row, int c) {
-    return *reinterpret_cast<const bf16x8*>(t + row * ROW + ((c / 8) ^ swz(row)) * 16);
-  }
-  static __device__ __forceinline__ bf16x4 rows4(const char* t, int row, int c) {     // four elements from column c
-    return *reinterpret_cast<const bf16x4*>(t + row * ROW + ((c / 8) ^ swz(row)) * 16 + (c & 4) * 2);
-  }
+  // where a lane (l = lane % 16, g = lane / 16) of an operand finds eight elements of row l from column 32 s + 8 g, and four from column 32 s + 4 g (the next
+  // sixteen columns' four: that ^ 32); rows 16 further lie 16 * ROW further
+  static __device__ __forceinline__ int at8(int l, int g, int s) { return l * ROW + ((4 * s + g) ^ swz(l)) * 16; }
+  static __device__ __forceinline__ int at4(int l, int g, int s) { return l * ROW + ((4 * s + (g >> 1)) ^ swz(l)) * 16 + (g & 1) * 8; }
   // LDS addresses, for columns(), of row 8 (lane / 16) + (lane % 16) / 4 and of the row four further: a transposing read gives lane i of 16 the i-th element
   // of four rows, of which lanes 4 r .. 4 r + 3 address the r-th
   static __device__ __forceinline__ void column_rows(const char* t, uint32_t (&at)[2]) {
@@ -129,23 +136,24 @@ struct Tile {
   }
   // N operands whose lanes have the columns 16 (t0 + n) + lane % 16 of rows 32 s + 8 (lane / 16) .. + 7, s = 0, 1.  The reads are written out, with their wait:
   // in front of one of its own the compiler waits for every load that is on its way to LDS, the next block's among them.
-  template <int N>
+  // AT: bytes from the tile that `at` belongs to.
+  template <int N, int AT = 0>
   static __device__ __forceinline__ void columns(const uint32_t (&at)[2], int t0, bf16x8 (&v)[N][2]) {
 #if __HIP_DEVICE_COMPILE__
     static_assert(N == 1 || N == 2, "one or two tiles of columns");
     u32x2 r[N][4];
     const uint32_t a0 = at[0] ^ (uint32_t)(t0 << 5), b0 = at[1] ^ (uint32_t)(t0 << 5);
     if constexpr (N == 1) {
-      asm volatile("ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %5\n\tds_read_b64_tr_b16 %2, %4 offset:%6\n\tds_read_b64_tr_b16 %3, %5 offset:%6\n\t"
+      asm volatile("ds_read_b64_tr_b16 %0, %4 offset:%7\n\tds_read_b64_tr_b16 %1, %5 offset:%7\n\tds_read_b64_tr_b16 %2, %4 offset:%6\n\tds_read_b64_tr_b16 %3, %5 offset:%6\n\t"
                    "s_waitcnt lgkmcnt(0)"
-                   : "=&v"(r[0][0]), "=&v"(r[0][1]), "=&v"(r[0][2]), "=&v"(r[0][3]) : "v"(a0), "v"(b0), "i"(32 * ROW) : "memory");
+                   : "=&v"(r[0][0]), "=&v"(r[0][1]), "=&v"(r[0][2]), "=&v"(r[0][3]) : "v"(a0), "v"(b0), "i"(AT + 32 * ROW), "i"(AT) : "memory");
     } else {
       const uint32_t a1 = at[0] ^ (uint32_t)((t0 + 1) << 5), b1 = at[1] ^ (uint32_t)((t0 + 1) << 5);
-      asm volatile("ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %9\n\tds_read_b64_tr_b16 %2, %8 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
-                   "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %11\n\tds_read_b64_tr_b16 %6, %10 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\t"
+      asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%13\n\tds_read_b64_tr_b16 %1, %9 offset:%13\n\tds_read_b64_tr_b16 %2, %8 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
+                   "ds_read_b64_tr_b16 %4, %10 offset:%13\n\tds_read_b64_tr_b16 %5, %11 offset:%13\n\tds_read_b64_tr_b16 %6, %10 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\t"
                    "s_waitcnt lgkmcnt(0)"
                    : "=&v"(r[0][0]), "=&v"(r[0][1]), "=&v"(r[0][2]), "=&v"(r[0][3]), "=&v"(r[1][0]), "=&v"(r[1][1]), "=&v"(r[1][2]), "=&v"(r[1][3])
-                   : "v"(a0), "v"(b0), "v"(a1), "v"(b1), "i"(32 * ROW) : "memory");
+                   : "v"(a0), "v"(b0), "v"(a1), "v"(b1), "i"(AT + 32 * ROW), "i"(AT) : "memory");
     }
 #pragma unroll
     for (int n = 0; n < N; ++n)
@@ -169,34 +177,29 @@ __device__ __forceinline__ void powers(float g, int n, float (&w)[2][8]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int left = n - 1 - (32 * s + 8 * grp + e);
-      w[s][e] = expf(g * (float)(left < 0 ? 0 : left));
+      w[s][e] = power(g, left < 0 ? 0 : left);
     }
 }
 
-// S = decay S + sum_j w_j k_j v_j^T over a block whose K and V lie in LDS; decayed values in PIECES pieces of bf16.
-template <int DK, int TV, int PIECES>
-__device__ __forceinline__ void add_block(State<DK>& st, const char* kt, const char* vt, float decay, const float (&w)[2][8]) {
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  bf16x8 v[2][PIECES], raw[1][2];
-  uint32_t at[2];
-  Tile<TV>::column_rows(vt, at);
-  Tile<TV>::template columns<1>(at, wave, raw);
+// S = decay S + sum_j w_j k_j v_j^T over a block: V as the wave's columns, K in LDS AT bytes from the tile of `kcol`; decayed values in PIECES pieces of bf16.
+template <int DK, int TV, int PIECES, int AT>
+__device__ __forceinline__ void add_block(State<DK>& st, const bf16x8 (&raw)[2], const uint32_t (&kcol)[2], float decay, const float (&w)[2][8]) {
+  bf16x8 v[2][PIECES];
 #pragma unroll
   for (int s = 0; s < 2; ++s)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      float x = (float)raw[0][s][e] * w[s][e];
+      float x = (float)raw[s][e] * w[s][e];
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
         v[s][i][e] = (bf16_t)x;
         x -= (float)v[s][i][e];
       }
     }
-  Tile<DK>::column_rows(kt, at);
 #pragma unroll
   for (int t = 0; t < DK / 16; t += 2) {
     bf16x8 k[2][2];
-    Tile<DK>::template columns<2>(at, t, k);
+    Tile<DK>::template columns<2, AT>(kcol, t, k);
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
 #pragma unroll
@@ -252,16 +255,28 @@ __global__ __launch_bounds__(TV * 4) void la_gain(const LaParams p) {
   for (int t = 0; t < DK / 16; ++t) st.s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
   float w[2][8];
   powers(u.g, C, w);
-  float decay = expf(u.g * (float)C);
-  for (int c = t0, i = 0; c < t1; c += C, i ^= 1) {
+  float decay = power(u.g, C);
+  uint32_t kcol[2], vcol[2];
+  Tile<DK>::column_rows(smem, kcol);
+  Tile<TV>::column_rows(smem + Tile<DK>::BYTES, vcol);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) vcol[h] ^= (uint32_t)(threadIdx.x >> 6) << 5;
+  auto block = [&](int c, auto stage_tag) {
+    constexpr int SO = decltype(stage_tag)::value * STAGE;
     wait_all_loads();
     barrier();                             // everybody's share of this block; and nobody reads the block before any more
-    if (c + C < t1) fetch(c + C, i ^ 1);
+    if (c + C < t1) fetch(c + C, 1 - decltype(stage_tag)::value);
     if (t1 - c < C) {
       powers(u.g, t1 - c, w);
-      decay = expf(u.g * (float)(t1 - c));
+      decay = power(u.g, t1 - c);
     }
-    add_block<DK, TV, 3>(st, smem + i * STAGE, smem + i * STAGE + Tile<DK>::BYTES, decay, w);
+    bf16x8 vf[1][2];
+    Tile<TV>::template columns<1, SO>(vcol, 0, vf);
+    add_block<DK, TV, 3, SO>(st, vf[0], kcol, decay, w);
+  };
+  for (int c = t0; c < t1; c += 2 * C) {
+    block(c, std::integral_constant<int, 0>{});
+    if (c + C < t1) block(c + C, std::integral_constant<int, 1>{});
   }
   float* ws = p.ws + (unit * p.nseg + sg) * (DK * TV);
 #pragma unroll
@@ -283,7 +298,7 @@ __global__ __launch_bounds__(TV * 4) void la_scan(const LaParams p) {
     for (int r = 0; r < 4; ++r) s[r] = p.s_in[at + (long)r * p.dv];
   float* w = p.ws + (long)blockIdx.y * p.nseg * (DK * TV) + ws_at<DK>(wave, t);
   const int n = (u.len + p.seg - 1) / p.seg;
-  const float d = expf(u.g * (float)p.seg), dl = expf(u.g * (float)(u.len - (n - 1) * p.seg));
+  const float d = power(u.g, p.seg), dl = power(u.g, u.len - (n - 1) * p.seg);
   for (int s0 = 0; s0 < n; s0 += 4) {      // four gains on their way at a time
     f32x4 gain[4];
 #pragma unroll
@@ -344,28 +359,40 @@ __global__ __launch_bounds__(TV * 4) void la_out(const LaParams p) {
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const int d = l - 4 * grp - r;
-    diag[r] = d < 0 ? 0.f : p.scale * expf(u.g * (float)d);
-    off[r] = p.scale * expf(u.g * (float)(16 + d));
-    rise[r] = p.scale * expf(u.g * (float)(16 * r + l + 1));   // of the state, for the tokens 16 r + l
+    diag[r] = d < 0 ? 0.f : p.scale * power(u.g, d);
+    off[r] = p.scale * power(u.g, 16 + d);
+    rise[r] = p.scale * power(u.g, 16 * r + l + 1);   // of the state, for the tokens 16 r + l
   }
 #pragma unroll
-  for (int m = 0; m < 3; ++m) far[m] = expf(u.g * (float)(16 * m));
+  for (int m = 0; m < 3; ++m) far[m] = power(u.g, 16 * m);
   powers(u.g, C, w);
-  float decay = expf(u.g * (float)C);
+  float decay = power(u.g, C);
   // the 16 tokens whose scores a wave computes, and (of eight waves) every other tile of the tokens before them
   const int it0 = wave & 3, j0 = NW == 8 ? wave >> 2 : 0;
   constexpr int JS = NW == 8 ? 2 : 1;
-  for (int c = t0, stage = 0; c < t1; c += C, stage ^= 1) {
-    const char* kt = smem + stage * Sh::STAGE;
-    const char* qt = kt + Tile<DK>::BYTES;
-    const char* vt = qt + Tile<DK>::BYTES;
+  int a8[DK / 32], a4[DK / 32];
+#pragma unroll
+  for (int s = 0; s < DK / 32; ++s) {
+    a8[s] = Tile<DK>::at8(l, grp, s);
+    a4[s] = Tile<DK>::at4(l, grp, s);
+  }
+  uint32_t kcol[2], vcol[2];
+  Tile<DK>::column_rows(smem, kcol);
+  Tile<TV>::column_rows(smem + 2 * Tile<DK>::BYTES, vcol);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) vcol[h] ^= (uint32_t)wave << 5;
+  const int p_to = (16 * it0 + l) * Sh::PP + (16 * j0 + 4 * grp) * 2, p_from = l * Sh::PP + grp * 16;
+  bf16_t* orow = p.o + u.o0 + (long)(t0 + l) * p.ldo + wave * 16 + grp * 4;
+
+  auto block = [&](int c, auto stage_tag) {
+    constexpr int SO = decltype(stage_tag)::value * Sh::STAGE, KT = SO, QT = SO + Tile<DK>::BYTES;
     wait_all_loads();
     barrier();                             // everybody's share of this block; and nobody reads the block before any more
-    if (c + C < t1) fetch(c + C, stage ^ 1);
+    if (c + C < t1) fetch(c + C, 1 - decltype(stage_tag)::value);
     {
       bf16x8 qf[DK / 32];
 #pragma unroll
-      for (int s = 0; s < DK / 32; ++s) qf[s] = Tile<DK>::rows8(qt, 16 * it0 + l, 32 * s + 8 * grp);
+      for (int s = 0; s < DK / 32; ++s) qf[s] = *reinterpret_cast<const bf16x8*>(smem + a8[s] + it0 * (16 * Tile<DK>::ROW) + QT);
 #pragma unroll
       for (int i = 0; i < 4 / JS; ++i) {
         const int jt = j0 + JS * i;        // (the tile behind an even one on the diagonal is read with it: zeros)
@@ -373,7 +400,7 @@ __global__ __launch_bounds__(TV * 4) void la_out(const LaParams p) {
         f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
         if (jt <= it0) {
 #pragma unroll
-          for (int s = 0; s < DK / 32; ++s) a = mfma(Tile<DK>::rows8(kt, 16 * jt + l, 32 * s + 8 * grp), qf[s], a);
+          for (int s = 0; s < DK / 32; ++s) a = mfma(*reinterpret_cast<const bf16x8*>(smem + a8[s] + j0 * (16 * Tile<DK>::ROW) + JS * i * (16 * Tile<DK>::ROW) + KT), qf[s], a);
           const int m = it0 - jt;
           const float f = m == 0 ? 1.f : m == 1 ? far[0] : m == 2 ? far[1] : far[2];
 #pragma unroll
@@ -382,9 +409,8 @@ __global__ __launch_bounds__(TV * 4) void la_out(const LaParams p) {
         bf16x4 hi, lo;
 #pragma unroll
         for (int r = 0; r < 4; ++r) { hi[r] = (bf16_t)a[r]; lo[r] = (bf16_t)(a[r] - (float)hi[r]); }
-        const int at = (16 * it0 + l) * Sh::PP + (16 * jt + 4 * grp) * 2;
-        *reinterpret_cast<bf16x4*>(ph + at) = hi;
-        *reinterpret_cast<bf16x4*>(pl + at) = lo;
+        *reinterpret_cast<bf16x4*>(ph + p_to + JS * i * 32) = hi;
+        *reinterpret_cast<bf16x4*>(pl + p_to + JS * i * 32) = lo;
       }
     }
     // the state's share of the outputs of this wave's 16 columns: rows of the product 4 grp + r of them, columns i = 16 it + l
@@ -404,10 +430,9 @@ __global__ __launch_bounds__(TV * 4) void la_out(const LaParams p) {
         a[it] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = 0; s < DK / 32; ++s) {
-          const bf16x4 q0 = Tile<DK>::rows4(qt, 16 * it + l, 32 * s + 4 * grp), q1 = Tile<DK>::rows4(qt, 16 * it + l, 32 * s + 16 + 4 * grp);
-          bf16x8 qf;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) { qf[e] = q0[e]; qf[4 + e] = q1[e]; }
+          const bf16x4 q0 = *reinterpret_cast<const bf16x4*>(smem + a4[s] + it * (16 * Tile<DK>::ROW) + QT);
+          const bf16x4 q1 = *reinterpret_cast<const bf16x4*>(smem + (a4[s] ^ 32) + it * (16 * Tile<DK>::ROW) + QT);
+          const bf16x8 qf = __builtin_shufflevector(q0, q1, 0, 1, 2, 3, 4, 5, 6, 7);
           a[it] = mfma(sh[s], qf, a[it]);
           a[it] = mfma(sl[s], qf, a[it]);
         }
@@ -417,30 +442,28 @@ __global__ __launch_bounds__(TV * 4) void la_out(const LaParams p) {
     }
     barrier();                             // the scores
     bf16x8 vf[1][2];
-    uint32_t vat[2];
-    Tile<TV>::column_rows(vt, vat);
-    Tile<TV>::template columns<1>(vat, wave, vf);
+    Tile<TV>::template columns<1, SO>(vcol, 0, vf);
 #pragma unroll
     for (int it = 0; it < 4; ++it) {
 #pragma unroll
       for (int s = 0; s <= it / 2; ++s) {
-        const int at = (16 * it + l) * Sh::PP + s * 64 + grp * 16;
-        a[it] = mfma(vf[0][s], *reinterpret_cast<const bf16x8*>(ph + at), a[it]);
-        a[it] = mfma(vf[0][s], *reinterpret_cast<const bf16x8*>(pl + at), a[it]);
+        a[it] = mfma(vf[0][s], *reinterpret_cast<const bf16x8*>(ph + p_from + it * (16 * Sh::PP) + s * 64), a[it]);
+        a[it] = mfma(vf[0][s], *reinterpret_cast<const bf16x8*>(pl + p_from + it * (16 * Sh::PP) + s * 64), a[it]);
       }
-      const int i = c + 16 * it + l;
-      if (i < t1) {
-        const u32x2 v = u32x2{pack_bf16x2(a[it][0], a[it][1]), pack_bf16x2(a[it][2], a[it][3])};
-        *reinterpret_cast<u32x2*>(p.o + u.o0 + (long)i * p.ldo + wave * 16 + grp * 4) = v;
-      }
+      if (c + 16 * it + l < t1) *reinterpret_cast<u32x2*>(orow + (long)(16 * it) * p.ldo) = u32x2{pack_bf16x2(a[it][0], a[it][1]), pack_bf16x2(a[it][2], a[it][3])};
     }
+    orow += (long)C * p.ldo;
     if (ONE || c + C < t1) {
       if (ONE && t1 - c < C) {
         powers(u.g, t1 - c, w);
-        decay = expf(u.g * (float)(t1 - c));
+        decay = power(u.g, t1 - c);
       }
-      add_block<DK, TV, ONE ? 3 : 2>(st, kt, vt, decay, w);   // (inside a segment the state only makes outputs)
+      add_block<DK, TV, ONE ? 3 : 2, SO>(st, vf[0], kcol, decay, w);   // (inside a segment the state only makes outputs)
     }
+  };
+  for (int c = t0; c < t1; c += 2 * C) {
+    block(c, std::integral_constant<int, 0>{});
+    if (c + C < t1) block(c + C, std::integral_constant<int, 1>{});
   }
   if (ONE)
 #pragma unroll
@@ -459,7 +482,7 @@ __global__ __launch_bounds__(256) void la_step(const LaParams p) {
   const int tiles = p.H * (p.dv / C);
   if (!unit_of(p, blockIdx.x / tiles, blockIdx.x % tiles, DK, C, u)) return;
   const int c4 = (threadIdx.x & 15) * 4, r0 = threadIdx.x >> 4;
-  const float d = expf(u.g);
+  const float d = power(u.g, 1);
   const bf16x4 vb = *reinterpret_cast<const bf16x4*>(p.v + u.v0 + c4);
   const long base = (((long)u.slot * p.H + u.h) * DK) * p.dv + u.tile * C + c4;
   f32x4 s[DK / 16], o = f32x4{0.f, 0.f, 0.f, 0.f};
