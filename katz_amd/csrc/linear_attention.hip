@@ -118,23 +118,24 @@ struct Tile {
     }
 #endif
   }
-  // where a lane (l = lane % 16, g = lane / 16) of an operand finds eight elements of row l from column 32 s + 8 g, and four from column 32 s + 4 g (the next
-  // sixteen columns' four: that ^ 32); rows 16 further lie 16 * ROW further
+  // where a lane (l = lane % 16, g = lane / 16) of an operand finds eight elements of row l from column 32 s + 8 g; rows 16 further lie 16 * ROW further
   static __device__ __forceinline__ int at8(int l, int g, int s) { return l * ROW + ((4 * s + g) ^ swz(l)) * 16; }
-  static __device__ __forceinline__ int at4(int l, int g, int s) { return l * ROW + ((4 * s + (g >> 1)) ^ swz(l)) * 16 + (g & 1) * 8; }
   // LDS addresses, for columns(), of row 8 (lane / 16) + (lane % 16) / 4 and of the row four further: a transposing read gives lane i of 16 the i-th element
-  // of four rows, of which lanes 4 r .. 4 r + 3 address the r-th
+  // of four rows, of which lanes 4 r .. 4 r + 3 address the r-th, four elements each.  PAIRS: the four are eight columns apart, and two tiles of 16 columns
+  // make 32: lane i of tile h has column 8 (i / 4) + 4 h + i % 4.  A product whose rows are such columns leaves them in the order in which the next one takes
+  // them as its operand, eight in a row to a lane.
+  template <bool PAIRS>
   static __device__ __forceinline__ void column_rows(const char* t, uint32_t (&at)[2]) {
 #if __HIP_DEVICE_COMPILE__
     const int lane = threadIdx.x & 63, l = lane & 15;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int row = 8 * (lane >> 4) + (l >> 2) + 4 * h;
-      at[h] = (uint32_t)(uintptr_t)(lptr_t)(const_cast<char*>(t)) + row * ROW + (((l & 3) >> 1) ^ swz(row)) * 16 + (l & 1) * 8;
+      at[h] = (uint32_t)(uintptr_t)(lptr_t)(const_cast<char*>(t)) + row * ROW + ((PAIRS ? l & 3 : (l & 3) >> 1) ^ swz(row)) * 16 + (PAIRS ? 0 : (l & 1) * 8);
     }
 #endif
   }
-  // N operands whose lanes have the columns 16 (t0 + n) + lane % 16 of rows 32 s + 8 (lane / 16) .. + 7, s = 0, 1.  The reads are written out, with their wait:
+  // N operands whose lanes have the columns of tile t0 + n (N 2: t0 is even, columns in PAIRS) of rows 32 s + 8 (lane / 16) .. + 7, s = 0, 1.  The reads are written out, with their wait:
   // in front of one of its own the compiler waits for every load that is on its way to LDS, the next block's among them.
   // AT: bytes from the tile that `at` belongs to.
   template <int N, int AT = 0>
@@ -148,12 +149,11 @@ struct Tile {
                    "s_waitcnt lgkmcnt(0)"
                    : "=&v"(r[0][0]), "=&v"(r[0][1]), "=&v"(r[0][2]), "=&v"(r[0][3]) : "v"(a0), "v"(b0), "i"(AT + 32 * ROW), "i"(AT) : "memory");
     } else {
-      const uint32_t a1 = at[0] ^ (uint32_t)((t0 + 1) << 5), b1 = at[1] ^ (uint32_t)((t0 + 1) << 5);
       asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%13\n\tds_read_b64_tr_b16 %1, %9 offset:%13\n\tds_read_b64_tr_b16 %2, %8 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
-                   "ds_read_b64_tr_b16 %4, %10 offset:%13\n\tds_read_b64_tr_b16 %5, %11 offset:%13\n\tds_read_b64_tr_b16 %6, %10 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\t"
+                   "ds_read_b64_tr_b16 %4, %8 offset:%11\n\tds_read_b64_tr_b16 %5, %9 offset:%11\n\tds_read_b64_tr_b16 %6, %8 offset:%10\n\tds_read_b64_tr_b16 %7, %9 offset:%10\n\t"
                    "s_waitcnt lgkmcnt(0)"
                    : "=&v"(r[0][0]), "=&v"(r[0][1]), "=&v"(r[0][2]), "=&v"(r[0][3]), "=&v"(r[1][0]), "=&v"(r[1][1]), "=&v"(r[1][2]), "=&v"(r[1][3])
-                   : "v"(a0), "v"(b0), "v"(a1), "v"(b1), "i"(AT + 32 * ROW), "i"(AT) : "memory");
+                   : "v"(a0), "v"(b0), "i"(AT + 8 + 32 * ROW), "i"(AT + 8), "i"(AT + 32 * ROW), "i"(AT) : "memory");
     }
 #pragma unroll
     for (int n = 0; n < N; ++n)
@@ -163,7 +163,8 @@ struct Tile {
   }
 };
 
-// A state (or a segment's gain) in registers: wave w has the columns 16 w .. 16 w + 15, lane l of a group g rows 16 t + 4 g + r of column l.
+// A state (or a segment's gain) in registers: wave w has the columns 16 w .. 16 w + 15, lane l of a group g the rows 16 (t & ~1) + 8 g + 4 (t & 1) + r of column l:
+// a pair of tiles is eight rows in a row, an operand's order.
 template <int DK>
 struct State {
   f32x4 s[DK / 16];
@@ -212,11 +213,11 @@ __device__ __forceinline__ void add_block(State<DK>& st, const bf16x8 (&raw)[2],
   }
 }
 
-// Row 16 t + 4 g of column l of a wave's share of a slot's state, dk x dv in rows.
+// First row of a lane's four of tile t in a slot's state, dk x dv in rows.
 template <int DK, int TV>
 __device__ __forceinline__ long state_at(const LaParams& p, const Unit& u, int wave, int t) {
   const int lane = threadIdx.x & 63;
-  return (((long)u.slot * p.H + u.h) * DK + 16 * t + 4 * (lane >> 4)) * p.dv + u.tile * TV + wave * 16 + (lane & 15);
+  return (((long)u.slot * p.H + u.h) * DK + 16 * (t & ~1) + 8 * (lane >> 4) + 4 * (t & 1)) * p.dv + u.tile * TV + wave * 16 + (lane & 15);
 }
 template <int DK>
 __device__ __forceinline__ int ws_at(int wave, int t) { return ((wave * (DK / 16) + t) * 64 + (threadIdx.x & 63)) * 4; }
@@ -257,8 +258,8 @@ __global__ __launch_bounds__(TV * 4) void la_gain(const LaParams p) {
   powers(u.g, C, w);
   float decay = power(u.g, C);
   uint32_t kcol[2], vcol[2];
-  Tile<DK>::column_rows(smem, kcol);
-  Tile<TV>::column_rows(smem + Tile<DK>::BYTES, vcol);
+  Tile<DK>::template column_rows<true>(smem, kcol);
+  Tile<TV>::template column_rows<false>(smem + Tile<DK>::BYTES, vcol);
 #pragma unroll
   for (int h = 0; h < 2; ++h) vcol[h] ^= (uint32_t)(threadIdx.x >> 6) << 5;
   auto block = [&](int c, auto stage_tag) {
@@ -323,7 +324,7 @@ struct OutShape {
   static constexpr int STAGE = 2 * Tile<DK>::BYTES + Tile<TV>::BYTES, LDS = 2 * STAGE + 2 * C * PP;
 };
 template <int DK, int TV, bool ONE>
-__global__ __launch_bounds__(TV * 4) void la_out(const LaParams p) {
+__global__ __launch_bounds__(TV * 4) __attribute__((amdgpu_waves_per_eu(2, 2))) void la_out(const LaParams p) {
   typedef OutShape<DK, TV> Sh;
   constexpr int NW = TV / 16;
   extern __shared__ __attribute__((aligned(16))) char smem[];   // two stages of K, Q, V; decayed scores, upper and lower pieces
@@ -370,19 +371,18 @@ __global__ __launch_bounds__(TV * 4) void la_out(const LaParams p) {
   // the 16 tokens whose scores a wave computes, and (of eight waves) every other tile of the tokens before them
   const int it0 = wave & 3, j0 = NW == 8 ? wave >> 2 : 0;
   constexpr int JS = NW == 8 ? 2 : 1;
-  int a8[DK / 32], a4[DK / 32];
+  int a8[DK / 32];
 #pragma unroll
-  for (int s = 0; s < DK / 32; ++s) {
-    a8[s] = Tile<DK>::at8(l, grp, s);
-    a4[s] = Tile<DK>::at4(l, grp, s);
-  }
+  for (int s = 0; s < DK / 32; ++s) a8[s] = Tile<DK>::at8(l, grp, s);
   uint32_t kcol[2], vcol[2];
-  Tile<DK>::column_rows(smem, kcol);
-  Tile<TV>::column_rows(smem + 2 * Tile<DK>::BYTES, vcol);
+  Tile<DK>::template column_rows<true>(smem, kcol);
+  Tile<TV>::template column_rows<false>(smem + 2 * Tile<DK>::BYTES, vcol);
 #pragma unroll
   for (int h = 0; h < 2; ++h) vcol[h] ^= (uint32_t)wave << 5;
   const int p_to = (16 * it0 + l) * Sh::PP + (16 * j0 + 4 * grp) * 2, p_from = l * Sh::PP + grp * 16;
-  bf16_t* orow = p.o + u.o0 + (long)(t0 + l) * p.ldo + wave * 16 + grp * 4;
+  // (a lane stores eight columns of one of two rows that are 16 apart)
+  const int orow_at = l + 16 * (grp & 1);
+  bf16_t* orow = p.o + u.o0 + (long)(t0 + orow_at) * p.ldo + wave * 16 + (grp >> 1) * 8;
 
   auto block = [&](int c, auto stage_tag) {
     constexpr int SO = decltype(stage_tag)::value * Sh::STAGE, KT = SO, QT = SO + Tile<DK>::BYTES;
@@ -416,7 +416,7 @@ __global__ __launch_bounds__(TV * 4) void la_out(const LaParams p) {
     // the state's share of the outputs of this wave's 16 columns: rows of the product 4 grp + r of them, columns i = 16 it + l
     f32x4 a[4];
     {
-      bf16x8 sh[DK / 32], sl[DK / 32];     // k-slots e < 4 are rows 32 s + 4 grp + e, the others 16 rows further
+      bf16x8 sh[DK / 32], sl[DK / 32];
 #pragma unroll
       for (int s = 0; s < DK / 32; ++s)
 #pragma unroll
@@ -430,9 +430,7 @@ __global__ __launch_bounds__(TV * 4) void la_out(const LaParams p) {
         a[it] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = 0; s < DK / 32; ++s) {
-          const bf16x4 q0 = *reinterpret_cast<const bf16x4*>(smem + a4[s] + it * (16 * Tile<DK>::ROW) + QT);
-          const bf16x4 q1 = *reinterpret_cast<const bf16x4*>(smem + (a4[s] ^ 32) + it * (16 * Tile<DK>::ROW) + QT);
-          const bf16x8 qf = __builtin_shufflevector(q0, q1, 0, 1, 2, 3, 4, 5, 6, 7);
+          const bf16x8 qf = *reinterpret_cast<const bf16x8*>(smem + a8[s] + it * (16 * Tile<DK>::ROW) + QT);
           a[it] = mfma(sh[s], qf, a[it]);
           a[it] = mfma(sl[s], qf, a[it]);
         }
@@ -450,7 +448,15 @@ __global__ __launch_bounds__(TV * 4) void la_out(const LaParams p) {
         a[it] = mfma(vf[0][s], *reinterpret_cast<const bf16x8*>(ph + p_from + it * (16 * Sh::PP) + s * 64), a[it]);
         a[it] = mfma(vf[0][s], *reinterpret_cast<const bf16x8*>(pl + p_from + it * (16 * Sh::PP) + s * 64), a[it]);
       }
-      if (c + 16 * it + l < t1) *reinterpret_cast<u32x2*>(orow + (long)(16 * it) * p.ldo) = u32x2{pack_bf16x2(a[it][0], a[it][1]), pack_bf16x2(a[it][2], a[it][3])};
+    }
+#pragma unroll
+    for (int it = 0; it < 4; it += 2) {
+      // a lane has four columns of row l of either tile; those of one tile and of the other trade places between the lanes of a pair of groups
+#if __HIP_DEVICE_COMPILE__
+      const auto s0 = __builtin_amdgcn_permlane16_swap(pack_bf16x2(a[it][0], a[it][1]), pack_bf16x2(a[it + 1][0], a[it + 1][1]), false, false);
+      const auto s1 = __builtin_amdgcn_permlane16_swap(pack_bf16x2(a[it][2], a[it][3]), pack_bf16x2(a[it + 1][2], a[it + 1][3]), false, false);
+      if (c + 16 * it + orow_at < t1) *reinterpret_cast<u32x4*>(orow + (long)(16 * it) * p.ldo) = u32x4{s0[0], s1[0], s0[1], s1[1]};
+#endif
     }
     orow += (long)C * p.ldo;
     if (ONE || c + C < t1) {
@@ -513,19 +519,34 @@ __global__ __launch_bounds__(256) void la_step(const LaParams p) {
 
 struct Plan { long units; int tv, nseg, seg; };
 
-// 128 columns of v to a workgroup (which computes the scores once for them) where dv has them.  Segments where the sequences are long enough that
-// units alone give the CUs too little: about two workgroups a CU, four blocks of 64 tokens each at least.
-Plan plan_of(long B, long H, long dv, long T, long rows) {
+// 128 columns of v to a workgroup (which computes the scores once for them) where dv has them.
+// Segments: a workgroup goes through its blocks one after the other (us a block as measured: 3.8 with dk 128, 2.3 with 64, whatever else runs), so long
+// sequences of few heads are cut; but every segment's state is written, read, written and read again, and the rounds that the workgroups make on 256 CUs are
+// whole ones.  Of a few lengths the one with the least of these sums.  Measured, us for 1 | the chosen length | 4 blocks: 16384 packed tokens of 16 heads of 128
+// 480 | 143 | 176, one sequence of 16384 956 | 119 | 160, 16 of 1024 78 (whole) | 78 | 164, 2 x 4096 tokens of 20 heads of 64 138 | 46 | 45.
+Plan plan_of(long B, long H, long dk, long dv, long T, long rows) {
   Plan r;
   r.tv = dv % 128 == 0 ? 128 : 64;
   r.units = B * H * (dv / r.tv);
-  const long blocks = (T + C - 1) / C, all = (rows + C - 1) / C;
-  long per = (all * H * (dv / r.tv) + 511) / 512;
-  if (per < 4) per = 4;
-  if (per > blocks) per = blocks;
+  const long blocks = (T + C - 1) / C, all = (rows + C - 1) / C, heads = H * (dv / r.tv);
+  const bool ragged = rows < B * T;
+  const double t_block = dk == 128 ? 3.8 : 2.3;
+  const long slots = dk == 128 ? 256 : 512;           // workgroups that LDS lets run at once
+  auto rounds = [](long wgs, long n) { return (double)((wgs + n - 1) / n); };
+  long per = blocks;
+  double best = rounds(r.units, slots) * blocks * t_block * 1.15;      // (in one piece the state needs its third piece everywhere)
+  if (r.units <= 65535) {                             // (la_scan's grid)
+    static const int lengths[] = {2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64, 96, 128, 192, 256};
+    for (const long n : lengths) {
+      if (n >= blocks) break;
+      const long wgs = (ragged ? (all + n - 1) / n + B / 2 : B * ((blocks + n - 1) / n)) * heads;
+      const double t = 8. + n * t_block * (rounds(wgs, slots) + 0.5 * rounds(wgs, 512)) + wgs * (double)(dk * r.tv * 8) / 4e6;
+      if (t < best) { best = t; per = n; }
+    }
+  }
+  if (per > (1L << 24)) per = 1L << 24;
   r.seg = (int)(per * C);
   r.nseg = (int)((blocks + per - 1) / per);
-  if (r.units > 65535) { r.nseg = 1; r.seg = (int)(blocks * C); }   // (la_scan's grid; CUs have enough)
   return r;
 }
 
@@ -571,7 +592,7 @@ KH_EXPORT int64_t kh_linear_attention_workspace_bytes(int64_t B, int64_t H, int6
   if (B <= 0 || H <= 0 || T <= 0 || rows <= 0 || dv <= 0) return KH_ERR_INVALID_ARG;
   if ((dk != 64 && dk != 128) || dv % C != 0 || dv > 1024) return KH_ERR_UNSUPPORTED;
   if (B > (1 << 20) || H > (1 << 16) || B * H * (dv / C) > (1L << 30) || T > (1L << 30)) return KH_ERR_TOO_LARGE;
-  const Plan r = plan_of(B, H, dv, T, rows);
+  const Plan r = plan_of(B, H, dk, dv, T, rows);
   return r.nseg > 1 ? (int64_t)r.units * r.nseg * dk * r.tv * 4 : 0;
 }
 
@@ -590,7 +611,7 @@ KH_EXPORT int kh_linear_attention_bf16(const void* q, const void* k, const void*
   if (ldq < H * dk || ldk < kv_heads * dk || ldv < kv_heads * dv || ldo < H * dv) return KH_ERR_INVALID_ARG;
   if (T > (1L << 30)) return KH_ERR_TOO_LARGE;
   if ((ldq | ldk | ldv) >= (1L << 24)) return KH_ERR_TOO_LARGE;
-  const Plan r = plan_of(B, H, dv, T, seg_start ? (rows > 0 ? rows : 1) : B * T);
+  const Plan r = plan_of(B, H, dk, dv, T, seg_start ? (rows > 0 ? rows : 1) : B * T);
   p.nseg = r.nseg;
   p.seg = r.seg;
   if (p.nseg > 1 && !workspace) return KH_ERR_INVALID_ARG;

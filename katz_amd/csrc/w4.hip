@@ -486,7 +486,7 @@ struct ManyStage {
 };
 
 template <typename T, int G, bool ZERO>
-__global__ __launch_bounds__(MR_W * 64) void w4_many_rows(const LinParams p) {
+__global__ __launch_bounds__(MR_W * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void w4_many_rows(const LinParams p) {
 #if __HIP_DEVICE_COMPILE__
   extern __shared__ __attribute__((aligned(16))) char smem[];
   typedef ManyStage<G, ZERO> Sg;
