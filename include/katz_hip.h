@@ -502,7 +502,8 @@ int kh_w4_linear(const void* x, const void* q, const void* scale, const void* ze
  * longest (a longer one is cut off there), batch strides unused; other rows of o are left as they were.
  * state_in / state_out: float [n_slots, H, dk, dv]; sequence b starts from and leaves slot b, or slots[b] (int32 [B], device; distinct): a slot
  * outside 0 .. n_slots - 1 leaves the whole sequence out.  state_in NULL: zeros (not for the step); the two may be the same.
- * workspace: kh_linear_attention_workspace_bytes with rows = B * T where they are dense (0: may be NULL).  kh_linear_attention_step_bf16: one token a sequence, rows [B]. */
+ * workspace: kh_linear_attention_workspace_bytes with rows = B * T where they are dense (0: may be NULL).  kh_linear_attention_step_bf16: one token a sequence, rows [B];
+ * flags bit 0: rows of o whose sequences are left out are zeroed (else left as they were). */
 int64_t kh_linear_attention_workspace_bytes(int64_t B, int64_t H, int64_t T, int64_t rows, int64_t dk, int64_t dv);
 int kh_linear_attention_bf16(const void* q, const void* k, const void* v, void* o, const float* log_decay, const float* state_in,
                              float* state_out, const int32_t* slots, int64_t n_slots, const int32_t* seg_start, int64_t rows, void* workspace,
@@ -510,7 +511,7 @@ int kh_linear_attention_bf16(const void* q, const void* k, const void* v, void* 
                              int64_t ldo, int64_t bsq, int64_t bsk, int64_t bsv, int64_t bso, float scale, void* stream);
 int kh_linear_attention_step_bf16(const void* q, const void* k, const void* v, void* o, const float* log_decay, const float* state_in,
                                   float* state_out, const int32_t* slots, int64_t n_slots, int64_t B, int64_t H, int64_t kv_heads, int64_t dk,
-                                  int64_t dv, int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo, float scale, void* stream);
+                                  int64_t dv, int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo, float scale, int flags, void* stream);
 
 #ifdef __cplusplus
 }

@@ -73,7 +73,7 @@ SIGNATURES = {
     "kh_w4_linear": (c_int, [_P] * 11 + [_I] * 5 + [c_int, _P]),
     "kh_linear_attention_workspace_bytes": (_I, [_I] * 6),
     "kh_linear_attention_bf16": (c_int, [_P] * 8 + [_I, _P, _I, _P] + [_I] * 14 + [c_float, _P]),
-    "kh_linear_attention_step_bf16": (c_int, [_P] * 8 + [_I] * 10 + [c_float, _P]),
+    "kh_linear_attention_step_bf16": (c_int, [_P] * 8 + [_I] * 10 + [c_float, c_int, _P]),
 }
 
 _lib = None

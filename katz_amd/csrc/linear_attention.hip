@@ -30,6 +30,7 @@ struct LaParams {
   int B, H, share;             // share: query heads of a key head
   int T, dv, n_slots, nseg, seg;   // seg: tokens of a segment, a multiple of C
   float scale;
+  int fill;                    // la_step: rows that are left out are zero
 };
 
 struct Unit {                  // one (sequence, head, range of columns of v)
@@ -486,7 +487,10 @@ __global__ __launch_bounds__(256) void la_step(const LaParams p) {
   __shared__ float red[4][C];
   Unit u;
   const int tiles = p.H * (p.dv / C);
-  if (!unit_of(p, blockIdx.x / tiles, blockIdx.x % tiles, DK, C, u)) return;
+  if (!unit_of(p, blockIdx.x / tiles, blockIdx.x % tiles, DK, C, u)) {
+    if (p.fill && threadIdx.x < C) p.o[(long)u.b * p.bso + (long)u.h * p.dv + u.tile * C + threadIdx.x] = (bf16_t)0.f;
+    return;
+  }
   const int c4 = (threadIdx.x & 15) * 4, r0 = threadIdx.x >> 4;
   const float d = power(u.g, 1);
   const bf16x4 vb = *reinterpret_cast<const bf16x4*>(p.v + u.v0 + c4);
@@ -604,7 +608,7 @@ KH_EXPORT int kh_linear_attention_bf16(const void* q, const void* k, const void*
   if (n_slots > (1L << 30) || rows > (1L << 31)) return KH_ERR_TOO_LARGE;
   LaParams p{(const bf16_t*)q, (const bf16_t*)k, (const bf16_t*)v, (bf16_t*)o, log_decay, state_in, state_out, seg_start, slots, (float*)workspace,
              ldq, ldk, ldv, ldo, bsq, bsk, bsv, bso, (long)rows, (int)B, (int)H, kv_heads > 0 ? (int)(H / kv_heads) : 1, (int)T, (int)dv, (int)n_slots,
-             1, 0, scale};
+             1, 0, scale, 0};
   const int rc = check(p, B, H, kv_heads, dk, dv, false);
   if (rc != KH_OK) return rc;
   if (T <= 0 || (seg_start && rows < 0)) return KH_ERR_INVALID_ARG;
@@ -624,10 +628,11 @@ KH_EXPORT int kh_linear_attention_bf16(const void* q, const void* k, const void*
 
 KH_EXPORT int kh_linear_attention_step_bf16(const void* q, const void* k, const void* v, void* o, const float* log_decay, const float* state_in,
                                             float* state_out, const int32_t* slots, int64_t n_slots, int64_t B, int64_t H, int64_t kv_heads,
-                                            int64_t dk, int64_t dv, int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo, float scale, void* stream) {
+                                            int64_t dk, int64_t dv, int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo, float scale, int flags, void* stream) {
+  if (flags & ~1) return KH_ERR_INVALID_ARG;
   if (n_slots > (1L << 30)) return KH_ERR_TOO_LARGE;
   LaParams p{(const bf16_t*)q, (const bf16_t*)k, (const bf16_t*)v, (bf16_t*)o, log_decay, state_in, state_out, nullptr, slots, nullptr,
-             0, 0, 0, 0, ldq, ldk, ldv, ldo, 0, (int)B, (int)H, kv_heads > 0 ? (int)(H / kv_heads) : 1, 1, (int)dv, (int)n_slots, 1, C, scale};
+             0, 0, 0, 0, ldq, ldk, ldv, ldo, 0, (int)B, (int)H, kv_heads > 0 ? (int)(H / kv_heads) : 1, 1, (int)dv, (int)n_slots, 1, C, scale, flags};
   const int rc = check(p, B, H, kv_heads, dk, dv, true);
   if (rc != KH_OK) return rc;
   if (ldq < H * dk || ldk < kv_heads * dk || ldv < kv_heads * dv || ldo < H * dv) return KH_ERR_INVALID_ARG;

@@ -24,8 +24,10 @@ __device__ __forceinline__ void load8(const T* at, long left, T (&v)[8]) {
 }
 
 // ---------------------------------------------------------------- quantisation
-// A thread takes eight weights of a row, G / 8 threads in a row a group.  Every row starts with a new group, so a group's threads lie
-// in one wave, aligned.
+// A thread takes eight weights of a row, G / 8 threads in a row a group: every row starts with a new group, so a group's threads lie in one wave, aligned.
+// A wave takes 64 such pieces of QR rows, all of whose loads are on their way before the first is used.  Bound by the bytes (2.5 a weight read and written).
+constexpr int QR = 4;
+
 struct QuantParams {
   const void* w;
   uint8_t* q;
@@ -38,56 +40,64 @@ struct QuantParams {
 template <typename T, int G, bool ZERO>
 __global__ __launch_bounds__(256) void quantize_kernel(const QuantParams p) {
   constexpr int GT = G / 8;
-  const int per_row = p.groups * GT;
-  const long id = (long)blockIdx.x * 256 + threadIdx.x;
-  const long row = id / per_row;
-  const int u = (int)(id - row * per_row);
-  if (row >= p.N) return;            // (whole groups: per_row is a multiple of GT)
-  T v[8];
-  load8<T>((const T*)p.w + row * p.K + (long)u * 8, (long)p.K - (long)u * 8, v);
-  float f[8], lo = 0.f, hi = 0.f;
-  bool nan = false;
+  const int u = blockIdx.x * 64 + (threadIdx.x & 63), wave = threadIdx.x >> 6;
+  if (u >= p.groups * GT) return;    // (whole groups)
+  const int left = p.K - u * 8, g = u / GT;
+  for (long row0 = ((long)blockIdx.y * 4 + wave) * QR; row0 < p.N; row0 += (long)gridDim.y * (4 * QR)) {
+    T v[QR][8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    f[e] = (float)v[e];
-    nan |= f[e] != f[e];
-    lo = fminf(lo, f[e]);
-    hi = fmaxf(hi, f[e]);
-  }
-  int bad = nan;
+    for (int i = 0; i < QR; ++i) {
+      const long row = row0 + i < p.N ? row0 + i : p.N - 1;
+      load8<T>((const T*)p.w + row * p.K + (long)u * 8, left, v[i]);
+    }
 #pragma unroll
-  for (int o = GT / 2; o > 0; o >>= 1) {
-    lo = fminf(lo, __shfl_xor(lo, o, 64));
-    hi = fmaxf(hi, __shfl_xor(hi, o, 64));
-    bad |= __shfl_xor(bad, o, 64);
-  }
-  float s = ZERO ? (hi - lo) / 15.f : fmaxf(hi, -lo) / 7.f;
-  if (bad) s = __builtin_nanf("");
-  const bf16_t sb = (bf16_t)s;
-  s = (float)sb;
-  const bool some = s > 0.f;
-  auto level = [&](float a) {        // rint(a / s), 0 where that is no number
-    const float r = some ? rintf(a / s) : 0.f;
-    return r == r ? r : 0.f;
-  };
-  const float z = ZERO ? fminf(fmaxf(level(-lo), 0.f), 15.f) : 8.f;
-  uint32_t word = 0;
+    for (int i = 0; i < QR; ++i) {
+      const long row = row0 + i;
+      if (row >= p.N) break;
+      float f[8], lo = 0.f, hi = 0.f;
+      int bad = 0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) word |= (uint32_t)(int)fminf(fmaxf(level(f[e]) + z, 0.f), 15.f) << (4 * e);
-  if (u < p.words) {
-    if (u * 8 >= p.K) word = 0;      // filling
-    else if (p.K - u * 8 < 8) word &= (1u << (4 * (p.K - u * 8))) - 1u;
-    reinterpret_cast<uint32_t*>(p.q)[row * p.words + u] = word;
-  }
-  const int g = u / GT;
-  if (u % GT == 0) {
-    p.scale[row * p.gstride + g] = sb;
-    if (ZERO) p.zero[row * p.gstride + g] = (uint8_t)(int)z;
-    if (g == p.groups - 1)
-      for (int i = p.groups; i < p.gstride; ++i) {
-        p.scale[row * p.gstride + i] = (bf16_t)0.f;
-        if (ZERO) p.zero[row * p.gstride + i] = 0;
+      for (int e = 0; e < 8; ++e) {
+        f[e] = (float)v[i][e];
+        bad |= f[e] != f[e];
+        lo = fminf(lo, f[e]);
+        hi = fmaxf(hi, f[e]);
       }
+      if (!ZERO) hi = fmaxf(hi, -lo);
+#pragma unroll
+      for (int o = GT / 2; o > 0; o >>= 1) {
+        if (ZERO) lo = fminf(lo, __shfl_xor(lo, o, 64));
+        hi = fmaxf(hi, __shfl_xor(hi, o, 64));
+        bad |= __shfl_xor(bad, o, 64);
+      }
+      float s = ZERO ? (hi - lo) / 15.f : hi / 7.f;
+      if (bad) s = __builtin_nanf("");
+      const bf16_t sb = (bf16_t)s;
+      s = (float)sb;
+      const bool some = s > 0.f;
+      auto level = [&](float a) {    // rint(a / s), 0 where that is no number
+        const float r = some ? rintf(a / s) : 0.f;
+        return r == r ? r : 0.f;
+      };
+      const float z = ZERO ? fminf(fmaxf(level(-lo), 0.f), 15.f) : 8.f;
+      uint32_t word = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) word |= (uint32_t)(int)fminf(fmaxf(level(f[e]) + z, 0.f), 15.f) << (4 * e);
+      if (u < p.words) {             // (behind the last weight: filling)
+        if (left <= 0) word = 0;
+        else if (left < 8) word &= (1u << (4 * left)) - 1u;
+        reinterpret_cast<uint32_t*>(p.q)[row * p.words + u] = word;
+      }
+      if (u % GT == 0) {
+        p.scale[row * p.gstride + g] = sb;
+        if (ZERO) p.zero[row * p.gstride + g] = (uint8_t)(int)z;
+        if (g == p.groups - 1)
+          for (int k = p.groups; k < p.gstride; ++k) {
+            p.scale[row * p.gstride + k] = (bf16_t)0.f;
+            if (ZERO) p.zero[row * p.gstride + k] = 0;
+          }
+      }
+    }
   }
 }
 
@@ -98,27 +108,40 @@ struct ValueParams {
   const uint8_t* zero;
   void* out;
   long N;
-  int K, G, gstride, words;
+  int K, gshift, gstride, words;     // gshift: log2 of a group's words of eight codes
 };
 
 template <typename T>
 __global__ __launch_bounds__(256) void values_kernel(const ValueParams p) {
-  const long id = (long)blockIdx.x * 256 + threadIdx.x;
-  const long row = id / p.words;
-  const int u = (int)(id - row * p.words);
-  if (row >= p.N || u * 8 >= p.K) return;
-  const uint32_t word = p.q[row * p.words + u];
-  const long at = row * p.gstride + u * 8 / p.G;
-  const float s = (float)p.scale[at];
-  const int z = p.zero ? p.zero[at] : 8;
-  T v[8];
+  const int u = blockIdx.x * 64 + (threadIdx.x & 63), wave = threadIdx.x >> 6, left = p.K - u * 8;
+  if (left <= 0) return;
+  const int g = u >> p.gshift;
+  for (long row0 = ((long)blockIdx.y * 4 + wave) * QR; row0 < p.N; row0 += (long)gridDim.y * (4 * QR)) {
+    uint32_t word[QR];
+    bf16_t s[QR];
+    int z[QR];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = (T)(s * (float)((int)((word >> (4 * e)) & 15u) - z));
-  T* o = (T*)p.out + row * p.K + u * 8;
-  if (p.K - u * 8 >= 8) {
-    __builtin_memcpy(o, v, sizeof(v));
-  } else {
-    for (int e = 0; e < p.K - u * 8; ++e) o[e] = v[e];
+    for (int i = 0; i < QR; ++i) {
+      const long row = row0 + i < p.N ? row0 + i : p.N - 1;
+      word[i] = p.q[row * p.words + u];
+      s[i] = p.scale[row * p.gstride + g];
+      z[i] = p.zero ? p.zero[row * p.gstride + g] : 8;
+    }
+#pragma unroll
+    for (int i = 0; i < QR; ++i) {
+      if (row0 + i >= p.N) break;
+      T v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = (T)((float)s[i] * (float)((int)((word[i] >> (4 * e)) & 15u) - z[i]));
+      T* o = (T*)p.out + (row0 + i) * p.K + u * 8;
+      if (left >= 8) {
+        __builtin_memcpy(o, v, sizeof(v));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e < left) o[e] = v[e];
+      }
+    }
   }
 }
 
@@ -831,6 +854,7 @@ int launch_linear(const LinParams& p, int G, hipStream_t s) {
   return G == 32 ? launch_few<T, 32, false>(p, s) : G == 64 ? launch_few<T, 64, false>(p, s) : launch_few<T, 128, false>(p, s);
 }
 
+unsigned rows_grid(long N) { return (unsigned)((N + 4 * QR - 1) / (4 * QR) < 65535 ? (N + 4 * QR - 1) / (4 * QR) : 65535); }
 bool group_ok(int64_t g) { return g == 32 || g == 64 || g == 128; }
 
 }  // namespace
@@ -839,11 +863,12 @@ KH_EXPORT int kh_quantize_w4(const void* w, void* q, void* scale, void* zero, in
   if (!w || !q || !scale || N <= 0 || K <= 0 || type < 0 || type > 2) return KH_ERR_INVALID_ARG;
   if (!group_ok(group)) return KH_ERR_UNSUPPORTED;
   if (!kh_aligned16(q) || !kh_aligned16(scale)) return KH_ERR_ALIGNMENT;
-  const long groups = (K + group - 1) / group, total = N * groups * (group / 8), wg = (total + 255) / 256;
-  if (K > (1L << 24) || N > (1L << 24) || wg > 0x7fffffffL) return KH_ERR_TOO_LARGE;
+  if (K > (1L << 24) || N > (1L << 24)) return KH_ERR_TOO_LARGE;
+  const long groups = (K + group - 1) / group, pieces = groups * (group / 8);
+  const dim3 grid((unsigned)((pieces + 63) / 64), rows_grid(N));
   QuantParams p{w, (uint8_t*)q, (bf16_t*)scale, (uint8_t*)zero, (long)N, (int)K, (int)groups, (int)((groups + 3) / 4 * 4), (int)((K + 31) / 32 * 4)};
   hipStream_t s = (hipStream_t)stream;
-  auto go = [&](auto kernel) { kh_launch(KH_TAG_W4_QUANTIZE, kernel, dim3((unsigned)wg), dim3(256), 0, s, p); };
+  auto go = [&](auto kernel) { kh_launch(KH_TAG_W4_QUANTIZE, kernel, grid, dim3(256), 0, s, p); };
 #define KH_BY_GROUP(T)                                                                            \
   if (group == 32) zero ? go(quantize_kernel<T, 32, true>) : go(quantize_kernel<T, 32, false>);     \
   else if (group == 64) zero ? go(quantize_kernel<T, 64, true>) : go(quantize_kernel<T, 64, false>); \
@@ -860,11 +885,12 @@ KH_EXPORT int kh_dequantize_w4(const void* q, const void* scale, const void* zer
   if (!q || !scale || !out || N <= 0 || K <= 0 || type < 0 || type > 2) return KH_ERR_INVALID_ARG;
   if (!group_ok(group)) return KH_ERR_UNSUPPORTED;
   if (!kh_aligned16(q) || !kh_aligned16(scale)) return KH_ERR_ALIGNMENT;
-  const long groups = (K + group - 1) / group, words = (K + 31) / 32 * 4, wg = (N * words + 255) / 256;
-  if (K > (1L << 24) || N > (1L << 24) || wg > 0x7fffffffL) return KH_ERR_TOO_LARGE;
-  ValueParams p{(const uint32_t*)q, (const bf16_t*)scale, (const uint8_t*)zero, out, (long)N, (int)K, (int)group, (int)((groups + 3) / 4 * 4), (int)words};
+  if (K > (1L << 24) || N > (1L << 24)) return KH_ERR_TOO_LARGE;
+  const long groups = (K + group - 1) / group, words = (K + 31) / 32 * 4;
+  const dim3 grid((unsigned)((words + 63) / 64), rows_grid(N));
+  ValueParams p{(const uint32_t*)q, (const bf16_t*)scale, (const uint8_t*)zero, out, (long)N, (int)K, group == 32 ? 2 : group == 64 ? 3 : 4, (int)((groups + 3) / 4 * 4), (int)words};
   hipStream_t s = (hipStream_t)stream;
-  auto go = [&](auto kernel) { kh_launch(KH_TAG_W4_VALUES, kernel, dim3((unsigned)wg), dim3(256), 0, s, p); };
+  auto go = [&](auto kernel) { kh_launch(KH_TAG_W4_VALUES, kernel, grid, dim3(256), 0, s, p); };
   type == 0 ? go(values_kernel<bf16_t>) : type == 1 ? go(values_kernel<_Float16>) : go(values_kernel<float>);
   KH_RETURN_LAST_ERROR();
 }

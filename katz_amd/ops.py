@@ -1305,19 +1305,24 @@ def conv_out_cfg_euler(x: torch.Tensor, w_packed: torch.Tensor, bias: Optional[t
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
-def _here(**tensors) -> None:
-    """Every given tensor lies on the current device: the launch goes to that device's stream."""
-    dev = torch._C._cuda_getDevice() if torch.cuda.is_available() else -1
-    for name, t in tensors.items():
-        if t is not None and (not t.is_cuda or t.get_device() != dev):
-            raise _lib.KatzHipError(f"{name} must live on the current GPU (got {t.device}); katz_hip has no CPU path")
+def _here(first: torch.Tensor, *others) -> None:
+    """Every given tensor lies on the current device: the launch goes to that device's stream.  (These checks run once a token: plain loops.)"""
+    dev = first.get_device()
+    if dev >= 0 and dev == torch._C._cuda_getDevice():
+        for t in others:
+            if t is not None and t.get_device() != dev:
+                break
+        else:
+            return
+    raise _lib.KatzHipError("every tensor must live on the current GPU (got "
+                            + ", ".join(str(t.device) for t in (first, *others) if t is not None) + "); katz_hip has no CPU path")
 
 
-def _vector(t: Optional[torch.Tensor], n: int, dtype, name: str) -> None:
-    if t is not None:
-        _req(t, dtype, name)
-        if t.shape != (n,):
-            raise ValueError(f"{name} must be [{n}], got {tuple(t.shape)}")
+def _fits(t: torch.Tensor, dtype, shape, name: str) -> None:
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous {tuple(shape)}, got {tuple(t.shape)}")
 
 
 def block_norm(y: Optional[torch.Tensor], h: torch.Tensor, post: bool = False, post_weight: Optional[torch.Tensor] = None,
@@ -1330,60 +1335,59 @@ def block_norm(y: Optional[torch.Tensor], h: torch.Tensor, post: bool = False, p
     kind: "rms" or "layer"; y is normed with post=True only.  y None: (h, N(h)), the norm before the first block.  h [..., D] is the stream, in
     y's type or fp32; u has y's (or h's, without y).  gate: [D], [B, D] for h [B, ..., D], or h's shape.  h_out may be h (in place), out may be y."""
     lib = _lib.load()
-    if kind not in ("rms", "layer"):
+    if kind != "rms" and kind != "layer":
         raise ValueError(f"unknown norm {kind!r}")
-    dt = (h if y is None else y).dtype
-    if h.dtype not in _TYPES or dt not in _TYPES or h.dtype not in (dt, torch.float32):
-        raise TypeError(f"y must be bf16, fp16 or fp32 and h the same or fp32, got {dt} and {h.dtype}")
-    if h.dim() < 1:
+    dt, st = (h if y is None else y).dtype, h.dtype
+    if dt not in _TYPES or (st is not dt and st is not torch.float32):
+        raise TypeError(f"y must be bf16, fp16 or fp32 and h the same or fp32, got {dt} and {st}")
+    shape = h.shape
+    if not shape:
         raise ValueError("h must have rows")
-    D = h.shape[-1]
-    _here(y=y, h=h, gate=gate, post_weight=post_weight, post_bias=post_bias, pre_weight=pre_weight, pre_bias=pre_bias, h_out=h_out, out=out)
-    _req(h, h.dtype, "h")
-    if y is None:
-        if post or gate is not None or h_out is not None or residual_scale != 1.0 or not pre:
-            raise ValueError("without y there is only the norm before the block")
-    else:
-        _req(y, dt, "y")
-        if y.shape != h.shape:
-            raise ValueError(f"y {tuple(y.shape)} and h {tuple(h.shape)} must have one shape")
+    D = shape[-1]
+    _here(h, y, gate, post_weight, post_bias, pre_weight, pre_bias, h_out, out)
+    _fits(h, st, shape, "h")
+    if y is not None:
+        _fits(y, dt, shape, "y")
+    elif post or gate is not None or h_out is not None or residual_scale != 1.0 or not pre:
+        raise ValueError("without y there is only the norm before the block")
     if not post and (post_weight is not None or post_bias is not None):
         raise ValueError("post_weight / post_bias without post=True")
     if not pre and (pre_weight is not None or pre_bias is not None or out is not None):
         raise ValueError("pre_weight / pre_bias / out with pre=False")
-    for name, t in (("post_weight", post_weight), ("post_bias", post_bias), ("pre_weight", pre_weight), ("pre_bias", pre_bias)):
-        _vector(t, D, dt, name)
+    if post_weight is not None:
+        _fits(post_weight, dt, (D,), "post_weight")
+    if post_bias is not None:
+        _fits(post_bias, dt, (D,), "post_bias")
+    if pre_weight is not None:
+        _fits(pre_weight, dt, (D,), "pre_weight")
+    if pre_bias is not None:
+        _fits(pre_bias, dt, (D,), "pre_bias")
     M = h.numel() // D if D else 0
     gate_rows = 1
     if gate is not None:
-        _req(gate, dt, "gate")
-        if gate.shape == (D,):
+        gs = gate.shape
+        if gs == (D,):
             gate_rows = M
-        elif gate.shape == h.shape:
-            gate_rows = 1
-        elif h.dim() > 2 and gate.shape == (h.shape[0], D):
-            gate_rows = M // max(h.shape[0], 1)
-        else:
-            raise ValueError(f"gate must be [{D}], [{h.shape[0]}, {D}] or {tuple(h.shape)}, got {tuple(gate.shape)}")
+        elif len(shape) > 2 and gs == (shape[0], D):
+            gate_rows = M // max(shape[0], 1)
+        elif gs != shape:
+            raise ValueError(f"gate must be [{D}], [{shape[0]}, {D}] or {tuple(shape)}, got {tuple(gs)}")
+        _fits(gate, dt, gs, "gate")
     if y is not None:
         if h_out is None:
             h_out = torch.empty_like(h)
         else:
-            _req(h_out, h.dtype, "h_out")
-            if h_out.shape != h.shape:
-                raise ValueError("h_out must have h's shape")
+            _fits(h_out, st, shape, "h_out")
     if pre:
         if out is None:
-            out = torch.empty(h.shape, dtype=dt, device=h.device)
+            out = torch.empty_like(h, dtype=dt)
         else:
-            _req(out, dt, "out")
-            if out.shape != h.shape:
-                raise ValueError("out must have h's shape")
+            _fits(out, dt, shape, "out")
     if M:
-        rc = lib.kh_block_norm(_ptr(y), _ptr(h), _ptr(gate), gate_rows, _ptr(post_weight), _ptr(post_bias), _ptr(pre_weight), _ptr(pre_bias),
-                               _ptr(h_out), _ptr(out), M, D, float(residual_scale), float(eps), (kind == "layer") | (bool(post) << 1),
-                               _TYPES[dt], _TYPES[h.dtype], _stream())
-        _lib.check(rc, "kh_block_norm")
+        rc = lib.kh_block_norm(_ptr(y), h.data_ptr(), _ptr(gate), gate_rows, _ptr(post_weight), _ptr(post_bias), _ptr(pre_weight), _ptr(pre_bias),
+                               _ptr(h_out), _ptr(out), M, D, residual_scale, eps, (kind == "layer") | (bool(post) << 1), _TYPES[dt], _TYPES[st], _stream())
+        if rc:
+            _lib.check(rc, "kh_block_norm")
     return (h if y is None else h_out), out
 
 
@@ -1395,21 +1399,19 @@ class W4Weight:
     __slots__ = ("q", "scale", "zero", "in_features", "out_features", "group", "groups")
 
     def __init__(self, q: torch.Tensor, scale: torch.Tensor, zero: Optional[torch.Tensor], in_features: int, group: int):
-        if group not in (32, 64, 128):
+        if group != 64 and group != 128 and group != 32:
             raise ValueError(f"group must be 32, 64 or 128, got {group}")
         if in_features < 1 or q.dim() != 2:
             raise ValueError("q must be [N, ceil(in_features / 32) * 16]")
         N, groups = q.shape[0], -(-in_features // group)
-        for name, t, dt, cols in (("q", q, torch.uint8, -(-in_features // 32) * 16), ("scale", scale, BF16, -(-groups // 4) * 4),
-                                  ("zero", zero, torch.uint8, -(-groups // 4) * 4)):
-            if t is None and name == "zero":
-                continue
-            if t.dtype != dt:
-                raise TypeError(f"{name} must be {dt}, got {t.dtype}")
-            if t.shape != (N, cols) or not t.is_contiguous():
-                raise ValueError(f"{name} must be contiguous [{N}, {cols}], got {tuple(t.shape)}")
-            if t.device != q.device:
-                raise ValueError(f"{name} lies on {t.device}, q on {q.device}")
+        marks = (N, groups + 3 & ~3)
+        _fits(q, torch.uint8, (N, (in_features + 31 >> 5) * 16), "q")
+        _fits(scale, BF16, marks, "scale")
+        if zero is not None:
+            _fits(zero, torch.uint8, marks, "zero")
+        dev = q.get_device()
+        if scale.get_device() != dev or (zero is not None and zero.get_device() != dev):
+            raise ValueError("q, scale and zero must lie on one device")
         self.q, self.scale, self.zero = q, scale, zero
         self.in_features, self.out_features, self.group, self.groups = in_features, N, group, groups
 
@@ -1422,17 +1424,18 @@ def quantize_w4(weight: torch.Tensor, group: int = 64, zeros: bool = False) -> W
         raise TypeError("weight must be [N, K] in bf16, fp16 or fp32")
     if group not in (32, 64, 128):
         raise ValueError(f"group must be 32, 64 or 128, got {group}")
-    _here(weight=weight)
-    _req(weight, weight.dtype, "weight")
+    _here(weight)
+    _fits(weight, weight.dtype, weight.shape, "weight")
     N, K = weight.shape
     if N < 1 or K < 1:
         raise ValueError("weight must not be empty")
     marks = -(-K // group) + 3 & ~3
-    q = torch.empty((N, -(-K // 32) * 16), dtype=torch.uint8, device=weight.device)
-    scale = torch.empty((N, marks), dtype=BF16, device=weight.device)
-    zero = torch.empty((N, marks), dtype=torch.uint8, device=weight.device) if zeros else None
-    rc = lib.kh_quantize_w4(_ptr(weight), _ptr(q), _ptr(scale), _ptr(zero), N, K, group, _TYPES[weight.dtype], _stream())
-    _lib.check(rc, "kh_quantize_w4")
+    q = weight.new_empty((N, (K + 31 >> 5) * 16), dtype=torch.uint8)
+    scale = weight.new_empty((N, marks), dtype=BF16)
+    zero = weight.new_empty((N, marks), dtype=torch.uint8) if zeros else None
+    rc = lib.kh_quantize_w4(weight.data_ptr(), q.data_ptr(), scale.data_ptr(), _ptr(zero), N, K, group, _TYPES[weight.dtype], _stream())
+    if rc:
+        _lib.check(rc, "kh_quantize_w4")
     return W4Weight(q, scale, zero, K, group)
 
 
@@ -1441,17 +1444,17 @@ def dequantize_w4(w: W4Weight, dtype: torch.dtype = BF16, out: Optional[torch.Te
     lib = _lib.load()
     if dtype not in _TYPES:
         raise TypeError(f"dtype must be bf16, fp16 or fp32, got {dtype}")
-    _here(q=w.q, out=out)
+    q = w.q
+    _here(q, out)
+    N, K = w.out_features, w.in_features
     if out is None:
-        out = torch.empty((w.out_features, w.in_features), dtype=dtype, device=w.q.device)
+        out = q.new_empty((N, K), dtype=dtype)
     else:
-        _req(out, dtype, "out")
-        if out.shape != (w.out_features, w.in_features):
-            raise ValueError("out has the wrong shape")
-    if w.out_features:
-        rc = lib.kh_dequantize_w4(_ptr(w.q), _ptr(w.scale), _ptr(w.zero), _ptr(out), w.out_features, w.in_features, w.group, _TYPES[dtype],
-                                  _stream())
-        _lib.check(rc, "kh_dequantize_w4")
+        _fits(out, dtype, (N, K), "out")
+    if N:
+        rc = lib.kh_dequantize_w4(q.data_ptr(), w.scale.data_ptr(), _ptr(w.zero), out.data_ptr(), N, K, w.group, _TYPES[dtype], _stream())
+        if rc:
+            _lib.check(rc, "kh_dequantize_w4")
     return out
 
 
@@ -1461,38 +1464,34 @@ def w4_linear(x: torch.Tensor, w: W4Weight, bias: Optional[torch.Tensor] = None,
     """y = x w^T + b + ((x A_cat^T) * col_scale) B_cat^T (+ residual) with weights in 4 bits, bf16 or fp16 by x.dtype; the adapter operands as
     for lora_linear (a_cat [R,K], b_cat [N,R], col_scale [R] fp32, R % 32 == 0, R <= 128).  Made for few rows, right for any number."""
     lib = _lib.load()
-    dt = x.dtype
-    if dt not in (torch.bfloat16, torch.float16):
+    dt, xs, q = x.dtype, x.shape, w.q
+    if dt is not torch.bfloat16 and dt is not torch.float16:
         raise TypeError(f"x must be bf16 or fp16, got {dt}")
-    _here(x=x, q=w.q, bias=bias, a_cat=a_cat, b_cat=b_cat, col_scale=col_scale, residual=residual, out=out)
-    _req(x, dt, "x")
     N, K = w.out_features, w.in_features
-    if x.dim() < 1 or x.shape[-1] != K:
-        raise ValueError(f"weight [{N}, {K}] does not match x {tuple(x.shape)}")
+    if not xs or xs[-1] != K:
+        raise ValueError(f"weight [{N}, {K}] does not match x {tuple(xs)}")
+    _here(x, q, bias, a_cat, b_cat, col_scale, residual, out)
+    _fits(x, dt, xs, "x")
     M = x.numel() // K
     R = 0
-    if a_cat is None:
-        if b_cat is not None or col_scale is not None:
-            raise ValueError("b_cat / col_scale without a_cat")
-    else:
+    if a_cat is not None:
         if b_cat is None or col_scale is None:
             raise ValueError("a_cat without b_cat / col_scale")
-        _req(a_cat, dt, "a_cat"); _req(b_cat, dt, "b_cat"); _req(col_scale, torch.float32, "col_scale")
         R = a_cat.shape[0]
-        if a_cat.shape != (R, K) or b_cat.shape != (N, R) or col_scale.shape != (R,):
-            raise ValueError("a_cat/b_cat/col_scale shapes must be [R,K], [N,R], [R]")
-    _vector(bias, N, dt, "bias")
-    shape = tuple(x.shape[:-1]) + (N,)
+        _fits(a_cat, dt, (R, K), "a_cat")
+        _fits(b_cat, dt, (N, R), "b_cat")
+        _fits(col_scale, torch.float32, (R,), "col_scale")
+    elif b_cat is not None or col_scale is not None:
+        raise ValueError("b_cat / col_scale without a_cat")
+    if bias is not None:
+        _fits(bias, dt, (N,), "bias")
+    shape = xs[:-1] + (N,)
     if residual is not None:
-        _req(residual, dt, "residual")
-        if residual.shape != shape:
-            raise ValueError("residual must have the shape of the output")
+        _fits(residual, dt, shape, "residual")
     if out is None:
-        out = torch.empty(shape, dtype=dt, device=x.device)
+        out = x.new_empty(shape)
     else:
-        _req(out, dt, "out")
-        if out.shape != shape:
-            raise ValueError("out has the wrong shape")
+        _fits(out, dt, shape, "out")
     if not M or not N:
         return out
     ws = None
@@ -1500,58 +1499,70 @@ def w4_linear(x: torch.Tensor, w: W4Weight, bias: Optional[torch.Tensor] = None,
         nbytes = lib.kh_w4_linear_workspace_bytes(M, K, R)
         if nbytes < 0:
             raise ValueError(f"the adapters' columns must be a multiple of 32 up to 128, got {R}")
-        ws = torch.empty(nbytes // 4, dtype=torch.float32, device=x.device)
-    rc = lib.kh_w4_linear(_ptr(x), _ptr(w.q), _ptr(w.scale), _ptr(w.zero), _ptr(bias), _ptr(a_cat), _ptr(b_cat), _ptr(col_scale), _ptr(residual),
-                          _ptr(out), _ptr(ws), M, N, K, R, w.group, _TYPES[dt], _stream())
-    _lib.check(rc, "kh_w4_linear")
+        ws = x.new_empty(nbytes // 2)          # (elements of two bytes)
+    rc = lib.kh_w4_linear(x.data_ptr(), q.data_ptr(), w.scale.data_ptr(), _ptr(w.zero), _ptr(bias), _ptr(a_cat), _ptr(b_cat), _ptr(col_scale),
+                          _ptr(residual), out.data_ptr(), _ptr(ws), M, N, K, R, w.group, _TYPES[dt], _stream())
+    if rc:
+        _lib.check(rc, "kh_w4_linear")
     return out
 
 
-def _la_sizes(q, k, v, heads: int, kv_heads: Optional[int], log_decay: torch.Tensor, rows_dim: int):
+def _la_sizes(q, k, v, heads: int, kv_heads: Optional[int], log_decay: torch.Tensor, dims: int):
+    """(kv_heads, dk, dv) of rows [.., heads * dk] with `dims` axes."""
     kv = heads if kv_heads is None else kv_heads
     if heads < 1 or kv < 1 or heads % kv:
         raise ValueError(f"{heads} heads cannot share the keys of {kv}")
-    for n, t in (("q", q), ("k", k), ("v", v)):
-        if t.dtype != BF16 or t.dim() != rows_dim or t.stride(-1) != 1:
-            raise TypeError(f"{n} must be bfloat16 with {rows_dim} axes, the last contiguous")
-        if t.shape[:-1] != q.shape[:-1]:
-            raise ValueError(f"{n} must have the rows of q")
-    if q.shape[-1] % heads or k.shape[-1] % kv or v.shape[-1] % kv or q.shape[-1] // heads != k.shape[-1] // kv:
+    for t in (q, k, v):
+        if t.dtype is not BF16 or t.dim() != dims or t.stride(-1) != 1:
+            raise TypeError(f"q, k and v must be bfloat16 with {dims} axes, the last contiguous, got {t.dtype} {tuple(t.shape)}")
+    qs, ks, vs = q.shape, k.shape, v.shape
+    if qs[:-1] != ks[:-1] or qs[:-1] != vs[:-1]:
+        raise ValueError("q, k and v must have the same rows")
+    dk, dv = qs[-1] // heads, vs[-1] // kv
+    if qs[-1] != heads * dk or ks[-1] != kv * dk or vs[-1] != kv * dv:
         raise ValueError("q must be [.., heads * dk], k [.., kv_heads * dk], v [.., kv_heads * dv]")
-    _req(log_decay, torch.float32, "log_decay")
-    if log_decay.shape != (heads,):
-        raise ValueError(f"log_decay must be [{heads}]")
-    return kv, q.shape[-1] // heads, v.shape[-1] // kv
+    _fits(log_decay, torch.float32, (heads,), "log_decay")
+    return kv, dk, dv
 
 
 def _la_strides(t: torch.Tensor):
     """(row, sequence) strides of [B, T, W] or (row, 0) of [rows, W]; those of an axis of one element, which may be anything, as W."""
-    s = [t.stride(i) if t.shape[i] > 1 else t.shape[-1] for i in range(t.dim() - 1)]
-    return (s[1], s[0]) if len(s) == 2 else (s[0], 0)
+    shape, st = t.shape, t.stride()
+    s0 = st[0] if shape[0] > 1 else shape[-1]
+    if len(st) == 2:
+        return s0, 0
+    return (st[1] if shape[1] > 1 else shape[-1]), s0
 
 
 def _la_out(out: torch.Tensor, shape) -> None:
-    if out.dtype != BF16 or out.shape != shape or out.stride(-1) != 1 or any(n > 1 and st < shape[-1] for n, st in zip(out.shape[:-1], out.stride())):
+    if out.dtype is not BF16 or out.shape != shape or out.stride(-1) != 1 or any(n > 1 and st < shape[-1] for n, st in zip(shape[:-1], out.stride())):
         raise ValueError(f"out must be bfloat16 {tuple(shape)}, rows apart and their last axis contiguous")
 
 
-def _la_states(state, state_out, slots, B: int, heads: int, dk: int, dv: int, device):
+def _la_states(state, state_out, slots, like, B: int, heads: int, dk: int, dv: int):
     """state_out to write to, and the number of its slots."""
     if state_out is None:
         state_out = state
-    if state_out is None:
-        if slots is not None:
-            raise ValueError("slots without a pool of states")
-        state_out = torch.empty((B, heads, dk, dv), dtype=torch.float32, device=device)
-    n = state_out.shape[0] if state_out.dim() else 0
-    for name, t in (("state", state), ("state_out", state_out)):
-        if t is not None:
-            _req(t, torch.float32, name)
-            if t.shape != (n, heads, dk, dv) or (slots is None and n != B):
-                raise ValueError(f"{name} must be [{B if slots is None else 'slots'}, {heads}, {dk}, {dv}], got {tuple(t.shape)}")
+        if state is None:
+            if slots is not None:
+                raise ValueError("slots without a pool of states")
+            return like.new_empty((B, heads, dk, dv), dtype=torch.float32), B
+    n = B
     if slots is not None:
-        _vector(slots, B, torch.int32, "slots")
+        _fits(slots, torch.int32, (B,), "slots")
+        n = state_out.shape[0] if state_out.dim() else 0
+    shape = (n, heads, dk, dv)
+    _fits(state_out, torch.float32, shape, "state_out" if state_out is not state else "state")
+    if state is not None and state is not state_out:
+        _fits(state, torch.float32, shape, "state")
     return state_out, n
+
+
+def _la_step(lib, q, k, v, out, log_decay, state, state_out, slots, n_slots, B, heads, kv, dk, dv, strides, scale, fill=0) -> None:
+    rc = lib.kh_linear_attention_step_bf16(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), log_decay.data_ptr(), state.data_ptr(),
+                                           state_out.data_ptr(), _ptr(slots), n_slots, B, heads, kv, dk, dv, *strides, scale, fill, _stream())
+    if rc:
+        _lib.check(rc, "kh_linear_attention_step_bf16")
 
 
 def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, log_decay: torch.Tensor, scale: Optional[float] = None,
@@ -1569,42 +1580,45 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: i
     lib = _lib.load()
     packed = seg_start is not None
     kv, dk, dv = _la_sizes(q, k, v, heads, kv_heads, log_decay, 2 if packed else 3)
-    _here(q=q, k=k, v=v, log_decay=log_decay, state=state, state_out=state_out, slots=slots, seg_start=seg_start, out=out)
+    _here(q, k, v, log_decay, state, state_out, slots, seg_start, out)
     if packed:
         _req(seg_start, torch.int32, "seg_start")
         if seg_start.dim() != 1 or seg_start.numel() < 2 or max_seg_rows < 1:
             raise ValueError("packed rows need seg_start [B + 1] and max_seg_rows")
-        B, T, rows = seg_start.numel() - 1, min(max_seg_rows, max(q.shape[0], 1)), q.shape[0]
+        rows = q.shape[0]
+        B, T = seg_start.numel() - 1, min(max_seg_rows, max(rows, 1))
     else:
-        B, T, rows = q.shape[0], q.shape[1], 0
-    state_out, n_slots = _la_states(state, state_out, slots, B, heads, dk, dv, q.device)
-    shape = tuple(q.shape[:-1]) + (heads * dv,)
+        B, T, _ = q.shape
+        rows = B * T
+    state_out, n_slots = _la_states(state, state_out, slots, q, B, heads, dk, dv)
+    shape = q.shape[:-1] + (heads * dv,)
     if out is None:
-        out = (torch.zeros if packed or slots is not None else torch.empty)(shape, dtype=BF16, device=q.device)
+        out = q.new_empty(shape) if not packed and slots is None else q.new_zeros(shape)
     else:
         _la_out(out, shape)
     if scale is None:
         scale = dk ** -0.5
-    if not B or not T or (packed and not rows):
-        if B and state is None:
+    if not B or not rows:
+        if state is None:
             state_out.zero_()
-        elif B and state_out is not state:
+        elif state_out is not state and B:
+            if slots is not None:
+                raise ValueError("sequences without tokens, from one pool into another")
             state_out.copy_(state)
         return out, state_out
-    s0 = [_la_strides(t)[1] for t in (q, k, v, out)]
-    if not packed and T == 1 and state is not None and all(st >= t.shape[-1] for st, t in zip(s0, (q, k, v, out))):   # one pass over the state
-        rc = lib.kh_linear_attention_step_bf16(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(log_decay), _ptr(state), _ptr(state_out), _ptr(slots), n_slots,
-                                               B, heads, kv, dk, dv, *s0, float(scale), _stream())
-        _lib.check(rc, "kh_linear_attention_step_bf16")
+    ld, bs = zip(*[_la_strides(t) for t in (q, k, v, out)])
+    if not packed and T == 1 and state is not None and all(st >= t.shape[-1] for st, t in zip(bs, (q, k, v, out))):   # one pass over the state
+        _la_step(lib, q, k, v, out, log_decay, state, state_out, slots, n_slots, B, heads, kv, dk, dv, bs, scale)
         return out, state_out
-    nbytes = lib.kh_linear_attention_workspace_bytes(B, heads, T, rows if packed else B * T, dk, dv)
+    nbytes = lib.kh_linear_attention_workspace_bytes(B, heads, T, rows, dk, dv)
     if nbytes < 0:
         _lib.check(int(nbytes), "kh_linear_attention_workspace_bytes")
-    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device) if nbytes else None
-    ld, bs = zip(*(_la_strides(t) for t in (q, k, v, out)))
-    rc = lib.kh_linear_attention_bf16(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(log_decay), _ptr(state), _ptr(state_out), _ptr(slots), n_slots,
-                                      _ptr(seg_start), rows, _ptr(ws), B, heads, kv, T, dk, dv, *ld, *bs, float(scale), _stream())
-    _lib.check(rc, "kh_linear_attention_bf16")
+    ws = q.new_empty(nbytes // 2) if nbytes else None      # (elements of two bytes)
+    rc = lib.kh_linear_attention_bf16(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), log_decay.data_ptr(), _ptr(state), state_out.data_ptr(),
+                                      _ptr(slots), n_slots, _ptr(seg_start), rows if packed else 0, _ptr(ws), B, heads, kv, T, dk, dv, *ld, *bs, scale,
+                                      _stream())
+    if rc:
+        _lib.check(rc, "kh_linear_attention_bf16")
     return out, state_out
 
 
@@ -1612,22 +1626,22 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, hea
                           scale: Optional[float] = None, kv_heads: Optional[int] = None, state_out: Optional[torch.Tensor] = None,
                           slots: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None):
     """linear_attention of one token a sequence: q [B,heads*dk], k [B,kv_heads*dk], v [B,kv_heads*dv]; (o, state), the state overwritten unless
-    state_out is given.  With slots, rows whose slot lies outside the pool are left out (padded batches in a captured graph)."""
+    state_out is given.  With slots, rows whose slot lies outside the pool are left out (padded batches in a captured graph): those of a given
+    out stay as they were, those of a new one are zero."""
     lib = _lib.load()
     kv, dk, dv = _la_sizes(q, k, v, heads, kv_heads, log_decay, 2)
-    _here(q=q, k=k, v=v, log_decay=log_decay, state=state, state_out=state_out, slots=slots, out=out)
+    _here(q, k, v, log_decay, state, state_out, slots, out)
     B = q.shape[0]
-    state_out, n_slots = _la_states(state, state_out, slots, B, heads, dk, dv, q.device)
+    state_out, n_slots = _la_states(state, state_out, slots, q, B, heads, dk, dv)
     shape = (B, heads * dv)
+    fill = 0
     if out is None:
-        out = (torch.empty if slots is None else torch.zeros)(shape, dtype=BF16, device=q.device)
+        out, fill = q.new_empty(shape), slots is not None
     else:
         _la_out(out, shape)
     if B:
-        rc = lib.kh_linear_attention_step_bf16(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(log_decay), _ptr(state), _ptr(state_out), _ptr(slots), n_slots,
-                                               B, heads, kv, dk, dv, *(_la_strides(t)[0] for t in (q, k, v, out)),
-                                               float(dk ** -0.5 if scale is None else scale), _stream())
-        _lib.check(rc, "kh_linear_attention_step_bf16")
+        _la_step(lib, q, k, v, out, log_decay, state, state_out, slots, n_slots, B, heads, kv, dk, dv, [_la_strides(t)[0] for t in (q, k, v, out)],
+                 dk ** -0.5 if scale is None else scale, fill)
     return out, state_out
 
 

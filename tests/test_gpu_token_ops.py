@@ -474,6 +474,9 @@ def test_linear_attention_step(B, H, Hk, dk, dv, pool):
         assert_within(S[at], rs, HALF[FP32] * rs.abs() + STATE_SLOP * ms, "state")
     for at in range(pool or B):
         assert at in seen or torch.equal(S[at].cpu(), s0[at])
+    if pool:                                               # rows of a new output that are left out are zero
+        new, _ = ops.linear_attention_step(on(q), on(k), on(v), H, on(g), on(s0), kv_heads=Hk, slots=on(slots))
+        assert not new[1].any() and not new[3].any() and torch.equal(new[[0, 2, 4]], got[[0, 2, 4]])
     # into another pool: the first one stays
     other, keep = torch.full_like(sd, 5.0), sd.clone()
     ops.linear_attention_step(on(q), on(k), on(v), H, on(g), sd, kv_heads=Hk, slots=on(slots), state_out=other)

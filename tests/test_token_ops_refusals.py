@@ -64,11 +64,11 @@ def test_linear_attention_entry_points(lib):
     assert size(2, 4, 0, 1, 64, 64) == -1 and size(2, 4, 10, 20, 80, 64) == -2 and size(2, 4, 64, 128, 64, 64) == 0
     assert size(1, 1, 1 << 20, 1 << 20, 128, 128) > 0 and size(1 << 21, 1, 1, 1 << 21, 64, 64) == -4
 
-    def step(s=16, so=16, B=2, dk=64, ld=256, n=2):
-        return lib.kh_linear_attention_step_bf16(16, 16, 16, 16, 16, s, so, None, n, B, 4, 4, dk, 64, *([ld] * 4), 0.1, None)
+    def step(s=16, so=16, B=2, dk=64, ld=256, n=2, flags=0):
+        return lib.kh_linear_attention_step_bf16(16, 16, 16, 16, 16, s, so, None, n, B, 4, 4, dk, 64, *([ld] * 4), 0.1, flags, None)
 
     assert step(s=None) == -1 and step(so=None) == -1 and step(B=0) == -1 and step(n=1) == -1 and step(ld=128) == -1
-    assert step(dk=96) == -2 and step(ld=258) == -3
+    assert step(flags=2) == -1 and step(dk=96) == -2 and step(ld=258) == -3
 
 
 def test_tensor_functions_refuse_what_is_not_on_the_gpu(lib):
