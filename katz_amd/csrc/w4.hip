@@ -7,6 +7,7 @@
 // zero points is filled up to 4.  Scales are bf16 whatever the activations' type: they have the weights' range, and the codes are
 // chosen against the rounded scale.
 #include "kh_common.h"
+#include <type_traits>
 
 namespace {
 
@@ -23,10 +24,51 @@ __device__ __forceinline__ void load8(const T* at, long left, T (&v)[8]) {
   }
 }
 
+// Sixteen bytes that pass by: weights that are quantised, the values of codes.  Kept out of the caches they leave room for what is read again, and lines that are
+// written whole need not be fetched: values of 16384 x 8192 110 -> 48 us, their codes 91 -> 76.
+template <typename T>
+__device__ __forceinline__ void load8_once(const T* at, long left, T (&v)[8]) {
+  if (left >= 8 && ((uintptr_t)at & 15) == 0) {
+    u32x4 t[sizeof(v) / 16];
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(v) / 16; ++i) t[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at) + i);
+    __builtin_memcpy(v, t, sizeof(v));
+  } else {
+    load8<T>(at, left, v);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8_once(T* at, int left, const T (&v)[8]) {
+  if (left >= 8 && ((uintptr_t)at & 15) == 0) {
+    u32x4 t[sizeof(v) / 16];
+    __builtin_memcpy(t, v, sizeof(v));
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(v) / 16; ++i) __builtin_nontemporal_store(t[i], reinterpret_cast<u32x4*>(at) + i);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < left) at[e] = v[e];
+  }
+}
+
 // ---------------------------------------------------------------- quantisation
-// A thread takes eight weights of a row, G / 8 threads in a row a group: every row starts with a new group, so a group's threads lie in one wave, aligned.
-// A wave takes 64 such pieces of QR rows, all of whose loads are on their way before the first is used.  Bound by the bytes (2.5 a weight read and written).
-constexpr int QR = 4;
+// Rows are cut into pieces of eight, filled up to whole groups (or to a row of codes), and the pieces of all rows numbered through: a wave takes PT * 64 in a
+// row, a thread one of every 64, all of whose loads are on their way before the first is used.  A group's G / 8 pieces lie in one wave, aligned.
+constexpr int PT = 4;
+
+struct Pieces {                      // of one row, and what divides a small number by that
+  uint32_t per_row, magic;
+  explicit Pieces(long n) : per_row((uint32_t)n), magic(n < 4 * PT * 64 ? (uint32_t)((1ull << 32) / (uint64_t)n + 1) : 0) {}
+};
+// Row and piece of the i-th of a thread's.  (A workgroup's first row comes from one long division; from there on numbers are below per_row + 1024.)
+__device__ __forceinline__ void piece_of(const Pieces& d, int i, long& row, int& u) {
+  const long first = (long)blockIdx.x * (4 * PT * 64);
+  const long r0 = first / d.per_row;
+  const uint32_t local = (uint32_t)(first - r0 * d.per_row) + (threadIdx.x >> 6) * (PT * 64) + i * 64 + (threadIdx.x & 63);
+  const uint32_t r = d.per_row >= 4 * PT * 64 ? (local >= d.per_row ? 1u : 0u) : __umulhi(local, d.magic);   // (exact: local * per_row < 2^32)
+  row = r0 + r;
+  u = (int)(local - r * d.per_row);
+}
 
 struct QuantParams {
   const void* w;
@@ -35,68 +77,92 @@ struct QuantParams {
   uint8_t* zero;
   long N;
   int K, groups, gstride, words;   // words: of eight codes in a row
+  Pieces pieces;
 };
+
+// The largest of a group of 4, 8 or 16 lanes, in all of them (bits of numbers that are not negative, which order like integers; a NaN is the largest).
+template <int GT>
+__device__ __forceinline__ int group_max(int v) {
+#if __HIP_DEVICE_COMPILE__
+  auto with = [](int x, auto ctrl) {
+    const int y = __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, 0xf, 0xf, false);
+    return x > y ? x : y;
+  };
+  v = with(v, std::integral_constant<int, 0xb1>{});    // quad_perm 1,0,3,2
+  v = with(v, std::integral_constant<int, 0x4e>{});    // quad_perm 2,3,0,1
+  if (GT >= 8) v = with(v, std::integral_constant<int, 0x141>{});    // row_half_mirror
+  if (GT >= 16) v = with(v, std::integral_constant<int, 0x140>{});   // row_mirror
+#endif
+  return v;
+}
 
 template <typename T, int G, bool ZERO>
 __global__ __launch_bounds__(256) void quantize_kernel(const QuantParams p) {
   constexpr int GT = G / 8;
-  const int u = blockIdx.x * 64 + (threadIdx.x & 63), wave = threadIdx.x >> 6;
-  if (u >= p.groups * GT) return;    // (whole groups)
-  const int left = p.K - u * 8, g = u / GT;
-  for (long row0 = ((long)blockIdx.y * 4 + wave) * QR; row0 < p.N; row0 += (long)gridDim.y * (4 * QR)) {
-    T v[QR][8];
+  long row[PT];
+  int u[PT];
+  T v[PT][8];
 #pragma unroll
-    for (int i = 0; i < QR; ++i) {
-      const long row = row0 + i < p.N ? row0 + i : p.N - 1;
-      load8<T>((const T*)p.w + row * p.K + (long)u * 8, left, v[i]);
+  for (int i = 0; i < PT; ++i) {
+    piece_of(p.pieces, i, row[i], u[i]);
+    const long r = row[i] < p.N ? row[i] : p.N - 1;
+    load8_once<T>((const T*)p.w + r * p.K + (long)u[i] * 8, p.K - u[i] * 8, v[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < PT; ++i) {
+    if (row[i] >= p.N) break;        // (whole groups)
+    float f[8];
+    int hi = 0, lo = 0;              // bits of the largest value and of the largest negated one, or of the largest magnitude
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      f[e] = (float)v[i][e];
+      const int bits = __float_as_int(f[e]);
+      hi = max(hi, ZERO ? bits : bits & 0x7fffffff);
+      if (ZERO) lo = max(lo, bits ^ (int)0x80000000);
     }
+    hi = group_max<GT>(hi);
+    if (ZERO) lo = group_max<GT>(lo);
+    const float below = ZERO ? __int_as_float(lo) : 0.f;
+    const float wide = ZERO ? (__int_as_float(hi) + below) / 15.f : __int_as_float(hi) / 7.f;
+    const bf16_t sb = (bf16_t)wide;
+    const float s = (float)sb;
+    float z = 8.f;
+    uint32_t word = 0;
+    auto code = [](float r, float z) { return (uint32_t)(int)fminf(fmaxf(r + z, 0.f), 15.f); };
+    if (s > 1e-30f && s < 1e30f) {
+      // The quotient as a division gives it (halves have to stay halves): the reciprocal is rounded correctly, so one step from its product is the rounded
+      // quotient (Markstein).
+      const float inv = 1.f / s;
+      auto level = [&](float a) {
+        const float q = a * inv;
+        return rintf(fmaf(fmaf(-q, s, a), inv, q));
+      };
+      if (ZERO) z = fminf(fmaxf(level(below), 0.f), 15.f);
 #pragma unroll
-    for (int i = 0; i < QR; ++i) {
-      const long row = row0 + i;
-      if (row >= p.N) break;
-      float f[8], lo = 0.f, hi = 0.f;
-      int bad = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        f[e] = (float)v[i][e];
-        bad |= f[e] != f[e];
-        lo = fminf(lo, f[e]);
-        hi = fmaxf(hi, f[e]);
-      }
-      if (!ZERO) hi = fmaxf(hi, -lo);
-#pragma unroll
-      for (int o = GT / 2; o > 0; o >>= 1) {
-        if (ZERO) lo = fminf(lo, __shfl_xor(lo, o, 64));
-        hi = fmaxf(hi, __shfl_xor(hi, o, 64));
-        bad |= __shfl_xor(bad, o, 64);
-      }
-      float s = ZERO ? (hi - lo) / 15.f : hi / 7.f;
-      if (bad) s = __builtin_nanf("");
-      const bf16_t sb = (bf16_t)s;
-      s = (float)sb;
-      const bool some = s > 0.f;
-      auto level = [&](float a) {    // rint(a / s), 0 where that is no number
-        const float r = some ? rintf(a / s) : 0.f;
+      for (int e = 0; e < 8; ++e) word |= code(level(f[e]), z) << (4 * e);
+    } else {                         // nothing but zeros, very small or very large numbers, or none: rint(a / s), 0 where that is no number
+      auto level = [&](float a) {
+        const float r = s > 0.f ? rintf(a / s) : 0.f;
         return r == r ? r : 0.f;
       };
-      const float z = ZERO ? fminf(fmaxf(level(-lo), 0.f), 15.f) : 8.f;
-      uint32_t word = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) word |= (uint32_t)(int)fminf(fmaxf(level(f[e]) + z, 0.f), 15.f) << (4 * e);
-      if (u < p.words) {             // (behind the last weight: filling)
-        if (left <= 0) word = 0;
-        else if (left < 8) word &= (1u << (4 * left)) - 1u;
-        reinterpret_cast<uint32_t*>(p.q)[row * p.words + u] = word;
-      }
-      if (u % GT == 0) {
-        p.scale[row * p.gstride + g] = sb;
-        if (ZERO) p.zero[row * p.gstride + g] = (uint8_t)(int)z;
-        if (g == p.groups - 1)
-          for (int k = p.groups; k < p.gstride; ++k) {
-            p.scale[row * p.gstride + k] = (bf16_t)0.f;
-            if (ZERO) p.zero[row * p.gstride + k] = 0;
-          }
-      }
+      if (ZERO) z = fminf(fmaxf(level(below), 0.f), 15.f);
+#pragma unroll 1
+      for (int e = 0; e < 8; ++e) word |= code(level(e < 4 ? (e < 2 ? (e == 0 ? f[0] : f[1]) : (e == 2 ? f[2] : f[3])) : (e < 6 ? (e == 4 ? f[4] : f[5]) : (e == 6 ? f[6] : f[7]))), z) << (4 * e);
+    }
+    const int left = p.K - u[i] * 8;
+    if (u[i] < p.words) {            // (behind the last weight: filling)
+      if (left < 8) word = left <= 0 ? 0u : word & ((1u << (4 * left)) - 1u);
+      __builtin_nontemporal_store(word, reinterpret_cast<uint32_t*>(p.q) + row[i] * p.words + u[i]);
+    }
+    if (u[i] % GT == 0) {
+      const int g = u[i] / GT;
+      p.scale[row[i] * p.gstride + g] = sb;
+      if (ZERO) p.zero[row[i] * p.gstride + g] = (uint8_t)(int)z;
+      if (g == p.groups - 1)
+        for (int k = p.groups; k < p.gstride; ++k) {
+          p.scale[row[i] * p.gstride + k] = (bf16_t)0.f;
+          if (ZERO) p.zero[row[i] * p.gstride + k] = 0;
+        }
     }
   }
 }
@@ -108,40 +174,33 @@ struct ValueParams {
   const uint8_t* zero;
   void* out;
   long N;
-  int K, gshift, gstride, words;     // gshift: log2 of a group's words of eight codes
+  int K, gshift, gstride;            // gshift: log2 of a group's words of eight codes
+  Pieces pieces;                     // words
 };
 
 template <typename T>
 __global__ __launch_bounds__(256) void values_kernel(const ValueParams p) {
-  const int u = blockIdx.x * 64 + (threadIdx.x & 63), wave = threadIdx.x >> 6, left = p.K - u * 8;
-  if (left <= 0) return;
-  const int g = u >> p.gshift;
-  for (long row0 = ((long)blockIdx.y * 4 + wave) * QR; row0 < p.N; row0 += (long)gridDim.y * (4 * QR)) {
-    uint32_t word[QR];
-    bf16_t s[QR];
-    int z[QR];
+  long row[PT];
+  int u[PT], z[PT];
+  uint32_t word[PT];
+  bf16_t s[PT];
 #pragma unroll
-    for (int i = 0; i < QR; ++i) {
-      const long row = row0 + i < p.N ? row0 + i : p.N - 1;
-      word[i] = p.q[row * p.words + u];
-      s[i] = p.scale[row * p.gstride + g];
-      z[i] = p.zero ? p.zero[row * p.gstride + g] : 8;
-    }
+  for (int i = 0; i < PT; ++i) {
+    piece_of(p.pieces, i, row[i], u[i]);
+    const long r = row[i] < p.N ? row[i] : p.N - 1;
+    const int last = (p.K - 1) >> (3 + p.gshift), g = u[i] >> p.gshift;      // (words behind the last weight may lie behind the last group)
+    word[i] = p.q[r * p.pieces.per_row + u[i]];
+    s[i] = p.scale[r * p.gstride + (g < last ? g : last)];
+    z[i] = p.zero ? p.zero[r * p.gstride + (g < last ? g : last)] : 8;
+  }
 #pragma unroll
-    for (int i = 0; i < QR; ++i) {
-      if (row0 + i >= p.N) break;
-      T v[8];
+  for (int i = 0; i < PT; ++i) {
+    if (row[i] >= p.N) break;
+    const int left = p.K - u[i] * 8;
+    T v[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = (T)((float)s[i] * (float)((int)((word[i] >> (4 * e)) & 15u) - z[i]));
-      T* o = (T*)p.out + (row0 + i) * p.K + u * 8;
-      if (left >= 8) {
-        __builtin_memcpy(o, v, sizeof(v));
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (e < left) o[e] = v[e];
-      }
-    }
+    for (int e = 0; e < 8; ++e) v[e] = (T)((float)s[i] * (float)((int)((word[i] >> (4 * e)) & 15u) - z[i]));
+    store8_once<T>((T*)p.out + row[i] * p.K + u[i] * 8, left, v);
   }
 }
 
@@ -854,7 +913,6 @@ int launch_linear(const LinParams& p, int G, hipStream_t s) {
   return G == 32 ? launch_few<T, 32, false>(p, s) : G == 64 ? launch_few<T, 64, false>(p, s) : launch_few<T, 128, false>(p, s);
 }
 
-unsigned rows_grid(long N) { return (unsigned)((N + 4 * QR - 1) / (4 * QR) < 65535 ? (N + 4 * QR - 1) / (4 * QR) : 65535); }
 bool group_ok(int64_t g) { return g == 32 || g == 64 || g == 128; }
 
 }  // namespace
@@ -865,8 +923,10 @@ KH_EXPORT int kh_quantize_w4(const void* w, void* q, void* scale, void* zero, in
   if (!kh_aligned16(q) || !kh_aligned16(scale)) return KH_ERR_ALIGNMENT;
   if (K > (1L << 24) || N > (1L << 24)) return KH_ERR_TOO_LARGE;
   const long groups = (K + group - 1) / group, pieces = groups * (group / 8);
-  const dim3 grid((unsigned)((pieces + 63) / 64), rows_grid(N));
-  QuantParams p{w, (uint8_t*)q, (bf16_t*)scale, (uint8_t*)zero, (long)N, (int)K, (int)groups, (int)((groups + 3) / 4 * 4), (int)((K + 31) / 32 * 4)};
+  const long wg = (N * pieces + 4 * PT * 64 - 1) / (4 * PT * 64);
+  if (wg > 0x7fffffffL) return KH_ERR_TOO_LARGE;
+  const dim3 grid((unsigned)wg);
+  QuantParams p{w, (uint8_t*)q, (bf16_t*)scale, (uint8_t*)zero, (long)N, (int)K, (int)groups, (int)((groups + 3) / 4 * 4), (int)((K + 31) / 32 * 4), Pieces(pieces)};
   hipStream_t s = (hipStream_t)stream;
   auto go = [&](auto kernel) { kh_launch(KH_TAG_W4_QUANTIZE, kernel, grid, dim3(256), 0, s, p); };
 #define KH_BY_GROUP(T)                                                                            \
@@ -887,8 +947,10 @@ KH_EXPORT int kh_dequantize_w4(const void* q, const void* scale, const void* zer
   if (!kh_aligned16(q) || !kh_aligned16(scale)) return KH_ERR_ALIGNMENT;
   if (K > (1L << 24) || N > (1L << 24)) return KH_ERR_TOO_LARGE;
   const long groups = (K + group - 1) / group, words = (K + 31) / 32 * 4;
-  const dim3 grid((unsigned)((words + 63) / 64), rows_grid(N));
-  ValueParams p{(const uint32_t*)q, (const bf16_t*)scale, (const uint8_t*)zero, out, (long)N, (int)K, group == 32 ? 2 : group == 64 ? 3 : 4, (int)((groups + 3) / 4 * 4), (int)words};
+  const long wg = (N * words + 4 * PT * 64 - 1) / (4 * PT * 64);
+  if (wg > 0x7fffffffL) return KH_ERR_TOO_LARGE;
+  const dim3 grid((unsigned)wg);
+  ValueParams p{(const uint32_t*)q, (const bf16_t*)scale, (const uint8_t*)zero, out, (long)N, (int)K, group == 32 ? 2 : group == 64 ? 3 : 4, (int)((groups + 3) / 4 * 4), Pieces(words)};
   hipStream_t s = (hipStream_t)stream;
   auto go = [&](auto kernel) { kh_launch(KH_TAG_W4_VALUES, kernel, grid, dim3(256), 0, s, p); };
   type == 0 ? go(values_kernel<bf16_t>) : type == 1 ? go(values_kernel<_Float16>) : go(values_kernel<float>);

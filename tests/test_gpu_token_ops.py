@@ -94,6 +94,9 @@ NORM_CASES = [
     ((515, 1000), "layer", BF, BF, True, True, "full", "wb", 1.0),
     ((5, 1, 512), "rms", BF, FP32, False, False, "sequence", "", 0.0),
     ((64,), "rms", BF, BF, True, True, "channel", "w", 1.0),
+    ((4100, 1280), "layer", BF, FP32, True, True, "channel", "w", 1.0),     # a wave a row, stored past the caches
+    ((4097, 1999), "rms", FP16, FP16, True, True, "none", "wb", 1.0),
+    ((4096, 1400), "rms", BF, BF, True, False, "channel", "", 0.5),
 ]
 
 
