@@ -51,6 +51,15 @@ def normed(t, kind, w, b, eps):
     return n if b is None else n + b.to(F64)
 
 
+def normed_magnitude(t, mag, kind, w, b, eps):
+    """What the roundings of a norm of t are relative to, for an element: t's own terms `mag`, and for a layer norm those of the mean that is taken off
+    (t - mean is off by 2^-24 of both however small it is), times what the norm multiplies with; the result itself; the bias."""
+    c = t - t.mean(-1, keepdim=True) if kind == "layer" else t
+    up = (mag + mag.mean(-1, keepdim=True)) / torch.sqrt((c * c).mean(-1, keepdim=True) + eps)
+    up = up if w is None else up * w.to(F64).abs()
+    return up + normed(t, kind, w, b, eps).abs() + (0 if b is None else b.to(F64).abs())
+
+
 def norm_reference(y, h, post, pw, pb, gate, rho, pre, qw, qb, kind, eps):
     """(h', magnitude of its terms, u, magnitude of u's terms)."""
     h = h.to(F64)
@@ -58,8 +67,7 @@ def norm_reference(y, h, post, pw, pb, gate, rho, pre, qw, qb, kind, eps):
         s, mag = h, h.abs()
     else:
         y = y.to(F64)
-        n = normed(y, kind, pw, pb, eps) if post else y
-        a = n.abs() + (0 if pb is None or not post else 2 * pb.to(F64).abs())
+        n, a = (normed(y, kind, pw, pb, eps), normed_magnitude(y, y.abs(), kind, pw, pb, eps)) if post else (y, y.abs())
         if gate is not None:
             g = gate.to(F64)
             g = g[:, None] if gate.dim() == 2 and h.dim() == 3 and gate.shape != h.shape else g
@@ -67,12 +75,7 @@ def norm_reference(y, h, post, pw, pb, gate, rho, pre, qw, qb, kind, eps):
         s, mag = rho * h + n, (rho * h).abs() + a
     if not pre:
         return s, mag, None, None
-    u = normed(s, kind, qw, qb, eps)
-    # the row's terms as the norm sees them: their magnitude times what the norm multiplies with
-    c = s - s.mean(-1, keepdim=True) if kind == "layer" else s
-    up = (mag + mag.mean(-1, keepdim=True)) / torch.sqrt((c * c).mean(-1, keepdim=True) + eps)
-    up = up if qw is None else up * qw.to(F64).abs()
-    return s, mag, u, up + (0 if qb is None else qb.to(F64).abs()) + u.abs()
+    return s, mag, normed(s, kind, qw, qb, eps), normed_magnitude(s, mag, kind, qw, qb, eps)
 
 
 # roundings in 32 bits that an element passes: a sum over at most 32768 elements held by 64 .. 1024 threads (32 in a chain at most, 10 in
