@@ -377,6 +377,129 @@ class LoRALinear(nn.Module):
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}, geglu={self.geglu}"
 
 
+class LoRALinearW4(nn.Module):
+    """LoRALinear with its base weights in 4 bits (ops.W4Weight) and the adapters beside them in the activations' type: the same named adapters, active
+    list, per-adapter weights and global scale (no counterpart in the reference, whose text encoders run once a prompt).  For layers that a few rows at a
+    time pass through, whose bytes are the time; any number of rows is right.
+
+    The buffers weight_q / weight_scale / weight_zero are what is saved; fuse() merges adapters into them in place, so a captured graph that reads them
+    stays valid."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, group: int = 64, zeros: bool = False, device=None,
+                 dtype=torch.bfloat16):
+        super().__init__()
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError(f"activations are bf16 or fp16, not {dtype}")
+        self.in_features, self.out_features, self.group, self.dtype = in_features, out_features, group, dtype
+        marks = -(-(-(-in_features // group)) // 4) * 4
+        self.register_buffer("weight_q", torch.zeros((out_features, -(-in_features // 32) * 16), dtype=torch.uint8, device=device))
+        self.register_buffer("weight_scale", torch.zeros((out_features, marks), dtype=torch.bfloat16, device=device))
+        self.register_buffer("weight_zero", torch.zeros((out_features, marks), dtype=torch.uint8, device=device) if zeros else None)
+        self.bias = nn.Parameter(torch.zeros(out_features, device=device, dtype=dtype), requires_grad=False) if bias else None
+        self.adapters: Dict[str, Adapter] = {}
+        self.active: List[str] = []
+        self.global_scale = 1.0
+        self.adapters_enabled = True
+        self._packed: Optional[PackedAdapters] = None
+        self._packed_key = None
+        self._fused: set = set()
+        self.packed_weight()
+
+    @classmethod
+    def from_linear(cls, layer: nn.Module, group: int = 64, zeros: bool = False) -> "LoRALinearW4":
+        """A linear's weights (nn.Linear's or LoRALinear's, on the GPU) quantised; a LoRALinear's adapters come along."""
+        if getattr(layer, "geglu", False):
+            raise ValueError("a GEGLU projection is not kept in 4 bits: its activation is part of the dense kernel")
+        w = layer.weight.detach()
+        new = cls(w.shape[1], w.shape[0], layer.bias is not None, group, zeros, w.device, w.dtype)
+        new._assign(ops.quantize_w4(w.contiguous(), group, zeros))
+        if layer.bias is not None:
+            new.bias.data.copy_(layer.bias.detach())
+        if isinstance(layer, LoRALinear):
+            new.adapters, new.global_scale, new.adapters_enabled = dict(layer.adapters), layer.global_scale, layer.adapters_enabled
+            new._fused = set(layer._fused)
+            new.set_active(layer.active)
+        return new
+
+    def packed_weight(self) -> "ops.W4Weight":
+        return ops.W4Weight(self.weight_q, self.weight_scale, self.weight_zero, self.in_features, self.group)
+
+    def _assign(self, w: "ops.W4Weight") -> None:
+        self.weight_q.copy_(w.q)
+        self.weight_scale.copy_(w.scale)
+        if w.zero is not None:
+            self.weight_zero.copy_(w.zero)
+
+    # ---- adapter state (host), as LoRALinear's ---------------------------------------------------
+    def add_adapter(self, name: str, down: torch.Tensor, up: torch.Tensor, alpha: Optional[float] = None, weight: float = 1.0) -> None:
+        if down.shape[1] != self.in_features or up.shape[0] != self.out_features or down.shape[0] != up.shape[1]:
+            raise ValueError(f"adapter {name!r} does not fit a [{self.out_features},{self.in_features}] layer: "
+                             f"down {tuple(down.shape)}, up {tuple(up.shape)}")
+        self.adapters[name] = Adapter(down.detach(), up.detach(), alpha, weight)
+        self._packed_key = None
+
+    def delete_adapter(self, name: str) -> None:
+        self.adapters.pop(name, None)
+        self.active = [n for n in self.active if n != name]
+        self.refresh_adapters()
+
+    def set_active(self, names: Sequence[str], weights: Optional[Sequence[float]] = None) -> None:
+        self.active = [n for n in names if n in self.adapters]
+        for n, w in zip(names, weights or ()):
+            if n in self.adapters:
+                self.adapters[n].weight = float(w)
+        self.refresh_adapters()
+
+    def set_global_scale(self, scale: float) -> None:
+        if scale != self.global_scale:
+            self.global_scale = float(scale)
+            self.refresh_adapters()
+
+    def refresh_adapters(self) -> None:
+        """(Re)build the packed buffers; a change of scales alone is written into them."""
+        names = [n for n in self.active if n not in self._fused] if self.adapters_enabled else []
+        key = (self.weight_q.device,) + tuple((n, id(self.adapters[n].down)) for n in names)
+        if names and key == self._packed_key and self._packed is not None:
+            rescale_(self._packed, self.adapters, self.global_scale)
+            return
+        self._packed = pack_adapters(self.adapters, names, self.in_features, self.out_features, self.dtype, self.weight_q.device, self.global_scale)
+        self._packed_key = key
+
+    def fuse(self, lora_scale: float = 1.0, names: Optional[Sequence[str]] = None) -> None:
+        """The adapters merged into the weights, which are quantised anew (there is no way back: what was rounded off is gone).  Not finite: left as it was."""
+        names = [n for n in (self.active if names is None else names) if n in self.adapters and n not in self._fused]
+        if not names:
+            return
+        w = ops.dequantize_w4(self.packed_weight(), torch.float32)
+        for n in dict.fromkeys(names):
+            ad = self.adapters[n]
+            w += lora_scale * ad.multiplier(1.0) * (ad.up.to(w.device).float() @ ad.down.to(w.device).float())
+        if not torch.isfinite(w).all():
+            raise ValueError("fusing produced non-finite weights; LoRA left unfused")
+        self._assign(ops.quantize_w4(w, self.group, self.weight_zero is not None))
+        self._fused.update(names)
+        self.refresh_adapters()
+
+    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+        p = self._packed
+        w, b = self.packed_weight(), None if self.bias is None else self.bias.detach()
+        if p is None:
+            return ops.w4_linear(x, w, b, residual=residual)
+        if p.a_cat.device != x.device:      # the layer was moved
+            self._packed_key = None
+            self.refresh_adapters()
+            p = self._packed
+        y = ops.w4_linear(x, w, b, p.a_cat, p.b_cat, p.col_scale, residual=residual)
+        for c in p.overflow:                # more rank columns than one launch takes, as LoRALinear does it
+            t = ops.lora_linear(x, c.a_cat, None)
+            t.mul_(c.col_scale.to(t.dtype))
+            y = ops.lora_linear(t, c.b_cat, None, residual=y)
+        return y
+
+    def extra_repr(self) -> str:
+        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}, group={self.group}, zeros={self.weight_zero is not None}"
+
+
 def refresh_many(modules) -> None:
     """refresh_adapters of many modules.  Linear layers on the GPU whose packs have to be built get them from two launches over
     all of them, those whose scales alone have changed from one; everything else refreshes by itself.  So does every module
