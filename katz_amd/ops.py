@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import math
 import os
 import threading
@@ -1318,6 +1319,12 @@ def _here(first: torch.Tensor, *others) -> None:
                             + ", ".join(str(t.device) for t in (first, *others) if t is not None) + "); katz_hip has no CPU path")
 
 
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(name: str, *sizes: int) -> int:
+    """What the library's function of that name says (a pure function of the sizes)."""
+    return int(getattr(_lib.load(), name)(*sizes))
+
+
 def _fits(t: torch.Tensor, dtype, shape, name: str) -> None:
     if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
@@ -1436,7 +1443,10 @@ def quantize_w4(weight: torch.Tensor, group: int = 64, zeros: bool = False) -> W
     rc = lib.kh_quantize_w4(weight.data_ptr(), q.data_ptr(), scale.data_ptr(), _ptr(zero), N, K, group, _TYPES[weight.dtype], _stream())
     if rc:
         _lib.check(rc, "kh_quantize_w4")
-    return W4Weight(q, scale, zero, K, group)
+    new = W4Weight.__new__(W4Weight)           # (its parts are what the checks would ask for)
+    new.q, new.scale, new.zero = q, scale, zero
+    new.in_features, new.out_features, new.group, new.groups = K, N, group, -(-K // group)
+    return new
 
 
 def dequantize_w4(w: W4Weight, dtype: torch.dtype = BF16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -1496,7 +1506,7 @@ def w4_linear(x: torch.Tensor, w: W4Weight, bias: Optional[torch.Tensor] = None,
         return out
     ws = None
     if R:
-        nbytes = lib.kh_w4_linear_workspace_bytes(M, K, R)
+        nbytes = _workspace_bytes("kh_w4_linear_workspace_bytes", M, K, R)
         if nbytes < 0:
             raise ValueError(f"the adapters' columns must be a multiple of 32 up to 128, got {R}")
         ws = x.new_empty(nbytes // 2)          # (elements of two bytes)
@@ -1610,9 +1620,9 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: i
     if not packed and T == 1 and state is not None and all(st >= t.shape[-1] for st, t in zip(bs, (q, k, v, out))):   # one pass over the state
         _la_step(lib, q, k, v, out, log_decay, state, state_out, slots, n_slots, B, heads, kv, dk, dv, bs, scale)
         return out, state_out
-    nbytes = lib.kh_linear_attention_workspace_bytes(B, heads, T, rows, dk, dv)
+    nbytes = _workspace_bytes("kh_linear_attention_workspace_bytes", B, heads, T, rows, dk, dv)
     if nbytes < 0:
-        _lib.check(int(nbytes), "kh_linear_attention_workspace_bytes")
+        _lib.check(nbytes, "kh_linear_attention_workspace_bytes")
     ws = q.new_empty(nbytes // 2) if nbytes else None      # (elements of two bytes)
     rc = lib.kh_linear_attention_bf16(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), log_decay.data_ptr(), _ptr(state), state_out.data_ptr(),
                                       _ptr(slots), n_slots, _ptr(seg_start), rows if packed else 0, _ptr(ws), B, heads, kv, T, dk, dv, *ld, *bs, scale,
