@@ -353,20 +353,23 @@ __global__ __launch_bounds__(LW * 64) void w4_few_rows(const LinParams p) {
   const uint8_t* z0 = ZERO ? p.zero + n0 * p.gstride : nullptr;
   const T* x0 = (const T*)p.x + m0 * p.K;
   const uint32_t last = (uint32_t)(p.N - 1 - n0 < NB * 16 - 1 ? p.N - 1 - n0 : NB * 16 - 1);
+  // Loads to LDS: four lanes in a row take the 64 bytes of a row (a lane to every row instead costs three and a half times as much: 54 and 15 bytes a clock and CU
+  // out of the L2); the reads put them in order.
+  const int dr = lane >> 2, dp = lane & 3, from = (l * 4 + g) * 16;
   uint32_t qo[NB];
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
-    const uint32_t r = j * 16 + l;
-    qo[j] = (r < last ? r : last) * (uint32_t)p.row_bytes + g * 16;
+    const uint32_t r = j * 16 + dr;
+    qo[j] = (r < last ? r : last) * (uint32_t)p.row_bytes + dp * 16;
   }
   const uint32_t mr = (g < NB ? g : NB - 1) * 16 + l, so = (mr < last ? mr : last) * (uint32_t)p.gstride;    // row whose scales the lane fetches
   int xm[MB];
   uint32_t xo[MB];
 #pragma unroll
   for (int b = 0; b < MB; ++b) {
-    const int r = FOUR ? l >> 2 : b * 16 + l;
+    const int r = FOUR ? l >> 2 : b * 16 + l, rd = b * 16 + dr;
     xm[b] = r < rows ? r : rows - 1;
-    xo[b] = (uint32_t)xm[b] * (uint32_t)p.K + g * 8;
+    xo[b] = ((uint32_t)(rd < rows ? rd : rows - 1) * (uint32_t)p.K + dp * 8) * 2;
   }
   const uint32_t x4 = ((uint32_t)(g < rows ? g : rows - 1) * (uint32_t)p.K + l * 8) * 2;   // FOUR: row g, piece l
   const Unpack<T> unpack;
@@ -443,7 +446,7 @@ __global__ __launch_bounds__(LW * 64) void w4_few_rows(const LinParams p) {
 #pragma unroll
       for (int b = 0; b < MB; ++b)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lptr_t)(to + Sg::XAT + (b * 4 + j) * 1024), 16, xo[b] * 2, kb * 256 + j * 64, 0, 0);
+        for (int j = 0; j < 4; ++j) __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lptr_t)(to + Sg::XAT + (b * 4 + j) * 1024), 16, xo[b], kb * 256 + j * 64, 0, 0);
     }
 #pragma unroll
     for (int j = 0; j < Sg::S; ++j) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lptr_t)(to + Sg::SAT + j * 256), 4, so * 2, s_word(kb) + j * 4, 0, 0);
@@ -457,7 +460,7 @@ __global__ __launch_bounds__(LW * 64) void w4_few_rows(const LinParams p) {
     ZW_t zw[NB];
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
-      w[j] = *reinterpret_cast<const u32x4*>(at + Sg::WAT + j * 1024 + lane * 16);
+      w[j] = *reinterpret_cast<const u32x4*>(at + Sg::WAT + j * 1024 + from);
       const char* sa = at + Sg::SAT + (j * 16 + l) * 4;
       if constexpr (G == 32) sw[j] = (SW_t)*reinterpret_cast<const uint32_t*>(sa) | (SW_t)((uint64_t)*reinterpret_cast<const uint32_t*>(sa + 256) << 32);
       else sw[j] = (SW_t)(*reinterpret_cast<const uint32_t*>(sa) >> (kb * GB * 16 & 31));
@@ -467,7 +470,7 @@ __global__ __launch_bounds__(LW * 64) void w4_few_rows(const LinParams p) {
     for (int b = 0; b < MB; ++b)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        x[b][j] = *reinterpret_cast<const u32x4*>(at + Sg::XAT + (FOUR ? (l >> 2) * 256 + (j * 4 + g) * 16 : (b * 4 + j) * 1024 + lane * 16));
+        x[b][j] = *reinterpret_cast<const u32x4*>(at + Sg::XAT + (FOUR ? (l >> 2) * 256 + (j * 4 + g) * 16 : (b * 4 + j) * 1024 + from));
     multiply(w, x, sw, zw, GB);
   };
   {
@@ -506,9 +509,9 @@ __global__ __launch_bounds__(LW * 64) void w4_few_rows(const LinParams p) {
     ZW_t zw[NB];
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
-      const uint32_t r = j * 16 + l, rc = (r < last ? r : last) * (uint32_t)p.gstride;
+      const uint32_t r = j * 16 + l < (int)last ? j * 16 + l : last, rc = r * (uint32_t)p.gstride;
       w[j] = u32x4{0, 0, 0, 0};
-      if (kb * 64 + g * 16 < p.row_bytes) w[j] = *reinterpret_cast<const u32x4*>(q0 + (long)kb * 64 + qo[j]);
+      if (kb * 64 + g * 16 < p.row_bytes) w[j] = *reinterpret_cast<const u32x4*>(q0 + (long)kb * 64 + r * (uint32_t)p.row_bytes + g * 16);
       sw[j] = *reinterpret_cast<const SW_t*>(s0 + kb * GB + rc);           // (rows of scales and zero points are filled up to whole blocks)
       if (ZERO) zw[j] = *reinterpret_cast<const ZW_t*>(z0 + kb * GB + rc);
     }
@@ -517,7 +520,7 @@ __global__ __launch_bounds__(LW * 64) void w4_few_rows(const LinParams p) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         T v[8];
-        load8<T>(x0 + kb * 128 + (xo[b] + j * 32), (long)p.K - (kb * 128 + j * 32 + g * 8), v);
+        load8<T>(x0 + (long)xm[b] * p.K + (kb * 128 + j * 32 + g * 8), (long)p.K - (kb * 128 + j * 32 + g * 8), v);
         x[b][j] = __builtin_bit_cast(u32x4, v);
       }
     const int left = (p.K - kb * 128 + G - 1) / G;
@@ -587,16 +590,17 @@ __global__ __launch_bounds__(MR_W * 64) __attribute__((amdgpu_waves_per_eu(2, 2)
   const T* x0 = (const T*)p.x + m0 * p.K;
   const uint32_t last = (uint32_t)(p.N - 1 - nb < MR_N * 16 - 1 ? p.N - 1 - nb : MR_N * 16 - 1);
   constexpr int XL = (MR_M * 4 + MR_W - 1) / MR_W;                             // loads of x of a wave, at most
+  const int dr = lane >> 2, dp = lane & 3, from = (l * 4 + g) * 16;            // (as for few rows)
   uint32_t qo[MR_N], xo[XL];
 #pragma unroll
   for (int j = 0; j < MR_N; ++j) {
-    const uint32_t r = j * 16 + l;
-    qo[j] = (r < last ? r : last) * (uint32_t)p.row_bytes + g * 16;
+    const uint32_t r = j * 16 + dr;
+    qo[j] = (r < last ? r : last) * (uint32_t)p.row_bytes + dp * 16;
   }
 #pragma unroll
   for (int i = 0; i < XL; ++i) {              // load wave + 8 i: step j of the operands of a tile of 16 rows
-    const int id = wave + i * MR_W, r = (id >> 2) * 16 + l;
-    xo[i] = (uint32_t)(r < rows ? r : rows - 1) * (uint32_t)p.K + (id & 3) * 32 + g * 8;
+    const int id = wave + i * MR_W, r = (id >> 2) * 16 + dr;
+    xo[i] = (uint32_t)(r < rows ? r : rows - 1) * (uint32_t)p.K + (id & 3) * 32 + dp * 8;
   }
   const uint32_t so = ((uint32_t)lane < last ? (uint32_t)lane : last) * (uint32_t)p.gstride;
   auto bytes = [](long n) { return (int)(uint32_t)(n < 0xffffffffL ? n : 0xffffffffL); };
@@ -618,7 +622,7 @@ __global__ __launch_bounds__(MR_W * 64) __attribute__((amdgpu_waves_per_eu(2, 2)
         const int r = (id >> 2) * 16 + l, k = kb * 128 + (id & 3) * 32 + g * 8;
         T v[8];
         load8<T>(x0 + (long)(r < rows ? r : rows - 1) * p.K + k, (long)p.K - k, v);
-        *reinterpret_cast<u32x4*>(to + Sg::XAT + id * 1024 + lane * 16) = __builtin_bit_cast(u32x4, v);
+        *reinterpret_cast<u32x4*>(to + Sg::XAT + id * 1024 + from) = __builtin_bit_cast(u32x4, v);
       }
     }
 #pragma unroll
@@ -630,7 +634,7 @@ __global__ __launch_bounds__(MR_W * 64) __attribute__((amdgpu_waves_per_eu(2, 2)
   };
   const f32x4 none = f32x4{0.f, 0.f, 0.f, 0.f};
   constexpr uint32_t over = (Num<T>::P | Num<T>::NEG) | (ZERO ? 0x00100010u : 0x00080008u);    // -(P + 16), -(P + 8)
-  auto x_at = [&](int st, int b, int j) { return *reinterpret_cast<const u32x4*>(smem + st * Sg::BYTES + Sg::XAT + (b * 4 + j) * 1024 + lane * 16); };
+  auto x_at = [&](int st, int b, int j) { return *reinterpret_cast<const u32x4*>(smem + st * Sg::BYTES + Sg::XAT + (b * 4 + j) * 1024 + from); };
   auto sums = [&](int st, int odd) {          // a constant's products with the groups of 16 rows
     if (wave >= MR_M) return;
 #pragma unroll
@@ -657,49 +661,62 @@ __global__ __launch_bounds__(MR_W * 64) __attribute__((amdgpu_waves_per_eu(2, 2)
     uint32_t zw[MR_N];
 #pragma unroll
     for (int j = 0; j < MR_N; ++j) {
-      w[j] = across_groups(*reinterpret_cast<const u32x4*>(at + Sg::WAT + (wave * MR_N + j) * 1024 + lane * 16));
+      w[j] = across_groups(*reinterpret_cast<const u32x4*>(at + Sg::WAT + (wave * MR_N + j) * 1024 + from));
       const char* sa = at + Sg::SAT + wave * Sg::S * 256 + (j * 16 + l) * 4;
       sw[j] = *reinterpret_cast<const uint32_t*>(sa);
       if constexpr (G == 32) sw[j] |= (uint64_t)*reinterpret_cast<const uint32_t*>(sa + 256) << 32;
       else sw[j] >>= (kb * GB * 16 & 31);
       if constexpr (ZERO) zw[j] = *reinterpret_cast<const uint32_t*>(at + Sg::ZAT + wave * 256 + (j * 16 + l) * 4) >> (kb * GB * 8 & 31);
     }
-#pragma unroll
-    for (int i = 0; i < GB; ++i) {
-      float s[MR_N];
-      uint32_t z[MR_N];
-#pragma unroll
-      for (int j = 0; j < MR_N; ++j) {
-        s[j] = kb * GB + i < groups ? bf16_bits_to_f32((uint32_t)(sw[j] >> (16 * i)) & 0xffffu) : 0.f;    // what rows of scales are filled up with is not used
-        if constexpr (ZERO) z[j] = ((zw[j] >> (8 * i)) & 15u) * 0x01010101u;
-      }
-      u32x4 xv[SG][MR_M];
-      f32x4 base[MR_M];
+    // Operands of the next k-step (and, where a group ends, what its sums start from) are on their way from LDS while one is multiplied: all eight waves read at
+    // once after the barrier, and the matrix unit would wait for every step's reads otherwise.
+    u32x4 xv[2][MR_M];
+    f32x4 base[2][MR_M];
+    auto step_in = [&](int t) {
 #pragma unroll
       for (int b = 0; b < MR_M; ++b) {
-        base[b] = *reinterpret_cast<const f32x4*>(smem + Sg::SUMS + ((odd * GB + i) * MR_M * 16 + b * 16 + g * 4) * 4);
-#pragma unroll
-        for (int k = 0; k < SG; ++k) xv[k][b] = x_at(st, b, i * SG + k);
+        xv[t & 1][b] = x_at(st, b, t);
+        if (t % SG == 0) base[t / SG & 1][b] = *reinterpret_cast<const f32x4*>(smem + Sg::SUMS + ((odd * GB + t / SG) * MR_M * 16 + b * 16 + g * 4) * 4);
       }
-      // A tile of columns at a time: the scaled sum of one and the operands of the next run beside the products
+    };
+    auto hold = [&](int t) {                  // (the compiler otherwise moves the reads down to their uses)
+      asm volatile("" ::: "memory");
 #pragma unroll
-      for (int j = 0; j < MR_N; ++j) {
-        f32x4 acc[MR_M];
+      for (int b = 0; b < MR_M; ++b) asm volatile("" : "+v"(xv[t & 1][b]));
+    };
+    step_in(0);
+    f32x4 acc[MR_M][MR_N];
+    float s[MR_N];
+    uint32_t z[MR_N];
 #pragma unroll
-        for (int k = 0; k < SG; ++k) {        // bytes of even and of odd codes, put beside one another: the order of x
-          const uint32_t word = w[j][i * SG + k];
-          const uint32_t even = ZERO ? ((word & low) | sixteen) - z[j] : word & low;
-          const uint32_t uneven = ZERO ? (((word >> 4) & low) | sixteen) - z[j] : (word >> 4) & low;
-          const u32x4 wv = u32x4{__builtin_amdgcn_perm(uneven, even, 0x0c040c00u) | power, __builtin_amdgcn_perm(uneven, even, 0x0c050c01u) | power,
-                                 __builtin_amdgcn_perm(uneven, even, 0x0c060c02u) | power, __builtin_amdgcn_perm(uneven, even, 0x0c070c03u) | power};
+    for (int t = 0; t < 4; ++t) {
+      const int i = t / SG;
+      if (t < 3) step_in(t + 1);
+      hold(t);
+      if (t % SG == 0) {
 #pragma unroll
-          for (int b = 0; b < MR_M; ++b) acc[b] = Num<T>::mfma(xv[k][b], wv, k == 0 ? base[b] : acc[b]);
+        for (int j = 0; j < MR_N; ++j) {
+          s[j] = kb * GB + i < groups ? bf16_bits_to_f32((uint32_t)(sw[j] >> (16 * i)) & 0xffffu) : 0.f;    // what rows of scales are filled up with is not used
+          if constexpr (ZERO) z[j] = ((zw[j] >> (8 * i)) & 15u) * 0x01010101u;
         }
-#pragma unroll
-        for (int b = 0; b < MR_M; ++b)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) out[b][j][e] = fmaf(s[j], acc[b][e], out[b][j][e]);
       }
+#pragma unroll
+      for (int j = 0; j < MR_N; ++j) {        // bytes of even and of odd codes, put beside one another: the order of x
+        const uint32_t word = w[j][t];
+        const uint32_t even = ZERO ? ((word & low) | sixteen) - z[j] : word & low;
+        const uint32_t uneven = ZERO ? (((word >> 4) & low) | sixteen) - z[j] : (word >> 4) & low;
+        const u32x4 wv = u32x4{__builtin_amdgcn_perm(uneven, even, 0x0c040c00u) | power, __builtin_amdgcn_perm(uneven, even, 0x0c050c01u) | power,
+                               __builtin_amdgcn_perm(uneven, even, 0x0c060c02u) | power, __builtin_amdgcn_perm(uneven, even, 0x0c070c03u) | power};
+#pragma unroll
+        for (int b = 0; b < MR_M; ++b) acc[b][j] = Num<T>::mfma(xv[t & 1][b], wv, t % SG == 0 ? base[i & 1][b] : acc[b][j]);
+      }
+      if (t % SG == SG - 1)
+#pragma unroll
+        for (int j = 0; j < MR_N; ++j)
+#pragma unroll
+          for (int b = 0; b < MR_M; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) out[b][j][e] = fmaf(s[j], acc[b][j][e], out[b][j][e]);
     }
   };
   auto barrier = []() {                       // what this wave has written to LDS is there, and everybody has arrived
