@@ -732,31 +732,46 @@ __global__ __launch_bounds__(MR_W * 64) __attribute__((amdgpu_waves_per_eu(2, 2)
   if (blocks > 1) fetch(turned(1), 1);
   // the adapters while the first blocks are on their way: t lies in two pieces of bf16, B_cat is exact in one (fp16: in two)
   const bf16_t* th = (const bf16_t*)p.t;
-  for (int r = 0; r < p.R; r += 32) {
-    bf16x8 bh[MR_N], bl[MR_N];
+  struct Ranks { u32x4 b[MR_N], hi[MR_M], lo[MR_M]; } ra, rb;
+  auto ranks_in = [&](int r, Ranks& o) {
 #pragma unroll
-    for (int j = 0; j < MR_N; ++j) {
-      T v[8];
-      const long n = nb + (j * 16 + l < (int)last ? j * 16 + l : (int)last);
-      __builtin_memcpy(v, (const T*)p.b_cat + n * p.R + r + g * 8, sizeof(v));
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        bh[j][e] = (bf16_t)(float)v[e];
-        bl[j][e] = (bf16_t)((float)v[e] - (float)bh[j][e]);
-      }
-    }
+    for (int j = 0; j < MR_N; ++j)
+      __builtin_memcpy(&o.b[j], (const T*)p.b_cat + (nb + (j * 16 + l < (int)last ? j * 16 + l : (int)last)) * p.R + r + g * 8, 16);
 #pragma unroll
     for (int b = 0; b < MR_M; ++b) {
       const int r0 = b * 16 + l;
       const bf16_t* at = th + (m0 + (r0 < rows ? r0 : rows - 1)) * p.R + r + g * 8;
-      const bf16x8 hi = *reinterpret_cast<const bf16x8*>(at), lo = *reinterpret_cast<const bf16x8*>(at + p.M * p.R);
+      o.hi[b] = *reinterpret_cast<const u32x4*>(at);
+      o.lo[b] = *reinterpret_cast<const u32x4*>(at + p.M * p.R);
+    }
+  };
+  auto ranks = [&](const Ranks& o) {
 #pragma unroll
-      for (int j = 0; j < MR_N; ++j) {
-        out[b][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, bh[j], out[b][j], 0, 0, 0);
-        out[b][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, bh[j], out[b][j], 0, 0, 0);
-        if constexpr (sizeof(T) == 2 && !__is_same(T, bf16_t)) out[b][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, bl[j], out[b][j], 0, 0, 0);
+    for (int j = 0; j < MR_N; ++j) {
+      bf16x8 bh, bl;
+      T v[8];
+      __builtin_memcpy(v, &o.b[j], 16);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        bh[e] = (bf16_t)(float)v[e];
+        bl[e] = (bf16_t)((float)v[e] - (float)bh[e]);
+      }
+#pragma unroll
+      for (int b = 0; b < MR_M; ++b) {
+        out[b][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, o.hi[b]), bh, out[b][j], 0, 0, 0);
+        out[b][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, o.lo[b]), bh, out[b][j], 0, 0, 0);
+        if constexpr (!__is_same(T, bf16_t)) out[b][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, o.hi[b]), bl, out[b][j], 0, 0, 0);
       }
     }
+  };
+  if (p.R > 0) ranks_in(0, ra);
+  for (int r = 0; r < p.R; r += 64) {
+    if (r + 32 < p.R) ranks_in(r + 32, rb);
+    asm volatile("" ::: "memory");
+    ranks(ra);
+    if (r + 64 < p.R) ranks_in(r + 64, ra);
+    asm volatile("" ::: "memory");
+    if (r + 32 < p.R) ranks(rb);
   }
   wait_vm<0>();
   barrier();
@@ -838,7 +853,18 @@ __global__ __launch_bounds__(SW * 64) void w4_shrink(const ShrinkParams p) {
   const T* xr = (const T*)p.x + (m0 + l < p.M ? m0 + l : p.M - 1) * p.K;
   const int k0 = blockIdx.z * p.per, k1 = k0 + p.per < p.K ? k0 + p.per : p.K;
   f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int k = k0 + wave * 32; k < k1; k += SW * 32) {
+  int k = k0 + wave * 32;
+  for (; k + 3 * SW * 32 + 32 <= k1; k += 4 * SW * 32) {      // four steps' loads on their way at once
+    u32x4 a[4], x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      __builtin_memcpy(&a[i], ar + k + i * (SW * 32) + g * 8, 16);
+      __builtin_memcpy(&x[i], xr + k + i * (SW * 32) + g * 8, 16);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc = Num<T>::mfma(x[i], a[i], acc);
+  }
+  for (; k < k1; k += SW * 32) {
     T a[8], x[8];
     load8<T>(ar + k + g * 8, (long)k1 - k - g * 8, a);
     load8<T>(xr + k + g * 8, (long)k1 - k - g * 8, x);
