@@ -941,9 +941,16 @@ int launch_many(const LinParams& p, hipStream_t s) {
   kh_launch(KH_TAG_W4_LINEAR, w4_many_rows<T, G, ZERO>, dim3((unsigned)units), dim3(MR_W * 64), ManyStage<G, ZERO>::LDS, s, p);
   return KH_OK;
 }
+// Which of the two kernels has the smaller time by what was measured over N 320 .. 16384, K 1280 .. 8192, 33 .. 2464 rows (us; a block is 128 codes): the one for many
+// rows 2.25 a block and round of its workgroups on 256 CUs, whatever the rows, the one for few 0.29 ns a block of 32 x 16 and 3.4 ns beside.  few | many:
+// 1280 x 1280 by 154 rows 5.7 | 28, by 616 14.1 | 28, by 2464 45 | 31; 10240 x 1280 by 154 24.4 | 28.5, by 308 41 | 29.7, by 616 74 | 32.7; 16384 x 8192 by 154
+// 109 | 158, by 400 267 | 166.
 bool many_rows(long M, long N, long K) {
-  const long units = (M + MR_M * 16 - 1) / (MR_M * 16) * ((N + MR_W * MR_N * 16 - 1) / (MR_W * MR_N * 16));
-  return M > 64 && units >= 64;
+  if (M <= 32) return false;
+  const long units = (M + MR_M * 16 - 1) / (MR_M * 16) * ((N + MR_W * MR_N * 16 - 1) / (MR_W * MR_N * 16)), blocks = (K + 127) / 128;
+  const double many = 6. + (double)((units + 255) / 256) * blocks * 2.25;
+  const double few = 4. + (double)((M + 31) / 32) * ((N + 15) / 16) * (blocks * 0.29 + 3.4) * 1e-3;
+  return many < few;
 }
 
 template <typename T>

@@ -303,6 +303,8 @@ LINEAR_CASES = [
     (200, 8209, 130, 128, False, 64, False, True, BF),
     (70, 16500, 64, 64, True, 0, True, False, FP16),
     (513, 3330, 1000, 32, False, 64, True, True, BF),
+    (700, 4100, 1000, 32, False, 64, True, True, BF),
+    (800, 5000, 1280, 128, True, 128, False, False, BF),
     (200, 1000, 96, 32, False, 0, False, True, BF),
 ]
 
@@ -354,6 +356,22 @@ def test_w4_linear_reads_only_its_rows():
         ops.w4_linear(xs[K + 1:K + 1 + M * K].view(M, K), w, out=ys[N + 1:N + 1 + M * N].view(M, N))
         assert torch.equal(ys[N + 1:N + 1 + M * N].view(M, N), want)
         assert (ys[:N + 1] == 7).all() and (ys[N + 1 + M * N:] == 7).all()
+
+
+def test_w4_linear_does_not_use_what_rows_are_filled_up_with():
+    """Behind the last code, scale and zero point of a row there may be anything."""
+    from katz_amd import ops
+
+    for M, N, K, group in ((2, 40, 300, 64), (20, 33, 650, 32), (700, 4100, 200, 128)):
+        g = gen(K)
+        w = ops.quantize_w4(on(randn(g, N, K, std=0.1)), group, zeros=True)
+        x = on(randn(g, M, K))
+        want, values_ = ops.w4_linear(x, w), ops.dequantize_w4(w)
+        q, s, z = w.q.clone(), w.scale.clone(), w.zero.clone()
+        q.view(N, -1)[:, (K + 1) // 2:] = 0xFF
+        s[:, w.groups:], z[:, w.groups:] = float("nan"), 255
+        other = ops.W4Weight(q, s, z, K, group)
+        assert torch.equal(ops.w4_linear(x, other), want) and torch.equal(ops.dequantize_w4(other), values_)
 
 
 def test_w4_linear_of_rows_that_are_no_numbers():
@@ -527,6 +545,22 @@ def test_linear_attention_tables_outside_the_tensors_stay_inside():
     lone = torch.tensor([20, 100], dtype=torch.int32, device=DEV)
     ol, last = ops.linear_attention(q, k, v, H, g, seg_start=lone, max_seg_rows=80)
     assert torch.equal(S[2], last[0]) and torch.equal(o[30:], ol[30:])
+
+
+def test_linear_attention_does_not_read_rows_of_no_sequence():
+    from katz_amd import ops
+
+    r = gen(13)
+    H, d, start = 2, 64, [3, 40, 40, 170]
+    q, k, v = (on(randn(r, 180, H * d)) for _ in range(3))
+    g = on(torch.tensor([-0.1, 0.0]))
+    table = torch.tensor(start, dtype=torch.int32, device=DEV)
+    o, S = ops.linear_attention(q, k, v, H, g, seg_start=table, max_seg_rows=130)
+    assert not o[:3].any() and not o[170:].any()                       # a new output's rows of no sequence are zero
+    for t in (q, k, v):
+        t[:3] = t[170:] = float("nan")
+    o2, S2 = ops.linear_attention(q, k, v, H, g, seg_start=table, max_seg_rows=130)
+    assert torch.equal(o, o2) and torch.equal(S, S2) and torch.isfinite(S).all()
 
 
 def test_empty_calls():
