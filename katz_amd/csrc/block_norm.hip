@@ -195,7 +195,7 @@ KH_EXPORT int kh_block_norm(const void* y, const void* h, const void* gate, int6
   if (gate && (gate_rows <= 0 || gate_rows > M || M % gate_rows != 0)) return KH_ERR_INVALID_ARG;
   if (stream_type != type && stream_type != 2) return KH_ERR_UNSUPPORTED;
   if (D > 32768) return KH_ERR_TOO_LARGE;
-  if (M > 0x7fffffffL) return KH_ERR_TOO_LARGE;
+  if (M > 0x7fffffffL || M * (D <= 1024 || (D <= 2048 && M >= 4096) ? 64 : D <= 8192 ? 256 : 1024) > 0xffff0000L) return KH_ERR_TOO_LARGE;   // (threads of a launch)
   NormParams p{y, h, gate, post_w, post_b, pre_w, pre_b, h_out, u, (long)M, (long)(gate ? gate_rows : 1), (int)D, residual_scale, eps, flags & 1, post, 0};
   auto size = [](int t) { return t == 2 ? 4 : 2; };
   p.once = M * D * ((h_out ? size(stream_type) : 0) + (u ? size(type) : 0)) >= 8 << 20;

@@ -171,6 +171,15 @@ struct State {
   f32x4 s[DK / 16];
 };
 
+__device__ __forceinline__ bool not_finite(const bf16x8 (&v)[2]) {
+  uint32_t any = 0;                        // an exponent of ones carries into the sign's place
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) any |= (__builtin_bit_cast(u32x4, v[s])[i] & 0x7fff7fffu) + 0x00800080u;
+  return (any & 0x80008000u) != 0;
+}
+
 // lambda^(n-1-j) of the tokens j = 32 s + 8 g + e of a block of n
 __device__ __forceinline__ void powers(float g, int n, float (&w)[2][8]) {
   const int grp = (threadIdx.x & 63) >> 4;
@@ -405,7 +414,7 @@ __global__ __launch_bounds__(TV * 4) __attribute__((amdgpu_waves_per_eu(2, 2))) 
           const int m = it0 - jt;
           const float f = m == 0 ? 1.f : m == 1 ? far[0] : m == 2 ? far[1] : far[2];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) a[r] *= m == 0 ? diag[r] : off[r] * f;
+          for (int r = 0; r < 4; ++r) a[r] = m == 0 && 4 * grp + r > l ? 0.f : a[r] * (m == 0 ? diag[r] : off[r] * f);   // (a later key may be no number)
         }
         bf16x4 hi, lo;
 #pragma unroll
@@ -442,6 +451,32 @@ __global__ __launch_bounds__(TV * 4) __attribute__((amdgpu_waves_per_eu(2, 2))) 
     barrier();                             // the scores
     bf16x8 vf[1][2];
     Tile<TV>::template columns<1, SO>(vcol, 0, vf);
+    if (__ballot(not_finite(vf[0])) != 0) {  // their products with the zeros of earlier tokens would be no numbers: taken out, and their columns marked from there on
+      int first = C;
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = (float)vf[0][s][e];
+          if (!(fabsf(x) <= 3.4e38f)) {
+            const int j = 32 * s + 8 * grp + e;
+            first = first < j ? first : j;
+            vf[0][s][e] = (bf16_t)0.f;
+          }
+        }
+      first = min(first, __shfl_xor(first, 16, 64));
+      first = min(first, __shfl_xor(first, 32, 64));
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int from = __shfl(first, 4 * grp + r, 64);
+#pragma unroll
+        for (int it = 0; it < 4; ++it)
+          if (16 * it + l >= from) a[it][r] = __builtin_nanf("");
+      }
+      if (first < C)
+#pragma unroll
+        for (int t = 0; t < DK / 16; ++t) st.s[t] = f32x4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+    }
 #pragma unroll
     for (int it = 0; it < 4; ++it) {
 #pragma unroll
@@ -543,6 +578,7 @@ Plan plan_of(long B, long H, long dk, long dv, long T, long rows) {
     static const int lengths[] = {2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64, 96, 128, 192, 256};
     for (const long n : lengths) {
       if (n >= blocks) break;
+      if (r.units * ((blocks + n - 1) / n) * dk * r.tv * 4 > 4L << 30) continue;   // (the gains' memory, by the longest sequence for all)
       const long wgs = (ragged ? (all + n - 1) / n + B / 2 : B * ((blocks + n - 1) / n)) * heads;
       const double t = 8. + n * t_block * (rounds(wgs, slots) + 0.5 * rounds(wgs, 512)) + wgs * (double)(dk * r.tv * 8) / 4e6;
       if (t < best) { best = t; per = n; }

@@ -970,7 +970,7 @@ bool group_ok(int64_t g) { return g == 32 || g == 64 || g == 128; }
 KH_EXPORT int kh_quantize_w4(const void* w, void* q, void* scale, void* zero, int64_t N, int64_t K, int64_t group, int type, void* stream) {
   if (!w || !q || !scale || N <= 0 || K <= 0 || type < 0 || type > 2) return KH_ERR_INVALID_ARG;
   if (!group_ok(group)) return KH_ERR_UNSUPPORTED;
-  if (!kh_aligned16(q) || !kh_aligned16(scale)) return KH_ERR_ALIGNMENT;
+  if (!kh_aligned16(q) || ((uintptr_t)scale & 7) || ((uintptr_t)zero & 3)) return KH_ERR_ALIGNMENT;   // (any whole rows of larger ones)
   if (K > (1L << 24) || N > (1L << 24)) return KH_ERR_TOO_LARGE;
   const long groups = (K + group - 1) / group, pieces = groups * (group / 8);
   const long wg = (N * pieces + 4 * PT * 64 - 1) / (4 * PT * 64);
@@ -994,7 +994,7 @@ KH_EXPORT int kh_dequantize_w4(const void* q, const void* scale, const void* zer
                                void* stream) {
   if (!q || !scale || !out || N <= 0 || K <= 0 || type < 0 || type > 2) return KH_ERR_INVALID_ARG;
   if (!group_ok(group)) return KH_ERR_UNSUPPORTED;
-  if (!kh_aligned16(q) || !kh_aligned16(scale)) return KH_ERR_ALIGNMENT;
+  if (!kh_aligned16(q) || ((uintptr_t)scale & 7) || ((uintptr_t)zero & 3)) return KH_ERR_ALIGNMENT;   // (any whole rows of larger ones)
   if (K > (1L << 24) || N > (1L << 24)) return KH_ERR_TOO_LARGE;
   const long groups = (K + group - 1) / group, words = (K + 31) / 32 * 4;
   const long wg = (N * words + 4 * PT * 64 - 1) / (4 * PT * 64);
@@ -1019,7 +1019,7 @@ KH_EXPORT int kh_w4_linear(const void* x, const void* q, const void* scale, cons
   if (R > 0 && (!a_cat || !b_cat || !col_scale || !workspace)) return KH_ERR_INVALID_ARG;
   if (!group_ok(group) || R % 32 != 0) return KH_ERR_UNSUPPORTED;
   if (R > 128 || K > (1L << 24) || N > (1L << 24) || (M + 15) / 16 > 65535) return KH_ERR_TOO_LARGE;
-  if (!kh_aligned16(q) || !kh_aligned16(scale)) return KH_ERR_ALIGNMENT;
+  if (!kh_aligned16(q) || ((uintptr_t)scale & 7) || ((uintptr_t)zero & 3)) return KH_ERR_ALIGNMENT;   // (any whole rows of larger ones)
   hipStream_t s = (hipStream_t)stream;
   const bool many = many_rows(M, N, K);
   const int splits = R == 0 ? 0 : many ? 1 : shrink_splits(M, K, R);

@@ -11,6 +11,7 @@ token view [N, H*W, C] the transformer blocks need is the same memory -- the NCH
 """
 from __future__ import annotations
 
+import dataclasses
 import os
 import weakref
 from typing import Dict, List, Optional, Sequence
@@ -416,10 +417,22 @@ class LoRALinearW4(nn.Module):
         if layer.bias is not None:
             new.bias.data.copy_(layer.bias.detach())
         if isinstance(layer, LoRALinear):
-            new.adapters, new.global_scale, new.adapters_enabled = dict(layer.adapters), layer.global_scale, layer.adapters_enabled
+            new.adapters = {n: dataclasses.replace(ad) for n, ad in layer.adapters.items()}     # (their weights are each layer's own)
+            new.global_scale, new.adapters_enabled = layer.global_scale, layer.adapters_enabled
             new._fused = set(layer._fused)
             new.set_active(layer.active)
         return new
+
+    def _apply(self, fn, *args, **kwargs):
+        dtype = fn(torch.empty(0, dtype=self.dtype)).dtype
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError(f"activations are bf16 or fp16, not {dtype}")
+        scale = self.weight_scale
+        super()._apply(fn, *args, **kwargs)
+        if self.weight_scale.dtype != torch.bfloat16:       # scales are bf16 whatever the activations are: moved, not converted
+            self.weight_scale = scale.to(self.weight_q.device)
+        self.dtype = dtype
+        return self
 
     def packed_weight(self) -> "ops.W4Weight":
         return ops.W4Weight(self.weight_q, self.weight_scale, self.weight_zero, self.in_features, self.group)
@@ -458,7 +471,7 @@ class LoRALinearW4(nn.Module):
     def refresh_adapters(self) -> None:
         """(Re)build the packed buffers; a change of scales alone is written into them."""
         names = [n for n in self.active if n not in self._fused] if self.adapters_enabled else []
-        key = (self.weight_q.device,) + tuple((n, id(self.adapters[n].down)) for n in names)
+        key = (self.weight_q.device, self.dtype) + tuple((n, id(self.adapters[n].down)) for n in names)
         if names and key == self._packed_key and self._packed is not None:
             rescale_(self._packed, self.adapters, self.global_scale)
             return
@@ -485,8 +498,7 @@ class LoRALinearW4(nn.Module):
         w, b = self.packed_weight(), None if self.bias is None else self.bias.detach()
         if p is None:
             return ops.w4_linear(x, w, b, residual=residual)
-        if p.a_cat.device != x.device:      # the layer was moved
-            self._packed_key = None
+        if p.a_cat.device != x.device or p.a_cat.dtype != self.dtype:      # the layer was moved or converted
             self.refresh_adapters()
             p = self._packed
         y = ops.w4_linear(x, w, b, p.a_cat, p.b_cat, p.col_scale, residual=residual)

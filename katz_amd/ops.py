@@ -1472,7 +1472,8 @@ def w4_linear(x: torch.Tensor, w: W4Weight, bias: Optional[torch.Tensor] = None,
               b_cat: Optional[torch.Tensor] = None, col_scale: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
               out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y = x w^T + b + ((x A_cat^T) * col_scale) B_cat^T (+ residual) with weights in 4 bits, bf16 or fp16 by x.dtype; the adapter operands as
-    for lora_linear (a_cat [R,K], b_cat [N,R], col_scale [R] fp32, R % 32 == 0, R <= 128).  Made for few rows, right for any number."""
+    for lora_linear (a_cat [R,K], b_cat [N,R], col_scale [R] fp32, R % 32 == 0, R <= 128).  Made for few rows, right for any number.  A row of x that
+    holds an infinity gives NaN."""
     lib = _lib.load()
     dt, xs, q = x.dtype, x.shape, w.q
     if dt is not torch.bfloat16 and dt is not torch.float16:
@@ -1586,7 +1587,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: i
     seg_start (int32 [B+1], on the GPU) and max_seg_rows, the longest sequence, packed rows [rows, ..]: sequence b is rows seg_start[b] to
     seg_start[b+1], other rows of a given out stay as they were (those of a new one are zero).  log_decay float32 [heads], <= 0.
     state: float32 [B,heads,dk,dv] to start from (None: zeros), overwritten unless state_out is given; with slots (int32 [B], distinct) it is a pool
-    and sequence b has slot slots[b]; a slot outside the pool leaves its sequence out."""
+    and sequence b has slot slots[b]; a slot outside the pool leaves its sequence out.  Tokens do not depend on later ones, also where those are no
+    numbers; an infinity in v gives NaN from its token on."""
     lib = _lib.load()
     packed = seg_start is not None
     kv, dk, dv = _la_sizes(q, k, v, heads, kv_heads, log_decay, 2 if packed else 3)
@@ -1608,13 +1610,15 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: i
         _la_out(out, shape)
     if scale is None:
         scale = dk ** -0.5
-    if not B or not rows:
-        if state is None:
-            state_out.zero_()
-        elif state_out is not state and B:
-            if slots is not None:
-                raise ValueError("sequences without tokens, from one pool into another")
-            state_out.copy_(state)
+    if not B or not rows:                      # no token: the states as they were
+        if B and state_out is not state:
+            if slots is None:
+                state_out.zero_() if state is None else state_out.copy_(state)
+            else:
+                named = torch.zeros(n_slots + 1, dtype=torch.bool, device=q.device)
+                named.index_fill_(0, torch.where((slots >= 0) & (slots < n_slots), slots, n_slots).long(), True)
+                named = named[:n_slots].view(-1, 1, 1, 1)
+                state_out.masked_fill_(named, 0.0) if state is None else state_out.copy_(torch.where(named, state, state_out))
         return out, state_out
     ld, bs = zip(*[_la_strides(t) for t in (q, k, v, out)])
     if not packed and T == 1 and state is not None and all(st >= t.shape[-1] for st, t in zip(bs, (q, k, v, out))):   # one pass over the state

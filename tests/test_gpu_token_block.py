@@ -238,3 +238,29 @@ def test_layer_with_adapters_follows_scales_and_fuses():
     other = LoRALinearW4(128, 96, device=DEV)
     other.load_state_dict(saved)
     assert torch.equal(other(x), layer(x))
+
+
+def test_layer_with_adapters_converts_and_keeps_its_own_weights():
+    """A layer of another type keeps the scales that its codes were chosen against; a LoRALinear that one was made from keeps its adapters' weights."""
+    from katz_amd.layers import LoRALinear, LoRALinearW4
+
+    g = torch.Generator().manual_seed(7)
+    src = LoRALinear(128, 96, bias=True, device=DEV, dtype=BF)
+    src.weight.data.copy_(torch.randn(96, 128, generator=g) * 0.05)
+    src.bias.data.copy_(torch.randn(96, generator=g))
+    src.add_adapter("a", (torch.randn(16, 128, generator=g) * 0.1).to(BF), (torch.randn(96, 16, generator=g) * 0.1).to(BF), weight=0.5)
+    src.set_active(["a"])
+    layer = LoRALinearW4.from_linear(src)
+    layer.set_active(["a"], [1.0])
+    assert src.adapters["a"].weight == 0.5 and layer.adapters["a"].weight == 1.0
+    x = torch.randn(5, 128, generator=g).to(DEV, BF)
+    y, scale = layer(x), layer.weight_scale.clone()
+    layer.to(torch.float16)
+    assert layer.dtype is torch.float16 and layer.weight_scale.dtype is BF and torch.equal(layer.weight_scale, scale)
+    close(layer(x.half()), y.cpu().to(F64), "in fp16")
+    layer.to(BF)
+    assert torch.equal(layer(x), y)
+    with pytest.raises(TypeError):
+        layer.float()
+    assert torch.equal(layer(x), y)
+    assert torch.equal(layer.cpu().to(DEV)(x), y)

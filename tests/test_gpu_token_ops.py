@@ -578,3 +578,60 @@ def test_empty_calls():
     assert ops.w4_linear(e(0, 32), w).shape == (0, 8)
     h, u = ops.block_norm(e(0, 64), e(0, 64))
     assert h.shape == u.shape == (0, 64)
+
+
+@pytest.mark.parametrize("T,H,dk,dv", [(200, 2, 64, 64), (200, 1, 128, 128), (1500, 1, 64, 128), (1500, 1, 128, 64)])
+def test_linear_attention_does_not_depend_on_later_tokens(T, H, dk, dv):
+    """What is no number in the keys or values of a token leaves the outputs of the tokens before it as they were; in a value it is seen in its column from
+    there on."""
+    from katz_amd import ops
+
+    r = gen(14)
+    q, k, v = randn(r, 1, T, H * dk), randn(r, 1, T, H * dk), randn(r, 1, T, H * dv)
+    g = on(torch.tensor([-0.02, -0.3][:H]))
+    clean, _ = ops.linear_attention(on(q), on(k), on(v), H, g)
+    for at, col, bad in ((T - 130, 5, float("nan")), (T - 97, dv - 1, float("inf")), (T - 1, 17, float("-inf")), (0, 0, float("nan"))):
+        v2 = v.clone()
+        v2[0, at, col] = bad
+        o, S = ops.linear_attention(on(q), on(k), on(v2), H, g)
+        others = [c for c in range(H * dv) if c != col]
+        assert torch.equal(o[:, :at], clean[:, :at]) and torch.equal(o[..., others], clean[..., others])
+        assert not torch.isfinite(o[:, at:, col]).any() and not torch.isfinite(S[0, 0, :, col]).any()
+    for at in (T - 130, T - 97, T - 1):
+        k2 = k.clone()
+        k2[0, at, :dk] = float("nan")
+        o, _ = ops.linear_attention(on(q), on(k2), on(v), H, g)
+        assert torch.equal(o[:, :at], clean[:, :at]) and torch.isnan(o[:, at:, :dv]).all()
+
+
+def test_sequences_without_tokens_leave_pools_as_they_are():
+    from katz_amd import ops
+
+    e = lambda *s: torch.empty(*s, dtype=BF, device=DEV)                    # noqa: E731
+    g = torch.zeros(2, device=DEV)
+    r = gen(15)
+    pool, other = (on(torch.randn(4, 2, 64, 64, generator=r)) for _ in range(2))
+    keep = other.clone()
+    slots = torch.tensor([2, -1, 9], dtype=torch.int32, device=DEV)
+    ops.linear_attention(e(3, 0, 128), e(3, 0, 128), e(3, 0, 128), 2, g, state=pool, state_out=other, slots=slots)
+    assert torch.equal(other[2], pool[2]) and torch.equal(other[[0, 1, 3]], keep[[0, 1, 3]])
+    ops.linear_attention(e(3, 0, 128), e(3, 0, 128), e(3, 0, 128), 2, g, state_out=other, slots=slots)
+    assert not other[2].any() and torch.equal(other[[0, 1, 3]], keep[[0, 1, 3]])
+    ops.linear_attention(e(0, 4, 128), e(0, 4, 128), e(0, 4, 128), 2, g, state_out=other, slots=slots[:0])
+    assert not other[2].any() and torch.equal(other[[0, 1, 3]], keep[[0, 1, 3]])
+
+
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True)])
+def test_w4_linear_of_rows_of_larger_weights(group, zeros):
+    """Rows first .. last of a weight are a weight: a part of a linear's outputs."""
+    from katz_amd import ops
+
+    r = gen(16)
+    w = ops.quantize_w4(on(randn(r, 71, 320, std=0.1)), group, zeros)
+    for M in (3, 40):
+        x = on(randn(r, M, 320))
+        y = ops.w4_linear(x, w)
+        for a, b in ((1, 71), (3, 20), (70, 71)):
+            part = ops.W4Weight(w.q[a:b], w.scale[a:b], None if w.zero is None else w.zero[a:b], 320, group)
+            assert torch.equal(ops.w4_linear(x, part), y[:, a:b])
+            assert torch.equal(ops.dequantize_w4(part), ops.dequantize_w4(w)[a:b])

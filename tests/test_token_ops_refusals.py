@@ -158,3 +158,11 @@ def test_tensor_functions_refuse_shapes_and_types():
         with pytest.raises(kind):
             call()
             pytest.fail(f"call {i} was not refused")
+
+
+def test_launches_that_would_be_too_large(lib):
+    """More threads than a launch takes; scales and zero points at addresses that whole rows cannot have."""
+    norm = lambda M, D: lib.kh_block_norm(16, 16, None, 1, None, None, None, None, 16, 16, M, D, 1.0, 1e-6, 0, 0, 0, None)      # noqa: E731
+    assert norm(1 << 26, 64) == -4 and norm(1 << 24, 4096) == -4 and norm(1 << 22, 32768) == -4
+    linear = lambda s=16, z=None: lib.kh_w4_linear(16, 16, s, z, None, None, None, None, None, 16, None, 2, 8, 64, 0, 64, 0, None)      # noqa: E731
+    assert linear(s=20) == -3 and linear(z=18) == -3
