@@ -448,7 +448,6 @@ __global__ __launch_bounds__(TV * 4) __attribute__((amdgpu_waves_per_eu(2, 2))) 
         for (int r = 0; r < 4; ++r) a[it][r] *= rise[it];
       }
     }
-    barrier();                             // the scores
     bf16x8 vf[1][2];
     Tile<TV>::template columns<1, SO>(vcol, 0, vf);
     if (__ballot(not_finite(vf[0])) != 0) {  // their products with the zeros of earlier tokens would be no numbers: taken out, and their columns marked from there on
@@ -477,6 +476,7 @@ __global__ __launch_bounds__(TV * 4) __attribute__((amdgpu_waves_per_eu(2, 2))) 
 #pragma unroll
         for (int t = 0; t < DK / 16; ++t) st.s[t] = f32x4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
     }
+    barrier();                             // the scores
 #pragma unroll
     for (int it = 0; it < 4; ++it) {
 #pragma unroll
