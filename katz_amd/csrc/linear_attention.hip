@@ -5,8 +5,9 @@
 //
 // Prompts.  In blocks of 64 tokens the recurrence is four products for the matrix unit: with positions i, j of a block
 //   o_i = scale * (sum_{j <= i} lambda^(i-j) (q_i k_j) v_j  +  lambda^(i+1) q_i S),   S' = lambda^n S + sum_j lambda^(n-1-j) k_j v_j^T
-// A sequence is cut into segments of whole blocks where there are few heads: each leaves what it adds to the state (la_gain), the sums over the
-// segments before each follow (la_scan), and then every segment runs on its own (la_out).
+// Where there are few heads, the blocks of all sequences of a head, one after the other, are cut into equal chunks, wherever a sequence ends: a chunk whose last
+// sequence goes on in the next leaves what it adds to that state (la_gain), the sums over the chunks before each follow (la_scan), and then every chunk runs on
+// its own (la_out).
 // bf16 operands carry 8 bits, so what is no input is fed to the matrix unit in pieces: scores and states as two (16 bits: their results are
 // rounded to bf16), the decayed values that make the state as three (24 bits: the state stays in 32).
 #include "kh_common.h"
@@ -24,11 +25,13 @@ struct LaParams {
   float* s_out;
   const int32_t* seg_start;    // NULL: [B][T] rows through batch strides
   const int32_t* slots;
-  float* ws;                   // [unit][segment][dk * TV]: a segment's gain, then the state before it
+  // [unit][chunk][dk * TV] twice: what a chunk adds to the state of its last sequence, then that state; what that sequence began with in the chunk (its slot may
+  // be written by the chunk in which it ends).  Then the chunks.
+  float* ws;
   long ldq, ldk, ldv, ldo, bsq, bsk, bsv, bso;
   long rows;                   // of packed tensors
   int B, H, share;             // share: query heads of a key head
-  int T, dv, n_slots, nseg, seg;   // seg: tokens of a segment, a multiple of C
+  int T, dv, n_slots, chunks;  // chunks: 0 where a workgroup has a whole sequence
   float scale;
   int fill;                    // la_step: rows that are left out are zero
 };
@@ -39,6 +42,20 @@ struct Unit {                  // one (sequence, head, range of columns of v)
   float g;                     // log2 of the decay
 };
 
+__device__ __forceinline__ int length_of(const LaParams& p, int b, long* first = nullptr) {
+  if (!p.seg_start) return p.T;
+  long a = p.seg_start[b], e = p.seg_start[b + 1];      // whatever the table holds, rows stay inside the tensors
+  a = a < 0 ? 0 : a > p.rows ? p.rows : a;
+  e = e < a ? a : e > p.rows ? p.rows : e;
+  if (first) *first = a;
+  return (int)(e - a < p.T ? e - a : p.T);
+}
+
+__device__ __forceinline__ float decay_of(const LaParams& p, int h) {
+  const float g = p.log_decay[h];
+  return (g < -1.0e4f ? -1.0e4f : g) * 1.4426950408889634f;     // (-inf, no memory at all, times a distance of 0 would be no number)
+}
+
 // TV: columns of v of a unit
 __device__ __forceinline__ bool unit_of(const LaParams& p, int b, int ht, int DK, int TV, Unit& r) {
   const int tiles = p.dv / TV;
@@ -48,23 +65,15 @@ __device__ __forceinline__ bool unit_of(const LaParams& p, int b, int ht, int DK
   r.slot = p.slots ? p.slots[r.b] : r.b;
   if (r.slot < 0 || r.slot >= p.n_slots) return false;
   long row = 0;
-  r.len = p.T;
+  r.len = length_of(p, r.b, &row);
   r.q0 = (long)r.b * p.bsq; r.k0 = (long)r.b * p.bsk; r.v0 = (long)r.b * p.bsv; r.o0 = (long)r.b * p.bso;
-  if (p.seg_start) {           // whatever the table holds, rows stay inside the tensors
-    long a = p.seg_start[r.b], e = p.seg_start[r.b + 1];
-    a = a < 0 ? 0 : a > p.rows ? p.rows : a;
-    e = e < a ? a : e > p.rows ? p.rows : e;
-    row = a;
-    r.len = (int)(e - a < p.T ? e - a : p.T);
-    r.q0 = r.k0 = r.v0 = r.o0 = 0;
-  }
+  if (p.seg_start) r.q0 = r.k0 = r.v0 = r.o0 = 0;
   const int hk = r.h / p.share;
   r.q0 += row * p.ldq + (long)r.h * DK;
   r.k0 += row * p.ldk + (long)hk * DK;
   r.v0 += row * p.ldv + (long)hk * p.dv + r.tile * TV;
   r.o0 += row * p.ldo + (long)r.h * p.dv + r.tile * TV;
-  const float g = p.log_decay[r.h];
-  r.g = (g < -1.0e4f ? -1.0e4f : g) * 1.4426950408889634f;     // (-inf, no memory at all, times a distance of 0 would be no number)
+  r.g = decay_of(p, r.h);
   return true;
 }
 
@@ -232,33 +241,100 @@ __device__ __forceinline__ long state_at(const LaParams& p, const Unit& u, int w
 template <int DK>
 __device__ __forceinline__ int ws_at(int wave, int t) { return ((wave * (DK / 16) + t) * 64 + (threadIdx.x & 63)) * 4; }
 
-// The workgroup's unit and segment.  Units that share keys and values are neighbours on one XCD; such clusters go round the eight, segment by segment, since
-// sequences differ in length.
-template <int DK, int TV>
-__device__ __forceinline__ bool work_of(const LaParams& p, Unit& u, int& sg, long& unit) {
+// The workgroup's head and columns, and its chunk or sequence.  Units that share keys and values are neighbours on one XCD; such clusters go round the eight.
+template <int TV>
+__device__ __forceinline__ bool work_of(const LaParams& p, int& ht, int& which) {
   const uint32_t tiles = (uint32_t)(p.dv / TV), size = tiles * (uint32_t)p.share, kv = (uint32_t)p.H / (uint32_t)p.share;
-  const uint32_t local = blockIdx.x / 8, cluster = local / size * 8 + blockIdx.x % 8, rest = cluster / kv;
-  const uint32_t b = rest / (uint32_t)p.nseg;
-  if (b >= (uint32_t)p.B) return false;
-  sg = (int)(rest % (uint32_t)p.nseg);
-  const int ht = (int)((cluster % kv) * size + local % size);
-  unit = (long)b * ((long)p.H * tiles) + ht;
-  return unit_of(p, (int)b, ht, DK, TV, u);
+  const uint32_t local = blockIdx.x / 8, cluster = local / size * 8 + blockIdx.x % 8;
+  which = (int)(cluster / kv);
+  ht = (int)((cluster % kv) * size + local % size);
+  return which < (p.chunks ? p.chunks : p.B);
+}
+
+// Blocks of a sequence: none where it is left out.
+__device__ __forceinline__ int blocks_of(const LaParams& p, int b) {
+  if (p.slots) {
+    const int slot = p.slots[b];
+    if (slot < 0 || slot >= p.n_slots) return 0;
+  }
+  return (length_of(p, b) + C - 1) / C;
+}
+
+struct Chunk {
+  int b, block, count;         // its first sequence and block in it, blocks
+  int tail;                    // blocks of its last sequence where that goes on in the next chunk: from the sequence's start, or, negative, from the chunk's
+};
+// The chunk's place among the blocks of all sequences, and the sequence that goes on (all NT threads; LDS: 8 NT / 64 + 16 bytes, dead afterwards).
+template <int NT>
+__device__ __forceinline__ Chunk chunk_of(const LaParams& p, int chunk, int& goes_on, char* lds) {
+  constexpr int NW = NT / 64;
+  long* sums = reinterpret_cast<long*>(lds);
+  int* at = reinterpret_cast<int*>(lds + NW * 8);
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, per = (p.B + NT - 1) / NT;
+  const int b0 = t * per < p.B ? t * per : p.B, b1 = b0 + per < p.B ? b0 + per : p.B;
+  long mine = 0;
+  for (int b = b0; b < b1; ++b) mine += blocks_of(p, b);
+  long upto = mine;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const long v = __shfl_up(upto, o, 64);
+    if (lane >= o) upto += v;
+  }
+  if (lane == 63) sums[wave] = upto;
+  __syncthreads();
+  long before = upto - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    if (w < wave) before += sums[w];
+    total += sums[w];
+  }
+  const uint32_t all = (uint32_t)(total < (1L << 30) ? total : 1L << 30);      // (more than that only where a table names the same rows again and again)
+  const uint32_t size = (all + (uint32_t)p.chunks - 1) / (uint32_t)p.chunks;
+  const long first = (long)size * chunk, next = first + size;
+  auto find = [&](long target, int to) {
+    if (target < before || target >= before + mine) return;
+    long r = target - before;
+    int b = b0;
+    for (int n; b < b1 - 1 && r >= (n = blocks_of(p, b)); ++b) r -= n;
+    at[to] = b;
+    at[to + 1] = (int)r;
+  };
+  find(first, 0);
+  find(next, 2);
+  __syncthreads();
+  Chunk c{0, 0, 0, 0};
+  if (first < all) {
+    c.b = __builtin_amdgcn_readfirstlane(at[0]);
+    c.block = __builtin_amdgcn_readfirstlane(at[1]);
+    c.count = (int)(next < all ? size : all - first);
+    if (next < all) {
+      goes_on = __builtin_amdgcn_readfirstlane(at[2]);
+      const int done = __builtin_amdgcn_readfirstlane(at[3]);
+      c.tail = done <= c.count ? done : -c.count;
+    }
+  }
+  __syncthreads();
+  return c;
+}
+__device__ __forceinline__ Chunk* chunks_at(const LaParams& p, int DK, int TV) {
+  return reinterpret_cast<Chunk*>(p.ws + 2 * (long)p.H * (p.dv / TV) * p.chunks * (DK * TV));
 }
 
 template <int DK, int TV>
 __global__ __launch_bounds__(TV * 4) void la_gain(const LaParams p) {
   constexpr int NW = TV / 16, STAGE = Tile<DK>::BYTES + Tile<TV>::BYTES;
   extern __shared__ __attribute__((aligned(16))) char smem[];   // two stages of K, V
+  int ht, chunk, b = 0;
+  if (!work_of<TV>(p, ht, chunk)) return;
+  const Chunk ch = chunk_of<TV * 4>(p, chunk, b, smem);
+  if (ht == 0 && threadIdx.x == 0) chunks_at(p, DK, TV)[chunk] = ch;
+  if (ch.tail == 0) return;
   Unit u;
-  int sg;
-  long unit;
-  if (!work_of<DK, TV>(p, u, sg, unit)) return;
-  const int t0 = sg * p.seg, t1 = u.len < t0 + p.seg ? u.len : t0 + p.seg;
-  if (t0 >= t1) return;
+  if (!unit_of(p, b, ht, DK, TV, u)) return;
+  const int t0 = ch.tail > 0 ? 0 : ch.block * C, t1 = t0 + (ch.tail > 0 ? ch.tail : -ch.tail) * C;     // (whole blocks: the sequence goes on)
   auto fetch = [&](int c, int st) {
-    Tile<DK>::template fetch<NW>(p.k + u.k0 + (long)c * p.ldk, p.ldk, t1 - c, smem + st * STAGE);
-    Tile<TV>::template fetch<NW>(p.v + u.v0 + (long)c * p.ldv, p.ldv, t1 - c, smem + st * STAGE + Tile<DK>::BYTES);
+    Tile<DK>::template fetch<NW>(p.k + u.k0 + (long)c * p.ldk, p.ldk, C, smem + st * STAGE);
+    Tile<TV>::template fetch<NW>(p.v + u.v0 + (long)c * p.ldv, p.ldv, C, smem + st * STAGE + Tile<DK>::BYTES);
   };
   fetch(t0, 0);
   State<DK> st;
@@ -266,7 +342,7 @@ __global__ __launch_bounds__(TV * 4) void la_gain(const LaParams p) {
   for (int t = 0; t < DK / 16; ++t) st.s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
   float w[2][8];
   powers(u.g, C, w);
-  float decay = power(u.g, C);
+  const float decay = power(u.g, C);
   uint32_t kcol[2], vcol[2];
   Tile<DK>::template column_rows<true>(smem, kcol);
   Tile<TV>::template column_rows<false>(smem + Tile<DK>::BYTES, vcol);
@@ -277,10 +353,6 @@ __global__ __launch_bounds__(TV * 4) void la_gain(const LaParams p) {
     wait_all_loads();
     barrier();                             // everybody's share of this block; and nobody reads the block before any more
     if (c + C < t1) fetch(c + C, 1 - decltype(stage_tag)::value);
-    if (t1 - c < C) {
-      powers(u.g, t1 - c, w);
-      decay = power(u.g, t1 - c);
-    }
     bf16x8 vf[1][2];
     Tile<TV>::template columns<1, SO>(vcol, 0, vf);
     add_block<DK, TV, 3, SO>(st, vf[0], kcol, decay, w);
@@ -289,45 +361,77 @@ __global__ __launch_bounds__(TV * 4) void la_gain(const LaParams p) {
     block(c, std::integral_constant<int, 0>{});
     if (c + C < t1) block(c + C, std::integral_constant<int, 1>{});
   }
-  float* ws = p.ws + (unit * p.nseg + sg) * (DK * TV);
+  float* ws = p.ws + ((long)ht * p.chunks + chunk) * (DK * TV);
 #pragma unroll
   for (int t = 0; t < DK / 16; ++t) *reinterpret_cast<f32x4*>(ws + ws_at<DK>(threadIdx.x >> 6, t)) = st.s[t];
 }
 
-// Gains to the states before each segment, in place; the state behind the last one to its slot.  A thread has the four rows of la_gain's lane: grid
-// (DK / 16, units).
+// Gains to the states that the next chunks begin with, in place, and the states of sequences without tokens to their slots.  A thread has the four rows of
+// la_gain's lane: grid (DK / 16, units).
 template <int DK, int TV>
 __global__ __launch_bounds__(TV * 4) void la_scan(const LaParams p) {
-  Unit u;
-  const int heads = p.H * (p.dv / TV);
-  if (!unit_of(p, blockIdx.y / heads, blockIdx.y % heads, DK, TV, u)) return;
-  const int t = blockIdx.x, wave = threadIdx.x >> 6;
-  const long at = state_at<DK, TV>(p, u, wave, t);
+  constexpr int NT = TV * 4, AHEAD = 8;
+  __shared__ int empty[NT], n_empty;
+  const int ht = blockIdx.y, t = blockIdx.x, wave = threadIdx.x >> 6;
+  const Chunk* ch = chunks_at(p, DK, TV);
+  float* w = p.ws + (long)ht * p.chunks * (DK * TV) + ws_at<DK>(wave, t);
+  const long starts = (long)gridDim.y * p.chunks * (DK * TV);
+  const float g = decay_of(p, ht / (p.dv / TV));
+  auto start_of = [&](int b) {             // the state that a sequence begins with
+    f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
+    Unit u;
+    if (p.s_in && unit_of(p, b, ht, DK, TV, u)) {
+      const long at = state_at<DK, TV>(p, u, wave, t);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[r] = p.s_in[at + (long)r * p.dv];
+    }
+    return s;
+  };
   f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
-  if (p.s_in)
+  for (int c0 = 0; c0 < p.chunks - 1; c0 += AHEAD) {     // so many on their way at a time
+    f32x4 gain[AHEAD], start[AHEAD];
+    int tail[AHEAD];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) s[r] = p.s_in[at + (long)r * p.dv];
-  float* w = p.ws + (long)blockIdx.y * p.nseg * (DK * TV) + ws_at<DK>(wave, t);
-  const int n = (u.len + p.seg - 1) / p.seg;
-  const float d = power(u.g, p.seg), dl = power(u.g, u.len - (n - 1) * p.seg);
-  for (int s0 = 0; s0 < n; s0 += 4) {      // four gains on their way at a time
-    f32x4 gain[4];
+    for (int i = 0; i < AHEAD; ++i) tail[i] = c0 + i < p.chunks - 1 ? __builtin_amdgcn_readfirstlane(ch[c0 + i].tail) : 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (s0 + i < n) gain[i] = *reinterpret_cast<const f32x4*>(w + (long)(s0 + i) * (DK * TV));
+    for (int i = 0; i < AHEAD; ++i) {
+      if (tail[i] != 0) gain[i] = *reinterpret_cast<const f32x4*>(w + (long)(c0 + i) * (DK * TV));
+      if (tail[i] > 0) start[i] = start_of(__builtin_amdgcn_readfirstlane(ch[c0 + i + 1].b));
+    }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (s0 + i < n) {
-        *reinterpret_cast<f32x4*>(w + (long)(s0 + i) * (DK * TV)) = s;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s[r] = fmaf(s0 + i == n - 1 ? dl : d, s[r], gain[i][r]);
+    for (int i = 0; i < AHEAD; ++i) {
+      if (tail[i] == 0) continue;
+      if (tail[i] > 0) {
+        s = start[i];
+        if (p.s_in) *reinterpret_cast<f32x4*>(w + starts + (long)(c0 + i) * (DK * TV)) = s;
       }
-  }
+      const float d = power(g, C * (tail[i] > 0 ? tail[i] : -tail[i]));
 #pragma unroll
-  for (int r = 0; r < 4; ++r) p.s_out[at + (long)r * p.dv] = s[r];
+      for (int r = 0; r < 4; ++r) s[r] = fmaf(d, s[r], gain[i][r]);
+      *reinterpret_cast<f32x4*>(w + (long)(c0 + i) * (DK * TV)) = s;
+    }
+  }
+  if (p.s_in == p.s_out) return;
+  for (int b0 = 0; b0 < p.B; b0 += NT) {
+    if (threadIdx.x == 0) n_empty = 0;
+    __syncthreads();
+    const int b = b0 + threadIdx.x;
+    if (b < p.B && length_of(p, b) == 0) empty[atomicAdd(&n_empty, 1)] = b;       // (in any order: their slots are distinct)
+    __syncthreads();
+    for (int i = 0; i < n_empty; ++i) {
+      Unit u;
+      const int e = empty[i];
+      if (!unit_of(p, e, ht, DK, TV, u)) continue;
+      const f32x4 s0 = start_of(e);
+      const long at = state_at<DK, TV>(p, u, wave, t);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) p.s_out[at + (long)r * p.dv] = s0[r];
+    }
+    __syncthreads();
+  }
 }
 
-// A segment's outputs from the state before it.  ONE: the whole sequence from the slot's state, whose successor it leaves.
+// The outputs of a chunk, sequence by sequence from the state before it, and the states behind those that end in it.  ONE: one whole sequence.
 template <int DK, int TV>
 struct OutShape {
   static constexpr int PP = C * 2 + 16;    // pitch of the scores in bytes: 16-byte pieces of neighbouring rows on other banks
@@ -341,12 +445,19 @@ __global__ __launch_bounds__(TV * 4) __attribute__((amdgpu_waves_per_eu(2, 2))) 
   char* const ph = smem + 2 * Sh::STAGE;
   char* const pl = ph + C * Sh::PP;
   Unit u;
-  int sg;
-  long unit;
-  if (!work_of<DK, TV>(p, u, sg, unit)) return;
+  int ht, which, left = 0, t0 = 0, t1;     // left: blocks of the chunk; t0, t1: tokens of the sequence
+  if (!work_of<TV>(p, ht, which)) return;
+  if constexpr (ONE) {
+    if (!unit_of(p, which, ht, DK, TV, u)) return;
+    t1 = u.len;
+  } else {
+    const Chunk ch = chunks_at(p, DK, TV)[which];
+    left = __builtin_amdgcn_readfirstlane(ch.count);
+    if (left == 0 || !unit_of(p, __builtin_amdgcn_readfirstlane(ch.b), ht, DK, TV, u)) return;
+    t0 = __builtin_amdgcn_readfirstlane(ch.block) * C;
+    t1 = u.len - t0 <= left * (long)C ? u.len : t0 + left * C;
+  }
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 15, grp = lane >> 4;
-  const int t0 = sg * p.seg, t1 = ONE || u.len < t0 + p.seg ? u.len : t0 + p.seg;
-  if (!ONE && t0 >= t1) return;
   auto fetch = [&](int c, int st) {
     char* to = smem + st * Sh::STAGE;
     Tile<DK>::template fetch<NW>(p.k + u.k0 + (long)c * p.ldk, p.ldk, t1 - c, to);
@@ -355,16 +466,22 @@ __global__ __launch_bounds__(TV * 4) __attribute__((amdgpu_waves_per_eu(2, 2))) 
   };
   if (t0 < t1) fetch(t0, 0);
   State<DK> st;
+  const long slot = ((long)ht * p.chunks + which) * (DK * TV), starts = (long)p.H * (p.dv / TV) * p.chunks * (DK * TV);
+  auto state_in = [&]() {                  // before token t0
+    if (ONE || (t0 == 0 && (t1 == u.len || !p.s_in))) {
 #pragma unroll
-  for (int t = 0; t < DK / 16; ++t) {
-    if (ONE) {
-      const long at = state_at<DK, TV>(p, u, wave, t);
+      for (int t = 0; t < DK / 16; ++t) {
+        const long at = state_at<DK, TV>(p, u, wave, t);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) st.s[t][r] = p.s_in ? p.s_in[at + (long)r * p.dv] : 0.f;
+        for (int r = 0; r < 4; ++r) st.s[t][r] = p.s_in ? p.s_in[at + (long)r * p.dv] : 0.f;
+      }
     } else {
-      st.s[t] = *reinterpret_cast<const f32x4*>(p.ws + (unit * p.nseg + sg) * (DK * TV) + ws_at<DK>(wave, t));
+      const float* from = p.ws + (t0 == 0 ? starts + slot : slot - DK * TV);
+#pragma unroll
+      for (int t = 0; t < DK / 16; ++t) st.s[t] = *reinterpret_cast<const f32x4*>(from + ws_at<DK>(wave, t));
     }
-  }
+  };
+  state_in();
   // scale * lambda^(i - j) of a tile of scores on the diagonal (rows j = 4 grp + r, column i = l) and, but for lambda^(16 m), of the tiles m + 1 beside it
   float diag[4], off[4], far[3], rise[4], w[2][8];
 #pragma unroll
@@ -392,7 +509,9 @@ __global__ __launch_bounds__(TV * 4) __attribute__((amdgpu_waves_per_eu(2, 2))) 
   const int p_to = (16 * it0 + l) * Sh::PP + (16 * j0 + 4 * grp) * 2, p_from = l * Sh::PP + grp * 16;
   // (a lane stores eight columns of one of two rows that are 16 apart)
   const int orow_at = l + 16 * (grp & 1);
-  bf16_t* orow = p.o + u.o0 + (long)(t0 + orow_at) * p.ldo + wave * 16 + (grp >> 1) * 8;
+  auto row_of = [&]() { return p.o + u.o0 + (long)(t0 + orow_at) * p.ldo + wave * 16 + (grp >> 1) * 8; };
+  bf16_t* orow = row_of();
+  bool ends = ONE || t1 == u.len;          // the sequence, in this chunk
 
   auto block = [&](int c, auto stage_tag) {
     constexpr int SO = decltype(stage_tag)::value * Sh::STAGE, KT = SO, QT = SO + Tile<DK>::BYTES;
@@ -495,25 +614,48 @@ __global__ __launch_bounds__(TV * 4) __attribute__((amdgpu_waves_per_eu(2, 2))) 
 #endif
     }
     orow += (long)C * p.ldo;
-    if (ONE || c + C < t1) {
-      if (ONE && t1 - c < C) {
+    if (ends) {
+      if (t1 - c < C) {
         powers(u.g, t1 - c, w);
         decay = power(u.g, t1 - c);
       }
-      add_block<DK, TV, ONE ? 3 : 2, SO>(st, vf[0], kcol, decay, w);   // (inside a segment the state only makes outputs)
+      add_block<DK, TV, 3, SO>(st, vf[0], kcol, decay, w);
+    } else if (c + C < t1) {               // (a state that is taken no further here only makes outputs)
+      add_block<DK, TV, 2, SO>(st, vf[0], kcol, decay, w);
     }
   };
-  for (int c = t0; c < t1; c += 2 * C) {
-    block(c, std::integral_constant<int, 0>{});
-    if (c + C < t1) block(c + C, std::integral_constant<int, 1>{});
-  }
-  if (ONE)
-#pragma unroll
-    for (int t = 0; t < DK / 16; ++t) {
-      const long at = state_at<DK, TV>(p, u, wave, t);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) p.s_out[at + (long)r * p.dv] = st.s[t][r];
+  for (;;) {
+    for (int c = t0; c < t1; c += 2 * C) {
+      block(c, std::integral_constant<int, 0>{});
+      if (c + C < t1) block(c + C, std::integral_constant<int, 1>{});
     }
+    const Unit was = u;
+    bool more = false;
+    if constexpr (!ONE) {                  // the next sequence with tokens
+      left -= (t1 - t0 + C - 1) / C;
+      if (left > 0)
+        for (int b = was.b + 1; b < p.B && !more; ++b) more = unit_of(p, b, ht, DK, TV, u) && u.len > 0;
+      if (more) {
+        t0 = 0;
+        t1 = u.len <= left * (long)C ? u.len : left * C;
+        barrier();                         // the stages are dead
+        fetch(0, 0);
+      }
+    }
+    if (ends)
+#pragma unroll
+      for (int t = 0; t < DK / 16; ++t) {
+        const long at = state_at<DK, TV>(p, was, wave, t);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) p.s_out[at + (long)r * p.dv] = st.s[t][r];
+      }
+    if (!more) break;
+    state_in();
+    orow = row_of();
+    ends = t1 == u.len;
+    powers(u.g, C, w);
+    decay = power(u.g, C);
+  }
 }
 
 // One token: the state is read and written once, which bounds it.  A workgroup has 64 columns of one head: 16 threads of four columns, 16 rows at a time.
@@ -556,37 +698,29 @@ __global__ __launch_bounds__(256) void la_step(const LaParams p) {
   }
 }
 
-struct Plan { long units; int tv, nseg, seg; };
+struct Plan { long heads; int tv, chunks; };      // heads: units of a sequence
 
 // 128 columns of v to a workgroup (which computes the scores once for them) where dv has them.
-// Segments: a workgroup goes through its blocks one after the other (us a block as measured: 3.8 with dk 128, 2.3 with 64, whatever else runs), so long
-// sequences of few heads are cut; but every segment's state is written, read, written and read again, and the rounds that the workgroups make on 256 CUs are
-// whole ones.  Of a few lengths the one with the least of these sums.  Measured, us for 1 | the chosen length | 4 blocks: 16384 packed tokens of 16 heads of 128
-// 480 | 143 | 176, one sequence of 16384 956 | 119 | 160, 16 of 1024 78 (whole) | 78 | 164, 2 x 4096 tokens of 20 heads of 64 138 | 46 | 45.
+// Chunks: a workgroup goes through its blocks one after the other (us a block as measured: 3.8 with dk 128, 2.3 with 64, whatever else runs), so few heads are
+// cut; but a chunk's state is written, read, written and read again, and the rounds that the workgroups make on 256 CUs are whole ones.
 Plan plan_of(long B, long H, long dk, long dv, long T, long rows) {
   Plan r;
   r.tv = dv % 128 == 0 ? 128 : 64;
-  r.units = B * H * (dv / r.tv);
-  const long blocks = (T + C - 1) / C, all = (rows + C - 1) / C, heads = H * (dv / r.tv);
-  const bool ragged = rows < B * T;
+  r.heads = H * (dv / r.tv);
+  r.chunks = 0;
+  const long blocks = (T + C - 1) / C, dense = B * blocks, packed = rows / C + B, all = dense < packed ? dense : packed;
   const double t_block = dk == 128 ? 3.8 : 2.3;
   const long slots = dk == 128 ? 256 : 512;           // workgroups that LDS lets run at once
   auto rounds = [](long wgs, long n) { return (double)((wgs + n - 1) / n); };
-  long per = blocks;
-  double best = rounds(r.units, slots) * blocks * t_block * 1.15;      // (in one piece the state needs its third piece everywhere)
-  if (r.units <= 65535) {                             // (la_scan's grid)
-    static const int lengths[] = {2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64, 96, 128, 192, 256};
-    for (const long n : lengths) {
-      if (n >= blocks) break;
-      if (r.units * ((blocks + n - 1) / n) * dk * r.tv * 4 > 4L << 30) continue;   // (the gains' memory, by the longest sequence for all)
-      const long wgs = (ragged ? (all + n - 1) / n + B / 2 : B * ((blocks + n - 1) / n)) * heads;
-      const double t = 8. + n * t_block * (rounds(wgs, slots) + 0.5 * rounds(wgs, 512)) + wgs * (double)(dk * r.tv * 8) / 4e6;
-      if (t < best) { best = t; per = n; }
-    }
+  double best = rounds(B * r.heads, slots) * blocks * t_block * 1.15;    // whole sequences (the state needs its third piece everywhere)
+  if (r.heads > 65535) return r;                      // (la_scan's grid)
+  static const int counts[] = {2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14, 15, 16, 18, 20, 22, 25, 28, 32, 36, 42, 51, 64, 85, 102, 128, 170, 256};
+  for (const long n : counts) {
+    const long size = (all + n - 1) / n;
+    if (n > all || n * r.heads * dk * r.tv * 8 > 4L << 30) break;
+    const double t = 14. + size * t_block * (rounds(n * r.heads, slots) + 0.6 * rounds(n * r.heads, 512)) + 0.3 * n + n * r.heads * (double)(dk * r.tv * 16) / 4e6;
+    if (t < best) { best = t; r.chunks = (int)n; }
   }
-  if (per > (1L << 24)) per = 1L << 24;
-  r.seg = (int)(per * C);
-  r.nseg = (int)((blocks + per - 1) / per);
   return r;
 }
 
@@ -604,11 +738,11 @@ int check(const LaParams& p, int64_t B, int64_t H, int64_t Hk, int64_t dk, int64
 }
 
 template <int DK, int TV>
-int prompt(const LaParams& p, long units, hipStream_t s) {
+int prompt(const LaParams& p, long heads, hipStream_t s) {
   constexpr int lds = OutShape<DK, TV>::LDS, gain_lds = 2 * (Tile<DK>::BYTES + Tile<TV>::BYTES);
-  const long size = p.share * (p.dv / TV), clusters = units / size * p.nseg;
+  const long size = p.share * (p.dv / TV), clusters = heads / size * (p.chunks ? p.chunks : p.B);
   const dim3 grid((unsigned)((clusters + 7) / 8 * 8 * size)), block(TV * 4);
-  if (p.nseg == 1) {
+  if (p.chunks == 0) {
     if (lds > 65536) {
       const hipError_t e = kh_allow_lds<la_out<DK, TV, true>>(lds);
       if (e != hipSuccess) return (int)e;
@@ -620,7 +754,7 @@ int prompt(const LaParams& p, long units, hipStream_t s) {
       if (e != hipSuccess) return (int)e;
     }
     kh_launch(KH_TAG_LINEAR_ATTENTION, la_gain<DK, TV>, grid, block, gain_lds, s, p);
-    kh_launch(KH_TAG_LINEAR_ATTENTION, la_scan<DK, TV>, dim3(DK / 16, (unsigned)units), block, 0, s, p);
+    kh_launch(KH_TAG_LINEAR_ATTENTION, la_scan<DK, TV>, dim3(DK / 16, (unsigned)heads), block, 0, s, p);
     kh_launch(KH_TAG_LINEAR_ATTENTION, la_out<DK, TV, false>, grid, block, lds, s, p);
   }
   KH_RETURN_LAST_ERROR();
@@ -633,7 +767,7 @@ KH_EXPORT int64_t kh_linear_attention_workspace_bytes(int64_t B, int64_t H, int6
   if ((dk != 64 && dk != 128) || dv % C != 0 || dv > 1024) return KH_ERR_UNSUPPORTED;
   if (B > (1 << 20) || H > (1 << 16) || B * H * (dv / C) > (1L << 30) || T > (1L << 30)) return KH_ERR_TOO_LARGE;
   const Plan r = plan_of(B, H, dk, dv, T, rows);
-  return r.nseg > 1 ? (int64_t)r.units * r.nseg * dk * r.tv * 4 : 0;
+  return r.chunks ? (int64_t)r.heads * r.chunks * dk * r.tv * 8 + r.chunks * (int64_t)sizeof(Chunk) : 0;
 }
 
 KH_EXPORT int kh_linear_attention_bf16(const void* q, const void* k, const void* v, void* o, const float* log_decay, const float* state_in,
@@ -644,7 +778,7 @@ KH_EXPORT int kh_linear_attention_bf16(const void* q, const void* k, const void*
   if (n_slots > (1L << 30) || rows > (1L << 31)) return KH_ERR_TOO_LARGE;
   LaParams p{(const bf16_t*)q, (const bf16_t*)k, (const bf16_t*)v, (bf16_t*)o, log_decay, state_in, state_out, seg_start, slots, (float*)workspace,
              ldq, ldk, ldv, ldo, bsq, bsk, bsv, bso, (long)rows, (int)B, (int)H, kv_heads > 0 ? (int)(H / kv_heads) : 1, (int)T, (int)dv, (int)n_slots,
-             1, 0, scale, 0};
+             0, scale, 0};
   const int rc = check(p, B, H, kv_heads, dk, dv, false);
   if (rc != KH_OK) return rc;
   if (T <= 0 || (seg_start && rows < 0)) return KH_ERR_INVALID_ARG;
@@ -652,14 +786,13 @@ KH_EXPORT int kh_linear_attention_bf16(const void* q, const void* k, const void*
   if (T > (1L << 30)) return KH_ERR_TOO_LARGE;
   if ((ldq | ldk | ldv) >= (1L << 24)) return KH_ERR_TOO_LARGE;
   const Plan r = plan_of(B, H, dk, dv, T, seg_start ? (rows > 0 ? rows : 1) : B * T);
-  p.nseg = r.nseg;
-  p.seg = r.seg;
-  if (p.nseg > 1 && !workspace) return KH_ERR_INVALID_ARG;
+  p.chunks = r.chunks;
+  if (p.chunks && !workspace) return KH_ERR_INVALID_ARG;
   if (!kh_aligned16(workspace)) return KH_ERR_ALIGNMENT;
-  if (r.units * r.nseg > 0x7fffffffL - 8 * r.units) return KH_ERR_TOO_LARGE;
+  if (r.heads * (r.chunks ? r.chunks : B) > 0x3fffffffL) return KH_ERR_TOO_LARGE;
   hipStream_t s = (hipStream_t)stream;
-  if (r.tv == 64) return dk == 64 ? prompt<64, 64>(p, r.units, s) : prompt<128, 64>(p, r.units, s);
-  return dk == 64 ? prompt<64, 128>(p, r.units, s) : prompt<128, 128>(p, r.units, s);
+  if (r.tv == 64) return dk == 64 ? prompt<64, 64>(p, r.heads, s) : prompt<128, 64>(p, r.heads, s);
+  return dk == 64 ? prompt<64, 128>(p, r.heads, s) : prompt<128, 128>(p, r.heads, s);
 }
 
 KH_EXPORT int kh_linear_attention_step_bf16(const void* q, const void* k, const void* v, void* o, const float* log_decay, const float* state_in,
@@ -668,7 +801,7 @@ KH_EXPORT int kh_linear_attention_step_bf16(const void* q, const void* k, const 
   if (flags & ~1) return KH_ERR_INVALID_ARG;
   if (n_slots > (1L << 30)) return KH_ERR_TOO_LARGE;
   LaParams p{(const bf16_t*)q, (const bf16_t*)k, (const bf16_t*)v, (bf16_t*)o, log_decay, state_in, state_out, nullptr, slots, nullptr,
-             0, 0, 0, 0, ldq, ldk, ldv, ldo, 0, (int)B, (int)H, kv_heads > 0 ? (int)(H / kv_heads) : 1, 1, (int)dv, (int)n_slots, 1, C, scale, flags};
+             0, 0, 0, 0, ldq, ldk, ldv, ldo, 0, (int)B, (int)H, kv_heads > 0 ? (int)(H / kv_heads) : 1, 1, (int)dv, (int)n_slots, 0, scale, flags};
   const int rc = check(p, B, H, kv_heads, dk, dv, true);
   if (rc != KH_OK) return rc;
   if (ldq < H * dk || ldk < kv_heads * dk || ldv < kv_heads * dv || ldo < H * dv) return KH_ERR_INVALID_ARG;

@@ -431,10 +431,14 @@ ATTENTION_CASES = [
     ((700, 63), True, 2, 1, 128, 64, True),
     ((16,) * 9, True, 40, 10, 64, 64, True),       # enough heads that no sequence is cut
     ((200,) * 3, False, 40, 10, 64, 576, False),
+    ((700, 0, 63, 1, 0, 1290, 64, 128, 5), True, 2, 1, 64, 64, True),      # cut wherever sequences end
+    ((0, 64, 700, 0), True, 2, 2, 128, 128, False),
+    ((1100, 1100), False, 3, 1, 64, 192, True),
+    ((2600,) + (10, 0, 3) * 101, True, 1, 1, 64, 64, True),                # more sequences than a workgroup has threads
 ]
 
 
-@pytest.mark.parametrize("case", ATTENTION_CASES, ids=lambda c: f"{'-'.join(map(str, c[0]))}-H{c[2]}of{c[3]}-{c[4]}x{c[5]}-{'packed' if c[1] else 'dense'}")
+@pytest.mark.parametrize("case", ATTENTION_CASES, ids=lambda c: f"{'-'.join(map(str, c[0][:9]))}-H{c[2]}of{c[3]}-{c[4]}x{c[5]}-{'packed' if c[1] else 'dense'}")
 def test_linear_attention(case):
     from katz_amd import ops
 
@@ -635,3 +639,33 @@ def test_w4_linear_of_rows_of_larger_weights(group, zeros):
             part = ops.W4Weight(w.q[a:b], w.scale[a:b], None if w.zero is None else w.zero[a:b], 320, group)
             assert torch.equal(ops.w4_linear(x, part), y[:, a:b])
             assert torch.equal(ops.dequantize_w4(part), ops.dequantize_w4(w)[a:b])
+
+
+def test_linear_attention_of_cut_sequences_with_slots():
+    """Sequences that are cut, of a pool, into another one or the same: slots that are named hold the states behind the last tokens (those of sequences without
+    tokens as they were), the others stay; sequences without a slot are left out."""
+    from katz_amd import ops
+
+    r = gen(17)
+    H, d, lengths, slots = 2, 64, (900, 77, 0, 640, 0, 200), (3, -1, 5, 0, 9, 6)
+    start = [sum(lengths[:i]) for i in range(len(lengths) + 1)]
+    q, k, v = (randn(r, start[-1], H * d) for _ in range(3))
+    g = torch.tensor([-0.3, -0.004])
+    pool = torch.randn(7, H, d, d, generator=r)
+    args = dict(seg_start=torch.tensor(start, dtype=torch.int32, device=DEV), max_seg_rows=900, slots=torch.tensor(slots, dtype=torch.int32, device=DEV))
+    src, dst = on(pool), torch.full((7, H, d, d), 8.0, device=DEV)
+    o, S = ops.linear_attention(on(q), on(k), on(v), H, on(g), state=src, state_out=dst, **args)
+    assert S is dst and torch.equal(src.cpu(), pool)
+    o2, S2 = ops.linear_attention(on(q), on(k), on(v), H, on(g), state=src, **args)
+    assert S2 is src and torch.equal(o, o2)
+    for b, (n, at) in enumerate(zip(lengths, slots)):
+        rows = slice(start[b], start[b] + n)
+        if not 0 <= at < 7:
+            assert not o[rows].any()
+            continue
+        ro, m, rs, ms = attention_reference(*[t[rows] for t in (q, k, v)], H, H, g, d ** -0.5, pool[at])
+        assert_within(o[rows], ro, HALF[BF] * ro.abs() + OUT_SLOP * m, f"o of sequence {b}")
+        for got in (S, S2):
+            assert_within(got[at], rs, HALF[FP32] * rs.abs() + STATE_SLOP * ms, f"state of sequence {b}")
+    others = [i for i in range(7) if i not in slots]
+    assert (dst[others] == 8).all() and torch.equal(src[others].cpu(), pool[others])
