@@ -51,6 +51,14 @@ __device__ __forceinline__ int length_of(const LaParams& p, int b, long* first =
   return (int)(e - a < p.T ? e - a : p.T);
 }
 
+__device__ __forceinline__ int uniform(int v) {
+#if __HIP_DEVICE_COMPILE__
+  return __builtin_amdgcn_readfirstlane(v);
+#else
+  return v;
+#endif
+}
+
 __device__ __forceinline__ float decay_of(const LaParams& p, int h) {
   const float g = p.log_decay[h];
   return (g < -1.0e4f ? -1.0e4f : g) * 1.4426950408889634f;     // (-inf, no memory at all, times a distance of 0 would be no number)
@@ -62,10 +70,11 @@ __device__ __forceinline__ bool unit_of(const LaParams& p, int b, int ht, int DK
   r.tile = ht % tiles;
   r.h = ht / tiles;
   r.b = b;
-  r.slot = p.slots ? p.slots[r.b] : r.b;
+  r.slot = p.slots ? uniform(p.slots[r.b]) : r.b;
   if (r.slot < 0 || r.slot >= p.n_slots) return false;
   long row = 0;
-  r.len = length_of(p, r.b, &row);
+  r.len = uniform(length_of(p, r.b, &row));
+  row = uniform((int)row);
   r.q0 = (long)r.b * p.bsq; r.k0 = (long)r.b * p.bsk; r.v0 = (long)r.b * p.bsv; r.o0 = (long)r.b * p.bso;
   if (p.seg_start) r.q0 = r.k0 = r.v0 = r.o0 = 0;
   const int hk = r.h / p.share;
@@ -97,8 +106,11 @@ __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
 typedef __attribute__((address_space(3))) void* lptr_t;
 typedef __amdgpu_buffer_rsrc_t rsrc_t;
 
-__device__ __forceinline__ void wait_all_loads() {
-  __builtin_amdgcn_s_waitcnt(0 | (7 << 4) | (15 << 8));   // vmcnt = 0, the other counters unconstrained (gfx9 encoding)
+// All loads and stores but the last VM are done (they end in the order of their issue).
+template <int VM = 0>
+__device__ __forceinline__ void wait_vm() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(VM | (7 << 4) | (15 << 8));   // the other counters unconstrained (gfx9 encoding)
   asm volatile("" ::: "memory");
 }
 __device__ __forceinline__ void barrier() {                // what this wave has written to LDS is there, and everybody has arrived
@@ -112,22 +124,31 @@ __device__ __forceinline__ void barrier() {                // what this wave has
 template <int W>
 struct Tile {
   static constexpr int PIECES = W / 8, ROW = W * 2, BYTES = C * ROW;
-  static __device__ __forceinline__ int swz(int row) { return row & (PIECES < 16 ? PIECES - 1 : 15); }
-  // rows 0 .. left-1 from src (rows behind them: zeros), NW waves
+  // Sixteen rows at one piece lie on all banks, and so do the four pieces of four rows in a row that a transposing read takes.
+  static __device__ __forceinline__ int swz(int row) { return (PIECES < 16 ? (row >> 1 & 1) << 2 : (row & 3) << 2) | (row >> 2 & 3); }
+  // Loads of a wave of NW, and what a lane's are from the first row (below 2^31: rows of 2^24 elements and more are refused).
   template <int NW>
-  static __device__ __forceinline__ void fetch(const bf16_t* src, long ld, int left, char* dst) {
-#if __HIP_DEVICE_COMPILE__
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16_t*>(src), 0, (int)(uint32_t)((((left < C ? left : C) - 1) * ld + W) * 2), 0x00020000);
+  struct Lanes {
+    static constexpr int N = BYTES / 1024 / NW;
+    uint32_t off[N];
+    __device__ __forceinline__ explicit Lanes(long ld) {
+      const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
-    for (int i = 0; i < BYTES / 1024 / NW; ++i) {
-      const int id = (wave * (BYTES / 1024 / NW) + i) * 64 + lane, row = id / PIECES, piece = (id % PIECES) ^ swz(row);
-      // (rows of 2^24 elements and more are refused, so offsets stay below 2^32; a row behind the last gets one that lies outside the buffer)
-      const uint32_t off = row < left ? (uint32_t)row * (uint32_t)ld * 2u + (uint32_t)piece * 16u : 0xfffffff0u;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lptr_t)(dst + (wave * (BYTES / 1024 / NW) + i) * 1024), 16, off, 0, 0, 0);
+      for (int i = 0; i < N; ++i) {
+        const int id = (wave * N + i) * 64 + lane, row = id / PIECES, piece = (id % PIECES) ^ swz(row);
+        off[i] = (uint32_t)row * (uint32_t)ld * 2u + (uint32_t)piece * 16u;
+      }
     }
+    // rows 0 .. left-1 from src; those behind them lie behind the buffer's end (ld >= W): zeros
+    __device__ __forceinline__ void fetch(const bf16_t* src, long ld, int left, char* dst) const {
+#if __HIP_DEVICE_COMPILE__
+      const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+      const rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16_t*>(src), 0, (int)(((uint32_t)((left < C ? left : C) - 1) * (uint32_t)ld + W) * 2), 0x00020000);
+#pragma unroll
+      for (int i = 0; i < N; ++i) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lptr_t)(dst + (wave * N + i) * 1024), 16, off[i], 0, 0, 0);
 #endif
-  }
+    }
+  };
   // where a lane (l = lane % 16, g = lane / 16) of an operand finds eight elements of row l from column 32 s + 8 g; rows 16 further lie 16 * ROW further
   static __device__ __forceinline__ int at8(int l, int g, int s) { return l * ROW + ((4 * s + g) ^ swz(l)) * 16; }
   // LDS addresses, for columns(), of row 8 (lane / 16) + (lane % 16) / 4 and of the row four further: a transposing read gives lane i of 16 the i-th element
@@ -145,25 +166,27 @@ struct Tile {
     }
 #endif
   }
-  // N operands whose lanes have the columns of tile t0 + n (N 2: t0 is even, columns in PAIRS) of rows 32 s + 8 (lane / 16) .. + 7, s = 0, 1.  The reads are written out, with their wait:
-  // in front of one of its own the compiler waits for every load that is on its way to LDS, the next block's among them.
-  // AT: bytes from the tile that `at` belongs to.
-  template <int N, int AT = 0>
+  // N operands whose lanes have the columns of tile t0 + n (N 4: t0 is a multiple of four, columns in PAIRS) of rows 32 s + 8 (lane / 16) .. + 7, s = 0, 1.  The reads are written out, with
+  // their wait: in front of one of its own the compiler waits for every load that is on its way to LDS, the next block's among them.
+  template <int N>
   static __device__ __forceinline__ void columns(const uint32_t (&at)[2], int t0, bf16x8 (&v)[N][2]) {
 #if __HIP_DEVICE_COMPILE__
-    static_assert(N == 1 || N == 2, "one or two tiles of columns");
+    static_assert(N == 1 || N == 4, "one or four tiles of columns");
     u32x2 r[N][4];
     const uint32_t a0 = at[0] ^ (uint32_t)(t0 << 5), b0 = at[1] ^ (uint32_t)(t0 << 5);
     if constexpr (N == 1) {
       asm volatile("ds_read_b64_tr_b16 %0, %4 offset:%7\n\tds_read_b64_tr_b16 %1, %5 offset:%7\n\tds_read_b64_tr_b16 %2, %4 offset:%6\n\tds_read_b64_tr_b16 %3, %5 offset:%6\n\t"
                    "s_waitcnt lgkmcnt(0)"
-                   : "=&v"(r[0][0]), "=&v"(r[0][1]), "=&v"(r[0][2]), "=&v"(r[0][3]) : "v"(a0), "v"(b0), "i"(AT + 32 * ROW), "i"(AT) : "memory");
+                   : "=&v"(r[0][0]), "=&v"(r[0][1]), "=&v"(r[0][2]), "=&v"(r[0][3]) : "v"(a0), "v"(b0), "i"(32 * ROW), "i"(0) : "memory");
     } else {
-      asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%13\n\tds_read_b64_tr_b16 %1, %9 offset:%13\n\tds_read_b64_tr_b16 %2, %8 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
-                   "ds_read_b64_tr_b16 %4, %8 offset:%11\n\tds_read_b64_tr_b16 %5, %9 offset:%11\n\tds_read_b64_tr_b16 %6, %8 offset:%10\n\tds_read_b64_tr_b16 %7, %9 offset:%10\n\t"
+      const uint32_t a1 = a0 ^ 64u, b1 = b0 ^ 64u;
+      asm volatile("ds_read_b64_tr_b16 %0, %16 offset:%21\n\tds_read_b64_tr_b16 %1, %17 offset:%21\n\tds_read_b64_tr_b16 %2, %16 offset:%20\n\tds_read_b64_tr_b16 %3, %17 offset:%20\n\t"
+                   "ds_read_b64_tr_b16 %4, %16 offset:%23\n\tds_read_b64_tr_b16 %5, %17 offset:%23\n\tds_read_b64_tr_b16 %6, %16 offset:%22\n\tds_read_b64_tr_b16 %7, %17 offset:%22\n\t"
+                   "ds_read_b64_tr_b16 %8, %18 offset:%21\n\tds_read_b64_tr_b16 %9, %19 offset:%21\n\tds_read_b64_tr_b16 %10, %18 offset:%20\n\tds_read_b64_tr_b16 %11, %19 offset:%20\n\t"
+                   "ds_read_b64_tr_b16 %12, %18 offset:%23\n\tds_read_b64_tr_b16 %13, %19 offset:%23\n\tds_read_b64_tr_b16 %14, %18 offset:%22\n\tds_read_b64_tr_b16 %15, %19 offset:%22\n\t"
                    "s_waitcnt lgkmcnt(0)"
-                   : "=&v"(r[0][0]), "=&v"(r[0][1]), "=&v"(r[0][2]), "=&v"(r[0][3]), "=&v"(r[1][0]), "=&v"(r[1][1]), "=&v"(r[1][2]), "=&v"(r[1][3])
-                   : "v"(a0), "v"(b0), "i"(AT + 8 + 32 * ROW), "i"(AT + 8), "i"(AT + 32 * ROW), "i"(AT) : "memory");
+                   : "=&v"(r[0][0]), "=&v"(r[0][1]), "=&v"(r[0][2]), "=&v"(r[0][3]), "=&v"(r[1][0]), "=&v"(r[1][1]), "=&v"(r[1][2]), "=&v"(r[1][3]), "=&v"(r[2][0]), "=&v"(r[2][1]), "=&v"(r[2][2]), "=&v"(r[2][3]), "=&v"(r[3][0]), "=&v"(r[3][1]), "=&v"(r[3][2]), "=&v"(r[3][3])
+                   : "v"(a0), "v"(b0), "v"(a1), "v"(b1), "i"(32 * ROW), "i"(0), "i"(8 + 32 * ROW), "i"(8) : "memory");
     }
 #pragma unroll
     for (int n = 0; n < N; ++n)
@@ -201,34 +224,45 @@ __device__ __forceinline__ void powers(float g, int n, float (&w)[2][8]) {
     }
 }
 
-// S = decay S + sum_j w_j k_j v_j^T over a block: V as the wave's columns, K in LDS AT bytes from the tile of `kcol`; decayed values in PIECES pieces of bf16.
-template <int DK, int TV, int PIECES, int AT>
-__device__ __forceinline__ void add_block(State<DK>& st, const bf16x8 (&raw)[2], const uint32_t (&kcol)[2], float decay, const float (&w)[2][8]) {
-  bf16x8 v[2][PIECES];
+// Two numbers' upper pieces of bf16, which are taken off them.
+__device__ __forceinline__ uint32_t take_pieces(float& x0, float& x1) {
+  const uint32_t h = pack_bf16x2(x0, x1);
+  x0 -= __uint_as_float(h << 16);
+  x1 -= __uint_as_float(h & 0xffff0000u);
+  return h;
+}
+
+// S = decay S + sum_j w_j k_j v_j^T over a block: V as the wave's columns, K in LDS; decayed values in two pieces of bf16, or three.
+template <int DK>
+__device__ __forceinline__ void add_block(State<DK>& st, const bf16x8 (&raw)[2], const uint32_t (&kcol)[2], float decay, const float (&w)[2][8], bool third) {
+  u32x4 v[3][2];
 #pragma unroll
   for (int s = 0; s < 2; ++s)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float x = (float)raw[s][e] * w[s][e];
-#pragma unroll
-      for (int i = 0; i < PIECES; ++i) {
-        v[s][i][e] = (bf16_t)x;
-        x -= (float)v[s][i][e];
-      }
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t two = __builtin_bit_cast(u32x4, raw[s])[e];
+      float x0 = __uint_as_float(two << 16) * w[s][2 * e], x1 = __uint_as_float(two & 0xffff0000u) * w[s][2 * e + 1];
+      v[0][s][e] = take_pieces(x0, x1);
+      v[1][s][e] = take_pieces(x0, x1);
+      v[2][s][e] = pack_bf16x2(x0, x1);
     }
 #pragma unroll
-  for (int t = 0; t < DK / 16; t += 2) {
-    bf16x8 k[2][2];
-    Tile<DK>::template columns<2, AT>(kcol, t, k);
+  for (int t = 0; t < DK / 16; t += 4) {
+    bf16x8 k[4][2];
+    Tile<DK>::template columns<4>(kcol, t, k);
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
+    for (int n = 0; n < 4; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) st.s[t + n][e] *= decay;
+    auto piece = [&](int i) {
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) st.s[t + n] = mfma(k[n][s], v[s][i], st.s[t + n]);
-    }
+        for (int n = 0; n < 4; ++n) st.s[t + n] = mfma(k[n][s], __builtin_bit_cast(bf16x8, v[i][s]), st.s[t + n]);   // (four sums in turn: a product waits for the one before it in its own)
+    };
+    piece(0);
+    piece(1);
+    if (third) piece(2);
   }
 }
 
@@ -332,9 +366,11 @@ __global__ __launch_bounds__(TV * 4) void la_gain(const LaParams p) {
   Unit u;
   if (!unit_of(p, b, ht, DK, TV, u)) return;
   const int t0 = ch.tail > 0 ? 0 : ch.block * C, t1 = t0 + (ch.tail > 0 ? ch.tail : -ch.tail) * C;     // (whole blocks: the sequence goes on)
-  auto fetch = [&](int c, int st) {
-    Tile<DK>::template fetch<NW>(p.k + u.k0 + (long)c * p.ldk, p.ldk, C, smem + st * STAGE);
-    Tile<TV>::template fetch<NW>(p.v + u.v0 + (long)c * p.ldv, p.ldv, C, smem + st * STAGE + Tile<DK>::BYTES);
+  const typename Tile<DK>::template Lanes<NW> kl(p.ldk);
+  const typename Tile<TV>::template Lanes<NW> vl(p.ldv);
+  auto fetch = [&](int c, int to) {
+    kl.fetch(p.k + u.k0 + (long)c * p.ldk, p.ldk, C, smem + to);
+    vl.fetch(p.v + u.v0 + (long)c * p.ldv, p.ldv, C, smem + to + Tile<DK>::BYTES);
   };
   fetch(t0, 0);
   State<DK> st;
@@ -348,18 +384,20 @@ __global__ __launch_bounds__(TV * 4) void la_gain(const LaParams p) {
   Tile<TV>::template column_rows<false>(smem + Tile<DK>::BYTES, vcol);
 #pragma unroll
   for (int h = 0; h < 2; ++h) vcol[h] ^= (uint32_t)(threadIdx.x >> 6) << 5;
-  auto block = [&](int c, auto stage_tag) {
-    constexpr int SO = decltype(stage_tag)::value * STAGE;
-    wait_all_loads();
+  for (int c = t0, st_at = 0; c < t1; c += C) {
+    wait_vm();
     barrier();                             // everybody's share of this block; and nobody reads the block before any more
-    if (c + C < t1) fetch(c + C, 1 - decltype(stage_tag)::value);
+    const int other = STAGE - st_at;
+    if (c + C < t1) fetch(c + C, other);
     bf16x8 vf[1][2];
-    Tile<TV>::template columns<1, SO>(vcol, 0, vf);
-    add_block<DK, TV, 3, SO>(st, vf[0], kcol, decay, w);
-  };
-  for (int c = t0; c < t1; c += 2 * C) {
-    block(c, std::integral_constant<int, 0>{});
-    if (c + C < t1) block(c + C, std::integral_constant<int, 1>{});
+    Tile<TV>::template columns<1>(vcol, 0, vf);
+    add_block<DK>(st, vf[0], kcol, decay, w, true);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      vcol[h] += other - st_at;
+      kcol[h] += other - st_at;
+    }
+    st_at = other;
   }
   float* ws = p.ws + ((long)ht * p.chunks + chunk) * (DK * TV);
 #pragma unroll
@@ -458,11 +496,13 @@ __global__ __launch_bounds__(TV * 4) __attribute__((amdgpu_waves_per_eu(2, 2))) 
     t1 = u.len - t0 <= left * (long)C ? u.len : t0 + left * C;
   }
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 15, grp = lane >> 4;
-  auto fetch = [&](int c, int st) {
-    char* to = smem + st * Sh::STAGE;
-    Tile<DK>::template fetch<NW>(p.k + u.k0 + (long)c * p.ldk, p.ldk, t1 - c, to);
-    Tile<DK>::template fetch<NW>(p.q + u.q0 + (long)c * p.ldq, p.ldq, t1 - c, to + Tile<DK>::BYTES);
-    Tile<TV>::template fetch<NW>(p.v + u.v0 + (long)c * p.ldv, p.ldv, t1 - c, to + 2 * Tile<DK>::BYTES);
+  const typename Tile<DK>::template Lanes<NW> kl(p.ldk), ql(p.ldq);
+  const typename Tile<TV>::template Lanes<NW> vl(p.ldv);
+  auto fetch = [&](int c, int stage) {
+    char* to = smem + stage;
+    kl.fetch(p.k + u.k0 + (long)c * p.ldk, p.ldk, t1 - c, to);
+    ql.fetch(p.q + u.q0 + (long)c * p.ldq, p.ldq, t1 - c, to + Tile<DK>::BYTES);
+    vl.fetch(p.v + u.v0 + (long)c * p.ldv, p.ldv, t1 - c, to + 2 * Tile<DK>::BYTES);
   };
   if (t0 < t1) fetch(t0, 0);
   State<DK> st;
@@ -509,15 +549,19 @@ __global__ __launch_bounds__(TV * 4) __attribute__((amdgpu_waves_per_eu(2, 2))) 
   const int p_to = (16 * it0 + l) * Sh::PP + (16 * j0 + 4 * grp) * 2, p_from = l * Sh::PP + grp * 16;
   // (a lane stores eight columns of one of two rows that are 16 apart)
   const int orow_at = l + 16 * (grp & 1);
-  auto row_of = [&]() { return p.o + u.o0 + (long)(t0 + orow_at) * p.ldo + wave * 16 + (grp >> 1) * 8; };
-  bf16_t* orow = row_of();
+  const uint32_t ocol = (wave * 16 + (grp >> 1) * 8) * 2;
   bool ends = ONE || t1 == u.len;          // the sequence, in this chunk
 
-  auto block = [&](int c, auto stage_tag) {
-    constexpr int SO = decltype(stage_tag)::value * Sh::STAGE, KT = SO, QT = SO + Tile<DK>::BYTES;
-    wait_all_loads();
+  bool first = true;                       // sequence of the chunk
+  int stage = 0;                           // the block's; a8, kcol and vcol lie in it
+  auto block = [&](int c) {
+    constexpr int KT = 0, QT = Tile<DK>::BYTES;
+    const int other = Sh::STAGE - stage;
+    if (c != t0) wait_vm<2>();             // (the outputs of the block before may still be on their way)
+    else if (first) wait_vm();
+    else wait_vm<DK / 4>();                // (or the state behind the sequence before: a store for each of a lane's numbers, behind this block's loads)
     barrier();                             // everybody's share of this block; and nobody reads the block before any more
-    if (c + C < t1) fetch(c + C, 1 - decltype(stage_tag)::value);
+    if (c + C < t1) fetch(c + C, other);
     {
       bf16x8 qf[DK / 32];
 #pragma unroll
@@ -531,44 +575,51 @@ __global__ __launch_bounds__(TV * 4) __attribute__((amdgpu_waves_per_eu(2, 2))) 
 #pragma unroll
           for (int s = 0; s < DK / 32; ++s) a = mfma(*reinterpret_cast<const bf16x8*>(smem + a8[s] + j0 * (16 * Tile<DK>::ROW) + JS * i * (16 * Tile<DK>::ROW) + KT), qf[s], a);
           const int m = it0 - jt;
-          const float f = m == 0 ? 1.f : m == 1 ? far[0] : m == 2 ? far[1] : far[2];
+          if (m == 0) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) a[r] = m == 0 && 4 * grp + r > l ? 0.f : a[r] * (m == 0 ? diag[r] : off[r] * f);   // (a later key may be no number)
+            for (int r = 0; r < 4; ++r) a[r] = 4 * grp + r > l ? 0.f : a[r] * diag[r];   // (a later key may be no number)
+          } else {
+            const float f = m == 1 ? far[0] : m == 2 ? far[1] : far[2];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) a[r] *= off[r] * f;
+          }
         }
-        bf16x4 hi, lo;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) { hi[r] = (bf16_t)a[r]; lo[r] = (bf16_t)(a[r] - (float)hi[r]); }
-        *reinterpret_cast<bf16x4*>(ph + p_to + JS * i * 32) = hi;
-        *reinterpret_cast<bf16x4*>(pl + p_to + JS * i * 32) = lo;
+        float x0 = a[0], x1 = a[1], x2 = a[2], x3 = a[3];
+        *reinterpret_cast<u32x2*>(ph + p_to + JS * i * 32) = u32x2{take_pieces(x0, x1), take_pieces(x2, x3)};
+        *reinterpret_cast<u32x2*>(pl + p_to + JS * i * 32) = u32x2{pack_bf16x2(x0, x1), pack_bf16x2(x2, x3)};
       }
     }
     // the state's share of the outputs of this wave's 16 columns: rows of the product 4 grp + r of them, columns i = 16 it + l
     f32x4 a[4];
     {
-      bf16x8 sh[DK / 32], sl[DK / 32];
+      u32x4 sh[DK / 32], sl[DK / 32];
 #pragma unroll
       for (int s = 0; s < DK / 32; ++s)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float x = st.s[2 * s + e / 4][e % 4];
-          sh[s][e] = (bf16_t)x;
-          sl[s][e] = (bf16_t)(x - (float)sh[s][e]);
+        for (int e = 0; e < 4; ++e) {
+          float x0 = st.s[2 * s + e / 2][2 * (e % 2)], x1 = st.s[2 * s + e / 2][2 * (e % 2) + 1];
+          sh[s][e] = take_pieces(x0, x1);
+          sl[s][e] = pack_bf16x2(x0, x1);
         }
 #pragma unroll
-      for (int it = 0; it < 4; ++it) {
-        a[it] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int it = 0; it < 4; ++it) a[it] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int s = 0; s < DK / 32; ++s) {
-          const bf16x8 qf = *reinterpret_cast<const bf16x8*>(smem + a8[s] + it * (16 * Tile<DK>::ROW) + QT);
-          a[it] = mfma(sh[s], qf, a[it]);
-          a[it] = mfma(sl[s], qf, a[it]);
-        }
+      for (int s = 0; s < DK / 32; ++s) {
+        bf16x8 qf[4];
+#pragma unroll
+        for (int it = 0; it < 4; ++it) qf[it] = *reinterpret_cast<const bf16x8*>(smem + a8[s] + it * (16 * Tile<DK>::ROW) + QT);
+#pragma unroll
+        for (int it = 0; it < 4; ++it) a[it] = mfma(__builtin_bit_cast(bf16x8, sh[s]), qf[it], a[it]);
+#pragma unroll
+        for (int it = 0; it < 4; ++it) a[it] = mfma(__builtin_bit_cast(bf16x8, sl[s]), qf[it], a[it]);
+      }
+#pragma unroll
+      for (int it = 0; it < 4; ++it)
 #pragma unroll
         for (int r = 0; r < 4; ++r) a[it][r] *= rise[it];
-      }
     }
     bf16x8 vf[1][2];
-    Tile<TV>::template columns<1, SO>(vcol, 0, vf);
+    Tile<TV>::template columns<1>(vcol, 0, vf);
     if (__ballot(not_finite(vf[0])) != 0) {  // their products with the zeros of earlier tokens would be no numbers: taken out, and their columns marked from there on
       int first = C;
 #pragma unroll
@@ -597,38 +648,43 @@ __global__ __launch_bounds__(TV * 4) __attribute__((amdgpu_waves_per_eu(2, 2))) 
     }
     barrier();                             // the scores
 #pragma unroll
-    for (int it = 0; it < 4; ++it) {
+    for (int s = 0; s < 2; ++s) {
 #pragma unroll
-      for (int s = 0; s <= it / 2; ++s) {
-        a[it] = mfma(vf[0][s], *reinterpret_cast<const bf16x8*>(ph + p_from + it * (16 * Sh::PP) + s * 64), a[it]);
-        a[it] = mfma(vf[0][s], *reinterpret_cast<const bf16x8*>(pl + p_from + it * (16 * Sh::PP) + s * 64), a[it]);
-      }
+      for (int it = 2 * s; it < 4; ++it) a[it] = mfma(vf[0][s], *reinterpret_cast<const bf16x8*>(ph + p_from + it * (16 * Sh::PP) + s * 64), a[it]);
+#pragma unroll
+      for (int it = 2 * s; it < 4; ++it) a[it] = mfma(vf[0][s], *reinterpret_cast<const bf16x8*>(pl + p_from + it * (16 * Sh::PP) + s * 64), a[it]);
     }
+#if __HIP_DEVICE_COMPILE__
+    const rsrc_t ro = __builtin_amdgcn_make_buffer_rsrc(p.o + u.o0 + (long)c * p.ldo, 0, (int)(uint32_t)((((t1 - c < C ? t1 - c : C) - 1) * p.ldo + TV) * 2), 0x00020000);
+#endif
 #pragma unroll
     for (int it = 0; it < 4; it += 2) {
       // a lane has four columns of row l of either tile; those of one tile and of the other trade places between the lanes of a pair of groups
 #if __HIP_DEVICE_COMPILE__
       const auto s0 = __builtin_amdgcn_permlane16_swap(pack_bf16x2(a[it][0], a[it][1]), pack_bf16x2(a[it + 1][0], a[it + 1][1]), false, false);
       const auto s1 = __builtin_amdgcn_permlane16_swap(pack_bf16x2(a[it][2], a[it][3]), pack_bf16x2(a[it + 1][2], a[it + 1][3]), false, false);
-      if (c + 16 * it + orow_at < t1) *reinterpret_cast<u32x4*>(orow + (long)(16 * it) * p.ldo) = u32x4{s0[0], s1[0], s0[1], s1[1]};
+      const int row = 16 * it + orow_at;     // (always a store: how many there are is what the next block's wait goes by)
+      __builtin_amdgcn_raw_buffer_store_b128(u32x4{s0[0], s1[0], s0[1], s1[1]}, ro, c + row < t1 ? (int)((uint32_t)row * (uint32_t)p.ldo * 2u + ocol) : (int)0xfffffff0u, 0, 0);
 #endif
     }
-    orow += (long)C * p.ldo;
-    if (ends) {
+    if (ends || c + C < t1) {
       if (t1 - c < C) {
         powers(u.g, t1 - c, w);
         decay = power(u.g, t1 - c);
       }
-      add_block<DK, TV, 3, SO>(st, vf[0], kcol, decay, w);
-    } else if (c + C < t1) {               // (a state that is taken no further here only makes outputs)
-      add_block<DK, TV, 2, SO>(st, vf[0], kcol, decay, w);
+      add_block<DK>(st, vf[0], kcol, decay, w, ends);   // (a state that is taken no further in the chunk only makes outputs)
     }
+#pragma unroll
+    for (int s = 0; s < DK / 32; ++s) a8[s] += other - stage;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      kcol[h] += other - stage;
+      vcol[h] += other - stage;
+    }
+    stage = other;
   };
   for (;;) {
-    for (int c = t0; c < t1; c += 2 * C) {
-      block(c, std::integral_constant<int, 0>{});
-      if (c + C < t1) block(c + C, std::integral_constant<int, 1>{});
-    }
+    for (int c = t0; c < t1; c += C) block(c);
     const Unit was = u;
     bool more = false;
     if constexpr (!ONE) {                  // the next sequence with tokens
@@ -639,7 +695,8 @@ __global__ __launch_bounds__(TV * 4) __attribute__((amdgpu_waves_per_eu(2, 2))) 
         t0 = 0;
         t1 = u.len <= left * (long)C ? u.len : left * C;
         barrier();                         // the stages are dead
-        fetch(0, 0);
+        fetch(0, stage);
+        asm volatile("" ::: "memory");     // (in front of the stores)
       }
     }
     if (ends)
@@ -650,8 +707,8 @@ __global__ __launch_bounds__(TV * 4) __attribute__((amdgpu_waves_per_eu(2, 2))) 
         for (int r = 0; r < 4; ++r) p.s_out[at + (long)r * p.dv] = st.s[t][r];
       }
     if (!more) break;
+    first = false;
     state_in();
-    orow = row_of();
     ends = t1 == u.len;
     powers(u.g, C, w);
     decay = power(u.g, C);
@@ -701,8 +758,10 @@ __global__ __launch_bounds__(256) void la_step(const LaParams p) {
 struct Plan { long heads; int tv, chunks; };      // heads: units of a sequence
 
 // 128 columns of v to a workgroup (which computes the scores once for them) where dv has them.
-// Chunks: a workgroup goes through its blocks one after the other (us a block as measured: 3.8 with dk 128, 2.3 with 64, whatever else runs), so few heads are
-// cut; but a chunk's state is written, read, written and read again, and the rounds that the workgroups make on 256 CUs are whole ones.
+// Chunks: a workgroup goes through its blocks one after the other (about 4 us a block with dk 128, 2.3 with 64, whatever else runs), so few heads are cut; but a
+// chunk's state is written, read, written and read again, and the rounds that the workgroups make on 256 CUs are whole ones.  Measured, us for whole sequences | 8 |
+// 16 | 24 | 32 chunks: 8 packed sequences of 1 .. 8192 tokens, 16384 in all, 16 heads of 128 458 | 194 | 122 | 148 | 136, one sequence of 16384 898 | 195 | 121 |
+// 148 | 137, 16 of 1024 81 | 150 | 92 | 154 | 133, 2 x 4096 tokens of 20 heads of 64 130 | 66 | 54 | 48 | 55, one of 1024 33 | 21 | 25 | 25 | 25.
 Plan plan_of(long B, long H, long dk, long dv, long T, long rows) {
   Plan r;
   r.tv = dv % 128 == 0 ? 128 : 64;
@@ -784,7 +843,7 @@ KH_EXPORT int kh_linear_attention_bf16(const void* q, const void* k, const void*
   if (T <= 0 || (seg_start && rows < 0)) return KH_ERR_INVALID_ARG;
   if (ldq < H * dk || ldk < kv_heads * dk || ldv < kv_heads * dv || ldo < H * dv) return KH_ERR_INVALID_ARG;
   if (T > (1L << 30)) return KH_ERR_TOO_LARGE;
-  if ((ldq | ldk | ldv) >= (1L << 24)) return KH_ERR_TOO_LARGE;
+  if ((ldq | ldk | ldv | ldo) >= (1L << 24)) return KH_ERR_TOO_LARGE;
   const Plan r = plan_of(B, H, dk, dv, T, seg_start ? (rows > 0 ? rows : 1) : B * T);
   p.chunks = r.chunks;
   if (p.chunks && !workspace) return KH_ERR_INVALID_ARG;
