@@ -281,20 +281,27 @@ struct LinParams {
   void* y;
   long M, N;
   int K, R, t_splits, row_bytes, gstride;
-  int dma;                 // rows of x are aligned to four bytes
+  int dma;                 // rows of x (and of A) are aligned to four bytes
+  const void* a_cat;       // few rows and a small A: every workgroup computes t by itself and keeps it in LDS from `t_at` on; else NULL
+  const float* col_scale;
+  int t_at;
 };
 
-// The rank-R product of a 16 x 16 tile in 32 bits, a step of 16 ranks: t [M][R] in `splits` parts, B_cat rows of T.
+// The rank-R product of a 16 x 16 tile in 32 bits, a step of 16 ranks: t from LDS, or [M][R] in `splits` parts, B_cat rows of T.
 template <typename T>
-__device__ __forceinline__ f32x4 rank_step(const LinParams& p, long m, long n, int r, f32x4 acc) {
-  const float* tr = p.t + m * p.R + r;
-  const long part = p.M * p.R;
+__device__ __forceinline__ f32x4 rank_step(const LinParams& p, const float* own, long m, long n, int r, f32x4 acc) {
   f32x4 t = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int sp = 0; sp < p.t_splits; sp += 4) {      // four on their way at a time, added in order
-    f32x4 v[4];
+  if (own) {
+    t = *reinterpret_cast<const f32x4*>(own);
+  } else {
+    const float* tr = p.t + m * p.R + r;
+    const long part = p.M * p.R;
+    for (int sp = 0; sp < p.t_splits; sp += 4) {      // four on their way at a time, added in order
+      f32x4 v[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = sp + i < p.t_splits ? *reinterpret_cast<const f32x4*>(tr + (sp + i) * part) : f32x4{0.f, 0.f, 0.f, 0.f};
-    t = (((t + v[0]) + v[1]) + v[2]) + v[3];
+      for (int i = 0; i < 4; ++i) v[i] = sp + i < p.t_splits ? *reinterpret_cast<const f32x4*>(tr + (sp + i) * part) : f32x4{0.f, 0.f, 0.f, 0.f};
+      t = (((t + v[0]) + v[1]) + v[2]) + v[3];
+    }
   }
   T b[4];
   __builtin_memcpy(b, (const T*)p.b_cat + n * p.R + r, sizeof(b));
@@ -327,6 +334,81 @@ struct Stage {
   static constexpr int P = NB + X + S + Z;
   static constexpr int WAT = 0, XAT = NB * 1024, SAT = XAT + X * 1024, ZAT = SAT + S * 256, BYTES = ZAT + Z * 256;
 };
+
+// t = (x A^T) * col_scale of up to 16 rows and RT tiles of 16 ranks into `tl`: a wave takes every LW-th step of 32 k, OWN_DEEP - 1 on their way ahead of the one that
+// is multiplied (as below, in a part of LDS of its own), and the waves are summed in order.
+constexpr int OWN_DEEP = 3, OWN_PITCH = 64 + 4;                 // of tl
+constexpr int own_wave(int rt) { return OWN_DEEP * (1 + rt) * 1024; }
+template <typename T, int LW, int RT>
+__device__ __forceinline__ void own_ranks(const LinParams& p, const T* x0, int rows, char* smem, float* tl) {
+#if __HIP_DEVICE_COMPILE__
+  constexpr int UNIT = (1 + RT) * 1024, R = RT * 16;            // a tile of x and those of A, 1 KB each
+  static_assert(16 * (R + 1) * 4 <= OWN_DEEP * UNIT && R <= OWN_PITCH - 4, "a wave's sums");
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int l = lane & 15, g = lane >> 4, dr = lane >> 2, dp = lane & 3, from = (l * 4 + g) * 16;
+  const T* a0 = (const T*)p.a_cat;
+  const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(x0), 0, (int)(rows * p.K * 2), 0x00020000);
+  const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(a0), 0, (int)(R * p.K * 2), 0x00020000);
+  const int xo = ((dr < rows ? dr : rows - 1) * p.K + dp * 8) * 2, ao = (dr * p.K + dp * 8) * 2;
+  const int steps = (p.K + 31) / 32, full = p.dma ? p.K / 32 : 0, mine = wave < full ? (full - 1 - wave) / LW + 1 : 0;
+  char* const here = smem + wave * own_wave(RT);
+  f32x4 acc[RT];
+#pragma unroll
+  for (int j = 0; j < RT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto fetch = [&](int i, int st) {
+    const int kb = (wave + i * LW) * 64;
+    char* to = here + st * UNIT;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lptr_t)to, 16, xo, kb, 0, 0);
+#pragma unroll
+    for (int j = 0; j < RT; ++j) __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lptr_t)(to + 1024 + j * 1024), 16, ao, j * 32 * p.K + kb, 0, 0);
+  };
+  auto use = [&](int st) {
+    const char* at = here + st * UNIT + from;
+    const u32x4 x = *reinterpret_cast<const u32x4*>(at);
+#pragma unroll
+    for (int j = 0; j < RT; ++j) acc[j] = Num<T>::mfma(x, *reinterpret_cast<const u32x4*>(at + 1024 + j * 1024), acc[j]);
+  };
+  if (mine > 0) fetch(0, 0);
+  if (mine > 1) fetch(1, 1);
+  int st = 0, i = 0;
+  auto next = [&]() { st = st == 2 ? 0 : st + 1; };
+  for (; i + 2 < mine; ++i) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");          // the step before has been read; its place is the next one's
+    fetch(i + 2, st == 0 ? 2 : st - 1);
+    wait_vm<2 * (1 + RT)>();
+    use(st);
+    next();
+  }
+  if (i + 1 < mine) { wait_vm<1 + RT>(); use(st); next(); ++i; }
+  if (i < mine) { wait_vm<0>(); use(st); }
+  for (int ks = full + (wave - full % LW + LW) % LW; ks < steps; ks += LW) {     // the end of the rows, or rows that are not aligned to four bytes
+    const int k = ks * 32 + g * 8;
+    T v[8];
+    load8<T>(x0 + (long)(l < rows ? l : rows - 1) * p.K + k, (long)p.K - k, v);
+    const u32x4 x = __builtin_bit_cast(u32x4, v);
+#pragma unroll
+    for (int j = 0; j < RT; ++j) {
+      load8<T>(a0 + (long)(j * 16 + l) * p.K + k, (long)p.K - k, v);
+      acc[j] = Num<T>::mfma(x, __builtin_bit_cast(u32x4, v), acc[j]);
+    }
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  float* part = reinterpret_cast<float*>(here);
+#pragma unroll
+  for (int j = 0; j < RT; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) part[(g * 4 + e) * (R + 1) + j * 16 + l] = acc[j][e];
+  __syncthreads();
+  for (int id = threadIdx.x; id < rows * R; id += LW * 64) {
+    const int r = id / R, c = id % R;
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < LW; ++w) v += reinterpret_cast<const float*>(smem + w * own_wave(RT))[r * (R + 1) + c];
+    tl[r * OWN_PITCH + c] = v * p.col_scale[c];
+  }
+  __syncthreads();
+#endif
+}
 
 // A few rows: NB * 16 columns of y (rows of codes) and MB * 16 rows of x to a workgroup.  Its LW waves take every LW-th block of 128 codes and are
 // summed in order at the end.  A wave's blocks go straight to a ring of ST of its own in LDS, ST - 1 ahead of the one that is multiplied: nobody else
@@ -427,6 +509,12 @@ __global__ __launch_bounds__(LW * 64) void w4_few_rows(const LinParams p) {
   const int full = p.dma ? p.K / 128 : 0, blocks = (p.row_bytes + 63) / 64;
   const int mine = wave < full ? (full - 1 - wave) / LW + 1 : 0;   // whole blocks of this wave
   char* ring = smem + wave * (ST * Sg::BYTES);
+  float* const tl = reinterpret_cast<float*>(smem + p.t_at);
+  if constexpr (MB == 1)
+    if (p.a_cat) {
+      if (p.R == 32) own_ranks<T, LW, 2>(p, x0, rows, smem, tl);
+      else own_ranks<T, LW, 4>(p, x0, rows, smem, tl);
+    }
   auto bytes = [](long n) { return (int)(uint32_t)(n < 0xffffffffL ? n : 0xffffffffL); };
   const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(q0), 0, bytes((p.N - n0) * p.row_bytes), 0x00020000);
   const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(x0), 0, bytes((p.M - m0) * p.K * 2), 0x00020000);
@@ -486,7 +574,7 @@ __global__ __launch_bounds__(LW * 64) void w4_few_rows(const LinParams p) {
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
           const long n = n0 + j * 16 + l;
-          out[b][j] = rank_step<T>(p, m0 + xm[b], n < p.N ? n : p.N - 1, r + 4 * g, out[b][j]);
+          out[b][j] = rank_step<T>(p, MB == 1 && p.a_cat ? tl + xm[b] * OWN_PITCH + r + 4 * g : nullptr, m0 + xm[b], n < p.N ? n : p.N - 1, r + 4 * g, out[b][j]);
         }
     int i = 0;
     for (; i + ST - 1 < mine; ++i) {
@@ -891,6 +979,12 @@ __global__ __launch_bounds__(SW * 64) void w4_shrink(const ShrinkParams p) {
   }
 }
 
+// Few rows with a small A: t is computed by every workgroup for itself, which reads all of A from its L2, and a launch (another 4 us of the host's) and its workspace
+// are gone.  On the GPU, us in one launch | in two: one row 1280 x 640 with rank 64 5.0 | 5.6, 1280 x 1280 with 32 5.3 | 6.3 and with 64 6.5 | 6.7, 1280 x 2560 with 32
+// 7.0 | 7.8, 10240 x 640 with 64 7.0 | 8.8, 65536 x 1280 with 32 31.6 | 31.9; 16 rows 1280 x 1280 with 64 7.4 | 7.7; beyond: one row 1280 x 4096 with 32 9 | 8.2,
+// 1280 x 1280 with 96 8.5 | 6.9.
+bool own_t(long M, long K, long R) { return (R == 32 || R == 64) && M <= 16 && R * K <= 80 << 10; }
+
 int shrink_splits(long M, long K, long R) {
   // enough workgroups that the rows of A are read by many CUs at once, at least 512 of k each (two steps of a wave)
   const long tiles = R / 16 * ((M + 15) / 16);
@@ -902,9 +996,12 @@ int shrink_splits(long M, long K, long R) {
 }
 
 template <typename T, int G, bool ZERO, int MB, int NB, int LW, int ST, bool FOUR>
-int launch_few_as(const LinParams& p, hipStream_t s) {
+int launch_few_as(LinParams p, hipStream_t s) {
   const long mt = (p.M + MB * 16 - 1) / (MB * 16), rows = p.M < MB * 16 ? p.M : MB * 16;
-  const int ring = LW * ST * Stage<G, ZERO, MB, NB, FOUR>::BYTES, part = LW * (int)rows * (NB * 16 + 1) * 4, lds = ring > part ? ring : part;
+  const int ring = LW * ST * Stage<G, ZERO, MB, NB, FOUR>::BYTES, part = (LW * (int)rows * (NB * 16 + 1) * 4 + 15) / 16 * 16;
+  const int own = p.a_cat ? LW * own_wave(p.R / 16) : 0, most = ring > part ? ring : part;
+  p.t_at = own > most ? own : most;
+  const int lds = p.t_at + (p.a_cat ? 16 * OWN_PITCH * 4 : 0);
   if (lds > 65536) {
     const hipError_t e = kh_allow_lds<w4_few_rows<T, G, ZERO, MB, NB, LW, ST, FOUR>>(lds);
     if (e != hipSuccess) return (int)e;
@@ -1009,21 +1106,22 @@ KH_EXPORT int kh_dequantize_w4(const void* q, const void* scale, const void* zer
 
 KH_EXPORT int64_t kh_w4_linear_workspace_bytes(int64_t M, int64_t K, int64_t R) {
   if (M <= 0 || K <= 0 || R < 0 || R % 32 != 0 || R > 128) return KH_ERR_INVALID_ARG;
-  return R == 0 ? 0 : (int64_t)shrink_splits(M, K, R) * M * R * 4;
+  return R == 0 || own_t(M, K, R) ? 0 : (int64_t)shrink_splits(M, K, R) * M * R * 4;
 }
 
 KH_EXPORT int kh_w4_linear(const void* x, const void* q, const void* scale, const void* zero, const void* bias, const void* a_cat,
                            const void* b_cat, const float* col_scale, const void* residual, void* y, void* workspace, int64_t M, int64_t N,
                            int64_t K, int64_t R, int64_t group, int type, void* stream) {
   if (!x || !q || !scale || !y || M <= 0 || N <= 0 || K <= 0 || R < 0 || type < 0 || type > 1) return KH_ERR_INVALID_ARG;
-  if (R > 0 && (!a_cat || !b_cat || !col_scale || !workspace)) return KH_ERR_INVALID_ARG;
+  const bool own = own_t(M, K, R);
+  if (R > 0 && (!a_cat || !b_cat || !col_scale || (!workspace && !own))) return KH_ERR_INVALID_ARG;
   if (!group_ok(group) || R % 32 != 0) return KH_ERR_UNSUPPORTED;
   if (R > 128 || K > (1L << 24) || N > (1L << 24) || (M + 15) / 16 > 65535) return KH_ERR_TOO_LARGE;
   if (!kh_aligned16(q) || ((uintptr_t)scale & 7) || ((uintptr_t)zero & 3)) return KH_ERR_ALIGNMENT;   // (any whole rows of larger ones)
   hipStream_t s = (hipStream_t)stream;
   const bool many = many_rows(M, N, K);
   const int splits = R == 0 ? 0 : many ? 1 : shrink_splits(M, K, R);
-  if (R > 0) {
+  if (R > 0 && !own) {
     const int per = (int)(((K + splits - 1) / splits + 31) / 32 * 32);
     ShrinkParams sp{x, a_cat, col_scale, (float*)workspace, (long)M, (int)K, (int)R, per, many};
     const dim3 grid((unsigned)(R / 16), (unsigned)((M + 15) / 16), (unsigned)splits);
@@ -1034,7 +1132,7 @@ KH_EXPORT int kh_w4_linear(const void* x, const void* q, const void* scale, cons
   }
   LinParams p{x, (const uint8_t*)q, (const bf16_t*)scale, (const uint8_t*)zero, bias, b_cat, residual, (const float*)workspace, y, (long)M,
               (long)N, (int)K, (int)R, splits, (int)((K + 31) / 32 * 16), (int)(((K + group - 1) / group + 3) / 4 * 4),
-              ((uintptr_t)x & 3) == 0 && K % 2 == 0};
+              ((uintptr_t)x & 3) == 0 && K % 2 == 0 && (!own || ((uintptr_t)a_cat & 3) == 0), own ? a_cat : nullptr, col_scale, 0};
   const int rc = type == 0 ? launch_linear<bf16_t>(p, (int)group, s) : launch_linear<_Float16>(p, (int)group, s);
   if (rc != KH_OK) return rc;
   KH_RETURN_LAST_ERROR();

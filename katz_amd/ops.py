@@ -1510,7 +1510,8 @@ def w4_linear(x: torch.Tensor, w: W4Weight, bias: Optional[torch.Tensor] = None,
         nbytes = _workspace_bytes("kh_w4_linear_workspace_bytes", M, K, R)
         if nbytes < 0:
             raise ValueError(f"the adapters' columns must be a multiple of 32 up to 128, got {R}")
-        ws = x.new_empty(nbytes // 2)          # (elements of two bytes)
+        if nbytes:
+            ws = x.new_empty(nbytes // 2)      # (elements of two bytes)
     rc = lib.kh_w4_linear(x.data_ptr(), q.data_ptr(), w.scale.data_ptr(), _ptr(w.zero), _ptr(bias), _ptr(a_cat), _ptr(b_cat), _ptr(col_scale),
                           _ptr(residual), out.data_ptr(), _ptr(ws), M, N, K, R, w.group, _TYPES[dt], _stream())
     if rc:

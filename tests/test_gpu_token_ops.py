@@ -295,6 +295,14 @@ LINEAR_CASES = [
     (2, 40, 20000, 128, True, 128, False, False, FP16),    # many blocks to a wave
     (30, 8300, 514, 64, True, 32, False, True, BF),
     (20, 5000, 1536, 128, False, 0, True, False, FP16),
+    # few rows whose rank products begin in the same launch
+    (16, 200, 1279, 64, False, 64, False, True, BF),
+    (6, 700, 33, 32, True, 32, True, False, FP16),
+    (1, 64, 1280, 64, False, 64, False, False, BF),
+    (4, 8400, 1000, 128, True, 64, True, False, FP16),
+    (12, 5000, 31, 32, False, 64, False, True, BF),
+    (16, 9000, 640, 64, True, 32, False, False, FP16),
+    (3, 40, 2560, 128, False, 32, True, True, BF),
     # many rows
     (130, 8200, 200, 64, False, 32, True, True, BF),
     (1100, 2050, 385, 32, True, 96, True, True, FP16),
@@ -339,6 +347,24 @@ def test_w4_linear(case):
     if res is not None:
         buf = on(res)
         assert torch.equal(ops.w4_linear(on(x), w, on(b), on(A), on(B), on(c), residual=buf, out=buf), y)
+
+
+@pytest.mark.parametrize("M,R", [(3, 32), (16, 64), (5, 96), (40, 64)])
+def test_w4_linear_of_operands_at_any_address(M, R):
+    from katz_amd import ops
+
+    g = gen(18)
+    w = ops.quantize_w4(on(randn(g, 100, 640, std=0.05)), 64)
+    x, A, B, c = randn(g, M, 640), randn(g, R, 640, std=0.05), randn(g, 100, R, std=0.05), torch.rand(R, generator=g)
+
+    def moved(t, by):                                       # a contiguous copy `by` elements behind an allocation's start
+        return torch.cat([torch.zeros(by, dtype=t.dtype), t.flatten()]).to(DEV)[by:].view(t.shape)
+
+    y = ops.w4_linear(on(x), w, None, on(A), on(B), on(c))
+    for dx, da, db in ((1, 0, 0), (0, 1, 1), (0, 3, 2), (5, 2, 0)):
+        got = ops.w4_linear(moved(x, dx), w, None, moved(A, da), moved(B, db), on(c))
+        bound = 2 * HALF[BF] * y.cpu().to(F64).abs() + LINEAR_SLOP * 64          # (blocks on other paths: sums in another order, magnitudes below 64)
+        assert_within(got, y.cpu().to(F64), bound, f"moved by {dx}, {da}, {db}")
 
 
 def test_w4_linear_reads_only_its_rows():

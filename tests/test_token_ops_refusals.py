@@ -43,11 +43,11 @@ def test_w4_entry_points(lib):
         return lib.kh_w4_linear(x, q, s, None, None, a, b, c, None, y, ws, M, N, K, R, g, t, None)
 
     assert linear(x=None) == -1 and linear(y=None) == -1 and linear(M=0) == -1 and linear(N=-1) == -1 and linear(t=2) == -1
-    assert linear(R=32) == -1 and linear(R=32, a=16, b=16, c=16) == -1          # operands, workspace missing
+    assert linear(R=32) == -1 and linear(R=32, a=16, b=16, c=16, K=8192) == -1          # operands, workspace missing
     assert linear(R=40, a=16, b=16, c=16, ws=16) == -2 and linear(R=160, a=16, b=16, c=16, ws=16) == -4
     assert linear(g=48) == -2 and linear(q=4) == -3 and linear(M=1 << 21) == -4
     size = lib.kh_w4_linear_workspace_bytes
-    assert size(4, 1280, 0) == 0 and size(4, 1280, 64) >= 4 * 64 * 4 and size(4, 1280, 48) == -1 and size(0, 1280, 32) == -1 and size(1, 64, 160) == -1
+    assert size(4, 1280, 0) == 0 and size(4, 1280, 64) == 0 and size(4, 8192, 64) >= 4 * 64 * 4 and size(40, 1280, 64) >= 40 * 64 * 4 and size(4, 1280, 48) == -1 and size(0, 1280, 32) == -1 and size(1, 64, 160) == -1
 
 
 def test_linear_attention_entry_points(lib):
