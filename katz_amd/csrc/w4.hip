@@ -285,6 +285,8 @@ struct LinParams {
   const void* a_cat;       // few rows and a small A: every workgroup computes t by itself and keeps it in LDS from `t_at` on; else NULL
   const float* col_scale;
   int t_at;
+  int b_dma;               // B_cat is aligned to four bytes
+  int once;                // y is larger than the caches: stored past them
 };
 
 // The rank-R product of a 16 x 16 tile in 32 bits, a step of 16 ranks: t from LDS, or [M][R] in `splits` parts, B_cat rows of T.
@@ -816,105 +818,141 @@ __global__ __launch_bounds__(MR_W * 64) __attribute__((amdgpu_waves_per_eu(2, 2)
   // place of the rows would ask few channels (616 x 10240 x 1280 38.0 -> 35.0 us).
   const int rot = (int)((unit / mt) * 5 % (uint32_t)blocks);
   auto turned = [&](int i) { return i + rot < blocks ? i + rot : i + rot - blocks; };
-  fetch(turned(0), 0);
-  if (blocks > 1) fetch(turned(1), 1);
-  // the adapters while the first blocks are on their way: t lies in two pieces of bf16, B_cat is exact in one (fp16: in two)
+  // The adapters' product, 32 ranks at a time, comes first through the same stages: t in two pieces of bf16 in the place of x, B_cat in the place of the codes.
   const bf16_t* th = (const bf16_t*)p.t;
-  struct Ranks { u32x4 b[MR_N], hi[MR_M], lo[MR_M]; } ra, rb;
-  auto ranks_in = [&](int r, Ranks& o) {
+  const int steps = p.R / 32, all = steps + blocks;
+  const __amdgpu_buffer_rsrc_t rt = __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16_t*>(th + m0 * p.R), 0, bytes((2 * p.M - m0) * p.R * 2), 0x00020000);
+  const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>((const T*)p.b_cat + nb * p.R), 0, bytes((p.N - nb) * p.R * 2), 0x00020000);
+  auto fetch_ranks = [&](int step, int st) {
+    char* to = smem + st * Sg::BYTES;
 #pragma unroll
-    for (int j = 0; j < MR_N; ++j)
-      __builtin_memcpy(&o.b[j], (const T*)p.b_cat + (nb + (j * 16 + l < (int)last ? j * 16 + l : (int)last)) * p.R + r + g * 8, 16);
-#pragma unroll
-    for (int b = 0; b < MR_M; ++b) {
-      const int r0 = b * 16 + l;
-      const bf16_t* at = th + (m0 + (r0 < rows ? r0 : rows - 1)) * p.R + r + g * 8;
-      o.hi[b] = *reinterpret_cast<const u32x4*>(at);
-      o.lo[b] = *reinterpret_cast<const u32x4*>(at + p.M * p.R);
+    for (int i = 0; i < (2 * MR_M + MR_W - 1) / MR_W; ++i) {
+      const int id = wave + i * MR_W, r = (id >> 1) * 16 + dr;
+      if (id < 2 * MR_M)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rt, (lptr_t)(to + Sg::XAT + id * 1024), 16, (int)(((uint32_t)(r < rows ? r : rows - 1) * (uint32_t)p.R + dp * 8) * 2),
+                                                 (int)((uint32_t)((id & 1) * p.M * p.R + step * 32) * 2), 0, 0);
     }
-  };
-  auto ranks = [&](const Ranks& o) {
 #pragma unroll
     for (int j = 0; j < MR_N; ++j) {
-      bf16x8 bh, bl;
-      T v[8];
-      __builtin_memcpy(v, &o.b[j], 16);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        bh[e] = (bf16_t)(float)v[e];
-        bl[e] = (bf16_t)((float)v[e] - (float)bh[e]);
-      }
-#pragma unroll
-      for (int b = 0; b < MR_M; ++b) {
-        out[b][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, o.hi[b]), bh, out[b][j], 0, 0, 0);
-        out[b][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, o.lo[b]), bh, out[b][j], 0, 0, 0);
-        if constexpr (!__is_same(T, bf16_t)) out[b][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, o.hi[b]), bl, out[b][j], 0, 0, 0);
+      char* at = to + Sg::WAT + (wave * MR_N + j) * 1024;
+      if (p.b_dma) {
+        const uint32_t r = j * 16 + dr;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lptr_t)at, 16, (int)(((r < last ? r : last) * (uint32_t)p.R + dp * 8) * 2), step * 64, 0, 0);
+      } else {
+        const uint32_t r = j * 16 + l;
+        u32x4 v;
+        __builtin_memcpy(&v, (const T*)p.b_cat + (nb + (r < last ? r : last)) * p.R + step * 32 + g * 8, 16);
+        *reinterpret_cast<u32x4*>(at + from) = v;
       }
     }
   };
-  if (p.R > 0) ranks_in(0, ra);
-  for (int r = 0; r < p.R; r += 64) {
-    if (r + 32 < p.R) ranks_in(r + 32, rb);
-    asm volatile("" ::: "memory");
-    ranks(ra);
-    if (r + 64 < p.R) ranks_in(r + 64, ra);
-    asm volatile("" ::: "memory");
-    if (r + 32 < p.R) ranks(rb);
-  }
+  auto multiply_ranks = [&](int st) {
+    const char* at = smem + st * Sg::BYTES;
+    u32x4 hi[MR_M], lo[MR_M];
+#pragma unroll
+    for (int b = 0; b < MR_M; ++b) {
+      hi[b] = *reinterpret_cast<const u32x4*>(at + Sg::XAT + 2 * b * 1024 + from);
+      lo[b] = *reinterpret_cast<const u32x4*>(at + Sg::XAT + (2 * b + 1) * 1024 + from);
+    }
+#pragma unroll
+    for (int j = 0; j < MR_N; ++j) {
+      const u32x4 raw = *reinterpret_cast<const u32x4*>(at + Sg::WAT + (wave * MR_N + j) * 1024 + from);
+      bf16x8 bh = __builtin_bit_cast(bf16x8, raw), bl;
+      if constexpr (!__is_same(T, bf16_t)) {       // (fp16 in two pieces)
+        T v[8];
+        __builtin_memcpy(v, &raw, 16);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          bh[e] = (bf16_t)(float)v[e];
+          bl[e] = (bf16_t)((float)v[e] - (float)bh[e]);
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < MR_M; ++b) out[b][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, hi[b]), bh, out[b][j], 0, 0, 0);
+#pragma unroll
+      for (int b = 0; b < MR_M; ++b) out[b][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, lo[b]), bh, out[b][j], 0, 0, 0);
+      if constexpr (!__is_same(T, bf16_t))
+#pragma unroll
+        for (int b = 0; b < MR_M; ++b) out[b][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, hi[b]), bl, out[b][j], 0, 0, 0);
+    }
+  };
+  auto fetch_any = [&](int i, int st) {
+    if (i < steps) fetch_ranks(i, st);
+    else fetch(turned(i - steps), st);
+  };
+  fetch_any(0, 0);
+  if (all > 1) fetch_any(1, 1);
   wait_vm<0>();
   barrier();
-  sums(0, 0);
-  for (int kb = 0, st = 0; kb < blocks; ++kb) {
-    const int s1 = st == MR_ST - 1 ? 0 : st + 1, s2 = s1 == MR_ST - 1 ? 0 : s1 + 1;
+  if (steps == 0) sums(0, 0);
+  int st = 0;
+  auto after = [](int st) { return st == MR_ST - 1 ? 0 : st + 1; };
+  for (int i = 0; i < steps; ++i) {
     wait_vm<0>();                             // this wave's share of the next block, requested a block ago
-    barrier();                                // everybody's; this block's sums; and nobody reads the block before any more
-    if (kb + 2 < blocks) fetch(turned(kb + 2), s2);
+    barrier();                                // everybody's; and nobody reads the block before any more
+    if (i + 2 < all) fetch_any(i + 2, after(after(st)));
+    if (i + 1 == steps) sums(after(st), 0);
+    multiply_ranks(st);
+    st = after(st);
+  }
+  for (int kb = 0; kb < blocks; ++kb) {
+    const int s1 = after(st);
+    wait_vm<0>();
+    barrier();                                // (and this block's sums)
+    if (kb + 2 < blocks) fetch(turned(kb + 2), after(s1));
     if (kb + 1 < blocks) sums(s1, (kb + 1) & 1);
     multiply(turned(kb), st, kb & 1);
     st = s1;
   }
+  // Outputs by way of LDS to whole rows of 768 bytes: 48 lanes of eight columns, a wave has every eighth row.  What is added to them is asked for all at once, before.
+  constexpr int ROWS = MR_M * 16 / MR_W, LANES = MR_W * MR_N * 2;
+  static_assert(ROWS * MR_W == MR_M * 16 && LANES <= 64, "a row to a wave");
+  const long n = n0 - wave * (MR_N * 16) + lane * 8;
+  const bool mine = lane < LANES && n < p.N, vec = n + 8 <= p.N;
+  float bias[8];
+  T res[ROWS][8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) bias[e] = mine && p.bias && n + e < p.N ? (float)((const T*)p.bias)[n + e] : 0.f;
+  if (mine && p.residual)
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i)
+      if (wave + i * MR_W < rows) load8<T>((const T*)p.residual + (m0 + wave + i * MR_W) * p.N + n, p.N - n, res[i]);
   barrier();                                  // the stages are dead
-  float* mine = reinterpret_cast<float*>(smem) + wave * (MR_M * 16 * Sg::PITCH);
+  float* part = reinterpret_cast<float*>(smem);
 #pragma unroll
   for (int b = 0; b < MR_M; ++b)
 #pragma unroll
     for (int j = 0; j < MR_N; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) mine[(b * 16 + g * 4 + e) * Sg::PITCH + j * 16 + l] = out[b][j][e];
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");         // (written and read by this wave alone)
-  if (!some) return;
-  constexpr int PIECES = MR_N * 2, AT_ONCE = 64 / PIECES;    // a lane's eight columns of ten rows at a time
-  const int c = lane % PIECES * 8;
-  if (lane >= PIECES * AT_ONCE) return;
-  const long n = n0 + c;
-  float bias[8];
+      for (int e = 0; e < 4; ++e) part[(wave * (MR_M * 16) + b * 16 + g * 4 + e) * Sg::PITCH + j * 16 + l] = out[b][j][e];
+  barrier();
+  if (!mine) return;
+  const float* from_lane = part + lane / (MR_N * 2) * (MR_M * 16 * Sg::PITCH) + lane % (MR_N * 2) * 8;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) bias[e] = p.bias && n + e < p.N ? (float)((const T*)p.bias)[n + e] : 0.f;
-  const bool vec = n + 8 <= p.N;
-  for (int r = lane / PIECES; r < rows; r += AT_ONCE) {
-    float v[8];
-#pragma unroll
-    for (int e = 0; e < 8; e += 4) {
-      const f32x4 t = *reinterpret_cast<const f32x4*>(mine + r * Sg::PITCH + c + e);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[e + i] = t[i] + bias[e + i];
-    }
-    const long at = (m0 + r) * p.N + n;
-    if (p.residual) {
-      T res[8];
-      load8<T>((const T*)p.residual + at, p.N - n, res);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] += (float)res[e];
-    }
+  for (int i = 0; i < ROWS; ++i) {
+    const int r = wave + i * MR_W;
+    if (r >= rows) break;
     T o[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = (T)v[e];
-    if (vec) {
-      __builtin_memcpy((T*)p.y + at, o, sizeof(o));
+    for (int e = 0; e < 8; e += 4) {
+      const f32x4 t = *reinterpret_cast<const f32x4*>(from_lane + r * Sg::PITCH + e);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float v = t[k] + bias[e + k];
+        o[e + k] = (T)(p.residual ? v + (float)res[i][e + k] : v);
+      }
+    }
+    T* to = (T*)p.y + (m0 + r) * p.N + n;
+    if (vec && p.once && ((uintptr_t)to & 15) == 0) {
+      u32x4 t;
+      __builtin_memcpy(&t, o, sizeof(t));
+      __builtin_nontemporal_store(t, reinterpret_cast<u32x4*>(to));
+    } else if (vec) {
+      __builtin_memcpy(to, o, sizeof(o));
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (n + e < p.N) ((T*)p.y)[at + e] = o[e];
+        if (n + e < p.N) to[e] = o[e];
     }
   }
 #endif
@@ -1132,7 +1170,7 @@ KH_EXPORT int kh_w4_linear(const void* x, const void* q, const void* scale, cons
   }
   LinParams p{x, (const uint8_t*)q, (const bf16_t*)scale, (const uint8_t*)zero, bias, b_cat, residual, (const float*)workspace, y, (long)M,
               (long)N, (int)K, (int)R, splits, (int)((K + 31) / 32 * 16), (int)(((K + group - 1) / group + 3) / 4 * 4),
-              ((uintptr_t)x & 3) == 0 && K % 2 == 0 && (!own || ((uintptr_t)a_cat & 3) == 0), own ? a_cat : nullptr, col_scale, 0};
+              ((uintptr_t)x & 3) == 0 && K % 2 == 0 && (!own || ((uintptr_t)a_cat & 3) == 0), own ? a_cat : nullptr, col_scale, 0, ((uintptr_t)b_cat & 3) == 0, M * N >= 4 << 20};
   const int rc = type == 0 ? launch_linear<bf16_t>(p, (int)group, s) : launch_linear<_Float16>(p, (int)group, s);
   if (rc != KH_OK) return rc;
   KH_RETURN_LAST_ERROR();
