@@ -695,3 +695,37 @@ def test_linear_attention_of_cut_sequences_with_slots():
             assert_within(got[at], rs, HALF[FP32] * rs.abs() + STATE_SLOP * ms, f"state of sequence {b}")
     others = [i for i in range(7) if i not in slots]
     assert (dst[others] == 8).all() and torch.equal(src[others].cpu(), pool[others])
+
+
+def test_a_captured_packed_prompt_takes_other_lengths():
+    """A graph of one packed call with its table and slots in buffers: other lengths, sequences without tokens or without a slot at every replay."""
+    from katz_amd import ops
+
+    r = gen(19)
+    rows, B, H, d = 1500, 4, 2, 64
+    q, k, v = (on(randn(r, rows, H * d)) for _ in range(3))
+    g = on(torch.tensor([-0.2, -0.003]))
+    pool = on(torch.randn(5, H, d, d, generator=r))
+    table, slots = torch.zeros(B + 1, dtype=torch.int32, device=DEV), torch.zeros(B, dtype=torch.int32, device=DEV)
+    state, out = pool.clone(), torch.zeros(rows, H * d, dtype=BF, device=DEV)
+    call = lambda s, o: ops.linear_attention(q, k, v, H, g, state=s, slots=slots, seg_start=table, max_seg_rows=rows, out=o)      # noqa: E731
+    slots.copy_(torch.arange(B, dtype=torch.int32))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(state, out)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(state, out)
+    for starts, places in (((0, 1500, 1500, 1500, 1500), (0, 1, 2, 3)), ((0, 10, 700, 700, 1400), (4, 0, -1, 2)), ((5, 5, 5, 5, 6), (0, 1, 2, 3)),
+                           ((0, 400, 800, 1200, 1499), (3, -1, 1, 7)), ((0, 1500, 1500, 1500, 1500), (1, 0, 2, 3))):
+        table.copy_(torch.tensor(starts, dtype=torch.int32))
+        slots.copy_(torch.tensor(places, dtype=torch.int32))
+        state.copy_(pool)
+        out.fill_(3.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        s2, o2 = pool.clone(), torch.full_like(out, 3.0)
+        call(s2, o2)
+        assert torch.equal(out, o2) and torch.equal(state, s2), (starts, places)
