@@ -1041,7 +1041,7 @@ int launch_few_as(LinParams p, hipStream_t s) {
   p.t_at = own > most ? own : most;
   const int lds = p.t_at + (p.a_cat ? 16 * OWN_PITCH * 4 : 0);
   if (lds > 65536) {
-    const hipError_t e = kh_allow_lds<w4_few_rows<T, G, ZERO, MB, NB, LW, ST, FOUR>>(lds);
+    const hipError_t e = kh_allow_lds<w4_few_rows<T, G, ZERO, MB, NB, LW, ST, FOUR>>(160 * 1024);      // (asked for once: the largest of all calls)
     if (e != hipSuccess) return (int)e;
   }
   kh_launch(KH_TAG_W4_LINEAR, w4_few_rows<T, G, ZERO, MB, NB, LW, ST, FOUR>, dim3((unsigned)((p.N + NB * 16 - 1) / (NB * 16)), (unsigned)mt), dim3(LW * 64), lds, s, p);

@@ -697,6 +697,22 @@ def test_linear_attention_of_cut_sequences_with_slots():
     assert (dst[others] == 8).all() and torch.equal(src[others].cpu(), pool[others])
 
 
+def test_w4_linear_with_and_without_adapters_in_turn():
+    """One kernel with more and with less LDS."""
+    from katz_amd import ops
+
+    g = gen(20)
+    for N, K in ((9000, 640), (5000, 512), (100, 640)):
+        w = ops.quantize_w4(on(randn(g, N, K, std=0.05)), 128, True)
+        A, B, c = on(randn(g, 64, K, std=0.05)), on(randn(g, N, 64, std=0.05)), on(torch.rand(64, generator=g))
+        for M in (2, 9):
+            x = on(randn(g, M, K))
+            plain = ops.w4_linear(x, w)
+            none = ops.w4_linear(x, w, None, A, B, torch.zeros_like(c))
+            some = ops.w4_linear(x, w, None, A, B, c)
+            assert torch.equal(plain, none) and not torch.equal(plain, some) and torch.equal(ops.w4_linear(x, w), plain)
+
+
 def test_a_captured_packed_prompt_takes_other_lengths():
     """A graph of one packed call with its table and slots in buffers: other lengths, sequences without tokens or without a slot at every replay."""
     from katz_amd import ops
