@@ -10,6 +10,9 @@
 // its own (la_out).
 // bf16 operands carry 8 bits, so what is no input is fed to the matrix unit in pieces: scores and states as two (16 bits: their results are
 // rounded to bf16), the decayed values that make the state as three (24 bits: the state stays in 32).
+// What bounds it: 16384 packed tokens of 16 heads of 128 on 8 are 36 us of la_gain, 8 of la_scan and 82 of la_out (the bytes of q, k, v and o take 42), 16 blocks a workgroup
+// one after the other at 2.2 and 4.4 us.  Of those 4.4 matrix and vector instructions, which a SIMD issues one after the other, are 3; the rest is reads from LDS and two
+// barriers, which two waves on a SIMD do not cover.  A workgroup takes 116 KB of LDS, so there is one to a CU.
 #include "kh_common.h"
 #include <type_traits>
 
@@ -718,7 +721,7 @@ __global__ __launch_bounds__(TV * 4) __attribute__((amdgpu_waves_per_eu(2, 2))) 
   }
 }
 
-// One token: the state is read and written once, which bounds it.  A workgroup has 64 columns of one head: 16 threads of four columns, 16 rows at a time.
+// One token: the state is read and written once, which bounds it (64 sequences of 32 heads of 128 x 128: 55 us, 52 at the rate of a copy).  A workgroup has 64 columns of one head: 16 threads of four columns, 16 rows at a time.
 template <int DK>
 __global__ __launch_bounds__(256) void la_step(const LaParams p) {
   __shared__ float red[4][C];

@@ -649,6 +649,8 @@ __global__ __launch_bounds__(LW * 64) void w4_few_rows(const LinParams p) {
 // LDS, where every wave's accumulators start from it.
 // A block is 1920 clocks of the matrix unit (two waves of 60 products of 16 x 16 x 32 on a SIMD), about 2100 of the vector unit (codes to operands, the scaled sum of
 // every group) and 1650 of LDS: sums of a group and of the row in 32 bits each are 120 registers of the 256 that two waves leave each other.
+// 616 rows, 10240 x 1280 with rank 96 and a residual, by the clock of a workgroup: 3 us to the first block, 4 for the ranks, 24 for ten blocks, 8 for the outputs, whose 25 MB
+// all CUs move at once.
 constexpr int MR_M = 5, MR_N = 3, MR_W = 8, MR_ST = 3;     // tiles of 16 rows; of 16 columns of a wave; waves; stages
 
 template <int G, bool ZERO>
@@ -1048,8 +1050,8 @@ int launch_few_as(LinParams p, hipStream_t s) {
   return KH_OK;
 }
 // Tiles of 16 columns to a workgroup: as few as leave every CU at most one workgroup, up to four (a tile's columns share the loads of x).  Waves and stages
-// as measured over N 320 .. 16384, K 640 .. 8192 (us, cold codes, groups of 64, tiles 1 | 2 | 4): one row 8192 x 8192 12.1 | 9.6 | 13.9, 16384 x 8192 21.7 | 18.4 | 18.7,
-// 1280 x 5120 4.9 | 6.0 | 8.9; 16 rows 5120 x 1280 5.6 | 4.6 | 5.7, 10240 x 1280 7.6 | 6.7 | 5.8, 16384 x 8192 45 | 30 | 24.6; 32 rows 16384 x 8192 73 | 46 | 33.
+// as measured over N 320 .. 16384, K 640 .. 8192 (us, cold codes, groups of 64, tiles 1 | 2 | 4): one row 8192 x 8192 10.3 | 9.6 | 12.6, 16384 x 8192 18.3 | 17.5 | 18.2,
+// 1280 x 5120 4.5 | 5.4 | 7.7; 16 rows 5120 x 1280 5.1 | 4.1 | 4.7, 10240 x 1280 7.6 | 5.6 | 5.1, 16384 x 8192 34.8 | 24.4 | 21.3; 32 rows 16384 x 8192 44 | 32 | 26.3.
 // Four, eight or sixteen waves and two, three or four stages are within 0.5 us of one another where LDS lets two workgroups on a CU or there is only one.
 template <typename T, int G, bool ZERO>
 int launch_few(const LinParams& p, hipStream_t s) {
