@@ -37,7 +37,6 @@ struct LaParams {
   int T, dv, n_slots, chunks;  // chunks: 0 where a workgroup has a whole sequence
   float scale;
   int fill;                    // la_step: rows that are left out are zero
-  int once;                    // outputs of 16 MB and more: stored past the caches (one sequence of 16384 tokens of 16 heads of 128 127 -> 118 us)
 };
 
 struct Unit {                  // one (sequence, head, range of columns of v)
@@ -668,9 +667,7 @@ __global__ __launch_bounds__(TV * 4) __attribute__((amdgpu_waves_per_eu(2, 2))) 
       const auto s0 = __builtin_amdgcn_permlane16_swap(pack_bf16x2(a[it][0], a[it][1]), pack_bf16x2(a[it + 1][0], a[it + 1][1]), false, false);
       const auto s1 = __builtin_amdgcn_permlane16_swap(pack_bf16x2(a[it][2], a[it][3]), pack_bf16x2(a[it + 1][2], a[it + 1][3]), false, false);
       const int row = 16 * it + orow_at;     // (always a store: how many there are is what the next block's wait goes by)
-      const int to = c + row < t1 ? (int)((uint32_t)row * (uint32_t)p.ldo * 2u + ocol) : (int)0xfffffff0u;
-      if (p.once) __builtin_amdgcn_raw_buffer_store_b128(u32x4{s0[0], s1[0], s0[1], s1[1]}, ro, to, 0, 2 /* nt */);
-      else __builtin_amdgcn_raw_buffer_store_b128(u32x4{s0[0], s1[0], s0[1], s1[1]}, ro, to, 0, 0);
+      __builtin_amdgcn_raw_buffer_store_b128(u32x4{s0[0], s1[0], s0[1], s1[1]}, ro, c + row < t1 ? (int)((uint32_t)row * (uint32_t)p.ldo * 2u + ocol) : (int)0xfffffff0u, 0, 0);
 #endif
     }
     if (ends || c + C < t1) {
@@ -843,7 +840,7 @@ KH_EXPORT int kh_linear_attention_bf16(const void* q, const void* k, const void*
   if (n_slots > (1L << 30) || rows > (1L << 31)) return KH_ERR_TOO_LARGE;
   LaParams p{(const bf16_t*)q, (const bf16_t*)k, (const bf16_t*)v, (bf16_t*)o, log_decay, state_in, state_out, seg_start, slots, (float*)workspace,
              ldq, ldk, ldv, ldo, bsq, bsk, bsv, bso, (long)rows, (int)B, (int)H, kv_heads > 0 ? (int)(H / kv_heads) : 1, (int)T, (int)dv, (int)n_slots,
-             0, scale, 0, (seg_start ? rows : B * T) * H * dv >= 8 << 20};
+             0, scale, 0};
   const int rc = check(p, B, H, kv_heads, dk, dv, false);
   if (rc != KH_OK) return rc;
   if (T <= 0 || (seg_start && rows < 0)) return KH_ERR_INVALID_ARG;
@@ -866,7 +863,7 @@ KH_EXPORT int kh_linear_attention_step_bf16(const void* q, const void* k, const 
   if (flags & ~1) return KH_ERR_INVALID_ARG;
   if (n_slots > (1L << 30)) return KH_ERR_TOO_LARGE;
   LaParams p{(const bf16_t*)q, (const bf16_t*)k, (const bf16_t*)v, (bf16_t*)o, log_decay, state_in, state_out, nullptr, slots, nullptr,
-             0, 0, 0, 0, ldq, ldk, ldv, ldo, 0, (int)B, (int)H, kv_heads > 0 ? (int)(H / kv_heads) : 1, 1, (int)dv, (int)n_slots, 0, scale, flags, 0};
+             0, 0, 0, 0, ldq, ldk, ldv, ldo, 0, (int)B, (int)H, kv_heads > 0 ? (int)(H / kv_heads) : 1, 1, (int)dv, (int)n_slots, 0, scale, flags};
   const int rc = check(p, B, H, kv_heads, dk, dv, true);
   if (rc != KH_OK) return rc;
   if (ldq < H * dk || ldk < kv_heads * dk || ldv < kv_heads * dv || ldo < H * dv) return KH_ERR_INVALID_ARG;
