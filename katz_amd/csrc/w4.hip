@@ -286,7 +286,7 @@ struct LinParams {
   const float* col_scale;
   int t_at;
   int b_dma;               // B_cat is aligned to four bytes
-  int once;                // y is larger than the caches: stored past them
+  int once;                // y of 8 MB and more is stored past the caches (616 x 10240 with a residual: 40.6 -> 37.4 us)
 };
 
 // The rank-R product of a 16 x 16 tile in 32 bits, a step of 16 ranks: t from LDS, or [M][R] in `splits` parts, B_cat rows of T.

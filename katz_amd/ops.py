@@ -1500,7 +1500,7 @@ def w4_linear(x: torch.Tensor, w: W4Weight, bias: Optional[torch.Tensor] = None,
     if residual is not None:
         _fits(residual, dt, shape, "residual")
     if out is None:
-        out = x.new_empty(shape)
+        out = x.new_empty(shape) if residual is None else torch.empty_like(residual)
     else:
         _fits(out, dt, shape, "out")
     if not M or not N:
@@ -1524,14 +1524,16 @@ def _la_sizes(q, k, v, heads: int, kv_heads: Optional[int], log_decay: torch.Ten
     kv = heads if kv_heads is None else kv_heads
     if heads < 1 or kv < 1 or heads % kv:
         raise ValueError(f"{heads} heads cannot share the keys of {kv}")
-    for t in (q, k, v):
-        if t.dtype is not BF16 or t.dim() != dims or t.stride(-1) != 1:
-            raise TypeError(f"q, k and v must be bfloat16 with {dims} axes, the last contiguous, got {t.dtype} {tuple(t.shape)}")
     qs, ks, vs = q.shape, k.shape, v.shape
-    if qs[:-1] != ks[:-1] or qs[:-1] != vs[:-1]:
+    if (q.dtype is not BF16 or k.dtype is not BF16 or v.dtype is not BF16 or len(qs) != dims or len(ks) != dims or len(vs) != dims
+            or q.stride(-1) != 1 or k.stride(-1) != 1 or v.stride(-1) != 1):
+        raise TypeError(f"q, k and v must be bfloat16 with {dims} axes, the last contiguous, got " + ", ".join(f"{t.dtype} {tuple(t.shape)}" for t in (q, k, v)))
+    rows = qs[0]
+    if rows != ks[0] or rows != vs[0] or (dims == 3 and (qs[1] != ks[1] or qs[1] != vs[1])):
         raise ValueError("q, k and v must have the same rows")
-    dk, dv = qs[-1] // heads, vs[-1] // kv
-    if qs[-1] != heads * dk or ks[-1] != kv * dk or vs[-1] != kv * dv:
+    wq, wv = qs[-1], vs[-1]
+    dk, dv = wq // heads, wv // kv
+    if wq != heads * dk or ks[-1] != kv * dk or wv != kv * dv:
         raise ValueError("q must be [.., heads * dk], k [.., kv_heads * dk], v [.., kv_heads * dv]")
     _fits(log_decay, torch.float32, (heads,), "log_decay")
     return kv, dk, dv
@@ -1621,8 +1623,12 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: i
                 named = named[:n_slots].view(-1, 1, 1, 1)
                 state_out.masked_fill_(named, 0.0) if state is None else state_out.copy_(torch.where(named, state, state_out))
         return out, state_out
-    ld, bs = zip(*[_la_strides(t) for t in (q, k, v, out)])
-    if not packed and T == 1 and state is not None and all(st >= t.shape[-1] for st, t in zip(bs, (q, k, v, out))):   # one pass over the state
+    if q.is_contiguous() and k.is_contiguous() and v.is_contiguous() and out.is_contiguous():
+        ld = wq, wk, wv, wo = heads * dk, kv * dk, kv * dv, heads * dv
+        bs = (0, 0, 0, 0) if packed else (T * wq, T * wk, T * wv, T * wo)
+    else:
+        ld, bs = zip(*[_la_strides(t) for t in (q, k, v, out)])
+    if T == 1 and not packed and state is not None and all(st >= t.shape[-1] for st, t in zip(bs, (q, k, v, out))):   # one pass over the state
         _la_step(lib, q, k, v, out, log_decay, state, state_out, slots, n_slots, B, heads, kv, dk, dv, bs, scale)
         return out, state_out
     nbytes = _workspace_bytes("kh_linear_attention_workspace_bytes", B, heads, T, rows, dk, dv)
@@ -1648,15 +1654,15 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, hea
     _here(q, k, v, log_decay, state, state_out, slots, out)
     B = q.shape[0]
     state_out, n_slots = _la_states(state, state_out, slots, q, B, heads, dk, dv)
-    shape = (B, heads * dv)
     fill = 0
     if out is None:
-        out, fill = q.new_empty(shape), slots is not None
+        out = torch.empty_like(q, memory_format=torch.contiguous_format) if dk == dv else q.new_empty((B, heads * dv))
+        fill = slots is not None
     else:
-        _la_out(out, shape)
+        _la_out(out, (B, heads * dv))
     if B:
-        _la_step(lib, q, k, v, out, log_decay, state, state_out, slots, n_slots, B, heads, kv, dk, dv, [_la_strides(t)[0] for t in (q, k, v, out)],
-                 dk ** -0.5 if scale is None else scale, fill)
+        strides = (q.stride(0), k.stride(0), v.stride(0), out.stride(0)) if B > 1 else (heads * dk, kv * dk, kv * dv, heads * dv)
+        _la_step(lib, q, k, v, out, log_decay, state, state_out, slots, n_slots, B, heads, kv, dk, dv, strides, dk ** -0.5 if scale is None else scale, fill)
     return out, state_out
 
 
