@@ -8,8 +8,10 @@
 // Where there are few heads, the blocks of all sequences of a head, one after the other, are cut into equal chunks, wherever a sequence ends: a chunk whose last
 // sequence goes on in the next leaves what it adds to that state (la_gain), the sums over the chunks before each follow (la_scan), and then every chunk runs on
 // its own (la_out).
-// bf16 operands carry 8 bits, so what is no input is fed to the matrix unit in pieces: scores and states as two (16 bits: their results are
-// rounded to bf16), the decayed values that make the state as three (24 bits: the state stays in 32).
+// bf16 operands carry 8 bits, so what is no input (scores, states, the decayed values that make the state) is fed to the matrix unit as three pieces of 8: 24 bits,
+// those of the 32-bit numbers that they are held in.  Two pieces of scores, states and of the values in chunks where no sequence ends left 2^-18 of a term and cost less (us, two | three:
+// 16384 packed tokens of 16 heads of 128 on 8 122 | 135, 2 x 4096 of 20 heads of 64 46.6 | 50.1, 16 x 1024 of 16 heads of 128 83.5 | 89.4, 2 x 77 of 20 heads of 64 the same): terms that cancel
+// one another lost what was left of them.
 // What bounds it: 16384 packed tokens of 16 heads of 128 on 8 are 36 us of la_gain, 8 of la_scan and 82 of la_out (the bytes of q, k, v and o take 42), 16 blocks a workgroup
 // one after the other at 2.2 and 4.4 us.  Of those 4.4 matrix and vector instructions, which a SIMD issues one after the other, are 3; the rest is reads from LDS and two
 // barriers, which two waves on a SIMD do not cover.  A workgroup takes 116 KB of LDS, so there is one to a CU.
@@ -235,9 +237,9 @@ __device__ __forceinline__ uint32_t take_pieces(float& x0, float& x1) {
   return h;
 }
 
-// S = decay S + sum_j w_j k_j v_j^T over a block: V as the wave's columns, K in LDS; decayed values in two pieces of bf16, or three.
+// S = decay S + sum_j w_j k_j v_j^T over a block: V as the wave's columns, K in LDS; decayed values in three pieces of bf16.
 template <int DK>
-__device__ __forceinline__ void add_block(State<DK>& st, const bf16x8 (&raw)[2], const uint32_t (&kcol)[2], float decay, const float (&w)[2][8], bool third) {
+__device__ __forceinline__ void add_block(State<DK>& st, const bf16x8 (&raw)[2], const uint32_t (&kcol)[2], float decay, const float (&w)[2][8]) {
   u32x4 v[3][2];
 #pragma unroll
   for (int s = 0; s < 2; ++s)
@@ -265,7 +267,7 @@ __device__ __forceinline__ void add_block(State<DK>& st, const bf16x8 (&raw)[2],
     };
     piece(0);
     piece(1);
-    if (third) piece(2);
+    piece(2);
   }
 }
 
@@ -394,7 +396,7 @@ __global__ __launch_bounds__(TV * 4) void la_gain(const LaParams p) {
     if (c + C < t1) fetch(c + C, other);
     bf16x8 vf[1][2];
     Tile<TV>::template columns<1>(vcol, 0, vf);
-    add_block<DK>(st, vf[0], kcol, decay, w, true);
+    add_block<DK>(st, vf[0], kcol, decay, w);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       vcol[h] += other - st_at;
@@ -476,15 +478,14 @@ __global__ __launch_bounds__(TV * 4) void la_scan(const LaParams p) {
 template <int DK, int TV>
 struct OutShape {
   static constexpr int PP = C * 2 + 16;    // pitch of the scores in bytes: 16-byte pieces of neighbouring rows on other banks
-  static constexpr int STAGE = 2 * Tile<DK>::BYTES + Tile<TV>::BYTES, LDS = 2 * STAGE + 2 * C * PP;
+  static constexpr int STAGE = 2 * Tile<DK>::BYTES + Tile<TV>::BYTES, LDS = 2 * STAGE + 3 * C * PP;
 };
 template <int DK, int TV, bool ONE>
 __global__ __launch_bounds__(TV * 4) __attribute__((amdgpu_waves_per_eu(2, 2))) void la_out(const LaParams p) {
   typedef OutShape<DK, TV> Sh;
   constexpr int NW = TV / 16;
-  extern __shared__ __attribute__((aligned(16))) char smem[];   // two stages of K, Q, V; decayed scores, upper and lower pieces
+  extern __shared__ __attribute__((aligned(16))) char smem[];   // two stages of K, Q, V; decayed scores in three pieces
   char* const ph = smem + 2 * Sh::STAGE;
-  char* const pl = ph + C * Sh::PP;
   Unit u;
   int ht, which, left = 0, t0 = 0, t1;     // left: blocks of the chunk; t0, t1: tokens of the sequence
   if (!work_of<TV>(p, ht, which)) return;
@@ -589,20 +590,22 @@ __global__ __launch_bounds__(TV * 4) __attribute__((amdgpu_waves_per_eu(2, 2))) 
         }
         float x0 = a[0], x1 = a[1], x2 = a[2], x3 = a[3];
         *reinterpret_cast<u32x2*>(ph + p_to + JS * i * 32) = u32x2{take_pieces(x0, x1), take_pieces(x2, x3)};
-        *reinterpret_cast<u32x2*>(pl + p_to + JS * i * 32) = u32x2{pack_bf16x2(x0, x1), pack_bf16x2(x2, x3)};
+        *reinterpret_cast<u32x2*>(ph + C * Sh::PP + p_to + JS * i * 32) = u32x2{take_pieces(x0, x1), take_pieces(x2, x3)};
+        *reinterpret_cast<u32x2*>(ph + 2 * C * Sh::PP + p_to + JS * i * 32) = u32x2{pack_bf16x2(x0, x1), pack_bf16x2(x2, x3)};
       }
     }
     // the state's share of the outputs of this wave's 16 columns: rows of the product 4 grp + r of them, columns i = 16 it + l
     f32x4 a[4];
     {
-      u32x4 sh[DK / 32], sl[DK / 32];
+      u32x4 piece[3][DK / 32];
 #pragma unroll
       for (int s = 0; s < DK / 32; ++s)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float x0 = st.s[2 * s + e / 2][2 * (e % 2)], x1 = st.s[2 * s + e / 2][2 * (e % 2) + 1];
-          sh[s][e] = take_pieces(x0, x1);
-          sl[s][e] = pack_bf16x2(x0, x1);
+          piece[0][s][e] = take_pieces(x0, x1);
+          piece[1][s][e] = take_pieces(x0, x1);
+          piece[2][s][e] = pack_bf16x2(x0, x1);
         }
 #pragma unroll
       for (int it = 0; it < 4; ++it) a[it] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -612,9 +615,9 @@ __global__ __launch_bounds__(TV * 4) __attribute__((amdgpu_waves_per_eu(2, 2))) 
 #pragma unroll
         for (int it = 0; it < 4; ++it) qf[it] = *reinterpret_cast<const bf16x8*>(smem + a8[s] + it * (16 * Tile<DK>::ROW) + QT);
 #pragma unroll
-        for (int it = 0; it < 4; ++it) a[it] = mfma(__builtin_bit_cast(bf16x8, sh[s]), qf[it], a[it]);
+        for (int i = 0; i < 3; ++i)
 #pragma unroll
-        for (int it = 0; it < 4; ++it) a[it] = mfma(__builtin_bit_cast(bf16x8, sl[s]), qf[it], a[it]);
+          for (int it = 0; it < 4; ++it) a[it] = mfma(__builtin_bit_cast(bf16x8, piece[i][s]), qf[it], a[it]);
       }
 #pragma unroll
       for (int it = 0; it < 4; ++it)
@@ -653,9 +656,9 @@ __global__ __launch_bounds__(TV * 4) __attribute__((amdgpu_waves_per_eu(2, 2))) 
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
 #pragma unroll
-      for (int it = 2 * s; it < 4; ++it) a[it] = mfma(vf[0][s], *reinterpret_cast<const bf16x8*>(ph + p_from + it * (16 * Sh::PP) + s * 64), a[it]);
+      for (int i = 0; i < 3; ++i)
 #pragma unroll
-      for (int it = 2 * s; it < 4; ++it) a[it] = mfma(vf[0][s], *reinterpret_cast<const bf16x8*>(pl + p_from + it * (16 * Sh::PP) + s * 64), a[it]);
+        for (int it = 2 * s; it < 4; ++it) a[it] = mfma(vf[0][s], *reinterpret_cast<const bf16x8*>(ph + i * C * Sh::PP + p_from + it * (16 * Sh::PP) + s * 64), a[it]);
     }
 #if __HIP_DEVICE_COMPILE__
     const rsrc_t ro = __builtin_amdgcn_make_buffer_rsrc(p.o + u.o0 + (long)c * p.ldo, 0, (int)(uint32_t)((((t1 - c < C ? t1 - c : C) - 1) * p.ldo + TV) * 2), 0x00020000);
@@ -675,7 +678,7 @@ __global__ __launch_bounds__(TV * 4) __attribute__((amdgpu_waves_per_eu(2, 2))) 
         powers(u.g, t1 - c, w);
         decay = power(u.g, t1 - c);
       }
-      add_block<DK>(st, vf[0], kcol, decay, w, ends);   // (a state that is taken no further in the chunk only makes outputs)
+      add_block<DK>(st, vf[0], kcol, decay, w);
     }
 #pragma unroll
     for (int s = 0; s < DK / 32; ++s) a8[s] += other - stage;

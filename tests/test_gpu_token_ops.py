@@ -745,3 +745,59 @@ def test_a_captured_packed_prompt_takes_other_lengths():
         s2, o2 = pool.clone(), torch.full_like(out, 3.0)
         call(s2, o2)
         assert torch.equal(out, o2) and torch.equal(state, s2), (starts, places)
+
+
+@pytest.mark.parametrize("dk,dv", [(64, 64), (64, 128), (128, 64), (128, 128)])
+@pytest.mark.parametrize("T", [2, 64, 65, 130, 1500])
+def test_linear_attention_multiplies_scores_states_and_values_of_24_bits(T, dk, dv):
+    """Terms that cancel but for their last 8 of 24 bits: every sum and product below is a number of 24 bits, so the result is the difference itself, rounded once."""
+    from katz_amd import ops
+
+    say("24 bits", T, dk, dv)
+    a = 171 / 128                                          # eight bits; three of them, 2^-8 apart, are 24 without a gap
+    far = torch.zeros(1, device=DEV)                       # no decay, and a scale of 1: nothing else is rounded
+    want = a * 2.0 ** -16
+    # two scores of the last token, a (1 + 2^-8 + 2^-16) and a (1 + 2^-8), with values 1 and -1
+    q, k, v = (torch.zeros(1, T, w, dtype=BF) for w in (dk, dk, dv))
+    first = max(0, T - 2 - (T - 1) % 64 // 2)              # (in the last block, with the other one where it has two)
+    q[0, -1, :3] = torch.tensor([1.0, 2.0 ** -8, 2.0 ** -16])
+    k[0, first, :3], k[0, -1, :2] = a, a
+    v[0, first, 3], v[0, -1, 3] = 1.0, -1.0
+    if first // 64 == (T - 1) // 64:
+        o, _ = ops.linear_attention(on(q), on(k), on(v), 1, far, scale=1.0)
+        assert o[0, -1, 3].item() == torch.tensor(want).to(BF).item()
+        assert not o[0, -1, :3].any() and not o[0, :-1, :3].any()
+    # a state of two such rows, which the last token's query takes off one another
+    s0 = torch.zeros(1, 1, dk, dv)
+    s0[0, 0, 5, 7], s0[0, 0, 40, 7] = a * (1 + 2.0 ** -8 + 2.0 ** -16), a * (1 + 2.0 ** -8)
+    q, k, v = (torch.zeros(1, T, w, dtype=BF) for w in (dk, dk, dv))
+    q[0, -1, 5], q[0, -1, 40] = 1.0, -1.0
+    o, S = ops.linear_attention(on(q), on(k), on(v), 1, far, scale=1.0, state=on(s0))
+    assert o[0, -1, 7].item() == torch.tensor(want).to(BF).item() and torch.equal(S.cpu(), s0)
+
+
+def test_linear_attention_of_cut_sequences_adds_decayed_values_of_24_bits():
+    """In a chunk where no sequence ends, too: a decayed value of 24 bits, less what a later block's query sees of it in 16."""
+    from katz_amd import ops
+
+    T, d, end = 16384, 64, 134                             # (the third block of one sequence, far from its end)
+    say("24 bits of decayed values")
+    g = torch.tensor([-0.6931471805599453 / 64])           # half a block on
+    lam = torch.exp(g.to(F64))
+    w = lam ** (63 - torch.arange(64, dtype=F64))          # what the values of the first block are multiplied with
+    rest = w - w.to(BF).to(F64)
+    rest = (rest - rest.to(BF).to(F64)).abs() / w
+    at = int(rest.argmax())                                # where two pieces of 8 bits would leave the most
+    assert rest[at] > 2.0 ** -17.5
+    q, k, v = (torch.zeros(1, T, d, dtype=BF) for _ in range(3))
+    k[0, at, 9], v[0, at, 11], q[0, end, 9] = 1.0, 1.0, 1.0
+    first = left = (lam ** (end - at)).item()
+    for t in (end - 6, end - 4, end - 2):                  # three tokens of the query's block take it away but for its last bits
+        power = (lam ** (end - t)).item()
+        v[0, t, 11], k[0, t, 9] = left / power, -1.0
+        left -= v[0, t, 11].item() * power
+    o, _ = ops.linear_attention(on(q), on(k), on(v), 1, on(g), scale=1.0)
+    # Of a term: three powers, of 2^-23 and of 2^-24 for their arguments below 1.5, four products, three sums, two times three pieces that leave 2^-25: 18 times
+    # 2^-24 at most; of the second and third later token 2^-8 and less of that
+    slop = 18 * 2.0 ** -24 * 2.02 * first
+    assert abs(o[0, end, 11].item() - left) <= slop + HALF[BF] * abs(left), (o[0, end, 11].item(), left, slop, rest[at].item() * first)
