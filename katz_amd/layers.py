@@ -384,7 +384,7 @@ class LoRALinearW4(nn.Module):
     time pass through, whose bytes are the time; any number of rows is right.
 
     The buffers weight_q / weight_scale / weight_zero are what is saved; fuse() merges adapters into them in place, so a captured graph that reads them
-    stays valid."""
+    stays valid.  What is merged is part of the weights from then on: its name is free for another adapter, and weights that are loaded take no adapter as merged."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, group: int = 64, zeros: bool = False, device=None,
                  dtype=torch.bfloat16):
@@ -434,6 +434,12 @@ class LoRALinearW4(nn.Module):
         self.dtype = dtype
         return self
 
+    def _load_from_state_dict(self, state_dict, prefix, *args, **kwargs):
+        super()._load_from_state_dict(state_dict, prefix, *args, **kwargs)
+        if self._fused and prefix + "weight_q" in state_dict:     # other weights: nothing that is known of them is merged
+            self._fused.clear()
+            self.refresh_adapters()
+
     def packed_weight(self) -> "ops.W4Weight":
         return ops.W4Weight(self.weight_q, self.weight_scale, self.weight_zero, self.in_features, self.group)
 
@@ -449,10 +455,14 @@ class LoRALinearW4(nn.Module):
             raise ValueError(f"adapter {name!r} does not fit a [{self.out_features},{self.in_features}] layer: "
                              f"down {tuple(down.shape)}, up {tuple(up.shape)}")
         self.adapters[name] = Adapter(down.detach(), up.detach(), alpha, weight)
+        self._fused.discard(name)           # (what was merged under that name stays merged: this is another adapter)
         self._packed_key = None
+        if name in self.active:
+            self.refresh_adapters()
 
     def delete_adapter(self, name: str) -> None:
         self.adapters.pop(name, None)
+        self._fused.discard(name)
         self.active = [n for n in self.active if n != name]
         self.refresh_adapters()
 

@@ -264,3 +264,44 @@ def test_layer_with_adapters_converts_and_keeps_its_own_weights():
         layer.float()
     assert torch.equal(layer(x), y)
     assert torch.equal(layer.cpu().to(DEV)(x), y)
+
+
+def test_names_that_were_fused_are_free_for_other_adapters():
+    """A merged adapter is part of the weights: one that is added under its name, or the same one over weights that are loaded anew, applies."""
+    from katz_amd import ops
+
+    g = torch.Generator().manual_seed(8)
+    layer = linear(g, 96, 128)
+    x = torch.randn(5, 128, generator=g).to(DEV, BF)
+    ads = [((torch.randn(16, 128, generator=g) * 0.1).to(BF), (torch.randn(96, 16, generator=g) * 0.1).to(BF)) for _ in range(2)]
+    saved = {k: v.clone() for k, v in layer.state_dict().items()}
+
+    def want(down, up):
+        w = ops.dequantize_w4(layer.packed_weight(), torch.float32).cpu().to(F64)
+        xd = x.cpu().to(F64)
+        return xd @ w.t() + layer.bias.detach().cpu().to(F64) + (xd @ down.to(F64).t()) @ up.to(F64).t()
+
+    def fused_first():
+        layer.load_state_dict(saved)
+        for n in list(layer.adapters):
+            layer.delete_adapter(n)
+        layer.add_adapter("a", *ads[0])
+        layer.set_active(["a"])
+        layer.fuse()
+        layer.set_active(["a"])
+        assert layer._packed is None                                 # (merged: not applied twice)
+
+    fused_first()                                                    # deleted, and another one under its name
+    layer.delete_adapter("a")
+    layer.add_adapter("a", *ads[1])
+    layer.set_active(["a"])
+    close(layer(x), want(*ads[1]), "deleted and added")
+    fused_first()                                                    # replaced while its name is active
+    layer.add_adapter("a", *ads[1])
+    close(layer(x), want(*ads[1]), "replaced")
+    before = layer.weight_q.clone()
+    layer.fuse()
+    assert layer._packed is None and not torch.equal(layer.weight_q, before)
+    fused_first()                                                    # the weights from before it was merged
+    layer.load_state_dict(saved)
+    close(layer(x), want(*ads[0]), "loaded anew")
