@@ -823,19 +823,19 @@ __global__ __launch_bounds__(MR_W * 64) __attribute__((amdgpu_waves_per_eu(2, 2)
   // place of the rows would ask few channels (616 x 10240 x 1280 38.0 -> 35.0 us).
   const int rot = (int)((unit / mt) * 5 % (uint32_t)blocks);
   auto turned = [&](int i) { return i + rot < blocks ? i + rot : i + rot - blocks; };
-  // The adapters' product, 32 ranks at a time, comes first through the same stages: t in two pieces of bf16 in the place of x, B_cat in the place of the codes.
+  // The adapters' product, 32 ranks at a time, comes first through the same stages: t in three pieces of bf16 (24 bits) in the place of x, B_cat in the place of the codes.
   const bf16_t* th = (const bf16_t*)p.t;
   const int steps = p.R / 32, all = steps + blocks;
-  const __amdgpu_buffer_rsrc_t rt = __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16_t*>(th + m0 * p.R), 0, bytes((2 * p.M - m0) * p.R * 2), 0x00020000);
+  const __amdgpu_buffer_rsrc_t rt = __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16_t*>(th + m0 * p.R), 0, bytes((3 * p.M - m0) * p.R * 2), 0x00020000);
   const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>((const T*)p.b_cat + nb * p.R), 0, bytes((p.N - nb) * p.R * 2), 0x00020000);
   auto fetch_ranks = [&](int step, int st) {
     char* to = smem + st * Sg::BYTES;
 #pragma unroll
-    for (int i = 0; i < (2 * MR_M + MR_W - 1) / MR_W; ++i) {
-      const int id = wave + i * MR_W, r = (id >> 1) * 16 + dr;
-      if (id < 2 * MR_M)
+    for (int i = 0; i < (3 * MR_M + MR_W - 1) / MR_W; ++i) {
+      const int id = wave + i * MR_W, r = id / 3 * 16 + dr;
+      if (id < 3 * MR_M)
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rt, (lptr_t)(to + Sg::XAT + id * 1024), 16, (int)(((uint32_t)(r < rows ? r : rows - 1) * (uint32_t)p.R + dp * 8) * 2),
-                                                 (int)((uint32_t)((id & 1) * p.M * p.R + step * 32) * 2), 0, 0);
+                                                 (int)((uint32_t)(id % 3 * p.M * p.R + step * 32) * 2), 0, 0);   // (below 2^32: M <= 2^20, R <= 128)
     }
 #pragma unroll
     for (int j = 0; j < MR_N; ++j) {
@@ -853,17 +853,20 @@ __global__ __launch_bounds__(MR_W * 64) __attribute__((amdgpu_waves_per_eu(2, 2)
   };
   auto multiply_ranks = [&](int st) {
     const char* at = smem + st * Sg::BYTES;
-    u32x4 hi[MR_M], lo[MR_M];
+    u32x4 t[MR_M][3];
 #pragma unroll
-    for (int b = 0; b < MR_M; ++b) {
-      hi[b] = *reinterpret_cast<const u32x4*>(at + Sg::XAT + 2 * b * 1024 + from);
-      lo[b] = *reinterpret_cast<const u32x4*>(at + Sg::XAT + (2 * b + 1) * 1024 + from);
-    }
+    for (int b = 0; b < MR_M; ++b)
+#pragma unroll
+      for (int k = 0; k < 3; ++k) t[b][k] = *reinterpret_cast<const u32x4*>(at + Sg::XAT + (3 * b + k) * 1024 + from);
+    auto add = [&](int j, int k, bf16x8 v) {
+#pragma unroll
+      for (int b = 0; b < MR_M; ++b) out[b][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, t[b][k]), v, out[b][j], 0, 0, 0);
+    };
 #pragma unroll
     for (int j = 0; j < MR_N; ++j) {
       const u32x4 raw = *reinterpret_cast<const u32x4*>(at + Sg::WAT + (wave * MR_N + j) * 1024 + from);
       bf16x8 bh = __builtin_bit_cast(bf16x8, raw), bl;
-      if constexpr (!__is_same(T, bf16_t)) {       // (fp16 in two pieces)
+      if constexpr (!__is_same(T, bf16_t)) {       // (fp16: 11 bits in two pieces)
         T v[8];
         __builtin_memcpy(v, &raw, 16);
 #pragma unroll
@@ -873,12 +876,11 @@ __global__ __launch_bounds__(MR_W * 64) __attribute__((amdgpu_waves_per_eu(2, 2)
         }
       }
 #pragma unroll
-      for (int b = 0; b < MR_M; ++b) out[b][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, hi[b]), bh, out[b][j], 0, 0, 0);
-#pragma unroll
-      for (int b = 0; b < MR_M; ++b) out[b][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, lo[b]), bh, out[b][j], 0, 0, 0);
-      if constexpr (!__is_same(T, bf16_t))
-#pragma unroll
-        for (int b = 0; b < MR_M; ++b) out[b][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, hi[b]), bl, out[b][j], 0, 0, 0);
+      for (int k = 0; k < 3; ++k) add(j, k, bh);
+      if constexpr (!__is_same(T, bf16_t)) {       // (the third piece's product with what is left of B is 2^-24 of the first's)
+        add(j, 0, bl);
+        add(j, 1, bl);
+      }
     }
   };
   auto fetch_any = [&](int i, int st) {
@@ -970,7 +972,7 @@ struct ShrinkParams {
   float* t;
   long M;
   int K, R, per;           // per: k of a split, a multiple of 32
-  int pieces;              // one split, and t in two pieces of bf16 [2][M][R] instead
+  int pieces;              // one split, and t in three pieces of bf16 [3][M][R] instead
 };
 constexpr int SW = 8;      // waves of a workgroup
 template <typename T>
@@ -1013,9 +1015,12 @@ __global__ __launch_bounds__(SW * 64) void w4_shrink(const ShrinkParams p) {
     v *= p.col_scale[r0 + col];
     if (p.pieces) {
       bf16_t* t = (bf16_t*)p.t + (m0 + r) * p.R + r0 + col;
-      const bf16_t hi = (bf16_t)v;
-      t[0] = hi;
-      t[p.M * p.R] = (bf16_t)(v - (float)hi);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        const bf16_t hi = (bf16_t)v;
+        t[k * p.M * p.R] = hi;
+        v -= (float)hi;
+      }
     } else {
       p.t[((long)blockIdx.z * p.M + m0 + r) * p.R + r0 + col] = v;
     }
@@ -1149,7 +1154,9 @@ KH_EXPORT int kh_dequantize_w4(const void* q, const void* scale, const void* zer
 
 KH_EXPORT int64_t kh_w4_linear_workspace_bytes(int64_t M, int64_t K, int64_t R) {
   if (M <= 0 || K <= 0 || R < 0 || R % 32 != 0 || R > 128) return KH_ERR_INVALID_ARG;
-  return R == 0 || own_t(M, K, R) ? 0 : (int64_t)shrink_splits(M, K, R) * M * R * 4;
+  if (R == 0 || own_t(M, K, R)) return 0;
+  const int64_t parts = (int64_t)shrink_splits(M, K, R) * 4;
+  return (M > 32 && parts < 6 ? 6 : parts) * M * R;         // (t in 32 bits for each split, or, for many rows, in three pieces of 16)
 }
 
 KH_EXPORT int kh_w4_linear(const void* x, const void* q, const void* scale, const void* zero, const void* bias, const void* a_cat,

@@ -801,3 +801,23 @@ def test_linear_attention_of_cut_sequences_adds_decayed_values_of_24_bits():
     # 2^-24 at most; of the second and third later token 2^-8 and less of that
     slop = 18 * 2.0 ** -24 * 2.02 * first
     assert abs(o[0, end, 11].item() - left) <= slop + HALF[BF] * abs(left), (o[0, end, 11].item(), left, slop, rest[at].item() * first)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP16])
+@pytest.mark.parametrize("M,N,R", [(1, 48, 32), (20, 40, 96), (700, 4100, 32), (700, 4100, 64), (1030, 4608, 128)])
+def test_w4_linear_keeps_rank_products_in_32_bits(M, N, R, dtype):
+    """Two ranks whose products cancel but for the last 8 of 24 bits, over weights that are zero, for few rows and for many."""
+    from katz_amd import ops
+
+    say("rank products", M, N, R, dtype)
+    K, a, b = 64, 171 / 128, 171 / 128 + (2.0 ** -10 if dtype is FP16 else 0)     # 8 bits, and 11 of them
+    w = ops.W4Weight(torch.full((N, K // 2), 0x88, dtype=torch.uint8, device=DEV), torch.zeros(N, 4, dtype=BF, device=DEV), None, K, 64)
+    x, A, B, c = torch.zeros(M, K, dtype=dtype), torch.zeros(R, K, dtype=dtype), torch.zeros(N, R, dtype=dtype), torch.zeros(R)
+    x[:, 3], A[2, 3], A[R - 1, 3], B[:, 2], B[:, R - 1] = 1.0, 1.0, 1.0, b, -b
+    c[2], c[R - 1] = a * (1 + 2.0 ** -8 + 2.0 ** -16), a * (1 + 2.0 ** -8)
+    y = ops.w4_linear(on(x), w, None, on(A), on(B), on(c))
+    want = a * 2.0 ** -16 * b
+    # products of 24 and 11 bits and their sums: fewer than 8 roundings of 2^-24 of the terms (none where B has 8 bits: sums of 32 at most, of which the upper 24
+    # cancel), then the type's, which is that of the numbers below the normal ones in fp16
+    bound = 8 * 2.0 ** -24 * 2 * a * b + max(HALF[dtype] * want, 2.0 ** -25 if dtype is FP16 else 0)
+    assert (y.cpu().to(F64) - want).abs().max() <= bound, ((y.cpu().to(F64) - want).abs().max().item(), bound, want)
