@@ -208,13 +208,16 @@ __global__ __launch_bounds__(256) void values_kernel(const ValueParams p) {
 }
 
 // ---------------------------------------------------------------- the linear
-// Codes become operands of the matrix unit without a conversion: with the bits of a power of two P above a code (128 in bf16, 1024
-// in fp16, whose unit in the last place is 1) the 16 bits are the number P + q, so two shifted and masked nibbles are two operands.
-// A second product of x with the constant -(P + z) takes P and z away again, exactly, in the same accumulator; scales are applied to
-// a group's sum in 32 bits.  The nibbles of a word come out as pairs (0,4) (1,5) (2,6) (3,7); x is put into the same order.
+// Codes become operands of the matrix unit without a conversion: below the bits of a power of two P = 16, in the four upper bits of its mantissa, a code makes the
+// 16 bits the number P + q, so two shifted and masked nibbles are two operands.  A second product of x with the constant -(P + z) takes P and z away again,
+// exactly, in the same accumulator; scales are applied to a group's sum in 32 bits.  P is the smallest power with the codes in one binade: what the sum carries of it
+// costs 32-bit sums the upper bits.  (Codes in the lower bits, under 128 in bf16 and 1024 in fp16, are one shift of eight instructions less, and left an fp16 row of x with
+// a mean of 3 twice the error of its rounding.)
+// The nibbles of a word come out as pairs (0,4) (1,5) (2,6) (3,7); x is put into the same order.
 template <typename T> struct Num;
 template <> struct Num<bf16_t> {
-  static constexpr uint32_t P = 0x43004300u, NEG = 0x80008000u;
+  static constexpr uint32_t P16 = 0x41804180u, P32 = 0x42004200u, NEG = 0x80008000u;
+  static constexpr int UNIT = 3;     // where the bit of 1 is in 16 .. 32 (one further down in 32 .. 64)
   typedef bf16x8 V8;
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
 #if __HIP_DEVICE_COMPILE__
@@ -225,7 +228,8 @@ template <> struct Num<bf16_t> {
   }
 };
 template <> struct Num<_Float16> {
-  static constexpr uint32_t P = 0x64006400u, NEG = 0x80008000u;
+  static constexpr uint32_t P16 = 0x4c004c00u, P32 = 0x50005000u, NEG = 0x80008000u;
+  static constexpr int UNIT = 6;
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
 #if __HIP_DEVICE_COMPILE__
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -248,7 +252,8 @@ __device__ __forceinline__ u32x4 interleaved(const u32x4 v) {
 // The mask and the power of two in registers: one instruction then takes both (and-or), where two constants in the code would take two.
 template <typename T>
 struct Unpack {
-  uint32_t mask = 0x000f000fu, power = Num<T>::P;
+  static constexpr int U = Num<T>::UNIT;
+  uint32_t mask = 0x000f000fu << U, power = Num<T>::P16;
   __device__ __forceinline__ Unpack() {
 #if __HIP_DEVICE_COMPILE__
     asm("" : "+s"(mask));
@@ -256,7 +261,8 @@ struct Unpack {
 #endif
   }
   __device__ __forceinline__ u32x4 operator()(uint32_t word) const {
-    return u32x4{(word & mask) | power, ((word >> 4) & mask) | power, ((word >> 8) & mask) | power, ((word >> 12) & mask) | power};
+    const uint32_t second = U > 4 ? word << (U - 4) & mask : word >> (4 - U) & mask;
+    return u32x4{((word << U) & mask) | power, second | power, ((word >> (8 - U)) & mask) | power, ((word >> (12 - U)) & mask) | power};
   }
 };
 
@@ -475,7 +481,7 @@ __global__ __launch_bounds__(LW * 64) void w4_few_rows(const LinParams p) {
       for (int j = 0; j < 4; ++j) xv[b][j] = interleaved(x[b][j]);
     f32x4 base[MB][GB];                       // without zero points the constant is the same for all columns
     if (!ZERO) {
-      constexpr uint32_t c = Num<T>::P | Num<T>::NEG | 0x00080008u;
+      constexpr uint32_t c = Num<T>::P16 | Num<T>::NEG | 0x00080008u << Num<T>::UNIT;
 #pragma unroll
       for (int b = 0; b < MB; ++b)
 #pragma unroll
@@ -490,7 +496,7 @@ __global__ __launch_bounds__(LW * 64) void w4_few_rows(const LinParams p) {
       for (int i = 0; i < GB; ++i) {
         const float s = i < groups ? bf16_bits_to_f32((uint32_t)(sw[j] >> (16 * i)) & 0xffffu) : 0.f;
         uint32_t c = 0;
-        if (ZERO) c = (Num<T>::P | Num<T>::NEG) | ((uint32_t)(zw[j] >> (8 * i)) & 15u) * 0x10001u;
+        if (ZERO) c = (Num<T>::P16 | Num<T>::NEG) | ((uint32_t)(zw[j] >> (8 * i)) & 15u) * (0x10001u << Num<T>::UNIT);
         f32x4 acc[MB];
 #pragma unroll
         for (int b = 0; b < MB; ++b) acc[b] = ZERO ? none : base[b][i];
@@ -647,7 +653,7 @@ __global__ __launch_bounds__(LW * 64) void w4_few_rows(const LinParams p) {
 
 // Many rows: 80 rows of x (a prompt of 77 tokens) and 384 columns of y to a workgroup of eight waves, 48 columns each.  Blocks of 128 codes with their x come
 // by DMA into three stages in LDS, x in the order of its operands, codes and scales to the wave that uses them.
-// The numbers multiplied are P + q without zero points and P + 16 + q - z with them (z taken off in the integers, four codes at a time); what they are too
+// The numbers multiplied are 16 + q without zero points and 32 + 16 + q - z with them (z taken off in the integers, four codes at a time); what they are too
 // large by is one constant then, and its product with a group's x the same for all columns: a wave computes it for 16 rows of the next block and leaves it in
 // LDS, where every wave's accumulators start from it.
 // A block is 1920 clocks of the matrix unit (two waves of 60 products of 16 x 16 x 32 on a SIMD), about 2100 of the vector unit (codes to operands, the scaled sum of
@@ -728,7 +734,8 @@ __global__ __launch_bounds__(MR_W * 64) __attribute__((amdgpu_waves_per_eu(2, 2)
     if constexpr (ZERO) __builtin_amdgcn_raw_ptr_buffer_load_lds(rz, (lptr_t)(to + Sg::ZAT + wave * 256), 4, so, kb * GB & ~3, 0, 0);
   };
   const f32x4 none = f32x4{0.f, 0.f, 0.f, 0.f};
-  constexpr uint32_t over = (Num<T>::P | Num<T>::NEG) | (ZERO ? 0x00100010u : 0x00080008u);    // -(P + 16), -(P + 8)
+  constexpr int U = ZERO ? Num<T>::UNIT - 1 : Num<T>::UNIT;
+  constexpr uint32_t P = ZERO ? Num<T>::P32 : Num<T>::P16, over = (P | Num<T>::NEG) | (ZERO ? 0x00100010u : 0x00080008u) << U;    // -(32 + 16), -(16 + 8)
   auto x_at = [&](int st, int b, int j) { return *reinterpret_cast<const u32x4*>(smem + st * Sg::BYTES + Sg::XAT + (b * 4 + j) * 1024 + from); };
   auto sums = [&](int st, int odd) {          // a constant's products with the groups of 16 rows
     if (wave >= MR_M) return;
@@ -745,7 +752,7 @@ __global__ __launch_bounds__(MR_W * 64) __attribute__((amdgpu_waves_per_eu(2, 2)
   for (int b = 0; b < MR_M; ++b)
 #pragma unroll
     for (int j = 0; j < MR_N; ++j) out[b][j] = none;
-  uint32_t low = 0x0f0f0f0fu, sixteen = 0x10101010u, power = Num<T>::P;
+  uint32_t low = 0x0f0f0f0fu, sixteen = 0x10101010u, power = P;
   asm("" : "+s"(low));
   asm("" : "+v"(sixteen));
   asm("" : "+s"(power));
@@ -800,8 +807,8 @@ __global__ __launch_bounds__(MR_W * 64) __attribute__((amdgpu_waves_per_eu(2, 2)
         const uint32_t word = w[j][t];
         const uint32_t even = ZERO ? ((word & low) | sixteen) - z[j] : word & low;
         const uint32_t uneven = ZERO ? (((word >> 4) & low) | sixteen) - z[j] : (word >> 4) & low;
-        const u32x4 wv = u32x4{__builtin_amdgcn_perm(uneven, even, 0x0c040c00u) | power, __builtin_amdgcn_perm(uneven, even, 0x0c050c01u) | power,
-                               __builtin_amdgcn_perm(uneven, even, 0x0c060c02u) | power, __builtin_amdgcn_perm(uneven, even, 0x0c070c03u) | power};
+        const u32x4 wv = u32x4{__builtin_amdgcn_perm(uneven, even, 0x0c040c00u) << U | power, __builtin_amdgcn_perm(uneven, even, 0x0c050c01u) << U | power,
+                               __builtin_amdgcn_perm(uneven, even, 0x0c060c02u) << U | power, __builtin_amdgcn_perm(uneven, even, 0x0c070c03u) << U | power};
 #pragma unroll
         for (int b = 0; b < MR_M; ++b) acc[b][j] = Num<T>::mfma(xv[t & 1][b], wv, t % SG == 0 ? base[i & 1][b] : acc[b][j]);
       }

@@ -821,3 +821,32 @@ def test_w4_linear_keeps_rank_products_in_32_bits(M, N, R, dtype):
     # cancel), then the type's, which is that of the numbers below the normal ones in fp16
     bound = 8 * 2.0 ** -24 * 2 * a * b + max(HALF[dtype] * want, 2.0 ** -25 if dtype is FP16 else 0)
     assert (y.cpu().to(F64) - want).abs().max() <= bound, ((y.cpu().to(F64) - want).abs().max().item(), bound, want)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP16])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("M,N,K,group", [(2, 1280, 1280, 64), (16, 320, 4096, 128), (30, 640, 1024, 32), (616, 2000, 1280, 64), (616, 2000, 2048, 128)])
+def test_w4_linear_of_activations_with_a_mean(M, N, K, group, zeros, dtype):
+    """Sums of products with codes lose nothing to what the codes are carried in, also where x does not average out."""
+    from katz_amd import ops
+
+    say("activations with a mean", M, N, K, group, zeros, dtype)
+    g = gen(M + K)
+    groups = K // group
+    codes = (torch.randn(N, K, generator=g) * 2.6 + 8).round().clamp(0, 15).to(torch.uint8)       # (weights without a mean)
+    s = ((torch.rand(N, groups, generator=g) + 0.5) * K ** -0.5 / 4).to(BF)
+    z = torch.randint(7, 10, (N, groups), generator=g).to(torch.uint8) if zeros else torch.full((N, groups), 8, dtype=torch.uint8)
+    x = (torch.randn(M, K, generator=g) + 3).to(dtype)
+    y = ops.w4_linear(on(x), packed(codes, s, z, group, zeros)).cpu().to(F64)
+    v = values(codes, s, z, group)
+    ref = x.to(F64) @ v.t()
+    # The sums are of products with numbers of 31 at most (48 + 15 and 48 with zero points and many rows), codes and what is taken off them: a group's 2 * 4 steps of
+    # the matrix unit with a tree of 32 in each (below 16 roundings in a row), a product, and the chains of groups and of waves, whose terms are the groups' results
+    carried = (63 if zeros and M > 32 else 31) * 2.0
+    mag = x.to(F64).abs() @ (s.to(F64).abs()[:, torch.arange(K) // group] * carried).t()
+    slop = 16 * 2.0 ** -24 * mag + (K // group + 16) * 2.0 ** -24 * (x.to(F64).abs() @ v.abs().t())
+    over = (y - ref).abs() - HALF[dtype] * ref.abs() - slop
+    assert over.max() <= 0, over.max().item()
+    # their errors are of either sign: all of them together are far below the type's rounding
+    nearest = ref.to(dtype).to(F64)
+    assert (y - ref).norm() <= 1.02 * (nearest - ref).norm(), ((y - ref).norm() / (nearest - ref).norm()).item()
