@@ -488,13 +488,18 @@ int kh_block_norm(const void* y, const void* h, const void* gate, int64_t gate_r
  * kh_dequantize_w4: the values in `type`, rounded once, [N, K].
  * kh_w4_linear: y[M,N] = x w^T + bias + ((x A_cat^T) * col_scale) B_cat^T (+ residual), the adapter operands as for kh_lora_linear_bf16 (R % 32 == 0,
  * R <= 128, any K and N), type 0 or 1.  Products with the codes are exact and summed in 32 bits; the rank-R product stays in 32 bits.  A row of x
- * that holds an infinity gives NaN.  workspace: kh_w4_linear_workspace_bytes (0, for instance without an adapter: it may be NULL). */
+ * that holds an infinity gives NaN.  workspace: kh_w4_linear_workspace_bytes (0, for instance without an adapter: it may be NULL).
+ * kh_w4_linear_wide: the same with R up to 65536, what the columns of many adapters add up to, and a workspace of its own size. */
 int kh_quantize_w4(const void* w, void* q, void* scale, void* zero, int64_t N, int64_t K, int64_t group, int type, void* stream);
 int kh_dequantize_w4(const void* q, const void* scale, const void* zero, void* out, int64_t N, int64_t K, int64_t group, int type, void* stream);
 int64_t kh_w4_linear_workspace_bytes(int64_t M, int64_t K, int64_t R);
+int64_t kh_w4_linear_wide_workspace_bytes(int64_t M, int64_t K, int64_t R);
 int kh_w4_linear(const void* x, const void* q, const void* scale, const void* zero, const void* bias, const void* a_cat, const void* b_cat,
                  const float* col_scale, const void* residual, void* y, void* workspace, int64_t M, int64_t N, int64_t K, int64_t R,
                  int64_t group, int type, void* stream);
+int kh_w4_linear_wide(const void* x, const void* q, const void* scale, const void* zero, const void* bias, const void* a_cat, const void* b_cat,
+                      const float* col_scale, const void* residual, void* y, void* workspace, int64_t M, int64_t N, int64_t K, int64_t R,
+                      int64_t group, int type, void* stream);
 /* Linear attention with a decay for each head:  S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T,   o_t = scale * q_t S_t.
  * q [.., H * dk], k [.., kv_heads * dk], v [.., kv_heads * dv], o [.., H * dv] bf16, dk 64 or 128, dv a multiple of 64 up to 1024; query head h takes
  * key head h / (H / kv_heads).  log_decay float [H], <= 0 (-inf: no memory).  Rows through strides in elements (multiples of 8): dense [B, T] with

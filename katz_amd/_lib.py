@@ -71,6 +71,8 @@ SIGNATURES = {
     "kh_dequantize_w4": (c_int, [_P] * 4 + [_I] * 3 + [c_int, _P]),
     "kh_w4_linear_workspace_bytes": (_I, [_I] * 3),
     "kh_w4_linear": (c_int, [_P] * 11 + [_I] * 5 + [c_int, _P]),
+    "kh_w4_linear_wide_workspace_bytes": (_I, [_I] * 3),
+    "kh_w4_linear_wide": (c_int, [_P] * 11 + [_I] * 5 + [c_int, _P]),
     "kh_linear_attention_workspace_bytes": (_I, [_I] * 6),
     "kh_linear_attention_bf16": (c_int, [_P] * 8 + [_I, _P, _I, _P] + [_I] * 14 + [c_float, _P]),
     "kh_linear_attention_step_bf16": (c_int, [_P] * 8 + [_I] * 10 + [c_float, c_int, _P]),

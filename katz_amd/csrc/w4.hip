@@ -842,7 +842,7 @@ __global__ __launch_bounds__(MR_W * 64) __attribute__((amdgpu_waves_per_eu(2, 2)
       const int id = wave + i * MR_W, r = id / 3 * 16 + dr;
       if (id < 3 * MR_M)
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rt, (lptr_t)(to + Sg::XAT + id * 1024), 16, (int)(((uint32_t)(r < rows ? r : rows - 1) * (uint32_t)p.R + dp * 8) * 2),
-                                                 (int)((uint32_t)(id % 3 * p.M * p.R + step * 32) * 2), 0, 0);   // (below 2^32: M <= 2^20, R <= 128)
+                                                 (int)((uint32_t)(id % 3 * p.M * p.R + step * 32) * 2), 0, 0);   // (below 2^32: see `many` at the entry)
     }
 #pragma unroll
     for (int j = 0; j < MR_N; ++j) {
@@ -1106,8 +1106,8 @@ bool many_rows(long M, long N, long K) {
 }
 
 template <typename T>
-int launch_linear(const LinParams& p, int G, hipStream_t s) {
-  if (many_rows(p.M, p.N, p.K)) {
+int launch_linear(const LinParams& p, int G, bool many, hipStream_t s) {
+  if (many) {
     if (p.zero) return G == 32 ? launch_many<T, 32, true>(p, s) : G == 64 ? launch_many<T, 64, true>(p, s) : launch_many<T, 128, true>(p, s);
     return G == 32 ? launch_many<T, 32, false>(p, s) : G == 64 ? launch_many<T, 64, false>(p, s) : launch_many<T, 128, false>(p, s);
   }
@@ -1159,24 +1159,26 @@ KH_EXPORT int kh_dequantize_w4(const void* q, const void* scale, const void* zer
   KH_RETURN_LAST_ERROR();
 }
 
-KH_EXPORT int64_t kh_w4_linear_workspace_bytes(int64_t M, int64_t K, int64_t R) {
-  if (M <= 0 || K <= 0 || R < 0 || R % 32 != 0 || R > 128) return KH_ERR_INVALID_ARG;
+namespace {
+
+int64_t linear_workspace(int64_t M, int64_t K, int64_t R, int64_t most) {
+  if (M <= 0 || K <= 0 || R < 0 || R % 32 != 0 || R > most) return KH_ERR_INVALID_ARG;
   if (R == 0 || own_t(M, K, R)) return 0;
   const int64_t parts = (int64_t)shrink_splits(M, K, R) * 4;
   return (M > 32 && parts < 6 ? 6 : parts) * M * R;         // (t in 32 bits for each split, or, for many rows, in three pieces of 16)
 }
 
-KH_EXPORT int kh_w4_linear(const void* x, const void* q, const void* scale, const void* zero, const void* bias, const void* a_cat,
-                           const void* b_cat, const float* col_scale, const void* residual, void* y, void* workspace, int64_t M, int64_t N,
-                           int64_t K, int64_t R, int64_t group, int type, void* stream) {
+int linear(const void* x, const void* q, const void* scale, const void* zero, const void* bias, const void* a_cat, const void* b_cat,
+           const float* col_scale, const void* residual, void* y, void* workspace, int64_t M, int64_t N,
+           int64_t K, int64_t R, int64_t most, int64_t group, int type, void* stream) {
   if (!x || !q || !scale || !y || M <= 0 || N <= 0 || K <= 0 || R < 0 || type < 0 || type > 1) return KH_ERR_INVALID_ARG;
   const bool own = own_t(M, K, R);
   if (R > 0 && (!a_cat || !b_cat || !col_scale || (!workspace && !own))) return KH_ERR_INVALID_ARG;
   if (!group_ok(group) || R % 32 != 0) return KH_ERR_UNSUPPORTED;
-  if (R > 128 || K > (1L << 24) || N > (1L << 24) || (M + 15) / 16 > 65535) return KH_ERR_TOO_LARGE;
+  if (R > most || K > (1L << 24) || N > (1L << 24) || (M + 15) / 16 > 65535) return KH_ERR_TOO_LARGE;
   if (!kh_aligned16(q) || ((uintptr_t)scale & 7) || ((uintptr_t)zero & 3)) return KH_ERR_ALIGNMENT;   // (any whole rows of larger ones)
   hipStream_t s = (hipStream_t)stream;
-  const bool many = many_rows(M, N, K);
+  const bool many = many_rows(M, N, K) && 3 * M * R <= 0x7fffffffL;      // (the ranks' pieces lie within 4 GB)
   const int splits = R == 0 ? 0 : many ? 1 : shrink_splits(M, K, R);
   if (R > 0 && !own) {
     const int per = (int)(((K + splits - 1) / splits + 31) / 32 * 32);
@@ -1190,7 +1192,26 @@ KH_EXPORT int kh_w4_linear(const void* x, const void* q, const void* scale, cons
   LinParams p{x, (const uint8_t*)q, (const bf16_t*)scale, (const uint8_t*)zero, bias, b_cat, residual, (const float*)workspace, y, (long)M,
               (long)N, (int)K, (int)R, splits, (int)((K + 31) / 32 * 16), (int)(((K + group - 1) / group + 3) / 4 * 4),
               ((uintptr_t)x & 3) == 0 && K % 2 == 0 && (!own || ((uintptr_t)a_cat & 3) == 0), own ? a_cat : nullptr, col_scale, 0, ((uintptr_t)b_cat & 3) == 0, M * N >= 4 << 20};
-  const int rc = type == 0 ? launch_linear<bf16_t>(p, (int)group, s) : launch_linear<_Float16>(p, (int)group, s);
+  const int rc = type == 0 ? launch_linear<bf16_t>(p, (int)group, many, s) : launch_linear<_Float16>(p, (int)group, many, s);
   if (rc != KH_OK) return rc;
   KH_RETURN_LAST_ERROR();
+}
+
+}  // namespace
+
+// Rank columns: as many as K1's entry points take, or (wide) what many adapters add up to.
+constexpr int64_t RANKS = 128, RANKS_WIDE = 1 << 16;
+
+KH_EXPORT int64_t kh_w4_linear_workspace_bytes(int64_t M, int64_t K, int64_t R) { return linear_workspace(M, K, R, RANKS); }
+KH_EXPORT int64_t kh_w4_linear_wide_workspace_bytes(int64_t M, int64_t K, int64_t R) { return linear_workspace(M, K, R, RANKS_WIDE); }
+
+KH_EXPORT int kh_w4_linear(const void* x, const void* q, const void* scale, const void* zero, const void* bias, const void* a_cat,
+                           const void* b_cat, const float* col_scale, const void* residual, void* y, void* workspace, int64_t M, int64_t N,
+                           int64_t K, int64_t R, int64_t group, int type, void* stream) {
+  return linear(x, q, scale, zero, bias, a_cat, b_cat, col_scale, residual, y, workspace, M, N, K, R, RANKS, group, type, stream);
+}
+KH_EXPORT int kh_w4_linear_wide(const void* x, const void* q, const void* scale, const void* zero, const void* bias, const void* a_cat,
+                                const void* b_cat, const float* col_scale, const void* residual, void* y, void* workspace, int64_t M, int64_t N,
+                                int64_t K, int64_t R, int64_t group, int type, void* stream) {
+  return linear(x, q, scale, zero, bias, a_cat, b_cat, col_scale, residual, y, workspace, M, N, K, R, RANKS_WIDE, group, type, stream);
 }

@@ -403,6 +403,7 @@ class LoRALinearW4(nn.Module):
         self.adapters_enabled = True
         self._packed: Optional[PackedAdapters] = None
         self._packed_key = None
+        self._operands = None    # of _packed, as the kernel takes them
         self._fused: set = set()
         self.packed_weight()
 
@@ -487,6 +488,21 @@ class LoRALinearW4(nn.Module):
             return
         self._packed = pack_adapters(self.adapters, names, self.in_features, self.out_features, self.dtype, self.weight_q.device, self.global_scale)
         self._packed_key = key
+        self._operands = None if self._packed is None else self._side_by_side(self._packed)
+
+    @staticmethod
+    def _side_by_side(p: PackedAdapters):
+        """(A_cat, B_cat, col_scale) of all packs as one, of which the packs become views: the kernel takes any number of rank columns at once, in 32 bits."""
+        if not p.wide:
+            return p.a_cat, p.b_cat, p.col_scale
+        packs = [p, *p.overflow]
+        a, b, s = torch.cat([k.a_cat for k in packs]), torch.cat([k.b_cat for k in packs], 1), torch.cat([k.col_scale for k in packs])
+        at = 0
+        for k in packs:
+            R = k.R
+            k.a_cat, k.b_cat, k.col_scale = a[at:at + R], b[:, at:at + R], s[at:at + R]
+            at += R
+        return a, b, s
 
     def fuse(self, lora_scale: float = 1.0, names: Optional[Sequence[str]] = None) -> None:
         """The adapters merged into the weights, which are quantised anew (there is no way back: what was rounded off is gone).  Not finite: left as it was."""
@@ -504,19 +520,14 @@ class LoRALinearW4(nn.Module):
         self.refresh_adapters()
 
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
-        p = self._packed
+        o = self._operands
         w, b = self.packed_weight(), None if self.bias is None else self.bias.detach()
-        if p is None:
+        if o is None:
             return ops.w4_linear(x, w, b, residual=residual)
-        if p.a_cat.device != x.device or p.a_cat.dtype != self.dtype:      # the layer was moved or converted
+        if o[0].device != x.device or o[0].dtype != self.dtype:            # the layer was moved or converted
             self.refresh_adapters()
-            p = self._packed
-        y = ops.w4_linear(x, w, b, p.a_cat, p.b_cat, p.col_scale, residual=residual)
-        for c in p.overflow:                # more rank columns than one launch takes, as LoRALinear does it
-            t = ops.lora_linear(x, c.a_cat, None)
-            t.mul_(c.col_scale.to(t.dtype))
-            y = ops.lora_linear(t, c.b_cat, None, residual=y)
-        return y
+            o = self._operands
+        return ops.w4_linear(x, w, b, *o, residual=residual, wide=o[0].shape[0] > MAX_PACKED_RANK)
 
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}, group={self.group}, zeros={self.weight_zero is not None}"

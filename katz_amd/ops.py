@@ -1470,9 +1470,9 @@ def dequantize_w4(w: W4Weight, dtype: torch.dtype = BF16, out: Optional[torch.Te
 
 def w4_linear(x: torch.Tensor, w: W4Weight, bias: Optional[torch.Tensor] = None, a_cat: Optional[torch.Tensor] = None,
               b_cat: Optional[torch.Tensor] = None, col_scale: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
-              out: Optional[torch.Tensor] = None) -> torch.Tensor:
+              out: Optional[torch.Tensor] = None, wide: bool = False) -> torch.Tensor:
     """y = x w^T + b + ((x A_cat^T) * col_scale) B_cat^T (+ residual) with weights in 4 bits, bf16 or fp16 by x.dtype; the adapter operands as
-    for lora_linear (a_cat [R,K], b_cat [N,R], col_scale [R] fp32, R % 32 == 0, R <= 128).  Made for few rows, right for any number.  A row of x that
+    for lora_linear (a_cat [R,K], b_cat [N,R], col_scale [R] fp32, R % 32 == 0, R <= 128; wide: <= 65536).  Made for few rows, right for any number.  A row of x that
     holds an infinity gives NaN."""
     lib = _lib.load()
     dt, xs, q = x.dtype, x.shape, w.q
@@ -1507,13 +1507,14 @@ def w4_linear(x: torch.Tensor, w: W4Weight, bias: Optional[torch.Tensor] = None,
         return out
     ws = None
     if R:
-        nbytes = _workspace_bytes("kh_w4_linear_workspace_bytes", M, K, R)
+        nbytes = _workspace_bytes("kh_w4_linear_wide_workspace_bytes" if wide else "kh_w4_linear_workspace_bytes", M, K, R)
         if nbytes < 0:
-            raise ValueError(f"the adapters' columns must be a multiple of 32 up to 128, got {R}")
+            raise ValueError(f"the adapters' columns must be a multiple of 32 up to {65536 if wide else 128}, got {R}")
         if nbytes:
             ws = x.new_empty(nbytes // 2)      # (elements of two bytes)
-    rc = lib.kh_w4_linear(x.data_ptr(), q.data_ptr(), w.scale.data_ptr(), _ptr(w.zero), _ptr(bias), _ptr(a_cat), _ptr(b_cat), _ptr(col_scale),
-                          _ptr(residual), out.data_ptr(), _ptr(ws), M, N, K, R, w.group, _TYPES[dt], _stream())
+    rc = (lib.kh_w4_linear_wide if wide else lib.kh_w4_linear)(
+        x.data_ptr(), q.data_ptr(), w.scale.data_ptr(), _ptr(w.zero), _ptr(bias), _ptr(a_cat), _ptr(b_cat), _ptr(col_scale),
+        _ptr(residual), out.data_ptr(), _ptr(ws), M, N, K, R, w.group, _TYPES[dt], _stream())
     if rc:
         _lib.check(rc, "kh_w4_linear")
     return out

@@ -305,3 +305,40 @@ def test_names_that_were_fused_are_free_for_other_adapters():
     fused_first()                                                    # the weights from before it was merged
     layer.load_state_dict(saved)
     close(layer(x), want(*ads[0]), "loaded anew")
+
+
+@pytest.mark.parametrize("M", [1, 5, 40, 700])
+@pytest.mark.parametrize("dtype,N,K,ranks", [(torch.float16, 96, 128, (64, 64, 16)), (BF, 1283, 2050, (96, 80)), (torch.float16, 4103, 70, (200,)), (BF, 4100, 640, (128, 128, 128, 5))])
+def test_layer_with_more_rank_columns_than_one_pack(M, dtype, N, K, ranks):
+    """Any type and size that the layer has, in one launch: no rounding between the packs."""
+    from katz_amd import ops
+    from katz_amd.layers import LoRALinearW4
+
+    g = torch.Generator().manual_seed(M + N)
+    layer = LoRALinearW4(K, N, group=32, zeros=True, device=DEV, dtype=dtype)
+    layer._assign(ops.quantize_w4((torch.randn(N, K, generator=g) * K ** -0.5).to(DEV), 32, True))
+    layer.bias.data.copy_(torch.randn(N, generator=g))
+    x, res = (torch.randn(M, n, generator=g).to(dtype) for n in (K, N))
+    xd = x.to(F64)
+    w = ops.dequantize_w4(layer.packed_weight(), torch.float32).cpu().to(F64)
+    parts = [xd @ w.t(), layer.bias.detach().cpu().to(F64), res.to(F64)]
+    mag = [48 * 2 * xd.abs() @ w.abs().amax(1, keepdim=True).expand(N, K).t(), parts[1].abs(), parts[2].abs()]       # (codes are carried in numbers of 63 at most: 9 values' steps each)
+    names = [f"a{i}" for i in range(len(ranks))]
+    for i, (n, r) in enumerate(zip(names, ranks)):
+        down, up = (torch.randn(r, K, generator=g) * K ** -0.5).to(dtype), (torch.randn(N, r, generator=g) * 0.1).to(dtype)
+        layer.add_adapter(n, down, up, alpha=r * (i + 1) / 4)
+        parts.append((i + 1) / 4 * (xd @ down.to(F64).t()) @ up.to(F64).t())
+        mag.append((i + 1) / 4 * (xd.abs() @ down.to(F64).abs().t()) @ up.to(F64).abs().t())
+    layer.set_active(names)
+    assert layer._packed.wide
+    # 64 roundings in 32 bits of a term at most: groups and waves, a rank's product and its sum
+    half = torch.finfo(dtype).eps / 2
+    for scale in (1.0, 0.5):
+        layer.set_global_scale(scale)
+        ref, slop = sum(parts[:3]) + scale * sum(parts[3:]), 64 * 2.0 ** -24 * (sum(mag[:3]) + scale * sum(mag[3:]))
+        y = layer(x.to(DEV), residual=res.to(DEV)).cpu().to(F64)
+        assert ((y - ref).abs() <= half * ref.abs() + slop).all()
+    before, operands = layer(x.to(DEV)), layer._operands
+    layer.set_global_scale(1.0)
+    assert all(a is b for a, b in zip(layer._operands, operands)) or layer._operands[2].data_ptr() == operands[2].data_ptr()   # a captured graph stays valid
+    assert not torch.equal(layer(x.to(DEV)), before)

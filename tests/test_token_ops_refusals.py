@@ -166,3 +166,11 @@ def test_launches_that_would_be_too_large(lib):
     assert norm(1 << 26, 64) == -4 and norm(1 << 24, 4096) == -4 and norm(1 << 22, 32768) == -4
     linear = lambda s=16, z=None: lib.kh_w4_linear(16, 16, s, z, None, None, None, None, None, 16, None, 2, 8, 64, 0, 64, 0, None)      # noqa: E731
     assert linear(s=20) == -3 and linear(z=18) == -3
+
+
+def test_wide_linears(lib):
+    """More rank columns than the adapters' other entry points take, up to a limit of its own."""
+    size = lib.kh_w4_linear_wide_workspace_bytes
+    assert size(1, 64, 160) > 0 and size(40, 1280, 160) >= 6 * 40 * 160 and size(1, 64, 150) == -1 and size(1, 64, 65568) == -1 and size(1, 64, 32) == 0
+    wide = lambda R, ws=16, g=64: lib.kh_w4_linear_wide(16, 16, 16, None, None, 16, 16, 16, None, 16, ws, 2, 8, 64, R, g, 0, None)      # noqa: E731
+    assert wide(65568) == -4 and wide(150) == -2 and wide(160, ws=None) == -1 and wide(160, g=48) == -2
