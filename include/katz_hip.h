@@ -488,7 +488,7 @@ int kh_block_norm(const void* y, const void* h, const void* gate, int64_t gate_r
  * kh_dequantize_w4: the values in `type`, rounded once, [N, K].
  * kh_w4_linear: y[M,N] = x w^T + bias + ((x A_cat^T) * col_scale) B_cat^T (+ residual), the adapter operands as for kh_lora_linear_bf16 (R % 32 == 0,
  * R <= 128, any K and N), type 0 or 1.  Products with the codes are exact and summed in 32 bits; the rank-R product stays in 32 bits.  A row of x
- * that holds an infinity gives NaN.  workspace: kh_w4_linear_workspace_bytes (0, for instance without an adapter: it may be NULL).
+ * that holds an infinity gives NaN.  workspace: kh_w4_linear_workspace_bytes (0, for instance without an adapter: it may be NULL), aligned to 16 bytes.
  * kh_w4_linear_wide: the same with R up to 65536, what the columns of many adapters add up to, and a workspace of its own size. */
 int kh_quantize_w4(const void* w, void* q, void* scale, void* zero, int64_t N, int64_t K, int64_t group, int type, void* stream);
 int kh_dequantize_w4(const void* q, const void* scale, const void* zero, void* out, int64_t N, int64_t K, int64_t group, int type, void* stream);

@@ -1177,6 +1177,7 @@ int linear(const void* x, const void* q, const void* scale, const void* zero, co
   if (!group_ok(group) || R % 32 != 0) return KH_ERR_UNSUPPORTED;
   if (R > most || K > (1L << 24) || N > (1L << 24) || (M + 15) / 16 > 65535) return KH_ERR_TOO_LARGE;
   if (!kh_aligned16(q) || ((uintptr_t)scale & 7) || ((uintptr_t)zero & 3)) return KH_ERR_ALIGNMENT;   // (any whole rows of larger ones)
+  if (R > 0 && ((!own && !kh_aligned16(workspace)) || ((uintptr_t)col_scale & 3))) return KH_ERR_ALIGNMENT;
   hipStream_t s = (hipStream_t)stream;
   const bool many = many_rows(M, N, K) && 3 * M * R <= 0x7fffffffL;      // (the ranks' pieces lie within 4 GB)
   const int splits = R == 0 ? 0 : many ? 1 : shrink_splits(M, K, R);

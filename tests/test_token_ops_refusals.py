@@ -174,3 +174,10 @@ def test_wide_linears(lib):
     assert size(1, 64, 160) > 0 and size(40, 1280, 160) >= 6 * 40 * 160 and size(1, 64, 150) == -1 and size(1, 64, 65568) == -1 and size(1, 64, 32) == 0
     wide = lambda R, ws=16, g=64: lib.kh_w4_linear_wide(16, 16, 16, None, None, 16, 16, 16, None, 16, ws, 2, 8, 64, R, g, 0, None)      # noqa: E731
     assert wide(65568) == -4 and wide(150) == -2 and wide(160, ws=None) == -1 and wide(160, g=48) == -2
+
+
+def test_w4_linear_refuses_workspaces_and_scales_off_their_alignment(lib):
+    """The ranks' products are read from the workspace 16 bytes at a time, column scales as floats."""
+    for f in (lib.kh_w4_linear, lib.kh_w4_linear_wide):
+        call = lambda ws=16, c=16, M=2, K=8192, R=64: f(16, 16, 16, None, None, 16, 16, c, None, 16, ws, M, 8, K, R, 64, 0, None)      # noqa: E731
+        assert call(ws=20) == -3 and call(ws=24, M=700) == -3 and call(c=18) == -3 and call(ws=None, c=18, K=64) == -3
