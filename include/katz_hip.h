@@ -482,7 +482,7 @@ int kh_block_norm(const void* y, const void* h, const void* gate, int64_t gate_r
                   int type, int stream_type, void* stream);
 /* Weights in 4 bits: w[n][k] = scale[n][k / group] * (code[n][k] - zero[n][k / group]), group 32, 64 or 128, zero = 8 where it is NULL.
  *   q      [N, ceil(K / 32) * 16] bytes: code 2i in the low half of byte i, 2i + 1 in the high one, filled up to 32 codes
- *   scale  [N, ceil(groups / 4) * 4] bf16, zero [the same] uint8 (0..15), groups = ceil(K / group)
+ *   scale  [N, ceil(groups / 4) * 4] bf16, zero [the same] uint8 (0..15: the lower four bits), groups = ceil(K / group)
  * kh_quantize_w4: scale = bf16(largest magnitude / 7), or with zero points bf16((max(w, 0) - min(w, 0)) / 15) and zero = rint(-min / scale); codes are
  * rint(w / scale) + zero within 0..15 (halves to even).  A group that holds a NaN gets a NaN as its scale, one that holds an infinity an infinity.
  * kh_dequantize_w4: the values in `type`, rounded once, [N, K].

@@ -194,7 +194,7 @@ __global__ __launch_bounds__(256) void values_kernel(const ValueParams p) {
     const int last = (p.K - 1) >> (3 + p.gshift), g = u[i] >> p.gshift;      // (words behind the last weight may lie behind the last group)
     word[i] = p.q[r * p.pieces.per_row + u[i]];
     s[i] = p.scale[r * p.gstride + (g < last ? g : last)];
-    z[i] = p.zero ? p.zero[r * p.gstride + (g < last ? g : last)] : 8;
+    z[i] = p.zero ? p.zero[r * p.gstride + (g < last ? g : last)] & 15 : 8;      // (as the linear takes it)
   }
 #pragma unroll
   for (int i = 0; i < PT; ++i) {

@@ -1402,7 +1402,7 @@ class W4Weight:
     """A linear's weights [N, K] in 4 bits by groups along K: w[n, k] = scale[n, k // group] * (code[n, k] - zero[n, k // group]).
 
     q uint8 [N, ceil(K / 32) * 16]: code 2 i in the low half of byte i, 2 i + 1 in the high one; scale bf16 [N, groups filled up to a multiple of 4];
-    zero None (8 everywhere) or uint8 of scale's shape, 0 .. 15; group 32, 64 or 128."""
+    zero None (8 everywhere) or uint8 of scale's shape, 0 .. 15 (the lower four bits); group 32, 64 or 128."""
     __slots__ = ("q", "scale", "zero", "in_features", "out_features", "group", "groups")
 
     def __init__(self, q: torch.Tensor, scale: torch.Tensor, zero: Optional[torch.Tensor], in_features: int, group: int):

@@ -850,3 +850,15 @@ def test_w4_linear_of_activations_with_a_mean(M, N, K, group, zeros, dtype):
     # their errors are of either sign: all of them together are far below the type's rounding
     nearest = ref.to(dtype).to(F64)
     assert (y - ref).norm() <= 1.02 * (nearest - ref).norm(), ((y - ref).norm() / (nearest - ref).norm()).item()
+
+
+@pytest.mark.parametrize("M,N", [(2, 40), (20, 40), (700, 4100)])
+def test_zero_points_are_their_lower_four_bits(M, N):
+    """For the values as for the linear, whatever the upper bits of their bytes hold."""
+    from katz_amd import ops
+
+    r = gen(21)
+    w = ops.quantize_w4(on(randn(r, N, 200, std=0.1)), 64, zeros=True)
+    x = on(randn(r, M, 200))
+    other = ops.W4Weight(w.q, w.scale, w.zero | 0xB0, 200, 64)
+    assert torch.equal(ops.dequantize_w4(other), ops.dequantize_w4(w)) and torch.equal(ops.w4_linear(x, other), ops.w4_linear(x, w))
