@@ -819,7 +819,11 @@ int prompt(const LaParams& p, long heads, hipStream_t s) {
       if (e != hipSuccess) return (int)e;
     }
     kh_launch(KH_TAG_LINEAR_ATTENTION, la_gain<DK, TV>, grid, block, gain_lds, s, p);
+    hipError_t e = hipGetLastError();                 // (the launch behind it reads what it writes)
+    if (e != hipSuccess) return (int)e;
     kh_launch(KH_TAG_LINEAR_ATTENTION, la_scan<DK, TV>, dim3(DK / 16, (unsigned)heads), block, 0, s, p);
+    e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
     kh_launch(KH_TAG_LINEAR_ATTENTION, la_out<DK, TV, false>, grid, block, lds, s, p);
   }
   KH_RETURN_LAST_ERROR();

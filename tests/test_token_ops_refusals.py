@@ -1,5 +1,9 @@
 """What the operators of a block that answers token by token refuse, without a GPU: the C entry points before any device call, the
 tensor functions by type, shape and place."""
+import shutil
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -181,3 +185,45 @@ def test_w4_linear_refuses_workspaces_and_scales_off_their_alignment(lib):
     for f in (lib.kh_w4_linear, lib.kh_w4_linear_wide):
         call = lambda ws=16, c=16, M=2, K=8192, R=64: f(16, 16, 16, None, None, 16, 16, c, None, 16, ws, M, 8, K, R, 64, 0, None)      # noqa: E731
         assert call(ws=20) == -3 and call(ws=24, M=700) == -3 and call(c=18) == -3 and call(ws=None, c=18, K=64) == -3
+
+
+# A HIP runtime's calls for launches, of which the fail_at-th fails as one does: an error that the next hipGetLastError returns and clears.
+LAUNCHES = """
+typedef struct { unsigned x, y, z; } dim3;
+int launches, fail_at;
+static int last;
+int __hipPushCallConfiguration(dim3 g, dim3 b, unsigned long lds, void* s) { return 0; }
+int __hipPopCallConfiguration(dim3* g, dim3* b, unsigned long* lds, void** s) { dim3 one = {1, 1, 1}; *g = *b = one; *lds = 0; *s = 0; return 0; }
+int hipLaunchKernel(const void* f, dim3 g, dim3 b, void** args, unsigned long lds, void* s) { if (++launches == fail_at) last = 719; return launches == fail_at ? 719 : 0; }
+int hipGetLastError(void) { int e = last; last = 0; return e; }
+int hipGetDevice(int* d) { *d = 0; return 0; }
+int hipFuncSetAttribute(const void* f, int a, int v) { return 0; }
+"""
+CALLS = """
+import ctypes, sys
+fake = ctypes.CDLL(sys.argv[1], mode=ctypes.RTLD_GLOBAL)
+from katz_amd import _lib
+lib = _lib.load()
+calls = {"prompt": (3, lambda: lib.kh_linear_attention_bf16(16, 16, 16, 16, 16, None, 16, None, 1, None, 0, 16, 1, 2, 2, 4096, 64, 64, *[128] * 4, *[0] * 4, 0.1, None)),
+         "linear": (2, lambda: lib.kh_w4_linear(16, 16, 16, None, None, 16, 16, 16, None, 16, 16, 2, 8, 8192, 64, 64, 0, None))}
+count, failing = ctypes.c_int.in_dll(fake, "launches"), ctypes.c_int.in_dll(fake, "fail_at")
+for name, (n, call) in calls.items():
+    for at in range(n + 1):
+        count.value, failing.value = 0, at
+        rc = call()
+        print(name, n, at, rc, count.value)
+"""
+
+
+def test_a_launch_that_fails_ends_its_call(lib, tmp_path):
+    """Whichever launch of a call fails, the call returns that error and launches nothing behind it, which would read what the failed one has not written."""
+    if not shutil.which("gcc"):
+        pytest.skip("no gcc")
+    (tmp_path / "launches.c").write_text(LAUNCHES)
+    subprocess.run(["gcc", "-shared", "-fPIC", "-w", "-o", str(tmp_path / "launches.so"), str(tmp_path / "launches.c")], check=True)
+    run = subprocess.run([sys.executable, "-c", CALLS, str(tmp_path / "launches.so")], capture_output=True, text=True, timeout=120)
+    assert run.returncode == 0, run.stderr
+    lines = [line.split() for line in run.stdout.splitlines()]
+    assert len(lines) == 7
+    for name, n, at, rc, count in lines:
+        assert (rc, count) == (("0", n) if at == "0" else ("719", at)), (name, at, rc, count)
