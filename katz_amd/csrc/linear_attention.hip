@@ -114,6 +114,7 @@ typedef __amdgpu_buffer_rsrc_t rsrc_t;
 // All loads and stores but the last VM are done (they end in the order of their issue).
 template <int VM = 0>
 __device__ __forceinline__ void wait_vm() {
+  static_assert(VM < 16, "the counter's lower four bits; the upper ones, 14 and 15, stay 0");
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_waitcnt(VM | (7 << 4) | (15 << 8));   // the other counters unconstrained (gfx9 encoding)
   asm volatile("" ::: "memory");
@@ -556,14 +557,12 @@ __global__ __launch_bounds__(TV * 4) __attribute__((amdgpu_waves_per_eu(2, 2))) 
   const uint32_t ocol = (wave * 16 + (grp >> 1) * 8) * 2;
   bool ends = ONE || t1 == u.len;          // the sequence, in this chunk
 
-  bool first = true;                       // sequence of the chunk
   int stage = 0;                           // the block's; a8, kcol and vcol lie in it
   auto block = [&](int c) {
     constexpr int KT = 0, QT = Tile<DK>::BYTES;
     const int other = Sh::STAGE - stage;
     if (c != t0) wait_vm<2>();             // (the outputs of the block before may still be on their way)
-    else if (first) wait_vm();
-    else wait_vm<DK / 4>();                // (or the state behind the sequence before: a store for each of a lane's numbers, behind this block's loads)
+    else wait_vm();                        // (a sequence's first block: the state behind the one before is waited for with it)
     barrier();                             // everybody's share of this block; and nobody reads the block before any more
     if (c + C < t1) fetch(c + C, other);
     {
@@ -702,7 +701,6 @@ __global__ __launch_bounds__(TV * 4) __attribute__((amdgpu_waves_per_eu(2, 2))) 
         t1 = u.len <= left * (long)C ? u.len : left * C;
         barrier();                         // the stages are dead
         fetch(0, stage);
-        asm volatile("" ::: "memory");     // (in front of the stores)
       }
     }
     if (ends)
@@ -713,7 +711,6 @@ __global__ __launch_bounds__(TV * 4) __attribute__((amdgpu_waves_per_eu(2, 2))) 
         for (int r = 0; r < 4; ++r) p.s_out[at + (long)r * p.dv] = st.s[t][r];
       }
     if (!more) break;
-    first = false;
     state_in();
     ends = t1 == u.len;
     powers(u.g, C, w);
