@@ -761,26 +761,30 @@ __global__ __launch_bounds__(256) void la_step(const LaParams p) {
 struct Plan { long heads; int tv, chunks; };      // heads: units of a sequence
 
 // 128 columns of v to a workgroup (which computes the scores once for them) where dv has them.
-// Chunks: a workgroup goes through its blocks one after the other (about 4 us a block with dk 128, 2.3 with 64, whatever else runs), so few heads are cut; but a
-// chunk's state is written, read, written and read again, and the rounds that the workgroups make on 256 CUs are whole ones.  Measured, us for whole sequences | 8 |
-// 16 | 24 | 32 chunks: 8 packed sequences of 1 .. 8192 tokens, 16384 in all, 16 heads of 128 458 | 194 | 122 | 148 | 136, one sequence of 16384 898 | 195 | 121 |
-// 148 | 137, 16 of 1024 81 | 150 | 92 | 154 | 133, 2 x 4096 tokens of 20 heads of 64 130 | 66 | 54 | 48 | 55, one of 1024 33 | 21 | 25 | 25 | 25.
+// Chunks: a workgroup goes through its blocks one after the other (t_block us each, whatever else runs), so few heads are cut; but a
+// chunk's state is written, read, written and read again, and the rounds that the workgroups make on 256 CUs, as many to one as its LDS holds, are whole ones.
+// Measured, us for whole sequences | 8 | 12 | 16 | 25 | 32 chunks, dk x dv: 8 packed sequences of 0 .. 8192 tokens, 16384 in all, 16 heads of 128 x 128
+// 530 | 220 | 157 | 134 | 170 | 157, 64 x 128 386 | 173 | 124 | 105 | 129 | 115, 128 x 64 412 | 182 | 130 | 110 | 129 | 115, 64 x 64 300 | 138 | 100 | 85 | 80 | 74;
+// 16 of 1024 128 x 128 87 | 171 | 153 | 99 | 166 | 142; 2 x 4096 of 20 heads 64 x 128 193 | 90 | 70 | 92 | 79 | 91, 64 x 64 152 | 72 | 57 | 58 | 50 | 57;
+// one of 1024 of 16 heads 64 x 64 39 | 21.5 | 22.5 | 22.5.  Over 36 such cases what is chosen here takes 0.3 % more than the best of 21 counts, 5 % at most.
 Plan plan_of(long B, long H, long dk, long dv, long T, long rows) {
   Plan r;
   r.tv = dv % 128 == 0 ? 128 : 64;
   r.heads = H * (dv / r.tv);
   r.chunks = 0;
   const long blocks = (T + C - 1) / C, dense = B * blocks, packed = rows / C + B, all = dense < packed ? dense : packed;
-  const double t_block = dk == 128 ? 3.8 : 2.3;
-  const long slots = dk == 128 ? 256 : 512;           // workgroups that LDS lets run at once
+  const bool wide = r.tv == 128;
+  const double t_block = dk == 128 ? (wide ? 4.15 : 3.2) : wide ? 3.0 : 2.33;
+  const int lds = dk == 128 ? (wide ? OutShape<128, 128>::LDS : OutShape<128, 64>::LDS) : wide ? OutShape<64, 128>::LDS : OutShape<64, 64>::LDS;
+  const long slots = 256 * (160 * 1024 / lds);        // workgroups of la_out that run at once
   auto rounds = [](long wgs, long n) { return (double)((wgs + n - 1) / n); };
-  double best = rounds(B * r.heads, slots) * blocks * t_block * 1.15;    // whole sequences (the state needs its third piece everywhere)
+  double best = rounds(B * r.heads, slots) * blocks * t_block * 1.03;    // whole sequences
   if (r.heads > 65535) return r;                      // (la_scan's grid)
   static const int counts[] = {2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14, 15, 16, 18, 20, 22, 25, 28, 32, 36, 42, 51, 64, 85, 102, 128, 170, 256};
   for (const long n : counts) {
     const long size = (all + n - 1) / n;
     if (n > all || n * r.heads * dk * r.tv * 8 > 4L << 30) break;
-    const double t = 14. + size * t_block * (rounds(n * r.heads, slots) + 0.6 * rounds(n * r.heads, 512)) + 0.3 * n + n * r.heads * (double)(dk * r.tv * 16) / 4e6;
+    const double t = 14. + size * t_block * (rounds(n * r.heads, slots) + 0.5 * rounds(n * r.heads, 512)) + 0.3 * n + n * r.heads * (double)(dk * r.tv * 16) / 4e6;
     if (t < best) { best = t; r.chunks = (int)n; }
   }
   return r;

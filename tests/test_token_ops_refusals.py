@@ -227,3 +227,17 @@ def test_a_launch_that_fails_ends_its_call(lib, tmp_path):
     assert len(lines) == 7
     for name, n, at, rc, count in lines:
         assert (rc, count) == (("0", n) if at == "0" else ("719", at)), (name, at, rc, count)
+
+
+def test_linear_attention_plans_for_as_many_workgroups_as_run_at_once(lib):
+    """Chunks of few long sequences fill the CUs once, whatever the shape of a head: the fastest of the counts that were measured."""
+    def chunks(B, H, T, dk, dv):
+        n = lib.kh_linear_attention_workspace_bytes(B, H, T, B * T, dk, dv)
+        one = H * dk * dv * 8 + 16                         # two states of every head and the chunk's place
+        assert n % one == 0
+        return n // one
+
+    assert chunks(1, 16, 16384, 64, 128) == 16 and chunks(2, 20, 4096, 64, 128) == 12
+    assert chunks(1, 16, 16384, 128, 64) == 16 and chunks(2, 20, 4096, 128, 64) == 12
+    assert chunks(1, 16, 16384, 128, 128) == 16 and chunks(1, 16, 16384, 64, 64) == 32         # (two workgroups to a CU)
+    assert chunks(16, 16, 1024, 128, 128) == chunks(4, 40, 512, 64, 64) == 0                    # whole sequences
