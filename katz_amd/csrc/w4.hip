@@ -194,15 +194,19 @@ __global__ __launch_bounds__(256) void values_kernel(const ValueParams p) {
     const int last = (p.K - 1) >> (3 + p.gshift), g = u[i] >> p.gshift;      // (words behind the last weight may lie behind the last group)
     word[i] = p.q[r * p.pieces.per_row + u[i]];
     s[i] = p.scale[r * p.gstride + (g < last ? g : last)];
-    z[i] = p.zero ? p.zero[r * p.gstride + (g < last ? g : last)] & 15 : 8;      // (as the linear takes it)
+    z[i] = p.zero ? p.zero[r * p.gstride + (g < last ? g : last)] : 8;
   }
 #pragma unroll
   for (int i = 0; i < PT; ++i) {
     if (row[i] >= p.N) break;
     const int left = p.K - u[i] * 8;
+#if __HIP_DEVICE_COMPILE__
+    asm volatile("" : "+v"(z[i]));   // (masked here: at its load the compiler would wait for it, and 16384 x 8191 take 78 us instead of 71)
+#endif
+    const int zero = z[i] & 15;      // (as the linear takes it)
     T v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = (T)((float)s[i] * (float)((int)((word[i] >> (4 * e)) & 15u) - z[i]));
+    for (int e = 0; e < 8; ++e) v[e] = (T)((float)s[i] * (float)((int)((word[i] >> (4 * e)) & 15u) - zero));
     store8_once<T>((T*)p.out + row[i] * p.K + u[i] * 8, left, v);
   }
 }
@@ -295,7 +299,7 @@ struct LinParams {
   const float* col_scale;
   int t_at;
   int b_dma;               // B_cat is aligned to four bytes
-  int once;                // y of 8 MB and more is stored past the caches (616 x 10240 with a residual: 40.6 -> 37.4 us)
+  int once;                // y of 8 MB and more is stored past the caches (616 x 10240 with rank 96 and a residual: 40.6 -> 37.4 us)
 };
 
 // The rank-R product of a 16 x 16 tile in 32 bits, a step of 16 ranks: t from LDS, or [M][R] in `splits` parts, B_cat rows of T.
@@ -658,8 +662,8 @@ __global__ __launch_bounds__(LW * 64) void w4_few_rows(const LinParams p) {
 // LDS, where every wave's accumulators start from it.
 // A block is 1920 clocks of the matrix unit (two waves of 60 products of 16 x 16 x 32 on a SIMD), about 2100 of the vector unit (codes to operands, the scaled sum of
 // every group) and 1650 of LDS: sums of a group and of the row in 32 bits each are 120 registers of the 256 that two waves leave each other.
-// 616 rows, 10240 x 1280 with rank 96 and a residual, by the clock of a workgroup: 3 us to the first block, 4 for the ranks, 24 for ten blocks, 8 for the outputs, whose 25 MB
-// all CUs move at once.
+// 616 rows, 10240 x 1280 with rank 96, by the clock of a workgroup: 2.3 us to the first block, 4.2 for the ranks, 23.6 for ten blocks (of which those instructions, one after the other, are
+// 17), 2.9 for the outputs; with a residual 7 .. 8 for those, whose 25 MB all CUs move at once.
 constexpr int MR_M = 5, MR_N = 3, MR_W = 8, MR_ST = 3;     // tiles of 16 rows; of 16 columns of a wave; waves; stages
 
 template <int G, bool ZERO>
