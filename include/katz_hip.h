@@ -487,8 +487,9 @@ int kh_block_norm(const void* y, const void* h, const void* gate, int64_t gate_r
  * rint(w / scale) + zero within 0..15 (halves to even).  A group that holds a NaN gets a NaN as its scale, one that holds an infinity an infinity.
  * kh_dequantize_w4: the values in `type`, rounded once, [N, K].
  * kh_w4_linear: y[M,N] = x w^T + bias + ((x A_cat^T) * col_scale) B_cat^T (+ residual), the adapter operands as for kh_lora_linear_bf16 (R % 32 == 0,
- * R <= 128, any K and N), type 0 or 1.  Products with the codes are exact and summed in 32 bits; the rank-R product stays in 32 bits.  A row of x
- * that holds an infinity gives NaN.  workspace: kh_w4_linear_workspace_bytes (0, for instance without an adapter: it may be NULL), aligned to 16 bytes.
+ * R <= 128, any K and N), type 0 or 1.  Products with the codes are exact and summed in 32 bits; the rank-R product stays in 32 bits.  Codes are
+ * multiplied as numbers of up to 63, of which the excess is taken off in the sum: a row of x that holds an infinity, or bf16 numbers (from 4e34 on) whose sums with those
+ * pass the largest in 32 bits, gives NaN.  workspace: kh_w4_linear_workspace_bytes (0, for instance without an adapter: it may be NULL), aligned to 16 bytes.
  * kh_w4_linear_wide: the same with R up to 65536, what the columns of many adapters add up to, and a workspace of its own size. */
 int kh_quantize_w4(const void* w, void* q, void* scale, void* zero, int64_t N, int64_t K, int64_t group, int type, void* stream);
 int kh_dequantize_w4(const void* q, const void* scale, const void* zero, void* out, int64_t N, int64_t K, int64_t group, int type, void* stream);
@@ -508,7 +509,9 @@ int kh_w4_linear_wide(const void* x, const void* q, const void* scale, const voi
  * state_in / state_out: float [n_slots, H, dk, dv]; sequence b starts from and leaves slot b, or slots[b] (int32 [B], device; distinct): a slot
  * outside 0 .. n_slots - 1 leaves the whole sequence out.  state_in NULL: zeros (not for the step); the two may be the same.
  * workspace: kh_linear_attention_workspace_bytes with rows = B * T where they are dense (0: may be NULL).  kh_linear_attention_step_bf16: one token a sequence, rows [B];
- * flags bit 0: rows of o whose sequences are left out are zeroed (else left as they were). */
+ * flags bit 0: rows of o whose sequences are left out are zeroed (else left as they were).
+ * Scores and states are multiplied in pieces: in a prompt an infinity in q, k, v or a state makes the sums that it goes into NaN, also where the formula gives an infinity; tokens before
+ * it stay as they are. */
 int64_t kh_linear_attention_workspace_bytes(int64_t B, int64_t H, int64_t T, int64_t rows, int64_t dk, int64_t dv);
 int kh_linear_attention_bf16(const void* q, const void* k, const void* v, void* o, const float* log_decay, const float* state_in,
                              float* state_out, const int32_t* slots, int64_t n_slots, const int32_t* seg_start, int64_t rows, void* workspace,

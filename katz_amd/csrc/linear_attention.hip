@@ -12,9 +12,10 @@
 // those of the 32-bit numbers that they are held in.  Two pieces of scores, states and of the values in chunks where no sequence ends left 2^-18 of a term and cost less (us, two | three:
 // 16384 packed tokens of 16 heads of 128 on 8 122 | 135, 2 x 4096 of 20 heads of 64 46.6 | 50.1, 16 x 1024 of 16 heads of 128 83.5 | 89.4, 2 x 77 of 20 heads of 64 the same): terms that cancel
 // one another lost what was left of them.
-// What bounds it: 16384 packed tokens of 16 heads of 128 on 8 are 36 us of la_gain, 8 of la_scan and 82 of la_out (the bytes of q, k, v and o take 42), 16 blocks a workgroup
-// one after the other at 2.2 and 4.4 us.  Of those 4.4 matrix and vector instructions, which a SIMD issues one after the other, are 3; the rest is reads from LDS and two
-// barriers, which two waves on a SIMD do not cover.  A workgroup takes 116 KB of LDS, so there is one to a CU.
+// What bounds it: of 16384 packed tokens of 16 heads of 128 on 8 the workgroups take 31 us in la_gain, 7 in la_scan and 84 .. 97 in la_out, 3 .. 4 lie between launches (the bytes of q, k, v
+// and o take 42): 17 blocks a workgroup one after the other at 1.8 and 5.1 us.  Of those 5.1 products are 1.7 (126 of 16 clocks a wave, two waves on a SIMD).  The next block's loads
+// are covered by the scores alone: the compiler waits for everything that is on its way in front of the state's first use in the loop, since a state comes from loads before it.
+// A workgroup takes 123 KB of LDS, so there is one to a CU.
 #include "kh_common.h"
 #include <type_traits>
 

@@ -381,7 +381,8 @@ class LoRALinear(nn.Module):
 class LoRALinearW4(nn.Module):
     """LoRALinear with its base weights in 4 bits (ops.W4Weight) and the adapters beside them in the activations' type: the same named adapters, active
     list, per-adapter weights and global scale (no counterpart in the reference, whose text encoders run once a prompt).  For layers that a few rows at a
-    time pass through, whose bytes are the time; any number of rows is right.
+    time pass through, whose bytes are the time; any number of rows is right.  It stands by itself: the UNet's modules call, load and list LoRALinears
+    only.  Converting a model that holds one to a type that is neither bf16 nor fp16 raises where it is met, after the modules before it.
 
     The buffers weight_q / weight_scale / weight_zero are what is saved; fuse() merges adapters into them in place, so a captured graph that reads them
     stays valid.  What is merged is part of the weights from then on: its name is free for another adapter, and weights that are loaded take no adapter as merged."""

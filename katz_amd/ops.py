@@ -1473,7 +1473,7 @@ def w4_linear(x: torch.Tensor, w: W4Weight, bias: Optional[torch.Tensor] = None,
               out: Optional[torch.Tensor] = None, wide: bool = False) -> torch.Tensor:
     """y = x w^T + b + ((x A_cat^T) * col_scale) B_cat^T (+ residual) with weights in 4 bits, bf16 or fp16 by x.dtype; the adapter operands as
     for lora_linear (a_cat [R,K], b_cat [N,R], col_scale [R] fp32, R % 32 == 0, R <= 128; wide: <= 65536).  Made for few rows, right for any number.  A row of x that
-    holds an infinity gives NaN."""
+    holds an infinity, or bf16 numbers of 4e34 and more whose sums with numbers of 63 pass the largest in 32 bits, gives NaN."""
     lib = _lib.load()
     dt, xs, q = x.dtype, x.shape, w.q
     if dt is not torch.bfloat16 and dt is not torch.float16:
@@ -1592,7 +1592,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: i
     seg_start[b+1], other rows of a given out stay as they were (those of a new one are zero).  log_decay float32 [heads], <= 0.
     state: float32 [B,heads,dk,dv] to start from (None: zeros), overwritten unless state_out is given; with slots (int32 [B], distinct) it is a pool
     and sequence b has slot slots[b]; a slot outside the pool leaves its sequence out.  Tokens do not depend on later ones, also where those are no
-    numbers; an infinity in v gives NaN from its token on."""
+    numbers; an infinity in q, k, v or a state gives NaN in the sums that it goes into (its token's, and
+    but for q's those of the tokens from there on), also where the formula gives an infinity."""
     lib = _lib.load()
     packed = seg_start is not None
     kv, dk, dv = _la_sizes(q, k, v, heads, kv_heads, log_decay, 2 if packed else 3)
