@@ -342,3 +342,38 @@ def test_layer_with_more_rank_columns_than_one_pack(M, dtype, N, K, ranks):
     layer.set_global_scale(1.0)
     assert all(a is b for a, b in zip(layer._operands, operands)) or layer._operands[2].data_ptr() == operands[2].data_ptr()   # a captured graph stays valid
     assert not torch.equal(layer(x.to(DEV)), before)
+
+
+@pytest.mark.parametrize("M,dtype", [(3, BF), (700, torch.float16)])
+def test_a_captured_layer_of_many_rank_columns_follows_its_scales(M, dtype):
+    """Packs that lie side by side are written to in place: replays take the scales that are set between them, beside eager calls on another stream."""
+    from katz_amd import ops
+    from katz_amd.layers import LoRALinearW4
+
+    g = torch.Generator().manual_seed(M)
+    layer = LoRALinearW4(200, 4100, device=DEV, dtype=dtype)
+    layer._assign(ops.quantize_w4((torch.randn(4100, 200, generator=g) * 0.1).to(DEV), 64))
+    for n, r in (("a", 100), ("b", 60), ("c", 9)):
+        layer.add_adapter(n, (torch.randn(r, 200, generator=g) * 0.1).to(dtype), (torch.randn(4100, r, generator=g) * 0.1).to(dtype))
+    layer.set_active(["a", "b", "c"], [1.0, 0.5, 2.0])
+    x, other = (torch.randn(M, 200, generator=g).to(DEV, dtype) for _ in range(2))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        layer(x)
+    torch.cuda.current_stream().wait_stream(side)
+    graph, held = torch.cuda.CUDAGraph(), torch.zeros_like(x)
+    with torch.cuda.graph(graph):
+        y = layer(held)
+    seen = []
+    for weights in ([1.0, 0.5, 2.0], [0.0, 0.0, 1.0], [2.0, 1.0, 0.0], [1.0, 0.5, 2.0]):
+        layer.set_active(["a", "b", "c"], weights)
+        held.copy_(x)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            beside = layer(other)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, layer(x)) and torch.equal(beside, layer(other))
+        seen.append(y.clone())
+    assert torch.equal(seen[0], seen[3]) and not torch.equal(seen[0], seen[1]) and not torch.equal(seen[1], seen[2])
