@@ -44,7 +44,8 @@ const char* kh_error_string(int code);
  * start/stop event pair on the launch stream.  kh_profile_end waits for them and writes, in launch
  * order, a kernel tag (1 lora_gemm, 2 lora_gemm_f32, 3 attention, 4 group_norm stats, 5 group_norm apply,
  * 6 layer_norm, 7 geglu, 8 residual_add, 9 concat_residual, 10 sgmv_shrink, 11 sgmv_expand, 12 lora_shrink, 13 conv3x3, 14 cfg_euler, 15 upsample, 16 lora_merge, 17 conv_out + guidance + Euler,
- * 18 fused segmented shrink + expand, 19 lora_pack, 20 block_norm, 21 quantize_w4, 22 dequantize_w4, 23 w4_linear, 24 its shrink, 25 linear attention) and the
+ * 18 fused segmented shrink + expand, 19 lora_pack, 20 block_norm, 21 quantize_w4, 22 dequantize_w4, 23 w4_linear, 24 its shrink, 25 linear attention,
+ * 26 rotary, 27 paged attention, 28 its join, 29 pages of a cache) and the
  * duration in ms into HOST arrays; returns the number of launches (or -hipError_t).  Do not use under
  * graph capture. */
 int kh_profile_begin(void);
@@ -520,6 +521,58 @@ int kh_linear_attention_bf16(const void* q, const void* k, const void* v, void* 
 int kh_linear_attention_step_bf16(const void* q, const void* k, const void* v, void* o, const float* log_decay, const float* state_in,
                                   float* state_out, const int32_t* slots, int64_t n_slots, int64_t B, int64_t H, int64_t kv_heads, int64_t dk,
                                   int64_t dv, int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo, float scale, int flags, void* stream);
+
+/* ---- Attention over a paged cache ----------------------------------------------------------------
+ * No counterpart in the reference; they stand beside K3 and the states of linear attention.
+ *
+ * KhPagedCache (HOST memory, device pointers inside): keys and values of sequences in pages of `page` tokens, for all layers of a model.
+ *   k, v       [layers, pages, page, kv_heads, d] through strides in elements, the last axis contiguous: bf16, fp16 or (type 3) e4m3, d % 8 == 0, d <= 256;
+ *              pointers and strides aligned to 16 bytes (e4m3: 8)
+ *   table      int32 [slots, width]: page i of slot s's sequence (tokens i * page ..); a number outside 0 .. pages - 1 is no page: its tokens are left out
+ *   lengths    int32 [slots], tokens of each sequence (at most width * page count)
+ *   refs       int32 [pages], how many sequences hold each page; 0: free.  kh_cache_extend, _reorder and _compact keep table, lengths and refs;
+ *              the others only read table and lengths, and take refs == NULL
+ *   k_scale, v_scale  float [layers, kv_heads], type 3 only, may be NULL (1): a code c stands for c * scale */
+typedef struct {
+  void *k, *v;
+  int32_t *table, *lengths, *refs;
+  const float *k_scale, *v_scale;
+  int64_t layers, pages, page, kv_heads, d, slots, width, type;
+  int64_t k_layer, k_page, k_token, k_head, v_layer, v_page, v_token, v_head;
+} KhPagedCache;
+/* Rotary positions with several axes: pair j of the `pairs` pairs of every head turns by the angle position[row][axis of j] * frequencies[j] (in 64
+ * bits), (a, b) -> (a cos - b sin, b cos + a sin), in 32 bits, rounded once.  Pairs are dimensions (j, j + pairs), with flags bit 0 (2 j, 2 j + 1);
+ * further dimensions of a head are copied.  q [rows, heads * d] to q_out, k [rows, kv_heads * d] to k_out, through row strides; in place where they
+ * are the same.  positions [rows, axes]: position_type 0 int32, 1 int64, 2 float32; axis a has pairs section_end[a - 1] .. section_end[a] - 1 (HOST
+ * memory, axes <= 4, the last is `pairs`; pairs may be 0).  frequencies: double, or with flags bit 2 float, [pairs].  d <= 1024.  type: 0 bf16, 1 fp16, 2 fp32.
+ * With a cache (type 0 or 1, the cache's unless that is e4m3; k_out unused): the turned k and v [rows, kv_heads * d] are written as token places[r] of slot slots[r] in
+ * `layer`; slots NULL: row r is slot r; places NULL: the last token of the slot's sequence; positions NULL: the place on every axis.  Rows whose slot
+ * lies outside the cache, or whose place outside its sequence, are left out: q_out stays as it was there, with flags bit 1 it is zeroed.  k and v of a place without a page are
+ * dropped.  e4m3: the nearest to value / scale, clamped at 448 (halves to even).  (slot, place) of the rows are distinct. */
+int kh_rotary(const void* q, const void* k, const void* v, void* q_out, void* k_out, const void* positions, int position_type,
+              const void* frequencies, const int64_t* section_end, int64_t axes, const KhPagedCache* cache, int64_t layer, const int32_t* slots,
+              const int32_t* places, int64_t rows, int64_t heads, int64_t kv_heads, int64_t d, int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldqo,
+              int64_t ldko, int flags, int type, void* stream);
+/* Attention of one token a row over the cache: o[r][h] = sum_t p_t v_t / sum_t p_t, p_t = exp(scale * q[r][h] . k_t - max), over the tokens t < n of slot slots[r]
+ * (NULL: row r is slot r), n = lengths[r] (NULL: the cache's for the slot; at most width * page), with a window > 0 only the last `window` of them.  Query
+ * head h takes key head h / (heads / kv_heads).  Nothing to attend to: zeros.  Rows whose slot lies outside the cache are left out: o stays as it
+ * was, with flags bit 0 it is zeroed.  q, o [rows, heads * d] through row strides, type 0 or 1, the cache's unless that is e4m3.  An infinity among the attended values gives NaN.
+ * workspace: kh_paged_attention_workspace_bytes(rows, heads, kv_heads, d, width * page) (0: may be NULL), aligned to 16 bytes. */
+int64_t kh_paged_attention_workspace_bytes(int64_t rows, int64_t heads, int64_t kv_heads, int64_t d, int64_t span);
+int kh_paged_attention(const void* q, void* o, const KhPagedCache* cache, int64_t layer, const int32_t* slots, const int32_t* lengths, void* workspace,
+                       int64_t rows, int64_t heads, int64_t ldq, int64_t ldo, int64_t window, float scale, int flags, int type, void* stream);
+/* The pages of a cache.  Whoever wants pages gets the lowest free ones, by slot and then by place; where there are none left the entry is -1, and *missing
+ * (device) is how many were wanted and not there (table rows that are too short counted in).
+ * kh_cache_extend: sequence s gets counts[s] (<= 0: no) more tokens, at most width * page in all.
+ * kh_cache_reorder: slot s keeps its sequence where parents[s] == s, takes over the one that slot parents[s] had before the call, or, where that is no
+ * slot, is emptied.  Whole pages are shared; the page not yet full is copied (its tokens, in all layers), but handed on as it is to the lowest taker
+ * of a sequence whose own slot gives it up.  Entries behind a changed sequence's pages become -1.
+ * kh_cache_compact: the pages in use, *in_use (device) of them, become pages 0 .. *in_use - 1: those behind go to the free ones before, both in order.
+ * workspace: kh_cache_workspace_bytes, aligned to 16 bytes.  Pages at addresses that the strides make overlap are not supported. */
+int64_t kh_cache_workspace_bytes(int64_t slots, int64_t width, int64_t pages);
+int kh_cache_extend(const KhPagedCache* cache, const int32_t* counts, int32_t* missing, void* workspace, void* stream);
+int kh_cache_reorder(const KhPagedCache* cache, const int32_t* parents, int32_t* missing, void* workspace, void* stream);
+int kh_cache_compact(const KhPagedCache* cache, int32_t* in_use, void* workspace, void* stream);
 
 #ifdef __cplusplus
 }

@@ -76,6 +76,13 @@ SIGNATURES = {
     "kh_linear_attention_workspace_bytes": (_I, [_I] * 6),
     "kh_linear_attention_bf16": (c_int, [_P] * 8 + [_I, _P, _I, _P] + [_I] * 14 + [c_float, _P]),
     "kh_linear_attention_step_bf16": (c_int, [_P] * 8 + [_I] * 10 + [c_float, c_int, _P]),
+    "kh_rotary": (c_int, [_P] * 6 + [c_int, _P, _P, _I, _P, _I, _P, _P] + [_I] * 9 + [c_int, c_int, _P]),
+    "kh_paged_attention_workspace_bytes": (_I, [_I] * 5),
+    "kh_paged_attention": (c_int, [_P, _P, _P, _I, _P, _P, _P] + [_I] * 5 + [c_float, c_int, c_int, _P]),
+    "kh_cache_workspace_bytes": (_I, [_I] * 3),
+    "kh_cache_extend": (c_int, [_P] * 5),
+    "kh_cache_reorder": (c_int, [_P] * 5),
+    "kh_cache_compact": (c_int, [_P] * 4),
 }
 
 _lib = None

@@ -44,7 +44,8 @@ enum KhKernelTag {
   KH_TAG_LAYER_NORM = 6, KH_TAG_GEGLU = 7, KH_TAG_RESIDUAL_ADD = 8, KH_TAG_CONCAT_RESIDUAL = 9,
   KH_TAG_SGMV_SHRINK = 10, KH_TAG_SGMV_EXPAND = 11, KH_TAG_LORA_SHRINK = 12, KH_TAG_CONV = 13, KH_TAG_CFG_EULER = 14,
   KH_TAG_UPSAMPLE = 15, KH_TAG_LORA_MERGE = 16, KH_TAG_CONV_OUT_STEP = 17, KH_TAG_SGMV_FUSED = 18, KH_TAG_LORA_PACK = 19,
-  KH_TAG_BLOCK_NORM = 20, KH_TAG_W4_QUANTIZE = 21, KH_TAG_W4_VALUES = 22, KH_TAG_W4_LINEAR = 23, KH_TAG_W4_SHRINK = 24, KH_TAG_LINEAR_ATTENTION = 25
+  KH_TAG_BLOCK_NORM = 20, KH_TAG_W4_QUANTIZE = 21, KH_TAG_W4_VALUES = 22, KH_TAG_W4_LINEAR = 23, KH_TAG_W4_SHRINK = 24, KH_TAG_LINEAR_ATTENTION = 25,
+  KH_TAG_ROTARY = 26, KH_TAG_PAGED_ATTENTION = 27, KH_TAG_PAGED_JOIN = 28, KH_TAG_CACHE_PAGES = 29
 };
 bool kh_prof_enabled();
 void kh_prof_events(int tag, hipEvent_t* start, hipEvent_t* stop);

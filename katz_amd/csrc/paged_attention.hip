@@ -1,0 +1,549 @@
+// K15: attention of one token a row over a paged cache:
+//   x_t = scale * q . k_t,   m = max x_t,   o = sum_t exp(x_t - m) v_t / sum_t exp(x_t - m)
+//
+// Bound by the bytes of the keys and values, which are read once for all query heads that share them.  The work is cut over the cache's length: the
+// tiles of 128 tokens of all rows and key heads stand in one line, and every workgroup takes an equal part of it, wherever sequences end (the lengths lie on
+// the device; a plan on the host would have to go by the longest).  A row and key head that one workgroup has whole is written by it; of others the
+// parts are left in 32 bits (maximum, sum, unscaled output) and a second launch joins them in order.
+//
+// A tile is four waves of 32 tokens, each on its own until the workgroup's part ends:
+//   S^T = K . Q^T     A = the keys as they lie in memory (lane l: token l % 16, 8 dimensions from 8 * (l / 16) on), B = up to 16 query heads in registers
+//   O^T += V^T . P^T  A = values of 8 tokens for a dimension, put together from the loads of 8 whole rows by byte permutes in the lane, B = P
+// The tokens of the keys' rows are chosen so that the scores a lane gets (query l % 16, eight tokens) are the P operand it needs: nothing crosses lanes but the
+// maximum.  Neither operand goes through LDS.  P is multiplied in all 24 bits: in three pieces of bf16 or two of fp16, since the matrix unit waits for memory anyway.
+#include "paged_cache.h"
+#include <type_traits>
+
+namespace {
+
+constexpr int NW = 4, STEP = 32, TILE = NW * STEP;       // waves, tokens of a wave's step, of a tile
+constexpr int QB = 16;                                  // query heads of a unit
+constexpr float RESCALE_LOG2 = 8.0f;                    // the running maximum moves only for jumps above 2^8
+
+struct PagedParams {
+  const void *q, *k, *v;
+  void* o;
+  const int32_t *table, *row_lengths, *lengths, *slots;
+  const float *k_scale, *v_scale;
+  float* part;                // [2 workgroups][group][d] outputs, then [2 workgroups][group][2] maxima and sums
+  int4* border;               // [workgroups]: row, unit, workgroups of the unit that a workgroup begins inside
+  long ldq, ldo;
+  long k_page, k_token, k_head, v_page, v_token, v_head;   // elements
+  int rows, kv_heads, group, blocks, d;                 // blocks: units of a key head
+  int n_slots, width, pages, page, window;
+  float scale_log2;
+  int fill, q_aligned;
+  KhDivide by_page;
+};
+
+typedef _Float16 f16_t;
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+template <typename T> struct Eight;
+template <> struct Eight<bf16_t> { using type = bf16x8; };
+template <> struct Eight<f16_t> { using type = f16x8; };
+
+__device__ __forceinline__ f32x4 mfma(const bf16x8& a, const bf16x8& b, const f32x4& c) {
+#if __HIP_DEVICE_COMPILE__
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+#else
+  return c;
+#endif
+}
+__device__ __forceinline__ f32x4 mfma(const f16x8& a, const f16x8& b, const f32x4& c) {
+#if __HIP_DEVICE_COMPILE__
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+#else
+  return c;
+#endif
+}
+
+__device__ __forceinline__ float swapped_max(float v) {  // over the four lanes of a query
+#if __HIP_DEVICE_COMPILE__
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+#else
+  return v;
+#endif
+}
+
+// The codes of a word's lower or upper two bytes as two numbers of T (exact).
+template <typename T, bool UP>
+__device__ __forceinline__ uint32_t two_of_e4m3(uint32_t w) {
+#if __HIP_DEVICE_COMPILE__
+  if constexpr (sizeof(T) == 2 && __is_same(T, bf16_t)) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, UP));
+  else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, UP));
+#else
+  return w;
+#endif
+}
+
+// P in pieces whose sum it is: three of bf16 (each the upper bits of what is left: exact), or two of fp16 (P <= 2^8, and below one what is
+// left out is under 2^-25 of the largest)
+template <typename T> struct Pieces;
+template <> struct Pieces<bf16_t> {
+  static constexpr int N = 3;
+  static __device__ __forceinline__ void of(const float (&p)[8], bf16x8 (&out)[3]) {
+    uint32_t w[3][4];
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      float a = p[i], b = p[i + 1];
+#pragma unroll
+      for (int n = 0; n < 3; ++n) {
+        w[n][i / 2] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);
+        a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u);
+        b -= __uint_as_float(__float_as_uint(b) & 0xffff0000u);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < 3; ++n) out[n] = __builtin_bit_cast(bf16x8, u32x4{w[n][0], w[n][1], w[n][2], w[n][3]});
+  }
+};
+template <> struct Pieces<f16_t> {
+  static constexpr int N = 2;
+  static __device__ __forceinline__ void of(const float (&p)[8], f16x8 (&out)[2]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      out[0][i] = (f16_t)p[i];
+      out[1][i] = (f16_t)(p[i] - (float)out[0][i]);
+    }
+  }
+};
+
+// A row's sequence: its pages and the tokens low .. n - 1 to attend to; tiles of 128 from `tile` on.
+struct Row { const int32_t* pages; int n, low, tile, tiles; bool there; };
+
+__device__ __forceinline__ Row row_of(const PagedParams& p, int r) {
+  Row w{p.table, 0, 0, 0, 0, false};
+  const int s = p.slots ? p.slots[r] : r;
+  if (s < 0 || s >= p.n_slots) return w;
+  w.there = true;
+  w.pages = p.table + (long)s * p.width;
+  const int n = p.row_lengths ? p.row_lengths[r] : p.lengths[s], most = p.width * p.page;
+  w.n = n < 0 ? 0 : n < most ? n : most;
+  w.low = p.window > 0 && w.n > p.window ? w.n - p.window : 0;
+  w.tile = w.low / TILE;
+  w.tiles = (w.n + TILE - 1) / TILE - w.tile;
+  return w;
+}
+
+// Shapes.  D: dimensions there is room for (d of them used: TAIL where fewer); CODES: the cache holds e4m3; EIGHT: pages of a multiple of eight tokens.
+template <int D, typename T, bool CODES, bool EIGHT, bool TAIL>
+struct Shape {
+  using X = typename Eight<T>::type;
+  using Raw = typename std::conditional<CODES, u32x2, u32x4>::type;      // eight elements of a row
+  static constexpr int KK = D / 32;                     // k-steps of the scores
+  static constexpr int NC = D >= 128 ? D / 128 : 1;     // pieces of a row of values in a lane
+  static constexpr int VE = D >= 128 ? 8 : 4;           // elements of one
+  static constexpr int ELT = CODES ? 1 : 2;
+};
+
+template <int D, typename T, bool CODES, bool EIGHT, bool TAIL>
+struct Wave {
+  using S = Shape<D, T, CODES, EIGHT, TAIL>;
+  using X = typename S::X;
+  X q[S::KK];
+  f32x4 o[S::NC * S::VE];                               // tile c * VE + j: dimensions c * 128 + VE * (4 * (l / 16) + r) + j of query l % 16
+  float m, l;
+
+  __device__ __forceinline__ void begin() {
+#pragma unroll
+    for (int i = 0; i < S::NC * S::VE; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m = -INFINITY;
+    l = 0.f;
+  }
+
+  // 32 tokens from t0 (a multiple of 32) on, of which low .. n - 1 count.
+  __device__ __forceinline__ void step(const PagedParams& p, const Row& row, int head, int t0, float factor) {
+    const int lane = threadIdx.x & 63, c16 = lane & 15, g4 = lane >> 4;
+    const char* kb = reinterpret_cast<const char*>(p.k) + head * p.k_head * S::ELT;
+    const char* vb = reinterpret_cast<const char*>(p.v) + head * p.v_head * S::ELT;
+    const int last = row.n - 1;
+    // where a token lies; a token behind the end is looked for at the last one, one without a page at the first of all
+    auto place = [&](int t, long page, long token, bool& good) -> long {
+      t = t < last ? t : last;
+      const int at = (int)p.by_page((uint32_t)t);
+      const int e = row.pages[at];
+      good = e >= 0 && e < p.pages;
+      return good ? (long)e * page + (long)(t - at * p.page) * token : 0;
+    };
+    bool good[8];
+    typename S::Raw kr[2][S::KK];
+    uint32_t vr[8][S::NC][S::VE * S::ELT / 4];
+    const int tv = t0 + 8 * g4;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      bool any;
+      const char* at = kb + place(t0 + 8 * (c16 >> 2) + 4 * s + (c16 & 3), p.k_page, p.k_token, any) * S::ELT;
+#pragma unroll
+      for (int kk = 0; kk < S::KK; ++kk) {
+        const int dim = kk * 32 + g4 * 8;
+        if (TAIL && kk * 32 >= p.d) kr[s][kk] = typename S::Raw{};
+        else {
+          kr[s][kk] = *reinterpret_cast<const typename S::Raw*>(at + (!TAIL || dim < p.d ? dim : 0) * S::ELT);
+          if (TAIL && dim >= p.d) kr[s][kk] = typename S::Raw{};
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const char* at = vb + place(tv + i, p.v_page, p.v_token, good[i]) * S::ELT;
+      good[i] = good[i] && tv + i >= row.low && tv + i < row.n;
+#pragma unroll
+      for (int c = 0; c < S::NC; ++c) {
+        const int dim = c * 128 + c16 * S::VE;
+        __builtin_memcpy(vr[i][c], __builtin_assume_aligned(at + (!TAIL || dim < p.d ? dim : 0) * S::ELT, S::VE * S::ELT), S::VE * S::ELT);
+      }
+    }
+    // what does not count may be anything
+    bool whole = true;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) whole = whole && good[i];
+    const bool cut = __any(!whole);
+    if (cut) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int c = 0; c < S::NC; ++c)
+#pragma unroll
+          for (int w = 0; w < S::VE * S::ELT / 4; ++w) vr[i][c][w] = good[i] ? vr[i][c][w] : 0;
+    }
+    // scores: x[4 s + r] is token tv + 4 s + r of query l % 16
+    float x[8];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      f32x4 acc{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kk = 0; kk < S::KK; ++kk) {
+        X a;
+        if constexpr (CODES) {
+          const u32x2 w = kr[s][kk];
+          a = __builtin_bit_cast(X, u32x4{two_of_e4m3<T, false>(w[0]), two_of_e4m3<T, true>(w[0]), two_of_e4m3<T, false>(w[1]), two_of_e4m3<T, true>(w[1])});
+        } else {
+          a = __builtin_bit_cast(X, kr[s][kk]);
+        }
+        acc = mfma(a, q[kk], acc);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[4 * s + r] = acc[r] * factor;
+    }
+    if (cut) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = good[i] ? x[i] : -INFINITY;
+    }
+    float top = x[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);
+    top = swapped_max(top);
+    if (__any(top > m + RESCALE_LOG2)) {
+      const float now = fmaxf(m, top), by = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - now);
+      m = now;
+      l *= by;
+#pragma unroll
+      for (int i = 0; i < S::NC * S::VE; ++i) o[i] *= by;
+    }
+    const float from = m == -INFINITY ? 0.f : m;
+    float pr[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      pr[i] = __builtin_amdgcn_exp2f(x[i] - from);
+      l += pr[i];
+    }
+    X pieces[Pieces<T>::N];
+    Pieces<T>::of(pr, pieces);
+#pragma unroll
+    for (int c = 0; c < S::NC; ++c)
+#pragma unroll
+      for (int j = 0; j < S::VE; ++j) {
+        u32x4 a;
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {                   // tokens 2 h, 2 h + 1
+          if constexpr (CODES) {
+            const uint32_t both = __builtin_amdgcn_perm(vr[2 * h + 1][c][j / 4], vr[2 * h][c][j / 4], 0x0400u + (j % 4) * 0x0101u);
+            a[h] = two_of_e4m3<T, false>(both);
+          } else {
+            a[h] = __builtin_amdgcn_perm(vr[2 * h + 1][c][j / 2], vr[2 * h][c][j / 2], j & 1 ? 0x07060302 : 0x05040100);
+          }
+        }
+        const X value = __builtin_bit_cast(X, a);
+#pragma unroll
+        for (int n = 0; n < Pieces<T>::N; ++n) o[c * S::VE + j] = mfma(value, pieces[n], o[c * S::VE + j]);
+      }
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void zero_row(const PagedParams& p, int r) {
+  T* to = reinterpret_cast<T*>(p.o) + (long)r * p.ldo;
+  for (int i = threadIdx.x; i < p.kv_heads * p.group * p.d; i += NW * 64) to[i] = (T)0.f;
+}
+
+template <int D, typename T, bool CODES, bool EIGHT, bool TAIL>
+__global__ __launch_bounds__(NW * 64) void attend(const PagedParams p) {
+  using S = Shape<D, T, CODES, EIGHT, TAIL>;
+  constexpr int OW = D + 4;                             // floats of a query's row in LDS
+  extern __shared__ float lds[];                        // [NW][QB][OW] outputs, [2][NW][QB] maxima and sums
+  float* const ms = lds + NW * QB * OW;
+  __shared__ long starts[NW];
+  __shared__ int where[2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c16 = lane & 15, g4 = lane >> 4;
+  const int units = p.kv_heads * p.blocks, G = gridDim.x, w = blockIdx.x;
+
+  // rows of this workgroup that have nothing to attend to, or no slot
+  for (int r = w; r < p.rows; r += G) {
+    const Row row = row_of(p, r);
+    if (row.tiles <= 0 && (row.there || p.fill)) zero_row<T>(p, r);
+  }
+
+  // the line of tiles: all of them, and the row in which this workgroup's part begins
+  const int each = (p.rows + NW * 64 - 1) / (NW * 64), r0 = tid * each, r1 = r0 + each < p.rows ? r0 + each : p.rows;
+  long mine = 0;
+  for (int r = r0; r < r1; ++r) mine += row_of(p, r).tiles;
+  long before = mine;
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    const long y = __shfl_up(before, s, 64);
+    if (lane >= s) before += y;
+  }
+  if (lane == 63) starts[wave] = before;
+  __syncthreads();
+  long total = 0;
+  before -= mine;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) {
+    if (i < wave) before += starts[i];
+    total += starts[i];
+  }
+  total *= units;
+  before *= units;
+  const long W = total < G ? total : G;                 // workgroups that have a tile
+  if (tid == 0) p.border[w] = int4{-1, 0, 0, 0};
+  if (w >= W) return;
+  const long begin = total * w / W, end = total * (w + 1) / W;
+  long at_row = before;                                 // where row r begins
+  for (int r = r0; r < r1; ++r) {
+    const long next = at_row + (long)row_of(p, r).tiles * units;
+    if (begin >= at_row && begin < next) {
+      where[0] = r;
+      where[1] = (int)(begin - at_row);
+    }
+    at_row = next;
+  }
+  __syncthreads();
+  int r = where[0];
+  long at = begin, row_at = begin - where[1];
+
+  Wave<D, T, CODES, EIGHT, TAIL> wv;
+  for (; at < end; ++r) {
+    const Row row = row_of(p, r);
+    const long row_end = row_at + (long)row.tiles * units;
+    while (at < end && at < row_end) {
+      const int unit = (int)((at - row_at) / row.tiles), head = unit / p.blocks, block = unit - head * p.blocks;
+      const long a = row_at + (long)unit * row.tiles, b = a + row.tiles;        // the unit in the line
+      const long stop = b < end ? b : end;
+      const int q0 = block * QB, queries = p.group - q0 < QB ? p.group - q0 : QB;
+      // queries as the scores' second operand
+      const T* qp = reinterpret_cast<const T*>(p.q) + (long)r * p.ldq + ((long)head * p.group + q0 + (c16 < queries ? c16 : 0)) * p.d;
+#pragma unroll
+      for (int kk = 0; kk < S::KK; ++kk) {
+        const int dim = kk * 32 + g4 * 8;
+        T e[8] = {};
+        if (c16 < queries && (!TAIL || dim < p.d)) {
+          if (p.q_aligned) __builtin_memcpy(e, __builtin_assume_aligned(qp + dim, 16), 16);
+          else
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e[i] = qp[dim + i];
+        }
+        __builtin_memcpy(&wv.q[kk], e, 16);
+      }
+      wv.begin();
+      const float factor = p.scale_log2 * (CODES && p.k_scale ? p.k_scale[head] : 1.f);
+      for (long t = at; t < stop; ++t) {
+        const int t0 = (row.tile + (int)(t - a)) * TILE + wave * STEP;
+        if (t0 < row.n && t0 + STEP > row.low) wv.step(p, row, head, t0, factor);
+      }
+      // the waves' parts together
+      float sum = wv.l;
+      sum += __shfl_xor(sum, 16, 64);
+      sum += __shfl_xor(sum, 32, 64);
+      if (g4 == 0) {
+        ms[wave * QB + c16] = wv.m;
+        ms[(NW + wave) * QB + c16] = sum;
+      }
+      __syncthreads();
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) top = fmaxf(top, ms[i * QB + c16]);
+      const float by = wv.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(wv.m - top);
+#pragma unroll
+      for (int c = 0; c < S::NC; ++c)
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int j = 0; j < S::VE; j += 4) {
+            f32x4 f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = wv.o[c * S::VE + j + i][n] * by;
+            *reinterpret_cast<f32x4*>(lds + (wave * QB + c16) * OW + c * 128 + S::VE * (4 * g4 + n) + j) = f;
+          }
+      __syncthreads();
+      const bool complete = a >= begin && b <= end;
+      const long slot = 2 * (long)w + (a >= begin ? 1 : 0);
+      const int q_max = p.group < QB ? p.group : QB;
+      for (int i = tid; i < queries * (D / 4); i += NW * 64) {
+        const int qi = i / (D / 4), dim = (i - qi * (D / 4)) * 4;
+        if (TAIL && dim >= p.d) continue;
+        f32x4 f{0.f, 0.f, 0.f, 0.f};
+        float top_q = -INFINITY, sum_q = 0.f;
+#pragma unroll
+        for (int x = 0; x < NW; ++x) {
+          f += *reinterpret_cast<const f32x4*>(lds + (x * QB + qi) * OW + dim);
+          top_q = fmaxf(top_q, ms[x * QB + qi]);
+        }
+#pragma unroll
+        for (int x = 0; x < NW; ++x) {
+          const float mx = ms[x * QB + qi];
+          sum_q += ms[(NW + x) * QB + qi] * (mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - top_q));
+        }
+        if (complete) {
+          const float scale = CODES && p.v_scale ? p.v_scale[head] : 1.f;
+          T* to = reinterpret_cast<T*>(p.o) + (long)r * p.ldo + ((long)head * p.group + q0 + qi) * p.d + dim;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) to[e] = (T)(sum_q == 0.f ? 0.f : f[e] / sum_q * scale);
+        } else {
+          *reinterpret_cast<f32x4*>(p.part + (slot * q_max + qi) * p.d + dim) = f;
+          if (dim == 0) {
+            float* stats = p.part + 2 * (long)G * q_max * p.d + (slot * q_max + qi) * 2;
+            stats[0] = top_q;
+            stats[1] = sum_q;
+          }
+        }
+      }
+      // where this workgroup begins in a unit that the one before it began: the unit's row, number and workgroups
+      if (tid == 0 && a < begin && total * (w - 1) / W <= a)
+        p.border[w] = int4{r, unit, w - 1, (int)((b * W - 1) / total)};
+      __syncthreads();                                  // (LDS is read)
+      at = stop;
+    }
+    row_at = row_end;
+  }
+}
+
+// The parts of a unit that several workgroups have, in their order; a workgroup for each border and query head.
+template <int D, typename T, bool CODES>
+__global__ __launch_bounds__(256) void join(const PagedParams p, const int G_all) {
+  const int4 u = p.border[blockIdx.x + 1];
+  if (u.x < 0) return;
+  const int qi = blockIdx.y, head = u.y / p.blocks, q0 = (u.y - head * p.blocks) * QB, q_max = p.group < QB ? p.group : QB;
+  if (qi >= p.group - q0) return;
+  constexpr int DL = D / 4, G = 256 / DL;               // lanes of an output, groups that take parts in turn
+  __shared__ float red[256], sums[256];
+  __shared__ f32x4 outs[G][DL];
+  const int tid = threadIdx.x, first = u.z, last = u.w;
+  const float* stats = p.part + 2 * (long)G_all * q_max * p.d;
+  auto slot = [&](int w) { return (2 * (long)w + (w == first ? 1 : 0)) * q_max + qi; };
+  float top = -INFINITY;
+  for (int w = first + tid; w <= last; w += 256) top = fmaxf(top, stats[slot(w) * 2]);
+  red[tid] = top;
+  __syncthreads();
+  for (int s = 128; s > 0; s >>= 1) {
+    if (tid < s) red[tid] = fmaxf(red[tid], red[tid + s]);
+    __syncthreads();
+  }
+  top = red[0];
+  const int g = tid / DL, dim = (tid - g * DL) * 4;
+  f32x4 f{0.f, 0.f, 0.f, 0.f};
+  float sum = 0.f;
+  for (int w = first + g; w <= last; w += G) {
+    const float mx = stats[slot(w) * 2], by = mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - top);
+    sum += stats[slot(w) * 2 + 1] * by;
+    if (dim < p.d) f += *reinterpret_cast<const f32x4*>(p.part + slot(w) * p.d + dim) * by;
+  }
+  outs[g][tid - g * DL] = f;
+  sums[tid] = sum;
+  __syncthreads();
+  if (g > 0 || dim >= p.d) return;
+  for (int i = 1; i < G; ++i) {
+    f += outs[i][tid];
+    sum += sums[i * DL + tid];
+  }
+  const float scale = CODES && p.v_scale ? p.v_scale[head] : 1.f;
+  T* to = reinterpret_cast<T*>(p.o) + (long)u.x * p.ldo + ((long)head * p.group + q0 + qi) * p.d + dim;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) to[e] = (T)(sum == 0.f ? 0.f : f[e] / sum * scale);
+}
+
+// Workgroups: as many as run at once (D 256: one a CU), but no more than there can be tiles.
+struct Plan { long workgroups; bool parts; };
+
+Plan plan_of(int64_t rows, int64_t kv_heads, int64_t group, int64_t d, int64_t span) {
+  const long tiles = (span + TILE - 1) / TILE, units = rows * kv_heads * ((group + QB - 1) / QB);
+  const long at_once = 256 * (d > 128 ? 1 : 3);
+  return Plan{units * tiles < at_once ? units * tiles : at_once, tiles > 1};
+}
+
+int64_t bytes_of(const Plan& plan, int64_t group, int64_t d) {
+  const int64_t q = group < QB ? group : QB;
+  return plan.workgroups * 16 + 2 * plan.workgroups * q * (d + 2) * 4;
+}
+
+template <int D, typename T, bool CODES, bool EIGHT, bool TAIL>
+int run(const PagedParams& p, const Plan& plan, hipStream_t s) {
+  constexpr int lds = (NW * QB * (D + 4) + 2 * NW * QB) * 4;
+  if (lds > 65536) {
+    const hipError_t e = kh_allow_lds<attend<D, T, CODES, EIGHT, TAIL>>(lds);
+    if (e != hipSuccess) return (int)e;
+  }
+  kh_launch(KH_TAG_PAGED_ATTENTION, attend<D, T, CODES, EIGHT, TAIL>, dim3((unsigned)plan.workgroups), dim3(NW * 64), lds, s, p);
+  if (plan.parts && plan.workgroups > 1) {
+    const hipError_t e = hipGetLastError();             // (the launch behind it reads what it writes)
+    if (e != hipSuccess) return (int)e;
+    kh_launch(KH_TAG_PAGED_JOIN, join<D, T, CODES>, dim3((unsigned)plan.workgroups - 1, (unsigned)(p.group < QB ? p.group : QB)), dim3(256), 0, s, p, (int)plan.workgroups);
+  }
+  KH_RETURN_LAST_ERROR();
+}
+template <int D, typename T, bool CODES>
+int run(const PagedParams& p, const Plan& plan, hipStream_t s) {
+  return p.d == D ? run<D, T, CODES, false, false>(p, plan, s) : run<D, T, CODES, false, true>(p, plan, s);
+}
+template <typename T, bool CODES>
+int run(const PagedParams& p, const Plan& plan, hipStream_t s) {
+  return p.d <= 64 ? run<64, T, CODES>(p, plan, s) : p.d <= 128 ? run<128, T, CODES>(p, plan, s) : run<256, T, CODES>(p, plan, s);
+}
+
+}  // namespace
+
+KH_EXPORT int64_t kh_paged_attention_workspace_bytes(int64_t rows, int64_t heads, int64_t kv_heads, int64_t d, int64_t span) {
+  if (rows <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || d <= 0 || span <= 0) return KH_ERR_INVALID_ARG;
+  if (d % 8 != 0 || d > 256) return KH_ERR_UNSUPPORTED;
+  if (rows > (1L << 24) || heads > (1L << 16) || span > (1L << 30)) return KH_ERR_TOO_LARGE;
+  return bytes_of(plan_of(rows, kv_heads, heads / kv_heads, d, span), heads / kv_heads, d);
+}
+
+KH_EXPORT int kh_paged_attention(const void* q, void* o, const KhPagedCache* cache, int64_t layer, const int32_t* slots, const int32_t* lengths,
+                                 void* workspace, int64_t rows, int64_t heads, int64_t ldq, int64_t ldo, int64_t window, float scale, int flags, int type,
+                                 void* stream) {
+  const int rc = kh_cache_check(cache);
+  if (rc != KH_OK) return rc;
+  const KhPagedCache& c = *cache;
+  if (!q || !o || !workspace || rows <= 0 || heads <= 0 || heads % c.kv_heads != 0 || window < 0 || (flags & ~1) || type < 0 || type > 1) return KH_ERR_INVALID_ARG;
+  if (layer < 0 || layer >= c.layers || ldq < heads * c.d || ldo < heads * c.d || (!slots && rows > c.slots)) return KH_ERR_INVALID_ARG;
+  if (c.type != KH_E4M3 && c.type != type) return KH_ERR_UNSUPPORTED;
+  if ((((uintptr_t)q | (uintptr_t)o) & 1) || (((uintptr_t)slots | (uintptr_t)lengths) & 3) || !kh_aligned16(workspace)) return KH_ERR_ALIGNMENT;
+  if (rows > (1L << 24) || heads > (1L << 16)) return KH_ERR_TOO_LARGE;
+  const long group = heads / c.kv_heads, e = kh_cache_element(c);
+  const Plan plan = plan_of(rows, c.kv_heads, group, c.d, c.width * c.page);
+  PagedParams p{q, (const char*)c.k + layer * c.k_layer * e, (const char*)c.v + layer * c.v_layer * e, o, c.table, lengths, c.lengths, slots,
+                c.k_scale ? c.k_scale + layer * c.kv_heads : nullptr, c.v_scale ? c.v_scale + layer * c.kv_heads : nullptr,
+                (float*)((char*)workspace + plan.workgroups * 16), (int4*)workspace, ldq, ldo, c.k_page, c.k_token, c.k_head, c.v_page, c.v_token, c.v_head,
+                (int)rows, (int)c.kv_heads, (int)group, (int)((group + QB - 1) / QB), (int)c.d, (int)c.slots, (int)c.width, (int)c.pages, (int)c.page,
+                (int)(window < (1L << 30) ? window : 0), scale * 1.4426950408889634f, flags & 1, 0, KhDivide((uint32_t)c.page)};
+  p.q_aligned = kh_aligned16(q) && ldq % 8 == 0;
+  hipStream_t s = (hipStream_t)stream;
+  const bool codes = c.type == KH_E4M3;
+  if (type == 0) return codes ? run<bf16_t, true>(p, plan, s) : run<bf16_t, false>(p, plan, s);
+  return codes ? run<f16_t, true>(p, plan, s) : run<f16_t, false>(p, plan, s);
+}

@@ -12,6 +12,7 @@ import ctypes
 import functools
 import math
 import os
+import struct
 import threading
 import weakref
 from typing import Optional, Sequence
@@ -1668,11 +1669,296 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, hea
     return out, state_out
 
 
+# Attention over a paged cache: rotary positions, the cache and its pages, single tokens.
+_CACHE_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float8_e4m3fn: 3}
+_POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+_pack_cache = struct.Struct("23q").pack          # KhPagedCache
+
+
+class PagedCache:
+    """Keys and values of sequences in pages of `page` tokens, for all layers of a model.
+
+    k, v [layers, pages, page, kv_heads, d] in bf16, fp16 or float8_e4m3fn (views allowed: the last axis contiguous, strides a multiple of 8), d a multiple
+    of 8 up to 256; table int32 [slots, width]: the pages of each slot's sequence in order, -1 where there is none; lengths int32 [slots], its tokens;
+    refs int32 [pages], how many sequences hold a page (0: free; None for a cache that somebody else keeps).  k_scale, v_scale float32 [layers, kv_heads],
+    float8 only: a code c stands for c * scale (None: 1).  `empty` makes one without sequences.  cache_extend, cache_reorder and cache_compact keep table,
+    lengths and refs, on the device; a program that fills them itself keeps shared pages whole: cache_append does not look at refs."""
+    __slots__ = ("k", "v", "table", "lengths", "refs", "k_scale", "v_scale", "layers", "pages", "page", "kv_heads", "d", "slots", "width", "desc")
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, refs: Optional[torch.Tensor] = None,
+                 k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None):
+        dt, shape = k.dtype, k.shape
+        kind = _CACHE_TYPES.get(dt)
+        if kind is None or v.dtype is not dt:
+            raise TypeError(f"k and v must both be bf16, fp16 or float8_e4m3fn, got {dt} and {v.dtype}")
+        if len(shape) != 5 or v.shape != shape or 0 in shape:
+            raise ValueError(f"k and v must be [layers, pages, page, kv_heads, d], got {tuple(shape)} and {tuple(v.shape)}")
+        layers, pages, page, kv_heads, d = shape
+        ks, vs = k.stride(), v.stride()
+        if ks[4] != 1 or vs[4] != 1 or d % 8 or d > 256:
+            raise ValueError("the last axis of k and v must be contiguous, a multiple of 8 up to 256")
+        if table.dim() != 2 or not table.shape[0] or not table.shape[1]:
+            raise ValueError("table must be [slots, width]")
+        slots, width = table.shape
+        _fits(table, torch.int32, (slots, width), "table")
+        _fits(lengths, torch.int32, (slots,), "lengths")
+        dev = k.get_device()
+        others = [v, table, lengths]
+        if refs is not None:
+            _fits(refs, torch.int32, (pages,), "refs")
+            others.append(refs)
+        for name, scale in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if scale is not None:
+                if kind != 3:
+                    raise ValueError(f"{name} with a cache that is not float8")
+                _fits(scale, torch.float32, (layers, kv_heads), name)
+                others.append(scale)
+        for t in others:
+            if t.get_device() != dev:
+                raise ValueError("the parts of a cache must lie on one device")
+        self.k, self.v, self.table, self.lengths, self.refs, self.k_scale, self.v_scale = k, v, table, lengths, refs, k_scale, v_scale
+        self.layers, self.pages, self.page, self.kv_heads, self.d, self.slots, self.width = layers, pages, page, kv_heads, d, slots, width
+        self.desc = _pack_cache(k.data_ptr(), v.data_ptr(), table.data_ptr(), lengths.data_ptr(), 0 if refs is None else refs.data_ptr(),
+                                0 if k_scale is None else k_scale.data_ptr(), 0 if v_scale is None else v_scale.data_ptr(),
+                                layers, pages, page, kv_heads, d, slots, width, kind, ks[0], ks[1], ks[2], ks[3], vs[0], vs[1], vs[2], vs[3])
+
+    @classmethod
+    def empty(cls, layers: int, pages: int, page: int, kv_heads: int, d: int, slots: int, width: int, dtype: torch.dtype = BF16, device="cuda",
+              k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None) -> "PagedCache":
+        """A cache whose pages are all free and whose slots hold nothing."""
+        k, v = (torch.zeros((layers, pages, page, kv_heads, d), dtype=dtype, device=device) for _ in range(2))
+        return cls(k, v, torch.full((slots, width), -1, dtype=torch.int32, device=device), torch.zeros(slots, dtype=torch.int32, device=device),
+                   torch.zeros(pages, dtype=torch.int32, device=device), k_scale, v_scale)
+
+
+def _cache_parts(cache: PagedCache):
+    return cache.v, cache.table, cache.lengths, cache.refs, cache.k_scale, cache.v_scale
+
+
+def _cache_call(name: str, cache: PagedCache, asked: Optional[torch.Tensor]) -> torch.Tensor:
+    """One of the calls that keep a cache's pages: what it tells, int32 [1] on the device."""
+    lib = _lib.load()
+    if cache.refs is None:
+        raise ValueError("a cache without refs has no pages to give")
+    lengths = cache.lengths
+    if asked is None:
+        _here(cache.k, lengths)
+    else:
+        _here(cache.k, lengths, asked)
+        _fits(asked, torch.int32, (cache.slots,), "counts" if name == "kh_cache_extend" else "parents")
+    nbytes = _workspace_bytes("kh_cache_workspace_bytes", cache.slots, cache.width, cache.pages)
+    if nbytes < 0:
+        _lib.check(nbytes, name)
+    told, ws = lengths.new_empty(1), lengths.new_empty(nbytes // 4)
+    rest = (told.data_ptr(), ws.data_ptr(), _stream())
+    rc = getattr(lib, name)(cache.desc, *rest) if asked is None else getattr(lib, name)(cache.desc, asked.data_ptr(), *rest)
+    if rc:
+        _lib.check(rc, name)
+    return told
+
+
+def cache_extend(cache: PagedCache, counts: torch.Tensor) -> torch.Tensor:
+    """Room for counts[s] (int32 [slots], on the GPU; <= 0: none) more tokens behind the sequence of every slot s: cache.lengths grow by that much (at most to
+    width * page) and what passes the last page gets new ones, the lowest free, by slot and then by place.  Returns int32 [1] on the GPU: how many pages were
+    wanted and not there; their entries are -1, cache_append drops what belongs there and attention leaves it out."""
+    return _cache_call("kh_cache_extend", cache, counts)
+
+
+def cache_reorder(cache: PagedCache, parents: torch.Tensor) -> torch.Tensor:
+    """Slot s keeps its sequence where parents[s] == s (int32 [slots], on the GPU), takes over the one that slot parents[s] had before the call, or, where that is
+    no slot (-1), is emptied and its pages freed as far as nobody else holds them: beams that go on from others, answers that fork from a prompt,
+    requests that end.  Whole pages are shared; the page not yet full is copied in all layers, or handed on to the lowest taker where its owner gives it
+    up.  Returns as cache_extend does."""
+    return _cache_call("kh_cache_reorder", cache, parents)
+
+
+def cache_compact(cache: PagedCache) -> torch.Tensor:
+    """Moves the pages in use together: those from their number n on go to the free ones below, in all layers and tables.  Returns n, int32 [1] on the GPU."""
+    return _cache_call("kh_cache_compact", cache, None)
+
+
+def rotary_frequencies(pairs: int, base: float = 10000.0, sections: Optional[Sequence[int]] = None, device="cuda") -> torch.Tensor:
+    """Angles of a step, float64 [pairs]: base^(-j / pairs) for pair j; with sections every axis has a row of its own, base^(-j / section)."""
+    if sections is not None and sum(sections) != pairs:
+        raise ValueError(f"sections {tuple(sections)} for {pairs} pairs")
+    parts = [float(base) ** (-torch.arange(n, dtype=torch.float64) / n) for n in ((pairs,) if sections is None else sections) if n]
+    return torch.cat(parts).to(device) if parts else torch.zeros(0, dtype=torch.float64, device=device)
+
+
+@functools.lru_cache(maxsize=1024)
+def _section_ends(sections):
+    """(ends as int64s, axes, pairs)."""
+    if not 1 <= len(sections) <= 4 or any(int(n) != n or n < 0 for n in sections):
+        raise ValueError(f"sections must be one to four numbers of pairs, got {sections}")
+    ends = [sum(sections[:i + 1]) for i in range(len(sections))]
+    return struct.pack("4q", *(ends + ends[-1:] * 3)[:4]), len(ends), ends[-1]
+
+
+def _token_rows(t: torch.Tensor, width: int, name: str):
+    """(rows, their stride) of [..., width] whose leading axes are one run of rows."""
+    shape, st = t.shape, t.stride()
+    if len(shape) < 2 or shape[-1] != width or (st[-1] != 1 and width > 1):
+        raise ValueError(f"{name} must be [.., {width}] with a contiguous last axis, got {tuple(shape)}")
+    rows, ld = shape[-2], st[-2]
+    for n, s in zip(shape[-3::-1], st[-3::-1]):
+        if rows == 1:
+            ld = s
+        elif n > 1 and s != ld * rows:
+            raise ValueError(f"the leading axes of {name} must be one run of rows")
+        rows *= n
+    return rows, ld if rows > 1 else width
+
+
+def _rotary_call(q, k, v, heads: int, kv: int, positions, frequencies, sections, pairs: bool, out, k_out, cache, layer, slots, places, fill: int):
+    lib = _lib.load()
+    dt = q.dtype
+    if dt not in _TYPES or k.dtype is not dt or (v is not None and v.dtype is not dt):
+        raise TypeError(f"q, k and v must have one type, bf16, fp16 or fp32, got {dt} and {k.dtype}")
+    if heads < 1 or kv < 1 or q.dim() < 2 or q.shape[-1] % heads:
+        raise ValueError(f"q must be [.., {heads} * d], got {tuple(q.shape)}")
+    d = q.shape[-1] // heads
+    rows, ldq = _token_rows(q, heads * d, "q")
+    k_rows, ldk = _token_rows(k, kv * d, "k")
+    v_rows, ldv = (rows, 0) if v is None else _token_rows(v, kv * d, "v")
+    o_rows, ldo = _token_rows(out, heads * d, "out")
+    ko_rows, ldko = (rows, 0) if k_out is None else _token_rows(k_out, kv * d, "k_out")
+    if k_rows != rows or v_rows != rows or o_rows != rows or ko_rows != rows:
+        raise ValueError("q, k, v and the outputs must have the same rows")
+    if out.dtype is not dt or (k_out is not None and k_out.dtype is not dt):
+        raise TypeError(f"outputs must be {dt}")
+    ends, axes, n = _section_ends(sections)
+    if 2 * n > d:
+        raise ValueError(f"{n} pairs in heads of {d}")
+    position_type = 0
+    if positions is not None:
+        position_type = _POSITION_TYPES.get(positions.dtype)
+        if position_type is None:
+            raise TypeError(f"positions must be int32, int64 or float32, got {positions.dtype}")
+        ps = positions.shape
+        if positions.numel() != rows * axes or not positions.is_contiguous() or (axes > 1 and ps[-1] != axes):
+            raise ValueError(f"positions must be contiguous [{rows}, {axes}], got {tuple(ps)}")
+    flags = bool(pairs) | fill << 1
+    if frequencies is not None:
+        ft = frequencies.dtype
+        if ft is torch.float32:
+            flags |= 4
+        elif ft is not torch.float64:
+            raise TypeError(f"frequencies must be float64 or float32, got {ft}")
+        if frequencies.shape != (n,) or not frequencies.is_contiguous():
+            raise ValueError(f"frequencies must be contiguous [{n}], got {tuple(frequencies.shape)}")
+    elif n:
+        raise ValueError("sections without frequencies")
+    if rows:
+        rc = lib.kh_rotary(q.data_ptr(), k.data_ptr(), _ptr(v), out.data_ptr(), _ptr(k_out), _ptr(positions), position_type, _ptr(frequencies), ends, axes,
+                           None if cache is None else cache.desc, layer, _ptr(slots), _ptr(places), rows, heads, kv, d, ldq, ldk, ldv, ldo, ldko, flags, _TYPES[dt], _stream())
+        if rc:
+            _lib.check(rc, "kh_rotary")
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor, heads: int, positions: torch.Tensor, frequencies: torch.Tensor, sections: Optional[Sequence[int]] = None,
+           kv_heads: Optional[int] = None, pairs: bool = False, out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None):
+    """(q', k') whose pairs are turned by their positions, on one to four axes (time, height, width): pair j of every head by the angle
+    positions[row, axis of j] * frequencies[j], worked out in 64 bits.
+
+    q [.., heads * d], k [.., kv_heads * d] (bf16, fp16 or fp32; the last axis contiguous, the leading ones one run of rows: slices of a stacked
+    projection's output are).  sections: how many pairs each axis has, in order (None: all frequencies on one axis); pairs are the dimensions (j, j + their number), or with
+    pairs=True (2 j, 2 j + 1); what a head has beyond them is copied.  positions [rows, axes] ([rows] for one axis) int32, int64 or float32;
+    frequencies float64 or float32 [pairs] (rotary_frequencies).  out may be q and k_out k (in place)."""
+    kv = heads if kv_heads is None else kv_heads
+    if out is None:
+        out = q.new_empty(q.shape)
+    if k_out is None:
+        k_out = k.new_empty(k.shape)
+    _here(q, k, positions, frequencies, out, k_out)
+    _rotary_call(q, k, None, heads, kv, positions, frequencies, (frequencies.numel(),) if sections is None else tuple(sections), pairs, out, k_out, None, 0, None, None, 0)
+    return out, k_out
+
+
+def cache_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: PagedCache, heads: int, positions: Optional[torch.Tensor] = None,
+                 frequencies: Optional[torch.Tensor] = None, sections: Optional[Sequence[int]] = None, layer: int = 0, slots: Optional[torch.Tensor] = None,
+                 places: Optional[torch.Tensor] = None, pairs: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """q' turned as by rotary, and k turned and v written into a layer of the cache, in one pass.
+
+    Row r is token places[r] of slot slots[r] (int32 [rows], on the GPU; together distinct), for which cache_extend has made room; without slots row r is slot r,
+    without places it is the last token of its sequence; without positions a token's position is its place, on every axis.  Without frequencies
+    nothing turns.  q [rows, heads * d], k and v [rows, kv_heads * d], bf16 or fp16, the cache's type unless that is float8 (then the nearest code to
+    value / scale, at most 448 off zero).  Rows whose slot lies outside the cache or whose place outside its sequence are left out (padded batches
+    in a captured graph): those of a given out stay as they were, those of a new one are zero.  out may be q."""
+    fill = out is None
+    if fill:
+        out = q.new_empty(q.shape)
+    if k.dtype not in (torch.bfloat16, torch.float16) or (cache.k.dtype is not k.dtype and cache.k.dtype is not torch.float8_e4m3fn):
+        raise TypeError(f"{k.dtype} rows for a cache of {cache.k.dtype}")
+    if not 0 <= layer < cache.layers:
+        raise ValueError(f"layer {layer} of a cache of {cache.layers}")
+    if q.shape[-1] != heads * cache.d:
+        raise ValueError(f"q must be [.., {heads} * {cache.d}], got {tuple(q.shape)}")
+    _here(q, k, v, positions, frequencies, slots, places, out, cache.k, *_cache_parts(cache))
+    rows = q.numel() // q.shape[-1]
+    if slots is not None:
+        _fits(slots, torch.int32, (rows,), "slots")
+    elif rows > cache.slots:
+        raise ValueError(f"{rows} rows without slots for a cache of {cache.slots}")
+    if places is not None:
+        _fits(places, torch.int32, (rows,), "places")
+    if sections is None:
+        sections = (0,) if frequencies is None else (frequencies.numel(),)
+    _rotary_call(q, k, v, heads, cache.kv_heads, positions, frequencies, tuple(sections), pairs, out, None, cache, layer, slots, places, fill)
+    return out
+
+
+def paged_attention(q: torch.Tensor, cache: PagedCache, heads: int, layer: int = 0, slots: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
+                    scale: Optional[float] = None, window: int = 0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """softmax(scale * q K^T) V of one token a row over a layer of the cache (scale: d^-0.5): q [rows, heads * d] (bf16 or fp16, the cache's type unless that is
+    float8), query head h on key head h // (heads // kv_heads).
+
+    Row r attends to the first lengths[r] tokens (int32 [rows], on the GPU; None: all that cache.lengths says) of slot slots[r] (None: slot r), of those with
+    window > 0 to the last `window`; tokens without a page are left out.  Several rows may have one slot: the tokens of a prompt, each with a length of
+    its own.  A row with nothing to attend to is zero.  Rows whose slot lies outside the cache are left out: those of a given out stay as they were, those of a
+    new one are zero.  An infinity among the values attended to gives NaN."""
+    lib = _lib.load()
+    dt, d = q.dtype, cache.d
+    if (dt is not torch.bfloat16 and dt is not torch.float16) or (cache.k.dtype is not dt and cache.k.dtype is not torch.float8_e4m3fn):
+        raise TypeError(f"q of {dt} over a cache of {cache.k.dtype}")
+    if heads < 1 or heads % cache.kv_heads:
+        raise ValueError(f"{heads} heads cannot share the keys of {cache.kv_heads}")
+    if not 0 <= layer < cache.layers or window < 0:
+        raise ValueError(f"layer {layer} of a cache of {cache.layers}, window {window}")
+    rows, ldq = _token_rows(q, heads * d, "q")
+    fill = out is None
+    if fill:
+        out = q.new_empty(q.shape)
+    elif out.dtype is not dt:
+        raise TypeError(f"out must be {dt}")
+    o_rows, ldo = _token_rows(out, heads * d, "out")
+    if o_rows != rows:
+        raise ValueError("q and out must have the same rows")
+    _here(q, slots, lengths, out, cache.k, *_cache_parts(cache))
+    if slots is not None:
+        _fits(slots, torch.int32, (rows,), "slots")
+    elif rows > cache.slots:
+        raise ValueError(f"{rows} rows without slots for a cache of {cache.slots}")
+    if lengths is not None:
+        _fits(lengths, torch.int32, (rows,), "lengths")
+    if not rows:
+        return out
+    nbytes = _workspace_bytes("kh_paged_attention_workspace_bytes", rows, heads, cache.kv_heads, d, cache.width * cache.page)
+    if nbytes < 0:
+        _lib.check(nbytes, "kh_paged_attention_workspace_bytes")
+    ws = q.new_empty(nbytes // 2)              # (elements of two bytes)
+    rc = lib.kh_paged_attention(q.data_ptr(), out.data_ptr(), cache.desc, layer, _ptr(slots), _ptr(lengths), ws.data_ptr(), rows, heads, ldq, ldo, window,
+                                d ** -0.5 if scale is None else scale, fill, _TYPES[dt], _stream())
+    if rc:
+        _lib.check(rc, "kh_paged_attention")
+    return out
+
+
 # --------------------------------------------------------------------------------------- per-launch timing
 KERNEL_TAGS = {1: "lora_gemm", 2: "lora_gemm_f32", 3: "attention", 4: "group_norm_stats", 5: "group_norm_apply",
                6: "layer_norm", 7: "geglu", 8: "residual_add", 9: "concat_residual", 10: "sgmv_shrink",
                11: "sgmv_expand", 12: "lora_shrink", 13: "conv3x3", 14: "cfg_euler", 15: "upsample", 16: "lora_merge", 17: "conv_out_step", 18: "sgmv_fused", 19: "lora_pack",
-               20: "block_norm", 21: "quantize_w4", 22: "dequantize_w4", 23: "w4_linear", 24: "w4_shrink", 25: "linear_attention"}
+               20: "block_norm", 21: "quantize_w4", 22: "dequantize_w4", 23: "w4_linear", 24: "w4_shrink", 25: "linear_attention",
+               26: "rotary", 27: "paged_attention", 28: "paged_join", 29: "cache_pages"}
 
 
 def profile_begin() -> None:
