@@ -18,6 +18,7 @@ namespace {
 
 constexpr int NW = 4, STEP = 32, TILE = NW * STEP;       // waves, tokens of a wave's step, of a tile
 constexpr int QB = 16;                                  // query heads of a unit
+constexpr int JT = 512, MOST = 1024;                    // threads that join, workgroups at most
 constexpr float RESCALE_LOG2 = 8.0f;                    // the running maximum moves only for jumps above 2^8
 
 struct PagedParams {
@@ -28,7 +29,8 @@ struct PagedParams {
   float* part;                // [2 workgroups][group][d] outputs, then [2 workgroups][group][2] maxima and sums
   int4* border;               // [workgroups]: row, unit, workgroups of the unit that a workgroup begins inside
   long ldq, ldo;
-  long k_page, k_token, k_head, v_page, v_token, v_head;   // elements
+  uint32_t k_page, k_token, v_page, v_token;            // bytes
+  long k_head, v_head;
   int rows, kv_heads, group, blocks, d;                 // blocks: units of a key head
   int n_slots, width, pages, page, window;
   float scale_log2;
@@ -130,7 +132,8 @@ __device__ __forceinline__ Row row_of(const PagedParams& p, int r) {
   return w;
 }
 
-// Shapes.  D: dimensions there is room for (d of them used: TAIL where fewer); CODES: the cache holds e4m3; EIGHT: pages of a multiple of eight tokens.
+// Shapes.  D: dimensions there is room for (d of them used: TAIL where fewer); CODES: the cache holds e4m3; EIGHT: pages of a multiple of eight tokens, so that
+// the eight tokens of a lane lie on one page.
 template <int D, typename T, bool CODES, bool EIGHT, bool TAIL>
 struct Shape {
   using X = typename Eight<T>::type;
@@ -139,139 +142,168 @@ struct Shape {
   static constexpr int NC = D >= 128 ? D / 128 : 1;     // pieces of a row of values in a lane
   static constexpr int VE = D >= 128 ? 8 : 4;           // elements of one
   static constexpr int ELT = CODES ? 1 : 2;
+  static constexpr int VW = VE * ELT / 4;               // words of one
 };
 
+// A wave's part of a unit.  Keys and values of a step are requested as soon as the registers of the step before are free (keys behind its scores, values behind
+// its products), the numbers of the pages a step earlier still, so that loads are on their way all the time.
 template <int D, typename T, bool CODES, bool EIGHT, bool TAIL>
 struct Wave {
   using S = Shape<D, T, CODES, EIGHT, TAIL>;
   using X = typename S::X;
+  struct Pages { int k[EIGHT ? 1 : 2], v[EIGHT ? 1 : 8]; };
+
   X q[S::KK];
   f32x4 o[S::NC * S::VE];                               // tile c * VE + j: dimensions c * 128 + VE * (4 * (l / 16) + r) + j of query l % 16
   float m, l;
+  typename S::Raw kr[2][S::KK];
+  uint32_t vr[8][S::NC][S::VW];
 
-  __device__ __forceinline__ void begin() {
+  // Tokens of lane l: of the keys 8 * (l % 16 / 4) + 4 s + l % 4, of the values (and of the scores it gets) 8 * (l / 16) + i.  One behind the end is
+  // looked for at the last one.
+  static __device__ __forceinline__ int key(int t0, int s) { return t0 + 8 * ((threadIdx.x & 15) >> 2) + 4 * s + (threadIdx.x & 3); }
+  static __device__ __forceinline__ int value(int t0, int i) { return t0 + 8 * ((threadIdx.x & 63) >> 4) + i; }
+  static __device__ __forceinline__ int kept(int t, int last) { return t < last ? t : last; }
+
+  __device__ __forceinline__ Pages pages_of(const PagedParams& p, const Row& row, int t0) const {
+    Pages e;
+    const int last = EIGHT ? (row.n - 1) & ~7 : row.n - 1;
 #pragma unroll
-    for (int i = 0; i < S::NC * S::VE; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    m = -INFINITY;
-    l = 0.f;
+    for (int s = 0; s < (EIGHT ? 1 : 2); ++s) e.k[s] = row.pages[p.by_page((uint32_t)kept(EIGHT ? key(t0, 0) & ~7 : key(t0, s), last))];
+#pragma unroll
+    for (int i = 0; i < (EIGHT ? 1 : 8); ++i) e.v[i] = row.pages[p.by_page((uint32_t)kept(value(t0, i), last))];
+    return e;
   }
-
-  // 32 tokens from t0 (a multiple of 32) on, of which low .. n - 1 count.
-  __device__ __forceinline__ void step(const PagedParams& p, const Row& row, int head, int t0, float factor) {
-    const int lane = threadIdx.x & 63, c16 = lane & 15, g4 = lane >> 4;
-    const char* kb = reinterpret_cast<const char*>(p.k) + head * p.k_head * S::ELT;
-    const char* vb = reinterpret_cast<const char*>(p.v) + head * p.v_head * S::ELT;
-    const int last = row.n - 1;
-    // where a token lies; a token behind the end is looked for at the last one, one without a page at the first of all
-    auto place = [&](int t, long page, long token, bool& good) -> long {
-      t = t < last ? t : last;
-      const int at = (int)p.by_page((uint32_t)t);
-      const int e = row.pages[at];
-      good = e >= 0 && e < p.pages;
-      return good ? (long)e * page + (long)(t - at * p.page) * token : 0;
-    };
-    bool good[8];
-    typename S::Raw kr[2][S::KK];
-    uint32_t vr[8][S::NC][S::VE * S::ELT / 4];
-    const int tv = t0 + 8 * g4;
+  // where a token's row lies; without a page: the first of all
+  static __device__ __forceinline__ const char* place(const PagedParams& p, const char* base, int e, int t, uint32_t page, uint32_t token) {
+    const uint32_t at = (uint32_t)t - p.by_page((uint32_t)t) * (uint32_t)p.page;
+    return (uint32_t)e < (uint32_t)p.pages ? base + (uint64_t)(uint32_t)e * page + (uint64_t)at * token : base;
+  }
+  __device__ __forceinline__ void load_keys(const PagedParams& p, const Row& row, const char* kb, const Pages& e, int t0) {
+    const int g4 = (threadIdx.x & 63) >> 4, last = EIGHT ? (row.n - 1) | 7 : row.n - 1;     // (a page of whole eights has the tokens up to there)
+    const char* at[2];
+    at[0] = place(p, kb, e.k[0], kept(key(t0, 0), last), p.k_page, p.k_token);
+    if (EIGHT) at[1] = place(p, kb, e.k[0], kept(key(t0, 1), last), p.k_page, p.k_token);
+    else at[1] = place(p, kb, e.k[EIGHT ? 0 : 1], kept(key(t0, 1), last), p.k_page, p.k_token);
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      bool any;
-      const char* at = kb + place(t0 + 8 * (c16 >> 2) + 4 * s + (c16 & 3), p.k_page, p.k_token, any) * S::ELT;
+    for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int kk = 0; kk < S::KK; ++kk) {
         const int dim = kk * 32 + g4 * 8;
         if (TAIL && kk * 32 >= p.d) kr[s][kk] = typename S::Raw{};
-        else {
-          kr[s][kk] = *reinterpret_cast<const typename S::Raw*>(at + (!TAIL || dim < p.d ? dim : 0) * S::ELT);
-          if (TAIL && dim >= p.d) kr[s][kk] = typename S::Raw{};
-        }
+        else kr[s][kk] = *reinterpret_cast<const typename S::Raw*>(at[s] + (!TAIL || dim < p.d ? dim : 0) * S::ELT);
       }
-    }
+  }
+  __device__ __forceinline__ void load_values(const PagedParams& p, const Row& row, const char* vb, const Pages& e, int t0) {
+    const int c16 = threadIdx.x & 15, last = EIGHT ? (row.n - 1) & ~7 : row.n - 1;
+    const char* first = place(p, vb, e.v[0], kept(value(t0, 0), last), p.v_page, p.v_token);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const char* at = vb + place(tv + i, p.v_page, p.v_token, good[i]) * S::ELT;
-      good[i] = good[i] && tv + i >= row.low && tv + i < row.n;
+      const char* at = EIGHT ? first + (uint64_t)p.v_token * i : i == 0 ? first : place(p, vb, e.v[EIGHT ? 0 : i], kept(value(t0, i), last), p.v_page, p.v_token);
 #pragma unroll
       for (int c = 0; c < S::NC; ++c) {
         const int dim = c * 128 + c16 * S::VE;
         __builtin_memcpy(vr[i][c], __builtin_assume_aligned(at + (!TAIL || dim < p.d ? dim : 0) * S::ELT, S::VE * S::ELT), S::VE * S::ELT);
       }
     }
-    // what does not count may be anything
-    bool whole = true;
+  }
+
+  // Tokens t0, t0 + TILE, .. of the row, `steps` times 32, of which low .. n - 1 count (steps 0: none).
+  __device__ __forceinline__ void run(const PagedParams& p, const Row& row, int head, int t0, int steps, float factor) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) whole = whole && good[i];
-    const bool cut = __any(!whole);
-    if (cut) {
+    for (int i = 0; i < S::NC * S::VE; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m = -INFINITY;
+    l = 0.f;
+    if (steps <= 0) return;
+    const char* kb = reinterpret_cast<const char*>(p.k) + head * p.k_head;
+    const char* vb = reinterpret_cast<const char*>(p.v) + head * p.v_head;
+    Pages now = pages_of(p, row, t0);
+    load_keys(p, row, kb, now, t0);
+    load_values(p, row, vb, now, t0);
+    Pages next = pages_of(p, row, t0 + (steps > 1 ? TILE : 0));
+    for (int n = 1;; ++n) {
+      const bool more = n < steps;
+      // scores: x[4 s + r] is token 8 * (l / 16) + 4 s + r of query l % 16
+      float x[8];
+      const int g4 = (threadIdx.x & 63) >> 4;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int s = 0; s < 2; ++s) {
+        f32x4 acc{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < S::NC; ++c)
-#pragma unroll
-          for (int w = 0; w < S::VE * S::ELT / 4; ++w) vr[i][c][w] = good[i] ? vr[i][c][w] : 0;
-    }
-    // scores: x[4 s + r] is token tv + 4 s + r of query l % 16
-    float x[8];
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      f32x4 acc{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int kk = 0; kk < S::KK; ++kk) {
-        X a;
-        if constexpr (CODES) {
-          const u32x2 w = kr[s][kk];
-          a = __builtin_bit_cast(X, u32x4{two_of_e4m3<T, false>(w[0]), two_of_e4m3<T, true>(w[0]), two_of_e4m3<T, false>(w[1]), two_of_e4m3<T, true>(w[1])});
-        } else {
-          a = __builtin_bit_cast(X, kr[s][kk]);
+        for (int kk = 0; kk < S::KK; ++kk) {
+          typename S::Raw w = kr[s][kk];
+          if (TAIL && kk * 32 + g4 * 8 >= p.d) w = typename S::Raw{};
+          X a;
+          if constexpr (CODES) a = __builtin_bit_cast(X, u32x4{two_of_e4m3<T, false>(w[0]), two_of_e4m3<T, true>(w[0]), two_of_e4m3<T, false>(w[1]), two_of_e4m3<T, true>(w[1])});
+          else a = __builtin_bit_cast(X, w);
+          acc = mfma(a, q[kk], acc);
         }
-        acc = mfma(a, q[kk], acc);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[4 * s + r] = acc[r] * factor;
       }
+      if (more) load_keys(p, row, kb, next, t0 + TILE);
+      // what does not count may be anything: scores and values of tokens outside, or without a page
+      const int first = value(t0, 0);
+      bool good[8], whole = true;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) x[4 * s + r] = acc[r] * factor;
-    }
-    if (cut) {
+      for (int i = 0; i < 8; ++i) {
+        good[i] = (uint32_t)now.v[EIGHT ? 0 : i] < (uint32_t)p.pages && first + i >= row.low && first + i < row.n;
+        whole = whole && good[i];
+      }
+      if (__any(!whole)) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = good[i] ? x[i] : -INFINITY;
-    }
-    float top = x[0];
+        for (int i = 0; i < 8; ++i) {
+          x[i] = good[i] ? x[i] : -INFINITY;
 #pragma unroll
-    for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);
-    top = swapped_max(top);
-    if (__any(top > m + RESCALE_LOG2)) {
-      const float now = fmaxf(m, top), by = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - now);
-      m = now;
-      l *= by;
+          for (int c = 0; c < S::NC; ++c)
 #pragma unroll
-      for (int i = 0; i < S::NC * S::VE; ++i) o[i] *= by;
-    }
-    const float from = m == -INFINITY ? 0.f : m;
-    float pr[8];
+            for (int w = 0; w < S::VW; ++w) vr[i][c][w] = good[i] ? vr[i][c][w] : 0;
+        }
+      }
+      float top = x[0];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      pr[i] = __builtin_amdgcn_exp2f(x[i] - from);
-      l += pr[i];
-    }
-    X pieces[Pieces<T>::N];
-    Pieces<T>::of(pr, pieces);
+      for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);
+      top = swapped_max(top);
+      if (__any(top > m + RESCALE_LOG2)) {
+        const float to = fmaxf(m, top), by = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - to);
+        m = to;
+        l *= by;
 #pragma unroll
-    for (int c = 0; c < S::NC; ++c)
+        for (int i = 0; i < S::NC * S::VE; ++i) o[i] *= by;
+      }
+      const float from = m == -INFINITY ? 0.f : m;
+      float pr[8];
 #pragma unroll
-      for (int j = 0; j < S::VE; ++j) {
-        u32x4 a;
+      for (int i = 0; i < 8; ++i) {
+        pr[i] = __builtin_amdgcn_exp2f(x[i] - from);
+        l += pr[i];
+      }
+      X pieces[Pieces<T>::N];
+      Pieces<T>::of(pr, pieces);
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {                   // tokens 2 h, 2 h + 1
-          if constexpr (CODES) {
-            const uint32_t both = __builtin_amdgcn_perm(vr[2 * h + 1][c][j / 4], vr[2 * h][c][j / 4], 0x0400u + (j % 4) * 0x0101u);
-            a[h] = two_of_e4m3<T, false>(both);
-          } else {
-            a[h] = __builtin_amdgcn_perm(vr[2 * h + 1][c][j / 2], vr[2 * h][c][j / 2], j & 1 ? 0x07060302 : 0x05040100);
+      for (int c = 0; c < S::NC; ++c)
+#pragma unroll
+        for (int j = 0; j < S::VE; ++j) {
+          u32x4 a;
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {                 // tokens 2 h, 2 h + 1
+            if constexpr (CODES) {
+              const uint32_t both = __builtin_amdgcn_perm(vr[2 * h + 1][c][j / 4], vr[2 * h][c][j / 4], 0x0400u + (j % 4) * 0x0101u);
+              a[h] = two_of_e4m3<T, false>(both);
+            } else {
+              a[h] = __builtin_amdgcn_perm(vr[2 * h + 1][c][j / 2], vr[2 * h][c][j / 2], j & 1 ? 0x07060302 : 0x05040100);
+            }
           }
-        }
-        const X value = __builtin_bit_cast(X, a);
+          const X value8 = __builtin_bit_cast(X, a);
 #pragma unroll
-        for (int n = 0; n < Pieces<T>::N; ++n) o[c * S::VE + j] = mfma(value, pieces[n], o[c * S::VE + j]);
-      }
+          for (int n2 = 0; n2 < Pieces<T>::N; ++n2) o[c * S::VE + j] = mfma(value8, pieces[n2], o[c * S::VE + j]);
+        }
+      if (!more) break;
+      t0 += TILE;
+      load_values(p, row, vb, next, t0);
+      now = next;
+      next = pages_of(p, row, t0 + (n + 1 < steps ? TILE : 0));
+    }
   }
 };
 
@@ -282,7 +314,7 @@ __device__ __forceinline__ void zero_row(const PagedParams& p, int r) {
 }
 
 template <int D, typename T, bool CODES, bool EIGHT, bool TAIL>
-__global__ __launch_bounds__(NW * 64) void attend(const PagedParams p) {
+__global__ __launch_bounds__(NW * 64, D > 128 ? 1 : D > 64 ? 3 : 4) void attend(const PagedParams p) {
   using S = Shape<D, T, CODES, EIGHT, TAIL>;
   constexpr int OW = D + 4;                             // floats of a query's row in LDS
   extern __shared__ float lds[];                        // [NW][QB][OW] outputs, [2][NW][QB] maxima and sums
@@ -359,12 +391,11 @@ __global__ __launch_bounds__(NW * 64) void attend(const PagedParams p) {
         }
         __builtin_memcpy(&wv.q[kk], e, 16);
       }
-      wv.begin();
       const float factor = p.scale_log2 * (CODES && p.k_scale ? p.k_scale[head] : 1.f);
-      for (long t = at; t < stop; ++t) {
-        const int t0 = (row.tile + (int)(t - a)) * TILE + wave * STEP;
-        if (t0 < row.n && t0 + STEP > row.low) wv.step(p, row, head, t0, factor);
-      }
+      int t0 = (row.tile + (int)(at - a)) * TILE + wave * STEP, steps = (int)(stop - at);
+      if (t0 + (steps - 1) * TILE >= row.n) --steps;     // (only the last tile may begin behind the end for some waves,
+      if (t0 + STEP <= row.low) t0 += TILE, --steps;     //  only the first end before the window)
+      wv.run(p, row, head, t0, steps, factor);
       // the waves' parts together
       float sum = wv.l;
       sum += __shfl_xor(sum, 16, 64);
@@ -434,42 +465,52 @@ __global__ __launch_bounds__(NW * 64) void attend(const PagedParams p) {
 
 // The parts of a unit that several workgroups have, in their order; a workgroup for each border and query head.
 template <int D, typename T, bool CODES>
-__global__ __launch_bounds__(256) void join(const PagedParams p, const int G_all) {
+__global__ __launch_bounds__(JT) void join(const PagedParams p, const int G_all) {
   const int4 u = p.border[blockIdx.x + 1];
   if (u.x < 0) return;
   const int qi = blockIdx.y, head = u.y / p.blocks, q0 = (u.y - head * p.blocks) * QB, q_max = p.group < QB ? p.group : QB;
   if (qi >= p.group - q0) return;
-  constexpr int DL = D / 4, G = 256 / DL;               // lanes of an output, groups that take parts in turn
-  __shared__ float red[256], sums[256];
+  constexpr int DL = D / 4, G = JT / DL;                // lanes of an output, groups that take parts in turn
+  __shared__ float weight[MOST], red[JT / 64], sums[JT / 64];
   __shared__ f32x4 outs[G][DL];
-  const int tid = threadIdx.x, first = u.z, last = u.w;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, first = u.z, parts = u.w - u.z + 1;
   const float* stats = p.part + 2 * (long)G_all * q_max * p.d;
-  auto slot = [&](int w) { return (2 * (long)w + (w == first ? 1 : 0)) * q_max + qi; };
-  float top = -INFINITY;
-  for (int w = first + tid; w <= last; w += 256) top = fmaxf(top, stats[slot(w) * 2]);
-  red[tid] = top;
+  auto slot = [&](int i) { return (2 * (long)(first + i) + (i == 0 ? 1 : 0)) * q_max + qi; };
+  // what every part's outputs and sum are multiplied with
+  float top = -INFINITY, sum = 0.f;
+  for (int i = tid; i < parts; i += JT) top = fmaxf(top, weight[i] = stats[slot(i) * 2]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+  if (lane == 0) red[wave] = top;
   __syncthreads();
-  for (int s = 128; s > 0; s >>= 1) {
-    if (tid < s) red[tid] = fmaxf(red[tid], red[tid + s]);
-    __syncthreads();
+#pragma unroll
+  for (int i = 0; i < JT / 64; ++i) top = fmaxf(top, red[i]);
+  for (int i = tid; i < parts; i += JT) {
+    const float mx = weight[i], by = mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - top);    // (its own: nobody else reads it before the barrier)
+    weight[i] = by;
+    sum += stats[slot(i) * 2 + 1] * by;
   }
-  top = red[0];
-  const int g = tid / DL, dim = (tid - g * DL) * 4;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  if (lane == 0) sums[wave] = sum;
+  __syncthreads();
+  const int g = tid / DL, dim = (tid - g * DL) * 4, at = dim < p.d ? dim : 0;
   f32x4 f{0.f, 0.f, 0.f, 0.f};
-  float sum = 0.f;
-  for (int w = first + g; w <= last; w += G) {
-    const float mx = stats[slot(w) * 2], by = mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - top);
-    sum += stats[slot(w) * 2 + 1] * by;
-    if (dim < p.d) f += *reinterpret_cast<const f32x4*>(p.part + slot(w) * p.d + dim) * by;
+  for (int i = g; i < parts; i += 4 * G) {              // four on their way at a time
+    f32x4 x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const f32x4*>(p.part + slot(i + k * G < parts ? i + k * G : i) * p.d + at);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (i + k * G < parts) f += x[k] * weight[i + k * G];
   }
   outs[g][tid - g * DL] = f;
-  sums[tid] = sum;
   __syncthreads();
   if (g > 0 || dim >= p.d) return;
-  for (int i = 1; i < G; ++i) {
-    f += outs[i][tid];
-    sum += sums[i * DL + tid];
-  }
+  for (int i = 1; i < G; ++i) f += outs[i][tid];
+  sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < JT / 64; ++i) sum += sums[i];
   const float scale = CODES && p.v_scale ? p.v_scale[head] : 1.f;
   T* to = reinterpret_cast<T*>(p.o) + (long)u.x * p.ldo + ((long)head * p.group + q0 + qi) * p.d + dim;
 #pragma unroll
@@ -481,7 +522,7 @@ struct Plan { long workgroups; bool parts; };
 
 Plan plan_of(int64_t rows, int64_t kv_heads, int64_t group, int64_t d, int64_t span) {
   const long tiles = (span + TILE - 1) / TILE, units = rows * kv_heads * ((group + QB - 1) / QB);
-  const long at_once = 256 * (d > 128 ? 1 : 3);
+  const long at_once = 256 * (d > 128 ? 1 : d > 64 ? 3 : 4);
   return Plan{units * tiles < at_once ? units * tiles : at_once, tiles > 1};
 }
 
@@ -501,12 +542,13 @@ int run(const PagedParams& p, const Plan& plan, hipStream_t s) {
   if (plan.parts && plan.workgroups > 1) {
     const hipError_t e = hipGetLastError();             // (the launch behind it reads what it writes)
     if (e != hipSuccess) return (int)e;
-    kh_launch(KH_TAG_PAGED_JOIN, join<D, T, CODES>, dim3((unsigned)plan.workgroups - 1, (unsigned)(p.group < QB ? p.group : QB)), dim3(256), 0, s, p, (int)plan.workgroups);
+    kh_launch(KH_TAG_PAGED_JOIN, join<D, T, CODES>, dim3((unsigned)plan.workgroups - 1, (unsigned)(p.group < QB ? p.group : QB)), dim3(JT), 0, s, p, (int)plan.workgroups);
   }
   KH_RETURN_LAST_ERROR();
 }
 template <int D, typename T, bool CODES>
 int run(const PagedParams& p, const Plan& plan, hipStream_t s) {
+  if (p.page % 8 == 0) return p.d == D ? run<D, T, CODES, true, false>(p, plan, s) : run<D, T, CODES, true, true>(p, plan, s);
   return p.d == D ? run<D, T, CODES, false, false>(p, plan, s) : run<D, T, CODES, false, true>(p, plan, s);
 }
 template <typename T, bool CODES>
@@ -538,7 +580,8 @@ KH_EXPORT int kh_paged_attention(const void* q, void* o, const KhPagedCache* cac
   const Plan plan = plan_of(rows, c.kv_heads, group, c.d, c.width * c.page);
   PagedParams p{q, (const char*)c.k + layer * c.k_layer * e, (const char*)c.v + layer * c.v_layer * e, o, c.table, lengths, c.lengths, slots,
                 c.k_scale ? c.k_scale + layer * c.kv_heads : nullptr, c.v_scale ? c.v_scale + layer * c.kv_heads : nullptr,
-                (float*)((char*)workspace + plan.workgroups * 16), (int4*)workspace, ldq, ldo, c.k_page, c.k_token, c.k_head, c.v_page, c.v_token, c.v_head,
+                (float*)((char*)workspace + plan.workgroups * 16), (int4*)workspace, ldq, ldo, (uint32_t)(c.k_page * e), (uint32_t)(c.k_token * e), (uint32_t)(c.v_page * e),
+                (uint32_t)(c.v_token * e), c.k_head * e, c.v_head * e,
                 (int)rows, (int)c.kv_heads, (int)group, (int)((group + QB - 1) / QB), (int)c.d, (int)c.slots, (int)c.width, (int)c.pages, (int)c.page,
                 (int)(window < (1L << 30) ? window : 0), scale * 1.4426950408889634f, flags & 1, 0, KhDivide((uint32_t)c.page)};
   p.q_aligned = kh_aligned16(q) && ldq % 8 == 0;

@@ -18,7 +18,7 @@ static inline int kh_cache_check(const KhPagedCache* c) {
   if (((uintptr_t)c->k | (uintptr_t)c->v) & mask) return KH_ERR_ALIGNMENT;
   if (((uintptr_t)c->table | (uintptr_t)c->lengths | (uintptr_t)c->refs | (uintptr_t)c->k_scale | (uintptr_t)c->v_scale) & 3) return KH_ERR_ALIGNMENT;
   if (c->pages > (1L << 30) || c->slots > (1L << 20) || c->layers > (1L << 16) || c->kv_heads > (1L << 16) || c->page > (1L << 20) ||
-      c->width > (1L << 30) / c->page || c->slots * c->width > (1L << 30))
+      c->width > (1L << 30) / c->page || c->slots * c->width > (1L << 30) || c->k_page >= (1L << 31) || c->k_token >= (1L << 31) || c->v_page >= (1L << 31) || c->v_token >= (1L << 31))
     return KH_ERR_TOO_LARGE;
   return KH_OK;
 }
