@@ -38,6 +38,7 @@ struct PagedParams {
   KhDivide by_page;
 };
 
+typedef uint32_t u32x1 __attribute__((ext_vector_type(1)));
 typedef _Float16 f16_t;
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -115,22 +116,30 @@ template <> struct Pieces<f16_t> {
   }
 };
 
-// A row's sequence: its pages and the tokens low .. n - 1 to attend to; tiles of 128 from `tile` on.
-struct Row { const int32_t* pages; int n, low, tile, tiles; bool there; };
+// a value that all lanes have, in scalar registers
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ long uniform(long v) { return (long)((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32 | (uint32_t)uniform((int)v)); }
 
-__device__ __forceinline__ Row row_of(const PagedParams& p, int r) {
-  Row w{p.table, 0, 0, 0, 0, false};
-  const int s = p.slots ? p.slots[r] : r;
-  if (s < 0 || s >= p.n_slots) return w;
-  w.there = true;
-  w.pages = p.table + (long)s * p.width;
-  const int n = p.row_lengths ? p.row_lengths[r] : p.lengths[s], most = p.width * p.page;
-  w.n = n < 0 ? 0 : n < most ? n : most;
-  w.low = p.window > 0 && w.n > p.window ? w.n - p.window : 0;
-  w.tile = w.low / TILE;
-  w.tiles = (w.n + TILE - 1) / TILE - w.tile;
-  return w;
+// A row's sequence: its slot (-1: none), the tokens low .. n - 1 to attend to; `tiles` tiles of 128 from `tile` on.
+struct Row { int slot, n, low, tile, tiles; };
+
+__device__ __forceinline__ Row row_of(const PagedParams& p, int slot, int n) {
+  const int low = p.window > 0 && n > p.window ? n - p.window : 0, tile = low / TILE;
+  return Row{slot, n, low, tile, (n + TILE - 1) / TILE - tile};
 }
+__device__ __forceinline__ Row row_of(const PagedParams& p, int r) {
+  const int s = p.slots ? p.slots[r] : r;
+  if (s < 0 || s >= p.n_slots) return row_of(p, -1, 0);
+  const int n = p.row_lengths ? p.row_lengths[r] : p.lengths[s], most = p.width * p.page;
+  return row_of(p, s, n < 0 ? 0 : n < most ? n : most);
+}
+
+// What a workgroup does of a unit (a row, a key head and up to 16 of its query heads): the unit in the line of tiles and the part at .. stop - 1 of it.
+struct Piece {
+  Row row;
+  int r, unit, head, q0, queries;
+  int row_at, a, b, at, stop;
+};
 
 // Shapes.  D: dimensions there is room for (d of them used: TAIL where fewer); CODES: the cache holds e4m3; EIGHT: pages of a multiple of eight tokens, so that
 // the eight tokens of a lane lie on one page.
@@ -143,6 +152,7 @@ struct Shape {
   static constexpr int VE = D >= 128 ? 8 : 4;           // elements of one
   static constexpr int ELT = CODES ? 1 : 2;
   static constexpr int VW = VE * ELT / 4;               // words of one
+  using Piece = typename std::conditional<VW == 4, u32x4, typename std::conditional<VW == 2, u32x2, u32x1>::type>::type;
 };
 
 // A wave's part of a unit.  Keys and values of a step are requested as soon as the registers of the step before are free (keys behind its scores, values behind
@@ -156,8 +166,10 @@ struct Wave {
   X q[S::KK];
   f32x4 o[S::NC * S::VE];                               // tile c * VE + j: dimensions c * 128 + VE * (4 * (l / 16) + r) + j of query l % 16
   float m, l;
+  Pages now, next;
+  int t0, steps;
   typename S::Raw kr[2][S::KK];
-  uint32_t vr[8][S::NC][S::VW];
+  typename S::Piece vr[8][S::NC];
 
   // Tokens of lane l: of the keys 8 * (l % 16 / 4) + 4 s + l % 4, of the values (and of the scores it gets) 8 * (l / 16) + i.  One behind the end is
   // looked for at the last one.
@@ -168,16 +180,18 @@ struct Wave {
   __device__ __forceinline__ Pages pages_of(const PagedParams& p, const Row& row, int t0) const {
     Pages e;
     const int last = EIGHT ? (row.n - 1) & ~7 : row.n - 1;
+    const int32_t* pages = p.table + (long)row.slot * p.width;
 #pragma unroll
-    for (int s = 0; s < (EIGHT ? 1 : 2); ++s) e.k[s] = row.pages[p.by_page((uint32_t)kept(EIGHT ? key(t0, 0) & ~7 : key(t0, s), last))];
+    for (int s = 0; s < (EIGHT ? 1 : 2); ++s) e.k[s] = pages[p.by_page((uint32_t)kept(EIGHT ? key(t0, 0) & ~7 : key(t0, s), last))];
 #pragma unroll
-    for (int i = 0; i < (EIGHT ? 1 : 8); ++i) e.v[i] = row.pages[p.by_page((uint32_t)kept(value(t0, i), last))];
+    for (int i = 0; i < (EIGHT ? 1 : 8); ++i) e.v[i] = pages[p.by_page((uint32_t)kept(value(t0, i), last))];
     return e;
   }
   // where a token's row lies; without a page: the first of all
   static __device__ __forceinline__ const char* place(const PagedParams& p, const char* base, int e, int t, uint32_t page, uint32_t token) {
+    const bool there = (uint32_t)e < (uint32_t)p.pages;
     const uint32_t at = (uint32_t)t - p.by_page((uint32_t)t) * (uint32_t)p.page;
-    return (uint32_t)e < (uint32_t)p.pages ? base + (uint64_t)(uint32_t)e * page + (uint64_t)at * token : base;
+    return base + (uint64_t)(there ? (uint32_t)e : 0u) * page + (uint64_t)(there ? at : 0u) * token;
   }
   __device__ __forceinline__ void load_keys(const PagedParams& p, const Row& row, const char* kb, const Pages& e, int t0) {
     const int g4 = (threadIdx.x & 63) >> 4, last = EIGHT ? (row.n - 1) | 7 : row.n - 1;     // (a page of whole eights has the tokens up to there)
@@ -191,7 +205,7 @@ struct Wave {
       for (int kk = 0; kk < S::KK; ++kk) {
         const int dim = kk * 32 + g4 * 8;
         if (TAIL && kk * 32 >= p.d) kr[s][kk] = typename S::Raw{};
-        else kr[s][kk] = *reinterpret_cast<const typename S::Raw*>(at[s] + (!TAIL || dim < p.d ? dim : 0) * S::ELT);
+        else kr[s][kk] = __builtin_nontemporal_load(reinterpret_cast<const typename S::Raw*>(at[s] + (!TAIL || dim < p.d ? dim : 0) * S::ELT));
       }
   }
   __device__ __forceinline__ void load_values(const PagedParams& p, const Row& row, const char* vb, const Pages& e, int t0) {
@@ -203,106 +217,136 @@ struct Wave {
 #pragma unroll
       for (int c = 0; c < S::NC; ++c) {
         const int dim = c * 128 + c16 * S::VE;
-        __builtin_memcpy(vr[i][c], __builtin_assume_aligned(at + (!TAIL || dim < p.d ? dim : 0) * S::ELT, S::VE * S::ELT), S::VE * S::ELT);
+        vr[i][c] = __builtin_nontemporal_load(reinterpret_cast<const typename S::Piece*>(at + (!TAIL || dim < p.d ? dim : 0) * S::ELT));
       }
     }
   }
 
-  // Tokens t0, t0 + TILE, .. of the row, `steps` times 32, of which low .. n - 1 count (steps 0: none).
-  __device__ __forceinline__ void run(const PagedParams& p, const Row& row, int head, int t0, int steps, float factor) {
+  // Requests the first step of a piece (and its queries): the tokens t0, t0 + TILE, .. of its row, `steps` times 32, of which low .. n - 1 count.
+  __device__ __forceinline__ void begin(const PagedParams& p, const Piece& u, int wave) {
+    const int c16 = threadIdx.x & 15, g4 = (threadIdx.x & 63) >> 4;
+    t0 = (u.row.tile + u.at - u.a) * TILE + wave * STEP;
+    steps = u.stop - u.at;
+    if (t0 + (steps - 1) * TILE >= u.row.n) --steps;     // (only the last tile may begin behind the end for some waves,
+    if (t0 + STEP <= u.row.low) t0 += TILE, --steps;     //  only the first end before the window)
+    if (steps > 0) {
+      now = pages_of(p, u.row, t0);
+      next = pages_of(p, u.row, t0 + (steps > 1 ? TILE : 0));
+    }
+    const T* qp = reinterpret_cast<const T*>(p.q) + (long)u.r * p.ldq + ((long)u.head * p.group + u.q0 + (c16 < u.queries ? c16 : 0)) * p.d;
+#pragma unroll
+    for (int kk = 0; kk < S::KK; ++kk) {
+      const int dim = kk * 32 + g4 * 8;
+      T e[8] = {};
+      if (c16 < u.queries && (!TAIL || dim < p.d)) {
+        if (p.q_aligned) __builtin_memcpy(e, __builtin_assume_aligned(qp + dim, 16), 16);
+        else
+#pragma unroll
+          for (int i = 0; i < 8; ++i) e[i] = qp[dim + i];
+      }
+      __builtin_memcpy(&q[kk], e, 16);
+    }
+    if (steps > 0) {
+      load_keys(p, u.row, reinterpret_cast<const char*>(p.k) + u.head * p.k_head, now, t0);
+      load_values(p, u.row, reinterpret_cast<const char*>(p.v) + u.head * p.v_head, now, t0);
+    }
+  }
+  __device__ __forceinline__ void run(const PagedParams& p, const Piece& u) {
 #pragma unroll
     for (int i = 0; i < S::NC * S::VE; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     m = -INFINITY;
     l = 0.f;
     if (steps <= 0) return;
-    const char* kb = reinterpret_cast<const char*>(p.k) + head * p.k_head;
-    const char* vb = reinterpret_cast<const char*>(p.v) + head * p.v_head;
-    Pages now = pages_of(p, row, t0);
-    load_keys(p, row, kb, now, t0);
-    load_values(p, row, vb, now, t0);
-    Pages next = pages_of(p, row, t0 + (steps > 1 ? TILE : 0));
-    for (int n = 1;; ++n) {
-      const bool more = n < steps;
-      // scores: x[4 s + r] is token 8 * (l / 16) + 4 s + r of query l % 16
-      float x[8];
-      const int g4 = (threadIdx.x & 63) >> 4;
+    const Row& row = u.row;
+    const char* kb = reinterpret_cast<const char*>(p.k) + u.head * p.k_head;
+    const char* vb = reinterpret_cast<const char*>(p.v) + u.head * p.v_head;
+    const float factor = p.scale_log2 * (CODES && p.k_scale ? p.k_scale[u.head] : 1.f);
+    for (int n = 1; n < steps; ++n) step<true>(p, row, kb, vb, factor, n + 1 < steps);
+    step<false>(p, row, kb, vb, factor, false);
+  }
+  // MORE: another step follows, on the pages `next`; `after`: and one behind that.
+  template <bool MORE>
+  __device__ __forceinline__ void step(const PagedParams& p, const Row& row, const char* kb, const char* vb, float factor, bool after) {
+    // scores: x[4 s + r] is token 8 * (l / 16) + 4 s + r of query l % 16
+    float x[8];
+    const int g4 = (threadIdx.x & 63) >> 4;
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        f32x4 acc{0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < 2; ++s) {
+      f32x4 acc{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int kk = 0; kk < S::KK; ++kk) {
-          typename S::Raw w = kr[s][kk];
-          if (TAIL && kk * 32 + g4 * 8 >= p.d) w = typename S::Raw{};
-          X a;
-          if constexpr (CODES) a = __builtin_bit_cast(X, u32x4{two_of_e4m3<T, false>(w[0]), two_of_e4m3<T, true>(w[0]), two_of_e4m3<T, false>(w[1]), two_of_e4m3<T, true>(w[1])});
-          else a = __builtin_bit_cast(X, w);
-          acc = mfma(a, q[kk], acc);
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) x[4 * s + r] = acc[r] * factor;
+      for (int kk = 0; kk < S::KK; ++kk) {
+        typename S::Raw w = kr[s][kk];
+        if (TAIL && kk * 32 + g4 * 8 >= p.d) w = typename S::Raw{};
+        X a;
+        if constexpr (CODES) a = __builtin_bit_cast(X, u32x4{two_of_e4m3<T, false>(w[0]), two_of_e4m3<T, true>(w[0]), two_of_e4m3<T, false>(w[1]), two_of_e4m3<T, true>(w[1])});
+        else a = __builtin_bit_cast(X, w);
+        acc = mfma(a, q[kk], acc);
       }
-      if (more) load_keys(p, row, kb, next, t0 + TILE);
-      // what does not count may be anything: scores and values of tokens outside, or without a page
-      const int first = value(t0, 0);
-      bool good[8], whole = true;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[4 * s + r] = acc[r] * factor;
+    }
+    if constexpr (MORE) load_keys(p, row, kb, next, t0 + TILE);
+    // what does not count may be anything: scores and values of tokens outside, or without a page
+    const int first = value(t0, 0);
+    bool good[8], whole = true;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      good[i] = (uint32_t)now.v[EIGHT ? 0 : i] < (uint32_t)p.pages && first + i >= row.low && first + i < row.n;
+      whole = whole && good[i];
+    }
+    if (__any(!whole)) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        good[i] = (uint32_t)now.v[EIGHT ? 0 : i] < (uint32_t)p.pages && first + i >= row.low && first + i < row.n;
-        whole = whole && good[i];
+        x[i] = good[i] ? x[i] : -INFINITY;
+#pragma unroll
+        for (int c = 0; c < S::NC; ++c)
+#pragma unroll
+          for (int w = 0; w < S::VW; ++w) vr[i][c][w] = good[i] ? vr[i][c][w] : 0;
       }
-      if (__any(!whole)) {
+    }
+    float top = x[0];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          x[i] = good[i] ? x[i] : -INFINITY;
+    for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);
+    top = swapped_max(top);
+    if (__any(top > m + RESCALE_LOG2)) {
+      const float to = fmaxf(m, top), by = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - to);
+      m = to;
+      l *= by;
 #pragma unroll
-          for (int c = 0; c < S::NC; ++c)
+      for (int i = 0; i < S::NC * S::VE; ++i) o[i] *= by;
+    }
+    const float from = m == -INFINITY ? 0.f : m;
+    float pr[8];
 #pragma unroll
-            for (int w = 0; w < S::VW; ++w) vr[i][c][w] = good[i] ? vr[i][c][w] : 0;
-        }
-      }
-      float top = x[0];
+    for (int i = 0; i < 8; ++i) {
+      pr[i] = __builtin_amdgcn_exp2f(x[i] - from);
+      l += pr[i];
+    }
+    X pieces[Pieces<T>::N];
+    Pieces<T>::of(pr, pieces);
 #pragma unroll
-      for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);
-      top = swapped_max(top);
-      if (__any(top > m + RESCALE_LOG2)) {
-        const float to = fmaxf(m, top), by = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - to);
-        m = to;
-        l *= by;
+    for (int c = 0; c < S::NC; ++c)
 #pragma unroll
-        for (int i = 0; i < S::NC * S::VE; ++i) o[i] *= by;
-      }
-      const float from = m == -INFINITY ? 0.f : m;
-      float pr[8];
+      for (int j = 0; j < S::VE; ++j) {
+        u32x4 a;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        pr[i] = __builtin_amdgcn_exp2f(x[i] - from);
-        l += pr[i];
-      }
-      X pieces[Pieces<T>::N];
-      Pieces<T>::of(pr, pieces);
-#pragma unroll
-      for (int c = 0; c < S::NC; ++c)
-#pragma unroll
-        for (int j = 0; j < S::VE; ++j) {
-          u32x4 a;
-#pragma unroll
-          for (int h = 0; h < 4; ++h) {                 // tokens 2 h, 2 h + 1
-            if constexpr (CODES) {
-              const uint32_t both = __builtin_amdgcn_perm(vr[2 * h + 1][c][j / 4], vr[2 * h][c][j / 4], 0x0400u + (j % 4) * 0x0101u);
-              a[h] = two_of_e4m3<T, false>(both);
-            } else {
-              a[h] = __builtin_amdgcn_perm(vr[2 * h + 1][c][j / 2], vr[2 * h][c][j / 2], j & 1 ? 0x07060302 : 0x05040100);
-            }
+        for (int h = 0; h < 4; ++h) {                 // tokens 2 h, 2 h + 1
+          if constexpr (CODES) {
+            const uint32_t both = __builtin_amdgcn_perm(vr[2 * h + 1][c][j / 4], vr[2 * h][c][j / 4], 0x0400u + (j % 4) * 0x0101u);
+            a[h] = two_of_e4m3<T, false>(both);
+          } else {
+            a[h] = __builtin_amdgcn_perm(vr[2 * h + 1][c][j / 2], vr[2 * h][c][j / 2], j & 1 ? 0x07060302 : 0x05040100);
           }
-          const X value8 = __builtin_bit_cast(X, a);
-#pragma unroll
-          for (int n2 = 0; n2 < Pieces<T>::N; ++n2) o[c * S::VE + j] = mfma(value8, pieces[n2], o[c * S::VE + j]);
         }
-      if (!more) break;
+        const X value8 = __builtin_bit_cast(X, a);
+#pragma unroll
+        for (int n2 = 0; n2 < Pieces<T>::N; ++n2) o[c * S::VE + j] = mfma(value8, pieces[n2], o[c * S::VE + j]);
+      }
+    if constexpr (MORE) {
       t0 += TILE;
-      load_values(p, row, vb, next, t0);
       now = next;
-      next = pages_of(p, row, t0 + (n + 1 < steps ? TILE : 0));
+      next = pages_of(p, row, t0 + (after ? TILE : 0));         // (before the values: its use does not wait for those)
+      load_values(p, row, vb, now, t0);
     }
   }
 };
@@ -314,88 +358,83 @@ __device__ __forceinline__ void zero_row(const PagedParams& p, int r) {
 }
 
 template <int D, typename T, bool CODES, bool EIGHT, bool TAIL>
-__global__ __launch_bounds__(NW * 64, D > 128 ? 1 : D > 64 ? 3 : 4) void attend(const PagedParams p) {
+__global__ __launch_bounds__(NW * 64, D > 128 ? 1 : D > 64 ? 2 : 3) void attend(const PagedParams p) {
   using S = Shape<D, T, CODES, EIGHT, TAIL>;
   constexpr int OW = D + 4;                             // floats of a query's row in LDS
   extern __shared__ float lds[];                        // [NW][QB][OW] outputs, [2][NW][QB] maxima and sums
   float* const ms = lds + NW * QB * OW;
-  __shared__ long starts[NW];
-  __shared__ int where[2];
+  __shared__ int starts[NW];
+  __shared__ int where[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c16 = lane & 15, g4 = lane >> 4;
   const int units = p.kv_heads * p.blocks, G = gridDim.x, w = blockIdx.x;
 
-  // rows of this workgroup that have nothing to attend to, or no slot
-  for (int r = w; r < p.rows; r += G) {
-    const Row row = row_of(p, r);
-    if (row.tiles <= 0 && (row.there || p.fill)) zero_row<T>(p, r);
-  }
-
   // the line of tiles: all of them, and the row in which this workgroup's part begins
   const int each = (p.rows + NW * 64 - 1) / (NW * 64), r0 = tid * each, r1 = r0 + each < p.rows ? r0 + each : p.rows;
-  long mine = 0;
-  for (int r = r0; r < r1; ++r) mine += row_of(p, r).tiles;
-  long before = mine;
+  Row one{};
+  int mine = 0;
+  for (int r = r0; r < r1; ++r) mine += (one = row_of(p, r)).tiles;
+  int before = mine;
 #pragma unroll
   for (int s = 1; s < 64; s <<= 1) {
-    const long y = __shfl_up(before, s, 64);
+    const int y = __shfl_up(before, s, 64);
     if (lane >= s) before += y;
   }
   if (lane == 63) starts[wave] = before;
   __syncthreads();
-  long total = 0;
+  int total = 0;
   before -= mine;
 #pragma unroll
   for (int i = 0; i < NW; ++i) {
     if (i < wave) before += starts[i];
     total += starts[i];
   }
-  total *= units;
-  before *= units;
-  const long W = total < G ? total : G;                 // workgroups that have a tile
+  total = uniform(total) * units;
+  const int W = total < G ? total : G;                  // workgroups that have a tile
   if (tid == 0) p.border[w] = int4{-1, 0, 0, 0};
-  if (w >= W) return;
-  const long begin = total * w / W, end = total * (w + 1) / W;
-  long at_row = before;                                 // where row r begins
-  for (int r = r0; r < r1; ++r) {
-    const long next = at_row + (long)row_of(p, r).tiles * units;
-    if (begin >= at_row && begin < next) {
-      where[0] = r;
-      where[1] = (int)(begin - at_row);
-    }
-    at_row = next;
-  }
-  __syncthreads();
-  int r = where[0];
-  long at = begin, row_at = begin - where[1];
-
-  Wave<D, T, CODES, EIGHT, TAIL> wv;
-  for (; at < end; ++r) {
-    const Row row = row_of(p, r);
-    const long row_end = row_at + (long)row.tiles * units;
-    while (at < end && at < row_end) {
-      const int unit = (int)((at - row_at) / row.tiles), head = unit / p.blocks, block = unit - head * p.blocks;
-      const long a = row_at + (long)unit * row.tiles, b = a + row.tiles;        // the unit in the line
-      const long stop = b < end ? b : end;
-      const int q0 = block * QB, queries = p.group - q0 < QB ? p.group - q0 : QB;
-      // queries as the scores' second operand
-      const T* qp = reinterpret_cast<const T*>(p.q) + (long)r * p.ldq + ((long)head * p.group + q0 + (c16 < queries ? c16 : 0)) * p.d;
-#pragma unroll
-      for (int kk = 0; kk < S::KK; ++kk) {
-        const int dim = kk * 32 + g4 * 8;
-        T e[8] = {};
-        if (c16 < queries && (!TAIL || dim < p.d)) {
-          if (p.q_aligned) __builtin_memcpy(e, __builtin_assume_aligned(qp + dim, 16), 16);
-          else
-#pragma unroll
-            for (int i = 0; i < 8; ++i) e[i] = qp[dim + i];
-        }
-        __builtin_memcpy(&wv.q[kk], e, 16);
+  if (w < W) {
+    const int begin = (int)((long)total * w / W), end = (int)((long)total * (w + 1) / W);
+    int at_row = before * units;                        // where row r begins
+    for (int r = r0; r < r1; ++r) {
+      if (each > 1) one = row_of(p, r);
+      const int next = at_row + one.tiles * units;
+      if (begin >= at_row && begin < next) {
+        where[0] = r;
+        where[1] = at_row;
+        where[2] = one.slot;
+        where[3] = one.n;
       }
-      const float factor = p.scale_log2 * (CODES && p.k_scale ? p.k_scale[head] : 1.f);
-      int t0 = (row.tile + (int)(at - a)) * TILE + wave * STEP, steps = (int)(stop - at);
-      if (t0 + (steps - 1) * TILE >= row.n) --steps;     // (only the last tile may begin behind the end for some waves,
-      if (t0 + STEP <= row.low) t0 += TILE, --steps;     //  only the first end before the window)
-      wv.run(p, row, head, t0, steps, factor);
+      at_row = next;
+    }
+    __syncthreads();
+    // the piece from `at` on in the line; false: none
+    auto advance = [&](Piece& u, int at) {
+      if (at >= end) return false;
+      while (at >= u.row_at + u.row.tiles * units) {
+        u.row_at += u.row.tiles * units;
+        u.row = row_of(p, ++u.r);
+      }
+      u.unit = (at - u.row_at) / u.row.tiles;
+      u.head = u.unit / p.blocks;
+      u.q0 = (u.unit - u.head * p.blocks) * QB;
+      u.queries = p.group - u.q0 < QB ? p.group - u.q0 : QB;
+      u.a = u.row_at + u.unit * u.row.tiles;
+      u.b = u.a + u.row.tiles;
+      u.at = at;
+      u.stop = u.b < end ? u.b : end;
+      return true;
+    };
+    Piece u;
+    u.r = uniform(where[0]);
+    u.row_at = uniform(where[1]);
+    u.row = row_of(p, uniform(where[2]), uniform(where[3]));
+    Wave<D, T, CODES, EIGHT, TAIL> wv;
+    bool more = advance(u, begin);
+    wv.begin(p, u, wave);
+    while (more) {
+      wv.run(p, u);
+      const Piece done = u;
+      more = advance(u, done.stop);
+      if (more) wv.begin(p, u, wave);                   // (on its way while the waves' parts are put together)
       // the waves' parts together
       float sum = wv.l;
       sum += __shfl_xor(sum, 16, 64);
@@ -421,10 +460,10 @@ __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : D > 64 ? 3 : 4) void attend(
             *reinterpret_cast<f32x4*>(lds + (wave * QB + c16) * OW + c * 128 + S::VE * (4 * g4 + n) + j) = f;
           }
       __syncthreads();
-      const bool complete = a >= begin && b <= end;
-      const long slot = 2 * (long)w + (a >= begin ? 1 : 0);
+      const bool complete = done.a >= begin && done.b <= end;
+      const long slot = 2 * (long)w + (done.a >= begin ? 1 : 0);
       const int q_max = p.group < QB ? p.group : QB;
-      for (int i = tid; i < queries * (D / 4); i += NW * 64) {
+      for (int i = tid; i < done.queries * (D / 4); i += NW * 64) {
         const int qi = i / (D / 4), dim = (i - qi * (D / 4)) * 4;
         if (TAIL && dim >= p.d) continue;
         f32x4 f{0.f, 0.f, 0.f, 0.f};
@@ -440,8 +479,8 @@ __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : D > 64 ? 3 : 4) void attend(
           sum_q += ms[(NW + x) * QB + qi] * (mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - top_q));
         }
         if (complete) {
-          const float scale = CODES && p.v_scale ? p.v_scale[head] : 1.f;
-          T* to = reinterpret_cast<T*>(p.o) + (long)r * p.ldo + ((long)head * p.group + q0 + qi) * p.d + dim;
+          const float scale = CODES && p.v_scale ? p.v_scale[done.head] : 1.f;
+          T* to = reinterpret_cast<T*>(p.o) + (long)done.r * p.ldo + ((long)done.head * p.group + done.q0 + qi) * p.d + dim;
 #pragma unroll
           for (int e = 0; e < 4; ++e) to[e] = (T)(sum_q == 0.f ? 0.f : f[e] / sum_q * scale);
         } else {
@@ -454,12 +493,15 @@ __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : D > 64 ? 3 : 4) void attend(
         }
       }
       // where this workgroup begins in a unit that the one before it began: the unit's row, number and workgroups
-      if (tid == 0 && a < begin && total * (w - 1) / W <= a)
-        p.border[w] = int4{r, unit, w - 1, (int)((b * W - 1) / total)};
+      if (tid == 0 && done.a < begin && (long)total * (w - 1) / W <= done.a)
+        p.border[w] = int4{done.r, done.unit, w - 1, (int)(((long)done.b * W - 1) / total)};
       __syncthreads();                                  // (LDS is read)
-      at = stop;
     }
-    row_at = row_end;
+  }
+  // rows that have nothing to attend to, or no slot
+  for (int r = w; r < p.rows; r += G) {
+    const Row row = row_of(p, r);
+    if (row.tiles <= 0 && (row.slot >= 0 || p.fill)) zero_row<T>(p, r);
   }
 }
 
@@ -522,8 +564,13 @@ struct Plan { long workgroups; bool parts; };
 
 Plan plan_of(int64_t rows, int64_t kv_heads, int64_t group, int64_t d, int64_t span) {
   const long tiles = (span + TILE - 1) / TILE, units = rows * kv_heads * ((group + QB - 1) / QB);
-  const long at_once = 256 * (d > 128 ? 1 : d > 64 ? 3 : 4);
+  const long at_once = 256 * (d > 128 ? 1 : d > 64 ? 2 : 3);
   return Plan{units * tiles < at_once ? units * tiles : at_once, tiles > 1};
+}
+
+// whether all tiles can be counted in 31 bits
+bool line_fits(int64_t rows, int64_t kv_heads, int64_t group, int64_t span) {
+  return rows * kv_heads * ((group + QB - 1) / QB) <= (1L << 30) / ((span + TILE - 1) / TILE);
 }
 
 int64_t bytes_of(const Plan& plan, int64_t group, int64_t d) {
@@ -562,6 +609,7 @@ KH_EXPORT int64_t kh_paged_attention_workspace_bytes(int64_t rows, int64_t heads
   if (rows <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || d <= 0 || span <= 0) return KH_ERR_INVALID_ARG;
   if (d % 8 != 0 || d > 256) return KH_ERR_UNSUPPORTED;
   if (rows > (1L << 24) || heads > (1L << 16) || span > (1L << 30)) return KH_ERR_TOO_LARGE;
+  if (!line_fits(rows, kv_heads, heads / kv_heads, span)) return KH_ERR_TOO_LARGE;
   return bytes_of(plan_of(rows, kv_heads, heads / kv_heads, d, span), heads / kv_heads, d);
 }
 
@@ -577,6 +625,7 @@ KH_EXPORT int kh_paged_attention(const void* q, void* o, const KhPagedCache* cac
   if ((((uintptr_t)q | (uintptr_t)o) & 1) || (((uintptr_t)slots | (uintptr_t)lengths) & 3) || !kh_aligned16(workspace)) return KH_ERR_ALIGNMENT;
   if (rows > (1L << 24) || heads > (1L << 16)) return KH_ERR_TOO_LARGE;
   const long group = heads / c.kv_heads, e = kh_cache_element(c);
+  if (!line_fits(rows, c.kv_heads, group, c.width * c.page)) return KH_ERR_TOO_LARGE;
   const Plan plan = plan_of(rows, c.kv_heads, group, c.d, c.width * c.page);
   PagedParams p{q, (const char*)c.k + layer * c.k_layer * e, (const char*)c.v + layer * c.v_layer * e, o, c.table, lengths, c.lengths, slots,
                 c.k_scale ? c.k_scale + layer * c.kv_heads : nullptr, c.v_scale ? c.v_scale + layer * c.kv_heads : nullptr,
