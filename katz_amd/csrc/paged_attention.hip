@@ -351,6 +351,14 @@ struct Wave {
   }
 };
 
+template <typename T, int N>
+__device__ __forceinline__ void store_row(const PagedParams& p, int row, int query, int dim, const float (&f)[N], float sum, float scale) {
+  T v[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) v[e] = (T)(sum == 0.f ? 0.f : f[e] / sum * scale);
+  __builtin_memcpy(reinterpret_cast<T*>(p.o) + (long)row * p.ldo + (long)query * p.d + dim, v, sizeof(v));
+}
+
 template <typename T>
 __device__ __forceinline__ void zero_row(const PagedParams& p, int r) {
   T* to = reinterpret_cast<T*>(p.o) + (long)r * p.ldo;
@@ -480,9 +488,8 @@ __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : D > 64 ? 2 : 3) void attend(
         }
         if (complete) {
           const float scale = CODES && p.v_scale ? p.v_scale[done.head] : 1.f;
-          T* to = reinterpret_cast<T*>(p.o) + (long)done.r * p.ldo + ((long)done.head * p.group + done.q0 + qi) * p.d + dim;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) to[e] = (T)(sum_q == 0.f ? 0.f : f[e] / sum_q * scale);
+          const float out[4] = {f[0], f[1], f[2], f[3]};
+          store_row<T>(p, done.r, done.head * p.group + done.q0 + qi, dim, out, sum_q, scale);
         } else {
           *reinterpret_cast<f32x4*>(p.part + (slot * q_max + qi) * p.d + dim) = f;
           if (dim == 0) {
@@ -505,22 +512,98 @@ __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : D > 64 ? 2 : 3) void attend(
   }
 }
 
-// The parts of a unit that several workgroups have, in their order; a workgroup for each border and query head.
+// The parts of a unit that several workgroups have, in their order.  Where a unit has few, a wave joins those of a query head; where it has many, a workgroup those
+// of 32 of its dimensions.
+struct Parts {
+  int row, head, q0, first, count;
+  const float *stats;
+  const PagedParams& p;
+  int q_max;
+  // u: row, unit, first and last workgroup
+  __device__ __forceinline__ Parts(const PagedParams& pp, const int4 u, int G) : p(pp) {
+    row = u.x;
+    head = u.y / p.blocks;
+    q0 = (u.y - head * p.blocks) * QB;
+    first = u.z;
+    count = u.w - u.z + 1;
+    q_max = p.group < QB ? p.group : QB;
+    stats = p.part + 2 * (long)G * q_max * p.d;
+  }
+  __device__ __forceinline__ long slot(int i, int qi) const { return (2 * (long)(first + i) + (i == 0 ? 1 : 0)) * q_max + qi; }
+  __device__ __forceinline__ float2 stat(int i, int qi) const { return *reinterpret_cast<const float2*>(stats + slot(i, qi) * 2); }
+  __device__ __forceinline__ const float* outputs(int i, int qi) const { return p.part + slot(i, qi) * p.d; }
+};
+
 template <int D, typename T, bool CODES>
-__global__ __launch_bounds__(JT) void join(const PagedParams p, const int G_all) {
-  const int4 u = p.border[blockIdx.x + 1];
-  if (u.x < 0) return;
-  const int qi = blockIdx.y, head = u.y / p.blocks, q0 = (u.y - head * p.blocks) * QB, q_max = p.group < QB ? p.group : QB;
-  if (qi >= p.group - q0) return;
-  constexpr int DL = D / 4, G = JT / DL;                // lanes of an output, groups that take parts in turn
+__global__ __launch_bounds__(NW * 64) void join_few(const PagedParams p, const int G) {
+  constexpr int N = D / 64;
+  const Parts u(p, p.border[blockIdx.x + 1], G);
+  const int lane = threadIdx.x & 63, qi = blockIdx.y * NW + (threadIdx.x >> 6);
+  if (u.row < 0 || qi >= u.q_max || qi >= p.group - u.q0) return;
+  const int dim = lane * N, at = dim < p.d ? dim : 0;
+  float f[N] = {}, top = -INFINITY, sum = 0.f;
+  for (int base = 0; base < u.count; base += 64) {      // (a lane a part; the maximum only moves between rounds of 64)
+    const float2 s = base + lane < u.count ? u.stat(base + lane, qi) : float2{-INFINITY, 0.f};
+    float now = s.x;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) now = fmaxf(now, __shfl_xor(now, o, 64));
+    now = fmaxf(now, top);
+    const float old = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top - now), by = s.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(s.x - now);
+    top = now;
+    float more = s.y * by;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) more += __shfl_xor(more, o, 64);
+    sum = sum * old + more;
+#pragma unroll
+    for (int e = 0; e < N; ++e) f[e] *= old;
+    const int n = u.count - base < 64 ? u.count - base : 64;
+    for (int i = 0; i < n; i += 4) {                    // four on their way at a time
+      float x[4][N];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) __builtin_memcpy(x[k], u.outputs(base + (i + k < n ? i + k : i), qi) + at, sizeof(x[k]));
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float w = __shfl(by, i + k < n ? i + k : i, 64);
+        if (i + k < n)
+#pragma unroll
+          for (int e = 0; e < N; ++e) f[e] += x[k][e] * w;
+      }
+    }
+  }
+  if (dim < p.d) store_row<T>(p, u.row, u.head * p.group + u.q0 + qi, dim, f, sum, CODES && p.v_scale ? p.v_scale[u.head] : 1.f);
+}
+
+template <typename T, bool CODES>
+__global__ __launch_bounds__(JT) void join_many(const PagedParams p, const int G) {
+  constexpr int DL = 8, GR = JT / DL;                   // lanes of 32 dimensions, groups that take parts in turn
+  // there are few rows (at most MOST / 16 units): a lane has one's tiles, and with them where this workgroup's unit lies in the line
+  const int units = p.kv_heads * p.blocks, r = blockIdx.x / units, unit = blockIdx.x - r * units, at_lane = threadIdx.x & 63;
+  const int tiles = at_lane < p.rows ? row_of(p, at_lane).tiles : 0;
+  int before = tiles;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(before, o, 64);
+    if (at_lane >= o) before += y;
+  }
+  const int total = __shfl(before, 63, 64) * units, here = __shfl(tiles, r, 64), a = (__shfl(before, r, 64) - here) * units + unit * here, W = total < G ? total : G;
+  if (here == 0) return;
+  const Parts u(p, int4{r, unit, (int)(((long)(a + 1) * W - 1) / total), (int)(((long)(a + here) * W - 1) / total)}, G);
+  const int qi = blockIdx.y;
+  if (u.count < 2 || qi >= p.group - u.q0) return;
   __shared__ float weight[MOST], red[JT / 64], sums[JT / 64];
-  __shared__ f32x4 outs[G][DL];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, first = u.z, parts = u.w - u.z + 1;
-  const float* stats = p.part + 2 * (long)G_all * q_max * p.d;
-  auto slot = [&](int i) { return (2 * (long)(first + i) + (i == 0 ? 1 : 0)) * q_max + qi; };
+  __shared__ f32x4 outs[GR][DL];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, parts = u.count;
+  const int g = tid / DL, dim = blockIdx.z * 32 + (tid - g * DL) * 4, at = dim < p.d ? dim : 0;
+  // (the outputs of the first parts do not wait for the weights)
+  f32x4 x[4];
+  auto request = [&](int i) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const f32x4*>(u.outputs(i + k * GR < parts ? i + k * GR : 0, qi) + at);
+  };
+  request(g);
   // what every part's outputs and sum are multiplied with
   float top = -INFINITY, sum = 0.f;
-  for (int i = tid; i < parts; i += JT) top = fmaxf(top, weight[i] = stats[slot(i) * 2]);
+  for (int i = tid; i < parts; i += JT) top = fmaxf(top, weight[i] = u.stat(i, qi).x);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
   if (lane == 0) red[wave] = top;
@@ -530,42 +613,43 @@ __global__ __launch_bounds__(JT) void join(const PagedParams p, const int G_all)
   for (int i = tid; i < parts; i += JT) {
     const float mx = weight[i], by = mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - top);    // (its own: nobody else reads it before the barrier)
     weight[i] = by;
-    sum += stats[slot(i) * 2 + 1] * by;
+    sum += u.stat(i, qi).y * by;
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
   if (lane == 0) sums[wave] = sum;
   __syncthreads();
-  const int g = tid / DL, dim = (tid - g * DL) * 4, at = dim < p.d ? dim : 0;
   f32x4 f{0.f, 0.f, 0.f, 0.f};
-  for (int i = g; i < parts; i += 4 * G) {              // four on their way at a time
-    f32x4 x[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const f32x4*>(p.part + slot(i + k * G < parts ? i + k * G : i) * p.d + at);
+  for (int i = g; i < parts;) {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      if (i + k * G < parts) f += x[k] * weight[i + k * G];
+      if (i + k * GR < parts) f += x[k] * weight[i + k * GR];
+    i += 4 * GR;
+    if (i < parts) request(i);
   }
   outs[g][tid - g * DL] = f;
   __syncthreads();
+#pragma unroll
+  for (int s = GR / 2; s > 0; s >>= 1) {
+    if (g < s) outs[g][tid - g * DL] += outs[g + s][tid - g * DL];
+    __syncthreads();
+  }
   if (g > 0 || dim >= p.d) return;
-  for (int i = 1; i < G; ++i) f += outs[i][tid];
   sum = 0.f;
 #pragma unroll
   for (int i = 0; i < JT / 64; ++i) sum += sums[i];
-  const float scale = CODES && p.v_scale ? p.v_scale[head] : 1.f;
-  T* to = reinterpret_cast<T*>(p.o) + (long)u.x * p.ldo + ((long)head * p.group + q0 + qi) * p.d + dim;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) to[e] = (T)(sum == 0.f ? 0.f : f[e] / sum * scale);
+  const float out[4] = {outs[0][tid][0], outs[0][tid][1], outs[0][tid][2], outs[0][tid][3]};
+  store_row<T>(p, u.row, u.head * p.group + u.q0 + qi, dim, out, sum, CODES && p.v_scale ? p.v_scale[u.head] : 1.f);
 }
 
 // Workgroups: as many as run at once (D 256: one a CU), but no more than there can be tiles.
-struct Plan { long workgroups; bool parts; };
+// `many`: parts of a unit, about the workgroups by the units, are more than a wave joins in passing.
+struct Plan { long workgroups; bool parts, many; };
 
 Plan plan_of(int64_t rows, int64_t kv_heads, int64_t group, int64_t d, int64_t span) {
   const long tiles = (span + TILE - 1) / TILE, units = rows * kv_heads * ((group + QB - 1) / QB);
   const long at_once = 256 * (d > 128 ? 1 : d > 64 ? 2 : 3);
-  return Plan{units * tiles < at_once ? units * tiles : at_once, tiles > 1};
+  return Plan{units * tiles < at_once ? units * tiles : at_once, tiles > 1, units * 16 < at_once};
 }
 
 // whether all tiles can be counted in 31 bits
@@ -589,7 +673,9 @@ int run(const PagedParams& p, const Plan& plan, hipStream_t s) {
   if (plan.parts && plan.workgroups > 1) {
     const hipError_t e = hipGetLastError();             // (the launch behind it reads what it writes)
     if (e != hipSuccess) return (int)e;
-    kh_launch(KH_TAG_PAGED_JOIN, join<D, T, CODES>, dim3((unsigned)plan.workgroups - 1, (unsigned)(p.group < QB ? p.group : QB)), dim3(JT), 0, s, p, (int)plan.workgroups);
+    const unsigned borders = (unsigned)plan.workgroups - 1, queries = p.group < QB ? p.group : QB;
+    if (plan.many) kh_launch(KH_TAG_PAGED_JOIN, join_many<T, CODES>, dim3((unsigned)(p.rows * p.kv_heads * p.blocks), queries, (unsigned)(p.d + 31) / 32), dim3(JT), 0, s, p, (int)plan.workgroups);
+    else kh_launch(KH_TAG_PAGED_JOIN, join_few<D, T, CODES>, dim3(borders, (queries + NW - 1) / NW), dim3(NW * 64), 0, s, p, (int)plan.workgroups);
   }
   KH_RETURN_LAST_ERROR();
 }
