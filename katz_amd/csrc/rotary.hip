@@ -22,9 +22,11 @@ struct RotaryParams {
   int heads, kv_heads, d, pairs, axes, end[4];
   int position_type, frequency_32, fill, per;   // per: rows of a workgroup
   int cached, n_slots, width, pages, page;
+  int units;                   // of a head
+  KhDivide by_pairs, by_units, by_heads;
 };
 
-constexpr int NT = 256;
+constexpr int NT = 256, MOST_ROWS = 16;   // threads, rows of a workgroup at most
 constexpr double ONE_TURN = 0.15915494309189533577;   // 1 / 2 pi
 
 // Where a row of k and v goes: its page (-1: nowhere), the place in it, and the place in the sequence (-1: the row is left out).
@@ -81,66 +83,85 @@ __device__ __forceinline__ void store_e4m3(uint8_t* to, const float (&f)[N], flo
   else to[0] = (uint8_t)w[0];
 }
 
-// Unit u of a head of d: pair(s) from u * N on while there are any, then elements that are copied.  TURN false: elements only.
-template <typename T, bool E4M3, bool PAIRS, int N, bool TURN>
-__device__ __forceinline__ void unit(const T* from, void* to, const float2* cs, int u, int pairs, float scale) {
+// A piece of work: unit u of a head.  Its elements are N from `first` and N from `second` on, the a and b of N pairs; with pairs in turn (and N > 1), or behind the
+// pairs, only the N from `first` on.
+template <typename T, bool PAIRS, int N>
+struct Unit {
+  const T* from;
+  void* to;
+  int first, second;           // second < 0: none
+  const float2* cs;            // of the first pair; nullptr: copied
+  float scale;                 // of an e4m3 code
+  int what;                    // 0 nothing, 1 to T, 2 to codes, 3 zeros
   float a[N], b[N];
-  const auto put = [&](int at, const float (&f)[N]) {
-    if constexpr (E4M3) store_e4m3(reinterpret_cast<uint8_t*>(to) + at, f, scale);
-    else store(reinterpret_cast<T*>(to) + at, f);
-  };
-  if constexpr (!TURN) {
-    load(from + u * N, a);
-    put(u * N, a);
-  } else if constexpr (!PAIRS || N == 1) {
-    const int turned = pairs / N;
-    if (u < turned) {
-      const int i = PAIRS ? 2 * u : u * N, j = PAIRS ? 2 * u + 1 : u * N + pairs;
-      load(from + i, a);
-      load(from + j, b);
-      float x[N], y[N];
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const float2 z = cs[u * N + e];
-        x[e] = a[e] * z.x - b[e] * z.y;
-        y[e] = b[e] * z.x + a[e] * z.y;
-      }
-      put(i, x);
-      put(j, y);
+
+  __device__ __forceinline__ void at(int u, int pairs, const float2* angles) {
+    second = -1;
+    cs = nullptr;
+    if (PAIRS && N > 1) {
+      first = u * N;
+      if (u * (N / 2) < pairs) cs = angles + u * (N / 2);
+    } else if (u * N < pairs) {
+      first = PAIRS ? 2 * u : u * N;
+      second = PAIRS ? 2 * u + 1 : u * N + pairs;
+      cs = angles + u * N;
     } else {
-      const int i = 2 * pairs + (u - turned) * N;
-      load(from + i, a);
-      put(i, a);
+      first = u * N + pairs;                              // (2 pairs + (u - pairs / N) * N)
     }
-  } else {
-    load(from + u * N, a);
-    if (u * (N / 2) < pairs) {
+  }
+  __device__ __forceinline__ void fetch() {
+    if (what == 0 || what == 3) return;
+    load(from + first, a);
+    if (second >= 0) load(from + second, b);
+  }
+  template <bool E4M3>
+  __device__ __forceinline__ void finish() {
+    if (what == 0) return;
+    if (what == 3) {
 #pragma unroll
-      for (int e = 0; e < N; e += 2) {
-        const float2 z = cs[u * (N / 2) + e / 2];
-        const float x = a[e] * z.x - a[e + 1] * z.y;
-        a[e + 1] = a[e + 1] * z.x + a[e] * z.y;
-        a[e] = x;
+      for (int e = 0; e < N; ++e) a[e] = b[e] = 0.f;
+    } else if (cs) {
+      if constexpr (PAIRS && N > 1) {
+#pragma unroll
+        for (int e = 0; e < N; e += 2) {
+          const float2 z = cs[e / 2];
+          const float x = a[e] * z.x - a[e + 1] * z.y;
+          a[e + 1] = a[e + 1] * z.x + a[e] * z.y;
+          a[e] = x;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const float2 z = cs[e];
+          const float x = a[e] * z.x - b[e] * z.y;
+          b[e] = b[e] * z.x + a[e] * z.y;
+          a[e] = x;
+        }
       }
     }
-    put(u * N, a);
+    if (E4M3 && what == 2) {
+      store_e4m3(reinterpret_cast<uint8_t*>(to) + first, a, scale);
+      if (second >= 0) store_e4m3(reinterpret_cast<uint8_t*>(to) + second, b, scale);
+    } else {
+      store(reinterpret_cast<T*>(to) + first, a);
+      if (second >= 0) store(reinterpret_cast<T*>(to) + second, b);
+    }
   }
-}
+};
 
 // N: elements of a piece, 8 where rows, heads and pairs allow it.
 template <typename T, bool E4M3, bool PAIRS, int N>
 __global__ __launch_bounds__(NT) void rotary_rows(const RotaryParams p) {
   extern __shared__ float2 angles[];                     // [per][pairs]
-  __shared__ Where at[16];
+  __shared__ Where at[MOST_ROWS];
   const int tid = threadIdx.x;
   const long first = (long)blockIdx.x * p.per;
   const int rows = (int)(p.rows - first < p.per ? p.rows - first : p.per);
-  if (p.cached) {
-    if (tid < rows) at[tid] = where(p, first + tid);
-    __syncthreads();
-  }
+  // (the last wave looks the pages up while the others begin with the angles)
+  if (p.cached && tid >= NT - 64 && tid - (NT - 64) < rows) at[tid - (NT - 64)] = where(p, first + tid - (NT - 64));
+  if (!p.positions) __syncthreads();
   for (int i = tid; i < rows * p.pairs; i += NT) {
-    const int r = i / p.pairs, j = i - r * p.pairs;
+    const int r = (int)p.by_pairs((uint32_t)i), j = i - r * p.pairs;
     const int axis = (j >= p.end[0]) + (j >= p.end[1]) + (j >= p.end[2]);
     double t;
     if (!p.positions) t = at[r].place;
@@ -155,48 +176,43 @@ __global__ __launch_bounds__(NT) void rotary_rows(const RotaryParams p) {
     angles[i] = z;
   }
   __syncthreads();
-  // q and k: units of a head, heads of a row, rows
-  {
-    const int units = PAIRS && N == 8 ? p.d / N : p.pairs / N + (p.d - 2 * p.pairs) / N, heads = p.heads + p.kv_heads;
-    for (long i = tid; i < (long)rows * heads * units; i += NT) {
-      const int u = (int)(i % units), hr = (int)(i / units), h = hr % heads, r = hr / heads;
-      const float2* cs = angles + r * p.pairs;
-      if (p.cached && at[r].place < 0) {
-        if (p.fill && h < p.heads) {                     // (a unit's elements: those that it would have written)
-          T* to = reinterpret_cast<T*>(p.q_out) + (first + r) * p.ldqo + (long)h * p.d;
-          const float none[N] = {};
-          if (PAIRS && N == 8) store(to + u * N, none);
-          else if (u < p.pairs / N) {
-            store(to + (PAIRS ? 2 * u : u * N), none);
-            store(to + (PAIRS ? 2 * u + 1 : u * N + p.pairs), none);
-          } else store(to + 2 * p.pairs + (u - p.pairs / N) * N, none);
-        }
-      } else if (h < p.heads) {
-        unit<T, false, PAIRS, N, true>(reinterpret_cast<const T*>(p.q) + (first + r) * p.ldq + (long)h * p.d,
-                                       reinterpret_cast<T*>(p.q_out) + (first + r) * p.ldqo + (long)h * p.d, cs, u, p.pairs, 1.f);
-      } else {
-        const int g = h - p.heads;
-        const T* from = reinterpret_cast<const T*>(p.k) + (first + r) * p.ldk + (long)g * p.d;
-        if (!p.cached) {
-          unit<T, false, PAIRS, N, true>(from, reinterpret_cast<T*>(p.k_out) + (first + r) * p.ldko + (long)g * p.d, cs, u, p.pairs, 1.f);
-        } else if (at[r].page >= 0) {
-          const long to = at[r].page * p.k_page + at[r].at * p.k_token + g * p.k_head;
-          unit<T, E4M3, PAIRS, N, true>(from, reinterpret_cast<char*>(p.k_out) + to * (E4M3 ? 1 : (long)sizeof(T)), cs, u, p.pairs,
-                                        E4M3 && p.k_scale ? p.k_scale[g] : 1.f);
-        }
+  // units of a head, heads of a row (of q, of k, with a cache of v), rows
+  const int units = p.units, heads = p.heads + p.kv_heads, all = p.cached ? heads + p.kv_heads : heads, count = rows * all * units;
+  auto piece = [&](int i, Unit<T, PAIRS, N>& x) {
+    x.what = 0;
+    if (i >= count) return;
+    const int hr = (int)p.by_units((uint32_t)i), u = i - hr * units, r = (int)p.by_heads((uint32_t)hr), h = hr - r * all;
+    x.at(u, p.pairs, angles + r * p.pairs);
+    const long row = first + r;
+    if (h < p.heads) {
+      x.from = reinterpret_cast<const T*>(p.q) + row * p.ldq + (long)h * p.d;
+      x.to = reinterpret_cast<T*>(p.q_out) + row * p.ldqo + (long)h * p.d;
+      x.what = !p.cached || at[r].place >= 0 ? 1 : p.fill ? 3 : 0;
+    } else {
+      const bool values = h >= heads;
+      const int g = h - (values ? heads : p.heads);
+      x.from = reinterpret_cast<const T*>(values ? p.v : p.k) + row * (values ? p.ldv : p.ldk) + (long)g * p.d;
+      if (values) x.cs = nullptr;
+      if (!p.cached) {
+        x.to = reinterpret_cast<T*>(p.k_out) + row * p.ldko + (long)g * p.d;
+        x.what = 1;
+      } else if (at[r].page >= 0) {
+        const long to = at[r].page * (values ? p.v_page : p.k_page) + at[r].at * (values ? p.v_token : p.k_token) + g * (values ? p.v_head : p.k_head);
+        x.to = reinterpret_cast<char*>(values ? p.v_out : p.k_out) + to * (E4M3 ? 1 : (long)sizeof(T));
+        x.what = E4M3 ? 2 : 1;
+        const float* scales = values ? p.v_scale : p.k_scale;
+        x.scale = E4M3 && scales ? scales[g] : 1.f;
       }
     }
-  }
-  if (p.cached) {
-    const int units = p.d / N;
-    for (long i = tid; i < (long)rows * p.kv_heads * units; i += NT) {
-      const int u = (int)(i % units), hr = (int)(i / units), g = hr % p.kv_heads, r = hr / p.kv_heads;
-      if (at[r].page < 0) continue;
-      const long to = at[r].page * p.v_page + at[r].at * p.v_token + g * p.v_head;
-      unit<T, E4M3, PAIRS, N, false>(reinterpret_cast<const T*>(p.v) + (first + r) * p.ldv + (long)g * p.d,
-                                     reinterpret_cast<char*>(p.v_out) + to * (E4M3 ? 1 : (long)sizeof(T)), nullptr, u, 0,
-                                     E4M3 && p.v_scale ? p.v_scale[g] : 1.f);
-    }
+  };
+  for (int i = tid; i < count; i += 2 * NT) {            // two on their way at a time
+    Unit<T, PAIRS, N> x, y;
+    piece(i, x);
+    piece(i + NT, y);
+    x.fetch();
+    y.fetch();
+    x.template finish<E4M3>();
+    y.template finish<E4M3>();
   }
 }
 
@@ -240,8 +256,8 @@ KH_EXPORT int kh_rotary(const void* q, const void* k, const void* v, void* q_out
   if ((positions && ((uintptr_t)positions & (position_type == 1 ? 7 : 3))) || ((uintptr_t)frequencies & (flags & 4 ? 3 : 7))) return KH_ERR_ALIGNMENT;
   if (((uintptr_t)slots | (uintptr_t)places) & 3) return KH_ERR_ALIGNMENT;
   if (d > 1024) return KH_ERR_UNSUPPORTED;
-  if (rows > (1L << 30) || heads > (1L << 20) || kv_heads > (1L << 20)) return KH_ERR_TOO_LARGE;
-  RotaryParams p{};
+  if (rows > (1L << 30) || heads * d > (1L << 24) || kv_heads * d > (1L << 24)) return KH_ERR_TOO_LARGE;   // (a workgroup counts its pieces in 31 bits)
+  RotaryParams p{.by_pairs = KhDivide(pairs > 0 ? (uint32_t)pairs : 1u), .by_units = KhDivide(1), .by_heads = KhDivide((uint32_t)(heads + kv_heads * (cache ? 2 : 1)))};
   p.q = q, p.k = k, p.v = v, p.q_out = q_out, p.k_out = k_out, p.positions = positions, p.frequencies = frequencies, p.slots = slots, p.places = places;
   p.rows = rows, p.ldq = ldq, p.ldk = ldk, p.ldv = ldv, p.ldqo = ldqo, p.ldko = ldko;
   p.heads = (int)heads, p.kv_heads = (int)kv_heads, p.d = (int)d, p.pairs = (int)pairs, p.axes = (int)axes;
@@ -261,11 +277,13 @@ KH_EXPORT int kh_rotary(const void* q, const void* k, const void* v, void* q_out
   // pieces of eight: whole ones in a head, its halves and its rows, at addresses of 16 bytes (the cache's are: kh_cache_check)
   const bool pieces = d % 8 == 0 && pairs % (in_turn ? 4 : 8) == 0 && (ldq | ldk | ldqo | (cache ? ldv : ldko)) % 8 == 0 && kh_aligned16(q) && kh_aligned16(k) &&
                       kh_aligned16(q_out) && kh_aligned16(cache ? v : k_out);
+  p.units = pieces ? (int)(in_turn ? d / 8 : pairs / 8 + (d - 2 * pairs) / 8) : (int)(d - pairs);
+  p.by_units = KhDivide((uint32_t)p.units);
   // a workgroup has a row, or as many as make one angle a thread, where 2048 workgroups are left
   long per = rows / 2048;
-  const long most = pairs > 0 ? (NT + pairs - 1) / pairs : 16;
+  const long most = pairs > 0 ? (NT + pairs - 1) / pairs : MOST_ROWS;
   per = per < 1 ? 1 : per > most ? most : per;
-  p.per = (int)(per < 16 ? per : 16);
+  p.per = (int)(per < MOST_ROWS ? per : MOST_ROWS);
   hipStream_t s = (hipStream_t)stream;
   const bool codes = cache && cache->type == KH_E4M3;
   if (type == 2) launch<float, false>(p, in_turn, pieces, s);
