@@ -135,28 +135,40 @@ __global__ __launch_bounds__(NT) void extend(const PagesParams p) {
   prefix(over, &all_over, red);                         // (and what was dealt out is there for all threads)
   if (threadIdx.x == 0) *p.told = wanted - got + all_over;
   __syncthreads();
-  const int lane = threadIdx.x & 63;
-  for (int s = threadIdx.x >> 6; s < p.slots; s += NT / 64) {
-    const int more = p.asked[s];
-    if (more <= 0) continue;
-    const int n = clamped(p.lengths[s], p), fits = more < most - n ? more : most - n;
-    const int first = (n + p.page - 1) / p.page, last = (n + fits + p.page - 1) / p.page, start = p.w.start[s];
-    for (int i = first + lane; i < last; i += 64) p.table[(long)s * p.width + i] = start + i - first < got ? p.w.free[start + i - first] : -1;
-    if (lane == 0) p.lengths[s] = n + fits;
+  // a thread enters the pages of a slot, a wave those of one that gets many
+  constexpr int FEW = 4;
+  for (int base = 0; base < p.slots; base += NT) {
+    const int s = base + (int)threadIdx.x, lane = threadIdx.x & 63;
+    int first = 0, need = 0, start = 0;
+    if (s < p.slots && p.asked[s] > 0) {
+      const int more = p.asked[s], n = clamped(p.lengths[s], p), fits = more < most - n ? more : most - n;
+      first = (n + p.page - 1) / p.page;
+      need = (n + fits + p.page - 1) / p.page - first;
+      start = p.w.start[s];
+      p.lengths[s] = n + fits;
+      if (need <= FEW)
+        for (int i = 0; i < need; ++i) p.table[(long)s * p.width + first + i] = start + i < got ? p.w.free[start + i] : -1;
+    }
+    for (uint64_t many = __ballot(need > FEW); many; many &= many - 1) {
+      const int who = __ffsll((unsigned long long)many) - 1, f = __shfl(first, who, 64), k = __shfl(need, who, 64), from = __shfl(start, who, 64);
+      int32_t* row = p.table + (long)(base + (threadIdx.x & ~63) + who) * p.width + f;
+      for (int i = lane; i < k; i += 64) row[i] = from + i < got ? p.w.free[from + i] : -1;
+    }
   }
 }
 
-// A workgroup a slot: what it gives up and what it takes over, counted; its new row of pages set aside, since others still read the old one.
-__global__ __launch_bounds__(NC) void reorder_count(const PagesParams p) {
-  const int s = blockIdx.x, parent = p.asked[s];
+// What slot s gives up and takes over, counted by N threads (a wave or a workgroup); its new row of pages set aside, since others still read the old one.
+template <int N>
+__device__ __forceinline__ void count(const PagesParams& p, int s) {
+  const int lane = threadIdx.x & (N - 1), parent = p.asked[s];
   const bool takes = parent >= 0 && parent < p.slots;
   if (parent == s) {
-    if (threadIdx.x == 0) p.w.state[s] = 0, p.w.want[s] = Copy{-1, -1, 0};
+    if (lane == 0) p.w.state[s] = 0, p.w.want[s] = Copy{-1, -1, 0};
     return;
   }
   const int32_t* mine = p.table + (long)s * p.width;
   const int used = (clamped(p.lengths[s], p) + p.page - 1) / p.page;
-  for (int i = threadIdx.x; i < used; i += NC) {
+  for (int i = lane; i < used; i += N) {
     const int e = mine[i];
     if (e >= 0 && e < p.pages) atomicSub(p.refs + e, 1);
   }
@@ -166,11 +178,11 @@ __global__ __launch_bounds__(NC) void reorder_count(const PagesParams p) {
   int other = 0;
   if (part) {
     other = p.asked[parent] == parent;
-    for (int i = threadIdx.x; i < s; i += NC) other |= i != parent && p.asked[i] == parent;
+    for (int i = lane; i < s; i += N) other |= i != parent && p.asked[i] == parent;
   }
-  const bool heir = !__syncthreads_or(other);
+  const bool heir = !(N == 64 ? __any(other) : __syncthreads_or(other));
   const int32_t* theirs = p.table + (long)(takes ? parent : 0) * p.width;
-  for (int i = threadIdx.x; i < p.width; i += NC) {
+  for (int i = lane; i < p.width; i += N) {
     int e = -1;
     if (i < full || (i == full && part && heir)) {
       e = theirs[i];
@@ -178,17 +190,25 @@ __global__ __launch_bounds__(NC) void reorder_count(const PagesParams p) {
     }
     row[i] = e;
   }
-  if (threadIdx.x == 0) {
+  if (lane == 0) {
     p.w.state[s] = takes ? 1 : 2;
     p.w.length[s] = n;
     const int e = part && !heir ? theirs[full] : -1;
     p.w.want[s] = e >= 0 && e < p.pages ? Copy{e, full, part} : Copy{-1, -1, 0};
   }
 }
+__global__ __launch_bounds__(NC) void reorder_count(const PagesParams p) {
+  count<NC>(p, blockIdx.x);
+}
 
-// Pages for the copies, by slot: none of them is one that is copied, since somebody holds those.
+// Pages for the copies, by slot: none of them is one that is copied, since somebody holds those.  ALL: counts first (few slots: a launch less).
+template <bool ALL>
 __global__ __launch_bounds__(NT) void reorder_deal(const PagesParams p) {
   __shared__ int red[NT / 64];
+  if constexpr (ALL) {
+    for (int s = threadIdx.x >> 6; s < p.slots; s += NT / 64) count<64>(p, s);
+    __syncthreads();
+  }
   int wanted = 0;
   for (int base = 0; base < p.slots; base += NT) {
     const int s = base + (int)threadIdx.x;
@@ -360,10 +380,16 @@ KH_EXPORT int kh_cache_reorder(const KhPagedCache* cache, const int32_t* parents
   if (rc != KH_OK) return rc;
   const PagesParams p = params(*cache, parents, missing, workspace);
   hipStream_t s = (hipStream_t)stream;
-  kh_launch(KH_TAG_CACHE_PAGES, reorder_count, dim3((unsigned)p.slots), dim3(NC), 0, s, p);
-  hipError_t e = hipGetLastError();                     // (the launches behind it go by what it writes)
-  if (e != hipSuccess) return (int)e;
-  kh_launch(KH_TAG_CACHE_PAGES, reorder_deal, dim3(1), dim3(NT), 0, s, p);
+  hipError_t e;
+  // one workgroup counts for few slots with short rows (four beams of 77 tokens: 3.8 + 4.4 us for the two launches)
+  if (cache->slots <= 32 && cache->slots * cache->width <= 4096) {
+    kh_launch(KH_TAG_CACHE_PAGES, reorder_deal<true>, dim3(1), dim3(NT), 0, s, p);
+  } else {
+    kh_launch(KH_TAG_CACHE_PAGES, reorder_count, dim3((unsigned)p.slots), dim3(NC), 0, s, p);
+    e = hipGetLastError();                              // (the launches behind it go by what it writes)
+    if (e != hipSuccess) return (int)e;
+    kh_launch(KH_TAG_CACHE_PAGES, reorder_deal<false>, dim3(1), dim3(NT), 0, s, p);
+  }
   e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
   copy<false>(*cache, p, s);

@@ -398,7 +398,7 @@ __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : D > 64 ? 2 : 3) void attend(
   }
   total = uniform(total) * units;
   const int W = total < G ? total : G;                  // workgroups that have a tile
-  if (tid == 0) p.border[w] = int4{-1, 0, 0, 0};
+  if (tid == 0 && p.border) p.border[w] = int4{-1, 0, 0, 0};
   if (w < W) {
     const int begin = (int)((long)total * w / W), end = (int)((long)total * (w + 1) / W);
     int at_row = before * units;                        // where row r begins
@@ -658,6 +658,7 @@ bool line_fits(int64_t rows, int64_t kv_heads, int64_t group, int64_t span) {
 }
 
 int64_t bytes_of(const Plan& plan, int64_t group, int64_t d) {
+  if (!plan.parts) return 0;                            // (every unit is one tile)
   const int64_t q = group < QB ? group : QB;
   return plan.workgroups * 16 + 2 * plan.workgroups * q * (d + 2) * 4;
 }
@@ -670,7 +671,7 @@ int run(const PagedParams& p, const Plan& plan, hipStream_t s) {
     if (e != hipSuccess) return (int)e;
   }
   kh_launch(KH_TAG_PAGED_ATTENTION, attend<D, T, CODES, EIGHT, TAIL>, dim3((unsigned)plan.workgroups), dim3(NW * 64), lds, s, p);
-  if (plan.parts && plan.workgroups > 1) {
+  if (plan.parts) {
     const hipError_t e = hipGetLastError();             // (the launch behind it reads what it writes)
     if (e != hipSuccess) return (int)e;
     const unsigned borders = (unsigned)plan.workgroups - 1, queries = p.group < QB ? p.group : QB;
@@ -705,7 +706,7 @@ KH_EXPORT int kh_paged_attention(const void* q, void* o, const KhPagedCache* cac
   const int rc = kh_cache_check(cache);
   if (rc != KH_OK) return rc;
   const KhPagedCache& c = *cache;
-  if (!q || !o || !workspace || rows <= 0 || heads <= 0 || heads % c.kv_heads != 0 || window < 0 || (flags & ~1) || type < 0 || type > 1) return KH_ERR_INVALID_ARG;
+  if (!q || !o || rows <= 0 || heads <= 0 || heads % c.kv_heads != 0 || window < 0 || (flags & ~1) || type < 0 || type > 1) return KH_ERR_INVALID_ARG;
   if (layer < 0 || layer >= c.layers || ldq < heads * c.d || ldo < heads * c.d || (!slots && rows > c.slots)) return KH_ERR_INVALID_ARG;
   if (c.type != KH_E4M3 && c.type != type) return KH_ERR_UNSUPPORTED;
   if ((((uintptr_t)q | (uintptr_t)o) & 1) || (((uintptr_t)slots | (uintptr_t)lengths) & 3) || !kh_aligned16(workspace)) return KH_ERR_ALIGNMENT;
@@ -713,9 +714,10 @@ KH_EXPORT int kh_paged_attention(const void* q, void* o, const KhPagedCache* cac
   const long group = heads / c.kv_heads, e = kh_cache_element(c);
   if (!line_fits(rows, c.kv_heads, group, c.width * c.page)) return KH_ERR_TOO_LARGE;
   const Plan plan = plan_of(rows, c.kv_heads, group, c.d, c.width * c.page);
+  if (plan.parts && !workspace) return KH_ERR_INVALID_ARG;
   PagedParams p{q, (const char*)c.k + layer * c.k_layer * e, (const char*)c.v + layer * c.v_layer * e, o, c.table, lengths, c.lengths, slots,
                 c.k_scale ? c.k_scale + layer * c.kv_heads : nullptr, c.v_scale ? c.v_scale + layer * c.kv_heads : nullptr,
-                (float*)((char*)workspace + plan.workgroups * 16), (int4*)workspace, ldq, ldo, (uint32_t)(c.k_page * e), (uint32_t)(c.k_token * e), (uint32_t)(c.v_page * e),
+                plan.parts ? (float*)((char*)workspace + plan.workgroups * 16) : nullptr, plan.parts ? (int4*)workspace : nullptr, ldq, ldo, (uint32_t)(c.k_page * e), (uint32_t)(c.k_token * e), (uint32_t)(c.v_page * e),
                 (uint32_t)(c.v_token * e), c.k_head * e, c.v_head * e,
                 (int)rows, (int)c.kv_heads, (int)group, (int)((group + QB - 1) / QB), (int)c.d, (int)c.slots, (int)c.width, (int)c.pages, (int)c.page,
                 (int)(window < (1L << 30) ? window : 0), scale * 1.4426950408889634f, flags & 1, 0, KhDivide((uint32_t)c.page)};

@@ -1731,10 +1731,6 @@ class PagedCache:
                    torch.zeros(pages, dtype=torch.int32, device=device), k_scale, v_scale)
 
 
-def _cache_parts(cache: PagedCache):
-    return cache.v, cache.table, cache.lengths, cache.refs, cache.k_scale, cache.v_scale
-
-
 def _cache_call(name: str, cache: PagedCache, asked: Optional[torch.Tensor]) -> torch.Tensor:
     """One of the calls that keep a cache's pages: what it tells, int32 [1] on the device."""
     lib = _lib.load()
@@ -1797,6 +1793,8 @@ def _section_ends(sections):
 def _token_rows(t: torch.Tensor, width: int, name: str):
     """(rows, their stride) of [..., width] whose leading axes are one run of rows."""
     shape, st = t.shape, t.stride()
+    if len(shape) == 2 and shape[1] == width and st[1] == 1:
+        return shape[0], (st[0] if shape[0] > 1 else width)
     if len(shape) < 2 or shape[-1] != width or (st[-1] != 1 and width > 1):
         raise ValueError(f"{name} must be [.., {width}] with a contiguous last axis, got {tuple(shape)}")
     rows, ld = shape[-2], st[-2]
@@ -1866,9 +1864,9 @@ def rotary(q: torch.Tensor, k: torch.Tensor, heads: int, positions: torch.Tensor
     frequencies float64 or float32 [pairs] (rotary_frequencies).  out may be q and k_out k (in place)."""
     kv = heads if kv_heads is None else kv_heads
     if out is None:
-        out = q.new_empty(q.shape)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if k_out is None:
-        k_out = k.new_empty(k.shape)
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
     _here(q, k, positions, frequencies, out, k_out)
     _rotary_call(q, k, None, heads, kv, positions, frequencies, (frequencies.numel(),) if sections is None else tuple(sections), pairs, out, k_out, None, 0, None, None, 0)
     return out, k_out
@@ -1886,14 +1884,14 @@ def cache_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: Paged
     in a captured graph): those of a given out stay as they were, those of a new one are zero.  out may be q."""
     fill = out is None
     if fill:
-        out = q.new_empty(q.shape)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if k.dtype not in (torch.bfloat16, torch.float16) or (cache.k.dtype is not k.dtype and cache.k.dtype is not torch.float8_e4m3fn):
         raise TypeError(f"{k.dtype} rows for a cache of {cache.k.dtype}")
     if not 0 <= layer < cache.layers:
         raise ValueError(f"layer {layer} of a cache of {cache.layers}")
     if q.shape[-1] != heads * cache.d:
         raise ValueError(f"q must be [.., {heads} * {cache.d}], got {tuple(q.shape)}")
-    _here(q, k, v, positions, frequencies, slots, places, out, cache.k, *_cache_parts(cache))
+    _here(q, k, v, positions, frequencies, slots, places, out, cache.k)      # (the cache's parts lie together)
     rows = q.numel() // q.shape[-1]
     if slots is not None:
         _fits(slots, torch.int32, (rows,), "slots")
@@ -1927,13 +1925,13 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, heads: int, layer: int =
     rows, ldq = _token_rows(q, heads * d, "q")
     fill = out is None
     if fill:
-        out = q.new_empty(q.shape)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.dtype is not dt:
         raise TypeError(f"out must be {dt}")
     o_rows, ldo = _token_rows(out, heads * d, "out")
     if o_rows != rows:
         raise ValueError("q and out must have the same rows")
-    _here(q, slots, lengths, out, cache.k, *_cache_parts(cache))
+    _here(q, slots, lengths, out, cache.k)      # (the cache's parts lie together)
     if slots is not None:
         _fits(slots, torch.int32, (rows,), "slots")
     elif rows > cache.slots:
@@ -1945,8 +1943,8 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, heads: int, layer: int =
     nbytes = _workspace_bytes("kh_paged_attention_workspace_bytes", rows, heads, cache.kv_heads, d, cache.width * cache.page)
     if nbytes < 0:
         _lib.check(nbytes, "kh_paged_attention_workspace_bytes")
-    ws = q.new_empty(nbytes // 2)              # (elements of two bytes)
-    rc = lib.kh_paged_attention(q.data_ptr(), out.data_ptr(), cache.desc, layer, _ptr(slots), _ptr(lengths), ws.data_ptr(), rows, heads, ldq, ldo, window,
+    ws = q.new_empty(nbytes // 2) if nbytes else None      # (elements of two bytes)
+    rc = lib.kh_paged_attention(q.data_ptr(), out.data_ptr(), cache.desc, layer, _ptr(slots), _ptr(lengths), _ptr(ws), rows, heads, ldq, ldo, window,
                                 d ** -0.5 if scale is None else scale, fill, _TYPES[dt], _stream())
     if rc:
         _lib.check(rc, "kh_paged_attention")

@@ -60,7 +60,7 @@ def test_attention_entry_point(lib):
     def call(q=16, o=16, c=None, layer=0, slots=None, lengths=None, ws=16, rows=2, H=4, ldq=256, ldo=256, window=0, flags=0, t=0):
         return lib.kh_paged_attention(q, o, c or cache(), layer, slots, lengths, ws, rows, H, ldq, ldo, window, 0.1, flags, t, None)
 
-    assert call(q=None) == -1 and call(o=None) == -1 and call(ws=None) == -1 and call(rows=0) == -1 and call(rows=5) == -1 and call(H=3) == -1 and call(H=0) == -1
+    assert call(q=None) == -1 and call(o=None) == -1 and call(rows=0) == -1 and call(rows=5) == -1 and call(H=3) == -1 and call(H=0) == -1
     assert call(layer=2) == -1 and call(layer=-1) == -1 and call(ldq=128) == -1 and call(ldo=128) == -1 and call(window=-1) == -1 and call(flags=2) == -1 and call(t=2) == -1
     assert call(t=1) == -2 and call(c=cache(kind=1)) == -2
     assert call(q=17) == -3 and call(ws=8) == -3 and call(slots=18) == -3 and call(lengths=17) == -3
@@ -68,7 +68,9 @@ def test_attention_entry_point(lib):
     assert lib.kh_paged_attention(16, 16, None, 0, None, None, 16, 2, 4, 256, 256, 0, 0.1, 0, 0, None) == -1
     size = lib.kh_paged_attention_workspace_bytes
     assert size(0, 4, 2, 64, 80) == -1 and size(2, 3, 2, 64, 80) == -1 and size(2, 4, 0, 64, 80) == -1 and size(2, 4, 2, 64, 0) == -1 and size(2, 4, 2, 60, 80) == -2 and size(2, 4, 2, 264, 80) == -2
-    assert size(1 << 25, 4, 2, 64, 80) == -4 and size(2, 4, 2, 64, 1 << 31) == -4 and size(1, 1, 1, 8, 1) > 0
+    assert call(ws=None, c=cache(width=9)) == -1                # a sequence may have more than one tile: there are parts to be joined
+    assert size(1 << 25, 4, 2, 64, 80) == -4 and size(2, 4, 2, 64, 1 << 31) == -4 and size(1 << 20, 1 << 10, 1 << 10, 64, 1 << 20) == -4
+    assert size(1, 1, 1, 8, 1) == 0 and size(64, 4, 2, 64, 128) == 0 and size(1, 1, 1, 8, 129) > 0
     assert size(1, 8, 1, 128, 1 << 20) < 1 << 25                # a workgroup's parts, however long the cache
 
 
