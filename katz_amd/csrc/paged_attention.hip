@@ -365,8 +365,12 @@ __device__ __forceinline__ void zero_row(const PagedParams& p, int r) {
   for (int i = threadIdx.x; i < p.kv_heads * p.group * p.d; i += NW * 64) to[i] = (T)0.f;
 }
 
+// Workgroups a CU, by what registers allow without spilling in the loop.  16 bits: two with D 128 (three spill and take 179 us where two take 123), three
+// with D 64; e4m3, whose steps have half the bytes: three with D 128 (70 us where two take 84, 32 sequences of 4096 tokens on 8 key heads).
+constexpr int wgs_a_cu(int D, bool codes) { return D > 128 ? 1 : D > 64 && !codes ? 2 : 3; }
+
 template <int D, typename T, bool CODES, bool EIGHT, bool TAIL>
-__global__ __launch_bounds__(NW * 64, D > 128 ? 1 : D > 64 ? 2 : 3) void attend(const PagedParams p) {
+__global__ __launch_bounds__(NW * 64, wgs_a_cu(D, CODES)) void attend(const PagedParams p) {
   using S = Shape<D, T, CODES, EIGHT, TAIL>;
   constexpr int OW = D + 4;                             // floats of a query's row in LDS
   extern __shared__ float lds[];                        // [NW][QB][OW] outputs, [2][NW][QB] maxima and sums
@@ -576,7 +580,7 @@ __global__ __launch_bounds__(NW * 64) void join_few(const PagedParams p, const i
 template <typename T, bool CODES>
 __global__ __launch_bounds__(JT) void join_many(const PagedParams p, const int G) {
   constexpr int DL = 8, GR = JT / DL;                   // lanes of 32 dimensions, groups that take parts in turn
-  // there are few rows (at most MOST / 16 units): a lane has one's tiles, and with them where this workgroup's unit lies in the line
+  // there are few rows (at most MOST / 32 units): a lane has one's tiles, and with them where this workgroup's unit lies in the line
   const int units = p.kv_heads * p.blocks, r = blockIdx.x / units, unit = blockIdx.x - r * units, at_lane = threadIdx.x & 63;
   const int tiles = at_lane < p.rows ? row_of(p, at_lane).tiles : 0;
   int before = tiles;
@@ -646,10 +650,10 @@ __global__ __launch_bounds__(JT) void join_many(const PagedParams p, const int G
 // `many`: parts of a unit, about the workgroups by the units, are more than a wave joins in passing.
 struct Plan { long workgroups; bool parts, many; };
 
-Plan plan_of(int64_t rows, int64_t kv_heads, int64_t group, int64_t d, int64_t span) {
+Plan plan_of(int64_t rows, int64_t kv_heads, int64_t group, int64_t d, int64_t span, bool codes) {
   const long tiles = (span + TILE - 1) / TILE, units = rows * kv_heads * ((group + QB - 1) / QB);
-  const long at_once = 256 * (d > 128 ? 1 : d > 64 ? 2 : 3);
-  return Plan{units * tiles < at_once ? units * tiles : at_once, tiles > 1, units * 16 < at_once};
+  const long at_once = 256 * wgs_a_cu((int)d, codes);
+  return Plan{units * tiles < at_once ? units * tiles : at_once, tiles > 1, units * 32 < at_once};
 }
 
 // whether all tiles can be counted in 31 bits
@@ -697,7 +701,7 @@ KH_EXPORT int64_t kh_paged_attention_workspace_bytes(int64_t rows, int64_t heads
   if (d % 8 != 0 || d > 256) return KH_ERR_UNSUPPORTED;
   if (rows > (1L << 24) || heads > (1L << 16) || span > (1L << 30)) return KH_ERR_TOO_LARGE;
   if (!line_fits(rows, kv_heads, heads / kv_heads, span)) return KH_ERR_TOO_LARGE;
-  return bytes_of(plan_of(rows, kv_heads, heads / kv_heads, d, span), heads / kv_heads, d);
+  return bytes_of(plan_of(rows, kv_heads, heads / kv_heads, d, span, true), heads / kv_heads, d);   // (e4m3 has no fewer workgroups)
 }
 
 KH_EXPORT int kh_paged_attention(const void* q, void* o, const KhPagedCache* cache, int64_t layer, const int32_t* slots, const int32_t* lengths,
@@ -713,7 +717,7 @@ KH_EXPORT int kh_paged_attention(const void* q, void* o, const KhPagedCache* cac
   if (rows > (1L << 24) || heads > (1L << 16)) return KH_ERR_TOO_LARGE;
   const long group = heads / c.kv_heads, e = kh_cache_element(c);
   if (!line_fits(rows, c.kv_heads, group, c.width * c.page)) return KH_ERR_TOO_LARGE;
-  const Plan plan = plan_of(rows, c.kv_heads, group, c.d, c.width * c.page);
+  const Plan plan = plan_of(rows, c.kv_heads, group, c.d, c.width * c.page, c.type == KH_E4M3);
   if (plan.parts && !workspace) return KH_ERR_INVALID_ARG;
   PagedParams p{q, (const char*)c.k + layer * c.k_layer * e, (const char*)c.v + layer * c.v_layer * e, o, c.table, lengths, c.lengths, slots,
                 c.k_scale ? c.k_scale + layer * c.kv_heads : nullptr, c.v_scale ? c.v_scale + layer * c.kv_heads : nullptr,
