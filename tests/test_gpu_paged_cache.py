@@ -632,3 +632,34 @@ def test_calls_without_rows():
     assert ops.paged_attention(none, pages.dev, 4).shape == (0, 256)
     assert ops.cache_append(none, none[:, :128], none[:, :128], pages.dev, 4).shape == (0, 256)
     assert ops.rotary(none, none[:, :128], 4, int32([]).view(0, 1), ops.rotary_frequencies(32, device=DEV), kv_heads=2)[1].shape == (0, 128)
+
+
+@pytest.mark.parametrize("rows,longest,kv,d", [(40, 20000, 1, 64), (3, 20000, 2, 64), (9, 9000, 1, 128)])
+def test_long_sequences_among_short_ones(rows, longest, kv, d):
+    """More parts of one sequence than a wave has lanes (the workgroups are dealt to few rows), and many of several."""
+    from katz_amd import ops
+
+    lengths = [0] * rows
+    lengths[rows // 2] = longest
+    if rows < 10:
+        lengths[0], lengths[-1] = 700, longest // 2
+    pages = Pages(25, lengths, 64, kv, d, spare=1)
+    q = randn(gen(26), rows, 2 * kv * d)
+    ref, off = attention_reference(q, pages, 2 * kv, range(rows), pages.held)
+    got = ops.paged_attention(q.to(DEV), pages.dev, 2 * kv)
+    assert_within(got.view(rows, 2 * kv, d), ref, HALF[BF] * ref.abs() + off, "long among short")
+
+
+def test_rows_by_the_hundred():
+    """More rows than a workgroup has threads."""
+    from katz_amd import ops
+
+    rows, heads, d = 700, 2, 64
+    lengths = [(i * 37) % 90 if i % 5 else 0 for i in range(rows)]
+    pages = Pages(27, lengths, 16, 1, d, width=10)
+    q = randn(gen(28), rows, heads * d)
+    slots = torch.arange(rows, dtype=torch.int32)
+    slots[::50] = -1
+    ref, off = attention_reference(q, pages, heads, slots.clamp(min=0), torch.where(slots < 0, 0, pages.held[slots.clamp(min=0).long()]))
+    got = ops.paged_attention(q.to(DEV), pages.dev, heads, slots=slots.to(DEV))
+    assert_within(got.view(rows, heads, d), ref, HALF[BF] * ref.abs() + off, "rows")
