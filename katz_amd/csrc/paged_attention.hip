@@ -365,9 +365,10 @@ __device__ __forceinline__ void zero_row(const PagedParams& p, int r) {
   for (int i = threadIdx.x; i < p.kv_heads * p.group * p.d; i += NW * 64) to[i] = (T)0.f;
 }
 
-// Workgroups a CU, by what registers allow without spilling in the loop.  16 bits: two with D 128 (three spill and take 179 us where two take 123), three
-// with D 64; e4m3, whose steps have half the bytes: three with D 128 (70 us where two take 84, 32 sequences of 4096 tokens on 8 key heads).
-constexpr int wgs_a_cu(int D, bool codes) { return D > 128 ? 1 : D > 64 && !codes ? 2 : 3; }
+// Workgroups a CU, by what registers allow without spilling in the loop.  32 sequences of 4096 tokens, 4096 bytes of keys and values a token in 16 bits: heads of
+// 128 97 us with two (three spill: 131 -> 179 where 64 requests took 123 with two), of 64 94 with three, of 256 85 with one; in e4m3, whose steps have half the
+// bytes, of 128 84 us with two and 68 with three, of 64 93 with three and 119 with four, of 256 72 with one and 70 with two.
+constexpr int wgs_a_cu(int D, bool codes) { return D > 128 ? (codes ? 2 : 1) : D > 64 && !codes ? 2 : 3; }
 
 template <int D, typename T, bool CODES, bool EIGHT, bool TAIL>
 __global__ __launch_bounds__(NW * 64, wgs_a_cu(D, CODES)) void attend(const PagedParams p) {
@@ -440,73 +441,77 @@ __global__ __launch_bounds__(NW * 64, wgs_a_cu(D, CODES)) void attend(const Page
     u.row_at = uniform(where[1]);
     u.row = row_of(p, uniform(where[2]), uniform(where[3]));
     Wave<D, T, CODES, EIGHT, TAIL> wv;
-    bool more = advance(u, begin);
-    wv.begin(p, u, wave);
-    while (more) {
+    Piece done;
+    int at = begin;
+    for (bool some = false;; some = true) {
+      const bool more = advance(u, at);
+      if (more) wv.begin(p, u, wave);                   // (on its way while the waves' parts of the piece before it are put together)
+      if (some) {
+        // the waves' parts together
+        float sum = wv.l;
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        if (g4 == 0) {
+          ms[wave * QB + c16] = wv.m;
+          ms[(NW + wave) * QB + c16] = sum;
+        }
+        __syncthreads();
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) top = fmaxf(top, ms[i * QB + c16]);
+        const float by = wv.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(wv.m - top);
+#pragma unroll
+        for (int c = 0; c < S::NC; ++c)
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int j = 0; j < S::VE; j += 4) {
+              f32x4 f;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) f[i] = wv.o[c * S::VE + j + i][n] * by;
+              *reinterpret_cast<f32x4*>(lds + (wave * QB + c16) * OW + c * 128 + S::VE * (4 * g4 + n) + j) = f;
+            }
+        __syncthreads();
+        const bool complete = done.a >= begin && done.b <= end;
+        const long slot = 2 * (long)w + (done.a >= begin ? 1 : 0);
+        const int q_max = p.group < QB ? p.group : QB;
+        for (int i = tid; i < done.queries * (D / 4); i += NW * 64) {
+          const int qi = i / (D / 4), dim = (i - qi * (D / 4)) * 4;
+          if (TAIL && dim >= p.d) continue;
+          f32x4 f{0.f, 0.f, 0.f, 0.f};
+          float top_q = -INFINITY, sum_q = 0.f;
+#pragma unroll
+          for (int x = 0; x < NW; ++x) {
+            f += *reinterpret_cast<const f32x4*>(lds + (x * QB + qi) * OW + dim);
+            top_q = fmaxf(top_q, ms[x * QB + qi]);
+          }
+#pragma unroll
+          for (int x = 0; x < NW; ++x) {
+            const float mx = ms[x * QB + qi];
+            sum_q += ms[(NW + x) * QB + qi] * (mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - top_q));
+          }
+          if (complete) {
+            const float scale = CODES && p.v_scale ? p.v_scale[done.head] : 1.f;
+            const float out[4] = {f[0], f[1], f[2], f[3]};
+            store_row<T>(p, done.r, done.head * p.group + done.q0 + qi, dim, out, sum_q, scale);
+          } else {
+            *reinterpret_cast<f32x4*>(p.part + (slot * q_max + qi) * p.d + dim) = f;
+            if (dim == 0) {
+              float* stats = p.part + 2 * (long)G * q_max * p.d + (slot * q_max + qi) * 2;
+              stats[0] = top_q;
+              stats[1] = sum_q;
+            }
+          }
+        }
+        // where this workgroup begins in a unit that the one before it began: the unit's row, number and workgroups
+        if (tid == 0 && done.a < begin && (long)total * (w - 1) / W <= done.a)
+          p.border[w] = int4{done.r, done.unit, w - 1, (int)(((long)done.b * W - 1) / total)};
+        __syncthreads();                                  // (LDS is read)
+      }
+      if (!more) break;
       wv.run(p, u);
-      const Piece done = u;
-      more = advance(u, done.stop);
-      if (more) wv.begin(p, u, wave);                   // (on its way while the waves' parts are put together)
-      // the waves' parts together
-      float sum = wv.l;
-      sum += __shfl_xor(sum, 16, 64);
-      sum += __shfl_xor(sum, 32, 64);
-      if (g4 == 0) {
-        ms[wave * QB + c16] = wv.m;
-        ms[(NW + wave) * QB + c16] = sum;
-      }
-      __syncthreads();
-      float top = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < NW; ++i) top = fmaxf(top, ms[i * QB + c16]);
-      const float by = wv.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(wv.m - top);
-#pragma unroll
-      for (int c = 0; c < S::NC; ++c)
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-#pragma unroll
-          for (int j = 0; j < S::VE; j += 4) {
-            f32x4 f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) f[i] = wv.o[c * S::VE + j + i][n] * by;
-            *reinterpret_cast<f32x4*>(lds + (wave * QB + c16) * OW + c * 128 + S::VE * (4 * g4 + n) + j) = f;
-          }
-      __syncthreads();
-      const bool complete = done.a >= begin && done.b <= end;
-      const long slot = 2 * (long)w + (done.a >= begin ? 1 : 0);
-      const int q_max = p.group < QB ? p.group : QB;
-      for (int i = tid; i < done.queries * (D / 4); i += NW * 64) {
-        const int qi = i / (D / 4), dim = (i - qi * (D / 4)) * 4;
-        if (TAIL && dim >= p.d) continue;
-        f32x4 f{0.f, 0.f, 0.f, 0.f};
-        float top_q = -INFINITY, sum_q = 0.f;
-#pragma unroll
-        for (int x = 0; x < NW; ++x) {
-          f += *reinterpret_cast<const f32x4*>(lds + (x * QB + qi) * OW + dim);
-          top_q = fmaxf(top_q, ms[x * QB + qi]);
-        }
-#pragma unroll
-        for (int x = 0; x < NW; ++x) {
-          const float mx = ms[x * QB + qi];
-          sum_q += ms[(NW + x) * QB + qi] * (mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - top_q));
-        }
-        if (complete) {
-          const float scale = CODES && p.v_scale ? p.v_scale[done.head] : 1.f;
-          const float out[4] = {f[0], f[1], f[2], f[3]};
-          store_row<T>(p, done.r, done.head * p.group + done.q0 + qi, dim, out, sum_q, scale);
-        } else {
-          *reinterpret_cast<f32x4*>(p.part + (slot * q_max + qi) * p.d + dim) = f;
-          if (dim == 0) {
-            float* stats = p.part + 2 * (long)G * q_max * p.d + (slot * q_max + qi) * 2;
-            stats[0] = top_q;
-            stats[1] = sum_q;
-          }
-        }
-      }
-      // where this workgroup begins in a unit that the one before it began: the unit's row, number and workgroups
-      if (tid == 0 && done.a < begin && (long)total * (w - 1) / W <= done.a)
-        p.border[w] = int4{done.r, done.unit, w - 1, (int)(((long)done.b * W - 1) / total)};
-      __syncthreads();                                  // (LDS is read)
+      done = u;
+      at = u.stop;
     }
   }
   // rows that have nothing to attend to, or no slot

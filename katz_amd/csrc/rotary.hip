@@ -279,11 +279,18 @@ KH_EXPORT int kh_rotary(const void* q, const void* k, const void* v, void* q_out
                       kh_aligned16(q_out) && kh_aligned16(cache ? v : k_out);
   p.units = pieces ? (int)(in_turn ? d / 8 : pairs / 8 + (d - 2 * pairs) / 8) : (int)(d - pairs);
   p.by_units = KhDivide((uint32_t)p.units);
-  // a workgroup has a row, or as many as make one angle a thread, where 2048 workgroups are left
-  long per = rows / 2048;
-  const long most = pairs > 0 ? (NT + pairs - 1) / pairs : MOST_ROWS;
-  per = per < 1 ? 1 : per > most ? most : per;
-  p.per = (int)(per < MOST_ROWS ? per : MOST_ROWS);
+  // A workgroup has a row, or, at most as make one angle a thread, as many as leave 2048 workgroups (7904 rows of 40 heads of 64: 15.8 us, with 1024 16.6, with
+  // 8192 18.3), up to twice that where its pieces then fill the threads better (8184 rows of 32 heads of 80 into pages: three rows 20.9 us, four 19.2).
+  long whole = pairs > 0 ? (NT + pairs - 1) / pairs : MOST_ROWS;
+  whole = whole < MOST_ROWS ? whole : MOST_ROWS;
+  const long least = rows / 2048 < 1 ? 1 : rows / 2048 < whole ? rows / 2048 : whole;
+  const long each = (heads + kv_heads * (cache ? 2 : 1)) * p.units;
+  double best = 0.;
+  for (long n = least; n <= (least > 1 ? (2 * least < whole ? 2 * least : whole) : 1); ++n) {
+    const long rounds = (n * each + 2 * NT - 1) / (2 * NT);
+    const double full = (double)(n * each) / (double)(rounds * 2 * NT);
+    if (full > best) best = full, p.per = (int)n;
+  }
   hipStream_t s = (hipStream_t)stream;
   const bool codes = cache && cache->type == KH_E4M3;
   if (type == 2) launch<float, false>(p, in_turn, pieces, s);
