@@ -566,7 +566,7 @@ int kh_paged_attention(const void* q, void* o, const KhPagedCache* cache, int64_
  * kh_cache_extend: sequence s gets counts[s] (<= 0: no) more tokens, at most width * page in all.
  * kh_cache_reorder: slot s keeps its sequence where parents[s] == s, takes over the one that slot parents[s] had before the call, or, where that is no
  * slot, is emptied.  Whole pages are shared; the page not yet full is copied (its tokens, in all layers), but handed on as it is to the lowest taker
- * of a sequence whose own slot gives it up.  Entries behind a changed sequence's pages become -1.
+ * of a sequence whose own slot gives it up.  Entries behind a changed sequence's pages become -1.  At most 65536 slots.
  * kh_cache_compact: the pages in use, *in_use (device) of them, become pages 0 .. *in_use - 1: those behind go to the free ones before, both in order.
  * workspace: kh_cache_workspace_bytes, aligned to 16 bytes.  Pages at addresses that the strides make overlap are not supported. */
 int64_t kh_cache_workspace_bytes(int64_t slots, int64_t width, int64_t pages);

@@ -378,6 +378,7 @@ KH_EXPORT int kh_cache_extend(const KhPagedCache* cache, const int32_t* counts, 
 KH_EXPORT int kh_cache_reorder(const KhPagedCache* cache, const int32_t* parents, int32_t* missing, void* workspace, void* stream) {
   const int rc = check(cache, parents, missing, workspace);
   if (rc != KH_OK) return rc;
+  if (cache->slots > (1L << 16)) return KH_ERR_TOO_LARGE;           // (every slot looks through those before it)
   const PagesParams p = params(*cache, parents, missing, workspace);
   hipStream_t s = (hipStream_t)stream;
   hipError_t e;

@@ -291,6 +291,7 @@ KH_EXPORT int kh_rotary(const void* q, const void* k, const void* v, void* q_out
     const double full = (double)(n * each) / (double)(rounds * 2 * NT);
     if (full > best) best = full, p.per = (int)n;
   }
+  if ((rows + p.per - 1) / p.per > (1L << 24) - 1) return KH_ERR_TOO_LARGE;     // (2^32 threads)
   hipStream_t s = (hipStream_t)stream;
   const bool codes = cache && cache->type == KH_E4M3;
   if (type == 2) launch<float, false>(p, in_turn, pieces, s);

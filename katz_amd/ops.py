@@ -1718,6 +1718,8 @@ class PagedCache:
                 raise ValueError("the parts of a cache must lie on one device")
         self.k, self.v, self.table, self.lengths, self.refs, self.k_scale, self.v_scale = k, v, table, lengths, refs, k_scale, v_scale
         self.layers, self.pages, self.page, self.kv_heads, self.d, self.slots, self.width = layers, pages, page, kv_heads, d, slots, width
+        if layers == 1 or pages == 1 or page == 1 or kv_heads == 1:      # (strides of an axis of one element may be anything)
+            ks, vs = ((0 if layers == 1 else st[0], 0 if pages == 1 else st[1], kv_heads * d if page == 1 else st[2], d if kv_heads == 1 else st[3]) for st in (ks, vs))
         self.desc = _pack_cache(k.data_ptr(), v.data_ptr(), table.data_ptr(), lengths.data_ptr(), 0 if refs is None else refs.data_ptr(),
                                 0 if k_scale is None else k_scale.data_ptr(), 0 if v_scale is None else v_scale.data_ptr(),
                                 layers, pages, page, kv_heads, d, slots, width, kind, ks[0], ks[1], ks[2], ks[3], vs[0], vs[1], vs[2], vs[3])
@@ -1810,32 +1812,34 @@ def _token_rows(t: torch.Tensor, width: int, name: str):
 def _rotary_call(q, k, v, heads: int, kv: int, positions, frequencies, sections, pairs: bool, out, k_out, cache, layer, slots, places, fill: int):
     lib = _lib.load()
     dt = q.dtype
-    if dt not in _TYPES or k.dtype is not dt or (v is not None and v.dtype is not dt):
+    kind = _TYPES.get(dt)
+    if kind is None or k.dtype is not dt or (v is not None and v.dtype is not dt):
         raise TypeError(f"q, k and v must have one type, bf16, fp16 or fp32, got {dt} and {k.dtype}")
     if heads < 1 or kv < 1 or q.dim() < 2 or q.shape[-1] % heads:
         raise ValueError(f"q must be [.., {heads} * d], got {tuple(q.shape)}")
-    d = q.shape[-1] // heads
-    rows, ldq = _token_rows(q, heads * d, "q")
+    wide = q.shape[-1]
+    d = wide // heads
+    rows, ldq = _token_rows(q, wide, "q")
     k_rows, ldk = _token_rows(k, kv * d, "k")
-    v_rows, ldv = (rows, 0) if v is None else _token_rows(v, kv * d, "v")
-    o_rows, ldo = _token_rows(out, heads * d, "out")
-    ko_rows, ldko = (rows, 0) if k_out is None else _token_rows(k_out, kv * d, "k_out")
-    if k_rows != rows or v_rows != rows or o_rows != rows or ko_rows != rows:
+    o_rows, ldo = _token_rows(out, wide, "out") if not fill else (rows, wide)
+    x_rows, ldx = _token_rows(k_out if v is None else v, kv * d, "k_out" if v is None else "v")
+    if k_rows != rows or o_rows != rows or x_rows != rows:
         raise ValueError("q, k, v and the outputs must have the same rows")
-    if out.dtype is not dt or (k_out is not None and k_out.dtype is not dt):
+    if out.dtype is not dt or (v is None and k_out.dtype is not dt):
         raise TypeError(f"outputs must be {dt}")
     ends, axes, n = _section_ends(sections)
     if 2 * n > d:
         raise ValueError(f"{n} pairs in heads of {d}")
-    position_type = 0
+    position_type, at = 0, None
     if positions is not None:
         position_type = _POSITION_TYPES.get(positions.dtype)
         if position_type is None:
             raise TypeError(f"positions must be int32, int64 or float32, got {positions.dtype}")
         ps = positions.shape
-        if positions.numel() != rows * axes or not positions.is_contiguous() or (axes > 1 and ps[-1] != axes):
+        if positions.numel() != rows * axes or (axes > 1 and ps[-1] != axes) or not positions.is_contiguous():
             raise ValueError(f"positions must be contiguous [{rows}, {axes}], got {tuple(ps)}")
-    flags = bool(pairs) | fill << 1
+        at = positions.data_ptr()
+    flags, steps = bool(pairs) | fill << 1, None
     if frequencies is not None:
         ft = frequencies.dtype
         if ft is torch.float32:
@@ -1844,13 +1848,19 @@ def _rotary_call(q, k, v, heads: int, kv: int, positions, frequencies, sections,
             raise TypeError(f"frequencies must be float64 or float32, got {ft}")
         if frequencies.shape != (n,) or not frequencies.is_contiguous():
             raise ValueError(f"frequencies must be contiguous [{n}], got {tuple(frequencies.shape)}")
+        steps = frequencies.data_ptr()
     elif n:
         raise ValueError("sections without frequencies")
-    if rows:
-        rc = lib.kh_rotary(q.data_ptr(), k.data_ptr(), _ptr(v), out.data_ptr(), _ptr(k_out), _ptr(positions), position_type, _ptr(frequencies), ends, axes,
-                           None if cache is None else cache.desc, layer, _ptr(slots), _ptr(places), rows, heads, kv, d, ldq, ldk, ldv, ldo, ldko, flags, _TYPES[dt], _stream())
-        if rc:
-            _lib.check(rc, "kh_rotary")
+    if not rows:
+        return
+    if cache is None:
+        rc = lib.kh_rotary(q.data_ptr(), k.data_ptr(), None, out.data_ptr(), k_out.data_ptr(), at, position_type, steps, ends, axes, None, 0, None, None,
+                           rows, heads, kv, d, ldq, ldk, 0, ldo, ldx, flags, kind, _stream())
+    else:
+        rc = lib.kh_rotary(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None, at, position_type, steps, ends, axes, cache.desc, layer,
+                           _ptr(slots), _ptr(places), rows, heads, kv, d, ldq, ldk, ldx, ldo, 0, flags, kind, _stream())
+    if rc:
+        _lib.check(rc, "kh_rotary")
 
 
 def rotary(q: torch.Tensor, k: torch.Tensor, heads: int, positions: torch.Tensor, frequencies: torch.Tensor, sections: Optional[Sequence[int]] = None,

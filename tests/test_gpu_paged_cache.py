@@ -663,3 +663,38 @@ def test_rows_by_the_hundred():
     ref, off = attention_reference(q, pages, heads, slots.clamp(min=0), torch.where(slots < 0, 0, pages.held[slots.clamp(min=0).long()]))
     got = ops.paged_attention(q.to(DEV), pages.dev, heads, slots=slots.to(DEV))
     assert_within(got.view(rows, heads, d), ref, HALF[BF] * ref.abs() + off, "rows")
+
+
+@pytest.mark.parametrize("dtype", [BF, FP16])
+def test_codes_are_the_nearest_ones(dtype):
+    """Every number of 16 bits, written as an 8-bit code: the nearest, halves to even, at most 448, as torch rounds."""
+    from katz_amd import ops
+
+    every = torch.arange(-32768, 32768, dtype=torch.int32).to(torch.int16).view(dtype)
+    x = every.view(256, 256).to(DEV)
+    cache = ops.PagedCache.empty(1, 16, 16, 1, 256, 1, 16, E4M3, DEV)
+    ops.cache_extend(cache, int32([256]))
+    rows = dict(slots=int32([0] * 256), places=int32(list(range(256))))
+    ops.cache_append(x, x, x, cache, 1, **rows)
+    want = every.float().clamp(-448, 448).to(E4M3)
+    order = cache.table[0].long().cpu()
+    for pool in (cache.k, cache.v):
+        got = pool[0].cpu().view(torch.uint8)[order].view(-1)
+        nan = torch.isnan(every)
+        assert torch.equal(got[~nan], want.view(torch.uint8)[~nan]) and (got[nan] & 127 == 127).all()
+
+
+def test_axes_of_one_element_have_any_stride():
+    from katz_amd import ops
+
+    g = gen(29)
+    base = torch.zeros(3, 1, 16, 1, 72, dtype=BF, device=DEV)[:, :, :, :, :64]
+    k, v = (base.as_strided((1, 1, 16, 1, 64), (5, 3, 72, 1 << 33, 1), o) for o in (0, 72 * 16))
+    k[0, 0, :9, 0], v[0, 0, :9, 0] = randn(g, 9, 64).to(DEV), randn(g, 9, 64).to(DEV)
+    cache = ops.PagedCache(k, v, int32([[0, -1]]), int32([9]), int32([1]))
+    pages = Pages.__new__(Pages)
+    pages.page, pages.ks, pages.vs, pages.table, pages.k, pages.v = 16, None, None, cache.table.cpu(), k.cpu(), v.cpu()
+    q = randn(g, 1, 128)
+    ref, off = attention_reference(q, pages, 2, [0], [9])
+    assert_within(ops.paged_attention(q.to(DEV), cache, 2).view(1, 2, 64), ref, HALF[BF] * ref.abs() + off, "one page")
+    assert ops.cache_reorder(cache, int32([0])).item() == 0 and ops.cache_compact(cache).item() == 1

@@ -48,6 +48,8 @@ def test_rotary_entry_point(lib):
     assert call(ldq=255) == -1 and call(ldk=100) == -1 and call(ldqo=8) == -1 and call(ldko=8) == -1
     assert call(q=17) == -3 and call(q=18, t=2) == -3 and call(pos=18) == -3 and call(pos=20, pt=1) == -3 and call(freq=20) == -3 and call(ko=17) == -3
     assert call(d=1026, ldq=1 << 13, ldk=1 << 13, ldqo=1 << 13, ldko=1 << 13) == -2 and call(rows=1 << 31) == -4
+    assert call(rows=1 << 30) == -4 and call(rows=1 << 24, d=1024, ends=(512,), ldq=1 << 12, ldk=1 << 11, ldqo=1 << 12, ldko=1 << 11) == -4    # more than 2^32 threads
+    assert call(H=1 << 19, ldq=1 << 25, ldqo=1 << 25) == -4
     held = cache()
     into = dict(c=held, v=16, ldv=128, ko=None, ldko=0)
     assert call(**{**into, "v": None}) == -1 and call(**into, layer=2) == -1 and call(**into, layer=-1) == -1 and call(**into, rows=5) == -1 and call(**{**into, "ldv": 64}) == -1
@@ -80,6 +82,7 @@ def test_entry_points_of_the_pages(lib):
         assert call(a=18) == -3 and call(t=17) == -3 and call(w=8) == -3
     assert lib.kh_cache_compact(cache(), None, 16, None) == -1 and lib.kh_cache_compact(cache(), 16, None, None) == -1 and lib.kh_cache_compact(cache(refs=0), 16, 16, None) == -1
     assert lib.kh_cache_compact(cache(), 18, 16, None) == -3 and lib.kh_cache_compact(cache(), 16, 24, None) == -3
+    assert lib.kh_cache_reorder(cache(slots=65537), 16, 16, 16, None) == -4
     size = lib.kh_cache_workspace_bytes
     assert size(0, 1, 1) == -1 and size(1, 0, 1) == -1 and size(1, 1, 0) == -1 and size(1 << 21, 1, 1) == -4 and size(1 << 16, 1 << 15, 9) == -4 and size(1, 1, 1) > 0
     slots, width, pages = 5, 7, 11                              # rows, three numbers and a copy a slot, three numbers and a copy a page, a count
