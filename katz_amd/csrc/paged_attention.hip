@@ -655,10 +655,11 @@ __global__ __launch_bounds__(JT) void join_many(const PagedParams p, const int G
 // `many`: parts of a unit, about the workgroups by the units, are more than a wave joins in passing.
 struct Plan { long workgroups; bool parts, many; };
 
-Plan plan_of(int64_t rows, int64_t kv_heads, int64_t group, int64_t d, int64_t span, bool codes) {
+Plan plan_of(int64_t rows, int64_t kv_heads, int64_t group, int64_t d, int64_t span, int64_t window, bool codes) {
+  if (window > 0 && window + TILE - 1 < span) span = window + TILE - 1;          // (wherever it begins in a tile)
   const long tiles = (span + TILE - 1) / TILE, units = rows * kv_heads * ((group + QB - 1) / QB);
-  const long at_once = 256 * wgs_a_cu((int)d, codes);
-  return Plan{units * tiles < at_once ? units * tiles : at_once, tiles > 1, units * 32 < at_once};
+  const long at_once = 256 * wgs_a_cu((int)d, codes), n = units * tiles < at_once ? units * tiles : at_once;
+  return Plan{n, tiles > 1, units * 32 < n};
 }
 
 // whether all tiles can be counted in 31 bits
@@ -706,7 +707,7 @@ KH_EXPORT int64_t kh_paged_attention_workspace_bytes(int64_t rows, int64_t heads
   if (d % 8 != 0 || d > 256) return KH_ERR_UNSUPPORTED;
   if (rows > (1L << 24) || heads > (1L << 16) || span > (1L << 30)) return KH_ERR_TOO_LARGE;
   if (!line_fits(rows, kv_heads, heads / kv_heads, span)) return KH_ERR_TOO_LARGE;
-  return bytes_of(plan_of(rows, kv_heads, heads / kv_heads, d, span, true), heads / kv_heads, d);   // (e4m3 has no fewer workgroups)
+  return bytes_of(plan_of(rows, kv_heads, heads / kv_heads, d, span, 0, true), heads / kv_heads, d);   // (nothing has more workgroups than e4m3 without a window)
 }
 
 KH_EXPORT int kh_paged_attention(const void* q, void* o, const KhPagedCache* cache, int64_t layer, const int32_t* slots, const int32_t* lengths,
@@ -722,7 +723,7 @@ KH_EXPORT int kh_paged_attention(const void* q, void* o, const KhPagedCache* cac
   if (rows > (1L << 24) || heads > (1L << 16)) return KH_ERR_TOO_LARGE;
   const long group = heads / c.kv_heads, e = kh_cache_element(c);
   if (!line_fits(rows, c.kv_heads, group, c.width * c.page)) return KH_ERR_TOO_LARGE;
-  const Plan plan = plan_of(rows, c.kv_heads, group, c.d, c.width * c.page, c.type == KH_E4M3);
+  const Plan plan = plan_of(rows, c.kv_heads, group, c.d, c.width * c.page, window, c.type == KH_E4M3);
   if (plan.parts && !workspace) return KH_ERR_INVALID_ARG;
   PagedParams p{q, (const char*)c.k + layer * c.k_layer * e, (const char*)c.v + layer * c.v_layer * e, o, c.table, lengths, c.lengths, slots,
                 c.k_scale ? c.k_scale + layer * c.kv_heads : nullptr, c.v_scale ? c.v_scale + layer * c.kv_heads : nullptr,
