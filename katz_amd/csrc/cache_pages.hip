@@ -5,7 +5,8 @@
 // refs once, in order, as far as it has to.  Only the copies need the whole chip: they take their list from memory, since how many there are is not
 // known to the host.
 //
-// Bound by the launches and the memory's latency for a few sequences, by the copies' bytes for many layers.
+// Bound by the launches and the memory's latency for a few sequences, by the copies' bytes for many layers.  us: three beams forked from 77 tokens, 2 layers, 6.7 + 3.9, then
+// their next tokens 4.0; 48 of 8 sequences, 24 layers, 4.4 + 5.2 + 24.6 (171 MB in and out), 6.2; 490 of 2048 pages moved in 4 layers 8.0 + 102 (515 MB, 5.0 TB/s).
 #include "paged_cache.h"
 
 namespace {
