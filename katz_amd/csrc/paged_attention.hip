@@ -12,9 +12,10 @@
 // The tokens of the keys' rows are chosen so that the scores a lane gets (query l % 16, eight tokens) are the P operand it needs: nothing crosses lanes but the
 // maximum.  Neither operand goes through LDS.  P is multiplied in all 24 bits: in three pieces of bf16 or two of fp16, since the matrix unit waits for memory anyway.
 //
-// us a launch (GB/s of keys and values): one token of 64 requests of 0 .. 8192 tokens, 32 heads of 128 on 8, bf16, 123 (5430) and 3.9 for the join; one of 131071 tokens, 16 heads on 2, 29.5 (4550) and
-// 4.5; 32 of 4096 with 4 KB a token, heads of 64, 128, 256: 94, 96, 86 (5.7, 5.6, 6.2 TB/s); 2 x 77 tokens 5.6, of which the chain of lengths, page numbers and first
-// rows is 4.  A copy of 1 GiB runs at 5146 GB/s.  With each step's loads waited for where they are used: 207 and 55.
+// us a launch (TB/s of keys and values): one token of 64 requests of 0 .. 8192 tokens, 32 heads of 128 on 8, bf16, 118 (5.6) and 3.9 for the join; one of 131071 tokens, 16 heads on 2, 25.6 (5.2)
+// and 4.6; 32 of 4096 tokens with 4 KB a token, heads of 64, 128, 256: 93, 91, 85 (5.8, 5.9, 6.3), with 2 KB in e4m3 87, 53, 63; 2 x 77 tokens 5.6, of which the chain of lengths,
+// page numbers and first rows is 4.  A copy of 1 GiB runs at 5.1 TB/s.  With each step's loads waited for where they are used: 207 and 55.  Values are read past
+// the caches (126 us where that is 119), keys are not (123, and the two halves of a line that a wave asks for one after the other are both there: e4m3 78 -> 59).
 #include "paged_cache.h"
 #include <type_traits>
 
@@ -45,7 +46,6 @@ struct PagedParams {
 typedef uint32_t u32x1 __attribute__((ext_vector_type(1)));
 typedef _Float16 f16_t;
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 template <typename T> struct Eight;
 template <> struct Eight<bf16_t> { using type = bf16x8; };
@@ -122,7 +122,16 @@ template <> struct Pieces<f16_t> {
 
 // a value that all lanes have, in scalar registers
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ long uniform(long v) { return (long)((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32 | (uint32_t)uniform((int)v)); }
+
+// the thread's number as something the compiler does not know: what is worked out from it stays where it is used, instead of in registers across the loop of the
+// steps (heads of 128: 232 of them and 219 so, in e4m3 spills and none: 32 sequences of 4096 tokens 59 -> 53 us)
+__device__ __forceinline__ int thread_here() {
+  int t = threadIdx.x;
+#if __HIP_DEVICE_COMPILE__
+  asm volatile("" : "+v"(t));
+#endif
+  return t;
+}
 
 // A row's sequence: its slot (-1: none), the tokens low .. n - 1 to attend to; `tiles` tiles of 128 from `tile` on.
 struct Row { int slot, n, low, tile, tiles; };
@@ -209,7 +218,7 @@ struct Wave {
       for (int kk = 0; kk < S::KK; ++kk) {
         const int dim = kk * 32 + g4 * 8;
         if (TAIL && kk * 32 >= p.d) kr[s][kk] = typename S::Raw{};
-        else kr[s][kk] = __builtin_nontemporal_load(reinterpret_cast<const typename S::Raw*>(at[s] + (!TAIL || dim < p.d ? dim : 0) * S::ELT));
+        else kr[s][kk] = *reinterpret_cast<const typename S::Raw*>(at[s] + (!TAIL || dim < p.d ? dim : 0) * S::ELT);
       }
   }
   __device__ __forceinline__ void load_values(const PagedParams& p, const Row& row, const char* vb, const Pages& e, int t0) {
@@ -228,7 +237,7 @@ struct Wave {
 
   // Requests the first step of a piece (and its queries): the tokens t0, t0 + TILE, .. of its row, `steps` times 32, of which low .. n - 1 count.
   __device__ __forceinline__ void begin(const PagedParams& p, const Piece& u, int wave) {
-    const int c16 = threadIdx.x & 15, g4 = (threadIdx.x & 63) >> 4;
+    const int c16 = thread_here() & 15, g4 = thread_here() >> 4 & 3;
     t0 = (u.row.tile + u.at - u.a) * TILE + wave * STEP;
     steps = u.stop - u.at;
     if (t0 + (steps - 1) * TILE >= u.row.n) --steps;     // (only the last tile may begin behind the end for some waves,
@@ -369,9 +378,9 @@ __device__ __forceinline__ void zero_row(const PagedParams& p, int r) {
   for (int i = threadIdx.x; i < p.kv_heads * p.group * p.d; i += NW * 64) to[i] = (T)0.f;
 }
 
-// Workgroups a CU, by what registers allow without spilling in the loop.  32 sequences of 4096 tokens, 4096 bytes of keys and values a token in 16 bits: heads of
-// 128 97 us with two (three spill: 131 -> 179 where 64 requests took 123 with two), of 64 94 with three, of 256 85 with one; in e4m3, whose steps have half the
-// bytes, of 128 84 us with two and 68 with three, of 64 93 with three and 119 with four, of 256 72 with one and 70 with two.
+// Workgroups a CU, by what registers allow without spilling in the loop.  us of 32 sequences of 4096 tokens, 4096 bytes of keys and values a token in 16 bits: heads of
+// 128 91 with two (three spill: 64 requests took 179 with three and 123 with two), of 64 93 with three (116 with four), of 256 85 with one; in e4m3, whose steps have
+// half the bytes, of 128 84 with two and 68 with three (53 since), of 64 85 with three and 104 with four, of 256 72 with one and 63 with two.
 constexpr int wgs_a_cu(int D, bool codes) { return D > 128 ? (codes ? 2 : 1) : D > 64 && !codes ? 2 : 3; }
 
 template <int D, typename T, bool CODES, bool EIGHT, bool TAIL>
@@ -382,7 +391,7 @@ __global__ __launch_bounds__(NW * 64, wgs_a_cu(D, CODES)) void attend(const Page
   float* const ms = lds + NW * QB * OW;
   __shared__ int starts[NW];
   __shared__ int where[4];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c16 = lane & 15, g4 = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int units = p.kv_heads * p.blocks, G = gridDim.x, w = blockIdx.x;
 
   // the line of tiles: all of them, and the row in which this workgroup's part begins
@@ -397,6 +406,7 @@ __global__ __launch_bounds__(NW * 64, wgs_a_cu(D, CODES)) void attend(const Page
     if (lane >= s) before += y;
   }
   if (lane == 63) starts[wave] = before;
+  if (tid < 4) where[tid] = tid == 2 ? -1 : 0;
   __syncthreads();
   int total = 0;
   before -= mine;
@@ -423,12 +433,14 @@ __global__ __launch_bounds__(NW * 64, wgs_a_cu(D, CODES)) void attend(const Page
       at_row = next;
     }
     __syncthreads();
-    // the piece from `at` on in the line; false: none
+    // the piece from `at` on in the line; false: none (nor behind the last row, should somebody write to the lengths meanwhile)
     auto advance = [&](Piece& u, int at) {
       if (at >= end) return false;
       while (at >= u.row_at + u.row.tiles * units) {
+        if (++u.r >= p.rows) return false;
         u.row_at += u.row.tiles * units;
-        u.row = row_of(p, ++u.r);
+        const Row x = row_of(p, u.r);
+        u.row = row_of(p, uniform(x.slot), uniform(x.n));
       }
       u.unit = (at - u.row_at) / u.row.tiles;
       u.head = u.unit / p.blocks;
@@ -452,6 +464,7 @@ __global__ __launch_bounds__(NW * 64, wgs_a_cu(D, CODES)) void attend(const Page
       if (more) wv.begin(p, u, wave);                   // (on its way while the waves' parts of the piece before it are put together)
       if (some) {
         // the waves' parts together
+        const int tid = thread_here(), c16 = tid & 15, g4 = tid >> 4 & 3;
         float sum = wv.l;
         sum += __shfl_xor(sum, 16, 64);
         sum += __shfl_xor(sum, 32, 64);

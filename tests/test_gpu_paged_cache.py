@@ -698,3 +698,47 @@ def test_axes_of_one_element_have_any_stride():
     ref, off = attention_reference(q, pages, 2, [0], [9])
     assert_within(ops.paged_attention(q.to(DEV), cache, 2).view(1, 2, 64), ref, HALF[BF] * ref.abs() + off, "one page")
     assert ops.cache_reorder(cache, int32([0])).item() == 0 and ops.cache_compact(cache).item() == 1
+
+
+@pytest.mark.parametrize("dtype", [BF, FP16])
+@pytest.mark.parametrize("n", [2, 64, 1500])
+def test_weights_that_no_type_of_16_bits_holds(dtype, n):
+    """As above, weights 1 and exp(-0.00137), which is 2^-12 off in 11 bits: a fifth of the result."""
+    from katz_amd import ops
+
+    d, step = 64, 0.00137
+    pages = Pages(30, [n], 16, 1, d, dtype)
+    first = torch.arange(n) < n // 2
+    for t in range(n):
+        e, at = pages.table[0, t // 16], t % 16
+        pages.k[0, e, at] = 0
+        pages.k[0, e, at, 0, 0] = 0.0 if first[t] else -1.0
+        pages.v[0, e, at] = 1.0 if first[t] else -1.0
+    pages.dev.k.copy_(pages.k)
+    pages.dev.v.copy_(pages.v)
+    q = torch.zeros(1, d, dtype=dtype)
+    q[0, 0] = 1.0
+    ref, _ = attention_reference(q, pages, 1, [0], [n], scale=step)
+    got = ops.paged_attention(q.to(DEV), pages.dev, 1, scale=step)
+    assert_within(got.view(1, 1, d), ref, HALF[dtype] * ref.abs() + 4 * U + 2 * (n / 4 + 64) * U, "weights")
+
+
+def test_the_smallest_numbers_of_fp16():
+    """Keys, queries and values below fp16's normal numbers are numbers: none is taken as zero."""
+    from katz_amd import ops
+
+    g, heads, d, n = gen(31), 4, 64, 200
+    pages = Pages(32, [n, n], 16, 2, d, FP16)
+    pages.v[:] = pages.v * 2.0 ** -18
+    pages.k[:] = torch.where(torch.arange(d) < 32, pages.k * 2.0 ** -16, pages.k)
+    pages.dev.k.copy_(pages.k)
+    pages.dev.v.copy_(pages.v)
+    q = randn(g, 2, heads * d, dtype=FP16).view(2, heads, d)
+    q[..., 32:] = q[..., 32:] * 2.0 ** -17
+    q = q.reshape(2, heads * d)
+    # (scores of 2^-13 or so, scaled up to some ones: a subnormal key or query taken as zero would change them all)
+    ref, off = attention_reference(q, pages, heads, range(2), [n] * 2, scale=2.0 ** 13)
+    got = ops.paged_attention(q.to(DEV), pages.dev, heads, scale=2.0 ** 13)
+    assert_within(got.view(2, heads, d), ref, HALF[FP16] * ref.abs() + off + TINY[FP16], "small numbers")
+    big, more = attention_reference(q, pages, heads, range(2), [n] * 2, scale=2.0 ** 13)
+    assert (big.abs().max() > 2.0 ** -20) and (got.abs().max().item() > 0)
