@@ -13,8 +13,8 @@
 // maximum.  Neither operand goes through LDS.  P is multiplied in all 24 bits: in three pieces of bf16 or two of fp16, since the matrix unit waits for memory anyway.
 //
 // us a launch (TB/s of keys and values): one token of 64 requests of 0 .. 8192 tokens, 32 heads of 128 on 8, bf16, 118 (5.6) and 3.9 for the join; one of 131071 tokens, 16 heads on 2, 25.6 (5.2)
-// and 4.6; 32 of 4096 tokens with 4 KB a token, heads of 64, 128, 256: 93, 91, 85 (5.8, 5.9, 6.3), with 2 KB in e4m3 87, 53, 63; 2 x 77 tokens 5.6, of which the chain of lengths,
-// page numbers and first rows is 4.  A copy of 1 GiB runs at 5.1 TB/s.  With each step's loads waited for where they are used: 207 and 55.  Values are read past
+// and 4.6; 32 of 4096 tokens with 4 KB a token, heads of 64, 128, 256: 93, 91, 85 (5.8, 5.9, 6.3), with 2 KB in e4m3 87, 53, 63; 2 x 77 tokens 4.7, a chain of lengths,
+// page numbers and rows.  A copy of 1 GiB runs at 5.1 TB/s.  With each step's loads waited for where they are used: 207 and 55.  Values are read past
 // the caches (126 us where that is 119), keys are not (123, and the two halves of a line that a wave asks for one after the other are both there: e4m3 78 -> 59).
 #include "paged_cache.h"
 #include <type_traits>
@@ -23,7 +23,8 @@ namespace {
 
 constexpr int NW = 4, STEP = 32, TILE = NW * STEP;       // waves, tokens of a wave's step, of a tile
 constexpr int QB = 16;                                  // query heads of a unit
-constexpr int JT = 512, MOST = 1024;                    // threads that join, workgroups at most
+constexpr int JT = 512, MOST = 1024;                    // threads that join, workgroups at most that share the line
+constexpr int WHOLE = 4;                                // tiles of a unit that is not cut
 constexpr float RESCALE_LOG2 = 8.0f;                    // the running maximum moves only for jumps above 2^8
 
 struct PagedParams {
@@ -40,6 +41,7 @@ struct PagedParams {
   int n_slots, width, pages, page, window;
   float scale_log2;
   int fill, q_aligned;
+  int whole;                  // every workgroup has a unit, and no unit parts
   int shared_lines;           // neighbouring key heads share lines of 128 bytes: neighbouring parts of the line of tiles on one XCD, whose L2 then has them
   KhDivide by_page;
 };
@@ -395,45 +397,64 @@ __global__ __launch_bounds__(NW * 64, wgs_a_cu(D, CODES)) void attend(const Page
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int units = p.kv_heads * p.blocks, G = gridDim.x, w = p.shared_lines ? (int)xcd_remap(blockIdx.x, gridDim.x) : (int)blockIdx.x;
 
-  // the line of tiles: all of them, and the row in which this workgroup's part begins
-  const int each = (p.rows + NW * 64 - 1) / (NW * 64), r0 = tid * each, r1 = r0 + each < p.rows ? r0 + each : p.rows;
-  Row one{};
-  int mine = 0;
-  for (int r = r0; r < r1; ++r) mine += (one = row_of(p, r)).tiles;
-  int before = mine;
+  int total = 0, W = G, begin, end;
+  Piece u;
+  bool active;
+  if (p.whole) {                                        // a unit each
+    u.r = w / units;
+    const Row x = row_of(p, u.r);
+    u.row = row_of(p, uniform(x.slot), uniform(x.n));
+    u.row_at = 0;
+    begin = (w - u.r * units) * u.row.tiles;
+    end = begin + u.row.tiles;
+    active = u.row.tiles > 0;
+  } else {
+    // the line of tiles: all of them, and the row in which this workgroup's part begins
+    const int each = (p.rows + NW * 64 - 1) / (NW * 64), r0 = tid * each, r1 = r0 + each < p.rows ? r0 + each : p.rows;
+    Row one{};
+    int mine = 0;
+    for (int r = r0; r < r1; ++r) mine += (one = row_of(p, r)).tiles;
+    int before = mine;
 #pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    const int y = __shfl_up(before, s, 64);
-    if (lane >= s) before += y;
-  }
-  if (lane == 63) starts[wave] = before;
-  if (tid < 4) where[tid] = tid == 2 ? -1 : 0;
-  __syncthreads();
-  int total = 0;
-  before -= mine;
-#pragma unroll
-  for (int i = 0; i < NW; ++i) {
-    if (i < wave) before += starts[i];
-    total += starts[i];
-  }
-  total = uniform(total) * units;
-  const int W = total < G ? total : G;                  // workgroups that have a tile
-  if (tid == 0 && p.border) p.border[w] = int4{-1, 0, 0, 0};
-  if (w < W) {
-    const int begin = (int)((long)total * w / W), end = (int)((long)total * (w + 1) / W);
-    int at_row = before * units;                        // where row r begins
-    for (int r = r0; r < r1; ++r) {
-      if (each > 1) one = row_of(p, r);
-      const int next = at_row + one.tiles * units;
-      if (begin >= at_row && begin < next) {
-        where[0] = r;
-        where[1] = at_row;
-        where[2] = one.slot;
-        where[3] = one.n;
-      }
-      at_row = next;
+    for (int s = 1; s < 64; s <<= 1) {
+      const int y = __shfl_up(before, s, 64);
+      if (lane >= s) before += y;
     }
+    if (lane == 63) starts[wave] = before;
+    if (tid < 4) where[tid] = tid == 2 ? -1 : 0;
     __syncthreads();
+    before -= mine;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      if (i < wave) before += starts[i];
+      total += starts[i];
+    }
+    total = uniform(total) * units;
+    W = total < G ? total : G;                          // workgroups that have a tile
+    if (tid == 0) p.border[w] = int4{-1, 0, 0, 0};
+    active = w < W;
+    begin = active ? (int)((long)total * w / W) : 0;
+    end = active ? (int)((long)total * (w + 1) / W) : 0;
+    if (active) {
+      int at_row = before * units;                      // where row r begins
+      for (int r = r0; r < r1; ++r) {
+        if (each > 1) one = row_of(p, r);
+        const int next = at_row + one.tiles * units;
+        if (begin >= at_row && begin < next) {
+          where[0] = r;
+          where[1] = at_row;
+          where[2] = one.slot;
+          where[3] = one.n;
+        }
+        at_row = next;
+      }
+      __syncthreads();
+      u.r = uniform(where[0]);
+      u.row_at = uniform(where[1]);
+      u.row = row_of(p, uniform(where[2]), uniform(where[3]));
+    }
+  }
+  if (active) {
     // the piece from `at` on in the line; false: none (nor behind the last row, should somebody write to the lengths meanwhile)
     auto advance = [&](Piece& u, int at) {
       if (at >= end) return false;
@@ -453,10 +474,6 @@ __global__ __launch_bounds__(NW * 64, wgs_a_cu(D, CODES)) void attend(const Page
       u.stop = u.b < end ? u.b : end;
       return true;
     };
-    Piece u;
-    u.r = uniform(where[0]);
-    u.row_at = uniform(where[1]);
-    u.row = row_of(p, uniform(where[2]), uniform(where[3]));
     Wave<D, T, CODES, EIGHT, TAIL> wv;
     Piece done;
     int at = begin;
@@ -670,6 +687,8 @@ __global__ __launch_bounds__(JT) void join_many(const PagedParams p, const int G
 }
 
 // Workgroups: as many as run at once (D 256: one a CU), but no more than there can be tiles.
+// Where units have at most WHOLE tiles, a workgroup has one: 4 sequences of 300 tokens on 8 key heads 8.9 us where line and join take 7.4 + 4.0, of 470 10.5 and 7.5 + 4.0, 256 of 300
+// 61.5 and 57.8 + 3.9 (and 3 of the host's for the second launch).
 // `many`: parts of a unit, about the workgroups by the units, are more than a wave joins in passing.
 struct Plan { long workgroups; bool parts, many; };
 
@@ -677,7 +696,8 @@ Plan plan_of(int64_t rows, int64_t kv_heads, int64_t group, int64_t d, int64_t s
   if (window > 0 && window + TILE - 1 < span) span = window + TILE - 1;          // (wherever it begins in a tile)
   const long tiles = (span + TILE - 1) / TILE, units = rows * kv_heads * ((group + QB - 1) / QB);
   const long at_once = 256 * wgs_a_cu((int)d, codes), n = units * tiles < at_once ? units * tiles : at_once;
-  return Plan{n, tiles > 1, units * 32 < n};
+  if (tiles <= WHOLE && units <= 1 << 20) return Plan{units, false, false};
+  return Plan{n, true, units * 32 < n};
 }
 
 // whether all tiles can be counted in 31 bits
@@ -686,7 +706,7 @@ bool line_fits(int64_t rows, int64_t kv_heads, int64_t group, int64_t span) {
 }
 
 int64_t bytes_of(const Plan& plan, int64_t group, int64_t d) {
-  if (!plan.parts) return 0;                            // (every unit is one tile)
+  if (!plan.parts) return 0;
   const int64_t q = group < QB ? group : QB;
   return plan.workgroups * 16 + 2 * plan.workgroups * q * (d + 2) * 4;
 }
@@ -748,7 +768,7 @@ KH_EXPORT int kh_paged_attention(const void* q, void* o, const KhPagedCache* cac
                 plan.parts ? (float*)((char*)workspace + plan.workgroups * 16) : nullptr, plan.parts ? (int4*)workspace : nullptr, ldq, ldo, (uint32_t)(c.k_page * e), (uint32_t)(c.k_token * e), (uint32_t)(c.v_page * e),
                 (uint32_t)(c.v_token * e), c.k_head * e, c.v_head * e,
                 (int)rows, (int)c.kv_heads, (int)group, (int)((group + QB - 1) / QB), (int)c.d, (int)c.slots, (int)c.width, (int)c.pages, (int)c.page,
-                (int)(window < (1L << 30) ? window : 0), scale * 1.4426950408889634f, flags & 1, 0, 0, KhDivide((uint32_t)c.page)};
+                (int)(window < (1L << 30) ? window : 0), scale * 1.4426950408889634f, flags & 1, 0, !plan.parts, 0, KhDivide((uint32_t)c.page)};
   // (32 sequences of 4096 tokens, 8 heads of 80 and 96 in bf16: 82 -> 77 us and 84 -> 76; heads of whole lines 91 -> 94)
   p.shared_lines = c.kv_heads > 1 && c.k_head * e % 128 != 0;
   p.q_aligned = kh_aligned16(q) && ldq % 8 == 0;

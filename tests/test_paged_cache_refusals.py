@@ -70,9 +70,9 @@ def test_attention_entry_point(lib):
     assert lib.kh_paged_attention(16, 16, None, 0, None, None, 16, 2, 4, 256, 256, 0, 0.1, 0, 0, None) == -1
     size = lib.kh_paged_attention_workspace_bytes
     assert size(0, 4, 2, 64, 80) == -1 and size(2, 3, 2, 64, 80) == -1 and size(2, 4, 0, 64, 80) == -1 and size(2, 4, 2, 64, 0) == -1 and size(2, 4, 2, 60, 80) == -2 and size(2, 4, 2, 264, 80) == -2
-    assert call(ws=None, c=cache(width=9)) == -1                # a sequence may have more than one tile: there are parts to be joined
+    assert call(ws=None, c=cache(width=40)) == -1               # sequences of more than four tiles may be cut: there are parts to be joined
     assert size(1 << 25, 4, 2, 64, 80) == -4 and size(2, 4, 2, 64, 1 << 31) == -4 and size(1 << 20, 1 << 10, 1 << 10, 64, 1 << 20) == -4
-    assert size(1, 1, 1, 8, 1) == 0 and size(64, 4, 2, 64, 128) == 0 and size(1, 1, 1, 8, 129) > 0
+    assert size(1, 1, 1, 8, 1) == 0 and size(64, 4, 2, 64, 512) == 0 and size(1, 1, 1, 8, 513) > 0
     assert size(1, 8, 1, 128, 1 << 20) < 1 << 25                # a workgroup's parts, however long the cache
 
 
