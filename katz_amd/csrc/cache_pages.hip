@@ -5,8 +5,8 @@
 // refs once, in order, as far as it has to.  Only the copies need the whole chip: they take their list from memory, since how many there are is not
 // known to the host.
 //
-// Bound by the launches and the memory's latency for a few sequences, by the copies' bytes for many layers.  us: three beams forked from 77 tokens, 2 layers, 6.7 + 3.9, then
-// their next tokens 4.0; 48 of 8 sequences, 24 layers, 4.4 + 5.2 + 24.6 (171 MB in and out), 6.2; 490 of 2048 pages moved in 4 layers 8.0 + 102 (515 MB, 5.0 TB/s).
+// Bound by the launches and the memory's latency for a few sequences, by the copies' bytes for many layers.  us: three beams forked from 77 tokens, 2 layers, 5.7 + 3.9, then
+// their next tokens 3.8; 48 of 8 sequences, 24 layers, 4.5 + 4.4 + 20.2 (171 MB in and out), 5.4; 490 of 2048 pages moved in 4 layers 6.0 + 96 (515 MB, 5.4 TB/s).
 #include "paged_cache.h"
 
 namespace {
@@ -80,17 +80,33 @@ __device__ __forceinline__ int prefix(int v, int* total, int* red) {
   return before + x - v;
 }
 
+constexpr int EACH = 16;                                // pages a thread looks at in one go
+
+// The counts of EACH pages from `at` on (1 behind the last).
+__device__ __forceinline__ void counts_of(const int32_t* refs, int pages, int at, int (&n)[EACH]) {
+  if (at + EACH <= pages && ((uintptr_t)refs & 15) == 0) {
+    int4 v[EACH / 4];
+#pragma unroll
+    for (int i = 0; i < EACH / 4; ++i) v[i] = reinterpret_cast<const int4*>(refs + at)[i];
+    __builtin_memcpy(n, v, sizeof(n));
+  } else {
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) n[i] = at + i < pages ? refs[at + i] : 1;
+  }
+}
+
 // Calls take(rank, page) for the lowest `wanted` pages without references, in order, and returns how many there were.
 template <typename F>
 __device__ int deal(const int32_t* refs, int pages, int wanted, int* red, F take) {
-  constexpr int EACH = 16;                              // pages a thread looks at in a round
   int got = 0;
   for (int base = 0; base < pages && got < wanted; base += NT * EACH) {
     const int at = base + (int)threadIdx.x * EACH;
+    int n[EACH];
+    counts_of(refs, pages, at, n);
     uint32_t free = 0;
 #pragma unroll
     for (int i = 0; i < EACH; ++i)
-      if (at + i < pages && refs[at + i] == 0) free |= 1u << i;
+      if (n[i] == 0) free |= 1u << i;
     int total;
     int rank = got + prefix(__popc(free), &total, red);
     while (free && rank < wanted) {
@@ -111,21 +127,24 @@ __device__ __forceinline__ int clamped(int n, const PagesParams& p) {
 __global__ __launch_bounds__(NT) void extend(const PagesParams p) {
   __shared__ int red[NT / 64];
   const int most = p.width * p.page;
-  int wanted = 0, over = 0;
+  // a slot's tokens, its first new page and how many
+  auto look = [&](int s, int* longer, int* first, int* need, int* too_long) {
+    const int n = clamped(p.lengths[s], p), more = p.asked[s] > 0 ? p.asked[s] : 0, fits = more < most - n ? more : most - n;
+    const long whole = ((long)n + more + p.page - 1) / p.page;
+    *longer = more > 0 ? n + fits : -1;
+    *first = (n + p.page - 1) / p.page;
+    *need = (n + fits + p.page - 1) / p.page - *first;
+    *too_long = whole > p.width ? (int)(whole - p.width) : 0;
+  };
+  int wanted = 0, over = 0, longer = -1, first = 0, need = 0, start = 0;
   for (int base = 0; base < p.slots; base += NT) {
     const int s = base + (int)threadIdx.x;
-    int need = 0, n = 0, more = 0;
-    if (s < p.slots) {
-      n = clamped(p.lengths[s], p);
-      more = p.asked[s] > 0 ? p.asked[s] : 0;
-      const int fits = more < most - n ? more : most - n;
-      need = (n + fits + p.page - 1) / p.page - (n + p.page - 1) / p.page;
-      const long whole = ((long)n + more + p.page - 1) / p.page;
-      if (whole > p.width) over += (int)(whole - p.width);
-    }
-    int total;
-    const int before = prefix(need, &total, red);
-    if (s < p.slots) p.w.start[s] = wanted + before;
+    int total, too_long = 0;
+    longer = -1, need = 0;
+    if (s < p.slots) look(s, &longer, &first, &need, &too_long);
+    over += too_long;
+    start = wanted + prefix(need, &total, red);
+    if (s < p.slots && p.slots > NT) p.w.start[s] = start;
     wanted += total;
   }
   const int got = deal(p.refs, p.pages, wanted, red, [&](int rank, int page) {
@@ -140,13 +159,16 @@ __global__ __launch_bounds__(NT) void extend(const PagesParams p) {
   constexpr int FEW = 4;
   for (int base = 0; base < p.slots; base += NT) {
     const int s = base + (int)threadIdx.x, lane = threadIdx.x & 63;
-    int first = 0, need = 0, start = 0;
-    if (s < p.slots && p.asked[s] > 0) {
-      const int more = p.asked[s], n = clamped(p.lengths[s], p), fits = more < most - n ? more : most - n;
-      first = (n + p.page - 1) / p.page;
-      need = (n + fits + p.page - 1) / p.page - first;
-      start = p.w.start[s];
-      p.lengths[s] = n + fits;
+    if (p.slots > NT) {                                 // (else it is at hand)
+      int too_long;
+      longer = -1, need = 0;
+      if (s < p.slots) {
+        look(s, &longer, &first, &need, &too_long);
+        start = p.w.start[s];
+      }
+    }
+    if (longer >= 0) {
+      p.lengths[s] = longer;
       if (need <= FEW)
         for (int i = 0; i < need; ++i) p.table[(long)s * p.width + first + i] = start + i < got ? p.w.free[start + i] : -1;
     }
@@ -238,19 +260,23 @@ __global__ __launch_bounds__(NT) void reorder_deal(const PagesParams p) {
 // The pages in use, their number n, and for those from n on the free ones below, both in order.
 __global__ __launch_bounds__(NT) void compact_plan(const PagesParams p) {
   __shared__ int red[NT / 64];
-  constexpr int EACH = 16;
-  int n = 0;
-  for (int at = threadIdx.x; at < p.pages; at += NT) n += p.refs[at] > 0;
-  int live;
-  prefix(n, &live, red);
+  int used = 0, live, count[EACH];
+  for (int base = 0; base < p.pages; base += NT * EACH) {
+    const int at = base + (int)threadIdx.x * EACH;
+    counts_of(p.refs, p.pages, at, count);
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) used += at + i < p.pages && count[i] > 0;
+  }
+  prefix(used, &live, red);
   int moves = 0, holes = 0;
   for (int base = 0; base < p.pages; base += NT * EACH) {
     const int at = base + (int)threadIdx.x * EACH;
     uint32_t hole = 0, moving = 0;
+    if (p.pages > NT * EACH) counts_of(p.refs, p.pages, at, count);     // (else they are at hand)
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
       const int e = at + i;
-      const bool there = e < p.pages, used = there && p.refs[e] > 0;
+      const bool there = e < p.pages, used = there && count[i] > 0;
       if (e < live && !used) hole |= 1u << i;
       if (there && e >= live) {
         if (used) moving |= 1u << i;
@@ -285,6 +311,8 @@ struct CopyParams {
   int packed;                  // the heads of a token and the tokens of a page lie behind one another
 };
 
+// Past the caches go what is written and, where pages move, what is read, which nobody reads again (us of 515 MB in and out: 104 with neither, 103 with the
+// stores, 96 with both and 8192 workgroups; of 171 MB copied from 8 pages a layer to 48: 24.7, 20.5, 35).
 // The rows of the list's pages, piece by piece in units of T, and beside them (the first workgroups) what the tables become.
 template <typename T, bool COMPACT>
 __global__ __launch_bounds__(NC) void carry_out(const PagesParams p, const CopyParams c, const int tables) {
@@ -317,13 +345,23 @@ __global__ __launch_bounds__(NC) void carry_out(const PagesParams p, const CopyP
     const char* from = base + what.src * page;
     char* to = base + what.dst * page;
     const int per = c.row / (int)sizeof(T), units = (last - first) * c.heads * per;
-    for (int u = threadIdx.x; u < units; u += NC) {
-      long off = (long)u * sizeof(T);
-      if (!c.packed) {
-        const int row = u / per;
-        off = row / c.heads * token + row % c.heads * head + (u - row * per) * (long)sizeof(T);
+    for (int u0 = threadIdx.x; u0 < units; u0 += 4 * NC) {              // four on their way at a time
+      T x[4];
+      long off[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int u = u0 + k * NC < units ? u0 + k * NC : u0;
+        off[k] = (long)u * sizeof(T);
+        if (!c.packed) {
+          const int row = u / per;
+          off[k] = row / c.heads * token + row % c.heads * head + (u - row * per) * (long)sizeof(T);
+        }
+        if constexpr (COMPACT) x[k] = __builtin_nontemporal_load(reinterpret_cast<const T*>(from + off[k]));
+        else x[k] = *reinterpret_cast<const T*>(from + off[k]);
       }
-      *reinterpret_cast<T*>(to + off) = *reinterpret_cast<const T*>(from + off);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (u0 + k * NC < units) __builtin_nontemporal_store(x[k], reinterpret_cast<T*>(to + off[k]));
     }
   }
 }
@@ -356,7 +394,7 @@ void copy(const KhPagedCache& c, const PagesParams& p, hipStream_t s) {
                     kh_aligned16(c.v);
   const long most = COMPACT ? c.pages / 2 : c.slots, works = most * c.layers * 2 * o.pieces;
   const int tables = COMPACT ? (int)(c.slots * c.width / 4096 < 1 ? 1 : c.slots * c.width / 4096 < 64 ? c.slots * c.width / 4096 : 64) : (int)(c.slots < 256 ? c.slots : 256);
-  const dim3 grid((unsigned)(tables + (works < 2048 ? works : 2048)));
+  const dim3 grid((unsigned)(tables + (works < 8192 ? works : 8192)));   // (2048 workgroups move 515 MB in 100 us, 4096 in 98, 8192 in 96)
   if (wide) kh_launch(KH_TAG_CACHE_PAGES, carry_out<u32x4, COMPACT>, grid, dim3(NC), 0, s, p, o, tables);
   else kh_launch(KH_TAG_CACHE_PAGES, carry_out<u32x2, COMPACT>, grid, dim3(NC), 0, s, p, o, tables);
 }

@@ -742,3 +742,33 @@ def test_the_smallest_numbers_of_fp16():
     assert_within(got.view(2, heads, d), ref, HALF[FP16] * ref.abs() + off + TINY[FP16], "small numbers")
     big, more = attention_reference(q, pages, heads, range(2), [n] * 2, scale=2.0 ** 13)
     assert (big.abs().max() > 2.0 ** -20) and (got.abs().max().item() > 0)
+
+
+@pytest.mark.parametrize("slots,page,longest,spare,shift", [(1500, 2, 9, 900, 0), (3, 1, 6500, 9000, 0), (40, 1, 300, 5000, 1)])
+def test_slots_and_pages_by_the_thousand(slots, page, longest, spare, shift):
+    """More slots than the workgroup that deals pages out has threads, more pages than it looks at in one go, counts at an address of four bytes."""
+    import random
+
+    from katz_amd import ops
+
+    rng = random.Random(slots)
+    held = [rng.choice([0, rng.randint(0, longest)]) for _ in range(slots)]
+    held[0] = longest
+    pages = Pages(33, held, page, 1, 8, BF, 1, spare, width=longest // page + 40)
+    if shift:
+        c = pages.dev
+        refs = torch.zeros(c.refs.numel() + 1, dtype=torch.int32, device=DEV)[1:]
+        refs.copy_(c.refs)
+        pages.dev = ops.PagedCache(c.k, c.v, c.table, c.lengths, refs)
+    model = Model(pages)
+    for call in range(4):
+        counts = [rng.choice([0, 1, 2, rng.randint(0, 12), -5]) for _ in range(slots)]
+        counts[-1] = 33 * page
+        assert ops.cache_extend(pages.dev, int32(counts)).tolist() == [model.extend(counts)]
+        model.same(f"extended, {call}")
+        parents = [rng.choice([s, s, s, rng.randrange(slots), -1]) for s in range(slots)]
+        assert ops.cache_reorder(pages.dev, int32(parents)).tolist() == [model.reorder(parents)]
+        model.same(f"reordered, {call}")
+        if call != 1:
+            assert ops.cache_compact(pages.dev).tolist() == [model.compact()]
+            model.same(f"moved together, {call}")
