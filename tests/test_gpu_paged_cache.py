@@ -772,3 +772,17 @@ def test_slots_and_pages_by_the_thousand(slots, page, longest, spare, shift):
         if call != 1:
             assert ops.cache_compact(pages.dev).tolist() == [model.compact()]
             model.same(f"moved together, {call}")
+
+
+def test_rotary_of_more_than_the_caches_hold():
+    from katz_amd import ops
+
+    g = torch.Generator(DEV).manual_seed(34)
+    rows, heads, kv, d = 70000, 6, 2, 64
+    q, k = (torch.randn(rows, h * d, generator=g, device=DEV, dtype=FP32) for h in (heads, kv))
+    pos, freq = torch.arange(rows, dtype=torch.int32, device=DEV)[:, None], ops.rotary_frequencies(32, device=DEV)
+    for pairs in (False, True):
+        got = ops.rotary(q, k, heads, pos, freq, kv_heads=kv, pairs=pairs)
+        for lo in range(0, rows, 10000):                 # the same as in parts that the caches hold
+            part = ops.rotary(q[lo:lo + 10000], k[lo:lo + 10000], heads, pos[lo:lo + 10000], freq, kv_heads=kv, pairs=pairs)
+            assert torch.equal(got[0][lo:lo + 10000], part[0]) and torch.equal(got[1][lo:lo + 10000], part[1])
