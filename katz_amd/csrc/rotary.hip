@@ -50,20 +50,11 @@ __device__ __forceinline__ Where where(const RotaryParams& p, long r) {
   return w;
 }
 
-// ONCE: past the caches
-template <bool ONCE, typename T, int N>
+template <typename T, int N>
 __device__ __forceinline__ void load(const T* from, float (&f)[N]) {
   T v[N];
-  if constexpr (N == 8 && ONCE) {
-    u32x4 w[sizeof(v) / 16];
-#pragma unroll
-    for (unsigned i = 0; i < sizeof(v) / 16; ++i) w[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(from) + i);
-    __builtin_memcpy(v, w, sizeof(v));
-  } else if constexpr (N == 8) {
-    __builtin_memcpy(v, __builtin_assume_aligned(from, 16), sizeof(v));
-  } else {
-    v[0] = from[0];
-  }
+  if constexpr (N == 8) __builtin_memcpy(v, __builtin_assume_aligned(from, 16), sizeof(v));
+  else v[0] = from[0];
 #pragma unroll
   for (int e = 0; e < N; ++e) f[e] = (float)v[e];
 }
@@ -121,11 +112,10 @@ struct Unit {
       first = u * N + pairs;                              // (2 pairs + (u - pairs / N) * N)
     }
   }
-  template <bool ONCE>
   __device__ __forceinline__ void fetch() {
     if (what == 0 || what == 3) return;
-    load<ONCE>(from + first, a);
-    if (second >= 0) load<ONCE>(from + second, b);
+    load(from + first, a);
+    if (second >= 0) load(from + second, b);
   }
   template <bool E4M3>
   __device__ __forceinline__ void finish() {
@@ -163,7 +153,7 @@ struct Unit {
 };
 
 // N: elements of a piece, 8 where rows, heads and pairs allow it.
-template <typename T, bool E4M3, bool PAIRS, int N, bool ONCE>
+template <typename T, bool E4M3, bool PAIRS, int N>
 __global__ __launch_bounds__(NT) void rotary_rows(const RotaryParams p) {
   extern __shared__ float2 angles[];                     // [per][pairs]
   __shared__ Where at[MOST_ROWS];
@@ -222,8 +212,8 @@ __global__ __launch_bounds__(NT) void rotary_rows(const RotaryParams p) {
     Unit<T, PAIRS, N> x, y;
     piece(i, x);
     piece(i + NT, y);
-    x.template fetch<ONCE>();
-    y.template fetch<ONCE>();
+    x.fetch();
+    y.fetch();
     x.template finish<E4M3>();
     y.template finish<E4M3>();
   }
@@ -233,11 +223,8 @@ template <typename T, bool E4M3, bool PAIRS>
 void launch(const RotaryParams& p, bool pieces, hipStream_t s) {
   const dim3 grid((unsigned)((p.rows + p.per - 1) / p.per));
   const size_t lds = (size_t)p.per * p.pairs * sizeof(float2);
-  // q and k that the 256 MB of the memory-side cache cannot hold with what becomes of them are read past it (us of 403 MB in and out: 77, with that 72; of 81 MB 15.8 and 18.9)
-  const bool once = !p.cached && p.rows * (p.heads + p.kv_heads) * p.d * (long)sizeof(T) * 2 > (256L << 20);
-  if (!pieces) kh_launch(KH_TAG_ROTARY, rotary_rows<T, E4M3, PAIRS, 1, false>, grid, dim3(NT), lds, s, p);
-  else if (!E4M3 && once) kh_launch(KH_TAG_ROTARY, rotary_rows<T, false, PAIRS, 8, true>, grid, dim3(NT), lds, s, p);
-  else kh_launch(KH_TAG_ROTARY, rotary_rows<T, E4M3, PAIRS, 8, false>, grid, dim3(NT), lds, s, p);
+  if (pieces) kh_launch(KH_TAG_ROTARY, rotary_rows<T, E4M3, PAIRS, 8>, grid, dim3(NT), lds, s, p);
+  else kh_launch(KH_TAG_ROTARY, rotary_rows<T, E4M3, PAIRS, 1>, grid, dim3(NT), lds, s, p);
 }
 template <typename T, bool E4M3>
 void launch(const RotaryParams& p, bool in_turn, bool pieces, hipStream_t s) {
