@@ -550,9 +550,13 @@ __global__ __launch_bounds__(NW * 64, wgs_a_cu(D, CODES)) void attend(const Page
     }
   }
   // rows that have nothing to attend to, or no slot
-  for (int r = w; r < p.rows; r += G) {
-    const Row row = row_of(p, r);
-    if (row.tiles <= 0 && (row.slot >= 0 || p.fill)) zero_row<T>(p, r);
+  if (p.whole) {
+    if (!active && w == u.r * units && (u.row.slot >= 0 || p.fill)) zero_row<T>(p, u.r);
+  } else {
+    for (int r = w; r < p.rows; r += G) {
+      const Row row = row_of(p, r);
+      if (row.tiles <= 0 && (row.slot >= 0 || p.fill)) zero_row<T>(p, r);
+    }
   }
 }
 
@@ -761,6 +765,7 @@ KH_EXPORT int kh_paged_attention(const void* q, void* o, const KhPagedCache* cac
   if (rows > (1L << 24) || heads > (1L << 16)) return KH_ERR_TOO_LARGE;
   const long group = heads / c.kv_heads, e = kh_cache_element(c);
   if (!line_fits(rows, c.kv_heads, group, c.width * c.page)) return KH_ERR_TOO_LARGE;
+  if (window > 1L << 30) window = 0;                    // (longer than any sequence)
   const Plan plan = plan_of(rows, c.kv_heads, group, c.d, c.width * c.page, window, c.type == KH_E4M3);
   if (plan.parts && !workspace) return KH_ERR_INVALID_ARG;
   PagedParams p{q, (const char*)c.k + layer * c.k_layer * e, (const char*)c.v + layer * c.v_layer * e, o, c.table, lengths, c.lengths, slots,
@@ -768,7 +773,7 @@ KH_EXPORT int kh_paged_attention(const void* q, void* o, const KhPagedCache* cac
                 plan.parts ? (float*)((char*)workspace + plan.workgroups * 16) : nullptr, plan.parts ? (int4*)workspace : nullptr, ldq, ldo, (uint32_t)(c.k_page * e), (uint32_t)(c.k_token * e), (uint32_t)(c.v_page * e),
                 (uint32_t)(c.v_token * e), c.k_head * e, c.v_head * e,
                 (int)rows, (int)c.kv_heads, (int)group, (int)((group + QB - 1) / QB), (int)c.d, (int)c.slots, (int)c.width, (int)c.pages, (int)c.page,
-                (int)(window < (1L << 30) ? window : 0), scale * 1.4426950408889634f, flags & 1, 0, !plan.parts, 0, KhDivide((uint32_t)c.page)};
+                (int)window, scale * 1.4426950408889634f, flags & 1, 0, !plan.parts, 0, KhDivide((uint32_t)c.page)};
   // (32 sequences of 4096 tokens, 8 heads of 80 and 96 in bf16: 82 -> 77 us and 84 -> 76; heads of whole lines 91 -> 94)
   p.shared_lines = c.kv_heads > 1 && c.k_head * e % 128 != 0;
   p.q_aligned = kh_aligned16(q) && ldq % 8 == 0;

@@ -9,7 +9,8 @@
 // threads go over the rows in pieces of eight elements of either half (or eight in a row), 16 bytes a load, two pieces on their way at a time
 // (one: 19.0 us where two take 15.8, three 19.8).
 //
-// us: 7904 rows of 20 + 20 heads of 64, bf16, 15.8 (5.1 TB/s in and out), 16384 of 16 + 8 of 128, fp32, 77 (5.2), 8184 of 16 + 8 of 80 into pages 19.2 (4.4), 2 rows into pages 4.0.
+// us: 7904 rows of 20 + 20 heads of 64, bf16, 15.8 (5.1 TB/s in and out), 16384 of 16 + 8 of 128, fp32, 77 (5.2; read past the caches 72, but 81 against 79 among
+// others of its kind), 8184 of 16 + 8 of 80 into pages 18.8 (4.5), 2 rows into pages 4.0.
 #include "paged_cache.h"
 
 namespace {

@@ -786,3 +786,16 @@ def test_rotary_of_more_than_the_caches_hold():
         for lo in range(0, rows, 10000):                 # the same as in parts that the caches hold
             part = ops.rotary(q[lo:lo + 10000], k[lo:lo + 10000], heads, pos[lo:lo + 10000], freq, kv_heads=kv, pairs=pairs)
             assert torch.equal(got[0][lo:lo + 10000], part[0]) and torch.equal(got[1][lo:lo + 10000], part[1])
+
+
+@pytest.mark.parametrize("window", [1, 127, 128, 129, 300, 2 ** 30, 2 ** 30 + 1, 2 ** 62])
+@pytest.mark.parametrize("longest", [300, 2000])
+def test_windows_of_every_size(window, longest):
+    from katz_amd import ops
+
+    heads, d = 4, 64
+    pages = Pages(35, [longest, 128, 0, longest - 1, 129], 16, 2, d)
+    q = randn(gen(36), 5, heads * d)
+    ref, off = attention_reference(q, pages, heads, range(5), pages.held, window=min(window, longest))
+    got = ops.paged_attention(q.to(DEV), pages.dev, heads, window=window)
+    assert_within(got.view(5, heads, d), ref, HALF[BF] * ref.abs() + off, "a window")
