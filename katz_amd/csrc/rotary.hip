@@ -3,7 +3,8 @@
 //
 // The angle is a number of whole turns and a rest; a position of 10^6 in 32 bits would leave the rest 0.06 off.  So the turns are counted in 64 bits
 // (position * frequency / 2 pi less the nearest integer) and only the rest goes to 32 (off by 2^-25 turns), where sine and cosine are taken of a
-// multiple of pi.  The products with the rows are in 32 bits and rounded once.
+// multiple of pi.  The products with the rows are in 32 bits and rounded once.  Codes of 8 bits have steps so wide that a key a little off in its last bits now and
+// then goes to the wrong side of a border, a sixteenth away: what becomes a code is turned and scaled in 64 bits.
 //
 // Bound by memory: every element is read and written once.  A workgroup takes some rows, works their angles out once for all heads (LDS), then its
 // threads go over the rows in pieces of eight elements of either half (or eight in a row), 16 bytes a load, two pieces on their way at a time
@@ -12,6 +13,7 @@
 // us: 7904 rows of 20 + 20 heads of 64, bf16, 15.8 (5.1 TB/s in and out), 16384 of 16 + 8 of 128, fp32, 77 (5.2; read past the caches 72, but 81 against 79 among
 // others of its kind), 8184 of 16 + 8 of 80 into pages 18.8 (4.5), 2 rows into pages 4.0.
 #include "paged_cache.h"
+#include <type_traits>
 
 namespace {
 
@@ -89,17 +91,18 @@ __device__ __forceinline__ void store_e4m3(uint8_t* to, const float (&f)[N], flo
 
 // A piece of work: unit u of a head.  Its elements are N from `first` and N from `second` on, the a and b of N pairs; with pairs in turn (and N > 1), or behind the
 // pairs, only the N from `first` on.
-template <typename T, bool PAIRS, int N>
+template <typename T, bool E4M3, bool PAIRS, int N>
 struct Unit {
+  using Turn = typename std::conditional<E4M3, double2, float2>::type;   // cosine and sine
   const T* from;
   void* to;
   int first, second;           // second < 0: none
-  const float2* cs;            // of the first pair; nullptr: copied
+  const Turn* cs;              // of the first pair; nullptr: copied
   float scale;                 // of an e4m3 code
   int what;                    // 0 nothing, 1 to T, 2 to codes, 3 zeros
   float a[N], b[N];
 
-  __device__ __forceinline__ void at(int u, int pairs, const float2* angles) {
+  __device__ __forceinline__ void at(int u, int pairs, const Turn* angles) {
     second = -1;
     cs = nullptr;
     if (PAIRS && N > 1) {
@@ -118,35 +121,38 @@ struct Unit {
     load(from + first, a);
     if (second >= 0) load(from + second, b);
   }
-  template <bool E4M3>
+  // The pair (a, b) turned by z, in the type of z and times `by`.
+  template <typename X>
+  static __device__ __forceinline__ void turn(float& a, float& b, const Turn& z, X by) {
+    const X c = (X)z.x, s = (X)z.y, x = (X)a * c - (X)b * s, y = (X)b * c + (X)a * s;
+    a = (float)(x * by);
+    b = (float)(y * by);
+  }
+  template <typename X>
+  __device__ __forceinline__ void turn_all(X by) {
+    if constexpr (PAIRS && N > 1) {
+#pragma unroll
+      for (int e = 0; e < N; e += 2) turn<X>(a[e], a[e + 1], cs[e / 2], by);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) turn<X>(a[e], b[e], cs[e], by);
+    }
+  }
   __device__ __forceinline__ void finish() {
     if (what == 0) return;
     if (what == 3) {
 #pragma unroll
       for (int e = 0; e < N; ++e) a[e] = b[e] = 0.f;
-    } else if (cs) {
-      if constexpr (PAIRS && N > 1) {
-#pragma unroll
-        for (int e = 0; e < N; e += 2) {
-          const float2 z = cs[e / 2];
-          const float x = a[e] * z.x - a[e + 1] * z.y;
-          a[e + 1] = a[e + 1] * z.x + a[e] * z.y;
-          a[e] = x;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const float2 z = cs[e];
-          const float x = a[e] * z.x - b[e] * z.y;
-          b[e] = b[e] * z.x + a[e] * z.y;
-          a[e] = x;
-        }
-      }
     }
     if (E4M3 && what == 2) {
+      if (cs) {
+        turn_all<double>(1.0 / (double)scale);
+        scale = 1.f;
+      }
       store_e4m3(reinterpret_cast<uint8_t*>(to) + first, a, scale);
       if (second >= 0) store_e4m3(reinterpret_cast<uint8_t*>(to) + second, b, scale);
     } else {
+      if (cs && what == 1) turn_all<float>(1.f);
       store(reinterpret_cast<T*>(to) + first, a);
       if (second >= 0) store(reinterpret_cast<T*>(to) + second, b);
     }
@@ -156,7 +162,10 @@ struct Unit {
 // N: elements of a piece, 8 where rows, heads and pairs allow it.
 template <typename T, bool E4M3, bool PAIRS, int N>
 __global__ __launch_bounds__(NT) void rotary_rows(const RotaryParams p) {
-  extern __shared__ float2 angles[];                     // [per][pairs]
+  using Piece = Unit<T, E4M3, PAIRS, N>;
+  using Turn = typename Piece::Turn;
+  extern __shared__ double2 lds[];                       // [per][pairs] cosines and sines
+  Turn* const angles = reinterpret_cast<Turn*>(lds);
   __shared__ Where at[MOST_ROWS];
   const int tid = threadIdx.x;
   const long first = (long)blockIdx.x * p.per;
@@ -175,14 +184,15 @@ __global__ __launch_bounds__(NT) void rotary_rows(const RotaryParams p) {
           : p.position_type == 1 ? (double)reinterpret_cast<const int64_t*>(p.positions)[x] : (double)reinterpret_cast<const float*>(p.positions)[x];
     }
     t *= (p.frequency_32 ? (double)reinterpret_cast<const float*>(p.frequencies)[j] : reinterpret_cast<const double*>(p.frequencies)[j]) * ONE_TURN;
-    float2 z;
-    sincospif((float)(2.0 * (t - rint(t))), &z.y, &z.x);
+    Turn z;
+    if constexpr (E4M3) sincospi(2.0 * (t - rint(t)), &z.y, &z.x);
+    else sincospif((float)(2.0 * (t - rint(t))), &z.y, &z.x);
     angles[i] = z;
   }
   __syncthreads();
   // units of a head, heads of a row (of q, of k, with a cache of v), rows
   const int units = p.units, heads = p.heads + p.kv_heads, all = p.cached ? heads + p.kv_heads : heads, count = rows * all * units;
-  auto piece = [&](int i, Unit<T, PAIRS, N>& x) {
+  auto piece = [&](int i, Piece& x) {
     x.what = 0;
     if (i >= count) return;
     const int hr = (int)p.by_units((uint32_t)i), u = i - hr * units, r = (int)p.by_heads((uint32_t)hr), h = hr - r * all;
@@ -210,20 +220,20 @@ __global__ __launch_bounds__(NT) void rotary_rows(const RotaryParams p) {
     }
   };
   for (int i = tid; i < count; i += 2 * NT) {            // two on their way at a time
-    Unit<T, PAIRS, N> x, y;
+    Piece x, y;
     piece(i, x);
     piece(i + NT, y);
     x.fetch();
     y.fetch();
-    x.template finish<E4M3>();
-    y.template finish<E4M3>();
+    x.finish();
+    y.finish();
   }
 }
 
 template <typename T, bool E4M3, bool PAIRS>
 void launch(const RotaryParams& p, bool pieces, hipStream_t s) {
   const dim3 grid((unsigned)((p.rows + p.per - 1) / p.per));
-  const size_t lds = (size_t)p.per * p.pairs * sizeof(float2);
+  const size_t lds = (size_t)p.per * p.pairs * (E4M3 ? sizeof(double2) : sizeof(float2));
   if (pieces) kh_launch(KH_TAG_ROTARY, rotary_rows<T, E4M3, PAIRS, 8>, grid, dim3(NT), lds, s, p);
   else kh_launch(KH_TAG_ROTARY, rotary_rows<T, E4M3, PAIRS, 1>, grid, dim3(NT), lds, s, p);
 }

@@ -799,3 +799,26 @@ def test_windows_of_every_size(window, longest):
     ref, off = attention_reference(q, pages, heads, range(5), pages.held, window=min(window, longest))
     got = ops.paged_attention(q.to(DEV), pages.dev, heads, window=window)
     assert_within(got.view(5, heads, d), ref, HALF[BF] * ref.abs() + off, "a window")
+
+
+@pytest.mark.parametrize("pairs", [False, True])
+def test_turned_keys_become_the_codes_that_64_bits_give(pairs):
+    """Three hundred thousand keys: in 32 bits (2^-23 off, codes 2^-3 apart) about one in a million would go to the wrong side of a border, in 64 (angles of 2 * 10^5 are 2^-33
+    off) one in ten thousand millions."""
+    from katz_amd import ops
+
+    g, rows, kv, d, page = gen(37), 600, 4, 128, 32
+    scale = torch.rand(1, kv, generator=g) * 0.01 + 0.01
+    cache = ops.PagedCache.empty(1, 20, page, kv, d, 1, 20, E4M3, DEV, scale.to(DEV))
+    ops.cache_extend(cache, int32([rows]))
+    x = randn(g, rows, 2 * kv * d)
+    pos = torch.randint(0, 200000, (rows, 1), generator=g, dtype=torch.int32)
+    freq = ops.rotary_frequencies(d // 2, device=DEV)
+    k = x[:, :kv * d].contiguous()
+    for _ in range(2):
+        ops.cache_append(x.to(DEV), k.to(DEV), x[:, kv * d:].to(DEV), cache, 2 * kv, pos.to(DEV), freq, slots=int32([0] * rows), places=int32(list(range(rows))), pairs=pairs)
+        ref, _ = turned(k, kv, pos, freq.cpu(), (d // 2,), pairs)
+        want = (ref / scale[0].to(F64)[:, None]).float().clamp(-448, 448).to(E4M3)
+        got = cache.k[0].cpu().view(torch.uint8)[cache.table[0].long().cpu()].view(-1, kv, d)[:rows]
+        assert torch.equal(got, want.view(torch.uint8))
+        k = (k.float() * 1.0009765625).to(BF)
