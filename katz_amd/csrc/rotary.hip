@@ -8,10 +8,10 @@
 //
 // Bound by memory: every element is read and written once.  A workgroup takes some rows, works their angles out once for all heads (LDS), then its
 // threads go over the rows in pieces of eight elements of either half (or eight in a row), 16 bytes a load, two pieces on their way at a time
-// (one: 19.0 us where two take 15.8, three 19.8).
+// (7904 rows of 40 heads of 64: one 19.0 us, two 15.8, three 19.8).
 //
-// us: 7904 rows of 20 + 20 heads of 64, bf16, 15.8 (5.1 TB/s in and out), 16384 of 16 + 8 of 128, fp32, 77 (5.2; read past the caches 72, but 81 against 79 among
-// others of its kind), 8184 of 16 + 8 of 80 into pages 18.8 (4.5), 2 rows into pages 4.0.
+// us: 7904 rows of 20 + 20 heads of 64, bf16, 15.2 (5.3 TB/s in and out), 16384 of 16 + 8 of 128, fp32, 74 (5.4; four rows to a workgroup and read past the caches 72, but 81
+// behind one another), 8184 of 16 + 8 of 80 into pages 17 (4.9), 2 rows into pages 4.0.
 #include "paged_cache.h"
 #include <type_traits>
 
@@ -293,12 +293,14 @@ KH_EXPORT int kh_rotary(const void* q, const void* k, const void* v, void* q_out
                       kh_aligned16(q_out) && kh_aligned16(cache ? v : k_out);
   p.units = pieces ? (int)(in_turn ? d / 8 : pairs / 8 + (d - 2 * pairs) / 8) : (int)(d - pairs);
   p.by_units = KhDivide((uint32_t)p.units);
-  // A workgroup has a row, or, at most as make one angle a thread, as many as leave 2048 workgroups (7904 rows of 40 heads of 64: 15.8 us, with 1024 16.6, with
-  // 8192 18.3), up to twice that where its pieces then fill the threads better (8184 rows of 32 heads of 80 into pages: three rows 20.9 us, four 19.2).
-  long whole = pairs > 0 ? (NT + pairs - 1) / pairs : MOST_ROWS;
+  // A workgroup has a row, or as many as make 12 KB, if 2048 workgroups are left and no thread has two angles (16384 rows of 12 KB, calls behind one another: one to a workgroup
+  // 74.3 us, two 77.5, four 80.7; 7904 rows of 5 KB by themselves: three 15.2, seven 16.6, one 18.3), up to twice that where its pieces then fill the threads better
+  // (8184 rows of 32 heads of 80 into pages: three rows 20.9 us, four 19.2; behind one another four 18.5, six 20.0).
+  const long each = (heads + kv_heads * (cache ? 2 : 1)) * p.units, bytes = (heads + kv_heads) * d * (long)element;
+  long whole = pairs > 0 ? (NT + pairs - 1) / pairs : MOST_ROWS, least = rows / 2048;
   whole = whole < MOST_ROWS ? whole : MOST_ROWS;
-  const long least = rows / 2048 < 1 ? 1 : rows / 2048 < whole ? rows / 2048 : whole;
-  const long each = (heads + kv_heads * (cache ? 2 : 1)) * p.units;
+  least = least < 12288 / bytes ? least : 12288 / bytes;
+  least = least < 1 ? 1 : least < whole ? least : whole;
   double best = 0.;
   for (long n = least; n <= (least > 1 ? (2 * least < whole ? 2 * least : whole) : 1); ++n) {
     const long rounds = (n * each + 2 * NT - 1) / (2 * NT);
