@@ -324,7 +324,7 @@ struct Wave {
 #pragma unroll
     for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);
     top = swapped_max(top);
-    if (__any(top > m + RESCALE_LOG2)) {
+    if (__any(top - m > RESCALE_LOG2)) {                    // (a difference of large numbers is exact, their sum with 2^3 is not)
       const float to = fmaxf(m, top), by = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - to);
       m = to;
       l *= by;
