@@ -10,7 +10,7 @@
 //   S^T = K . Q^T     A = the keys as they lie in memory (lane l: token l % 16, 8 dimensions from 8 * (l / 16) on), B = up to 16 query heads in registers
 //   O^T += V^T . P^T  A = values of 8 tokens for a dimension, put together from the loads of 8 whole rows by byte permutes in the lane, B = P
 // The tokens of the keys' rows are chosen so that the scores a lane gets (query l % 16, eight tokens) are the P operand it needs: nothing crosses lanes but the
-// maximum.  Neither operand goes through LDS.  P is multiplied in all 24 bits: in three pieces of bf16 or two of fp16, since the matrix unit waits for memory anyway.
+// maximum.  Neither operand goes through LDS.  P is multiplied in all 24 bits, in three pieces of 16: the matrix unit waits for memory anyway.
 //
 // us a launch (TB/s of keys and values): one token of 64 requests of 0 .. 8192 tokens, 32 heads of 128 on 8, bf16, 118 (5.6) and 3.9 for the join; one of 131071 tokens, 16 heads on 2, 25.6 (5.2)
 // and 4.6; 32 of 4096 tokens with 4 KB a token, heads of 64, 128, 256: 93, 91, 85 (5.8, 5.9, 6.3), with 2 KB in e4m3 87, 53, 63; 2 x 77 tokens 4.7, a chain of lengths,
@@ -91,11 +91,14 @@ __device__ __forceinline__ uint32_t two_of_e4m3(uint32_t w) {
 #endif
 }
 
-// P in pieces whose sum it is: three of bf16 (each the upper bits of what is left: exact), or two of fp16 (P <= 2^8, and below one what is
-// left out is under 2^-25 of the largest)
-template <typename T> struct Pieces;
+// P in three pieces.  Of bf16 they are the upper bits of what is left each time, and P is their sum: bf16 reaches as far down as 32 bits do.  fp16 does not: P is held
+// 2^7 times as large (it stays under 2^15, the running maximum may be 2^8 behind), and the third piece is what two leave times 2^23, with a product of its own.  That is all
+// of P down to 2^-31 of the largest and 11 bits down to 2^-44; what is lost of n weights is under n 2^-55 (two pieces of P as it is lose n 2^-25, a hundredth of what
+// tokens 16 below one whose value is zero give).  us: one sequence of 131071 tokens 25.1 with two pieces, 25.8 so, 28.0 with products in 32 bits.
+template <typename W> struct Pieces;
 template <> struct Pieces<bf16_t> {
-  static constexpr int N = 3;
+  static constexpr float UP_LOG2 = 0.f;
+  static constexpr bool APART = false;                  // whether the third has its own product
   static __device__ __forceinline__ void of(const float (&p)[8], bf16x8 (&out)[3]) {
     uint32_t w[3][4];
 #pragma unroll
@@ -113,12 +116,15 @@ template <> struct Pieces<bf16_t> {
   }
 };
 template <> struct Pieces<f16_t> {
-  static constexpr int N = 2;
-  static __device__ __forceinline__ void of(const float (&p)[8], f16x8 (&out)[2]) {
+  static constexpr float UP_LOG2 = 7.f, REST = 0x1p23f;
+  static constexpr bool APART = true;
+  static __device__ __forceinline__ void of(const float (&p)[8], f16x8 (&out)[3]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       out[0][i] = (f16_t)p[i];
-      out[1][i] = (f16_t)(p[i] - (float)out[0][i]);
+      const float rest = p[i] - (float)out[0][i];
+      out[1][i] = (f16_t)rest;
+      out[2][i] = (f16_t)((rest - (float)out[1][i]) * REST);
     }
   }
 };
@@ -177,6 +183,8 @@ template <int D, typename T, bool CODES, bool EIGHT, bool TAIL>
 struct Wave {
   using S = Shape<D, T, CODES, EIGHT, TAIL>;
   using X = typename S::X;
+  using W = typename std::conditional<CODES, bf16_t, T>::type;           // the type that values and weights are multiplied in: codes are numbers of bf16, whatever the queries are
+  using X8 = typename Eight<W>::type;
   struct Pages { int k[EIGHT ? 1 : 2], v[EIGHT ? 1 : 8]; };
 
   X q[S::KK];
@@ -335,11 +343,11 @@ struct Wave {
     float pr[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      pr[i] = __builtin_amdgcn_exp2f(x[i] - from);
+      pr[i] = __builtin_amdgcn_exp2f(x[i] - from + Pieces<W>::UP_LOG2);
       l += pr[i];
     }
-    X pieces[Pieces<T>::N];
-    Pieces<T>::of(pr, pieces);
+    X8 pieces[3];
+    Pieces<W>::of(pr, pieces);
 #pragma unroll
     for (int c = 0; c < S::NC; ++c)
 #pragma unroll
@@ -349,14 +357,21 @@ struct Wave {
         for (int h = 0; h < 4; ++h) {                 // tokens 2 h, 2 h + 1
           if constexpr (CODES) {
             const uint32_t both = __builtin_amdgcn_perm(vr[2 * h + 1][c][j / 4], vr[2 * h][c][j / 4], 0x0400u + (j % 4) * 0x0101u);
-            a[h] = two_of_e4m3<T, false>(both);
+            a[h] = two_of_e4m3<W, false>(both);
           } else {
             a[h] = __builtin_amdgcn_perm(vr[2 * h + 1][c][j / 2], vr[2 * h][c][j / 2], j & 1 ? 0x07060302 : 0x05040100);
           }
         }
-        const X value8 = __builtin_bit_cast(X, a);
+        const X8 value8 = __builtin_bit_cast(X8, a);
+        f32x4& to = o[c * S::VE + j];
+        to = mfma(value8, pieces[1], mfma(value8, pieces[0], to));
+        if constexpr (Pieces<W>::APART) {
+          const f32x4 rest = mfma(value8, pieces[2], f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-        for (int n2 = 0; n2 < Pieces<T>::N; ++n2) o[c * S::VE + j] = mfma(value8, pieces[n2], o[c * S::VE + j]);
+          for (int r = 0; r < 4; ++r) to[r] += rest[r] * (1.f / Pieces<W>::REST);
+        } else {
+          to = mfma(value8, pieces[2], to);
+        }
       }
     if constexpr (MORE) {
       t0 += TILE;
