@@ -548,7 +548,7 @@ typedef struct {
  * With a cache (type 0 or 1, the cache's unless that is e4m3; k_out unused): the turned k and v [rows, kv_heads * d] are written as token places[r] of slot slots[r] in
  * `layer`; slots NULL: row r is slot r; places NULL: the last token of the slot's sequence; positions NULL: the place on every axis.  Rows whose slot
  * lies outside the cache, or whose place outside its sequence, are left out: q_out stays as it was there, with flags bit 1 it is zeroed.  k and v of a place without a page are
- * dropped.  e4m3: the nearest to value / scale, clamped at 448 (halves to even).  (slot, place) of the rows are distinct. */
+ * dropped.  e4m3: the nearest to value / scale rounded to 32 bits, clamped at 448 (halves to even); a turned key's quotient is worked out in 64.  (slot, place) of the rows are distinct. */
 int kh_rotary(const void* q, const void* k, const void* v, void* q_out, void* k_out, const void* positions, int position_type,
               const void* frequencies, const int64_t* section_end, int64_t axes, const KhPagedCache* cache, int64_t layer, const int32_t* slots,
               const int32_t* places, int64_t rows, int64_t heads, int64_t kv_heads, int64_t d, int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldqo,

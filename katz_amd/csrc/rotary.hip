@@ -4,7 +4,9 @@
 // The angle is a number of whole turns and a rest; a position of 10^6 in 32 bits would leave the rest 0.06 off.  So the turns are counted in 64 bits
 // (position * frequency / 2 pi less the nearest integer) and only the rest goes to 32 (off by 2^-25 turns), where sine and cosine are taken of a
 // multiple of pi.  The products with the rows are in 32 bits and rounded once.  Codes of 8 bits have steps so wide that a key a little off in its last bits now and
-// then goes to the wrong side of a border, a sixteenth away: what becomes a code is turned and scaled in 64 bits.
+// then goes to the wrong side of a border, a sixteenth away: keys that turn on the way to a code are turned and scaled in 64 bits.  A code is that of the quotient in 32
+// bits, as (x.float() / scale).to(float8) has it, for values, dimensions beyond the pairs and turned keys alike: a quotient that 32 bits round to a border between two codes
+// goes to the even one (one in four million; of numbers over a scale of the kind "largest / 448", many of whose quotients lie on borders, one in a thousand).
 //
 // Bound by memory: every element is read and written once.  A workgroup takes some rows, works their angles out once for all heads (LDS), then its
 // threads go over the rows in pieces of eight elements of either half (or eight in a row), 16 bytes a load, two pieces on their way at a time
@@ -69,7 +71,7 @@ __device__ __forceinline__ void store(T* to, const float (&f)[N]) {
   if constexpr (N == 8) __builtin_memcpy(__builtin_assume_aligned(to, 16), v, sizeof(v));
   else to[0] = v[0];
 }
-// to e4m3: the nearest code to f / scale (halves to even), no further than the largest; NaN stays one
+// to e4m3: the nearest code to f / scale in 32 bits (halves to even), no further than the largest; NaN stays one
 template <int N>
 __device__ __forceinline__ void store_e4m3(uint8_t* to, const float (&f)[N], float scale) {
   uint32_t w[(N + 3) / 4] = {};

@@ -1890,7 +1890,7 @@ def cache_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: Paged
     Row r is token places[r] of slot slots[r] (int32 [rows], on the GPU; together distinct), for which cache_extend has made room; without slots row r is slot r,
     without places it is the last token of its sequence; without positions a token's position is its place, on every axis.  Without frequencies
     nothing turns.  q [rows, heads * d], k and v [rows, kv_heads * d], bf16 or fp16, the cache's type unless that is float8 (then the nearest code to
-    value / scale, at most 448 off zero).  Rows whose slot lies outside the cache or whose place outside its sequence are left out (padded batches
+    value / scale in 32 bits, at most 448 off zero).  Rows whose slot lies outside the cache or whose place outside its sequence are left out (padded batches
     in a captured graph): those of a given out stay as they were, those of a new one are zero.  out may be q."""
     fill = out is None
     if fill:

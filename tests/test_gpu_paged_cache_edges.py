@@ -57,3 +57,32 @@ def test_weights_far_below_the_largest_count(dtype, cache, gap, n, heads, kv, d)
     ref, off = attention_reference(q, pages, heads, [0], [n], scale=1.0)
     got = ops.paged_attention(q.to(DEV), pages.dev, heads, scale=1.0)
     assert_within(got.view(1, heads, d), ref, HALF[dtype] * ref.abs() + off + TINY[dtype], "weights far below the largest")
+
+
+@pytest.mark.parametrize("dtype", [BF, FP16])
+@pytest.mark.parametrize("d,turn", [(128, 32), (40, 12), (72, 0)])
+def test_codes_are_those_of_the_quotient_in_32_bits(dtype, d, turn):
+    """Scales as calibration makes them (the largest number / 448): multiples of sevenths lie on borders between codes, or a rounding of the scale beside them, and one quotient in a
+    thousand goes to a border in 32 bits.  Values, dimensions beyond the pairs and keys at place 0, which turn by nothing: what (x.float() / scale).to(float8) gives."""
+    from katz_amd import ops
+
+    g, rows, kv, layers = gen(50 + d), 500, 6, 2
+    x = randn(g, rows, (2 + 2) * kv * d, dtype=dtype, std=2.0)
+    x[:, ::7] = (torch.randint(-200, 200, x[:, ::7].shape, generator=g) * 2.0 ** -6).to(dtype)
+    x[0, 2 * kv * d::kv * d // 2], x[1, 2 * kv * d + 1::kv * d // 2] = float("inf"), -float("inf")
+    most = (torch.randint(1, 64, (2, layers, kv), generator=g) * 2.0 ** -4).float()
+    scales = [(m / 448).to(DEV) for m in most]
+    k, v = (torch.zeros(layers, 63, 8, kv, d, device=DEV).to(E4M3) for _ in range(2))
+    cache = ops.PagedCache(k, v, int32([list(range(63))]), int32([rows]), None, *scales)
+    dev = x.to(DEV)
+    freq = ops.rotary_frequencies(turn, device=DEV) if turn else None
+    ops.cache_append(dev[:, :2 * kv * d], dev[:, 2 * kv * d:3 * kv * d], dev[:, 3 * kv * d:], cache, 2 * kv, torch.zeros(rows, 1, dtype=torch.int32, device=DEV) if turn else None, freq,
+                     layer=1, slots=int32([0] * rows), places=int32(list(range(rows))))
+    for pool, at, scale in ((cache.k, 2, scales[0]), (cache.v, 3, scales[1])):
+        y = x[:, at * kv * d:(at + 1) * kv * d].to(F64).view(rows, kv, d)
+        if at == 2:                                      # cosine 1, sine 0: an infinity leaves its pair's other half no number
+            y[..., :turn], y[..., turn:2 * turn] = y[..., :turn] - 0 * y[..., turn:2 * turn], y[..., turn:2 * turn] + 0 * y[..., :turn]
+        want = (y.float() / scale[1].cpu()[:, None]).clamp(-448, 448).to(E4M3)
+        got = pool[1].cpu().view(-1, kv, d)[:rows]
+        bad = (raw(got) != raw(want)) & ~torch.isnan(want.float())
+        assert not bad.any() and torch.equal(torch.isnan(got.float()), torch.isnan(want.float())), f"{bad.sum()} of {got.numel()} codes"
