@@ -526,7 +526,7 @@ int kh_linear_attention_step_bf16(const void* q, const void* k, const void* v, v
  * No counterpart in the reference; they stand beside K3 and the states of linear attention.
  *
  * KhPagedCache (HOST memory, device pointers inside): keys and values of sequences in pages of `page` tokens, for all layers of a model.
- *   k, v       [layers, pages, page, kv_heads, d] through strides in elements, the last axis contiguous: bf16, fp16 or (type 3) e4m3, d % 8 == 0, d <= 256;
+ *   k, v       [layers, pages, page, kv_heads, d] through strides in elements (none below zero), the last axis contiguous: bf16, fp16 or (type 3) e4m3, d % 8 == 0, d <= 256;
  *              pointers and strides aligned to 16 bytes (e4m3: 8)
  *   table      int32 [slots, width]: page i of slot s's sequence (tokens i * page ..); a number outside 0 .. pages - 1 is no page: its tokens are left out
  *   lengths    int32 [slots], tokens of each sequence (at most width * page count)

@@ -13,7 +13,9 @@ static inline int kh_cache_check(const KhPagedCache* c) {
   if (c->type != 0 && c->type != 1 && c->type != KH_E4M3) return KH_ERR_INVALID_ARG;
   if (c->type != KH_E4M3 && (c->k_scale || c->v_scale)) return KH_ERR_INVALID_ARG;
   if (c->d % 8 != 0 || c->d > 256) return KH_ERR_UNSUPPORTED;
-  if ((c->k_layer | c->k_page | c->k_token | c->k_head | c->v_layer | c->v_page | c->v_token | c->v_head) % 8 != 0) return KH_ERR_ALIGNMENT;
+  const int64_t strides = c->k_layer | c->k_page | c->k_token | c->k_head | c->v_layer | c->v_page | c->v_token | c->v_head;
+  if (strides < 0) return KH_ERR_INVALID_ARG;           // (one below zero: the kernels count bytes from the first element on)
+  if (strides % 8 != 0) return KH_ERR_ALIGNMENT;
   const uintptr_t mask = c->type == KH_E4M3 ? 7 : 15;
   if (((uintptr_t)c->k | (uintptr_t)c->v) & mask) return KH_ERR_ALIGNMENT;
   if (((uintptr_t)c->table | (uintptr_t)c->lengths | (uintptr_t)c->refs | (uintptr_t)c->k_scale | (uintptr_t)c->v_scale) & 3) return KH_ERR_ALIGNMENT;
