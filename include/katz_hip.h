@@ -562,7 +562,7 @@ int64_t kh_paged_attention_workspace_bytes(int64_t rows, int64_t heads, int64_t 
 int kh_paged_attention(const void* q, void* o, const KhPagedCache* cache, int64_t layer, const int32_t* slots, const int32_t* lengths, void* workspace,
                        int64_t rows, int64_t heads, int64_t ldq, int64_t ldo, int64_t window, float scale, int flags, int type, void* stream);
 /* The pages of a cache.  Whoever wants pages gets the lowest free ones, by slot and then by place; where there are none left the entry is -1, and *missing
- * (device) is how many were wanted and not there (table rows that are too short counted in).
+ * (device) is how many were wanted and not there (table rows that are too short counted in; no more than 2^31 - 1).
  * kh_cache_extend: sequence s gets counts[s] (<= 0: no) more tokens, at most width * page in all.
  * kh_cache_reorder: slot s keeps its sequence where parents[s] == s, takes over the one that slot parents[s] had before the call, or, where that is no
  * slot, is emptied.  Whole pages are shared; the page not yet full is copied (its tokens, in all layers), but handed on as it is to the lowest taker

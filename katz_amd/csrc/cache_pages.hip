@@ -8,6 +8,7 @@
 // Bound by the launches and the memory's latency for a few sequences, by the copies' bytes for many layers.  us: three beams forked from 77 tokens, 2 layers, 5.7 + 3.9, then
 // their next tokens 3.8; 48 of 8 sequences, 24 layers, 4.5 + 4.4 + 20.2 (171 MB in and out), 5.4; 490 of 2048 pages moved in 4 layers 6.0 + 96 (515 MB, 5.4 TB/s).
 #include "paged_cache.h"
+#include <climits>
 
 namespace {
 
@@ -126,6 +127,8 @@ __device__ __forceinline__ int clamped(int n, const PagesParams& p) {
 // Sequence s grows by counts[s]: the pages behind its last one, dealt out by slot and then by place.
 __global__ __launch_bounds__(NT) void extend(const PagesParams p) {
   __shared__ int red[NT / 64];
+  __shared__ unsigned long long all_over;               // pages that no row has room for: slots can want 2^31 each
+  if (threadIdx.x == 0) all_over = 0;
   const int most = p.width * p.page;
   // a slot's tokens, its first new page and how many
   auto look = [&](int s, int* longer, int* first, int* need, int* too_long) {
@@ -136,13 +139,14 @@ __global__ __launch_bounds__(NT) void extend(const PagesParams p) {
     *need = (n + fits + p.page - 1) / p.page - *first;
     *too_long = whole > p.width ? (int)(whole - p.width) : 0;
   };
-  int wanted = 0, over = 0, longer = -1, first = 0, need = 0, start = 0;
+  int wanted = 0, longer = -1, first = 0, need = 0, start = 0;
+  unsigned long long over = 0;
   for (int base = 0; base < p.slots; base += NT) {
     const int s = base + (int)threadIdx.x;
     int total, too_long = 0;
     longer = -1, need = 0;
     if (s < p.slots) look(s, &longer, &first, &need, &too_long);
-    over += too_long;
+    over += (unsigned)too_long;
     start = wanted + prefix(need, &total, red);
     if (s < p.slots && p.slots > NT) p.w.start[s] = start;
     wanted += total;
@@ -151,10 +155,12 @@ __global__ __launch_bounds__(NT) void extend(const PagesParams p) {
     p.w.free[rank] = page;
     p.refs[page] = 1;
   });
-  int all_over;
-  prefix(over, &all_over, red);                         // (and what was dealt out is there for all threads)
-  if (threadIdx.x == 0) *p.told = wanted - got + all_over;
-  __syncthreads();
+  if (over) atomicAdd(&all_over, over);
+  __syncthreads();                                      // (and what was dealt out is there for all threads)
+  if (threadIdx.x == 0) {
+    const unsigned long long missing = (unsigned)(wanted - got) + all_over;
+    *p.told = missing < INT_MAX ? (int)missing : INT_MAX;
+  }
   // a thread enters the pages of a slot, a wave those of one that gets many
   constexpr int FEW = 4;
   for (int base = 0; base < p.slots; base += NT) {

@@ -86,3 +86,15 @@ def test_codes_are_those_of_the_quotient_in_32_bits(dtype, d, turn):
         got = pool[1].cpu().view(-1, kv, d)[:rows]
         bad = (raw(got) != raw(want)) & ~torch.isnan(want.float())
         assert not bad.any() and torch.equal(torch.isnan(got.float()), torch.isnan(want.float())), f"{bad.sum()} of {got.numel()} codes"
+
+
+@pytest.mark.parametrize("page,width,counts", [(1, 4, [2 ** 31 - 1] * 3), (1, 4, [2 ** 31 - 1, 5, 0]), (2, 3, [2 ** 31 - 1] * 4), (1, 1, [2 ** 31 - 1] * 1500), (16, 2, [2 ** 31 - 1, 1 << 30, 7])])
+def test_pages_that_are_missing_are_counted_as_far_as_32_bits_go(page, width, counts):
+    from katz_amd import ops
+
+    slots = len(counts)
+    cache = ops.PagedCache.empty(1, 9, page, 1, 8, slots, width, BF, DEV)
+    got = ops.cache_extend(cache, int32(counts)).item()
+    wanted = sum(-(-n // page) for n in counts)
+    assert got == min(wanted - min(9, sum(min(-(-n // page), width) for n in counts)), 2 ** 31 - 1)
+    assert cache.lengths.tolist() == [min(n, width * page) for n in counts]
