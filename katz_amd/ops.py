@@ -1799,6 +1799,8 @@ def _token_rows(t: torch.Tensor, width: int, name: str):
         return shape[0], (st[0] if shape[0] > 1 else width)
     if len(shape) < 2 or shape[-1] != width or (st[-1] != 1 and width > 1):
         raise ValueError(f"{name} must be [.., {width}] with a contiguous last axis, got {tuple(shape)}")
+    if 0 in shape[:-1]:                                  # (no rows lie in any run)
+        return 0, width
     rows, ld = shape[-2], st[-2]
     for n, s in zip(shape[-3::-1], st[-3::-1]):
         if rows == 1:

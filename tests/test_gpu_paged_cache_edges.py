@@ -98,3 +98,16 @@ def test_pages_that_are_missing_are_counted_as_far_as_32_bits_go(page, width, co
     wanted = sum(-(-n // page) for n in counts)
     assert got == min(wanted - min(9, sum(min(-(-n // page), width) for n in counts)), 2 ** 31 - 1)
     assert cache.lengths.tolist() == [min(n, width * page) for n in counts]
+
+
+def test_calls_without_rows_in_any_shape():
+    from katz_amd import ops
+
+    pages = Pages(45, [5], 16, 2, 64)
+    freq = ops.rotary_frequencies(32, device=DEV)
+    for shape in ((2, 0), (0, 3), (3, 0, 2), (3, 2, 0), (1, 0)):
+        none = torch.zeros(*shape, 4 * 64, dtype=BF, device=DEV)
+        q, k = ops.rotary(none, none[..., :128], 4, int32([]).view(0, 1), freq, kv_heads=2)
+        assert q.shape == none.shape and k.shape == (*shape, 128)
+        assert ops.cache_append(none, none[..., :128], none[..., :128], pages.dev, 4).shape == none.shape
+        assert ops.paged_attention(none, pages.dev, 4).shape == none.shape
