@@ -11,6 +11,7 @@ import contextlib
 import ctypes
 import functools
 import math
+import operator
 import os
 import struct
 import threading
@@ -1675,6 +1676,15 @@ _POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 _pack_cache = struct.Struct("23q").pack          # KhPagedCache
 
 
+def _cache_part(at: int, slot: str) -> property:
+    """One of a cache's tensors: another that takes its place is checked and described to the library with the rest."""
+    def put(cache, t):
+        parts = list(cache._tensors())
+        parts[at] = t
+        PagedCache.__init__(cache, *parts)
+    return property(operator.attrgetter(slot), put)
+
+
 class PagedCache:
     """Keys and values of sequences in pages of `page` tokens, for all layers of a model.
 
@@ -1682,8 +1692,10 @@ class PagedCache:
     of 8 up to 256; table int32 [slots, width]: the pages of each slot's sequence in order, -1 where there is none; lengths int32 [slots], its tokens;
     refs int32 [pages], how many sequences hold a page (0: free; None for a cache that somebody else keeps).  k_scale, v_scale float32 [layers, kv_heads],
     float8 only: a code c stands for c * scale (None: 1).  `empty` makes one without sequences.  cache_extend, cache_reorder and cache_compact keep table,
-    lengths and refs, on the device; a program that fills them itself keeps shared pages whole: cache_append does not look at refs."""
-    __slots__ = ("k", "v", "table", "lengths", "refs", "k_scale", "v_scale", "layers", "pages", "page", "kv_heads", "d", "slots", "width", "desc")
+    lengths and refs, on the device; a program that fills them itself keeps shared pages whole: cache_append does not look at refs.
+
+    Another tensor may take the place of one of them (cache.lengths = ...; what does not fit the rest is refused); sizes are read only, they follow the tensors."""
+    __slots__ = ("_k", "_v", "_table", "_lengths", "_refs", "_k_scale", "_v_scale", "_layers", "_pages", "_page", "_kv_heads", "_d", "_slots", "_width", "_desc")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, refs: Optional[torch.Tensor] = None,
                  k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None):
@@ -1716,13 +1728,22 @@ class PagedCache:
         for t in others:
             if t.get_device() != dev:
                 raise ValueError("the parts of a cache must lie on one device")
-        self.k, self.v, self.table, self.lengths, self.refs, self.k_scale, self.v_scale = k, v, table, lengths, refs, k_scale, v_scale
-        self.layers, self.pages, self.page, self.kv_heads, self.d, self.slots, self.width = layers, pages, page, kv_heads, d, slots, width
+        self._k, self._v, self._table, self._lengths, self._refs, self._k_scale, self._v_scale = k, v, table, lengths, refs, k_scale, v_scale
+        self._layers, self._pages, self._page, self._kv_heads, self._d, self._slots, self._width = layers, pages, page, kv_heads, d, slots, width
         if layers == 1 or pages == 1 or page == 1 or kv_heads == 1:      # (strides of an axis of one element may be anything)
             ks, vs = ((0 if layers == 1 else st[0], 0 if pages == 1 else st[1], kv_heads * d if page == 1 else st[2], d if kv_heads == 1 else st[3]) for st in (ks, vs))
-        self.desc = _pack_cache(k.data_ptr(), v.data_ptr(), table.data_ptr(), lengths.data_ptr(), 0 if refs is None else refs.data_ptr(),
-                                0 if k_scale is None else k_scale.data_ptr(), 0 if v_scale is None else v_scale.data_ptr(),
-                                layers, pages, page, kv_heads, d, slots, width, kind, ks[0], ks[1], ks[2], ks[3], vs[0], vs[1], vs[2], vs[3])
+        self._desc = _pack_cache(k.data_ptr(), v.data_ptr(), table.data_ptr(), lengths.data_ptr(), 0 if refs is None else refs.data_ptr(),
+                                 0 if k_scale is None else k_scale.data_ptr(), 0 if v_scale is None else v_scale.data_ptr(),
+                                 layers, pages, page, kv_heads, d, slots, width, kind, ks[0], ks[1], ks[2], ks[3], vs[0], vs[1], vs[2], vs[3])
+
+    def _tensors(self):
+        return self._k, self._v, self._table, self._lengths, self._refs, self._k_scale, self._v_scale
+
+    k, v, table, lengths, refs, k_scale, v_scale = map(_cache_part, range(7), __slots__)
+    layers, pages, page, kv_heads, d, slots, width, desc = map(property, map(operator.attrgetter, __slots__[7:]))
+
+    def __reduce__(self):                                # (copies have a description of their own)
+        return type(self), self._tensors()
 
     @classmethod
     def empty(cls, layers: int, pages: int, page: int, kv_heads: int, d: int, slots: int, width: int, dtype: torch.dtype = BF16, device="cuda",

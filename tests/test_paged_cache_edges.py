@@ -30,3 +30,58 @@ def test_rows_of_empty_tensors():
     for bad in (torch.zeros(2, 4, 8)[:, :2], torch.zeros(2, 0, 9), torch.zeros(0, 4, 16)[..., ::2], torch.zeros(8)):
         with pytest.raises(ValueError):
             _token_rows(bad, 8, "q")
+
+
+def describes(c):
+    """Whether the description that the library gets is that of the tensors the cache has."""
+    from katz_amd.ops import PagedCache
+
+    return c.desc == PagedCache(c.k, c.v, c.table, c.lengths, c.refs, c.k_scale, c.v_scale).desc and (c.layers, c.pages, c.page, c.kv_heads, c.d) == tuple(c.k.shape) and (c.slots, c.width) == tuple(c.table.shape)
+
+
+def test_a_cache_follows_the_tensors_that_it_is_given():
+    from katz_amd.ops import PagedCache
+
+    c = PagedCache(**parts())
+    lengths = c.lengths
+    c.lengths = c.lengths + 1
+    assert c.lengths is not lengths and describes(c)
+    c.lengths += 1
+    assert c.lengths.tolist() == [2] * 4 and describes(c)
+    c.k, c.v, c.refs = torch.ones_like(c.k), torch.ones_like(c.v), None
+    assert c.refs is None and describes(c)
+    c.table = torch.zeros(4, 9, dtype=torch.int32)       # wider rows of the same slots
+    assert c.width == 9 and describes(c)
+    eight = PagedCache(**parts(dtype=torch.float8_e4m3fn))
+    eight.k_scale = torch.ones(2, 2)
+    assert describes(eight)
+    eight.k_scale = None
+    assert describes(eight)
+
+
+def test_a_cache_refuses_tensors_that_do_not_fit_and_stays_as_it_was():
+    from katz_amd.ops import PagedCache
+
+    c = PagedCache(**parts())
+    before = c.desc
+    for name, bad, kind in (("lengths", torch.zeros(5, dtype=torch.int32), ValueError), ("table", torch.zeros(3, 5, dtype=torch.int32), ValueError), ("k", c.k[:, :8], ValueError),
+                            ("v", c.v.half(), TypeError), ("refs", c.refs.long(), TypeError), ("k_scale", torch.ones(2, 2), ValueError)):
+        old = getattr(c, name)
+        with pytest.raises(kind):
+            setattr(c, name, bad)
+        assert getattr(c, name) is old and c.desc == before
+    for name in ("layers", "pages", "page", "kv_heads", "d", "slots", "width", "desc", "other"):
+        with pytest.raises(AttributeError):
+            setattr(c, name, 1)
+    assert describes(c)
+
+
+def test_copies_of_a_cache_describe_themselves():
+    from katz_amd.ops import PagedCache
+
+    c = PagedCache(**parts())
+    c.lengths[1] = 7
+    for other in (copy.deepcopy(c), pickle.loads(pickle.dumps(c))):
+        assert other.lengths.tolist() == [0, 7, 0, 0] and other.lengths.data_ptr() != c.lengths.data_ptr() and describes(other)
+    same = copy.copy(c)
+    assert same.k is c.k and describes(same)
