@@ -2,8 +2,8 @@
 //   angle(r, j) = position[r][axis of j] * frequency[j],   (a, b) -> (a cos - b sin, b cos + a sin)   for every pair j of every head
 //
 // The angle is a number of whole turns and a rest; a position of 10^6 in 32 bits would leave the rest 0.06 off.  So the turns are counted in 64 bits
-// (position * frequency / 2 pi less the nearest integer) and only the rest goes to 32 (off by 2^-25 turns), where sine and cosine are taken of a
-// multiple of pi.  The products with the rows are in 32 bits and rounded once.  Codes of 8 bits have steps so wide that a key a little off in its last bits now and
+// (position * frequency / 2 pi less the nearest integer) and only the rest goes to 32 (off by 2^-26 turns), where sine and cosine are taken of a
+// multiple of pi; for rows of 32 bits what it is off by turns them once more.  The products with the rows are in 32 bits and rounded once.  Codes of 8 bits have steps so wide that a key a little off in its last bits now and
 // then goes to the wrong side of a border, a sixteenth away: keys that turn on the way to a code are turned and scaled in 64 bits.  A code is that of the quotient in 32
 // bits, as (x.float() / scale).to(float8) has it, for values, dimensions beyond the pairs and turned keys alike: a quotient that 32 bits round to a border between two codes
 // goes to the even one (one in four million; of numbers over a scale of the kind "largest / 448", many of whose quotients lie on borders, one in a thousand).
@@ -188,7 +188,16 @@ __global__ __launch_bounds__(NT) void rotary_rows(const RotaryParams p) {
     t *= (p.frequency_32 ? (double)reinterpret_cast<const float*>(p.frequencies)[j] : reinterpret_cast<const double*>(p.frequencies)[j]) * ONE_TURN;
     Turn z;
     if constexpr (E4M3) sincospi(2.0 * (t - rint(t)), &z.y, &z.x);
-    else sincospif((float)(2.0 * (t - rint(t))), &z.y, &z.x);
+    else {
+      const double half = 2.0 * (t - rint(t));
+      const float near = (float)half;
+      sincospif(near, &z.y, &z.x);
+      if constexpr (sizeof(T) == 4) {                     // (rows of 16 bits do not show it)
+        const float rest = (float)(half - (double)near) * 3.14159265f, x = z.x;
+        z.x -= z.y * rest;
+        z.y += x * rest;
+      }
+    }
     angles[i] = z;
   }
   __syncthreads();

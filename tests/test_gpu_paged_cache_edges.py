@@ -111,3 +111,24 @@ def test_calls_without_rows_in_any_shape():
         assert q.shape == none.shape and k.shape == (*shape, 128)
         assert ops.cache_append(none, none[..., :128], none[..., :128], pages.dev, 4).shape == none.shape
         assert ops.paged_attention(none, pages.dev, 4).shape == none.shape
+
+
+@pytest.mark.parametrize("pairs", [False, True])
+@pytest.mark.parametrize("positions", ["near", "far", "fractions"])
+def test_sine_and_cosine_of_32_bits_are_those_of_the_whole_angle(positions, pairs):
+    """(1, 0) turned is the angle's cosine and sine themselves: a step of theirs (2^-24) and the rounding of what the angle's last bits add to them (2^-25)."""
+    from katz_amd import ops
+
+    g, rows, n = gen(61), 4000, 64
+    pos = {"near": torch.arange(rows, dtype=torch.int32), "far": torch.randint(0, 1 << 24, (rows,), generator=g, dtype=torch.int32), "fractions": torch.rand(rows, generator=g) * 500}[positions]
+    freq = ops.rotary_frequencies(n, device=DEV)
+    x = torch.zeros(rows, n, 2) if pairs else torch.zeros(rows, 2, n)
+    (x[..., 0] if pairs else x[:, 0])[:] = 1
+    got, _ = ops.rotary(x.view(rows, 2 * n).to(DEV), x.view(rows, 2 * n).to(DEV), 1, pos[:, None].to(DEV), freq, pairs=pairs)
+    got = got.cpu().view_as(x)
+    c, s = (got[..., 0], got[..., 1]) if pairs else (got[:, 0], got[:, 1])
+    angle = pos.to(F64)[:, None] * freq.cpu()
+    far = 2.0 ** 24 * 2.0 ** -52                         # (an angle of up to 2^24 in 64 bits, in the reference and there)
+    assert_within(c, angle.cos(), torch.full_like(angle, 1.5 * U + far), "cosine")
+    assert_within(s, angle.sin(), torch.full_like(angle, 1.5 * U + far), "sine")
+    assert (c[0] == 1).all() and (s[0] == 0).all() or positions != "near"
