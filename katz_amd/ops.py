@@ -1946,7 +1946,8 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, heads: int, layer: int =
     Row r attends to the first lengths[r] tokens (int32 [rows], on the GPU; None: all that cache.lengths says) of slot slots[r] (None: slot r), of those with
     window > 0 to the last `window`; tokens without a page are left out.  Several rows may have one slot: the tokens of a prompt, each with a length of
     its own.  A row with nothing to attend to is zero.  Rows whose slot lies outside the cache are left out: those of a given out stay as they were, those of a
-    new one are zero.  An infinity among the values attended to gives NaN."""
+    new one are zero.  An infinity among the values attended to gives NaN, and so does a score of plus infinity; a row whose scores are all minus infinity has nothing
+    to attend to."""
     lib = _lib.load()
     dt, d = q.dtype, cache.d
     if (dt is not torch.bfloat16 and dt is not torch.float16) or (cache.k.dtype is not dt and cache.k.dtype is not torch.float8_e4m3fn):

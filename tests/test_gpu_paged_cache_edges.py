@@ -132,3 +132,21 @@ def test_sine_and_cosine_of_32_bits_are_those_of_the_whole_angle(positions, pair
     assert_within(c, angle.cos(), torch.full_like(angle, 1.5 * U + far), "cosine")
     assert_within(s, angle.sin(), torch.full_like(angle, 1.5 * U + far), "sine")
     assert (c[0] == 1).all() and (s[0] == 0).all() or positions != "near"
+
+
+def test_scores_that_are_infinite():
+    """All scores of a row minus infinity: nothing to attend to.  One that is plus infinity: no number."""
+    from katz_amd import ops
+
+    for dtype in (BF, FP16):
+        pages = Pages(43, [200, 700, 40], 16, 1, 64, dtype)
+        q = randn(gen(44), 3, 2 * 64, dtype=dtype)
+        q[:, 3] = 1.0                                    # (of the first head)
+        q[:, 64 + 3] = 0.0
+        for s, n in enumerate([200, 700, 40]):
+            for t in range(n):
+                pages.k[0, pages.table[s, t // 16], t % 16, 0, 3] = -float("inf") if s < 2 else 0.5
+        pages.k[0, pages.table[2, 1], 3, 0, 3] = float("inf")
+        pages.dev.k.copy_(pages.k)
+        got = ops.paged_attention(q.to(DEV), pages.dev, 2).view(3, 2, 64)
+        assert (got[:2, 0] == 0).all() and torch.isnan(got[:2, 1]).all() and torch.isnan(got[2]).all()       # (0 times infinity is no number either)
