@@ -1,6 +1,4 @@
 """Attention over a paged cache where a type, a size or a number is at its edge, against plain implementations in 64 bits (tolerances as in test_gpu_paged_cache)."""
-import math
-
 import pytest
 import torch
 
@@ -150,3 +148,29 @@ def test_scores_that_are_infinite():
         pages.dev.k.copy_(pages.k)
         got = ops.paged_attention(q.to(DEV), pages.dev, 2).view(3, 2, 64)
         assert (got[:2, 0] == 0).all() and torch.isnan(got[:2, 1]).all() and torch.isnan(got[2]).all()       # (0 times infinity is no number either)
+
+
+LONG = [  # lengths, heads, kv, d, page, type, cache: more than 16 query heads on a key head, and heads that no kernel has the size of, where sequences are cut
+    ([2000, 0, 900], 40, 2, 64, 16, BF, BF),
+    ([2000, 0, 900], 34, 2, 72, 12, FP16, FP16),
+    ([20000], 33, 1, 80, 24, FP16, E4M3),
+    ([9000], 17, 1, 40, 5, BF, BF),
+    ([30, 12000], 48, 1, 256, 32, BF, BF),
+    ([6000, 1], 20, 1, 200, 16, BF, E4M3),
+    ([700] * 9, 32, 1, 128, 16, FP16, FP16),
+    ([9000], 7, 1, 96, 64, FP16, FP16),
+]
+
+
+@pytest.mark.parametrize("window", [0, 1000])
+@pytest.mark.parametrize("case", LONG, ids=lambda c: f"{'-'.join(map(str, c[0][:3]))}-H{c[1]}of{c[2]}-{c[3]}-p{c[4]}-{str(c[5])[6:]}-{str(c[6])[6:]}")
+def test_many_query_heads_on_a_key_head_over_long_sequences(case, window):
+    from katz_amd import ops
+
+    lengths, heads, kv, d, page, dtype, cache = case
+    pages = Pages(41, lengths, page, kv, d, cache)
+    q = randn(gen(42), len(lengths), heads * d, dtype=dtype)
+    ref, off = attention_reference(q, pages, heads, range(len(lengths)), pages.held, window=window)
+    got = ops.paged_attention(q.to(DEV), pages.dev, heads, window=window)
+    assert_within(got.view(-1, heads, d), ref, HALF[dtype] * ref.abs() + off + TINY[dtype], "long")
+    assert torch.equal(got, ops.paged_attention(q.to(DEV), pages.dev, heads, window=window))
