@@ -174,3 +174,40 @@ def test_many_query_heads_on_a_key_head_over_long_sequences(case, window):
     got = ops.paged_attention(q.to(DEV), pages.dev, heads, window=window)
     assert_within(got.view(-1, heads, d), ref, HALF[dtype] * ref.abs() + off + TINY[dtype], "long")
     assert torch.equal(got, ops.paged_attention(q.to(DEV), pages.dev, heads, window=window))
+
+
+def test_entries_and_lengths_outside_the_cache_change_nothing_else():
+    """Entries that are no pages and lengths that no table holds, through every call: table, lengths, refs and the bits of the pages are those of the model."""
+    from katz_amd import ops
+
+    pages = Pages(22, [40, 40, 8, 61], 16, 2, 64, spare=3)
+    big, most = 2 ** 31 - 1, pages.table.shape[1] * 16
+    pages.table[0] = torch.tensor([big, -7, int(pages.table[0, 2]), -1, -1], dtype=torch.int32)
+    pages.table[1, 2] = 999                              # the page not yet full of a sequence that is taken over
+    pages.table[3, 1] = pages.refs.numel()
+    lengths = torch.tensor([big, 40, -9, 61], dtype=torch.int32)
+    pages.dev.table.copy_(pages.table)
+    pages.dev.lengths.copy_(lengths)
+    pages.held = lengths
+    model = Model(pages)
+    clamped = [min(max(n, 0), most) for n in model.held]
+
+    def same(what):
+        c = pages.dev
+        assert c.table.tolist() == model.table and c.lengths.tolist() == model.held and c.refs.tolist() == model.refs, what
+        assert torch.equal(raw(c.k), model.k) and torch.equal(raw(c.v), model.v), f"{what}: pages"
+
+    counts = [5, 0, 100, -1]
+    kept = [n for n, m in zip(model.held, counts)]
+    model.held = clamped
+    want = model.extend(counts)
+    model.held = [n if m > 0 else k for n, m, k in zip(model.held, counts, kept)]        # (a slot that gets nothing keeps what it says)
+    assert ops.cache_extend(pages.dev, int32(counts)).item() == want
+    same("extended")
+    assert model.compact() == ops.cache_compact(pages.dev).item()
+    same("moved together")
+    for parents in ([1, 1, 0, 3], [3, 9, 3, -1], [0, 0, 0, 0]):
+        assert model.reorder(parents) == ops.cache_reorder(pages.dev, int32(parents)).item()
+        same(f"reordered {parents}")
+    assert model.compact() == ops.cache_compact(pages.dev).item()
+    same("moved together again")
