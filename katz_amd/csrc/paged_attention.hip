@@ -639,7 +639,8 @@ __global__ __launch_bounds__(NW * 64) void join_few(const PagedParams p, const i
 template <typename T, bool CODES>
 __global__ __launch_bounds__(JT) void join_many(const PagedParams p, const int G) {
   constexpr int DL = 8, GR = JT / DL;                   // lanes of 32 dimensions, groups that take parts in turn
-  // there are few rows (at most MOST / 32 units): a lane has one's tiles, and with them where this workgroup's unit lies in the line
+  // there are few rows (fewer units than a sixteenth of the workgroups): a lane has one's tiles, and with them where this workgroup's unit lies in the line
+  static_assert(MOST / 16 <= 64);
   const int units = p.kv_heads * p.blocks, r = blockIdx.x / units, unit = blockIdx.x - r * units, at_lane = threadIdx.x & 63;
   const int tiles = at_lane < p.rows ? row_of(p, at_lane).tiles : 0;
   int before = tiles;
@@ -708,7 +709,8 @@ __global__ __launch_bounds__(JT) void join_many(const PagedParams p, const int G
 // Workgroups: as many as run at once (D 256: one a CU), but no more than there can be tiles.
 // Where units have at most WHOLE tiles, a workgroup has one: 4 sequences of 300 tokens on 8 key heads 8.9 us where line and join take 7.4 + 4.0, of 470 10.5 and 7.5 + 4.0, 256 of 300
 // 61.5 and 57.8 + 3.9 (and 3 of the host's for the second launch).
-// `many`: parts of a unit, about the workgroups by the units, are more than a wave joins in passing.
+// `many`: a unit has more than 16 parts or so, the workgroups by the units.  us of the join, by a wave a query head and by 32 dimensions a workgroup: 512 workgroups, heads of 128,
+// 4 units 23.1 and 4.3, 16 7.5 and 4.3, 24 6.2 and 4.9, 32 5.1 and 5.1, 64 4.1 and 6.7; 768, heads of 64, 32 units 5.0 and 4.3, 48 4.4 and 4.9.
 struct Plan { long workgroups; bool parts, many; };
 
 Plan plan_of(int64_t rows, int64_t kv_heads, int64_t group, int64_t d, int64_t span, int64_t window, bool codes) {
@@ -716,7 +718,7 @@ Plan plan_of(int64_t rows, int64_t kv_heads, int64_t group, int64_t d, int64_t s
   const long tiles = (span + TILE - 1) / TILE, units = rows * kv_heads * ((group + QB - 1) / QB);
   const long at_once = 256 * wgs_a_cu((int)d, codes), n = units * tiles < at_once ? units * tiles : at_once;
   if (tiles <= WHOLE && units <= 1 << 20) return Plan{units, false, false};
-  return Plan{n, true, units * 32 < n};
+  return Plan{n, true, units * 16 < n};
 }
 
 // whether all tiles can be counted in 31 bits

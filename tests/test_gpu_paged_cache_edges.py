@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from test_gpu_paged_cache import BF, DEV, E4M3, F64, FP16, FP32, HALF, TINY, U, Model, Pages, assert_within, attention_reference, gen, int32, randn, raw, turned
+from test_gpu_paged_cache import BF, DEV, E4M3, F64, FP16, FP32, HALF, TINY, U, Model, Pages, assert_within, attention_reference, gen, int32, randn, raw
 
 pytestmark = pytest.mark.gpu
 
@@ -211,3 +211,17 @@ def test_entries_and_lengths_outside_the_cache_change_nothing_else():
         same(f"reordered {parents}")
     assert model.compact() == ops.cache_compact(pages.dev).item()
     same("moved together again")
+
+
+def test_a_long_sequence_among_many_rows():
+    """Parts of one sequence by the hundred where the rows are too many for the join that goes by parts."""
+    from katz_amd import ops
+
+    rows, longest, d = 60, 20000, 64
+    lengths = [0] * rows
+    lengths[17], lengths[59] = longest, 130
+    pages = Pages(47, lengths, 64, 1, d, spare=1)
+    q = randn(gen(48), rows, 2 * d)
+    ref, off = attention_reference(q, pages, 2, range(rows), pages.held)
+    got = ops.paged_attention(q.to(DEV), pages.dev, 2)
+    assert_within(got.view(rows, 2, d), ref, HALF[BF] * ref.abs() + off, "one long")
