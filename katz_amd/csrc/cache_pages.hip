@@ -427,8 +427,9 @@ KH_EXPORT int kh_cache_reorder(const KhPagedCache* cache, const int32_t* parents
   const PagesParams p = params(*cache, parents, missing, workspace);
   hipStream_t s = (hipStream_t)stream;
   hipError_t e;
-  // one workgroup counts for few slots with short rows (four beams of 77 tokens: 3.8 + 4.4 us for the two launches)
-  if (cache->slots <= 32 && cache->slots * cache->width <= 4096) {
+  // one workgroup counts for few slots with short rows, a wave a slot.  us with one launch and with two, the copies' 4 among them: 4 slots with rows of 8 pages 9.9 and 12.3, of
+  // 128 10.9 and 13.2, of 1024 21.5 and 14.8; 8 of 32 10.5 and 14.1, of 512 16.3 and 13.7; 16 of 8 11.3 and 14.0, of 256 14.6 and 14.1; 32 of 8 14.0 and 14.4, of 128 17.0 and 14.1.
+  if (cache->slots <= 16 && cache->width <= 128) {
     kh_launch(KH_TAG_CACHE_PAGES, reorder_deal<true>, dim3(1), dim3(NT), 0, s, p);
   } else {
     kh_launch(KH_TAG_CACHE_PAGES, reorder_count, dim3((unsigned)p.slots), dim3(NC), 0, s, p);
