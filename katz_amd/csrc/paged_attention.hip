@@ -12,9 +12,9 @@
 // The tokens of the keys' rows are chosen so that the scores a lane gets (query l % 16, eight tokens) are the P operand it needs: nothing crosses lanes but the
 // maximum.  Neither operand goes through LDS.  P is multiplied in all 24 bits, in three pieces of 16: the matrix unit waits for memory anyway.
 //
-// us a launch (TB/s of keys and values): one token of 64 requests of 0 .. 8192 tokens, 32 heads of 128 on 8, bf16, 118 (5.6) and 3.9 for the join; one of 131071 tokens, 16 heads on 2, 25.6 (5.2)
-// and 4.6; 32 of 4096 tokens with 4 KB a token, heads of 64, 128, 256: 93, 91, 85 (5.8, 5.9, 6.3), with 2 KB in e4m3 87, 53, 63; 2 x 77 tokens 4.7, a chain of lengths,
-// page numbers and rows.  A copy of 1 GiB runs at 5.1 TB/s.  With each step's loads waited for where they are used: 207 and 55.  Values are read past
+// us a launch, the middle of 12 (TB/s of keys and values): one token of 64 requests of 0 .. 8192 tokens, 32 heads of 128 on 8, bf16, 121 (5.5) and 5.0 for the join; one of 131071 tokens,
+// 16 heads on 2, fp16, 26.9 (5.0) and 5.3; 2 x 77 tokens 5.6, a chain of lengths, page numbers and rows.  32 of 4096 tokens with 4 KB a token, heads of 64, 128, 256: 93, 91, 85 (5.8, 5.9, 6.3)
+// on one card and 116, 113, 102 on another, with 2 KB in e4m3 87, 53, 63 and 98, 63, 66.  A copy of 1 GiB runs at 5.1 TB/s.  With each step's loads waited for where they are used: 207 and 55.  Values are read past
 // the caches (126 us where that is 119), keys are not (123, and the two halves of a line that a wave asks for one after the other are both there: e4m3 78 -> 59).
 #include "paged_cache.h"
 #include <type_traits>
@@ -24,7 +24,7 @@ namespace {
 constexpr int NW = 4, STEP = 32, TILE = NW * STEP;       // waves, tokens of a wave's step, of a tile
 constexpr int QB = 16;                                  // query heads of a unit
 constexpr int JT = 512, MOST = 1024;                    // threads that join, workgroups at most that share the line
-constexpr int WHOLE = 4;                                // tiles of a unit that is not cut
+constexpr int WHOLE = 4;                                // tiles that a table (or window) holds at most where units are not cut
 constexpr float RESCALE_LOG2 = 8.0f;                    // the running maximum moves only for jumps above 2^8
 
 struct PagedParams {
@@ -343,7 +343,9 @@ struct Wave {
     float pr[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      pr[i] = __builtin_amdgcn_exp2f(x[i] - from + Pieces<W>::UP_LOG2);
+      float at = x[i] - from;
+      if constexpr (Pieces<W>::UP_LOG2 > 0.f) at += Pieces<W>::UP_LOG2;
+      pr[i] = __builtin_amdgcn_exp2f(at);
       l += pr[i];
     }
     X8 pieces[3];
@@ -707,7 +709,7 @@ __global__ __launch_bounds__(JT) void join_many(const PagedParams p, const int G
 }
 
 // Workgroups: as many as run at once (D 256: one a CU), but no more than there can be tiles.
-// Where units have at most WHOLE tiles, a workgroup has one: 4 sequences of 300 tokens on 8 key heads 8.9 us where line and join take 7.4 + 4.0, of 470 10.5 and 7.5 + 4.0, 256 of 300
+// Where the table or the window has room for at most WHOLE tiles (how long the sequences are the host does not know), a workgroup has a unit, and there is no second launch: 4 sequences of 300 tokens on 8 key heads 8.9 us where line and join take 7.4 + 4.0, of 470 10.5 and 7.5 + 4.0, 256 of 300
 // 61.5 and 57.8 + 3.9 (and 3 of the host's for the second launch).
 // `many`: a unit has more than 16 parts or so, the workgroups by the units.  us of the join, by a wave a query head and by 32 dimensions a workgroup: 512 workgroups, heads of 128,
 // 4 units 23.1 and 4.3, 16 7.5 and 4.3, 24 6.2 and 4.9, 32 5.1 and 5.1, 64 4.1 and 6.7; 768, heads of 64, 32 units 5.0 and 4.3, 48 4.4 and 4.9.

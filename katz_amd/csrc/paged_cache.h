@@ -25,7 +25,8 @@ static inline int kh_cache_check(const KhPagedCache* c) {
   return KH_OK;
 }
 
-// t / n for 0 <= t < 2^31 by a multiplication (n is the size of a page: any number)
+// t / n for 0 <= t < 2^31 by a multiplication (n is the size of a page: any number), the method of Granlund and Montgomery, "Division by Invariant Integers using
+// Multiplication" (1994)
 struct KhDivide {
   uint32_t n, mul, s1, s2;
   __host__ explicit KhDivide(uint32_t by) : n(by) {
