@@ -1809,6 +1809,7 @@ def _section_ends(sections):
     """(ends as int64s, axes, pairs)."""
     if not 1 <= len(sections) <= 4 or any(int(n) != n or n < 0 for n in sections):
         raise ValueError(f"sections must be one to four numbers of pairs, got {sections}")
+    sections = [int(n) for n in sections]
     ends = [sum(sections[:i + 1]) for i in range(len(sections))]
     return struct.pack("4q", *(ends + ends[-1:] * 3)[:4]), len(ends), ends[-1]
 

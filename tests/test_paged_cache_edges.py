@@ -85,3 +85,14 @@ def test_copies_of_a_cache_describe_themselves():
         assert other.lengths.tolist() == [0, 7, 0, 0] and other.lengths.data_ptr() != c.lengths.data_ptr() and describes(other)
     same = copy.copy(c)
     assert same.k is c.k and describes(same)
+
+
+def test_sections_are_whole_numbers_of_any_kind():
+    from katz_amd.ops import _section_ends
+
+    want = struct.pack("4q", 9, 21, 21, 21), 2, 21
+    for sections in ((9.0, 12.0), (9, 12), (torch.tensor(9), 12)):
+        assert _section_ends(sections) == want
+    for bad in ((9.5, 12), (-1, 4), (), (1, 1, 1, 1, 1), (float("nan"),)):
+        with pytest.raises(ValueError):
+            _section_ends(bad)
