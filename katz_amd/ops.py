@@ -1923,7 +1923,7 @@ def cache_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: Paged
         raise TypeError(f"{k.dtype} rows for a cache of {cache.k.dtype}")
     if not 0 <= layer < cache.layers:
         raise ValueError(f"layer {layer} of a cache of {cache.layers}")
-    if q.shape[-1] != heads * cache.d:
+    if heads < 1 or q.shape[-1] != heads * cache.d:
         raise ValueError(f"q must be [.., {heads} * {cache.d}], got {tuple(q.shape)}")
     _here(q, k, v, positions, frequencies, slots, places, out, cache.k)      # (the cache's parts lie together)
     rows = q.numel() // q.shape[-1]

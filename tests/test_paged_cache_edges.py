@@ -96,3 +96,14 @@ def test_sections_are_whole_numbers_of_any_kind():
     for bad in ((9.5, 12), (-1, 4), (), (1, 1, 1, 1, 1), (float("nan"),)):
         with pytest.raises(ValueError):
             _section_ends(bad)
+
+
+@pytest.mark.parametrize("heads", [0, -4])
+def test_heads_that_are_none_are_refused(lib, heads):  # noqa: F811
+    from katz_amd import ops
+
+    c = ops.PagedCache(**parts())
+    none, k = torch.zeros(4, 0, dtype=torch.bfloat16), torch.zeros(4, 128, dtype=torch.bfloat16)
+    for call in (lambda: ops.cache_append(none, k, k, c, heads), lambda: ops.paged_attention(none, c, heads)):
+        with pytest.raises(ValueError):
+            call()
