@@ -557,7 +557,8 @@ int kh_rotary(const void* q, const void* k, const void* v, void* q_out, void* k_
  * (NULL: row r is slot r), n = lengths[r] (NULL: the cache's for the slot; at most width * page), with a window > 0 only the last `window` of them.  Query
  * head h takes key head h / (heads / kv_heads).  Nothing to attend to: zeros.  Rows whose slot lies outside the cache are left out: o stays as it
  * was, with flags bit 0 it is zeroed.  q, o [rows, heads * d] through row strides, type 0 or 1, the cache's unless that is e4m3.  An infinity among the attended
- * values gives NaN, and so does a score of plus infinity; where all scores are minus infinity there is nothing to attend to.
+ * values gives NaN, and so does a score of plus infinity; where all scores are minus infinity there is nothing to attend to.  Weights are held in 32 bits (over fp16 values to
+ * 2^-54 of the largest).
  * workspace: kh_paged_attention_workspace_bytes(rows, heads, kv_heads, d, width * page) (0: may be NULL), aligned to 16 bytes. */
 int64_t kh_paged_attention_workspace_bytes(int64_t rows, int64_t heads, int64_t kv_heads, int64_t d, int64_t span);
 int kh_paged_attention(const void* q, void* o, const KhPagedCache* cache, int64_t layer, const int32_t* slots, const int32_t* lengths, void* workspace,

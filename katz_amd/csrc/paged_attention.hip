@@ -92,13 +92,13 @@ __device__ __forceinline__ uint32_t two_of_e4m3(uint32_t w) {
 }
 
 // P in three pieces.  Of bf16 they are the upper bits of what is left each time, and P is their sum: bf16 reaches as far down as 32 bits do.  fp16 does not: P is held
-// 2^7 times as large (it stays under 2^15, the running maximum may be 2^8 behind), and the third piece is what two leave times 2^23, with a product of its own.  That is all
-// of P down to 2^-31 of the largest and 11 bits down to 2^-44; what is lost of n weights is under n 2^-55 (two pieces of P as it is lose n 2^-25, a hundredth of what
-// tokens 16 below one whose value is zero give).  us: one sequence of 131071 tokens 25.1 with two pieces, 25.8 so, 28.0 with products in 32 bits.
+// 2^7 times as large (it stays under 2^15, the running maximum may be 2^8 behind), and what a piece leaves goes to the next one 2^11 times as large, with a product of its
+// own.  That is all of P down to 2^-30 of the largest, 17 bits down to 2^-36 and 11 down to 2^-42; what is lost of n weights is under n 2^-54 (of two pieces of P as it is
+// n 2^-25, a hundredth of what tokens 16 below one whose value is zero give).  us: one sequence of 131071 tokens 25.1 with two pieces, 26.0 so, 28.4 with products in 32 bits.
 template <typename W> struct Pieces;
 template <> struct Pieces<bf16_t> {
   static constexpr float UP_LOG2 = 0.f;
-  static constexpr bool APART = false;                  // whether the third has its own product
+  static constexpr bool APART = false;                  // whether a piece has a product of its own
   static __device__ __forceinline__ void of(const float (&p)[8], bf16x8 (&out)[3]) {
     uint32_t w[3][4];
 #pragma unroll
@@ -116,13 +116,13 @@ template <> struct Pieces<bf16_t> {
   }
 };
 template <> struct Pieces<f16_t> {
-  static constexpr float UP_LOG2 = 7.f, REST = 0x1p23f;
+  static constexpr float UP_LOG2 = 7.f, REST = 0x1p11f;
   static constexpr bool APART = true;
   static __device__ __forceinline__ void of(const float (&p)[8], f16x8 (&out)[3]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       out[0][i] = (f16_t)p[i];
-      const float rest = p[i] - (float)out[0][i];
+      const float rest = (p[i] - (float)out[0][i]) * REST;
       out[1][i] = (f16_t)rest;
       out[2][i] = (f16_t)((rest - (float)out[1][i]) * REST);
     }
@@ -366,13 +366,16 @@ struct Wave {
         }
         const X8 value8 = __builtin_bit_cast(X8, a);
         f32x4& to = o[c * S::VE + j];
-        to = mfma(value8, pieces[1], mfma(value8, pieces[0], to));
+        to = mfma(value8, pieces[0], to);
         if constexpr (Pieces<W>::APART) {
-          const f32x4 rest = mfma(value8, pieces[2], f32x4{0.f, 0.f, 0.f, 0.f});
+          f32x4 rest = mfma(value8, pieces[2], f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+          for (int r = 0; r < 4; ++r) rest[r] *= 1.f / Pieces<W>::REST;
+          rest = mfma(value8, pieces[1], rest);
 #pragma unroll
           for (int r = 0; r < 4; ++r) to[r] += rest[r] * (1.f / Pieces<W>::REST);
         } else {
-          to = mfma(value8, pieces[2], to);
+          to = mfma(value8, pieces[2], mfma(value8, pieces[1], to));
         }
       }
     if constexpr (MORE) {

@@ -58,6 +58,35 @@ def test_weights_far_below_the_largest_count(dtype, cache, gap, n, heads, kv, d)
 
 
 @pytest.mark.parametrize("dtype", [BF, FP16])
+@pytest.mark.parametrize("n,d", [(40, 64), (700, 128), (2500, 256)])
+def test_equal_weights_far_below_the_largest_have_no_error_in_common(dtype, n, d):
+    """As above with the rest of the tokens alike: what their weights lack is lacking from the whole output.  Weights of 2^-12 .. 2^-35; the values are as large as
+    fp16 has them.  Scores are one product of two exact numbers: off by the roundings of the factor, the product and the difference, 4 * 2^-24 of themselves, and the exponential's 2^-22; the
+    sums as in the reference."""
+    from katz_amd import ops
+
+    g = gen(n)
+    gaps = [8.0 + 0.37 * i for i in range(44)]
+    pages = Pages(49, [n], 16, 1, d, dtype)
+    v = (torch.rand(n, d, generator=g) + 1) * 20000
+    v[5] = 0
+    for t in range(n):
+        e, at = pages.table[0, t // 16], t % 16
+        pages.k[0, e, at, 0], pages.v[0, e, at, 0] = 0, v[t].to(dtype)
+    pages.k[0, pages.table[0, 0], 5, 0, 0] = 1
+    pages.dev.k.copy_(pages.k)
+    pages.dev.v.copy_(pages.v)
+    q = torch.zeros(len(gaps), d, dtype=dtype)
+    q[:, 0] = torch.tensor(gaps).to(dtype)               # (the score of the fifth; the others have 0)
+    slots = torch.zeros(len(gaps), dtype=torch.int32)
+    ref, _ = attention_reference(q, pages, 1, slots, [n] * len(gaps), scale=1.0)
+    got = ops.paged_attention(q.to(DEV), pages.dev, 1, slots=slots.to(DEV), scale=1.0)
+    slack = 2 * (4 * U * max(gaps) + 2.0 ** -22) + 2 * (n / 4 + 64) * U
+    half = torch.exp2(torch.floor(torch.log2(ref * (1 + slack)))) * HALF[dtype]          # (of the value's own step)
+    assert_within(got.view(-1, 1, d), ref, half.clamp(min=TINY[dtype]) + slack * ref, "equal weights")
+
+
+@pytest.mark.parametrize("dtype", [BF, FP16])
 @pytest.mark.parametrize("d,turn", [(128, 32), (40, 12), (72, 0)])
 def test_codes_are_those_of_the_quotient_in_32_bits(dtype, d, turn):
     """Scales as calibration makes them (the largest number / 448): multiples of sevenths lie on borders between codes, or a rounding of the scale beside them, and one quotient in a
