@@ -5,8 +5,8 @@
 // refs once, in order, as far as it has to.  Only the copies need the whole chip: they take their list from memory, since how many there are is not
 // known to the host.
 //
-// Bound by the launches and the memory's latency for a few sequences, by the copies' bytes for many layers.  us, the middle of 12: three beams forked from 77 tokens, 2 layers, 6.6 + 3.5, then
-// their next tokens 2.8; 48 of 8 sequences, 24 layers, 5.1 + 4.6 + 22.6 (171 MB in and out), 5.1; 490 of 2048 pages moved in 4 layers 6.3 + 102 (515 MB, 5.1 TB/s).
+// Bound by the launches and the memory's latency for a few sequences, by the copies' bytes for many layers.  us, the middle of 12: three beams forked from 77 tokens, 2 layers, 6.8 + 3.4, then
+// their next tokens 2.8; 48 of 8 sequences, 24 layers, 5.1 + 4.7 + 21.3 (171 MB in and out), 5.1; 490 of 2048 pages moved in 4 layers 6.4 + 102 (515 MB, 5.1 TB/s).
 #include "paged_cache.h"
 #include <climits>
 

@@ -12,8 +12,8 @@
 // The tokens of the keys' rows are chosen so that the scores a lane gets (query l % 16, eight tokens) are the P operand it needs: nothing crosses lanes but the
 // maximum.  Neither operand goes through LDS.  P is multiplied in all 24 bits, in three pieces of 16: the matrix unit waits for memory anyway.
 //
-// us a launch, the middle of 12 (TB/s of keys and values): one token of 64 requests of 0 .. 8192 tokens, 32 heads of 128 on 8, bf16, 121 (5.5) and 5.0 for the join; one of 131071 tokens,
-// 16 heads on 2, fp16, 26.9 (5.0) and 5.3; 2 x 77 tokens 5.6, a chain of lengths, page numbers and rows.  32 of 4096 tokens with 4 KB a token, heads of 64, 128, 256: 93, 91, 85 (5.8, 5.9, 6.3)
+// us a launch, the middle of 12 (TB/s of keys and values): one token of 64 requests of 0 .. 8192 tokens, 32 heads of 128 on 8, bf16, 120 (5.5) and 4.9 for the join; one of 131071 tokens,
+// 16 heads on 2, fp16, 27.0 (5.0) and 5.7; 2 x 77 tokens 5.7, a chain of lengths, page numbers and rows.  32 of 4096 tokens with 4 KB a token, heads of 64, 128, 256: 93, 91, 85 (5.8, 5.9, 6.3)
 // on one card and 116, 113, 102 on another, with 2 KB in e4m3 87, 53, 63 and 98, 63, 66.  A copy of 1 GiB runs at 5.1 TB/s.  With each step's loads waited for where they are used: 207 and 55.  Values are read past
 // the caches (126 us where that is 119), keys are not (123, and the two halves of a line that a wave asks for one after the other are both there: e4m3 78 -> 59).
 #include "paged_cache.h"

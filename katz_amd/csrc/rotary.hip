@@ -12,8 +12,8 @@
 // threads go over the rows in pieces of eight elements of either half (or eight in a row), 16 bytes a load, two pieces on their way at a time
 // (7904 rows of 40 heads of 64: one 19.0 us, two 15.8, three 19.8).
 //
-// us, the middle of 12 launches: 7904 rows of 20 + 20 heads of 64, bf16, 15.9 (5.1 TB/s in and out), 16384 of 16 + 8 of 128, fp32, 75 (5.4; four rows to a workgroup and read past the
-// caches 72, but 81 behind one another), 8184 of 16 + 8 of 80 into pages 20.3 (4.1), 2 rows into pages 3.3.  Of 24: 8184 rows of 16 + 8 of 128 into bf16 pages 30 (4.5), into e4m3, every
+// us, the middle of 12 launches: 7904 rows of 20 + 20 heads of 64, bf16, 15.6 (5.2 TB/s in and out), 16384 of 16 + 8 of 128, fp32, 74 (5.4; four rows to a workgroup and read past the
+// caches 72, but 81 behind one another), 8184 of 16 + 8 of 80 into pages 20.6 (4.1), 2 rows into pages 3.2.  Of 24: 8184 rows of 16 + 8 of 128 into bf16 pages 30 (4.5), into e4m3, every
 // key turned and scaled in 64 bits, 31 (3.8), with pairs in turn 35; heads of 80 with 20 pairs, no whole eights and so an element at a time, 66 for the 14 of their bytes.
 #include "paged_cache.h"
 #include <type_traits>
